@@ -1,7 +1,7 @@
 /* ogle_cuda.h - C ABI of the B200 (sm_100a) backend for the OGLE graph runtime's
  * data-parallel hot path: conv2d family with fused bias/BN/activation, gemm,
  * pooling, elementwise, concat, layout conversion and the SSD box decoder and
- * post-process.
+ * post-process; and the operators of a language model's decoding step.
  *
  * The reference runtime (kl456123/OGLE) has no foreign-function interface: each
  * operator's Kernel::Compute binds OpenGL textures and draws. Every entry point
@@ -411,6 +411,106 @@ int ogle_cuda_ssd_detect(const OgleDetectParams* p, const float* logits, const f
 int ogle_cuda_ssd_decode_detect(const OgleDetectParams* p, const float* logits, const float* pred, const float* anchors,
                                 const float variances[4], float* out_score, int* out_anchor, int* out_class,
                                 float* out_box, int* out_count, ogle_stream_t stream);
+
+/* --------------------------------------------------- language-model steps */
+/* What a decoding step of a language model needs beside the products above: new keys and values into a paged cache held
+ * in 8 bits, attention over that cache, and the adjustment of logits before a token is chosen. The reference, a graph
+ * runtime for image networks, has no counterpart. Activations are in 32 or 16 bits with strides of their own (no padding
+ * to 4). */
+typedef enum { OGLE_F32 = 0, OGLE_F16 = 1, OGLE_BF16 = 2 } OgleDataType;
+
+/* A batch of sequences and the cache their keys and values lie in.
+ * Cache: e4m3 bytes, page p, key/value head h, token t of the page, element d at
+ * p * page_stride + h * head_stride + t * token_stride + d (bytes; the same for keys and values; multiples of 16). One scale
+ * for each page and head, a power of two: value = e4m3 * scale[p * kv_heads + h].
+ * Token j of sequence b lies in page block_table[b * table_stride + j / page_tokens]. A page of a sequence that is
+ * appended to belongs to that sequence alone; full pages may be shared. An entry outside [0, n_pages) names no page:
+ * nothing is stored there, and its tokens are not attended.
+ * Rows: sequence b has rows row_start[b] .. row_start[b + 1] of the call's q, k, v and out, the last of the kv_len[b] tokens
+ * it has once they are appended: row i of n stands at position kv_len[b] - n + i. row_start NULL: one row a sequence.
+ * The host gives bounds of what the device holds, so that nothing waits for it: max_rows (rows of a sequence) and
+ * max_kv_len; rows and tokens beyond them are ignored. */
+typedef struct {
+    int n_seqs, n_rows;            /* sequences; rows of all of them */
+    int max_rows, max_kv_len;
+    int q_heads, kv_heads;         /* q_heads a multiple of kv_heads: query head h reads kv head h / (q_heads / kv_heads) */
+    int head_dim;                  /* a multiple of 16, at most 256 */
+    int page_tokens;               /* 16, 32, ... 1024: a power of two */
+    int n_pages, table_stride;
+    int dtype;                     /* OgleDataType of q, k, v and out */
+    int reserved;
+    long long page_stride, head_stride, token_stride;
+    const int *row_start, *kv_len, *block_table;
+    void *k_cache, *v_cache;
+    float *k_scale, *v_scale;
+} OglePagedBatch;
+
+/* Stores the rows' keys and values in their pages and rotates keys and queries by their positions on the way.
+ * Rotation of a pair (x1, x2) by row `position` of the table: (x1 c - x2 s, x2 c + x1 s), in fp32, with c = rotary[position][i],
+ * s = rotary[position][rotary_dim / 2 + i]; the pairs are (x[i], x[i + rotary_dim / 2]), or neighbours with `interleaved`. Elements
+ * from rotary_dim on stay as they are; rotary NULL rotates nothing.
+ * A page's scale is the smallest power of two with |x| <= 448 scale for what it has taken since its first slot was last
+ * written; where a row needs a larger one, what is in the page is moved by the exponent. An infinity is stored as the largest
+ * value, a NaN as NaN; neither counts for the scale.
+ * q may be NULL (nothing to rotate); q_out may be q. Strides in elements, multiples of 16 bytes, elements side by side. */
+typedef struct {
+    const void *k, *v, *q;
+    void* q_out;
+    long long k_row, k_head, v_row, v_head, q_row, q_head, q_out_row, q_out_head;
+    const float* rotary;           /* [rotary_rows][rotary_dim], rotary_rows >= max_kv_len */
+    int rotary_dim;                /* a multiple of 8, at most head_dim */
+    int rotary_rows;
+    int interleaved;
+    int reserved;
+} OgleAppendParams;
+int ogle_cuda_kv_append(const OglePagedBatch* batch, const OgleAppendParams* p, ogle_stream_t stream);
+
+/* out[row][h] = sum_j softmax_j(scale q.k_j) v_j over the tokens j < kv_len of the row's sequence - with `causal` those up to the
+ * row's own position, with window > 0 those after position - window. lse (may be NULL), [n_rows][q_heads]: the natural logarithm
+ * of the sum of exponentials. A row without a token has out 0 and lse minus infinity. A token that a row does not attend does
+ * not reach it, whatever its bytes are. Scores, statistics and sums are in fp32; for fp32 activations the queries and weights enter
+ * the products as two 16-bit parts.
+ * The caller lends `workspace` (>= ogle_cuda_paged_attention_workspace_bytes, 16-byte aligned); nothing in it has to be
+ * cleared, and it may be reused once the stream has passed the call. Strides in elements, multiples of 16 bytes. */
+typedef struct {
+    const void* q;
+    void* out;
+    float* lse;
+    long long q_row, q_head, out_row, out_head;
+    float scale;
+    int causal;
+    int window;
+    int reserved;
+} OgleAttentionParams;
+size_t ogle_cuda_paged_attention_workspace_bytes(const OglePagedBatch* batch, const OgleAttentionParams* p);
+int ogle_cuda_paged_attention(const OglePagedBatch* batch, const OgleAttentionParams* p, void* workspace,
+                              size_t workspace_bytes, ogle_stream_t stream);
+
+/* y[r][t] from x = logits[r][t], in this order, each step rounded to fp32:
+ *   x > 0 ? x / repetition[r] : x * repetition[r]      where t is among the row's tokens
+ *   x - frequency[r] * n - presence[r]                  where t is n > 0 times among the row's tokens after its first prompt_len[r]
+ *   x + bias_value[i]                                   where bias_token[i] == t (the last such i of the row's)
+ *   minus infinity                                      where bit t % 32 of allowed[r * allowed_stride + t / 32] is 0 (a stride
+ *                                                       of 0: one mask for all rows)
+ * Row r's tokens are tokens[token_start[r]] .. tokens[token_start[r + 1]], its biases bias_start[r] .. bias_start[r + 1]; tokens
+ * outside [0, vocab) are ignored. Any of tokens, bias_token, allowed and of the four row vectors may be NULL (no such step,
+ * repetition 1, presence and frequency 0, no prompt). Row strides in elements; out may be logits where the types are the
+ * same. out_dtype: dtype or OGLE_F32. */
+typedef struct {
+    int rows, vocab;
+    int dtype, out_dtype;          /* OgleDataType */
+    int n_tokens, n_biases;        /* entries of tokens and of bias_token: nothing behind them is read */
+    long long logits_stride, out_stride, allowed_stride;
+    const void* logits;
+    void* out;
+    const int *tokens, *token_start, *prompt_len;
+    const float *repetition, *presence, *frequency;
+    const int* bias_token;
+    const float* bias_value;
+    const int* bias_start;
+    const unsigned* allowed;
+} OgleLogitsParams;
+int ogle_cuda_adjust_logits(const OgleLogitsParams* p, ogle_stream_t stream);
 
 #ifdef __cplusplus
 }

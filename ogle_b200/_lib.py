@@ -13,6 +13,7 @@ RT_LIB_PATH = os.path.join(_HERE, "libogle_rt.so")
 OGLE_MAX_CONCAT_INPUTS = 16
 
 MATH_FP32, MATH_TF32, MATH_TF32X3 = 0, 1, 2
+DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 ACT_NONE, ACT_CLIP, ACT_RELU = 0, 1, 2
 
 
@@ -55,6 +56,47 @@ class DetectParams(C.Structure):
         ("N", C.c_int), ("A", C.c_int), ("C", C.c_int), ("logit_stride", C.c_int), ("mode", C.c_int),
         ("score_thr", C.c_float), ("top_k", C.c_int), ("nms_thr", C.c_float),
         ("image_w", C.c_int), ("image_h", C.c_int), ("frame_sizes", C.c_void_p),
+    ]
+
+
+class PagedBatch(C.Structure):
+    _fields_ = [
+        ("n_seqs", C.c_int), ("n_rows", C.c_int), ("max_rows", C.c_int), ("max_kv_len", C.c_int),
+        ("q_heads", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int), ("page_tokens", C.c_int),
+        ("n_pages", C.c_int), ("table_stride", C.c_int), ("dtype", C.c_int), ("reserved", C.c_int),
+        ("page_stride", C.c_longlong), ("head_stride", C.c_longlong), ("token_stride", C.c_longlong),
+        ("row_start", C.c_void_p), ("kv_len", C.c_void_p), ("block_table", C.c_void_p),
+        ("k_cache", C.c_void_p), ("v_cache", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+    ]
+
+
+class AppendParams(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("q", C.c_void_p), ("q_out", C.c_void_p),
+        ("k_row", C.c_longlong), ("k_head", C.c_longlong), ("v_row", C.c_longlong), ("v_head", C.c_longlong),
+        ("q_row", C.c_longlong), ("q_head", C.c_longlong), ("q_out_row", C.c_longlong), ("q_out_head", C.c_longlong),
+        ("rotary", C.c_void_p), ("rotary_dim", C.c_int), ("rotary_rows", C.c_int), ("interleaved", C.c_int),
+        ("reserved", C.c_int),
+    ]
+
+
+class AttentionParams(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p),
+        ("q_row", C.c_longlong), ("q_head", C.c_longlong), ("out_row", C.c_longlong), ("out_head", C.c_longlong),
+        ("scale", C.c_float), ("causal", C.c_int), ("window", C.c_int), ("reserved", C.c_int),
+    ]
+
+
+class LogitsParams(C.Structure):
+    _fields_ = [
+        ("rows", C.c_int), ("vocab", C.c_int), ("dtype", C.c_int), ("out_dtype", C.c_int),
+        ("n_tokens", C.c_int), ("n_biases", C.c_int),
+        ("logits_stride", C.c_longlong), ("out_stride", C.c_longlong), ("allowed_stride", C.c_longlong),
+        ("logits", C.c_void_p), ("out", C.c_void_p),
+        ("tokens", C.c_void_p), ("token_start", C.c_void_p), ("prompt_len", C.c_void_p),
+        ("repetition", C.c_void_p), ("presence", C.c_void_p), ("frequency", C.c_void_p),
+        ("bias_token", C.c_void_p), ("bias_value", C.c_void_p), ("bias_start", C.c_void_p), ("allowed", C.c_void_p),
     ]
 
 
@@ -109,6 +151,10 @@ CUDA_SYMBOLS = {
     "ogle_cuda_reshape_placed": (C.c_int, [_vp, _vp, C.c_long, C.c_int, C.c_int, C.c_long, C.c_long, _vp]),
     "ogle_cuda_ssd_decode": (C.c_int, [_vp, _vp, _vp, C.c_int, C.c_int, C.POINTER(C.c_float), _vp]),
     "ogle_cuda_ssd_detect": (C.c_int, [C.POINTER(DetectParams)] + [_vp] * 8),
+    "ogle_cuda_kv_append": (C.c_int, [C.POINTER(PagedBatch), C.POINTER(AppendParams), _vp]),
+    "ogle_cuda_paged_attention_workspace_bytes": (C.c_size_t, [C.POINTER(PagedBatch), C.POINTER(AttentionParams)]),
+    "ogle_cuda_paged_attention": (C.c_int, [C.POINTER(PagedBatch), C.POINTER(AttentionParams), _vp, C.c_size_t, _vp]),
+    "ogle_cuda_adjust_logits": (C.c_int, [C.POINTER(LogitsParams), _vp]),
     "ogle_cuda_ssd_decode_detect": (C.c_int, [C.POINTER(DetectParams), _vp, _vp, _vp, C.POINTER(C.c_float)] + [_vp] * 6),
 }
 

@@ -1,0 +1,297 @@
+// Appending to the paged 8-bit cache: rotation by position, one power-of-two scale for each page and head, e4m3.
+//
+// A block has one page of one sequence and either one head of the keys, one of the values, or a few heads of the queries: the
+// page's scale depends on all rows that come to it, and nothing else does, so no block waits for another and no sum has an
+// order to depend on. The rows' values stay in registers between the maximum and the rounding.
+#include <type_traits>
+
+#include "paged.cuh"
+
+namespace ogle {
+namespace {
+
+using paged::Batch;
+
+struct AppendArgs {
+    Batch b;
+    const void *k, *v, *q;
+    void* q_out;
+    long long k_row, k_head, v_row, v_head, q_row, q_head, qo_row, qo_head;
+    const float* rotary;
+    int rotary_dim, interleaved;
+    int q_blocks;                 // blocks of kQHeads query heads
+};
+
+constexpr int kQHeads = 4;        // query heads of a block
+constexpr int kHold = 4;          // pieces of 8 values a thread keeps
+constexpr int kMaxThreads = 256;
+
+// 8 values of a head: `at` and the four behind it, `at2` and the four behind that. A piece inside the rotated part with pairs
+// rotary_dim / 2 apart has both halves of its pairs; every other piece is 8 neighbours.
+struct Piece { int at, at2, angle; };  // angle: first column of the table's cosines, -1: not rotated
+
+__device__ __forceinline__ Piece piece_of(int i, int rotary_dim, bool interleaved) {
+    Piece p;
+    p.at = i * 8;
+    p.at2 = p.at + 4;
+    p.angle = -1;
+    if (p.at < rotary_dim) {
+        if (interleaved) {
+            p.angle = i * 4;
+        } else {
+            p.at = i * 4;
+            p.at2 = p.at + rotary_dim / 2;
+            p.angle = p.at;
+        }
+    }
+    return p;
+}
+
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, float* x) {
+    if constexpr (std::is_same<T, float>::value) {
+        const float4 v = *reinterpret_cast<const float4*>(p);
+        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    } else {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        const T* h = reinterpret_cast<const T*>(&v);
+#pragma unroll
+        for (int l = 0; l < 4; ++l) x[l] = float(h[l]);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T* p, const float* x) {
+    if constexpr (std::is_same<T, float>::value) {
+        *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    } else {
+        uint2 v;
+        T* h = reinterpret_cast<T*>(&v);
+#pragma unroll
+        for (int l = 0; l < 4; ++l) h[l] = T(x[l]);
+        *reinterpret_cast<uint2*>(p) = v;
+    }
+}
+
+// The piece's values, rotated. Products and sums are rounded one by one (no fused multiply-add): what is stored in 8 bits is
+// then the same as from any other evaluation of the formula in fp32, where a fused one crosses a rounding boundary now and then.
+template <typename T>
+__device__ __forceinline__ void load_piece(const T* row, const Piece& p, const float* cs, int half, bool interleaved, float (&x)[8]) {
+    load4(row + p.at, x);
+    load4(row + p.at2, x + 4);
+    if (p.angle < 0) return;
+    float c[4], s[4];
+    load4(cs + p.angle, c);
+    load4(cs + half + p.angle, s);
+#pragma unroll
+    for (int l = 0; l < 4; ++l) {
+        float& a = interleaved ? x[2 * l] : x[l];
+        float& b = interleaved ? x[2 * l + 1] : x[4 + l];
+        const float u = __fsub_rn(__fmul_rn(a, c[l]), __fmul_rn(b, s[l]));
+        const float v = __fadd_rn(__fmul_rn(b, c[l]), __fmul_rn(a, s[l]));
+        a = u;
+        b = v;
+    }
+}
+
+// The smallest power of two s with amax <= 448 s, from the bits: 448 = 0.875 * 2^9. At least 2^-120, so that 1 / s is a normal number.
+__device__ __forceinline__ float scale_for(float amax) {
+    const uint32_t u = __float_as_uint(amax);
+    const int e = int(u >> 23) - 126 - 9 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);     // amax = f * 2^(e + 9), f in [0.5, 1)
+    return __uint_as_float(uint32_t(max(e, -120) + 127) << 23);
+}
+
+__device__ __forceinline__ float finite_abs(float x) {
+    const float a = fabsf(x);
+    return a <= 3.402823466e38f ? a : 0.f;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kMaxThreads) paged_append_kernel(AppendArgs a) {
+    __shared__ int where[4];
+    __shared__ float warp_max[kMaxThreads / 32];
+    const Batch& B = a.b;
+    const int tid = threadIdx.x, page_tokens = 1 << B.page_shift;
+    grid_dependency_trigger();
+    grid_dependency_wait();
+    // which sequence, and which of the pages that it appends to
+    int b = blockIdx.x, nth = 0;
+    if (B.max_rows > 1) {
+        if (tid < 32) {
+            int before = 0, found = -1;
+            for (int b0 = 0; b0 < B.n_seqs; b0 += 32) {
+                int pages = 0;
+                if (b0 + tid < B.n_seqs) {
+                    const paged::Sequence s = paged::sequence(B, b0 + tid);
+                    const int p0 = max(s.len - s.n, 0);
+                    pages = s.n > 0 && s.len > 0 ? ((s.len - 1) >> B.page_shift) - (p0 >> B.page_shift) + 1 : 0;
+                }
+                int sum = pages;
+#pragma unroll
+                for (int d = 1; d < 32; d *= 2) {
+                    const int o = __shfl_up_sync(~0u, sum, d);
+                    if (tid >= d) sum += o;
+                }
+                const int at = int(blockIdx.x) - before;
+                const unsigned hit = __ballot_sync(~0u, at >= sum - pages && at < sum);
+                if (hit) {
+                    const int l = __ffs(hit) - 1;
+                    found = b0 + l;
+                    nth = at - (__shfl_sync(~0u, sum, l) - __shfl_sync(~0u, pages, l));
+                    break;
+                }
+                before += __shfl_sync(~0u, sum, 31);
+            }
+            if (tid == 0) { where[0] = found; where[1] = nth; }
+        }
+        __syncthreads();
+        b = where[0];
+        nth = where[1];
+        if (b < 0) return;
+    }
+    const paged::Sequence s = paged::sequence(B, b);
+    if (s.n <= 0 || s.len <= 0) return;
+    const int begin = max(s.len - s.n, 0);                       // the first new token
+    const int block = (begin >> B.page_shift) + nth;             // of the sequence's blocks of tokens
+    const int t0 = max(begin, block << B.page_shift), t1 = min(s.len, (block + 1) << B.page_shift);
+    const int row0 = s.row0 + s.n - s.len;                       // row of token t: row0 + t
+    const int pieces = B.dim / 8, half = a.rotary_dim / 2;
+    const bool inter = a.interleaved != 0;
+
+    if (int(blockIdx.y) >= 2 * B.kv_heads) {                     // queries: rotated and stored as they came
+        const int h0 = (blockIdx.y - 2 * B.kv_heads) * kQHeads, heads = min(kQHeads, B.q_heads - h0);
+        const int per_token = pieces * heads, total = (t1 - t0) * per_token;
+        for (int i = tid; i < total; i += blockDim.x) {
+            const int t = t0 + i / per_token, r = i % per_token, h = h0 + r / pieces;
+            const Piece p = piece_of(r % pieces, a.rotary_dim, inter);
+            float x[8];
+            load_piece(static_cast<const T*>(a.q) + (row0 + t) * a.q_row + h * a.q_head, p, a.rotary + (long long)t * a.rotary_dim, half, inter, x);
+            T* y = static_cast<T*>(a.q_out) + (row0 + t) * a.qo_row + h * a.qo_head;
+            store4(y + p.at, x);
+            store4(y + p.at2, x + 4);
+        }
+        return;
+    }
+    const int page = paged::page_of(B, b, block);
+    if (page < 0) return;
+    const bool keys = int(blockIdx.y) < B.kv_heads;
+    const int h = keys ? blockIdx.y : blockIdx.y - B.kv_heads;
+    const T* x0 = static_cast<const T*>(keys ? a.k : a.v) + h * (keys ? a.k_head : a.v_head);
+    const long long x_row = keys ? a.k_row : a.v_row;
+    unsigned char* out = (keys ? B.k_cache : B.v_cache) + page * B.page_stride + h * B.head_stride;
+    float* scale = (keys ? B.k_scale : B.v_scale) + (long long)page * B.kv_heads + h;
+    const int rotary_dim = keys ? a.rotary_dim : 0, total = (t1 - t0) * pieces, slot0 = t0 & (page_tokens - 1);
+
+    float x[kHold][8], top = 0.f;
+#pragma unroll
+    for (int u = 0; u < kHold; ++u) {
+        const int i = tid + u * blockDim.x;
+        if (i < total) {
+            const int t = t0 + i / pieces;
+            load_piece(x0 + (row0 + t) * x_row, piece_of(i % pieces, rotary_dim, inter), a.rotary + (long long)t * rotary_dim, half, inter, x[u]);
+#pragma unroll
+            for (int l = 0; l < 8; ++l) top = fmaxf(top, finite_abs(x[u][l]));
+        }
+    }
+    for (int i = tid + kHold * blockDim.x; i < total; i += blockDim.x) {      // pages of more than the registers hold
+        const int t = t0 + i / pieces;
+        float z[8];
+        load_piece(x0 + (row0 + t) * x_row, piece_of(i % pieces, rotary_dim, inter), a.rotary + (long long)t * rotary_dim, half, inter, z);
+#pragma unroll
+        for (int l = 0; l < 8; ++l) top = fmaxf(top, finite_abs(z[l]));
+    }
+#pragma unroll
+    for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+    const float old = slot0 > 0 ? *scale : 0.f;                  // read by every thread before one of them writes it
+    if (blockDim.x > 32) {
+        if ((tid & 31) == 0) warp_max[tid / 32] = top;
+        __syncthreads();
+        for (int w = 0; w < int(blockDim.x) / 32; ++w) top = fmaxf(top, warp_max[w]);
+    } else {
+        __syncwarp();
+    }
+    float now = fmaxf(old, top > 0.f ? scale_for(top) : 0.f);
+    if (now <= 0.f) now = 1.f;
+    const float inverse = 1.f / now;                             // a power of two: exact
+
+    auto store = [&](int i, const float (&z)[8]) {
+        const Piece p = piece_of(i % pieces, rotary_dim, inter);
+        unsigned char* y = out + (long long)(slot0 + i / pieces) * B.token_stride;
+        const uint32_t lo = paged::e4m3x2(z[0] * inverse, z[1] * inverse) | paged::e4m3x2(z[2] * inverse, z[3] * inverse) << 16;
+        const uint32_t hi = paged::e4m3x2(z[4] * inverse, z[5] * inverse) | paged::e4m3x2(z[6] * inverse, z[7] * inverse) << 16;
+        if (p.at2 == p.at + 4) {
+            *reinterpret_cast<uint2*>(y + p.at) = make_uint2(lo, hi);
+        } else {
+            *reinterpret_cast<uint32_t*>(y + p.at) = lo;
+            *reinterpret_cast<uint32_t*>(y + p.at2) = hi;
+        }
+    };
+#pragma unroll
+    for (int u = 0; u < kHold; ++u)
+        if (tid + u * int(blockDim.x) < total) store(tid + u * blockDim.x, x[u]);
+    for (int i = tid + kHold * blockDim.x; i < total; i += blockDim.x) {
+        const int t = t0 + i / pieces;
+        float z[8];
+        load_piece(x0 + (row0 + t) * x_row, piece_of(i % pieces, rotary_dim, inter), a.rotary + (long long)t * rotary_dim, half, inter, z);
+        store(i, z);
+    }
+    if (slot0 > 0 && old < now) {                                // what the page has already moves to the new scale
+        const float ratio = old * inverse;
+        const int words = B.dim / 4, slots = page_tokens - (t1 - t0);
+        for (int i = tid; i < slots * words; i += blockDim.x) {
+            int slot = i / words;
+            if (slot >= slot0) slot += t1 - t0;
+            uint32_t* w = reinterpret_cast<uint32_t*>(out + (long long)slot * B.token_stride) + i % words;
+            const uint32_t v = *w, l2 = paged::e4m3x2_to_half2(uint16_t(v)), h2 = paged::e4m3x2_to_half2(uint16_t(v >> 16));
+            const float2 fl = __half22float2(*reinterpret_cast<const __half2*>(&l2)), fh = __half22float2(*reinterpret_cast<const __half2*>(&h2));
+            *w = paged::e4m3x2(fl.x * ratio, fl.y * ratio) | paged::e4m3x2(fh.x * ratio, fh.y * ratio) << 16;
+        }
+    }
+    if (tid == 0 && old != now) *scale = now;
+}
+
+}  // namespace
+}  // namespace ogle
+
+using namespace ogle;
+
+extern "C" int ogle_cuda_kv_append(const OglePagedBatch* batch, const OgleAppendParams* p, ogle_stream_t stream) {
+    AppendArgs a = {};
+    int rc = paged::translate(batch, a.b);
+    if (rc != OGLE_OK) return rc;
+    if (!p) return OGLE_ERR_INVALID;
+    if (p->rotary && (p->rotary_dim < 8 || p->rotary_dim % 8 != 0 || p->rotary_dim > batch->head_dim || p->rotary_rows < batch->max_kv_len))
+        return OGLE_ERR_INVALID;
+    if (!aligned16(p->rotary)) return OGLE_ERR_ALIGNMENT;
+    if (p->q && !p->q_out) return OGLE_ERR_INVALID;
+    if (a.b.n_seqs == 0) return OGLE_OK;
+    if (!p->k || !p->v) return OGLE_ERR_INVALID;
+    const int dt = batch->dtype;
+    if (!paged::strides_ok(p->k, p->k_row, p->k_head, dt) || !paged::strides_ok(p->v, p->v_row, p->v_head, dt) ||
+        !paged::strides_ok(p->q, p->q_row, p->q_head, dt) || !paged::strides_ok(p->q_out, p->q_out_row, p->q_out_head, dt))
+        return OGLE_ERR_ALIGNMENT;
+    const Batch& B = a.b;
+    if (B.max_rows == 0 || B.max_kv_len == 0) return OGLE_OK;
+    a.k = p->k; a.v = p->v; a.q = p->q; a.q_out = p->q_out;
+    a.k_row = p->k_row; a.k_head = p->k_head; a.v_row = p->v_row; a.v_head = p->v_head;
+    a.q_row = p->q_row; a.q_head = p->q_head; a.qo_row = p->q_out_row; a.qo_head = p->q_out_head;
+    a.rotary = p->rotary;
+    a.rotary_dim = p->rotary ? p->rotary_dim : 0;
+    a.interleaved = p->interleaved;
+    a.q_blocks = p->q ? div_up(B.q_heads, kQHeads) : 0;
+    // pages appended to: at most one a row, and at most two that it shares with what a sequence has already or will have
+    long pages = B.max_rows == 1 ? B.n_seqs : (long)(B.n_rows >> B.page_shift) + 2L * B.n_seqs;
+    if (B.max_rows > 1 && pages > B.n_rows) pages = B.n_rows;
+    const int tokens = B.max_rows < (1 << B.page_shift) ? B.max_rows : 1 << B.page_shift;
+    int threads = div_up((long)tokens * B.dim / 8, kHold) * (tokens == 1 ? kHold : 1);
+    threads = (threads + 31) / 32 * 32;
+    if (threads > kMaxThreads) threads = kMaxThreads;
+    const dim3 grid((unsigned)pages, unsigned(2 * B.kv_heads + a.q_blocks));
+    cudaStream_t s = stream;
+    cudaError_t e;
+    if (dt == OGLE_F32) e = launch_overlapped(paged_append_kernel<float>, grid, dim3(threads), 0, s, a);
+    else if (dt == OGLE_F16) e = launch_overlapped(paged_append_kernel<__half>, grid, dim3(threads), 0, s, a);
+    else e = launch_overlapped(paged_append_kernel<__nv_bfloat16>, grid, dim3(threads), 0, s, a);
+    if (e != cudaSuccess) { set_last_error(e); (void)cudaGetLastError(); return OGLE_ERR_CUDA; }
+    return finish_launch();
+}

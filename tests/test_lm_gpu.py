@@ -1,0 +1,428 @@
+"""The language-model operators (ogle_b200/lm.py) against plain implementations in 64 bits."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import lm_checks as ref
+from ogle_b200 import _lib, lm
+
+pytestmark = pytest.mark.gpu
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def rows_of(rows, heads, dim, dtype, seed=1, amplitude=1.5):
+    return (amplitude * torch.randn(rows, heads, dim, generator=torch.Generator().manual_seed(seed))).to(dtype).cuda()
+
+
+# ------------------------------------------------------------------------------------------------------ attention
+CASES = [
+    # new rows, earlier tokens, page, q heads, kv heads, dim, window
+    ([1], [0], 16, 1, 1, 16, 0),                                # a first token: one key
+    ([1], [700], 64, 32, 8, 128, 0),
+    ([1, 1, 1, 1], [0, 15, 16, 1000], 16, 8, 2, 64, 0),         # ends on and around a page's
+    ([1] * 9, [3, 63, 64, 65, 127, 511, 2047, 0, 300], 64, 8, 8, 128, 0),    # one query head to a kv head
+    ([1, 1], [130, 4000], 128, 16, 1, 128, 0),                  # sixteen query heads to one
+    ([1, 1, 1], [77, 300, 5], 32, 15, 5, 80, 0),                # three to one, 80 elements
+    ([1, 1], [260, 1029], 256, 6, 2, 256, 0),
+    ([1, 1], [40, 500], 32, 12, 2, 48, 0),
+    ([1, 1, 1], [5, 200, 3000], 64, 8, 2, 128, 100),            # windows shorter and longer than what there is
+    ([1, 1], [31, 2000], 16, 4, 4, 64, 1),                      # a window of the row alone
+    ([5, 5, 5], [0, 62, 1500], 32, 8, 4, 256, 64),              # drafts in a window
+    ([3, 1, 7, 2], [10, 900, 61, 0], 16, 8, 2, 64, 0),
+    ([40, 1, 17], [0, 333, 100], 64, 8, 2, 128, 0),             # prompts and single tokens together
+    ([70], [0], 16, 4, 4, 96, 20),
+    ([129, 64], [5, 0], 128, 4, 1, 64, 0),
+    ([33], [50], 32, 16, 1, 256, 0),
+]
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("case", range(len(CASES)))
+def test_attention(case, dtype):
+    new, past, page, heads, kv_heads, dim, window = CASES[case]
+    batch, total = ref.make_batch(new, past, page, kv_heads, dim, seed=case)
+    q = rows_of(sum(new), heads, dim, dtype)
+    got = lm.attention(q, window=window, **batch)
+    ref.check_attention(got, ref.attention64(q, batch, total, new, window=window), dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_of_all_tokens(dtype):
+    """Not causal: every row attends every token of its sequence; with a window, none before it."""
+    new, past = [4, 1, 20], [60, 9, 0]
+    batch, total = ref.make_batch(new, past, 16, 2, 64)
+    q = rows_of(sum(new), 6, 64, dtype)
+    for window in (0, 7):
+        got = lm.attention(q, causal=False, window=window, scale=0.3, **batch)
+        ref.check_attention(got, ref.attention64(q, batch, total, new, scale=0.3, causal=False, window=window), dtype)
+
+
+def test_sequences_without_tokens_or_rows():
+    new, past = [1, 0, 1, 3, 0], [10, 5, 0, 100, 0]
+    batch, total = ref.make_batch(new, past, 16, 2, 128)
+    q = rows_of(5, 8, 128, F32)
+    ref.check_attention(lm.attention(q, **batch), ref.attention64(q, batch, total, new), F32)
+    # the device says that a sequence has no token: its rows have no key
+    batch["kv_len"][0] = 0
+    batch["kv_len"][3] = 2                                       # of three rows the first stands before the text
+    out, lse = lm.attention(q, **batch)
+    assert bool((out[0] == 0).all()) and bool((lse[0] == -math.inf).all())
+    assert bool((out[2] == 0).all()) and bool((lse[2] == -math.inf).all())
+    assert bool(torch.isfinite(lse[1]).all()) and bool(torch.isfinite(lse[3:]).all())
+    assert lm.attention(q[:0], **{**batch, "block_table": batch["block_table"][:0], "kv_len": batch["kv_len"][:0],
+                                  "row_start": batch["row_start"][:1]})[0].shape == (0, 8, 128)
+    none = {**batch, "kv_len": torch.zeros_like(batch["kv_len"]), "max_kv_len": 0}
+    out, lse = lm.attention(q, **none)
+    assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+
+
+def test_without_row_start_every_sequence_has_a_row():
+    new, past = [1] * 5, [3, 100, 0, 64, 500]
+    batch, total = ref.make_batch(new, past, 64, 2, 128)
+    q = rows_of(5, 8, 128, BF16)
+    with_it = lm.attention(q, **batch)
+    del batch["row_start"], batch["max_rows"]
+    without = lm.attention(q, **batch)
+    assert torch.equal(with_it[0], without[0]) and torch.equal(with_it[1], without[1])
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_strides_of_queries_cache_and_results(dtype):
+    """Queries that are a slice of a joint projection, a token-major cache, results into a slice."""
+    new, past = [1, 4], [200, 30]
+    batch, total = ref.make_batch(new, past, 32, 2, 64, token_major=True)
+    assert not batch["cache"][0].is_contiguous()
+    wide = rows_of(5, 12, 64, dtype)
+    q, out = wide[:, :8], torch.full((5, 10, 64), 7.0, dtype=dtype, device="cuda")
+    got = lm.attention(q, out=out[:, 1:9], **batch)
+    ref.check_attention(got, ref.attention64(q, batch, total, new), dtype)
+    assert bool((out[:, 0] == 7).all()) and bool((out[:, 9] == 7).all())
+
+
+def test_table_entries_that_name_no_page():
+    """Their tokens are not attended, whatever stands there."""
+    batch, total = ref.make_batch([1, 2], [120, 90], 16, 2, 64)
+    q = rows_of(3, 4, 64, F32)
+    batch["block_table"][0, 2] = -1
+    batch["block_table"][0, 5] = batch["cache"][0].shape[0]
+    batch["block_table"][1, 0] = 2 ** 31 - 1
+    out, lse = lm.attention(q, **batch)
+    k_cache, v_cache, ks, vs = batch["cache"]
+    row = 0
+    for b, n in ((0, 1), (1, 2)):
+        gone = torch.zeros(total[b], dtype=torch.bool)
+        table = batch["block_table"][b].cpu().clone()
+        for i in ((2, 5) if b == 0 else (0,)):
+            gone[i * 16:(i + 1) * 16] = True
+            table[i] = 0
+        k, v = ref.cached(k_cache, ks, table, total[b]), ref.cached(v_cache, vs, table, total[b])
+        for i in range(n):
+            keep = ~gone & (torch.arange(total[b]) <= total[b] - n + i)
+            for h in range(4):
+                s = k[keep, h // 2] @ q[row, h].cpu().double() / 8
+                want = torch.softmax(s, 0) @ v[keep, h // 2]
+                assert float((out[row, h].cpu().double() - want).abs().max()) <= 2e-5 * float(v[keep].abs().max())
+                assert abs(float(lse[row, h]) - float(torch.logsumexp(s, 0))) <= 2e-5 * max(1, abs(float(lse[row, h])))
+            row += 1
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_nan_reaches_only_the_rows_that_attend_it(dtype):
+    """A NaN among a token's keys or values: rows that stand before it, or whose window has passed it, are as without it."""
+    new, past = [6, 1, 40], [30, 100, 0]
+    batch, total = ref.make_batch(new, past, 16, 2, 64, seed=3)
+    q = rows_of(sum(new), 4, 64, dtype)
+    k_cache, v_cache = batch["cache"][:2]
+    clean = lm.attention(q, window=24, **batch)
+
+    def put(cache, b, token, head, element):
+        at = int(batch["block_table"][b, token // 16])
+        cache.view(torch.uint8)[at, head, token % 16, element] = 0xff
+
+    put(v_cache, 0, 33, 0, 5)          # rows 3.. of sequence 0 attend it
+    put(k_cache, 0, 34, 1, 0)
+    put(v_cache, 1, 10, 0, 1)          # out of the window of the only row
+    put(k_cache, 1, 40, 1, 9)
+    put(v_cache, 2, 7, 1, 63)          # rows 7..30
+    out, lse = lm.attention(q, window=24, **batch)
+    hit = torch.zeros(out.shape, dtype=torch.bool, device="cuda")
+    hit[3:6, 0:2, 5] = True
+    hit[4:6, 2:4] = True
+    hit[7 + 7:7 + 31, 2:4, 63] = True
+    assert torch.equal(torch.isnan(out), hit)
+    # other rows may move their unit of weights at another key than before: as near as rounding
+    assert float((out[~hit] - clean[0][~hit]).abs().max()) <= 2 * ref.LIMIT[dtype] * float(batch["cache"][1].float().nan_to_num().abs().max() * batch["cache"][3].max())
+    keys_hit = torch.zeros(lse.shape, dtype=torch.bool, device="cuda")
+    keys_hit[4:6, 2:4] = True
+    assert torch.equal(torch.isnan(lse), keys_hit) and torch.allclose(lse[~keys_hit], clean[1][~keys_hit], rtol=2e-5, atol=2e-5)
+
+
+def test_scores_far_apart_and_values_of_many_sizes():
+    """Weights that vanish against later ones, pages whose scales differ by 2^20, queries from tiny to large."""
+    new, past = [1, 1, 1], [600, 40, 1000]
+    batch, total = ref.make_batch(new, past, 16, 2, 64, seed=8)
+    batch["cache"][3].mul_(torch.exp2(torch.randint(-10, 11, batch["cache"][3].shape, generator=torch.Generator().manual_seed(0)).float()).cuda())
+    for amplitude in (1e-6, 20.0, 3000.0):
+        q = rows_of(3, 8, 64, F32, amplitude=amplitude)
+        out, lse = lm.attention(q, **batch)
+        want, want_lse, top = ref.attention64(q, batch, total, new)
+        # a score's error grows with it: a few roundings of 2^-23 of the largest, on weights and statistics
+        tol = max(2e-5, 2.0 ** -20 * float(want_lse.abs().max()))
+        assert float((out.cpu().double() - want).abs().max()) <= 4 * tol * top, amplitude
+        assert float((lse.cpu().double() - want_lse).abs().max()) <= 2 * tol, amplitude
+
+
+def test_offsets_beyond_32_bits():
+    """Pages that lie more than 4 GB into the cache."""
+    page, heads, dim = 256, 2, 256
+    stride = heads * page * dim
+    pages = (5 << 30) // stride
+    k = torch.empty(pages, heads, page, dim, dtype=torch.uint8, device="cuda").view(ref.E4M3)
+    v = torch.empty(pages, heads, page, dim, dtype=torch.uint8, device="cuda").view(ref.E4M3)
+    ks, vs = torch.ones(pages, heads, device="cuda"), torch.ones(pages, heads, device="cuda")
+    new, total = [1, 1], [300, 256]
+    table = torch.tensor([[pages - 1, pages - 3], [pages - 2, -1]], dtype=torch.int32, device="cuda")
+    g = torch.Generator().manual_seed(0)
+    for c in (k, v):
+        for p in (1, 2, 3):
+            c[pages - p] = torch.randn(heads, page, dim, generator=g).to(ref.E4M3).cuda()
+    batch = dict(cache=(k, v, ks, vs), block_table=table, kv_len=torch.tensor(total, dtype=torch.int32, device="cuda"), max_kv_len=300)
+    q = rows_of(2, 4, dim, BF16)
+    small = dict(cache=(k[pages - 3:], v[pages - 3:], ks[pages - 3:], vs[pages - 3:]), block_table=(table - (pages - 3)).clamp(min=-1))
+    ref.check_attention(lm.attention(q, **batch), ref.attention64(q, small, total, new), BF16)
+    kn, vn = rows_of(2, heads, dim, BF16, seed=5), rows_of(2, heads, dim, BF16, seed=6)
+    lm.append(kn, vn, **batch)
+    got = k[pages - 3].float()[:, (300 - 1) % page] * ks[pages - 3][:, None]
+    assert float((got - kn[0].float()).abs().max()) <= float(kn[0].abs().max()) * 2.0 ** -4
+
+
+def test_calls_on_another_stream_and_in_a_graph():
+    new, past = [1] * 6, [50, 100, 2000, 7, 0, 900]
+    batch, total = ref.make_batch(new, past, 64, 2, 128)
+    q = rows_of(6, 8, 128, BF16)
+    want = lm.attention(q, **batch)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = lm.attention(q, **batch)
+    side.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = lm.attention(q, **batch)
+    batch["kv_len"] -= torch.tensor([0, 1, 64, 7, 0, 500], dtype=torch.int32, device="cuda")   # shorter: the device's lengths count
+    graph.replay()
+    shorter = lm.attention(q, **batch)
+    torch.cuda.synchronize()
+    assert torch.equal(captured[0], shorter[0]) and torch.equal(captured[1], shorter[1])
+    assert not torch.equal(shorter[0], want[0])
+
+
+def test_the_same_call_gives_the_same_bits():
+    new, past = [1] * 3 + [5], [5000, 1, 800, 77]
+    batch, total = ref.make_batch(new, past, 32, 4, 128)
+    q = rows_of(8, 16, 128, F32)
+    a, b = lm.attention(q, **batch), lm.attention(q, **batch)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+# --------------------------------------------------------------------------------------------------------- append
+def check_append(new, past, page, heads, kv_heads, dim, rotary, interleaved, dtype, seed=0, spoil=None, token_major=False):
+    batch, total = ref.make_batch(new, past, page, kv_heads, dim, seed=seed, token_major=token_major)
+    rows = sum(new)
+    qkv = rows_of(rows, heads + 2 * kv_heads, dim, dtype, seed=seed + 1, amplitude=2.0)
+    q, k, v = qkv[:, :heads], qkv[:, heads:heads + kv_heads], qkv[:, heads + kv_heads:]
+    if spoil:
+        spoil(k, v, batch)
+    table = lm.rotary_table(max(max(total), 1), rotary) if rotary else None
+    before = [t.clone() for t in batch["cache"]]
+    positions = torch.tensor([p + i for n, p in zip(new, past) for i in range(n)])
+    kr, qr = k.cpu().float(), q.cpu().float()
+    if rotary:
+        kr, qr = ref.rotated32(k.cpu(), table.cpu(), positions, interleaved), ref.rotated32(q.cpu(), table.cpu(), positions, interleaved)
+    want = [ref.append32(x, before[i], before[2 + i], batch["block_table"].cpu(), new, total) for i, x in ((0, kr), (1, v.cpu().float()))]
+    out = lm.append(k, v, q=q, rotary=table, interleaved=interleaved, **batch)
+    got = batch["cache"]
+    for i in range(2):
+        assert torch.equal(got[2 + i].cpu(), want[i][1]), "scales"
+        assert ref.same_bytes(got[i], want[i][0]), "values"
+    assert out.dtype == dtype and torch.equal(out.cpu().nan_to_num(), qr.to(dtype).nan_to_num())
+    return batch, total
+
+
+APPENDS = [
+    # new, past, page, q heads, kv heads, dim, rotary, neighbours
+    ([1], [0], 16, 4, 1, 64, 64, False),
+    ([1], [700], 64, 32, 8, 128, 128, False),
+    ([1] * 7, [15, 16, 17, 0, 300, 63, 1], 16, 6, 2, 64, 32, True),
+    ([1, 1], [100, 31], 32, 3, 3, 80, 80, False),
+    ([1, 1], [100, 31], 32, 5, 1, 80, 40, True),
+    ([2, 1, 9], [14, 0, 70], 16, 4, 2, 48, 0, False),
+    ([40, 1, 17], [3, 333, 0], 16, 8, 2, 128, 64, False),
+    ([130, 300], [0, 60], 256, 2, 1, 256, 256, False),          # more of a page than the registers hold
+    ([0, 5, 0, 33], [10, 5, 0, 1], 32, 2, 2, 16, 8, False),
+    ([70] * 40, [0] * 40, 64, 2, 1, 32, 32, False),             # more sequences than a warp has lanes
+]
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("case", range(len(APPENDS)))
+def test_append(case, dtype):
+    check_append(*APPENDS[case], dtype, seed=case)
+
+
+def test_append_to_a_token_major_cache():
+    check_append([3, 1], [20, 40], 16, 4, 2, 64, 64, False, BF16, token_major=True)
+
+
+def test_append_of_values_that_are_not_finite():
+    """An infinity becomes the largest value, a NaN stays one, and the page's scale is that of the others."""
+    def spoil(k, v, batch):
+        v[0, 0, 3] = math.inf
+        v[1, 1, 4] = -math.inf
+        v[2, 0, 5] = math.nan
+        v[5] = 0
+        v[6, 1] = math.nan
+    check_append([7], [16], 16, 2, 2, 64, 0, False, F32, spoil=spoil)
+
+
+def test_append_without_a_page_stores_nothing():
+    def spoil(k, v, batch):
+        batch["block_table"][0, 1] = -1
+    check_append([20, 3], [5, 0], 16, 2, 2, 64, 64, False, F32, spoil=spoil)
+
+
+def test_tokens_one_by_one():
+    """A text appended token by token: each value within half a step of e4m3 at its page's final scale, which is the one that the page's
+    largest value needs. (A value that a growing scale has made subnormal is rounded once more.)"""
+    page, heads, dim, n = 16, 2, 64, 50
+    g = torch.Generator().manual_seed(4)
+    x = torch.randn(n, heads, dim, generator=g) * torch.exp2(torch.linspace(-6, 6, n))[:, None, None]
+    cache = lm.new_cache(8, heads, page, dim)
+    table = torch.tensor([[5, 0, 3, 7]], dtype=torch.int32, device="cuda")
+    for t in range(n):
+        row = x[t:t + 1].cuda()
+        assert lm.append(row, row, cache, table, torch.tensor([t + 1], dtype=torch.int32, device="cuda"), n) is None
+    for c, s in ((cache[0], cache[2]), (cache[1], cache[3])):
+        got = ref.cached(c, s, table[0], n)
+        for first in range(0, n, page):
+            part = x[first:first + page]
+            scale = ref.scale_for(part.abs().amax((0, 2)))
+            assert torch.equal(s[int(table[0, first // page])].cpu(), scale)
+            step = torch.maximum(part.abs().double() * 2.0 ** -4, scale.double()[None, :, None] * 2.0 ** -9)
+            assert bool(((got[first:first + page] - part.double()).abs() <= step).all())
+
+
+def test_rotation_in_place():
+    batch, total = ref.make_batch([2, 1], [3, 9], 16, 1, 64)
+    table = lm.rotary_table(16, 64)
+    k, q = rows_of(3, 1, 64, F16), rows_of(3, 4, 64, F16, seed=9)
+    want = lm.append(k, k, q=q.clone(), rotary=table, **batch)
+    got = lm.append(k, k, q=q, rotary=table, out=q, **batch)
+    assert got.data_ptr() == q.data_ptr() and torch.equal(got, want)
+
+
+# --------------------------------------------------------------------------------------------------------- logits
+def logits32(x, tokens, starts, prompt, rep, pres, freq, biases, allowed):
+    """Row by row in fp32, each step rounded."""
+    x = x.astype(np.float32).copy()
+    rows, vocab = x.shape
+    for r in range(rows):
+        if tokens is not None:
+            t = tokens[starts[r]:starts[r + 1]]
+            inside = (t >= 0) & (t < vocab)
+            n_prompt = prompt[r] if prompt is not None else 0
+            seen = np.unique(t[inside])
+            counts = np.bincount(t[n_prompt:][inside[n_prompt:]], minlength=vocab)
+            if rep is not None:
+                x[r, seen] = np.where(x[r, seen] > 0, x[r, seen] / rep[r], x[r, seen] * rep[r])
+            said = np.nonzero(counts)[0]
+            f = freq[r] if freq is not None else np.float32(0)
+            p = pres[r] if pres is not None else np.float32(0)
+            x[r, said] = (x[r, said] - f * counts[said].astype(np.float32)) - p
+        if biases is not None:
+            last = {int(t): v for t, v in zip(*biases[r])}
+            for t, v in last.items():
+                if 0 <= t < vocab:
+                    x[r, t] = x[r, t] + v
+        if allowed is not None:
+            words = allowed[r if allowed.ndim == 2 else slice(None)]
+            bits = (words[np.arange(vocab) // 32].view(np.uint32) >> (np.arange(vocab) % 32).astype(np.uint32)) & 1
+            x[r, bits == 0] = -np.inf
+    return x
+
+
+def logits_case(rows, vocab, history, n_bias, masked, dtype, seed=0):
+    rng = np.random.default_rng(seed)
+    x = torch.from_numpy((4 * rng.standard_normal((rows, vocab))).astype(np.float32)).to(dtype)
+    counts = rng.integers(0, history + 1, rows)
+    starts = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    tokens = (rng.random(starts[-1]) ** 3 * (vocab + 2)).astype(np.int32) - 1          # some outside
+    prompt = rng.integers(0, history + 1, rows).astype(np.int32)
+    rep, pres, freq = ((1 + rng.random(rows)).astype(np.float32), rng.random(rows).astype(np.float32), rng.standard_normal(rows).astype(np.float32))
+    biases = [(rng.integers(-1, vocab + 1, n_bias).astype(np.int32), rng.standard_normal(n_bias).astype(np.float32)) for _ in range(rows)] if n_bias else None
+    allowed = rng.integers(-2 ** 31, 2 ** 31, (rows, (vocab + 31) // 32)).astype(np.int32) if masked else None
+    return x, tokens, starts, prompt, rep, pres, freq, biases, allowed
+
+
+def run_logits(x, tokens, starts, prompt, rep, pres, freq, biases, allowed, **more):
+    d = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda() if a is not None else None  # noqa: E731
+    bt = bv = bs = None
+    if biases is not None:
+        bt, bv = np.concatenate([b[0] for b in biases]), np.concatenate([b[1] for b in biases])
+        bs = np.concatenate([[0], np.cumsum([len(b[0]) for b in biases])]).astype(np.int32)
+    return lm.adjust_logits(x.cuda(), d(tokens), d(starts), d(prompt), d(rep), d(pres), d(freq), d(bt), d(bv), d(bs), d(allowed), **more)
+
+
+@pytest.mark.parametrize("rows,vocab,history,n_bias,masked", [
+    (1, 1, 3, 1, True), (1, 31, 10, 0, True), (3, 33, 40, 5, True), (2, 4095, 300, 20, False), (5, 4096, 0, 7, True),
+    (4, 4097, 5000, 0, True), (3, 32000, 800, 20, True), (2, 50001, 3000, 300, True), (33, 1003, 50, 3, False), (7, 8190, 200, 40, True)])
+@pytest.mark.parametrize("dtype,out_dtype", [(F32, F32), (F16, F16), (F16, F32), (BF16, BF16), (BF16, F32)])
+def test_logits(rows, vocab, history, n_bias, masked, dtype, out_dtype):
+    """Equal to the formula in fp32, rounded once to the result's type. (Odd vocabularies: rows begin anywhere.)"""
+    case = logits_case(rows, vocab, history, n_bias, masked, dtype, seed=vocab)
+    got = run_logits(*case, out_dtype=out_dtype)
+    want = torch.from_numpy(logits32(case[0].float().numpy(), *case[1:])).to(out_dtype)
+    assert got.dtype == out_dtype and torch.equal(got.cpu(), want)
+
+
+def test_logits_steps_that_are_left_out():
+    x, tokens, starts, prompt, rep, pres, freq, biases, allowed = logits_case(4, 3000, 100, 6, True, F32)
+    full = (tokens, starts, prompt, rep, pres, freq, biases, allowed)
+    for gone in ((0, 1, 2, 3, 4, 5, 6), (2,), (3,), (4, 5), (6,), (7,), (0, 1, 2, 3, 4, 5, 7), (0, 1, 2, 3, 4, 5, 6, 7)):
+        part = [None if i in gone else a for i, a in enumerate(full)]
+        assert torch.equal(run_logits(x, *part).cpu(), torch.from_numpy(logits32(x.numpy(), *part)))
+    one_mask = allowed[1]
+    assert torch.equal(run_logits(x, *full[:-1], one_mask).cpu(), torch.from_numpy(logits32(x.numpy(), *full[:-1], one_mask)))
+
+
+def test_logits_in_place_in_slices_and_not_finite():
+    x, tokens, starts, prompt, rep, pres, freq, biases, allowed = logits_case(5, 777, 60, 4, True, F32)
+    x[0, 5], x[1, 6], x[2, 7] = math.inf, -math.inf, math.nan
+    allowed[2, 0] &= ~(1 << 7)                                  # the NaN is masked: it becomes minus infinity
+    want = torch.from_numpy(logits32(x.numpy(), tokens, starts, prompt, rep, pres, freq, biases, allowed))
+    for offset in (0, 1, 2, 3):
+        wide = torch.full((5, 800), 9.0, device="cuda")
+        wide[:, offset:offset + 777] = x.cuda()
+        view = wide[:, offset:offset + 777]
+        d = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+        bt, bv = np.concatenate([b[0] for b in biases]), np.concatenate([b[1] for b in biases])
+        got = lm.adjust_logits(view, d(tokens), d(starts), d(prompt), d(rep), d(pres), d(freq), d(bt), d(bv),
+                               d(np.arange(6, dtype=np.int32) * 4), d(allowed), out=view)
+        assert got.data_ptr() == view.data_ptr() and torch.equal(got.cpu(), want)
+        assert bool((wide[:, :offset] == 9).all()) and bool((wide[:, offset + 777:] == 9).all())
+    assert float(want[2, 7]) == -math.inf
+
+
+def test_logits_between_unlike_strides():
+    """A result that lies differently from the logits: element by element."""
+    x, *rest = logits_case(3, 500, 30, 2, True, BF16)
+    out = torch.zeros(3, 511, device="cuda")[:, 3:503]
+    got = run_logits(x, *rest, out=out)
+    assert torch.equal(got.cpu(), torch.from_numpy(logits32(x.float().numpy(), *rest)))
+
+
+def test_nothing_waited_in_vain():
+    assert _lib.cuda_lib().ogle_cuda_device_status() == 0
