@@ -22,75 +22,99 @@ struct AppendArgs {
     int q_blocks;                 // blocks of kQHeads query heads
 };
 
-constexpr int kQHeads = 4;        // query heads of a block
-constexpr int kHold = 4;          // pieces of 8 values a thread keeps
+constexpr int kQHeads = 4;        // query heads of a block: they share a row's angles
+constexpr int kHoldValues = 32;   // values a thread keeps
 constexpr int kMaxThreads = 256;
 
-// 8 values of a head: `at` and the four behind it, `at2` and the four behind that. A piece inside the rotated part with pairs
-// rotary_dim / 2 apart has both halves of its pairs; every other piece is 8 neighbours.
+// A piece is 2 W values of a head in two vectors of W: at `at` and at `at2`. Inside the rotated part, with pairs rotary_dim / 2
+// apart, they are both halves of W pairs; every other piece is neighbours.
 struct Piece { int at, at2, angle; };  // angle: first column of the table's cosines, -1: not rotated
 
+template <int W>
 __device__ __forceinline__ Piece piece_of(int i, int rotary_dim, bool interleaved) {
     Piece p;
-    p.at = i * 8;
-    p.at2 = p.at + 4;
+    p.at = i * 2 * W;
+    p.at2 = p.at + W;
     p.angle = -1;
     if (p.at < rotary_dim) {
-        if (interleaved) {
-            p.angle = i * 4;
-        } else {
-            p.at = i * 4;
+        p.angle = i * W;
+        if (!interleaved) {
+            p.at = i * W;
             p.at2 = p.at + rotary_dim / 2;
-            p.angle = p.at;
         }
     }
     return p;
 }
 
-template <typename T>
-__device__ __forceinline__ void load4(const T* p, float* x) {
-    if constexpr (std::is_same<T, float>::value) {
-        const float4 v = *reinterpret_cast<const float4*>(p);
-        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+// W values as they lie: one vector of 16 bytes, or of 8.
+template <typename T, int W>
+struct Raw { uint32_t w[W * sizeof(T) / 4]; };
+template <typename T, int W>
+__device__ __forceinline__ Raw<T, W> load_raw(const T* p) {
+    Raw<T, W> r;
+    if constexpr (W * sizeof(T) == 16) {
+        const uint4 v = *reinterpret_cast<const uint4*>(p);
+        r.w[0] = v.x; r.w[1] = v.y; r.w[2] = v.z; r.w[3] = v.w;
     } else {
         const uint2 v = *reinterpret_cast<const uint2*>(p);
-        const T* h = reinterpret_cast<const T*>(&v);
+        r.w[0] = v.x; r.w[1] = v.y;
+    }
+    return r;
+}
+template <typename T, int W>
+__device__ __forceinline__ void unpack(const Raw<T, W>& r, float* x) {
+    const T* h = reinterpret_cast<const T*>(r.w);
 #pragma unroll
-        for (int l = 0; l < 4; ++l) x[l] = float(h[l]);
+    for (int l = 0; l < W; ++l) x[l] = float(h[l]);
+}
+template <typename T, int W>
+__device__ __forceinline__ void store_values(T* p, const float* x) {
+    Raw<T, W> r;
+    T* h = reinterpret_cast<T*>(r.w);
+#pragma unroll
+    for (int l = 0; l < W; ++l) h[l] = T(x[l]);
+    if constexpr (W * sizeof(T) == 16) *reinterpret_cast<uint4*>(p) = make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]);
+    else *reinterpret_cast<uint2*>(p) = make_uint2(r.w[0], r.w[1]);
+}
+
+template <int W>
+__device__ __forceinline__ void load_angles(const float* p, float (&c)[W]) {
+#pragma unroll
+    for (int l = 0; l < W; l += 4) {
+        const float4 v = __ldg(reinterpret_cast<const float4*>(p + l));
+        c[l] = v.x; c[l + 1] = v.y; c[l + 2] = v.z; c[l + 3] = v.w;
     }
 }
 
-template <typename T>
-__device__ __forceinline__ void store4(T* p, const float* x) {
-    if constexpr (std::is_same<T, float>::value) {
-        *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
-    } else {
-        uint2 v;
-        T* h = reinterpret_cast<T*>(&v);
+// Products and sums are rounded one by one (no fused multiply-add): what is stored in 8 bits is then the same as from any other
+// evaluation of the formula in fp32, where a fused one crosses a rounding boundary now and then.
+template <int W>
+__device__ __forceinline__ void rotate(float (&x)[2 * W], const float (&c)[W], const float (&s)[W], bool interleaved) {
 #pragma unroll
-        for (int l = 0; l < 4; ++l) h[l] = T(x[l]);
-        *reinterpret_cast<uint2*>(p) = v;
-    }
-}
-
-// The piece's values, rotated. Products and sums are rounded one by one (no fused multiply-add): what is stored in 8 bits is
-// then the same as from any other evaluation of the formula in fp32, where a fused one crosses a rounding boundary now and then.
-template <typename T>
-__device__ __forceinline__ void load_piece(const T* row, const Piece& p, const float* cs, int half, bool interleaved, float (&x)[8]) {
-    load4(row + p.at, x);
-    load4(row + p.at2, x + 4);
-    if (p.angle < 0) return;
-    float c[4], s[4];
-    load4(cs + p.angle, c);
-    load4(cs + half + p.angle, s);
-#pragma unroll
-    for (int l = 0; l < 4; ++l) {
+    for (int l = 0; l < W; ++l) {
         float& a = interleaved ? x[2 * l] : x[l];
-        float& b = interleaved ? x[2 * l + 1] : x[4 + l];
+        float& b = interleaved ? x[2 * l + 1] : x[W + l];
         const float u = __fsub_rn(__fmul_rn(a, c[l]), __fmul_rn(b, s[l]));
         const float v = __fadd_rn(__fmul_rn(b, c[l]), __fmul_rn(a, s[l]));
         a = u;
         b = v;
+    }
+}
+
+template <typename T, int W>
+__device__ __forceinline__ void load_piece(const T* row, const Piece& p, const float* cs, int half, bool interleaved, float (&x)[2 * W]) {
+    const Raw<T, W> lo = load_raw<T, W>(row + p.at), hi = load_raw<T, W>(row + p.at2);
+    if (p.angle >= 0) {
+        float c[W], s[W];
+        load_angles<W>(cs + p.angle, c);
+        load_angles<W>(cs + half + p.angle, s);
+        unpack<T, W>(lo, x);
+        unpack<T, W>(hi, x + W);
+        if (interleaved) rotate<W>(x, c, s, true);
+        else rotate<W>(x, c, s, false);
+    } else {
+        unpack<T, W>(lo, x);
+        unpack<T, W>(hi, x + W);
     }
 }
 
@@ -106,7 +130,7 @@ __device__ __forceinline__ float finite_abs(float x) {
     return a <= 3.402823466e38f ? a : 0.f;
 }
 
-template <typename T>
+template <typename T, int W>
 __global__ void __launch_bounds__(kMaxThreads) paged_append_kernel(AppendArgs a) {
     __shared__ int where[4];
     __shared__ float warp_max[kMaxThreads / 32];
@@ -155,20 +179,43 @@ __global__ void __launch_bounds__(kMaxThreads) paged_append_kernel(AppendArgs a)
     const int block = (begin >> B.page_shift) + nth;             // of the sequence's blocks of tokens
     const int t0 = max(begin, block << B.page_shift), t1 = min(s.len, (block + 1) << B.page_shift);
     const int row0 = s.row0 + s.n - s.len;                       // row of token t: row0 + t
-    const int pieces = B.dim / 8, half = a.rotary_dim / 2;
+    // a thread has one piece of every `stride`-th token
+    const int pieces = B.dim / (2 * W), half = a.rotary_dim / 2, stride = int(blockDim.x) / pieces, my_piece = tid % pieces;
+    const int my_t = tid / pieces < stride ? t0 + tid / pieces : t1;
     const bool inter = a.interleaved != 0;
 
     if (int(blockIdx.y) >= 2 * B.kv_heads) {                     // queries: rotated and stored as they came
         const int h0 = (blockIdx.y - 2 * B.kv_heads) * kQHeads, heads = min(kQHeads, B.q_heads - h0);
-        const int per_token = pieces * heads, total = (t1 - t0) * per_token;
-        for (int i = tid; i < total; i += blockDim.x) {
-            const int t = t0 + i / per_token, r = i % per_token, h = h0 + r / pieces;
-            const Piece p = piece_of(r % pieces, a.rotary_dim, inter);
-            float x[8];
-            load_piece(static_cast<const T*>(a.q) + (row0 + t) * a.q_row + h * a.q_head, p, a.rotary + (long long)t * a.rotary_dim, half, inter, x);
-            T* y = static_cast<T*>(a.q_out) + (row0 + t) * a.qo_row + h * a.qo_head;
-            store4(y + p.at, x);
-            store4(y + p.at2, x + 4);
+        const Piece p = piece_of<W>(my_piece, a.rotary_dim, inter);
+        for (int t = my_t; t < t1; t += stride) {
+            const T* x0 = static_cast<const T*>(a.q) + (row0 + t) * a.q_row + h0 * a.q_head;
+            T* y0 = static_cast<T*>(a.q_out) + (row0 + t) * a.qo_row + h0 * a.qo_head;
+            Raw<T, W> lo[kQHeads], hi[kQHeads];
+#pragma unroll
+            for (int h = 0; h < kQHeads; ++h)
+                if (h < heads) {
+                    lo[h] = load_raw<T, W>(x0 + h * a.q_head + p.at);
+                    hi[h] = load_raw<T, W>(x0 + h * a.q_head + p.at2);
+                }
+            float c[W], s[W];
+            if (p.angle >= 0) {
+                const float* cs = a.rotary + (long long)t * a.rotary_dim + p.angle;
+                load_angles<W>(cs, c);
+                load_angles<W>(cs + half, s);
+            }
+#pragma unroll
+            for (int h = 0; h < kQHeads; ++h)
+                if (h < heads) {
+                    float x[2 * W];
+                    unpack<T, W>(lo[h], x);
+                    unpack<T, W>(hi[h], x + W);
+                    if (p.angle >= 0) {
+                        if (inter) rotate<W>(x, c, s, true);
+                        else rotate<W>(x, c, s, false);
+                    }
+                    store_values<T, W>(y0 + h * a.qo_head + p.at, x);
+                    store_values<T, W>(y0 + h * a.qo_head + p.at2, x + W);
+                }
         }
         return;
     }
@@ -180,25 +227,27 @@ __global__ void __launch_bounds__(kMaxThreads) paged_append_kernel(AppendArgs a)
     const long long x_row = keys ? a.k_row : a.v_row;
     unsigned char* out = (keys ? B.k_cache : B.v_cache) + page * B.page_stride + h * B.head_stride;
     float* scale = (keys ? B.k_scale : B.v_scale) + (long long)page * B.kv_heads + h;
-    const int rotary_dim = keys ? a.rotary_dim : 0, total = (t1 - t0) * pieces, slot0 = t0 & (page_tokens - 1);
+    const int rotary_dim = keys ? a.rotary_dim : 0, slot0 = t0 & (page_tokens - 1);
+    const Piece p = piece_of<W>(my_piece, rotary_dim, inter);
 
-    float x[kHold][8], top = 0.f;
+    constexpr int kHold = kHoldValues / (2 * W);
+    float x[kHold][2 * W], top = 0.f;
 #pragma unroll
     for (int u = 0; u < kHold; ++u) {
-        const int i = tid + u * blockDim.x;
-        if (i < total) {
-            const int t = t0 + i / pieces;
-            load_piece(x0 + (row0 + t) * x_row, piece_of(i % pieces, rotary_dim, inter), a.rotary + (long long)t * rotary_dim, half, inter, x[u]);
-#pragma unroll
-            for (int l = 0; l < 8; ++l) top = fmaxf(top, finite_abs(x[u][l]));
-        }
+        const int t = my_t + u * stride;
+        if (t < t1) load_piece<T, W>(x0 + (row0 + t) * x_row, p, a.rotary + (long long)t * rotary_dim, half, inter, x[u]);
     }
-    for (int i = tid + kHold * blockDim.x; i < total; i += blockDim.x) {      // pages of more than the registers hold
-        const int t = t0 + i / pieces;
-        float z[8];
-        load_piece(x0 + (row0 + t) * x_row, piece_of(i % pieces, rotary_dim, inter), a.rotary + (long long)t * rotary_dim, half, inter, z);
 #pragma unroll
-        for (int l = 0; l < 8; ++l) top = fmaxf(top, finite_abs(z[l]));
+    for (int u = 0; u < kHold; ++u)
+        if (my_t + u * stride < t1) {
+#pragma unroll
+            for (int l = 0; l < 2 * W; ++l) top = fmaxf(top, finite_abs(x[u][l]));
+        }
+    for (int t = my_t + kHold * stride; t < t1; t += stride) {    // pages of more than the registers hold
+        float z[2 * W];
+        load_piece<T, W>(x0 + (row0 + t) * x_row, p, a.rotary + (long long)t * rotary_dim, half, inter, z);
+#pragma unroll
+        for (int l = 0; l < 2 * W; ++l) top = fmaxf(top, finite_abs(z[l]));
     }
 #pragma unroll
     for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
@@ -214,26 +263,27 @@ __global__ void __launch_bounds__(kMaxThreads) paged_append_kernel(AppendArgs a)
     if (now <= 0.f) now = 1.f;
     const float inverse = 1.f / now;                             // a power of two: exact
 
-    auto store = [&](int i, const float (&z)[8]) {
-        const Piece p = piece_of(i % pieces, rotary_dim, inter);
-        unsigned char* y = out + (long long)(slot0 + i / pieces) * B.token_stride;
-        const uint32_t lo = paged::e4m3x2(z[0] * inverse, z[1] * inverse) | paged::e4m3x2(z[2] * inverse, z[3] * inverse) << 16;
-        const uint32_t hi = paged::e4m3x2(z[4] * inverse, z[5] * inverse) | paged::e4m3x2(z[6] * inverse, z[7] * inverse) << 16;
-        if (p.at2 == p.at + 4) {
-            *reinterpret_cast<uint2*>(y + p.at) = make_uint2(lo, hi);
+    auto store = [&](int t, const float (&z)[2 * W]) {
+        unsigned char* y = out + (long long)(t & (page_tokens - 1)) * B.token_stride;
+        uint32_t w[W / 2];
+#pragma unroll
+        for (int l = 0; l < W / 2; ++l)
+            w[l] = paged::e4m3x2(z[4 * l] * inverse, z[4 * l + 1] * inverse) | paged::e4m3x2(z[4 * l + 2] * inverse, z[4 * l + 3] * inverse) << 16;
+        if constexpr (W == 8) {
+            *reinterpret_cast<uint2*>(y + p.at) = make_uint2(w[0], w[1]);
+            *reinterpret_cast<uint2*>(y + p.at2) = make_uint2(w[2], w[3]);
         } else {
-            *reinterpret_cast<uint32_t*>(y + p.at) = lo;
-            *reinterpret_cast<uint32_t*>(y + p.at2) = hi;
+            *reinterpret_cast<uint32_t*>(y + p.at) = w[0];
+            *reinterpret_cast<uint32_t*>(y + p.at2) = w[1];
         }
     };
 #pragma unroll
     for (int u = 0; u < kHold; ++u)
-        if (tid + u * int(blockDim.x) < total) store(tid + u * blockDim.x, x[u]);
-    for (int i = tid + kHold * blockDim.x; i < total; i += blockDim.x) {
-        const int t = t0 + i / pieces;
-        float z[8];
-        load_piece(x0 + (row0 + t) * x_row, piece_of(i % pieces, rotary_dim, inter), a.rotary + (long long)t * rotary_dim, half, inter, z);
-        store(i, z);
+        if (my_t + u * stride < t1) store(my_t + u * stride, x[u]);
+    for (int t = my_t + kHold * stride; t < t1; t += stride) {
+        float z[2 * W];
+        load_piece<T, W>(x0 + (row0 + t) * x_row, p, a.rotary + (long long)t * rotary_dim, half, inter, z);
+        store(t, z);
     }
     if (slot0 > 0 && old < now) {                                // what the page has already moves to the new scale
         const float ratio = old * inverse;
@@ -283,15 +333,17 @@ extern "C" int ogle_cuda_kv_append(const OglePagedBatch* batch, const OgleAppend
     long pages = B.max_rows == 1 ? B.n_seqs : (long)(B.n_rows >> B.page_shift) + 2L * B.n_seqs;
     if (B.max_rows > 1 && pages > B.n_rows) pages = B.n_rows;
     const int tokens = B.max_rows < (1 << B.page_shift) ? B.max_rows : 1 << B.page_shift;
-    int threads = div_up((long)tokens * B.dim / 8, kHold) * (tokens == 1 ? kHold : 1);
-    threads = (threads + 31) / 32 * 32;
+    // 16 bytes of 16-bit values at a time where the rotated part is whole pieces of that
+    const bool wide = dt != OGLE_F32 && a.rotary_dim % 16 == 0;
+    const int pieces = B.dim / (wide ? 16 : 8), hold = kHoldValues / (wide ? 16 : 8);
+    int threads = (div_up(tokens, hold) * pieces + 31) / 32 * 32;
     if (threads > kMaxThreads) threads = kMaxThreads;
     const dim3 grid((unsigned)pages, unsigned(2 * B.kv_heads + a.q_blocks));
-    cudaStream_t s = stream;
+    const auto run = [&](auto kernel) { return launch_overlapped(kernel, grid, dim3(threads), 0, stream, a); };
     cudaError_t e;
-    if (dt == OGLE_F32) e = launch_overlapped(paged_append_kernel<float>, grid, dim3(threads), 0, s, a);
-    else if (dt == OGLE_F16) e = launch_overlapped(paged_append_kernel<__half>, grid, dim3(threads), 0, s, a);
-    else e = launch_overlapped(paged_append_kernel<__nv_bfloat16>, grid, dim3(threads), 0, s, a);
+    if (dt == OGLE_F32) e = run(paged_append_kernel<float, 4>);
+    else if (dt == OGLE_F16) e = wide ? run(paged_append_kernel<__half, 8>) : run(paged_append_kernel<__half, 4>);
+    else e = wide ? run(paged_append_kernel<__nv_bfloat16, 8>) : run(paged_append_kernel<__nv_bfloat16, 4>);
     if (e != cudaSuccess) { set_last_error(e); (void)cudaGetLastError(); return OGLE_ERR_CUDA; }
     return finish_launch();
 }
