@@ -32,7 +32,7 @@ inline int translate(const OglePagedBatch* b, Batch& out) {
     // rows x heads and tokens are counted in 32 bits
     if ((long long)b->n_rows * b->q_heads > (1LL << 30) || b->max_kv_len > (1 << 30)) return OGLE_ERR_UNSUPPORTED;
     if ((b->page_stride | b->head_stride | b->token_stride) & 15) return OGLE_ERR_ALIGNMENT;
-    if (b->page_stride < 0 || b->head_stride < 0 || b->token_stride < b->head_dim) return OGLE_ERR_INVALID;
+    if (b->page_stride < 1 || b->head_stride < 1 || b->token_stride < b->head_dim) return OGLE_ERR_INVALID;
     out = Batch{};
     if (b->n_seqs == 0 || b->n_rows == 0) return OGLE_OK;
     if (!b->kv_len || !b->block_table || !b->k_cache || !b->v_cache || !b->k_scale || !b->v_scale) return OGLE_ERR_INVALID;
@@ -89,6 +89,11 @@ __device__ __forceinline__ uint32_t e4m3x2_to_half2(uint16_t v) {
     uint32_t r;
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(v));
     return r;
+}
+// Four of them: the lower two, the upper two.
+__device__ __forceinline__ void e4m3x4_to_half2(uint32_t v, uint32_t& lower, uint32_t& upper) {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(lower), "=r"(upper) : "r"(v));
 }
 // Two fp32 as e4m3, round to nearest even, beyond 448 the largest value, NaN as NaN.
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {

@@ -16,6 +16,8 @@
 #include <type_traits>
 
 #include "paged.cuh"
+#include "tc_common.cuh"
+#include "tma_host.h"
 
 namespace ogle {
 namespace {
@@ -25,6 +27,8 @@ using paged::Batch;
 constexpr int kWarps = 4;
 constexpr int kChunk = 16;                       // keys of a warp's step; a page holds whole steps
 constexpr int kTileKeys = kWarps * kChunk;
+constexpr int kSegmentCost = 2;                  // tiles that a segment's beginning and end take as long as
+constexpr int kGaveUp = 9;                       // in the library's device status word: a copy did not come
 constexpr float kHeadroom = 8.f;                 // a row's m moves only when an x exceeds it by more: w stays below 2^(8 + 7)
 constexpr float kLift = 7.f;                     // of all weights, away from fp16's smallest numbers
 
@@ -36,19 +40,27 @@ struct AttnArgs {
     long long q_row, q_head, out_row, out_head;
     float scale_log2;
     int causal, window;
-    float* parts;                                // [blocks][2][kRows] x (DP + 2)
+    float* parts;                                // [ranges][2][kRows] x (DP + 2)
+    struct Boundary* boundaries;                 // [ranges]
+    uint32_t spin_limit;
+    int* error;
 };
+
+// Where a range begins, for the join: the sequence it falls in, the tiles before that one's and those of all.
+struct Boundary { long long first, total; int b, unused; };
 
 template <int DP, int MT, bool kSplit>
 struct Form {
     static constexpr int kRows = MT * (kSplit ? 8 : 16);
     static constexpr int kStages = DP == 64 ? 6 : (DP == 128 ? 4 : 3);
+    static constexpr int kBoxBytes = kChunk * (DP == 64 ? 64 : 128);                // of one copy
+    static constexpr int kBoxes = DP == 256 ? 2 : 1;                                // to a step's keys, or values
     static constexpr int kStageBytes = 2 * kChunk * DP;
     static constexpr int kRing = kWarps * kStages * kStageBytes;
     static constexpr int kJoin = kWarps * kRows * (DP + 4) * 4;
-    static constexpr int kSmem = kRing > kJoin ? kRing : kJoin;
+    static constexpr int kSmem = (kRing > kJoin ? kRing : kJoin) + 1024;            // the ring begins on a swizzle's boundary
     static constexpr int kPart = kRows * (DP + 2);      // floats of a part: values, then m, then sums
-    static constexpr int kBlocks = DP == 64 ? 4 : (DP == 128 && MT == 1 ? 3 : 2);   // that fit an SM at once
+    static constexpr int kBlocks = (DP == 64 ? 4 : (DP == 128 ? 3 : 2)) - (MT == 2 ? 1 : 0);   // that fit an SM at once
 };
 
 // ---- the ranges
@@ -70,6 +82,8 @@ __device__ __forceinline__ int tiles_of(const paged::Sequence& s, int causal, in
     const Span k = span_of(s, 0, s.n - 1, causal, window);
     return k.hi > k.lo ? (k.hi - 1) / kTileKeys - k.lo / kTileKeys + 1 : 0;
 }
+// What a segment of so many tiles counts in the ranges.
+__device__ __forceinline__ int cost_of(int tiles) { return tiles > 0 ? tiles + kSegmentCost : 0; }
 
 // Sums the tiles of all sequences and finds the one that position total * num / den (or its end) falls in. All threads of a
 // block of 128; `shared` holds 130 values.
@@ -121,13 +135,23 @@ __device__ __forceinline__ Place locate(int n_seqs, int num, int den, long long*
 }
 
 // ---- copies and products
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
-    const int n = there ? 16 : 0;
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+__device__ __forceinline__ bool wait_copy(uint32_t bar, uint32_t parity, uint32_t limit) {
+    for (uint32_t spin = 0; spin < limit; ++spin) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+        if (done) return true;
+    }
+    return false;
 }
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void copy_box(uint32_t dst, const CUtensorMap* map, uint32_t bar, int element, int token, int head, int page) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+        ::"r"(dst), "l"(map), "r"(bar), "r"(element), "r"(token), "r"(head), "r"(page) : "memory");
+}
 
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -175,56 +199,134 @@ __device__ __forceinline__ void store_row(const AttnArgs& a, long long row, int 
     if (d == 0 && a.lse) a.lse[row * a.b.q_heads + head] = sum == 0.f ? -INFINITY : (m - kLift + log2f(sum)) * 0.6931471805599453f;
 }
 
-// Where unit u (16 bytes) of row r of a step lies: rows that are read together fall into different banks.
+// Where unit u (16 bytes) of row r of a step's keys or values lies: as the copies' swizzle puts it.
 template <int DP>
-__device__ __forceinline__ int key_at(int r, int u) { return r * DP + (DP == 64 ? u : u ^ ((r & 1) << 2)) * 16; }
+__device__ __forceinline__ int unit_at(int r, int u) {
+    return DP == 64 ? r * 64 + (u ^ ((r >> 1) & 3)) * 16 : (u >> 3) * (kChunk * 128) + r * 128 + ((u & 7) ^ (r & 7)) * 16;
+}
+// The key (of eight) that stands for column n of a product's block: eight lanes that read together get rows in different banks.
 template <int DP>
-__device__ __forceinline__ int value_at(int r, int u) { return r * DP + (DP == 64 ? u ^ ((r >> 1) & 3) : u ^ (r & 7)) * 16; }
+__device__ __forceinline__ int key_of(int n) { return DP == 64 ? n : (n >> 1) + (n & 1) * 4; }
+
+// 16 values of a row from element d on, as fp32; zeros behind the head's end.
+__device__ __forceinline__ void load16(const void* q, long long at, int d, int dim, int dtype, float* f) {
+    if (d >= dim) {
+#pragma unroll
+        for (int l = 0; l < 16; ++l) f[l] = 0.f;
+    } else if (dtype == OGLE_F32) {
+        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(q) + at + d);
+#pragma unroll
+        for (int l = 0; l < 4; ++l) {
+            const float4 v = p[l];
+            f[4 * l] = v.x; f[4 * l + 1] = v.y; f[4 * l + 2] = v.z; f[4 * l + 3] = v.w;
+        }
+    } else {
+        const uint4* p = reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(q) + at + d);
+        const uint4 v[2] = {p[0], p[1]};
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(v);
+#pragma unroll
+        for (int l = 0; l < 8; ++l) {
+            const float2 g = dtype == OGLE_F16 ? __half22float2(*reinterpret_cast<const __half2*>(w + l)) : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(w + l));
+            f[2 * l] = g.x; f[2 * l + 1] = g.y;
+        }
+    }
+}
 
 template <int DP, int MT, bool kSplit>
-__global__ void __launch_bounds__(kWarps * 32, (Form<DP, MT, kSplit>::kBlocks)) paged_attention_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(kWarps * 32, (Form<DP, MT, kSplit>::kBlocks))
+paged_attention_kernel(AttnArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
     using F = Form<DP, MT, kSplit>;
     constexpr int kRows = F::kRows, NR = kSplit ? 1 : 2, KS = DP / 16, NB = DP / 8;
-    extern __shared__ __align__(16) unsigned char smem[];
+    extern __shared__ __align__(16) unsigned char dynamic[];
     __shared__ long long shared[8];
+    __shared__ __align__(8) uint64_t bars[kWarps][F::kStages];
+    __shared__ int gave_up;
+    unsigned char* const smem = dynamic + ((1024 - (tc::smem_u32(dynamic) & 1023)) & 1023);
     const Batch& B = a.b;
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, c4 = lane & 3, r8 = lane >> 2;
+    if (tid < kWarps * F::kStages) tc::mbar_init(&bars[0][0] + tid, 1);
+    if (tid == 0) {
+        gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
     grid_dependency_trigger();
     grid_dependency_wait();
     const auto weight = [&](int b) {
         const paged::Sequence s = paged::sequence(B, b);
-        return (long long)B.kv_heads * row_tiles(B, s.n, kRows) * tiles_of(s, a.causal, a.window);
+        return (long long)B.kv_heads * row_tiles(B, s.n, kRows) * cost_of(tiles_of(s, a.causal, a.window));
     };
-    const Place place = locate(B.n_seqs, blockIdx.x, gridDim.x, shared, weight);
+    const Place place = locate(B.n_seqs, blockIdx.x, gridDim.x, shared, weight);    // its barriers: `bars` is set up
+    if (tid == 0) a.boundaries[blockIdx.x] = Boundary{place.first, place.total, place.b, 0};
     long long at = place.total * blockIdx.x / gridDim.x, first = place.first;
     const long long end = place.total * (blockIdx.x + 1) / gridDim.x;
     int b = place.b;
-    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * F::kStages * F::kStageBytes;
-    const uint32_t value_lane = (lane & 7) + ((lane >> 3) & 1) * 8;   // key of this lane's row of the transposed loads
+    const uint32_t ring = tc::smem_u32(smem) + warp * F::kStages * F::kStageBytes, bar0 = tc::smem_u32(&bars[warp][0]);
+    const int nowhere = max(B.n_pages, 1);
+    int put = 0, get = 0;                         // stages of the ring: the next to fill, the next to read
+    uint32_t parity = 0;                          // of the next to read
+    // this lane's rows of the two kinds of loads, as offsets into a step
+    const uint32_t value_row = key_of<DP>(lane & 7) + ((lane >> 3) & 1) * 8;
 
     while (at < end && b < B.n_seqs) {
         paged::Sequence s = paged::sequence(B, b);
-        int tiles = tiles_of(s, a.causal, a.window), rts = row_tiles(B, s.n, kRows);
-        const long long all = (long long)B.kv_heads * rts * tiles;
+        const int tiles = tiles_of(s, a.causal, a.window), cost = cost_of(tiles), rts = row_tiles(B, s.n, kRows);
+        const long long all = (long long)B.kv_heads * rts * cost;
         if (at >= first + all) { first += all; ++b; continue; }
-        // segment: kv head, tile of rows; within it tiles [t0, t1)
-        const long long seg = (at - first) / tiles;
+        // segment: kv head, tile of rows; of what it counts this range has [c0, c1), its tiles behind the segment's cost
+        const long long seg = (at - first) / cost;
         const int h = int(seg / rts), rt = int(seg % rts);
-        const long long seg_first = first + seg * tiles;
-        const int t0 = int(at - seg_first), t1 = int(min((long long)tiles, end - seg_first));
+        const long long seg_first = first + seg * cost;
+        const int c0 = int(at - seg_first), c1 = int(min((long long)cost, end - seg_first));
+        const int t0 = max(c0 - kSegmentCost, 0), t1 = max(c1 - kSegmentCost, 0);
         const Span all_keys = span_of(s, 0, s.n - 1, a.causal, a.window);
         const int m0 = rt * kRows, m_end = min(s.n * B.group, m0 + kRows);
         const Span keys = span_of(s, m0 / B.group, (m_end - 1) / B.group, a.causal, a.window);
         const int inner_lo = span_of(s, (m_end - 1) / B.group, 0, a.causal, a.window).lo;
         const int inner_hi = span_of(s, 0, m0 / B.group, a.causal, a.window).hi;
         const int base = all_keys.lo / kTileKeys;
-        int j_begin = max((base + t0) * kTileKeys, keys.lo / kChunk * kChunk), j_end = min((base + t1) * kTileKeys, keys.hi);
+        const int j_begin = max((base + t0) * kTileKeys, keys.lo / kChunk * kChunk), j_end = min((base + t1) * kTileKeys, keys.hi);
         const int steps = max(0, (j_end - j_begin + kChunk - 1) / kChunk);
         const int count = steps > warp ? (steps - warp + kWarps - 1) / kWarps : 0;   // of this warp: warp, warp + 4, ...
 
+        // pages and scales of the warp's next 32 steps, a lane each; the 32 behind them are on their way
+        int page[2] = {nowhere, nowhere};         // where there is no page: the copies find themselves outside and bring zeros
+        float ks[2] = {0.f, 0.f}, vs[2] = {0.f, 0.f};
+        const auto look_up = [&](int which, int i) {
+            int p = -1;
+            if (i < count) p = paged::page_of(B, b, (j_begin + (i * kWarps + warp) * kChunk) >> B.page_shift);
+            page[which] = p >= 0 ? p : nowhere;
+            ks[which] = vs[which] = 0.f;
+            if (p >= 0) {
+                const long long o = (long long)p * B.kv_heads + h;
+                ks[which] = __ldg(B.k_scale + o);
+                vs[which] = __ldg(B.v_scale + o);
+            }
+        };
+        look_up(0, lane);
+        look_up(1, 32 + lane);
+        const int in_page = (1 << B.page_shift) - 1;
+        const auto issue = [&](int i, int p) {    // step i, whose page is p
+            if (lane == 0) {
+                const uint32_t dst = ring + put * F::kStageBytes, bar = bar0 + put * 8;
+                const int token = (j_begin + (i * kWarps + warp) * kChunk) & in_page;
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(F::kStageBytes) : "memory");
+#pragma unroll
+                for (int x = 0; x < F::kBoxes; ++x) {
+                    copy_box(dst + x * F::kBoxBytes, &k_map, bar, x * 128, token, h, p);
+                    copy_box(dst + kChunk * DP + x * F::kBoxBytes, &v_map, bar, x * 128, token, h, p);
+                }
+            }
+            put = put + 1 == F::kStages ? 0 : put + 1;
+        };
+#pragma unroll
+        for (int i = 0; i < F::kStages - 1; ++i) {
+            const int p = __shfl_sync(~0u, page[0], i);
+            if (i < count) issue(i, p);
+        }
+
         // queries: this thread's parts of the rows it has
         uint32_t Q[MT][KS][4];
-        float rs[MT][NR], m[MT][NR], l[MT][NR];
+        float rs[MT][NR], off[MT][NR], bar_x[MT][NR], l[MT][NR];      // weight 2^(x - off); an x above bar_x moves both
         int lo_row[MT][NR], hi_row[MT][NR];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
@@ -236,27 +338,30 @@ __global__ void __launch_bounds__(kWarps * 32, (Form<DP, MT, kSplit>::kBlocks)) 
                 const Span k = span_of(s, i, i, a.causal, a.window);
                 lo_row[mt][r] = k.lo;
                 hi_row[mt][r] = k.hi;
-                float top = 0.f;
-                for (int d = c4; d < B.dim; d += 4) top = fmaxf(top, fabsf(paged::to_float(a.q, q0 + d, B.dtype)));
+                off[mt][r] = 0.f;
+                bar_x[mt][r] = -INFINITY;
+                l[mt][r] = 0.f;
+                rs[mt][r] = 0.f;
+                if (steps == 0) continue;         // a range that has the segment's cost alone
+                float f[DP / 4], top = 0.f;
+#pragma unroll
+                for (int u = 0; u < DP / 64; ++u) load16(a.q, q0, 16 * (c4 + 4 * u), B.dim, B.dtype, f + 16 * u);
+#pragma unroll
+                for (int x = 0; x < DP / 4; ++x) top = fmaxf(top, fabsf(f[x]));
                 top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
                 // 2^e with |q| 2^-e below 2^12; an infinite or vanishing row stays as it is
                 const int e = top > 1e-30f && top <= 3e38f ? int(__float_as_uint(top) >> 23) - 126 - 12 : 0;
                 const float down = __uint_as_float(uint32_t(127 - e) << 23);
                 rs[mt][r] = a.scale_log2 * __uint_as_float(uint32_t(127 + e) << 23);
-                m[mt][r] = -INFINITY;
-                l[mt][r] = 0.f;
 #pragma unroll
-                for (int t = 0; t < KS; ++t) {
-                    // step t, this thread: word t % 4 of unit c4 + 4 (t / 4) - the order in which it reads keys
-                    const int d = 16 * (c4 + 4 * (t / 4)) + 4 * (t % 4);
-                    float f[4];
+                for (int x = 0; x < DP / 4; ++x) f[x] *= down;
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) f[x] = d < B.dim ? paged::to_float(a.q, q0 + d + x, B.dtype) * down : 0.f;
-                    const uint32_t u = half2_bits(f[0], f[1]), v = half2_bits(f[2], f[3]);
+                for (int t = 0; t < KS; ++t) {    // step t: word t % 4 of unit c4 + 4 (t / 4) - the order in which keys are read
+                    const uint32_t u = half2_bits(f[4 * t], f[4 * t + 1]), v = half2_bits(f[4 * t + 2], f[4 * t + 3]);
                     if (kSplit) {
-                        Q[mt][t][0] = u; Q[mt][t][1] = rest_bits(u, f[0], f[1]);
-                        Q[mt][t][2] = v; Q[mt][t][3] = rest_bits(v, f[2], f[3]);
+                        Q[mt][t][0] = u; Q[mt][t][1] = rest_bits(u, f[4 * t], f[4 * t + 1]);
+                        Q[mt][t][2] = v; Q[mt][t][3] = rest_bits(v, f[4 * t + 2], f[4 * t + 3]);
                     } else {
                         Q[mt][t][r] = u; Q[mt][t][2 + r] = v;
                     }
@@ -269,58 +374,31 @@ __global__ void __launch_bounds__(kWarps * 32, (Form<DP, MT, kSplit>::kBlocks)) 
             for (int n = 0; n < NB; ++n)
 #pragma unroll
                 for (int x = 0; x < 4; ++x) O[mt][n][x] = 0.f;
-        float vref = 1.1754944e-38f;              // the unit of O: the largest value scale met
-
-        // pages and scales of the warp's next 32 steps, a lane each; the 32 behind them are on their way
-        int page[2] = {-1, -1};
-        float ks[2] = {0.f, 0.f}, vs[2] = {0.f, 0.f};
-        const auto look_up = [&](int which, int i) {
-            page[which] = -1;
-            ks[which] = vs[which] = 0.f;
-            if (i < count) {
-                page[which] = paged::page_of(B, b, (j_begin + (i * kWarps + warp) * kChunk) >> B.page_shift);
-                if (page[which] >= 0) {
-                    const long long o = (long long)page[which] * B.kv_heads + h;
-                    ks[which] = __ldg(B.k_scale + o);
-                    vs[which] = __ldg(B.v_scale + o);
-                }
-            }
-        };
-        look_up(0, lane);
-        look_up(1, 32 + lane);
-        const auto issue = [&](int i, int now) {
-            if (i < count) {
-                const int j0 = j_begin + (i * kWarps + warp) * kChunk;
-                const int p0 = __shfl_sync(~0u, page[0], i & 31), p1 = __shfl_sync(~0u, page[1], i & 31);
-                const int p = (i >> 5) == (now >> 5) ? p0 : p1;
-                const long long o = (long long)max(p, 0) * B.page_stride + h * B.head_stride + (long long)(j0 & ((1 << B.page_shift) - 1)) * B.token_stride;
-                const uint32_t dst = ring + (i % F::kStages) * F::kStageBytes;
-#pragma unroll
-                for (int x = 0; x < DP / 32; ++x) {
-                    const int idx = x * 32 + lane, r = idx / (DP / 16), u = idx % (DP / 16);
-                    const bool there = p >= 0 && j0 + r >= keys.lo && j0 + r < keys.hi && u * 16 < B.dim;
-                    const long long from = there ? o + r * B.token_stride + u * 16 : 0;
-                    copy16(dst + key_at<DP>(r, u), B.k_cache + from, there);
-                    copy16(dst + kChunk * DP + value_at<DP>(r, u), B.v_cache + from, there);
-                }
-            }
-            copies_commit();
-        };
-#pragma unroll
-        for (int i = 0; i < F::kStages - 1; ++i) issue(i, 0);
+        float vref = 1.1754944e-38f, vinv = 8.507059e37f;     // the unit of O, the largest value scale met; 1 / vref
 
         for (int i = 0; i < count; ++i) {
             if ((i & 31) == 0 && i > 0) {
                 page[0] = page[1]; ks[0] = ks[1]; vs[0] = vs[1];
                 look_up(1, i + 32 + lane);
             }
-            copies_wait<F::kStages - 2>();
-            __syncwarp();
-            const uint32_t at_k = ring + (i % F::kStages) * F::kStageBytes, at_v = at_k + kChunk * DP;
+            const uint32_t at_k = ring + get * F::kStageBytes, at_v = at_k + kChunk * DP;
+            const bool came = wait_copy(bar0 + get * 8, parity, a.spin_limit);
+            if (!__all_sync(~0u, came)) {
+                // nothing more is asked for; the copies under way are waited for, this one's among them
+                for (int j = i; j < min(count, i + F::kStages - 1); ++j) {
+                    wait_copy(bar0 + get * 8, parity, tc::kSpinLimit);
+                    if (++get == F::kStages) { get = 0; parity ^= 1; }
+                }
+                if (lane == 0) {
+                    gave_up = 1;
+                    tc::record_error(a.error, kGaveUp);
+                }
+                break;
+            }
+            if (++get == F::kStages) { get = 0; parity ^= 1; }
             const int j0 = j_begin + (i * kWarps + warp) * kChunk;
             const float k_scale = __shfl_sync(~0u, ks[0], i & 31), v_scale = __shfl_sync(~0u, vs[0], i & 31);
-            const bool no_page = __shfl_sync(~0u, page[0], i & 31) < 0;
-            const bool edge = j0 < inner_lo || j0 + kChunk > inner_hi || no_page;
+            const bool edge = j0 < inner_lo || j0 + kChunk > inner_hi || k_scale == 0.f;
             // x = q . k
             float x[MT][2][NR * 2];
 #pragma unroll
@@ -334,10 +412,12 @@ __global__ void __launch_bounds__(kWarps * 32, (Form<DP, MT, kSplit>::kBlocks)) 
                 for (int u = 0; u < DP / 64; ++u) {
                     uint32_t w[4];
                     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at_k + key_at<DP>(nb * 8 + r8, c4 + 4 * u)) : "memory");
+                                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                                 : "r"(at_k + unit_at<DP>(nb * 8 + key_of<DP>(r8), c4 + 4 * u)) : "memory");
 #pragma unroll
                     for (int y = 0; y < 4; ++y) {
-                        const uint32_t b0 = paged::e4m3x2_to_half2(uint16_t(w[y])), b1 = paged::e4m3x2_to_half2(uint16_t(w[y] >> 16));
+                        uint32_t b0, b1;
+                        paged::e4m3x4_to_half2(w[y], b0, b1);
 #pragma unroll
                         for (int mt = 0; mt < MT; ++mt) mma(S[mt], Q[mt][4 * u + y], b0, b1);
                     }
@@ -354,13 +434,14 @@ __global__ void __launch_bounds__(kWarps * 32, (Form<DP, MT, kSplit>::kBlocks)) 
                 }
             }
             if (edge) {
+                const bool no_page = __shfl_sync(~0u, page[0], i & 31) == nowhere;
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                     for (int nb = 0; nb < 2; ++nb)
 #pragma unroll
                         for (int y = 0; y < 2 * NR; ++y) {
-                            const int j = j0 + nb * 8 + c4 * 2 + (y & 1);
+                            const int j = j0 + nb * 8 + key_of<DP>(c4 * 2 + (y & 1));
                             if (no_page || j < lo_row[mt][y / 2] || j >= hi_row[mt][y / 2]) x[mt][nb][y] = -INFINITY;
                         }
             }
@@ -371,10 +452,11 @@ __global__ void __launch_bounds__(kWarps * 32, (Form<DP, MT, kSplit>::kBlocks)) 
 #pragma unroll
                 for (int nb = 0; nb < 2; ++nb)
 #pragma unroll
-                    for (int y = 0; y < 2 * NR; ++y) more |= x[mt][nb][y] > m[mt][y / 2] + kHeadroom;
+                    for (int y = 0; y < 2 * NR; ++y) more |= x[mt][nb][y] > bar_x[mt][y / 2];
             if (__any_sync(~0u, more)) {
                 const float vnew = fmaxf(vref, v_scale), vratio = vref / vnew;
                 vref = vnew;
+                vinv = 1.f / vnew;
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
                     float f[NR];
@@ -383,9 +465,13 @@ __global__ void __launch_bounds__(kWarps * 32, (Form<DP, MT, kSplit>::kBlocks)) 
                         float top = fmaxf(fmaxf(x[mt][0][2 * r], x[mt][0][2 * r + 1]), fmaxf(x[mt][1][2 * r], x[mt][1][2 * r + 1]));
                         top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
                         top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-                        top = fmaxf(top, m[mt][r]);
-                        f[r] = top == -INFINITY ? 1.f : exp2_fast(m[mt][r] - top);
-                        m[mt][r] = top;
+                        top = fmaxf(top, bar_x[mt][r] - kHeadroom);
+                        f[r] = 1.f;
+                        if (top > -INFINITY) {
+                            f[r] = exp2_fast(bar_x[mt][r] - kHeadroom - top);
+                            off[mt][r] = top - kLift;
+                            bar_x[mt][r] = top + kHeadroom;
+                        }
                         l[mt][r] *= f[r];
                         f[r] *= vratio;
                     }
@@ -396,79 +482,89 @@ __global__ void __launch_bounds__(kWarps * 32, (Form<DP, MT, kSplit>::kBlocks)) 
                 }
             }
             // weights, and with the values' scale as A operands of the second product
-            const float v_unit = v_scale / vref;
+            const float v_unit = v_scale * vinv;
             uint32_t P[MT][4];
-            uint32_t seen[MT][4];                       // 1 where the row attends the key, for NaN among the values
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                 for (int nb = 0; nb < 2; ++nb)
 #pragma unroll
                     for (int r = 0; r < NR; ++r) {
-                        const float off = m[mt][r] == -INFINITY ? 0.f : m[mt][r] - kLift;
                         float p[2];
 #pragma unroll
                         for (int y = 0; y < 2; ++y) {
-                            p[y] = exp2_fast(x[mt][nb][2 * r + y] - off);
+                            p[y] = exp2_fast(x[mt][nb][2 * r + y] - off[mt][r]);
                             l[mt][r] += p[y];
                             p[y] *= v_unit;
                         }
                         const uint32_t hi = half2_bits(p[0], p[1]);
-                        const uint32_t see = (x[mt][nb][2 * r] == -INFINITY ? 0u : 0x3c00u) | (x[mt][nb][2 * r + 1] == -INFINITY ? 0u : 0x3c000000u);
                         if (kSplit) {
                             P[mt][2 * nb] = hi;
                             P[mt][2 * nb + 1] = rest_bits(hi, p[0], p[1]);
-                            seen[mt][2 * nb] = see;
-                            seen[mt][2 * nb + 1] = 0;
                         } else {
                             P[mt][2 * nb + r] = hi;
-                            seen[mt][2 * nb + r] = see;
                         }
                     }
-            // the stage's values, two units (32 elements) at a time
+            // the step's values, two units (32 elements) at a time
+            const auto values = [&](auto at_edge) {
+                constexpr bool kEdge = decltype(at_edge)::value;
+                uint32_t seen[MT][4];             // 1 where the row attends the key
+                if (kEdge) {
 #pragma unroll
-            for (int u = 0; u < DP / 32; ++u) {
-                uint32_t w[4];
-                ldmatrix_trans(w, at_v + value_at<DP>(value_lane, 2 * u + (lane >> 4)));
-                uint32_t v[4][2];
+                    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                    const uint32_t t = __byte_perm(w[y], 0, 0x3120);   // (key, key + 1) of the even element, then of the odd one
-                    v[y][0] = paged::e4m3x2_to_half2(uint16_t(t));
-                    v[y][1] = paged::e4m3x2_to_half2(uint16_t(t >> 16));
+                        for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+                            for (int r = 0; r < 2; ++r) {
+                                const float* e = &x[mt][nb][2 * (r % NR)];
+                                seen[mt][2 * nb + r] = r >= NR ? 0u : (e[0] == -INFINITY ? 0u : 0x3c00u) | (e[1] == -INFINITY ? 0u : 0x3c000000u);
+                            }
                 }
 #pragma unroll
-                for (int y = 0; y < 2; ++y)
+                for (int u = 0; u < DP / 32; ++u) {
+                    uint32_t w[4];
+                    ldmatrix_trans(w, at_v + unit_at<DP>(value_row, 2 * u + (lane >> 4)));
+                    uint32_t v[4][2];
 #pragma unroll
-                    for (int odd = 0; odd < 2; ++odd) {
-                        uint32_t b0 = v[2 * y][odd], b1 = v[2 * y + 1][odd];
-                        if (edge) {
-                            // a row that does not attend a key has weight 0 for it, and 0 x NaN would still be NaN: NaNs are
-                            // taken out, and counted for the rows that do attend them
-                            const __half2 h0 = *reinterpret_cast<const __half2*>(&b0), h1 = *reinterpret_cast<const __half2*>(&b1);
-                            const uint32_t n0 = __hneu2_mask(h0, h0), n1 = __hneu2_mask(h1, h1);
-                            if (__any_sync(~0u, (n0 | n1) != 0)) {
-                                b0 &= ~n0;
-                                b1 &= ~n1;
+                    for (int y = 0; y < 4; ++y)   // (a key, the next) of the even element, then of the odd one
+                        paged::e4m3x4_to_half2(__byte_perm(w[y], 0, 0x3120), v[y][0], v[y][1]);
 #pragma unroll
-                                for (int mt = 0; mt < MT; ++mt) {
-                                    float nan[4] = {0.f, 0.f, 0.f, 0.f};
-                                    mma(nan, seen[mt], n0 & 0x3c003c00u, n1 & 0x3c003c00u);
+                    for (int y = 0; y < 2; ++y)
 #pragma unroll
-                                    for (int z = 0; z < 4; ++z)
-                                        if (nan[z] > 0.f) O[mt][4 * u + 2 * y + odd][z] = NAN;
+                        for (int odd = 0; odd < 2; ++odd) {
+                            uint32_t b0 = v[2 * y][odd], b1 = v[2 * y + 1][odd];
+                            if (kEdge) {
+                                // a row that does not attend a key has weight 0 for it, and 0 x NaN would still be NaN: NaNs are
+                                // taken out, and counted for the rows that do attend them
+                                const __half2 h0 = *reinterpret_cast<const __half2*>(&b0), h1 = *reinterpret_cast<const __half2*>(&b1);
+                                const uint32_t n0 = __hneu2_mask(h0, h0), n1 = __hneu2_mask(h1, h1);
+                                if (__any_sync(~0u, (n0 | n1) != 0)) {
+                                    b0 &= ~n0;
+                                    b1 &= ~n1;
+#pragma unroll
+                                    for (int mt = 0; mt < MT; ++mt) {
+                                        float nan[4] = {0.f, 0.f, 0.f, 0.f};
+                                        mma(nan, seen[mt], n0 & 0x3c003c00u, n1 & 0x3c003c00u);
+#pragma unroll
+                                        for (int z = 0; z < 4; ++z)
+                                            if (nan[z] > 0.f) O[mt][4 * u + 2 * y + odd][z] = NAN;
+                                    }
                                 }
                             }
-                        }
 #pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) mma(O[mt][4 * u + 2 * y + odd], P[mt], b0, b1);
-                    }
-            }
+                            for (int mt = 0; mt < MT; ++mt) mma(O[mt][4 * u + 2 * y + odd], P[mt], b0, b1);
+                        }
+                }
+            };
+            if (edge) values(std::true_type());
+            else values(std::false_type());
             __syncwarp();
-            issue(i + F::kStages - 1, i);
+            const int n = i + F::kStages - 1;
+            const int p0 = __shfl_sync(~0u, page[0], n & 31), p1 = __shfl_sync(~0u, page[1], n & 31);
+            if (n < count) issue(n, (n ^ i) >> 5 ? p1 : p0);
         }
-        copies_wait<0>();
         __syncthreads();                          // every warp is through with its ring: the parts take its place
+        if (gave_up) return;
 
         // the warps' parts: values [kRows][DP + 4], then m and l
         float* const mine = reinterpret_cast<float*>(smem) + warp * kRows * (DP + 4);
@@ -493,11 +589,11 @@ __global__ void __launch_bounds__(kWarps * 32, (Form<DP, MT, kSplit>::kBlocks)) 
                     v.x *= vref; v.y *= vref; v.z *= vref; v.w *= vref;
                     *reinterpret_cast<float4*>(row + u * 16 + c4 * 4) = v;
                 }
-                if (c4 == 0) { row[DP] = m[mt][r]; row[DP + 1] = sum; }
+                if (c4 == 0) { row[DP] = bar_x[mt][r] - kHeadroom; row[DP + 1] = sum; }
             }
         __syncthreads();
-        const bool whole = t0 == 0 && t1 == tiles;
-        float* const part = a.parts + ((long long)blockIdx.x * 2 + (t0 > 0 ? 0 : 1)) * F::kPart;
+        const bool whole = c0 == 0 && c1 == cost;
+        float* const part = a.parts + ((long long)blockIdx.x * 2 + (c0 > 0 ? 0 : 1)) * F::kPart;
         for (int idx = tid; idx < kRows * (DP / 4); idx += kWarps * 32) {
             const int r = idx / (DP / 4), d = idx % (DP / 4) * 4, row = m0 + r;
             if (row >= m_end) continue;
@@ -523,63 +619,93 @@ __global__ void __launch_bounds__(kWarps * 32, (Form<DP, MT, kSplit>::kBlocks)) 
             }
             store_row(a, s.row0 + row / B.group, h * B.group + row % B.group, d, v, top, sum);
         }
-        __syncthreads();                          // the next segment's copies take the parts' place
-        at = seg_first + t1;
+        // the next segment's copies take the parts' place
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncthreads();
+        at = seg_first + c1;
     }
 }
 
-// Adds up the parts of segments that were cut, in the order of their ranges, and answers for sequences without a key. Block c
-// stands for the boundary before range c + 1 and has the segment that this is the first boundary inside of.
-template <int DP, int MT, bool kSplit>
-__global__ void __launch_bounds__(kWarps * 32) paged_join_kernel(AttnArgs a, int ranges) {
-    using F = Form<DP, MT, kSplit>;
-    constexpr int kRows = F::kRows;
-    __shared__ long long shared[8];
+// Adds up the parts of segments that were cut, in the order of their ranges, and answers for sequences without a key. Block
+// (c, r) stands for the boundary before range c + 1 and row r of the segment that this is the first boundary inside of: its
+// warps take every eighth part.
+constexpr int kJoinWarps = 8;
+template <int DP>
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(AttnArgs a, int ranges, int rows_of_tile) {
+    constexpr int kVecs = DP / 4, kPerLane = (kVecs + 31) / 32;
+    __shared__ float4 sums[kJoinWarps][kVecs];
+    __shared__ float weights[kJoinWarps];
     const Batch& B = a.b;
-    const int tid = threadIdx.x, c = blockIdx.x + 1;
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, c = blockIdx.x + 1, r = blockIdx.y;
     grid_dependency_trigger();
     grid_dependency_wait();
-    for (int b = blockIdx.x; b < B.n_seqs; b += gridDim.x) {
-        const paged::Sequence s = paged::sequence(B, b);
-        if (s.n <= 0 || tiles_of(s, a.causal, a.window) > 0) continue;
-        for (int idx = tid; idx < s.n * B.q_heads * (DP / 4); idx += blockDim.x) {
-            const int row = idx / (B.q_heads * (DP / 4)), r = idx % (B.q_heads * (DP / 4));
-            store_row(a, s.row0 + row, r / (DP / 4), r % (DP / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f), 0.f, 0.f);
+    if (r == 0) {
+        for (int b = blockIdx.x; b < B.n_seqs; b += gridDim.x) {
+            const paged::Sequence s = paged::sequence(B, b);
+            if (s.n <= 0 || tiles_of(s, a.causal, a.window) > 0) continue;
+            for (int idx = tid; idx < s.n * B.q_heads; idx += blockDim.x)
+                for (int d = 0; d < B.dim; d += 4)
+                    store_row(a, s.row0 + idx / B.q_heads, idx % B.q_heads, d, make_float4(0.f, 0.f, 0.f, 0.f), 0.f, 0.f);
         }
     }
     if (c >= ranges) return;
-    const auto weight = [&](int b) {
-        const paged::Sequence s = paged::sequence(B, b);
-        return (long long)B.kv_heads * row_tiles(B, s.n, kRows) * tiles_of(s, a.causal, a.window);
-    };
-    const Place place = locate(B.n_seqs, c, ranges, shared, weight);
+    const Boundary place = a.boundaries[c];
     if (place.b < 0) return;
     const paged::Sequence s = paged::sequence(B, place.b);
-    const int tiles = tiles_of(s, a.causal, a.window), rts = row_tiles(B, s.n, kRows);
+    const int cost = cost_of(tiles_of(s, a.causal, a.window)), rts = row_tiles(B, s.n, rows_of_tile);
     const auto bound = [&](int k) { return place.total * k / ranges; };
-    const long long x = bound(c), seg = (x - place.first) / tiles, begin = place.first + seg * tiles, end = begin + tiles;
+    const long long x = bound(c), seg = (x - place.first) / cost, begin = place.first + seg * cost, end = begin + cost;
     if (x == begin || bound(c - 1) > begin) return;
-    const int h = int(seg / rts), m0 = int(seg % rts) * kRows, m_end = min(s.n * B.group, m0 + kRows);
-    int last = c;                                 // ranges c - 1 .. last - 1 have parts
+    const int h = int(seg / rts), row = int(seg % rts) * rows_of_tile + r;
+    if (row >= s.n * B.group) return;
+    // ranges c - 1 .. last - 1 have parts: the first range whose beginning is at or behind the end
+    int last = int((end * ranges + place.total - 1) / place.total);
+    while (last > c && bound(last - 1) >= end) --last;
     while (last < ranges && bound(last) < end) ++last;
-    for (int idx = tid; idx < kRows * (DP / 4); idx += kWarps * 32) {
-        const int r = idx / (DP / 4), d = idx % (DP / 4) * 4, row = m0 + r;
-        if (row >= m_end) continue;
-        float top = -INFINITY, sum = 0.f;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int k = c - 1; k < last; ++k) {
-            if (bound(k) == bound(k + 1)) continue;             // more ranges than tiles
-            const float* p = a.parts + ((long long)k * 2 + (k == c - 1 ? 1 : 0)) * F::kPart;
-            const float m = p[kRows * DP + r], l = p[kRows * DP + kRows + r];
-            if (l == 0.f) continue;
-            const float4 o = *reinterpret_cast<const float4*>(p + r * DP + d);
-            const float now = fmaxf(top, m), f = top == -INFINITY ? 0.f : exp2_fast(top - now), g = exp2_fast(m - now);
-            sum = sum * f + l * g;
-            v.x = v.x * f + o.x * g; v.y = v.y * f + o.y * g; v.z = v.z * f + o.z * g; v.w = v.w * f + o.w * g;
-            top = now;
+    const int part_floats = rows_of_tile * (DP + 2);
+    const auto part = [&](int k) { return a.parts + ((long long)k * 2 + (k == c - 1 ? 1 : 0)) * part_floats; };
+    const bool gaps = place.total < ranges;       // more ranges than tiles: some have none
+    float top = -INFINITY;
+    for (int k = c - 1 + lane; k < last; k += 32)
+        if (!gaps || bound(k) != bound(k + 1)) {
+            const float* p = part(k) + rows_of_tile * DP + r;
+            if (p[rows_of_tile] != 0.f) top = fmaxf(top, p[0]);
         }
-        store_row(a, s.row0 + row / B.group, h * B.group + row % B.group, d, v, top, sum);
+#pragma unroll
+    for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+    float sum = 0.f;
+    float4 v[kPerLane];
+#pragma unroll
+    for (int u = 0; u < kPerLane; ++u) v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int k = c - 1 + warp; k < last; k += kJoinWarps) {
+        if (gaps && bound(k) == bound(k + 1)) continue;
+        const float* p = part(k);
+        const float m = p[rows_of_tile * DP + r], l = p[rows_of_tile * DP + rows_of_tile + r];
+        const float f = l == 0.f ? 0.f : exp2_fast(m - top);    // a part without a weight has zeros
+        sum += l * f;
+#pragma unroll
+        for (int u = 0; u < kPerLane; ++u)
+            if (u * 32 + lane < kVecs) {
+                const float4 o = *reinterpret_cast<const float4*>(p + r * DP + (u * 32 + lane) * 4);
+                v[u].x += o.x * f; v[u].y += o.y * f; v[u].z += o.z * f; v[u].w += o.w * f;
+            }
     }
+#pragma unroll
+    for (int u = 0; u < kPerLane; ++u)
+        if (u * 32 + lane < kVecs) sums[warp][u * 32 + lane] = v[u];
+    if (lane == 0) weights[warp] = sum;
+    __syncthreads();
+    if (tid >= kVecs) return;
+    sum = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) {
+        const float4 q = sums[w][tid];
+        sum += weights[w];
+        o.x += q.x; o.y += q.y; o.z += q.z; o.w += q.w;
+    }
+    store_row(a, s.row0 + row / B.group, h * B.group + row % B.group, tid * 4, o, top, sum);
 }
 
 // ---- host
@@ -621,6 +747,19 @@ int ranges_of(const OglePagedBatch* b, int rows, int blocks) {
     return all < double(kNumSMs * blocks) ? (all < 1 ? 1 : int(all)) : kNumSMs * blocks;
 }
 
+// Map of the cache's bytes whose boxes are 16 tokens of one page and head, swizzled as unit_at says. Elements behind the head's
+// end and pages behind the last read zero.
+bool cache_map(CUtensorMap* m, const Batch& b, const void* cache, int dp) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[4] = {(cuuint64_t)b.dim, (cuuint64_t)1 << b.page_shift, (cuuint64_t)b.kv_heads, (cuuint64_t)(b.n_pages > 0 ? b.n_pages : 1)};
+    const cuuint64_t strides[3] = {(cuuint64_t)b.token_stride, (cuuint64_t)b.head_stride, (cuuint64_t)b.page_stride};
+    const cuuint32_t box[4] = {dp == 64 ? 64u : 128u, kChunk, 1, 1}, es[4] = {1, 1, 1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(cache), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              dp == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 }  // namespace
 }  // namespace ogle
 
@@ -633,7 +772,7 @@ size_t ogle_cuda_paged_attention_workspace_bytes(const OglePagedBatch* batch, co
     if (!p || paged::translate(batch, b) != OGLE_OK || b.n_seqs == 0) return 0;
     return with_form(choose(batch), [&](auto dp, auto mt, auto split) {
         using F = Form<decltype(dp)::value, decltype(mt)::value, decltype(split)::value>;
-        return size_t(ranges_of(batch, F::kRows, F::kBlocks)) * 2 * F::kPart * sizeof(float);
+        return size_t(ranges_of(batch, F::kRows, F::kBlocks)) * (2 * F::kPart * sizeof(float) + sizeof(Boundary));
     });
 }
 
@@ -653,12 +792,15 @@ int ogle_cuda_paged_attention(const OglePagedBatch* batch, const OgleAttentionPa
     a.scale_log2 = p->scale * 1.4426950408889634f;
     a.causal = p->causal; a.window = p->window;
     a.parts = static_cast<float*>(workspace);
+    a.spin_limit = tc::role_wait_limit();
+    a.error = error_flag_ptr();
     return with_form(choose(batch), [&](auto dp, auto mt, auto split) -> int {
         constexpr int DP = decltype(dp)::value, MT = decltype(mt)::value;
         constexpr bool kSplit = decltype(split)::value;
         using F = Form<DP, MT, kSplit>;
         const int ranges = ranges_of(batch, F::kRows, F::kBlocks);
         auto kernel = paged_attention_kernel<DP, MT, kSplit>;
+        a.boundaries = reinterpret_cast<Boundary*>(a.parts + size_t(ranges) * 2 * F::kPart);
         static std::atomic<uint64_t> sized{0};           // devices whose limit of shared memory is raised
         int device = 0;
         cudaError_t e = cudaGetDevice(&device);
@@ -666,12 +808,19 @@ int ogle_cuda_paged_attention(const OglePagedBatch* batch, const OgleAttentionPa
             e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
             if (e == cudaSuccess) sized.fetch_or(1ull << (device & 63), std::memory_order_relaxed);
         }
-        if (e == cudaSuccess) e = launch_overlapped(kernel, dim3(ranges), dim3(kWarps * 32), F::kSmem, stream, a);
+        CUtensorMap k_map, v_map;
+        if (e == cudaSuccess && (!a.error || !cache_map(&k_map, a.b, a.b.k_cache, DP) || !cache_map(&v_map, a.b, a.b.v_cache, DP))) {
+            set_last_error("paged_attention: no tensor map of the cache");
+            return OGLE_ERR_CUDA;
+        }
+        if (e == cudaSuccess) e = launch_overlapped(kernel, dim3(ranges), dim3(kWarps * 32), F::kSmem, stream, a, k_map, v_map);
         if (e != cudaSuccess) { set_last_error(e); (void)cudaGetLastError(); return OGLE_ERR_CUDA; }
         int rc = finish_launch();
         if (rc != OGLE_OK) return rc;
-        e = launch_overlapped_if(overlapped_launches_enabled(true), paged_join_kernel<DP, MT, kSplit>, dim3(ranges > 1 ? ranges - 1 : 1),
-                                 dim3(kWarps * 32), 0, stream, a, ranges);
+        const long long rows = (long long)(a.b.max_rows < a.b.n_rows ? a.b.max_rows : a.b.n_rows) * a.b.group;
+        e = launch_overlapped_if(overlapped_launches_enabled(true), paged_join_kernel<DP>,
+                                 dim3(ranges > 1 ? ranges - 1 : 1, unsigned(rows < F::kRows ? (rows < 1 ? 1 : rows) : F::kRows)),
+                                 dim3(kJoinWarps * 32), 0, stream, a, ranges, F::kRows);
         if (e != cudaSuccess) { set_last_error(e); (void)cudaGetLastError(); return OGLE_ERR_CUDA; }
         return finish_launch();
     });
