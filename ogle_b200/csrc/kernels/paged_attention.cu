@@ -27,7 +27,7 @@ using paged::Batch;
 constexpr int kWarps = 4;
 constexpr int kChunk = 16;                       // keys of a warp's step; a page holds whole steps
 constexpr int kTileKeys = kWarps * kChunk;
-constexpr int kSegmentCost = 2;                  // tiles that a segment's beginning and end take as long as
+constexpr int kSegmentCost = 2;                  // tiles that a segment's beginning and end take as long as, where there are many
 constexpr int kGaveUp = 9;                       // in the library's device status word: a copy did not come
 constexpr float kHeadroom = 8.f;                 // a row's m moves only when an x exceeds it by more: w stays below 2^(8 + 7)
 constexpr float kLift = 7.f;                     // of all weights, away from fp16's smallest numbers
@@ -41,13 +41,19 @@ struct AttnArgs {
     float scale_log2;
     int causal, window;
     float* parts;                                // [ranges][2][kRows] x (DP + 2)
-    struct Boundary* boundaries;                 // [ranges]
+    struct Cut* cuts;                            // [ranges]
+    int segment_cost;
     uint32_t spin_limit;
     int* error;
 };
 
-// Where a range begins, for the join: the sequence it falls in, the tiles before that one's and those of all.
-struct Boundary { long long first, total; int b, unused; };
+// What the join needs of a segment that was cut: kept at the range behind its first cut. rows 0: there is none.
+struct __align__(16) Cut {
+    int rows, row0, h, m0;         // rows of the tile; row of the sequence's first row; kv head; the tile's first row
+    int first, last;               // ranges [first, last) have parts ...
+    int gaps, unused;              // ... but for those that have no tile, where there are more ranges than tiles
+    long long total;               // tiles of all segments
+};
 
 template <int DP, int MT, bool kSplit>
 struct Form {
@@ -83,7 +89,7 @@ __device__ __forceinline__ int tiles_of(const paged::Sequence& s, int causal, in
     return k.hi > k.lo ? (k.hi - 1) / kTileKeys - k.lo / kTileKeys + 1 : 0;
 }
 // What a segment of so many tiles counts in the ranges.
-__device__ __forceinline__ int cost_of(int tiles) { return tiles > 0 ? tiles + kSegmentCost : 0; }
+__device__ __forceinline__ int cost_of(int tiles, int segment_cost) { return tiles > 0 ? tiles + segment_cost : 0; }
 
 // Sums the tiles of all sequences and finds the one that position total * num / den (or its end) falls in. All threads of a
 // block of 128; `shared` holds 130 values.
@@ -253,10 +259,11 @@ paged_attention_kernel(AttnArgs a, const __grid_constant__ CUtensorMap k_map, co
     grid_dependency_wait();
     const auto weight = [&](int b) {
         const paged::Sequence s = paged::sequence(B, b);
-        return (long long)B.kv_heads * row_tiles(B, s.n, kRows) * cost_of(tiles_of(s, a.causal, a.window));
+        return (long long)B.kv_heads * row_tiles(B, s.n, kRows) * cost_of(tiles_of(s, a.causal, a.window), a.segment_cost);
     };
     const Place place = locate(B.n_seqs, blockIdx.x, gridDim.x, shared, weight);    // its barriers: `bars` is set up
-    if (tid == 0) a.boundaries[blockIdx.x] = Boundary{place.first, place.total, place.b, 0};
+    if (tid == 0) a.cuts[blockIdx.x].rows = 0;
+    bool begun = false;
     long long at = place.total * blockIdx.x / gridDim.x, first = place.first;
     const long long end = place.total * (blockIdx.x + 1) / gridDim.x;
     int b = place.b;
@@ -269,7 +276,7 @@ paged_attention_kernel(AttnArgs a, const __grid_constant__ CUtensorMap k_map, co
 
     while (at < end && b < B.n_seqs) {
         paged::Sequence s = paged::sequence(B, b);
-        const int tiles = tiles_of(s, a.causal, a.window), cost = cost_of(tiles), rts = row_tiles(B, s.n, kRows);
+        const int tiles = tiles_of(s, a.causal, a.window), cost = cost_of(tiles, a.segment_cost), rts = row_tiles(B, s.n, kRows);
         const long long all = (long long)B.kv_heads * rts * cost;
         if (at >= first + all) { first += all; ++b; continue; }
         // segment: kv head, tile of rows; of what it counts this range has [c0, c1), its tiles behind the segment's cost
@@ -277,12 +284,22 @@ paged_attention_kernel(AttnArgs a, const __grid_constant__ CUtensorMap k_map, co
         const int h = int(seg / rts), rt = int(seg % rts);
         const long long seg_first = first + seg * cost;
         const int c0 = int(at - seg_first), c1 = int(min((long long)cost, end - seg_first));
-        const int t0 = max(c0 - kSegmentCost, 0), t1 = max(c1 - kSegmentCost, 0);
+        const int t0 = max(c0 - a.segment_cost, 0), t1 = max(c1 - a.segment_cost, 0);
         const Span all_keys = span_of(s, 0, s.n - 1, a.causal, a.window);
         const int m0 = rt * kRows, m_end = min(s.n * B.group, m0 + kRows);
         const Span keys = span_of(s, m0 / B.group, (m_end - 1) / B.group, a.causal, a.window);
         const int inner_lo = span_of(s, (m_end - 1) / B.group, 0, a.causal, a.window).lo;
         const int inner_hi = span_of(s, 0, m0 / B.group, a.causal, a.window).hi;
+        if (!begun && c0 > 0 && tid == 0) {       // this range begins with a cut: the segment's first?
+            const auto bound = [&](int k) { return place.total * k / gridDim.x; };
+            int before = blockIdx.x - 1, last = blockIdx.x + 1;
+            while (bound(before) == at) --before; // ranges without a tile
+            if (bound(before) <= seg_first) {
+                while (last < int(gridDim.x) && bound(last) < seg_first + cost) ++last;
+                a.cuts[blockIdx.x] = Cut{m_end - m0, s.row0, h, m0, before, last, place.total < gridDim.x, 0, place.total};
+            }
+        }
+        begun = true;
         const int base = all_keys.lo / kTileKeys;
         const int j_begin = max((base + t0) * kTileKeys, keys.lo / kChunk * kChunk), j_end = min((base + t1) * kTileKeys, keys.hi);
         const int steps = max(0, (j_end - j_begin + kChunk - 1) / kChunk);
@@ -627,19 +644,21 @@ paged_attention_kernel(AttnArgs a, const __grid_constant__ CUtensorMap k_map, co
 }
 
 // Adds up the parts of segments that were cut, in the order of their ranges, and answers for sequences without a key. Block
-// (c, r) stands for the boundary before range c + 1 and row r of the segment that this is the first boundary inside of: its
-// warps take every eighth part.
+// (c, y) has the segment whose first cut is the beginning of range c + 1, and of its rows y, y + gridDim.y, ...: kWarpsOfRow
+// warps have a row, and each every so-many-th of its parts.
 constexpr int kJoinWarps = 8;
-template <int DP>
+template <int DP, int kWarpsOfRow>
 __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(AttnArgs a, int ranges, int rows_of_tile) {
-    constexpr int kVecs = DP / 4, kPerLane = (kVecs + 31) / 32;
+    constexpr int kVecs = DP / 4, kPerLane = (kVecs + 31) / 32, kRowsAtOnce = kJoinWarps / kWarpsOfRow;
     __shared__ float4 sums[kJoinWarps][kVecs];
     __shared__ float weights[kJoinWarps];
     const Batch& B = a.b;
-    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, c = blockIdx.x + 1, r = blockIdx.y;
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, c = blockIdx.x + 1;
     grid_dependency_trigger();
     grid_dependency_wait();
-    if (r == 0) {
+    Cut cut = {};
+    if (c < ranges) cut = a.cuts[c];
+    if (blockIdx.y == 0) {
         for (int b = blockIdx.x; b < B.n_seqs; b += gridDim.x) {
             const paged::Sequence s = paged::sequence(B, b);
             if (s.n <= 0 || tiles_of(s, a.causal, a.window) > 0) continue;
@@ -648,64 +667,68 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(AttnArgs a,
                     store_row(a, s.row0 + idx / B.q_heads, idx % B.q_heads, d, make_float4(0.f, 0.f, 0.f, 0.f), 0.f, 0.f);
         }
     }
-    if (c >= ranges) return;
-    const Boundary place = a.boundaries[c];
-    if (place.b < 0) return;
-    const paged::Sequence s = paged::sequence(B, place.b);
-    const int cost = cost_of(tiles_of(s, a.causal, a.window)), rts = row_tiles(B, s.n, rows_of_tile);
-    const auto bound = [&](int k) { return place.total * k / ranges; };
-    const long long x = bound(c), seg = (x - place.first) / cost, begin = place.first + seg * cost, end = begin + cost;
-    if (x == begin || bound(c - 1) > begin) return;
-    const int h = int(seg / rts), row = int(seg % rts) * rows_of_tile + r;
-    if (row >= s.n * B.group) return;
-    // ranges c - 1 .. last - 1 have parts: the first range whose beginning is at or behind the end
-    int last = int((end * ranges + place.total - 1) / place.total);
-    while (last > c && bound(last - 1) >= end) --last;
-    while (last < ranges && bound(last) < end) ++last;
     const int part_floats = rows_of_tile * (DP + 2);
-    const auto part = [&](int k) { return a.parts + ((long long)k * 2 + (k == c - 1 ? 1 : 0)) * part_floats; };
-    const bool gaps = place.total < ranges;       // more ranges than tiles: some have none
-    float top = -INFINITY;
-    for (int k = c - 1 + lane; k < last; k += 32)
-        if (!gaps || bound(k) != bound(k + 1)) {
-            const float* p = part(k) + rows_of_tile * DP + r;
-            if (p[rows_of_tile] != 0.f) top = fmaxf(top, p[0]);
-        }
+    const auto part = [&](int k) { return a.parts + ((long long)k * 2 + (k == cut.first ? 1 : 0)) * part_floats; };
+    const auto none = [&](int k) { return cut.gaps && cut.total * k / ranges == cut.total * (k + 1) / ranges; };
+    for (int r0 = blockIdx.y * kRowsAtOnce; r0 < cut.rows; r0 += gridDim.y * kRowsAtOnce) {
+        const int r = r0 + warp / kWarpsOfRow;
+        float top = -INFINITY, sum = 0.f;
+        float4 v[kPerLane];
 #pragma unroll
-    for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-    float sum = 0.f;
-    float4 v[kPerLane];
+        for (int u = 0; u < kPerLane; ++u) v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < cut.rows) {
+            for (int k = cut.first + lane; k < cut.last; k += 32)
+                if (!none(k)) {
+                    const float* p = part(k) + rows_of_tile * DP + r;
+                    if (p[rows_of_tile] != 0.f) top = fmaxf(top, p[0]);
+                }
 #pragma unroll
-    for (int u = 0; u < kPerLane; ++u) v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
 #pragma unroll 4
-    for (int k = c - 1 + warp; k < last; k += kJoinWarps) {
-        if (gaps && bound(k) == bound(k + 1)) continue;
-        const float* p = part(k);
-        const float m = p[rows_of_tile * DP + r], l = p[rows_of_tile * DP + rows_of_tile + r];
-        const float f = l == 0.f ? 0.f : exp2_fast(m - top);    // a part without a weight has zeros
-        sum += l * f;
+            for (int k = cut.first + warp % kWarpsOfRow; k < cut.last; k += kWarpsOfRow) {
+                if (none(k)) continue;
+                const float* p = part(k);
+                const float m = p[rows_of_tile * DP + r], l = p[rows_of_tile * DP + rows_of_tile + r];
+                const float f = l == 0.f ? 0.f : exp2_fast(m - top);    // a part without a weight has zeros
+                sum += l * f;
 #pragma unroll
-        for (int u = 0; u < kPerLane; ++u)
-            if (u * 32 + lane < kVecs) {
-                const float4 o = *reinterpret_cast<const float4*>(p + r * DP + (u * 32 + lane) * 4);
-                v[u].x += o.x * f; v[u].y += o.y * f; v[u].z += o.z * f; v[u].w += o.w * f;
+                for (int u = 0; u < kPerLane; ++u)
+                    if (u * 32 + lane < kVecs) {
+                        const float4 o = *reinterpret_cast<const float4*>(p + r * DP + (u * 32 + lane) * 4);
+                        v[u].x += o.x * f; v[u].y += o.y * f; v[u].z += o.z * f; v[u].w += o.w * f;
+                    }
             }
-    }
+        }
+        if (kWarpsOfRow > 1) {
 #pragma unroll
-    for (int u = 0; u < kPerLane; ++u)
-        if (u * 32 + lane < kVecs) sums[warp][u * 32 + lane] = v[u];
-    if (lane == 0) weights[warp] = sum;
-    __syncthreads();
-    if (tid >= kVecs) return;
-    sum = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int u = 0; u < kPerLane; ++u)
+                if (u * 32 + lane < kVecs) sums[warp][u * 32 + lane] = v[u];
+            if (lane == 0) weights[warp] = sum;
+            __syncthreads();
+            sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) {
-        const float4 q = sums[w][tid];
-        sum += weights[w];
-        o.x += q.x; o.y += q.y; o.z += q.z; o.w += q.w;
+            for (int u = 0; u < kPerLane; ++u) {
+                v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (warp % kWarpsOfRow == 0 && u * 32 + lane < kVecs)
+#pragma unroll
+                    for (int w = 0; w < kWarpsOfRow; ++w) {
+                        const float4 q = sums[warp + w][u * 32 + lane];
+                        v[u].x += q.x; v[u].y += q.y; v[u].z += q.z; v[u].w += q.w;
+                    }
+            }
+            if (warp % kWarpsOfRow == 0)
+#pragma unroll
+                for (int w = 0; w < kWarpsOfRow; ++w) sum += weights[warp + w];
+            __syncthreads();
+        }
+        if (r < cut.rows && warp % kWarpsOfRow == 0) {
+            const int row = cut.m0 + r;
+#pragma unroll
+            for (int u = 0; u < kPerLane; ++u)
+                if (u * 32 + lane < kVecs)
+                    store_row(a, cut.row0 + row / B.group, cut.h * B.group + row % B.group, (u * 32 + lane) * 4, v[u], top, sum);
+        }
     }
-    store_row(a, s.row0 + row / B.group, h * B.group + row % B.group, tid * 4, o, top, sum);
 }
 
 // ---- host
@@ -772,7 +795,7 @@ size_t ogle_cuda_paged_attention_workspace_bytes(const OglePagedBatch* batch, co
     if (!p || paged::translate(batch, b) != OGLE_OK || b.n_seqs == 0) return 0;
     return with_form(choose(batch), [&](auto dp, auto mt, auto split) {
         using F = Form<decltype(dp)::value, decltype(mt)::value, decltype(split)::value>;
-        return size_t(ranges_of(batch, F::kRows, F::kBlocks)) * (2 * F::kPart * sizeof(float) + sizeof(Boundary));
+        return size_t(ranges_of(batch, F::kRows, F::kBlocks)) * (2 * F::kPart * sizeof(float) + sizeof(Cut));
     });
 }
 
@@ -800,7 +823,8 @@ int ogle_cuda_paged_attention(const OglePagedBatch* batch, const OgleAttentionPa
         using F = Form<DP, MT, kSplit>;
         const int ranges = ranges_of(batch, F::kRows, F::kBlocks);
         auto kernel = paged_attention_kernel<DP, MT, kSplit>;
-        a.boundaries = reinterpret_cast<Boundary*>(a.parts + size_t(ranges) * 2 * F::kPart);
+        a.segment_cost = 2LL * a.b.n_seqs * a.b.kv_heads > ranges ? kSegmentCost : 0;
+        a.cuts = reinterpret_cast<Cut*>(a.parts + size_t(ranges) * 2 * F::kPart);
         static std::atomic<uint64_t> sized{0};           // devices whose limit of shared memory is raised
         int device = 0;
         cudaError_t e = cudaGetDevice(&device);
@@ -817,10 +841,13 @@ int ogle_cuda_paged_attention(const OglePagedBatch* batch, const OgleAttentionPa
         if (e != cudaSuccess) { set_last_error(e); (void)cudaGetLastError(); return OGLE_ERR_CUDA; }
         int rc = finish_launch();
         if (rc != OGLE_OK) return rc;
+        // one warp to a row, or eight where few segments are cut into many parts
         const long long rows = (long long)(a.b.max_rows < a.b.n_rows ? a.b.max_rows : a.b.n_rows) * a.b.group;
-        e = launch_overlapped_if(overlapped_launches_enabled(true), paged_join_kernel<DP>,
-                                 dim3(ranges > 1 ? ranges - 1 : 1, unsigned(rows < F::kRows ? (rows < 1 ? 1 : rows) : F::kRows)),
-                                 dim3(kJoinWarps * 32), 0, stream, a, ranges, F::kRows);
+        const int tile = int(rows < F::kRows ? (rows < 1 ? 1 : rows) : F::kRows);
+        const bool many = ranges > 4LL * a.b.n_seqs * a.b.kv_heads;
+        e = launch_overlapped_if(overlapped_launches_enabled(true), many ? paged_join_kernel<DP, kJoinWarps> : paged_join_kernel<DP, 1>,
+                                 dim3(ranges > 1 ? ranges - 1 : 1, many ? tile : div_up(tile, kJoinWarps)), dim3(kJoinWarps * 32), 0, stream,
+                                 a, ranges, F::kRows);
         if (e != cudaSuccess) { set_last_error(e); (void)cudaGetLastError(); return OGLE_ERR_CUDA; }
         return finish_launch();
     });
