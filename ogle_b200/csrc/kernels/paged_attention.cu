@@ -27,7 +27,7 @@ using paged::Batch;
 constexpr int kWarps = 4;
 constexpr int kChunk = 16;                       // keys of a warp's step; a page holds whole steps
 constexpr int kTileKeys = kWarps * kChunk;
-constexpr int kSegmentCost = 2;                  // tiles that a segment's beginning and end take as long as, where there are many
+constexpr int kSegmentCost = 8;                  // tiles that a segment's beginning and end take as long as
 constexpr int kGaveUp = 9;                       // in the library's device status word: a copy did not come
 constexpr float kHeadroom = 8.f;                 // a row's m moves only when an x exceeds it by more: w stays below 2^(8 + 7)
 constexpr float kLift = 7.f;                     // of all weights, away from fp16's smallest numbers
@@ -42,12 +42,13 @@ struct AttnArgs {
     int causal, window;
     float* parts;                                // [ranges][2][kRows] x (DP + 2)
     struct Cut* cuts;                            // [ranges]
-    int segment_cost;
+    int by_segment;                              // tiles of rows a sequence can have, where cuts are kept by segment; else 0
     uint32_t spin_limit;
     int* error;
 };
 
-// What the join needs of a segment that was cut: kept at the range behind its first cut. rows 0: there is none.
+// What the join needs of a segment that was cut. rows 0: it was not. Kept by segment where there are fewer segments than
+// ranges, else by the range that the segment begins in, its last.
 struct __align__(16) Cut {
     int rows, row0, h, m0;         // rows of the tile; row of the sequence's first row; kv head; the tile's first row
     int first, last;               // ranges [first, last) have parts ...
@@ -70,7 +71,12 @@ struct Form {
 };
 
 // ---- the ranges
-struct Place { long long total, first; int b; };   // sum of all tiles; those of the sequences before b; the sequence of the position asked for
+// A 64-bit division takes some hundred instructions, one in 32 bits twenty: nearly all are of small numbers.
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+    return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
+struct Place { long long total, first; int b, cost; };   // sum of all; what comes before b; the sequence of the position asked for; of a segment
 
 __device__ __forceinline__ int row_tiles(const Batch& a, int n, int rows) { return (n * a.group + rows - 1) / rows; }
 
@@ -88,55 +94,63 @@ __device__ __forceinline__ int tiles_of(const paged::Sequence& s, int causal, in
     const Span k = span_of(s, 0, s.n - 1, causal, window);
     return k.hi > k.lo ? (k.hi - 1) / kTileKeys - k.lo / kTileKeys + 1 : 0;
 }
-// What a segment of so many tiles counts in the ranges.
-__device__ __forceinline__ int cost_of(int tiles, int segment_cost) { return tiles > 0 ? tiles + segment_cost : 0; }
+// What a segment of so many tiles counts in the ranges, its beginning and end being worth `cost` tiles.
+__device__ __forceinline__ int counts(int tiles, int cost) { return tiles > 0 ? tiles + cost : 0; }
 
-// Sums the tiles of all sequences and finds the one that position total * num / den (or its end) falls in. All threads of a
-// block of 128; `shared` holds 130 values.
-template <typename F>
-__device__ __forceinline__ Place locate(int n_seqs, int num, int den, long long* shared, F tiles) {
-    const int tid = threadIdx.x, per = (n_seqs + 127) / 128;
-    long long mine = 0;
-    for (int i = 0; i < per; ++i) {
-        const int b = tid * per + i;
-        if (b < n_seqs) mine += tiles(b);
+// Sums what all segments count and finds the sequence that range `num` of `den` begins in. A block of 128 threads; `shared`
+// holds 10 values. A segment's beginning and end - queries, the first copies, the sum over warps - take a block as long as some
+// tiles; they count as a quarter of a range at most, so that short ranges are not spent on them.
+__device__ __forceinline__ Place locate(const AttnArgs& a, int rows, int num, int den, long long* shared) {
+    const Batch& B = a.b;
+    const int tid = threadIdx.x, per = (B.n_seqs + 127) / 128;
+    const auto segments = [&](int b, int& tiles) {
+        const paged::Sequence s = paged::sequence(B, b);
+        tiles = tiles_of(s, a.causal, a.window);
+        return tiles > 0 ? (long long)B.kv_heads * row_tiles(B, s.n, rows) : 0LL;
+    };
+    long long my_tiles = 0, my_segments = 0;
+    for (int i = 0; i < per && tid * per + i < B.n_seqs; ++i) {
+        int tiles;
+        const long long n = segments(tid * per + i, tiles);
+        my_tiles += n * tiles;
+        my_segments += n;
     }
-    long long sum = mine;
+    long long t = my_tiles, n = my_segments;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
-        const long long o = __shfl_up_sync(~0u, sum, d);
-        if ((tid & 31) >= d) sum += o;
+        const long long u = __shfl_up_sync(~0u, t, d), m = __shfl_up_sync(~0u, n, d);
+        if ((tid & 31) >= d) { t += u; n += m; }
     }
-    if ((tid & 31) == 31) shared[tid / 32] = sum;
-    if (tid == 0) shared[5] = -1;
+    if ((tid & 31) == 31) { shared[tid / 32] = t; shared[4 + tid / 32] = n; }
+    if (tid == 0) shared[9] = -1;
     __syncthreads();
-    long long total = 0, before = 0;
+    long long tiles = 0, all = 0;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-        if (w < tid / 32) before += shared[w];
-        total += shared[w];
+        if (w < tid / 32) { t += shared[w]; n += shared[4 + w]; }
+        tiles += shared[w];
+        all += shared[4 + w];
     }
-    const long long at = total * num / den;
-    sum += before;
-    if (at >= sum - mine && at < sum) {
-        long long first = sum - mine;
-        for (int i = 0; i < per; ++i) {
-            const int b = tid * per + i;
-            const long long t = b < n_seqs ? tiles(b) : 0;
-            if (at < first + t) {
-                shared[4] = first;
-                shared[5] = b;
+    Place p;
+    p.cost = int(min((long long)kSegmentCost, quotient(tiles, 4LL * den)));
+    p.total = tiles + all * p.cost;
+    const long long at = quotient(p.total * num, den), sum = t + n * p.cost;
+    long long first = sum - my_tiles - my_segments * p.cost;
+    if (at >= first && at < sum) {
+        for (int i = 0; i < per && tid * per + i < B.n_seqs; ++i) {
+            int k;
+            const long long m = segments(tid * per + i, k), c = m * (k + p.cost);
+            if (at < first + c) {
+                shared[8] = first;
+                shared[9] = tid * per + i;
                 break;
             }
-            first += t;
+            first += c;
         }
     }
     __syncthreads();
-    Place p;
-    p.total = total;
-    p.first = shared[4];
-    p.b = int(shared[5]);
-    __syncthreads();
+    p.first = shared[8];
+    p.b = int(shared[9]);
     return p;
 }
 
@@ -160,7 +174,7 @@ __device__ __forceinline__ void copy_box(uint32_t dst, const CUtensorMap* map, u
 }
 
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -238,15 +252,69 @@ __device__ __forceinline__ void load16(const void* q, long long at, int d, int d
     }
 }
 
+// A block's place in its range and the segment that it has: in shared memory, so that no thread keeps them in registers
+// while it goes through keys.
+struct Walk { long long at, first, end, total; int b, cost; };
+struct Segment {
+    paged::Sequence s;
+    int b, h, m0, m_end;                          // sequence, kv head, rows of the tile
+    int c0, c1, cost;                             // of what the segment counts, the range has [c0, c1)
+    int j_begin, steps;                           // the range's keys in steps
+    Span keys;                                    // that some row attends
+    int inner_lo, inner_hi;                       // that every row attends
+};
+
+// One thread: the next segment of the range; false where there is none.
+template <int kRows>
+__device__ __forceinline__ bool next_segment(const AttnArgs& a, Walk& w, Segment& g) {
+    const Batch& B = a.b;
+    for (; w.at < w.end && w.b < B.n_seqs; ++w.b) {
+        g.s = paged::sequence(B, w.b);
+        const int tiles = tiles_of(g.s, a.causal, a.window), rts = row_tiles(B, g.s.n, kRows);
+        g.cost = counts(tiles, w.cost);
+        const long long all = (long long)B.kv_heads * rts * g.cost;
+        if (w.at >= w.first + all) { w.first += all; continue; }
+        const long long seg = quotient(w.at - w.first, g.cost), seg_first = w.first + seg * g.cost;
+        g.b = w.b;
+        g.h = int(quotient(seg, rts));
+        const int rt = int(seg - (long long)g.h * rts);
+        g.c0 = int(w.at - seg_first);
+        g.c1 = int(min((long long)g.cost, w.end - seg_first));
+        g.m0 = rt * kRows;
+        g.m_end = min(g.s.n * B.group, g.m0 + kRows);
+        const int first_row = g.m0 / B.group, last_row = (g.m_end - 1) / B.group;
+        g.keys = span_of(g.s, first_row, last_row, a.causal, a.window);
+        g.inner_lo = span_of(g.s, last_row, 0, a.causal, a.window).lo;
+        g.inner_hi = span_of(g.s, 0, first_row, a.causal, a.window).hi;
+        // its tiles come behind the segment's cost
+        const int base = span_of(g.s, 0, g.s.n - 1, a.causal, a.window).lo / kTileKeys;
+        const int t0 = max(g.c0 - w.cost, 0), t1 = max(g.c1 - w.cost, 0);
+        g.j_begin = max((base + t0) * kTileKeys, g.keys.lo / kChunk * kChunk);
+        g.steps = max(0, (min((base + t1) * kTileKeys, g.keys.hi) - g.j_begin + kChunk - 1) / kChunk);
+        if (g.c0 == 0 && (a.by_segment || g.c1 < g.cost)) {
+            // up to the first range that begins at or behind the segment's end
+            const long long seg_end = seg_first + g.cost;
+            const int last = min(int(quotient(seg_end * gridDim.x + w.total - 1, w.total)), int(gridDim.x));
+            a.cuts[a.by_segment ? ((long long)g.b * B.kv_heads + g.h) * a.by_segment + rt : blockIdx.x] =
+                Cut{g.c1 < g.cost ? g.m_end - g.m0 : 0, g.s.row0, g.h, g.m0, int(blockIdx.x), last, w.total < gridDim.x, 0, w.total};
+        }
+        w.at = seg_first + g.c1;
+        return true;
+    }
+    return false;
+}
+
 template <int DP, int MT, bool kSplit>
 __global__ void __launch_bounds__(kWarps * 32, (Form<DP, MT, kSplit>::kBlocks))
 paged_attention_kernel(AttnArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
     using F = Form<DP, MT, kSplit>;
     constexpr int kRows = F::kRows, NR = kSplit ? 1 : 2, KS = DP / 16, NB = DP / 8;
     extern __shared__ __align__(16) unsigned char dynamic[];
-    __shared__ long long shared[8];
+    __shared__ long long shared[10];
     __shared__ __align__(8) uint64_t bars[kWarps][F::kStages];
-    __shared__ int gave_up;
+    __shared__ int gave_up, more_segments;
+    __shared__ Walk walk;
+    __shared__ Segment segment;
     unsigned char* const smem = dynamic + ((1024 - (tc::smem_u32(dynamic) & 1023)) & 1023);
     const Batch& B = a.b;
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, c4 = lane & 3, r8 = lane >> 2;
@@ -257,60 +325,31 @@ paged_attention_kernel(AttnArgs a, const __grid_constant__ CUtensorMap k_map, co
     }
     grid_dependency_trigger();
     grid_dependency_wait();
-    const auto weight = [&](int b) {
-        const paged::Sequence s = paged::sequence(B, b);
-        return (long long)B.kv_heads * row_tiles(B, s.n, kRows) * cost_of(tiles_of(s, a.causal, a.window), a.segment_cost);
-    };
-    const Place place = locate(B.n_seqs, blockIdx.x, gridDim.x, shared, weight);    // its barriers: `bars` is set up
-    if (tid == 0) a.cuts[blockIdx.x].rows = 0;
-    bool begun = false;
-    long long at = place.total * blockIdx.x / gridDim.x, first = place.first;
-    const long long end = place.total * (blockIdx.x + 1) / gridDim.x;
-    int b = place.b;
-    const uint32_t ring = tc::smem_u32(smem) + warp * F::kStages * F::kStageBytes, bar0 = tc::smem_u32(&bars[warp][0]);
+    const Place place = locate(a, kRows, blockIdx.x, gridDim.x, shared);    // its barriers: `bars` is set up
+    if (tid == 0) {
+        if (!a.by_segment) a.cuts[blockIdx.x].rows = 0;
+        walk = Walk{quotient(place.total * blockIdx.x, gridDim.x), place.first, quotient(place.total * (blockIdx.x + 1), gridDim.x), place.total, place.b, place.cost};
+        more_segments = place.b >= 0 && next_segment<kRows>(a, walk, segment);
+    }
+    __syncthreads();
+    const unsigned char* const my_ring = smem + warp * F::kStages * F::kStageBytes;
+    const uint32_t ring = tc::smem_u32(my_ring), bar0 = tc::smem_u32(&bars[warp][0]);
     const int nowhere = max(B.n_pages, 1);
     int put = 0, get = 0;                         // stages of the ring: the next to fill, the next to read
     uint32_t parity = 0;                          // of the next to read
     // this lane's rows of the two kinds of loads, as offsets into a step
     const uint32_t value_row = key_of<DP>(lane & 7) + ((lane >> 3) & 1) * 8;
 
-    while (at < end && b < B.n_seqs) {
-        paged::Sequence s = paged::sequence(B, b);
-        const int tiles = tiles_of(s, a.causal, a.window), cost = cost_of(tiles, a.segment_cost), rts = row_tiles(B, s.n, kRows);
-        const long long all = (long long)B.kv_heads * rts * cost;
-        if (at >= first + all) { first += all; ++b; continue; }
-        // segment: kv head, tile of rows; of what it counts this range has [c0, c1), its tiles behind the segment's cost
-        const long long seg = (at - first) / cost;
-        const int h = int(seg / rts), rt = int(seg % rts);
-        const long long seg_first = first + seg * cost;
-        const int c0 = int(at - seg_first), c1 = int(min((long long)cost, end - seg_first));
-        const int t0 = max(c0 - a.segment_cost, 0), t1 = max(c1 - a.segment_cost, 0);
-        const Span all_keys = span_of(s, 0, s.n - 1, a.causal, a.window);
-        const int m0 = rt * kRows, m_end = min(s.n * B.group, m0 + kRows);
-        const Span keys = span_of(s, m0 / B.group, (m_end - 1) / B.group, a.causal, a.window);
-        const int inner_lo = span_of(s, (m_end - 1) / B.group, 0, a.causal, a.window).lo;
-        const int inner_hi = span_of(s, 0, m0 / B.group, a.causal, a.window).hi;
-        if (!begun && c0 > 0 && tid == 0) {       // this range begins with a cut: the segment's first?
-            const auto bound = [&](int k) { return place.total * k / gridDim.x; };
-            int before = blockIdx.x - 1, last = blockIdx.x + 1;
-            while (bound(before) == at) --before; // ranges without a tile
-            if (bound(before) <= seg_first) {
-                while (last < int(gridDim.x) && bound(last) < seg_first + cost) ++last;
-                a.cuts[blockIdx.x] = Cut{m_end - m0, s.row0, h, m0, before, last, place.total < gridDim.x, 0, place.total};
-            }
-        }
-        begun = true;
-        const int base = all_keys.lo / kTileKeys;
-        const int j_begin = max((base + t0) * kTileKeys, keys.lo / kChunk * kChunk), j_end = min((base + t1) * kTileKeys, keys.hi);
-        const int steps = max(0, (j_end - j_begin + kChunk - 1) / kChunk);
-        const int count = steps > warp ? (steps - warp + kWarps - 1) / kWarps : 0;   // of this warp: warp, warp + 4, ...
+    while (more_segments) {
+        const int j_begin = segment.j_begin, h = segment.h, inner_lo = segment.inner_lo, inner_hi = segment.inner_hi;
+        const int count = segment.steps > warp ? (segment.steps - warp + kWarps - 1) / kWarps : 0;   // of this warp: warp, warp + 4, ...
 
         // pages and scales of the warp's next 32 steps, a lane each; the 32 behind them are on their way
         int page[2] = {nowhere, nowhere};         // where there is no page: the copies find themselves outside and bring zeros
         float ks[2] = {0.f, 0.f}, vs[2] = {0.f, 0.f};
         const auto look_up = [&](int which, int i) {
             int p = -1;
-            if (i < count) p = paged::page_of(B, b, (j_begin + (i * kWarps + warp) * kChunk) >> B.page_shift);
+            if (i < count) p = paged::page_of(B, segment.b, (j_begin + (i * kWarps + warp) * kChunk) >> B.page_shift);
             page[which] = p >= 0 ? p : nowhere;
             ks[which] = vs[which] = 0.f;
             if (p >= 0) {
@@ -344,22 +383,18 @@ paged_attention_kernel(AttnArgs a, const __grid_constant__ CUtensorMap k_map, co
         // queries: this thread's parts of the rows it has
         uint32_t Q[MT][KS][4];
         float rs[MT][NR], off[MT][NR], bar_x[MT][NR], l[MT][NR];      // weight 2^(x - off); an x above bar_x moves both
-        int lo_row[MT][NR], hi_row[MT][NR];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
-                const int row = min(m0 + mt * (kSplit ? 8 : 16) + r * 8 + r8, m_end - 1);   // rows that are not there repeat the last
-                const int i = row / B.group, g = row % B.group;
-                const long long q0 = (s.row0 + i) * a.q_row + (h * B.group + g) * a.q_head;
-                const Span k = span_of(s, i, i, a.causal, a.window);
-                lo_row[mt][r] = k.lo;
-                hi_row[mt][r] = k.hi;
+                // rows that are not there repeat the last
+                const int row = min(segment.m0 + mt * (kSplit ? 8 : 16) + r * 8 + r8, segment.m_end - 1);
+                const long long q0 = (segment.s.row0 + row / B.group) * a.q_row + (h * B.group + row % B.group) * a.q_head;
                 off[mt][r] = 0.f;
                 bar_x[mt][r] = -INFINITY;
                 l[mt][r] = 0.f;
                 rs[mt][r] = 0.f;
-                if (steps == 0) continue;         // a range that has the segment's cost alone
+                if (segment.steps == 0) continue; // a range that has the segment's cost alone
                 float f[DP / 4], top = 0.f;
 #pragma unroll
                 for (int u = 0; u < DP / 64; ++u) load16(a.q, q0, 16 * (c4 + 4 * u), B.dim, B.dtype, f + 16 * u);
@@ -398,7 +433,8 @@ paged_attention_kernel(AttnArgs a, const __grid_constant__ CUtensorMap k_map, co
                 page[0] = page[1]; ks[0] = ks[1]; vs[0] = vs[1];
                 look_up(1, i + 32 + lane);
             }
-            const uint32_t at_k = ring + get * F::kStageBytes, at_v = at_k + kChunk * DP;
+            const unsigned char* const step = my_ring + get * F::kStageBytes;
+            const uint32_t at_v = ring + get * F::kStageBytes + kChunk * DP;
             const bool came = wait_copy(bar0 + get * 8, parity, a.spin_limit);
             if (!__all_sync(~0u, came)) {
                 // nothing more is asked for; the copies under way are waited for, this one's among them
@@ -417,50 +453,56 @@ paged_attention_kernel(AttnArgs a, const __grid_constant__ CUtensorMap k_map, co
             const float k_scale = __shfl_sync(~0u, ks[0], i & 31), v_scale = __shfl_sync(~0u, vs[0], i & 31);
             const bool edge = j0 < inner_lo || j0 + kChunk > inner_hi || k_scale == 0.f;
             // x = q . k
-            float x[MT][2][NR * 2];
+            float x[MT][2][NR * 2], S[2][MT][4];
 #pragma unroll
-            for (int nb = 0; nb < 2; ++nb) {
-                float S[MT][4];
+            for (int nb = 0; nb < 2; ++nb)
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                    for (int y = 0; y < 4; ++y) S[mt][y] = 0.f;
+                    for (int y = 0; y < 4; ++y) S[nb][mt][y] = 0.f;
 #pragma unroll
-                for (int u = 0; u < DP / 64; ++u) {
-                    uint32_t w[4];
-                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                                 : "r"(at_k + unit_at<DP>(nb * 8 + key_of<DP>(r8), c4 + 4 * u)) : "memory");
+            for (int u = 0; u < DP / 64; ++u) {
+                uint4 w[2];
 #pragma unroll
-                    for (int y = 0; y < 4; ++y) {
+                for (int nb = 0; nb < 2; ++nb) w[nb] = *reinterpret_cast<const uint4*>(step + unit_at<DP>(nb * 8 + key_of<DP>(r8), c4 + 4 * u));
+#pragma unroll
+                for (int y = 0; y < 4; ++y)       // the two blocks in turn: neither waits for its own last product
+#pragma unroll
+                    for (int nb = 0; nb < 2; ++nb) {
                         uint32_t b0, b1;
-                        paged::e4m3x4_to_half2(w[y], b0, b1);
+                        paged::e4m3x4_to_half2(reinterpret_cast<const uint32_t*>(&w[nb])[y], b0, b1);
 #pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) mma(S[mt], Q[mt][4 * u + y], b0, b1);
+                        for (int mt = 0; mt < MT; ++mt) mma(S[nb][mt], Q[mt][4 * u + y], b0, b1);
                     }
-                }
+            }
+#pragma unroll
+            for (int nb = 0; nb < 2; ++nb)
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
                     if (kSplit) {
-                        x[mt][nb][0] = (S[mt][0] + S[mt][2]) * (rs[mt][0] * k_scale);
-                        x[mt][nb][1] = (S[mt][1] + S[mt][3]) * (rs[mt][0] * k_scale);
+                        x[mt][nb][0] = (S[nb][mt][0] + S[nb][mt][2]) * (rs[mt][0] * k_scale);
+                        x[mt][nb][1] = (S[nb][mt][1] + S[nb][mt][3]) * (rs[mt][0] * k_scale);
                     } else {
 #pragma unroll
-                        for (int y = 0; y < 4; ++y) x[mt][nb][y % (2 * NR)] = S[mt][y] * (rs[mt][(y / 2) % NR] * k_scale);
+                        for (int y = 0; y < 4; ++y) x[mt][nb][y % (2 * NR)] = S[nb][mt][y] * (rs[mt][(y / 2) % NR] * k_scale);
                     }
                 }
-            }
             if (edge) {
                 const bool no_page = __shfl_sync(~0u, page[0], i & 31) == nowhere;
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                    for (int nb = 0; nb < 2; ++nb)
+                    for (int r = 0; r < NR; ++r) {
+                        const int row = min(segment.m0 + mt * (kSplit ? 8 : 16) + r * 8 + r8, segment.m_end - 1) / B.group;
+                        const Span k = span_of(segment.s, row, row, a.causal, a.window);
 #pragma unroll
-                        for (int y = 0; y < 2 * NR; ++y) {
-                            const int j = j0 + nb * 8 + key_of<DP>(c4 * 2 + (y & 1));
-                            if (no_page || j < lo_row[mt][y / 2] || j >= hi_row[mt][y / 2]) x[mt][nb][y] = -INFINITY;
-                        }
+                        for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+                            for (int y = 0; y < 2; ++y) {
+                                const int j = j0 + nb * 8 + key_of<DP>(c4 * 2 + y);
+                                if (no_page || j < k.lo || j >= k.hi) x[mt][nb][2 * r + y] = -INFINITY;
+                            }
+                    }
             }
             // a larger unit for a row's weights or for the values: rare
             bool more = v_scale > vref;
@@ -609,11 +651,11 @@ paged_attention_kernel(AttnArgs a, const __grid_constant__ CUtensorMap k_map, co
                 if (c4 == 0) { row[DP] = bar_x[mt][r] - kHeadroom; row[DP + 1] = sum; }
             }
         __syncthreads();
-        const bool whole = c0 == 0 && c1 == cost;
-        float* const part = a.parts + ((long long)blockIdx.x * 2 + (c0 > 0 ? 0 : 1)) * F::kPart;
+        const bool whole = segment.c0 == 0 && segment.c1 == segment.cost;
+        float* const part = a.parts + ((long long)blockIdx.x * 2 + (segment.c0 > 0 ? 0 : 1)) * F::kPart;
         for (int idx = tid; idx < kRows * (DP / 4); idx += kWarps * 32) {
-            const int r = idx / (DP / 4), d = idx % (DP / 4) * 4, row = m0 + r;
-            if (row >= m_end) continue;
+            const int r = idx / (DP / 4), d = idx % (DP / 4) * 4, row = segment.m0 + r;
+            if (row >= segment.m_end) continue;
             const float* p = reinterpret_cast<const float*>(smem) + r * (DP + 4);
             float top = -INFINITY, sum = 0.f;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -634,18 +676,19 @@ paged_attention_kernel(AttnArgs a, const __grid_constant__ CUtensorMap k_map, co
                 if (d == 0) { part[kRows * DP + r] = top; part[kRows * DP + kRows + r] = sum; }
                 continue;
             }
-            store_row(a, s.row0 + row / B.group, h * B.group + row % B.group, d, v, top, sum);
+            store_row(a, segment.s.row0 + row / B.group, segment.h * B.group + row % B.group, d, v, top, sum);
         }
         // the next segment's copies take the parts' place
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncthreads();
-        at = seg_first + c1;
+        if (tid == 0) more_segments = next_segment<kRows>(a, walk, segment);
+        __syncthreads();
     }
 }
 
 // Adds up the parts of segments that were cut, in the order of their ranges, and answers for sequences without a key. Block
-// (c, y) has the segment whose first cut is the beginning of range c + 1, and of its rows y, y + gridDim.y, ...: kWarpsOfRow
-// warps have a row, and each every so-many-th of its parts.
+// (c, y) has segment c, or the one that begins in range c and goes on in the next; of its rows y, y + gridDim.y, ...:
+// kWarpsOfRow warps have a row, and each every so-many-th of its parts.
 constexpr int kJoinWarps = 8;
 template <int DP, int kWarpsOfRow>
 __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(AttnArgs a, int ranges, int rows_of_tile) {
@@ -653,11 +696,15 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(AttnArgs a,
     __shared__ float4 sums[kJoinWarps][kVecs];
     __shared__ float weights[kJoinWarps];
     const Batch& B = a.b;
-    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, c = blockIdx.x + 1;
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, c = blockIdx.x;
     grid_dependency_trigger();
     grid_dependency_wait();
-    Cut cut = {};
-    if (c < ranges) cut = a.cuts[c];
+    Cut cut = a.cuts[c];
+    if (a.by_segment) {
+        // what nobody has written of: tiles of rows that the sequence does not have, sequences without a key
+        const paged::Sequence s = paged::sequence(B, c / (B.kv_heads * a.by_segment));
+        if (c % a.by_segment >= row_tiles(B, s.n, rows_of_tile) || tiles_of(s, a.causal, a.window) == 0) cut.rows = 0;
+    }
     if (blockIdx.y == 0) {
         for (int b = blockIdx.x; b < B.n_seqs; b += gridDim.x) {
             const paged::Sequence s = paged::sequence(B, b);
@@ -669,7 +716,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(AttnArgs a,
     }
     const int part_floats = rows_of_tile * (DP + 2);
     const auto part = [&](int k) { return a.parts + ((long long)k * 2 + (k == cut.first ? 1 : 0)) * part_floats; };
-    const auto none = [&](int k) { return cut.gaps && cut.total * k / ranges == cut.total * (k + 1) / ranges; };
+    const auto none = [&](int k) { return cut.gaps && quotient(cut.total * k, ranges) == quotient(cut.total * (k + 1), ranges); };
     for (int r0 = blockIdx.y * kRowsAtOnce; r0 < cut.rows; r0 += gridDim.y * kRowsAtOnce) {
         const int r = r0 + warp / kWarpsOfRow;
         float top = -INFINITY, sum = 0.f;
@@ -823,7 +870,9 @@ int ogle_cuda_paged_attention(const OglePagedBatch* batch, const OgleAttentionPa
         using F = Form<DP, MT, kSplit>;
         const int ranges = ranges_of(batch, F::kRows, F::kBlocks);
         auto kernel = paged_attention_kernel<DP, MT, kSplit>;
-        a.segment_cost = 2LL * a.b.n_seqs * a.b.kv_heads > ranges ? kSegmentCost : 0;
+        const long long max_tiles = ((long long)(a.b.max_rows < a.b.n_rows ? a.b.max_rows : a.b.n_rows) * a.b.group + F::kRows - 1) / F::kRows;
+        const long long segments = max_tiles * a.b.n_seqs * a.b.kv_heads;
+        a.by_segment = segments < ranges ? int(max_tiles) : 0;
         a.cuts = reinterpret_cast<Cut*>(a.parts + size_t(ranges) * 2 * F::kPart);
         static std::atomic<uint64_t> sized{0};           // devices whose limit of shared memory is raised
         int device = 0;
@@ -844,9 +893,9 @@ int ogle_cuda_paged_attention(const OglePagedBatch* batch, const OgleAttentionPa
         // one warp to a row, or eight where few segments are cut into many parts
         const long long rows = (long long)(a.b.max_rows < a.b.n_rows ? a.b.max_rows : a.b.n_rows) * a.b.group;
         const int tile = int(rows < F::kRows ? (rows < 1 ? 1 : rows) : F::kRows);
-        const bool many = ranges > 4LL * a.b.n_seqs * a.b.kv_heads;
+        const bool many = ranges > 4 * segments;
         e = launch_overlapped_if(overlapped_launches_enabled(true), many ? paged_join_kernel<DP, kJoinWarps> : paged_join_kernel<DP, 1>,
-                                 dim3(ranges > 1 ? ranges - 1 : 1, many ? tile : div_up(tile, kJoinWarps)), dim3(kJoinWarps * 32), 0, stream,
+                                 dim3(a.by_segment ? unsigned(segments < 1 ? 1 : segments) : ranges, many ? tile : div_up(tile, kJoinWarps)), dim3(kJoinWarps * 32), 0, stream,
                                  a, ranges, F::kRows);
         if (e != cudaSuccess) { set_last_error(e); (void)cudaGetLastError(); return OGLE_ERR_CUDA; }
         return finish_launch();
