@@ -15,47 +15,16 @@
 // then in the same thread, and up to 8 rows cost nothing more.
 #include <type_traits>
 
-#include "paged.cuh"
-#include "tc_common.cuh"
-#include "tma_host.h"
+#include "paged_attention.cuh"
 
 namespace ogle {
 namespace {
 
-using paged::Batch;
+using namespace paged;
 
 constexpr int kWarps = 4;
-constexpr int kChunk = 16;                       // keys of a warp's step; a page holds whole steps
 constexpr int kTileKeys = kWarps * kChunk;
 constexpr int kSegmentCost = 8;                  // tiles that a segment's beginning and end take as long as
-constexpr int kGaveUp = 9;                       // in the library's device status word: a copy did not come
-constexpr float kHeadroom = 8.f;                 // a row's m moves only when an x exceeds it by more: w stays below 2^(8 + 7)
-constexpr float kLift = 7.f;                     // of all weights, away from fp16's smallest numbers
-
-struct AttnArgs {
-    Batch b;
-    const void* q;
-    void* out;
-    float* lse;
-    long long q_row, q_head, out_row, out_head;
-    float scale_log2;
-    int causal, window;
-    float* parts;                                // [ranges][2][kRows] x (DP + 2)
-    struct Cut* cuts;                            // [ranges]
-    int by_segment;                              // tiles of rows a sequence can have, where cuts are kept by segment; else 0
-    uint32_t spin_limit;
-    int* error;
-};
-
-// What the join needs of a segment that was cut. rows 0: it was not. Kept by segment where there are fewer segments than
-// ranges, else by the range that the segment begins in, its last.
-struct __align__(16) Cut {
-    int rows, row0, h, m0;         // rows of the tile; row of the sequence's first row; kv head; the tile's first row
-    int first, last;               // ranges [first, last) have parts ...
-    int gaps, unused;              // ... but for those that have no tile, where there are more ranges than tiles
-    long long total;               // tiles of all segments
-};
-
 template <int DP, int MT, bool kSplit>
 struct Form {
     static constexpr int kRows = MT * (kSplit ? 8 : 16);
@@ -71,24 +40,14 @@ struct Form {
 };
 
 // ---- the ranges
-// A 64-bit division takes some hundred instructions, one in 32 bits twenty: nearly all are of small numbers.
-__device__ __forceinline__ long long quotient(long long a, long long b) {
-    return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
+__device__ __forceinline__ Sequence few_sequence(const AttnArgs& a, int b) {
+    Sequence s = sequence(a.b, b);
+    if (a.few_limit && (long long)s.n * a.b.group > a.few_limit) s.n = 0;
+    return s;
 }
 
 struct Place { long long total, first; int b, cost; };   // sum of all; what comes before b; the sequence of the position asked for; of a segment
 
-__device__ __forceinline__ int row_tiles(const Batch& a, int n, int rows) { return (n * a.group + rows - 1) / rows; }
-
-// Keys that some row of the sequence attends: [lo, hi), lo down to a tile.
-struct Span { int lo, hi; };
-__device__ __forceinline__ Span span_of(const paged::Sequence& s, int first_row, int last_row, int causal, int window) {
-    Span k;
-    k.hi = causal ? min(s.len, s.len - s.n + last_row + 1) : s.len;
-    k.lo = window > 0 ? max(0, s.len - s.n + first_row - window + 1) : 0;
-    k.hi = max(k.hi, 0);
-    return k;
-}
 __device__ __forceinline__ int tiles_of(const paged::Sequence& s, int causal, int window) {
     if (s.n <= 0) return 0;
     const Span k = span_of(s, 0, s.n - 1, causal, window);
@@ -104,7 +63,7 @@ __device__ __forceinline__ Place locate(const AttnArgs& a, int rows, int num, in
     const Batch& B = a.b;
     const int tid = threadIdx.x, per = (B.n_seqs + 127) / 128;
     const auto segments = [&](int b, int& tiles) {
-        const paged::Sequence s = paged::sequence(B, b);
+        const Sequence s = few_sequence(a, b);
         tiles = tiles_of(s, a.causal, a.window);
         return tiles > 0 ? (long long)B.kv_heads * row_tiles(B, s.n, rows) : 0LL;
     };
@@ -167,12 +126,6 @@ __device__ __forceinline__ bool wait_copy(uint32_t bar, uint32_t parity, uint32_
     }
     return false;
 }
-__device__ __forceinline__ void copy_box(uint32_t dst, const CUtensorMap* map, uint32_t bar, int element, int token, int head, int page) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
-        ::"r"(dst), "l"(map), "r"(bar), "r"(element), "r"(token), "r"(head), "r"(page) : "memory");
-}
-
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -182,43 +135,6 @@ __device__ __forceinline__ void ldmatrix_trans(uint32_t (&r)[4], uint32_t addr) 
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-__device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-// What rounding to fp16 left over, as fp16 again.
-__device__ __forceinline__ uint32_t rest_bits(uint32_t rounded, float lo, float hi) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&rounded));
-    return half2_bits(lo - f.x, hi - f.y);
-}
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// Four values of a row of the result from its weighted sum v, its m and its sum of weights; with the first four, its lse.
-__device__ __forceinline__ void store_row(const AttnArgs& a, long long row, int head, int d, float4 v, float m, float sum) {
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;             // no weight: no token attended
-    v.x *= inv; v.y *= inv; v.z *= inv; v.w *= inv;
-    if (d < a.b.dim) {
-        const long long y = row * a.out_row + head * a.out_head + d;
-        if (a.b.dtype == OGLE_F32) {
-            *reinterpret_cast<float4*>(static_cast<float*>(a.out) + y) = v;
-        } else {
-            uint2 z;
-            if (a.b.dtype == OGLE_F16) {
-                z.x = half2_bits(v.x, v.y); z.y = half2_bits(v.z, v.w);
-            } else {
-                const __nv_bfloat162 e = __floats2bfloat162_rn(v.x, v.y), f = __floats2bfloat162_rn(v.z, v.w);
-                z.x = *reinterpret_cast<const uint32_t*>(&e); z.y = *reinterpret_cast<const uint32_t*>(&f);
-            }
-            *reinterpret_cast<uint2*>(static_cast<unsigned short*>(a.out) + y) = z;
-        }
-    }
-    if (d == 0 && a.lse) a.lse[row * a.b.q_heads + head] = sum == 0.f ? -INFINITY : (m - kLift + log2f(sum)) * 0.6931471805599453f;
-}
-
 // Where unit u (16 bytes) of row r of a step's keys or values lies: as the copies' swizzle puts it.
 template <int DP>
 __device__ __forceinline__ int unit_at(int r, int u) {
@@ -227,30 +143,6 @@ __device__ __forceinline__ int unit_at(int r, int u) {
 // The key (of eight) that stands for column n of a product's block: eight lanes that read together get rows in different banks.
 template <int DP>
 __device__ __forceinline__ int key_of(int n) { return DP == 64 ? n : (n >> 1) + (n & 1) * 4; }
-
-// 16 values of a row from element d on, as fp32; zeros behind the head's end.
-__device__ __forceinline__ void load16(const void* q, long long at, int d, int dim, int dtype, float* f) {
-    if (d >= dim) {
-#pragma unroll
-        for (int l = 0; l < 16; ++l) f[l] = 0.f;
-    } else if (dtype == OGLE_F32) {
-        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(q) + at + d);
-#pragma unroll
-        for (int l = 0; l < 4; ++l) {
-            const float4 v = p[l];
-            f[4 * l] = v.x; f[4 * l + 1] = v.y; f[4 * l + 2] = v.z; f[4 * l + 3] = v.w;
-        }
-    } else {
-        const uint4* p = reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(q) + at + d);
-        const uint4 v[2] = {p[0], p[1]};
-        const uint32_t* w = reinterpret_cast<const uint32_t*>(v);
-#pragma unroll
-        for (int l = 0; l < 8; ++l) {
-            const float2 g = dtype == OGLE_F16 ? __half22float2(*reinterpret_cast<const __half2*>(w + l)) : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(w + l));
-            f[2 * l] = g.x; f[2 * l + 1] = g.y;
-        }
-    }
-}
 
 // A block's place in its range and the segment that it has: in shared memory, so that no thread keeps them in registers
 // while it goes through keys.
@@ -269,7 +161,7 @@ template <int kRows>
 __device__ __forceinline__ bool next_segment(const AttnArgs& a, Walk& w, Segment& g) {
     const Batch& B = a.b;
     for (; w.at < w.end && w.b < B.n_seqs; ++w.b) {
-        g.s = paged::sequence(B, w.b);
+        g.s = few_sequence(a, w.b);
         const int tiles = tiles_of(g.s, a.causal, a.window), rts = row_tiles(B, g.s.n, kRows);
         g.cost = counts(tiles, w.cost);
         const long long all = (long long)B.kv_heads * rts * g.cost;
@@ -702,7 +594,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(AttnArgs a,
     Cut cut = a.cuts[c];
     if (a.by_segment) {
         // what nobody has written of: tiles of rows that the sequence does not have, sequences without a key
-        const paged::Sequence s = paged::sequence(B, c / (B.kv_heads * a.by_segment));
+        const Sequence s = few_sequence(a, c / (B.kv_heads * a.by_segment));
         if (c % a.by_segment >= row_tiles(B, s.n, rows_of_tile) || tiles_of(s, a.causal, a.window) == 0) cut.rows = 0;
     }
     if (blockIdx.y == 0) {
@@ -781,9 +673,13 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(AttnArgs a,
 // ---- host
 struct Choice { int dp, mt; bool split; };
 
+constexpr int kFewRows = 64;
+int few_limit(const OglePagedBatch* b);
+
 Choice choose(const OglePagedBatch* b) {
     Choice c;
-    const long long rows = (long long)(b->max_rows < b->n_rows ? b->max_rows : b->n_rows) * (b->q_heads / b->kv_heads);
+    long long rows = (long long)(b->max_rows < b->n_rows ? b->max_rows : b->n_rows) * (b->q_heads / b->kv_heads);
+    if (few_limit(b) && rows > kFewRows) rows = kFewRows;
     c.dp = b->head_dim <= 64 ? 64 : (b->head_dim <= 128 ? 128 : 256);
     c.split = b->dtype == OGLE_F32 || rows <= 8;
     c.mt = c.dp == 256 || rows <= (c.split ? 8 : 16) ? 1 : 2;
@@ -817,6 +713,27 @@ int ranges_of(const OglePagedBatch* b, int rows, int blocks) {
     return all < double(kNumSMs * blocks) ? (all < 1 ? 1 : int(all)) : kNumSMs * blocks;
 }
 
+// Rows x query heads of a group above which a sequence is the prompt form's, or 0: every sequence is taken here. The prompt form reads a
+// key once for 256 rows, where this one reads it for 16 or 32, and needs about 64 of them to be the faster.
+int few_limit(const OglePagedBatch* b) {
+    const long long rows = (long long)(b->max_rows < b->n_rows ? b->max_rows : b->n_rows) * (b->q_heads / b->kv_heads);
+    return b->dtype != OGLE_F32 && b->head_dim <= 128 && rows > kFewRows ? kFewRows : 0;
+}
+// Whether some sequence can have few rows, as far as the host knows.
+bool some_few(const OglePagedBatch* b) { return !few_limit(b) || (long long)b->n_seqs * b->max_rows != b->n_rows; }
+
+size_t few_workspace(const OglePagedBatch* b) {
+    if (!some_few(b)) return 0;
+    return with_form(choose(b), [&](auto dp, auto mt, auto split) {
+        using F = Form<decltype(dp)::value, decltype(mt)::value, decltype(split)::value>;
+        return size_t(ranges_of(b, F::kRows, F::kBlocks)) * (2 * F::kPart * sizeof(float) + sizeof(Cut));
+    });
+}
+
+}  // namespace
+
+namespace paged {
+
 // Map of the cache's bytes whose boxes are 16 tokens of one page and head, swizzled as unit_at says. Elements behind the head's
 // end and pages behind the last read zero.
 bool cache_map(CUtensorMap* m, const Batch& b, const void* cache, int dp) {
@@ -830,7 +747,19 @@ bool cache_map(CUtensorMap* m, const Batch& b, const void* cache, int dp) {
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-}  // namespace
+int launch_join(const AttnArgs& a, int dp, bool many, int entries, int ranges, int tile_rows, int rows, cudaStream_t stream) {
+    const auto run = [&](auto kernel, int y) {
+        const cudaError_t e = launch_overlapped_if(overlapped_launches_enabled(true), kernel, dim3(unsigned(entries), unsigned(y)),
+                                                   dim3(kJoinWarps * 32), 0, stream, a, ranges, tile_rows);
+        if (e != cudaSuccess) { set_last_error(e); (void)cudaGetLastError(); return int(OGLE_ERR_CUDA); }
+        return finish_launch();
+    };
+    if (dp == 64) return many ? run(paged_join_kernel<64, kJoinWarps>, rows) : run(paged_join_kernel<64, 1>, div_up(rows, kJoinWarps));
+    if (dp == 128) return many ? run(paged_join_kernel<128, kJoinWarps>, rows) : run(paged_join_kernel<128, 1>, div_up(rows, kJoinWarps));
+    return many ? run(paged_join_kernel<256, kJoinWarps>, rows) : run(paged_join_kernel<256, 1>, div_up(rows, kJoinWarps));
+}
+
+}  // namespace paged
 }  // namespace ogle
 
 using namespace ogle;
@@ -840,10 +769,9 @@ extern "C" {
 size_t ogle_cuda_paged_attention_workspace_bytes(const OglePagedBatch* batch, const OgleAttentionParams* p) {
     Batch b;
     if (!p || paged::translate(batch, b) != OGLE_OK || b.n_seqs == 0) return 0;
-    return with_form(choose(batch), [&](auto dp, auto mt, auto split) {
-        using F = Form<decltype(dp)::value, decltype(mt)::value, decltype(split)::value>;
-        return size_t(ranges_of(batch, F::kRows, F::kBlocks)) * (2 * F::kPart * sizeof(float) + sizeof(Cut));
-    });
+    // the forms run one after the other: what one has left there the other may overwrite
+    const size_t few = few_workspace(batch), prompts = few_limit(batch) ? prompt_workspace(batch) : 0;
+    return few > prompts ? few : prompts;
 }
 
 int ogle_cuda_paged_attention(const OglePagedBatch* batch, const OgleAttentionParams* p, void* workspace, size_t workspace_bytes,
@@ -864,6 +792,12 @@ int ogle_cuda_paged_attention(const OglePagedBatch* batch, const OgleAttentionPa
     a.parts = static_cast<float*>(workspace);
     a.spin_limit = tc::role_wait_limit();
     a.error = error_flag_ptr();
+    if (!a.error) return OGLE_ERR_CUDA;
+    a.few_limit = few_limit(batch);
+    if (a.few_limit) {
+        rc = launch_prompts(batch, a, workspace, stream);
+        if (rc != OGLE_OK || !some_few(batch)) return rc;
+    }
     return with_form(choose(batch), [&](auto dp, auto mt, auto split) -> int {
         constexpr int DP = decltype(dp)::value, MT = decltype(mt)::value;
         constexpr bool kSplit = decltype(split)::value;
@@ -882,7 +816,7 @@ int ogle_cuda_paged_attention(const OglePagedBatch* batch, const OgleAttentionPa
             if (e == cudaSuccess) sized.fetch_or(1ull << (device & 63), std::memory_order_relaxed);
         }
         CUtensorMap k_map, v_map;
-        if (e == cudaSuccess && (!a.error || !cache_map(&k_map, a.b, a.b.k_cache, DP) || !cache_map(&v_map, a.b, a.b.v_cache, DP))) {
+        if (e == cudaSuccess && (!cache_map(&k_map, a.b, a.b.k_cache, DP) || !cache_map(&v_map, a.b, a.b.v_cache, DP))) {
             set_last_error("paged_attention: no tensor map of the cache");
             return OGLE_ERR_CUDA;
         }
@@ -894,11 +828,7 @@ int ogle_cuda_paged_attention(const OglePagedBatch* batch, const OgleAttentionPa
         const long long rows = (long long)(a.b.max_rows < a.b.n_rows ? a.b.max_rows : a.b.n_rows) * a.b.group;
         const int tile = int(rows < F::kRows ? (rows < 1 ? 1 : rows) : F::kRows);
         const bool many = ranges > 4 * segments;
-        e = launch_overlapped_if(overlapped_launches_enabled(true), many ? paged_join_kernel<DP, kJoinWarps> : paged_join_kernel<DP, 1>,
-                                 dim3(a.by_segment ? unsigned(segments < 1 ? 1 : segments) : ranges, many ? tile : div_up(tile, kJoinWarps)), dim3(kJoinWarps * 32), 0, stream,
-                                 a, ranges, F::kRows);
-        if (e != cudaSuccess) { set_last_error(e); (void)cudaGetLastError(); return OGLE_ERR_CUDA; }
-        return finish_launch();
+        return launch_join(a, DP, many, a.by_segment ? int(segments < 1 ? 1 : segments) : ranges, ranges, F::kRows, tile, stream);
     });
 }
 

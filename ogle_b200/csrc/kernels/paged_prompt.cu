@@ -1,0 +1,723 @@
+// Attention over the paged 8-bit cache for many rows of a sequence: prompts, on the tensor cores (tcgen05).
+//
+// A block has 256 rows (row of the sequence x query head of the group) of one sequence and kv head, as two tiles of 128, and goes
+// through the keys 128 at a time:
+//   one warp      brings a tile of keys and of values, as 8-bit boxes of 16 tokens of a page, and looks up their scales
+//   four warps    turn them into fp16 operands: e4m3 is exact in fp16, and a page's scale relative to the largest of the item is
+//                 a power of two that is multiplied in on the way (exact down to 2^-15 of the largest; what lies below is
+//                 rounded to 2^-33 of the largest value), so that scores and weights know nothing of pages
+//   one thread    issues the products: S = Q K^T per tile, O += P V per tile, P taken from tensor memory
+//   2 x 4 warps   a row a thread: maximum, weights 2^(x - off), their sum; P in fp16 over S; O rescaled when a row's maximum
+//                 has grown by more than 2^8
+// While one tile of rows is being weighted, the other's products run. P lies over S in tensor memory (2 x 128 columns for S,
+// 2 x DP for O), so the next S of a tile is asked for once its P V is through.
+//
+// Work: items (sequence, tile of 256 rows, kv head) laid end to end by their tiles of keys, cut into one range a block; parts
+// of items that were cut go to the workspace and are joined as in the form for few rows (paged_attention.cu). The ranges'
+// beginnings are found by a launch of one block (paged_plan_kernel).
+#include "paged_attention.cuh"
+
+namespace ogle {
+namespace {
+
+using namespace paged;
+
+constexpr int kKeys = 128;                       // of a tile
+constexpr int kTileRows = 128, kItemRows = 2 * kTileRows;
+constexpr int kItemCost = 3;                     // tiles that an item's beginning and end take as long as
+constexpr int kThreads = 14 * 32;                // 8 warps of rows, 4 of conversion, copies, products
+constexpr int kConvertWarp = 8, kCopyWarp = 12, kProductWarp = 13;
+constexpr int kNanKeys = 8192;                   // pieces of 16 values with a NaN that an item's edges can have: 1024 keys x 8
+
+// A piece of 16 values of a token at an item's edge: which of them are NaN.
+struct NanPiece { int key; uint16_t bits, unit; };
+
+struct Start { int b, rt, h, off; };             // where a range begins: sequence, tile of rows, kv head, what of the item lies before; b -1: it is empty
+struct Plan { long long total; int unused[2]; };
+
+struct PromptArgs {
+    AttnArgs a;
+    const Plan* plan;
+    const Start* starts;
+    NanPiece* nans;                              // [ranges][kNanKeys]
+    int max_tiles;                               // tiles of rows that a sequence can have
+};
+
+template <int DP>
+struct Layout {
+    static constexpr int kHalf = kTileRows * 128;                 // 64 elements of 128 rows
+    static constexpr int kTile = DP / 64 * kHalf;                 // a tile of fp16
+    static constexpr int kBytes = kKeys * DP;                     // of e4m3
+    static constexpr int kQ = 0, kK = kQ + 2 * kTile, kV = kK + 2 * kTile, kStageK = kV + 2 * kTile, kStageV = kStageK + kBytes;
+    static constexpr int kSmem = kStageV + kBytes + 1024;
+    static constexpr int kPart = kItemRows * (DP + 2);
+    static constexpr int kO = 256;                                // first column of O in tensor memory
+};
+
+__device__ __forceinline__ Sequence prompt_sequence(const AttnArgs& a, int b) {
+    Sequence s = sequence(a.b, b);
+    if ((long long)s.n * a.b.group <= a.few_limit) s.n = 0;
+    return s;
+}
+
+// Tiles of keys that rows [m0, m_end) of the sequence attend.
+__device__ __forceinline__ int key_tiles(const Span& k) { return k.hi > k.lo ? (k.hi - (k.lo & ~(kChunk - 1)) + kKeys - 1) / kKeys : 0; }
+__device__ __forceinline__ Span item_span(const AttnArgs& a, const Sequence& s, int rt) {
+    const int m0 = rt * kItemRows, m_end = min(s.n * a.b.group, m0 + kItemRows);
+    return span_of(s, m0 / a.b.group, (m_end - 1) / a.b.group, a.causal, a.window);
+}
+// What tile rt of a sequence's rows counts, for each kv head; 0 where there is none, or no key for the whole sequence.
+__device__ __forceinline__ int item_cost(const AttnArgs& a, const Sequence& s, int rt) {
+    if (s.n <= 0 || rt >= row_tiles(a.b, s.n, kItemRows)) return 0;
+    const Span all = span_of(s, 0, s.n - 1, a.causal, a.window);
+    return all.hi > all.lo ? key_tiles(item_span(a, s, rt)) + kItemCost : 0;
+}
+
+// One block: sums all items and writes down where each range begins.
+__global__ void __launch_bounds__(1024) paged_plan_kernel(AttnArgs a, int max_tiles, int ranges, Plan* plan, Start* starts) {
+    __shared__ long long sums[32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const long long n = (long long)a.b.n_seqs * max_tiles;
+    grid_dependency_trigger();
+    grid_dependency_wait();
+    for (int k = tid; k < ranges; k += 1024) starts[k].b = -1;
+    long long total = 0;
+    for (int pass = 0; pass < 2; ++pass) {
+        long long before = 0;
+        for (long long i0 = 0; i0 < n; i0 += 1024) {
+            const long long i = i0 + tid;
+            const int b = int(quotient(i, max_tiles)), rt = int(i - (long long)b * max_tiles);
+            const int cost = i < n ? item_cost(a, prompt_sequence(a, b), rt) : 0;
+            const long long mine = (long long)cost * a.b.kv_heads;
+            long long sum = mine;
+#pragma unroll
+            for (int d = 1; d < 32; d *= 2) {
+                const long long u = __shfl_up_sync(~0u, sum, d);
+                if (lane >= d) sum += u;
+            }
+            __syncthreads();
+            if (lane == 31) sums[warp] = sum;
+            __syncthreads();
+            long long all = 0;
+            for (int w = 0; w < 32; ++w) {
+                if (w < warp) sum += sums[w];
+                all += sums[w];
+            }
+            if (pass == 1 && mine > 0) {
+                const long long begin = before + sum - mine, end = begin + mine;
+                for (int k = int((begin * ranges + total - 1) / total); k < ranges; ++k) {
+                    const long long x = total * k / ranges;
+                    if (x >= end) break;
+                    if (x >= begin && (k == ranges - 1 || x != total * (k + 1) / ranges))   // the last of ranges that begin alike has the tiles
+                        starts[k] = Start{b, rt, int((x - begin) / cost), int((x - begin) % cost)};
+                }
+            }
+            before += all;
+        }
+        total = before;
+        if (pass == 0 && tid == 0) plan->total = total;
+        if (total == 0) break;
+        __syncthreads();
+    }
+}
+
+// A block's place in its range, and the item that it has.
+struct Walk { long long at, end, total; int b, rt, h, off; };
+struct Item {
+    Sequence s;
+    int b, h, m0, m_end;
+    int c0, c1, cost;
+    int j0, tiles;                               // first key of its first tile; tiles of this part
+    Span keys;
+    int inner_lo, inner_hi;                      // keys that every row attends
+};
+
+__device__ __forceinline__ bool next_item(const PromptArgs& p, Walk& w, Item& g) {
+    const AttnArgs& a = p.a;
+    const Batch& B = a.b;
+    while (w.at < w.end && w.b < B.n_seqs) {
+        g.s = prompt_sequence(a, w.b);
+        g.cost = item_cost(a, g.s, w.rt);
+        if (g.cost == 0) {
+            w.rt = w.h = w.off = 0;
+            ++w.b;
+            continue;
+        }
+        g.b = w.b;
+        g.h = w.h;
+        g.m0 = w.rt * kItemRows;
+        g.m_end = min(g.s.n * B.group, g.m0 + kItemRows);
+        g.keys = item_span(a, g.s, w.rt);
+        g.inner_lo = span_of(g.s, (g.m_end - 1) / B.group, 0, a.causal, a.window).lo;
+        g.inner_hi = span_of(g.s, 0, g.m0 / B.group, a.causal, a.window).hi;
+        g.c0 = w.off;
+        g.c1 = int(min((long long)g.cost, w.off + (w.end - w.at)));
+        const int t0 = max(g.c0 - kItemCost, 0), t1 = max(g.c1 - kItemCost, 0);
+        g.j0 = (g.keys.lo & ~(kChunk - 1)) + t0 * kKeys;
+        g.tiles = t1 - t0;
+        if (g.c0 == 0 && g.c1 < g.cost) {
+            const long long item_end = w.at + g.cost;
+            const int last = min(int(quotient(item_end * gridDim.x + w.total - 1, w.total)), int(gridDim.x));
+            a.cuts[blockIdx.x] = Cut{g.m_end - g.m0, g.s.row0, g.h, g.m0, int(blockIdx.x), last, w.total < gridDim.x, 0, w.total};
+        }
+        w.at += g.c1 - g.c0;
+        w.off = 0;
+        if (++w.h == B.kv_heads) { w.h = 0; ++w.rt; }
+        return true;
+    }
+    return false;
+}
+
+// ---- tensor memory
+__device__ __forceinline__ void tmem_load32(uint32_t (&r)[32], uint32_t addr) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr));
+}
+// Nothing that uses the loaded values may come before this.
+__device__ __forceinline__ void tmem_loaded(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+        : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+          "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+          "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+          "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) :: "memory");
+}
+__device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// Operand whose rows run along the multiply's row or column side, 64 of them side by side in 128 bytes of the 128-byte swizzle
+// (values: a token's elements): 8 tokens are 1024 bytes on, the next 64 elements `next` bytes.
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t next) {
+    uint64_t d = (uint64_t)((addr & 0x3FFFFu) >> 4);
+    d |= (uint64_t)(next >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+__device__ __forceinline__ void product(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void product_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+
+// Where 16 bytes, `unit` of row r, of the copied e4m3 tile lie: boxes of 16 rows, as the copies' swizzle puts them.
+template <int DP>
+__device__ __forceinline__ int stage_at(int r, int unit) {
+    return DP == 64 ? r * 64 + (unit ^ ((r >> 1) & 3)) * 16 : r * 128 + (unit ^ (r & 7)) * 16;
+}
+
+struct Bars {
+    uint64_t k_came, k_taken, v_came, v_taken;   // the copied tiles
+    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+    uint64_t q_full, s_full[2], p_full[2], pv_done[2], drain;
+};
+
+template <int DP>
+__global__ void __launch_bounds__(kThreads, 1)
+paged_prompt_kernel(PromptArgs p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
+    using L = Layout<DP>;
+    extern __shared__ __align__(16) unsigned char dynamic[];
+    __shared__ __align__(8) Bars bars;
+    __shared__ Walk walk;
+    __shared__ Item item;
+    __shared__ uint32_t tmem_slot, top_scale[2];   // bits of the item's largest scales of keys and values
+    __shared__ float ratio[2][8];                  // scales of the copied tile's 16-token groups, against those
+    __shared__ int more_items, holes, nan_count;
+    __shared__ volatile int gave_up;
+    unsigned char* const smem = dynamic + ((1024 - (tc::smem_u32(dynamic) & 1023)) & 1023);
+    const uint32_t base = tc::smem_u32(smem);
+    const AttnArgs& a = p.a;
+    const Batch& B = a.b;
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+    if (tid == 0) {
+        tc::mbar_init(&bars.k_came, 1); tc::mbar_init(&bars.v_came, 1);
+        tc::mbar_init(&bars.k_taken, 4); tc::mbar_init(&bars.v_taken, 4);
+        for (int i = 0; i < 2; ++i) {
+            tc::mbar_init(&bars.k_full[i], 4); tc::mbar_init(&bars.v_full[i], 4);
+            tc::mbar_init(&bars.k_empty[i], 1); tc::mbar_init(&bars.v_empty[i], 1);
+            tc::mbar_init(&bars.s_full[i], 1); tc::mbar_init(&bars.p_full[i], 4); tc::mbar_init(&bars.pv_done[i], 1);
+        }
+        tc::mbar_init(&bars.q_full, 8);
+        tc::mbar_init(&bars.drain, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        gave_up = 0;
+        top_scale[0] = top_scale[1] = 0;
+        holes = nan_count = 0;
+    }
+    if (warp == kProductWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(&tmem_slot)), "r"(512u));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+    }
+    grid_dependency_trigger();
+    grid_dependency_wait();
+    if (tid == 0) {
+        a.cuts[blockIdx.x].rows = 0;
+        const Start s = p.starts[blockIdx.x];
+        const long long total = p.plan->total;
+        walk = Walk{quotient(total * blockIdx.x, gridDim.x), quotient(total * (blockIdx.x + 1), gridDim.x), total, s.b, s.rt, s.h, s.off};
+        more_items = s.b >= 0 && next_item(p, walk, item);
+    }
+    before_sync();
+    __syncthreads();
+    after_sync();
+    const uint32_t tmem = tmem_slot;
+    const uint32_t limit = a.spin_limit;
+    volatile int* const abort = &gave_up;
+    // tiles that this thread's role has been through, whatever item they were of
+    uint32_t kv_tiles = 0, q_items = 0, my_tiles = 0, second_tiles = 0;
+    bool failed = false;
+    const auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (!failed && !tc::wait_turn(bar, parity & 1, abort, limit)) {
+            failed = true;
+            if (!*abort) {
+                *abort = 1;
+                tc::record_error(a.error, kGaveUp);
+            }
+        }
+        return !failed;
+    };
+
+    while (more_items) {
+        // the item's largest scales, and whether some of its tokens have no page
+        const int j_first = item.j0, j_last = min(item.keys.hi, item.j0 + item.tiles * kKeys), tiles = item.tiles, h = item.h;
+        const int in_page = (1 << B.page_shift) - 1;
+        if (tiles > 0) {
+            uint32_t top_k = 0, top_v = 0, hole = 0;
+            for (int i = (j_first >> B.page_shift) + tid; i <= (j_last - 1) >> B.page_shift; i += kThreads) {
+                const int page = page_of(B, item.b, i);
+                if (page < 0) { hole = 1; continue; }
+                top_k = max(top_k, __float_as_uint(__ldg(B.k_scale + (long long)page * B.kv_heads + h)) & 0x7fffffffu);
+                top_v = max(top_v, __float_as_uint(__ldg(B.v_scale + (long long)page * B.kv_heads + h)) & 0x7fffffffu);
+            }
+            if (top_k) atomicMax(&top_scale[0], top_k);
+            if (top_v) atomicMax(&top_scale[1], top_v);
+            if (hole) atomicOr(&holes, 1);
+        }
+        __syncthreads();
+        const float k_unit = top_scale[0] ? __uint_as_float(top_scale[0]) : 1.f, v_unit = top_scale[1] ? __uint_as_float(top_scale[1]) : 1.f;
+        const int halves = item.m_end - item.m0 > kTileRows ? 2 : 1;       // tiles of rows that exist
+        const bool with_holes = holes != 0;
+
+        if (warp == kCopyWarp) {
+            // lane g has the 16 tokens of group g
+            const int nowhere = max(B.n_pages, 1);
+            const auto look_up = [&](int t, int& page, float& rk, float& rv) {
+                const int j = j_first + t * kKeys + (lane & 7) * kChunk;
+                page = nowhere;
+                rk = rv = 0.f;
+                if (t >= tiles || j >= item.keys.hi) return;
+                const int x = page_of(B, item.b, j >> B.page_shift);
+                if (x < 0) return;
+                page = x;
+                const long long o = (long long)x * B.kv_heads + h;
+                rk = __ldg(B.k_scale + o) / k_unit;
+                rv = __ldg(B.v_scale + o) / v_unit;
+            };
+            int page;
+            float rk, rv;
+            look_up(0, page, rk, rv);
+            for (int t = 0; t < tiles && !failed; ++t) {
+                const int token = (j_first + t * kKeys + (lane & 7) * kChunk) & in_page, now = page;
+                const float now_k = rk, now_v = rv;
+                look_up(t + 1, page, rk, rv);
+#pragma unroll
+                for (int v = 0; v < 2; ++v) {
+                    uint64_t* const came = v ? &bars.v_came : &bars.k_came;
+                    const bool free = wait(v ? &bars.v_taken : &bars.k_taken, kv_tiles + 1);
+                    if (__any_sync(~0u, !free)) { failed = true; break; }
+                    if (lane < 8) ratio[v][lane] = v ? now_v : now_k;
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_expect_tx(came, L::kBytes);
+                    __syncwarp();
+                    if (lane < 8) copy_box(base + (v ? L::kStageV : L::kStageK) + lane * kChunk * DP, v ? &v_map : &k_map, tc::smem_u32(came), 0, token, h, now);
+                    my_tiles = kv_tiles * 2 + v + 1;                          // copies asked for
+                }
+                ++kv_tiles;
+            }
+        } else if (warp >= kConvertWarp && warp < kCopyWarp) {
+            // a piece is 16 values of a token; eight lanes that store together have two tokens' four pieces: different banks
+            const int piece = lane & 3, row8 = lane >> 2, cw = warp - kConvertWarp;
+            for (int t = 0; t < tiles && !failed; ++t) {
+                const uint32_t st = kv_tiles & 1, use = kv_tiles >> 1;
+                const int j0 = j_first + t * kKeys;
+                const bool edge = j0 < item.inner_lo || j0 + kKeys > item.inner_hi;
+#pragma unroll 1
+                for (int v = 0; v < 2; ++v) {
+                    wait(v ? &bars.v_came : &bars.k_came, kv_tiles);
+                    wait(v ? &bars.v_empty[st] : &bars.k_empty[st], use + 1);
+                    if (__any_sync(~0u, failed)) { failed = true; break; }
+                    const unsigned char* from = smem + (v ? L::kStageV : L::kStageK);
+                    unsigned char* to = smem + (v ? L::kV : L::kK) + st * L::kTile;
+#pragma unroll 2
+                    for (int x = 0; x < kKeys / 32; ++x) {
+                        const int r = cw * 32 + x * 8 + row8;
+                        const __half2 f = __float2half2_rn(ratio[v][r / kChunk]);
+                        uint4 in[DP / 64];
+#pragma unroll
+                        for (int half = 0; half < DP / 64; ++half) in[half] = *reinterpret_cast<const uint4*>(from + stage_at<DP>(r, half * 4 + piece));
+#pragma unroll
+                        for (int half = 0; half < DP / 64; ++half) {
+                            uint32_t y[8];
+                            const uint32_t w[4] = {in[half].x, in[half].y, in[half].z, in[half].w};
+#pragma unroll
+                            for (int z = 0; z < 4; ++z) e4m3x4_to_half2(w[z], y[2 * z], y[2 * z + 1]);
+                            if (v && edge) {
+                                // a NaN of a token that some row does not attend: out of the operand, its rows get it at the end
+                                uint32_t bits = 0;
+#pragma unroll
+                                for (int z = 0; z < 8; ++z) {
+                                    const __half2 g = *reinterpret_cast<const __half2*>(&y[z]);
+                                    const uint32_t n = __hneu2_mask(g, g);
+                                    y[z] &= ~n;
+                                    bits |= ((n & 1) | (n >> 30 & 2)) << (2 * z);
+                                }
+                                const int key = j0 + r;
+                                if (bits && key >= item.keys.lo && key < item.keys.hi) {
+                                    const int at = atomicAdd(&nan_count, 1);
+                                    if (at < kNanKeys) p.nans[(long long)blockIdx.x * kNanKeys + at] = NanPiece{key, uint16_t(bits), uint16_t(half * 4 + piece)};
+                                }
+                            }
+#pragma unroll
+                            for (int z = 0; z < 8; ++z) {
+                                const __half2 g = __hmul2(*reinterpret_cast<const __half2*>(&y[z]), f);
+                                y[z] = *reinterpret_cast<const uint32_t*>(&g);
+                            }
+                            unsigned char* row = to + half * L::kHalf + r * 128;
+                            *reinterpret_cast<uint4*>(row + ((2 * piece) ^ (r & 7)) * 16) = make_uint4(y[0], y[1], y[2], y[3]);
+                            *reinterpret_cast<uint4*>(row + ((2 * piece + 1) ^ (r & 7)) * 16) = make_uint4(y[4], y[5], y[6], y[7]);
+                        }
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) {
+                        tc::mbar_arrive(v ? &bars.v_full[st] : &bars.k_full[st]);
+                        tc::mbar_arrive(v ? &bars.v_taken : &bars.k_taken);
+                    }
+                }
+                ++kv_tiles;
+            }
+        } else if (warp == kProductWarp) {
+            if (tiles > 0 && tc::elect_one()) {
+                constexpr uint32_t kF16 = (1u << 4) | ((uint32_t)(kTileRows >> 4) << 24);     // fp16 x fp16 into fp32, 128 rows
+                constexpr uint32_t kScores = kF16 | ((uint32_t)(kKeys >> 3) << 17);
+                constexpr uint32_t kSums = kF16 | (1u << 16) | ((uint32_t)(DP >> 3) << 17);   // values: elements side by side
+                uint32_t done = kv_tiles;                   // tiles of keys whose products have been asked for
+                const auto scores = [&](int q) {            // S = Q K^T of tile `done`'s keys
+                    const uint64_t qd = tc::umma_desc(base + L::kQ + q * L::kTile), kd = tc::umma_desc(base + L::kK + (done & 1) * L::kTile);
+#pragma unroll
+                    for (int k = 0; k < DP / 16; ++k) {
+                        const uint64_t o = (uint64_t)((k / 4) * (L::kHalf >> 4) + (k % 4) * 2);
+                        product(tmem + q * kKeys, qd + o, kd + o, kScores, k > 0);
+                    }
+                    tc::umma_commit(&bars.s_full[q]);
+                };
+                bool ok = wait(&bars.q_full, q_items) && wait(&bars.k_full[done & 1], done >> 1);
+                if (ok) {
+                    after_sync();
+                    for (int q = 0; q < halves; ++q) scores(q);
+                    tc::umma_commit(&bars.k_empty[done & 1]);
+                }
+                for (int t = 0; ok && t < tiles; ++t) {
+                    const uint32_t now = done++;            // values of `now`, keys of `done`
+                    ok = wait(&bars.v_full[now & 1], now >> 1);
+                    for (int q = 0; ok && q < halves; ++q) {
+                        const uint32_t turn = (q ? second_tiles : my_tiles) + t;
+                        ok = wait(&bars.p_full[q], turn);
+                        if (!ok) break;
+                        after_sync();
+                        const uint32_t vbase = base + L::kV + (now & 1) * L::kTile;
+#pragma unroll
+                        for (int k = 0; k < kKeys / 16; ++k)
+                            product_tmem(tmem + L::kO + q * DP, tmem + q * kKeys + k * 8, desc_mn(vbase + k * 2048, L::kHalf), kSums, t > 0 || k > 0);
+                        tc::umma_commit(&bars.pv_done[q]);
+                        if (t + 1 < tiles) {
+                            if (q == 0) ok = wait(&bars.k_full[done & 1], done >> 1);
+                            ok = ok && wait(&bars.pv_done[q], turn);          // P lies where the next S will
+                            if (ok) {
+                                after_sync();
+                                scores(q);
+                            }
+                        }
+                    }
+                    if (ok) {
+                        tc::umma_commit(&bars.v_empty[now & 1]);
+                        if (t + 1 < tiles) tc::umma_commit(&bars.k_empty[done & 1]);
+                    }
+                }
+                if (!ok) {                                  // products under way end before tensor memory is given back
+                    tc::umma_commit(&bars.drain);
+                    tc::mbar_wait(&bars.drain, 0);
+                }
+            }
+            __syncwarp();
+            kv_tiles += tiles;
+            my_tiles += tiles;
+            if (halves == 2) second_tiles += tiles;
+            if (tiles > 0) ++q_items;
+        } else {
+            const int q = warp / 4, r = tid & 127;           // tile, row of it
+            const bool mine = q < halves;
+            const int row = min(item.m0 + q * kTileRows + r, item.m_end - 1);
+            const bool exists = item.m0 + q * kTileRows + r < item.m_end;
+            const int seq_row = row / B.group, head = h * B.group + row % B.group;
+            const Span k = span_of(item.s, seq_row, seq_row, a.causal, a.window);
+            float rs = 0.f;
+            if (tiles > 0 && mine) {
+                const long long q0 = (item.s.row0 + seq_row) * a.q_row + head * a.q_head;
+                float top = 0.f, f[16];
+                for (int d = 0; d < B.dim; d += 16) {
+                    load16(a.q, q0, d, B.dim, B.dtype, f);
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) top = fmaxf(top, fabsf(f[x]));
+                }
+                const int e = top > 1e-30f && top <= 3e38f ? int(__float_as_uint(top) >> 23) - 126 - 12 : 0;
+                float down = __uint_as_float(uint32_t(127 - e) << 23);
+                rs = a.scale_log2 * __uint_as_float(uint32_t(127 + e) << 23) * k_unit;
+                if (rs < 0.f) { rs = -rs; down = -down; }    // the largest product is then the largest x
+                rs = fmaxf(rs, 1e-37f);                      // scores scaled by 0 are alike, hidden ones are not
+#pragma unroll 1
+                for (int d = 0; d < DP; d += 16) {
+                    load16(a.q, q0, d, B.dim, B.dtype, f);
+                    uint32_t y[8];
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) y[x] = half2_bits(f[2 * x] * down, f[2 * x + 1] * down);
+                    unsigned char* to = smem + L::kQ + q * L::kTile + (d / 64) * L::kHalf + r * 128;
+                    const int c = d % 64 / 8;
+                    *reinterpret_cast<uint4*>(to + (c ^ (r & 7)) * 16) = make_uint4(y[0], y[1], y[2], y[3]);
+                    *reinterpret_cast<uint4*>(to + ((c + 1) ^ (r & 7)) * 16) = make_uint4(y[4], y[5], y[6], y[7]);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            }
+            __syncwarp();
+            if (tiles > 0 && lane == 0) tc::mbar_arrive(&bars.q_full);
+
+            const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_at = tmem + lanes + q * kKeys, o_at = tmem + lanes + L::kO + q * DP;
+            float off = 0.f, bar_x = -INFINITY, l = 0.f;
+            for (int t = 0; mine && t < tiles; ++t) {
+                wait(&bars.s_full[q], my_tiles + t);
+                if (__any_sync(~0u, failed)) { failed = true; break; }
+                after_sync();
+                const int j0 = j_first + t * kKeys;
+                const bool edge = with_holes || j0 < item.inner_lo || j0 + kKeys > item.inner_hi;
+                // columns of 32 keys that the row does not attend become minus infinity
+                const auto hide = [&](uint32_t (&s)[32], int c) {
+                    const int lo = k.lo - j0 - c * 32, hi = k.hi - j0 - c * 32;
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) if (x < lo || x >= hi) s[x] = 0xff800000u;
+                    if (with_holes) {
+#pragma unroll
+                        for (int g = 0; g < 2; ++g) {
+                            const int j = j0 + c * 32 + g * 16;
+                            if (j < item.keys.hi && page_of(B, item.b, j >> B.page_shift) < 0)
+#pragma unroll
+                                for (int x = 0; x < 16; ++x) s[g * 16 + x] = 0xff800000u;
+                        }
+                    }
+                };
+                float top = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < kKeys / 32; ++c) {
+                    uint32_t s[32];
+                    tmem_load32(s, s_at + c * 32);
+                    tmem_loaded(s);
+                    if (edge) hide(s, c);
+                    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) m[x & 3] = fmaxf(m[x & 3], __uint_as_float(s[x]));
+                    top = fmaxf(top, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
+                }
+                top *= rs;
+                if (__any_sync(~0u, top > bar_x)) {
+                    const float old = bar_x - kHeadroom, now = fmaxf(top, old);
+                    float f = 1.f;
+                    if (now > -INFINITY) {
+                        f = exp2_fast(old - now);
+                        off = now - kLift;
+                        bar_x = now + kHeadroom;
+                    }
+                    l *= f;
+                    if (t > 0) {
+#pragma unroll 1
+                        for (int c = 0; c < DP / 32; ++c) {
+                            uint32_t o[32];
+                            tmem_load32(o, o_at + c * 32);
+                            tmem_loaded(o);
+#pragma unroll
+                            for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+                            tc::tmem_st16(o_at + c * 32, reinterpret_cast<const uint32_t(&)[16]>(o[0]));
+                            tc::tmem_st16(o_at + c * 32 + 16, reinterpret_cast<const uint32_t(&)[16]>(o[16]));
+                        }
+                    }
+                }
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < kKeys / 32; ++c) {
+                    uint32_t s[32], w[16];
+                    tmem_load32(s, s_at + c * 32);
+                    tmem_loaded(s);
+                    if (edge) hide(s, c);
+#pragma unroll
+                    for (int x = 0; x < 32; x += 2) {
+                        const float u = exp2_fast(fmaf(__uint_as_float(s[x]), rs, -off)), v = exp2_fast(fmaf(__uint_as_float(s[x + 1]), rs, -off));
+                        sum[x & 2] += u;
+                        sum[(x & 2) + 1] += v;
+                        w[x / 2] = half2_bits(u, v);
+                    }
+                    tc::tmem_st16(s_at + c * 16, w);          // over columns that have been read
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tmem_stored();
+                before_sync();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&bars.p_full[q]);
+            }
+            if (mine && tiles > 0) {
+                wait(&bars.pv_done[q], my_tiles + tiles - 1);
+                if (__any_sync(~0u, failed)) failed = true;
+                after_sync();
+            }
+            asm volatile("bar.sync 1, 384;" ::: "memory");    // the conversion's notes of NaNs
+            const bool whole = item.c0 == 0 && item.c1 == item.cost;
+            if (mine && !failed) {
+                uint32_t nan[4] = {0, 0, 0, 0};
+                const int n = min(*(volatile int*)&nan_count, kNanKeys);
+                for (int i = 0; i < n; ++i) {
+                    const NanPiece* g = p.nans + (long long)blockIdx.x * kNanKeys + i;
+                    const int key = *(volatile const int*)&g->key;
+                    const uint32_t bits = *(volatile const uint16_t*)&g->bits, unit = *(volatile const uint16_t*)&g->unit;
+                    if (key >= k.lo && key < k.hi)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) if (x == int(unit / 2)) nan[x] |= bits << (16 * (unit & 1));
+                }
+                float* const part = a.parts + ((long long)blockIdx.x * 2 + (item.c0 > 0 ? 0 : 1)) * L::kPart;
+                const int part_row = q * kTileRows + r;
+                const float m = bar_x - kHeadroom;
+#pragma unroll
+                for (int c = 0; c < DP / 32; ++c) {
+                    uint32_t o[32];
+                    if (tiles > 0) {
+                        tmem_load32(o, o_at + c * 32);
+                        tmem_loaded(o);
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < 32; ++x) o[x] = 0;
+                    }
+                    if (!exists) continue;
+#pragma unroll
+                    for (int x = 0; x < 32; x += 4) {
+                        float4 v;
+                        v.x = nan[c] >> x & 1 ? NAN : __uint_as_float(o[x]) * v_unit;
+                        v.y = nan[c] >> (x + 1) & 1 ? NAN : __uint_as_float(o[x + 1]) * v_unit;
+                        v.z = nan[c] >> (x + 2) & 1 ? NAN : __uint_as_float(o[x + 2]) * v_unit;
+                        v.w = nan[c] >> (x + 3) & 1 ? NAN : __uint_as_float(o[x + 3]) * v_unit;
+                        if (whole) store_row(a, item.s.row0 + seq_row, head, c * 32 + x, v, m, l);
+                        else *reinterpret_cast<float4*>(part + part_row * DP + c * 32 + x) = v;
+                    }
+                }
+                if (!whole && exists) {
+                    part[kItemRows * DP + part_row] = m;
+                    part[kItemRows * DP + kItemRows + part_row] = l;
+                }
+                before_sync();
+            }
+            if (mine) my_tiles += tiles;
+        }
+        if (warp >= kConvertWarp && warp < kCopyWarp) asm volatile("bar.sync 1, 384;" ::: "memory");
+        before_sync();
+        __syncthreads();
+        after_sync();
+        if (gave_up) break;
+        if (tid == 0) {
+            top_scale[0] = top_scale[1] = 0;
+            holes = nan_count = 0;
+            more_items = next_item(p, walk, item);
+        }
+        __syncthreads();
+    }
+    // a copy that nobody has waited for lands before the block ends
+    if (warp == kCopyWarp && gave_up && my_tiles > 0) {
+        const uint32_t last = my_tiles - 1;                    // copy `last`: keys and values in turn
+        tc::mbar_wait(last & 1 ? &bars.v_came : &bars.k_came, (last >> 1) & 1);
+        if (last > 0) tc::mbar_wait(last & 1 ? &bars.k_came : &bars.v_came, ((last - 1) >> 1) & 1);
+    }
+    before_sync();
+    __syncthreads();
+    after_sync();
+    if (warp == kProductWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+}
+
+// Blocks: one to an SM, and no more than there can be tiles.
+int prompt_ranges(const OglePagedBatch* b) { return kNumSMs; }
+long long prompt_tiles(const OglePagedBatch* b) {
+    const long long rows = b->max_rows < b->n_rows ? b->max_rows : b->n_rows;
+    return (rows * (b->q_heads / b->kv_heads) + kItemRows - 1) / kItemRows;
+}
+size_t up16(size_t n) { return (n + 15) & ~size_t(15); }
+
+template <int DP>
+int launch_form(const OglePagedBatch* b, PromptArgs p, void* workspace, cudaStream_t stream) {
+    using L = Layout<DP>;
+    const int ranges = prompt_ranges(b);
+    unsigned char* w = static_cast<unsigned char*>(workspace);
+    p.a.parts = reinterpret_cast<float*>(w); w += up16(size_t(ranges) * 2 * L::kPart * sizeof(float));
+    p.a.cuts = reinterpret_cast<Cut*>(w); w += up16(ranges * sizeof(Cut));
+    Plan* plan = reinterpret_cast<Plan*>(w); w += sizeof(Plan);
+    Start* starts = reinterpret_cast<Start*>(w); w += ranges * sizeof(Start);
+    p.nans = reinterpret_cast<NanPiece*>(w);
+    p.plan = plan; p.starts = starts;
+    p.max_tiles = int(prompt_tiles(b));
+    auto kernel = paged_prompt_kernel<DP>;
+    static std::atomic<uint64_t> sized{0};               // devices whose limit of shared memory is raised
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e == cudaSuccess && !(sized.load(std::memory_order_relaxed) >> (device & 63) & 1)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
+        if (e == cudaSuccess) sized.fetch_or(1ull << (device & 63), std::memory_order_relaxed);
+    }
+    CUtensorMap k_map, v_map;
+    if (e == cudaSuccess && (!cache_map(&k_map, p.a.b, p.a.b.k_cache, DP) || !cache_map(&v_map, p.a.b, p.a.b.v_cache, DP))) {
+        set_last_error("paged_attention: no tensor map of the cache");
+        return OGLE_ERR_CUDA;
+    }
+    if (e == cudaSuccess) e = launch_overlapped(paged_plan_kernel, dim3(1), dim3(1024), 0, stream, p.a, p.max_tiles, ranges, plan, starts);
+    if (e != cudaSuccess) { set_last_error(e); (void)cudaGetLastError(); return OGLE_ERR_CUDA; }
+    int rc = finish_launch();
+    if (rc != OGLE_OK) return rc;
+    e = launch_overlapped_if(overlapped_launches_enabled(true), kernel, dim3(ranges), dim3(kThreads), L::kSmem, stream, p, k_map, v_map);
+    if (e != cudaSuccess) { set_last_error(e); (void)cudaGetLastError(); return OGLE_ERR_CUDA; }
+    rc = finish_launch();
+    if (rc != OGLE_OK) return rc;
+    p.a.by_segment = 0;
+    return launch_join(p.a, DP, false, ranges, ranges, kItemRows, kItemRows, stream);
+}
+
+}  // namespace
+
+namespace paged {
+
+size_t prompt_workspace(const OglePagedBatch* b) {
+    const int ranges = prompt_ranges(b);
+    const size_t part = b->head_dim <= 64 ? Layout<64>::kPart : Layout<128>::kPart;
+    return up16(size_t(ranges) * 2 * part * sizeof(float)) + up16(ranges * sizeof(Cut)) + sizeof(Plan) + ranges * sizeof(Start) +
+           size_t(ranges) * kNanKeys * sizeof(NanPiece);
+}
+
+int launch_prompts(const OglePagedBatch* b, AttnArgs a, void* workspace, cudaStream_t stream) {
+    PromptArgs p = {};
+    p.a = a;
+    return b->head_dim <= 64 ? launch_form<64>(b, p, workspace, stream) : launch_form<128>(b, p, workspace, stream);
+}
+
+}  // namespace paged
+}  // namespace ogle
