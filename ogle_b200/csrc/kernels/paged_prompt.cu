@@ -25,7 +25,9 @@ using namespace paged;
 constexpr int kKeys = 128;                       // of a tile
 constexpr int kTileRows = 128, kItemRows = 2 * kTileRows;
 constexpr int kItemCost = 3;                     // tiles that an item's beginning and end take as long as
-constexpr int kThreads = 14 * 32;                // 8 warps of rows, 4 of conversion, copies, products
+constexpr int kThreads = 16 * 32;                // 8 warps of rows, 4 of conversion, copies, products, and two that fill up their group
+// Registers of a thread: a row has its 128 scores in them. (2 x 184 + 96 + 48) x 128 = the 128 of 512 threads at launch.
+constexpr int kRowRegisters = 184, kConvertRegisters = 96, kIssueRegisters = 48;
 constexpr int kConvertWarp = 8, kCopyWarp = 12, kProductWarp = 13;
 constexpr int kNanKeys = 8192;                   // pieces of 16 values with a NaN that an item's edges can have: 1024 keys x 8
 
@@ -188,6 +190,38 @@ __device__ __forceinline__ void tmem_loaded(uint32_t (&r)[32]) {
           "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
           "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) :: "memory");
 }
+__device__ __forceinline__ void tmem_load16(uint32_t (&r)[16], uint32_t addr) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr) : "memory");
+}
+// Four loads of 32 columns and one wait.
+__device__ __forceinline__ void tmem_load128(uint32_t (&s)[4][32], uint32_t addr) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) tmem_load32(s[c], addr + c * 32);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) tmem_loaded(s[c]);
+}
+__device__ __forceinline__ unsigned long long pair(float lo, float hi) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpair(unsigned long long v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 __device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -232,6 +266,7 @@ paged_prompt_kernel(PromptArgs p, const __grid_constant__ CUtensorMap k_map, con
     __shared__ Walk walk;
     __shared__ Item item;
     __shared__ uint32_t tmem_slot, top_scale[2];   // bits of the item's largest scales of keys and values
+    __shared__ float row_scale[2][kTileRows];      // 2^e that a row's queries were divided by
     __shared__ float ratio[2][8];                  // scales of the copied tile's 16-token groups, against those
     __shared__ int more_items, holes, nan_count;
     __shared__ volatile int gave_up;
@@ -288,66 +323,249 @@ paged_prompt_kernel(PromptArgs p, const __grid_constant__ CUtensorMap k_map, con
         return !failed;
     };
 
-    while (more_items) {
-        // the item's largest scales, and whether some of its tokens have no page
-        const int j_first = item.j0, j_last = min(item.keys.hi, item.j0 + item.tiles * kKeys), tiles = item.tiles, h = item.h;
-        const int in_page = (1 << B.page_shift) - 1;
+    // Every role goes through the items together: all threads look at the item's scales before it, and meet behind it.
+    int j_first = 0, tiles = 0, halves = 0;        // first key, tiles of keys, tiles of rows that exist
+    float k_unit = 1.f, v_unit = 1.f;              // the largest scales
+    bool with_holes = false;                       // some of its tokens have no page
+    const auto begin_item = [&]() {
+        j_first = item.j0;
+        tiles = item.tiles;
+        const int j_last = min(item.keys.hi, j_first + tiles * kKeys);
         if (tiles > 0) {
             uint32_t top_k = 0, top_v = 0, hole = 0;
             for (int i = (j_first >> B.page_shift) + tid; i <= (j_last - 1) >> B.page_shift; i += kThreads) {
                 const int page = page_of(B, item.b, i);
                 if (page < 0) { hole = 1; continue; }
-                top_k = max(top_k, __float_as_uint(__ldg(B.k_scale + (long long)page * B.kv_heads + h)) & 0x7fffffffu);
-                top_v = max(top_v, __float_as_uint(__ldg(B.v_scale + (long long)page * B.kv_heads + h)) & 0x7fffffffu);
+                const long long o = (long long)page * B.kv_heads + item.h;
+                top_k = max(top_k, __float_as_uint(__ldg(B.k_scale + o)) & 0x7fffffffu);
+                top_v = max(top_v, __float_as_uint(__ldg(B.v_scale + o)) & 0x7fffffffu);
             }
             if (top_k) atomicMax(&top_scale[0], top_k);
             if (top_v) atomicMax(&top_scale[1], top_v);
             if (hole) atomicOr(&holes, 1);
         }
         __syncthreads();
-        const float k_unit = top_scale[0] ? __uint_as_float(top_scale[0]) : 1.f, v_unit = top_scale[1] ? __uint_as_float(top_scale[1]) : 1.f;
-        const int halves = item.m_end - item.m0 > kTileRows ? 2 : 1;       // tiles of rows that exist
-        const bool with_holes = holes != 0;
+        k_unit = top_scale[0] ? __uint_as_float(top_scale[0]) : 1.f;
+        v_unit = top_scale[1] ? __uint_as_float(top_scale[1]) : 1.f;
+        halves = item.m_end - item.m0 > kTileRows ? 2 : 1;
+        with_holes = holes != 0;
+    };
+    const auto end_item = [&]() {                  // false: no item is left, or a wait has run out
+        before_sync();
+        __syncthreads();
+        after_sync();
+        if (gave_up) return false;
+        if (tid == 0) {
+            top_scale[0] = top_scale[1] = 0;
+            holes = nan_count = 0;
+            more_items = next_item(p, walk, item);
+        }
+        __syncthreads();
+        return more_items != 0;
+    };
 
-        if (warp == kCopyWarp) {
-            // lane g has the 16 tokens of group g
-            const int nowhere = max(B.n_pages, 1);
-            const auto look_up = [&](int t, int& page, float& rk, float& rv) {
-                const int j = j_first + t * kKeys + (lane & 7) * kChunk;
-                page = nowhere;
-                rk = rv = 0.f;
-                if (t >= tiles || j >= item.keys.hi) return;
-                const int x = page_of(B, item.b, j >> B.page_shift);
-                if (x < 0) return;
-                page = x;
-                const long long o = (long long)x * B.kv_heads + h;
-                rk = __ldg(B.k_scale + o) / k_unit;
-                rv = __ldg(B.v_scale + o) / v_unit;
-            };
-            int page;
-            float rk, rv;
-            look_up(0, page, rk, rv);
-            for (int t = 0; t < tiles && !failed; ++t) {
-                const int token = (j_first + t * kKeys + (lane & 7) * kChunk) & in_page, now = page;
-                const float now_k = rk, now_v = rv;
-                look_up(t + 1, page, rk, rv);
+    if (warp < kConvertWarp) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRowRegisters));
+        const int q = warp / 4, r = tid & 127;           // tile, row of it
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_at = tmem + lanes + q * kKeys, o_at = tmem + lanes + L::kO + q * DP;
+        for (bool more = more_items != 0; more; more = end_item()) {
+            begin_item();
+            const int h = item.h;
+            const bool mine = q < halves;
+            const int row = min(item.m0 + q * kTileRows + r, item.m_end - 1);
+            const int seq_row = row / B.group, head = h * B.group + row % B.group;
+            const Span k = span_of(item.s, seq_row, seq_row, a.causal, a.window);
+            if (tiles > 0 && mine) {
+                // queries of the warp's 32 rows, 16 values a lane: rows side by side are read together
+                constexpr int kLanes = DP / 16, kTogether = 32 / kLanes, kRounds = 32 / kTogether;
+                const int d = lane % kLanes * 16;
+                const bool back = a.scale_log2 < 0.f;        // the largest product is then the largest x
+#pragma unroll 2
+                for (int x = 0; x < kRounds; ++x) {
+                    const int at = (warp & 3) * 32 + x * kTogether + lane / kLanes, m = min(item.m0 + q * kTileRows + at, item.m_end - 1);
+                    float f[16], top = 0.f;
+                    load16(a.q, (item.s.row0 + m / B.group) * a.q_row + (h * B.group + m % B.group) * a.q_head, d, B.dim, B.dtype, f);
 #pragma unroll
-                for (int v = 0; v < 2; ++v) {
-                    uint64_t* const came = v ? &bars.v_came : &bars.k_came;
-                    const bool free = wait(v ? &bars.v_taken : &bars.k_taken, kv_tiles + 1);
-                    if (__any_sync(~0u, !free)) { failed = true; break; }
-                    if (lane < 8) ratio[v][lane] = v ? now_v : now_k;
-                    __syncwarp();
-                    if (lane == 0) tc::mbar_expect_tx(came, L::kBytes);
-                    __syncwarp();
-                    if (lane < 8) copy_box(base + (v ? L::kStageV : L::kStageK) + lane * kChunk * DP, v ? &v_map : &k_map, tc::smem_u32(came), 0, token, h, now);
-                    my_tiles = kv_tiles * 2 + v + 1;                          // copies asked for
+                    for (int y = 0; y < 16; ++y) top = fmaxf(top, fabsf(f[y]));
+#pragma unroll
+                    for (int y = 1; y < kLanes; y *= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, y));
+                    const int e = top > 1e-30f && top <= 3e38f ? int(__float_as_uint(top) >> 23) - 126 - 12 : 0;
+                    const float down = __uint_as_float(uint32_t(127 - e) << 23 | (back ? 0x80000000u : 0u));
+                    if (lane % kLanes == 0) row_scale[q][at] = __uint_as_float(uint32_t(127 + e) << 23);
+                    uint32_t y[8];
+#pragma unroll
+                    for (int z = 0; z < 8; ++z) y[z] = half2_bits(f[2 * z] * down, f[2 * z + 1] * down);
+                    unsigned char* to = smem + L::kQ + q * L::kTile + (d / 64) * L::kHalf + at * 128;
+                    const int c = d % 64 / 8;
+                    *reinterpret_cast<uint4*>(to + (c ^ (at & 7)) * 16) = make_uint4(y[0], y[1], y[2], y[3]);
+                    *reinterpret_cast<uint4*>(to + ((c + 1) ^ (at & 7)) * 16) = make_uint4(y[4], y[5], y[6], y[7]);
                 }
-                ++kv_tiles;
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             }
-        } else if (warp >= kConvertWarp && warp < kCopyWarp) {
-            // a piece is 16 values of a token; eight lanes that store together have two tokens' four pieces: different banks
-            const int piece = lane & 3, row8 = lane >> 2, cw = warp - kConvertWarp;
+            __syncwarp();
+            if (tiles > 0 && lane == 0) tc::mbar_arrive(&bars.q_full);
+            // scores scaled by 0 are alike, hidden ones are not
+            const float rs = mine && tiles > 0 ? fmaxf(fabsf(a.scale_log2) * row_scale[q][r] * k_unit, 1e-37f) : 0.f;
+
+            float off = 0.f, bar_x = -INFINITY, l = 0.f;
+            for (int t = 0; mine && t < tiles; ++t) {
+                wait(&bars.s_full[q], my_tiles + t);
+                if (__any_sync(~0u, failed)) { failed = true; break; }
+                after_sync();
+                const int j0 = j_first + t * kKeys;
+                uint32_t s[4][32];
+                tmem_load128(s, s_at);
+                if (with_holes || j0 < item.inner_lo || j0 + kKeys > item.inner_hi) {
+                    // keys that the row does not attend
+                    const int lo = k.lo - j0, hi = k.hi - j0;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int x = 0; x < 32; ++x) if (c * 32 + x < lo || c * 32 + x >= hi) s[c][x] = 0xff800000u;
+                    if (with_holes) {
+#pragma unroll
+                        for (int g = 0; g < kKeys / kChunk; ++g) {
+                            const int j = j0 + g * kChunk;
+                            if (j < item.keys.hi && page_of(B, item.b, j >> B.page_shift) < 0)
+#pragma unroll
+                                for (int x = 0; x < kChunk; ++x) s[g / 2][g % 2 * kChunk + x] = 0xff800000u;
+                        }
+                    }
+                }
+                float m[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    m[c] = __uint_as_float(s[c][0]);
+#pragma unroll
+                    for (int x = 1; x < 32; ++x) m[c] = fmaxf(m[c], __uint_as_float(s[c][x]));
+                }
+                const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * rs;
+                if (__any_sync(~0u, top > bar_x)) {
+                    const float old = bar_x - kHeadroom, now = fmaxf(top, old);
+                    float f = 1.f;
+                    if (now > -INFINITY) {
+                        f = exp2_fast(old - now);
+                        off = now - kLift;
+                        bar_x = now + kHeadroom;
+                    }
+                    l *= f;
+                    if (t > 0) {
+#pragma unroll 1
+                        for (int c = 0; c < DP / 16; ++c) {
+                            uint32_t o[16];
+                            tmem_load16(o, o_at + c * 16);
+#pragma unroll
+                            for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+                            tc::tmem_st16(o_at + c * 16, o);
+                        }
+                    }
+                }
+                const unsigned long long rs2 = pair(rs, rs), off2 = pair(-off, -off);
+                unsigned long long sum[2] = {0, 0};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int x = 0; x < 32; x += 2) {
+                        float u, v;
+                        unpair(fma2(pair(__uint_as_float(s[c][x]), __uint_as_float(s[c][x + 1])), rs2, off2), u, v);
+                        u = exp2_fast(u);
+                        v = exp2_fast(v);
+                        sum[x / 2 & 1] = add2(sum[x / 2 & 1], pair(u, v));
+                        w[x / 2] = half2_bits(u, v);
+                    }
+                    tc::tmem_st16(s_at + c * 16, w);          // over scores, all of which have been read
+                }
+                float u, v;
+                unpair(add2(sum[0], sum[1]), u, v);
+                l += u + v;
+                tmem_stored();
+                before_sync();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&bars.p_full[q]);
+            }
+            if (mine && tiles > 0) {
+                wait(&bars.pv_done[q], my_tiles + tiles - 1);
+                if (__any_sync(~0u, failed)) failed = true;
+                after_sync();
+            }
+            asm volatile("bar.sync 1, 384;" ::: "memory");    // the conversion's notes of NaNs
+            if (mine && !failed) {
+                uint32_t nan[4] = {0, 0, 0, 0};
+                const int n = min(*(volatile int*)&nan_count, kNanKeys);
+                for (int i = 0; i < n; ++i) {
+                    const NanPiece* g = p.nans + (long long)blockIdx.x * kNanKeys + i;
+                    const int key = *(volatile const int*)&g->key;
+                    const uint32_t bits = *(volatile const uint16_t*)&g->bits, unit = *(volatile const uint16_t*)&g->unit;
+                    if (key >= k.lo && key < k.hi)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) if (x == int(unit / 2)) nan[x] |= bits << (16 * (unit & 1));
+                }
+                const bool whole = item.c0 == 0 && item.c1 == item.cost, exists = item.m0 + q * kTileRows + r < item.m_end;
+                // A row is a thread's; its values go through shared memory - where the tile's queries were - so that a warp stores
+                // whole lines: 64 bytes of each of its rows at a time, pieces of 16 bytes turned by the row.
+                unsigned char* const turn = smem + L::kQ + q * L::kTile + (warp & 3) * 32 * (DP * 2);
+                const float inv = !whole ? v_unit : (l == 0.f ? 0.f : v_unit / l);
+#pragma unroll
+                for (int c = 0; c < DP / 32; ++c) {
+                    uint32_t o[32];
+                    if (tiles > 0) {
+                        tmem_load32(o, o_at + c * 32);
+                        tmem_loaded(o);
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < 32; ++x) o[x] = 0;
+                    }
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) o[x] = nan[c] >> x & 1 ? 0x7fc00000u : __float_as_uint(__uint_as_float(o[x]) * inv);
+                    if (!whole) {
+                        float* const to = a.parts + ((long long)blockIdx.x * 2 + (item.c0 > 0 ? 0 : 1)) * L::kPart + (q * kTileRows + r) * DP + c * 32;
+                        if (exists)
+#pragma unroll
+                            for (int x = 0; x < 32; x += 4) *reinterpret_cast<uint4*>(to + x) = make_uint4(o[x], o[x + 1], o[x + 2], o[x + 3]);
+                        continue;
+                    }
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) {
+                            const float u = __uint_as_float(o[x * 8 + y * 2]), v = __uint_as_float(o[x * 8 + y * 2 + 1]);
+                            const __nv_bfloat162 z = __floats2bfloat162_rn(u, v);
+                            w[y] = B.dtype == OGLE_F16 ? half2_bits(u, v) : *reinterpret_cast<const uint32_t*>(&z);
+                        }
+                        *reinterpret_cast<uint4*>(turn + lane * (DP * 2) + ((c * 4 + x) ^ (lane & 7)) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+                if (whole) {
+                    __syncwarp();
+                    constexpr int kPieces = DP / 8, kTogether = 32 / kPieces;
+                    const int piece = lane % kPieces;
+#pragma unroll 4
+                    for (int x = 0; x < 32; x += kTogether) {
+                        const int at = x + lane / kPieces, m = item.m0 + q * kTileRows + (warp & 3) * 32 + at;
+                        if (m < item.m_end && piece * 8 < B.dim) {
+                            const uint4 z = *reinterpret_cast<const uint4*>(turn + at * (DP * 2) + (piece ^ (at & 7)) * 16);
+                            const long long y = (item.s.row0 + m / B.group) * a.out_row + (h * B.group + m % B.group) * a.out_head + piece * 8;
+                            *reinterpret_cast<uint4*>(static_cast<unsigned short*>(a.out) + y) = z;
+                        }
+                    }
+                    if (exists && a.lse)
+                        a.lse[(long long)(item.s.row0 + seq_row) * B.q_heads + head] = l == 0.f ? -INFINITY : (bar_x - kHeadroom - kLift + log2f(l)) * 0.6931471805599453f;
+                } else if (exists) {
+                    float* const part = a.parts + ((long long)blockIdx.x * 2 + (item.c0 > 0 ? 0 : 1)) * L::kPart + kItemRows * DP + q * kTileRows + r;
+                    part[0] = bar_x - kHeadroom;
+                    part[kItemRows] = l;
+                }
+            }
+            if (mine) my_tiles += tiles;
+        }
+    } else if (warp < kCopyWarp) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvertRegisters));
+        // a piece is 16 values of a token; eight lanes that store together have two tokens' four pieces: different banks
+        const int piece = lane & 3, row8 = lane >> 2, cw = warp - kConvertWarp;
+        for (bool more = more_items != 0; more; more = end_item()) {
+            begin_item();
             for (int t = 0; t < tiles && !failed; ++t) {
                 const uint32_t st = kv_tiles & 1, use = kv_tiles >> 1;
                 const int j0 = j_first + t * kKeys;
@@ -407,243 +625,109 @@ paged_prompt_kernel(PromptArgs p, const __grid_constant__ CUtensorMap k_map, con
                 }
                 ++kv_tiles;
             }
-        } else if (warp == kProductWarp) {
-            if (tiles > 0 && tc::elect_one()) {
-                constexpr uint32_t kF16 = (1u << 4) | ((uint32_t)(kTileRows >> 4) << 24);     // fp16 x fp16 into fp32, 128 rows
-                constexpr uint32_t kScores = kF16 | ((uint32_t)(kKeys >> 3) << 17);
-                constexpr uint32_t kSums = kF16 | (1u << 16) | ((uint32_t)(DP >> 3) << 17);   // values: elements side by side
-                uint32_t done = kv_tiles;                   // tiles of keys whose products have been asked for
-                const auto scores = [&](int q) {            // S = Q K^T of tile `done`'s keys
-                    const uint64_t qd = tc::umma_desc(base + L::kQ + q * L::kTile), kd = tc::umma_desc(base + L::kK + (done & 1) * L::kTile);
-#pragma unroll
-                    for (int k = 0; k < DP / 16; ++k) {
-                        const uint64_t o = (uint64_t)((k / 4) * (L::kHalf >> 4) + (k % 4) * 2);
-                        product(tmem + q * kKeys, qd + o, kd + o, kScores, k > 0);
-                    }
-                    tc::umma_commit(&bars.s_full[q]);
+            asm volatile("bar.sync 1, 384;" ::: "memory");
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegisters));
+        for (bool more = more_items != 0; more; more = end_item()) {
+            begin_item();
+            const int h = item.h;
+            if (warp == kCopyWarp) {
+                // lane g has the 16 tokens of group g
+                const int nowhere = max(B.n_pages, 1), in_page = (1 << B.page_shift) - 1;
+                const auto look_up = [&](int t, int& page, float& rk, float& rv) {
+                    const int j = j_first + t * kKeys + (lane & 7) * kChunk;
+                    page = nowhere;
+                    rk = rv = 0.f;
+                    if (t >= tiles || j >= item.keys.hi) return;
+                    const int x = page_of(B, item.b, j >> B.page_shift);
+                    if (x < 0) return;
+                    page = x;
+                    const long long o = (long long)x * B.kv_heads + h;
+                    rk = __ldg(B.k_scale + o) / k_unit;
+                    rv = __ldg(B.v_scale + o) / v_unit;
                 };
-                bool ok = wait(&bars.q_full, q_items) && wait(&bars.k_full[done & 1], done >> 1);
-                if (ok) {
-                    after_sync();
-                    for (int q = 0; q < halves; ++q) scores(q);
-                    tc::umma_commit(&bars.k_empty[done & 1]);
+                int page;
+                float rk, rv;
+                look_up(0, page, rk, rv);
+                for (int t = 0; t < tiles && !failed; ++t) {
+                    const int token = (j_first + t * kKeys + (lane & 7) * kChunk) & in_page, now = page;
+                    const float now_k = rk, now_v = rv;
+                    look_up(t + 1, page, rk, rv);
+    #pragma unroll
+                    for (int v = 0; v < 2; ++v) {
+                        uint64_t* const came = v ? &bars.v_came : &bars.k_came;
+                        const bool free = wait(v ? &bars.v_taken : &bars.k_taken, kv_tiles + 1);
+                        if (__any_sync(~0u, !free)) { failed = true; break; }
+                        if (lane < 8) ratio[v][lane] = v ? now_v : now_k;
+                        __syncwarp();
+                        if (lane == 0) tc::mbar_expect_tx(came, L::kBytes);
+                        __syncwarp();
+                        if (lane < 8) copy_box(base + (v ? L::kStageV : L::kStageK) + lane * kChunk * DP, v ? &v_map : &k_map, tc::smem_u32(came), 0, token, h, now);
+                        my_tiles = kv_tiles * 2 + v + 1;                          // copies asked for
+                    }
+                    ++kv_tiles;
                 }
-                for (int t = 0; ok && t < tiles; ++t) {
-                    const uint32_t now = done++;            // values of `now`, keys of `done`
-                    ok = wait(&bars.v_full[now & 1], now >> 1);
-                    for (int q = 0; ok && q < halves; ++q) {
-                        const uint32_t turn = (q ? second_tiles : my_tiles) + t;
-                        ok = wait(&bars.p_full[q], turn);
-                        if (!ok) break;
+            } else if (warp == kProductWarp) {
+                if (tiles > 0 && tc::elect_one()) {
+                    constexpr uint32_t kF16 = (1u << 4) | ((uint32_t)(kTileRows >> 4) << 24);     // fp16 x fp16 into fp32, 128 rows
+                    constexpr uint32_t kScores = kF16 | ((uint32_t)(kKeys >> 3) << 17);
+                    constexpr uint32_t kSums = kF16 | (1u << 16) | ((uint32_t)(DP >> 3) << 17);   // values: elements side by side
+                    uint32_t done = kv_tiles;                   // tiles of keys whose products have been asked for
+                    const auto scores = [&](int q) {            // S = Q K^T of tile `done`'s keys
+                        const uint64_t qd = tc::umma_desc(base + L::kQ + q * L::kTile), kd = tc::umma_desc(base + L::kK + (done & 1) * L::kTile);
+    #pragma unroll
+                        for (int k = 0; k < DP / 16; ++k) {
+                            const uint64_t o = (uint64_t)((k / 4) * (L::kHalf >> 4) + (k % 4) * 2);
+                            product(tmem + q * kKeys, qd + o, kd + o, kScores, k > 0);
+                        }
+                        tc::umma_commit(&bars.s_full[q]);
+                    };
+                    bool ok = wait(&bars.q_full, q_items) && wait(&bars.k_full[done & 1], done >> 1);
+                    if (ok) {
                         after_sync();
-                        const uint32_t vbase = base + L::kV + (now & 1) * L::kTile;
-#pragma unroll
-                        for (int k = 0; k < kKeys / 16; ++k)
-                            product_tmem(tmem + L::kO + q * DP, tmem + q * kKeys + k * 8, desc_mn(vbase + k * 2048, L::kHalf), kSums, t > 0 || k > 0);
-                        tc::umma_commit(&bars.pv_done[q]);
-                        if (t + 1 < tiles) {
-                            if (q == 0) ok = wait(&bars.k_full[done & 1], done >> 1);
-                            ok = ok && wait(&bars.pv_done[q], turn);          // P lies where the next S will
-                            if (ok) {
-                                after_sync();
-                                scores(q);
+                        for (int q = 0; q < halves; ++q) scores(q);
+                        tc::umma_commit(&bars.k_empty[done & 1]);
+                    }
+                    for (int t = 0; ok && t < tiles; ++t) {
+                        const uint32_t now = done++;            // values of `now`, keys of `done`
+                        ok = wait(&bars.v_full[now & 1], now >> 1);
+                        for (int q = 0; ok && q < halves; ++q) {
+                            const uint32_t turn = (q ? second_tiles : my_tiles) + t;
+                            ok = wait(&bars.p_full[q], turn);
+                            if (!ok) break;
+                            after_sync();
+                            const uint32_t vbase = base + L::kV + (now & 1) * L::kTile;
+    #pragma unroll
+                            for (int k = 0; k < kKeys / 16; ++k)
+                                product_tmem(tmem + L::kO + q * DP, tmem + q * kKeys + k * 8, desc_mn(vbase + k * 2048, L::kHalf), kSums, t > 0 || k > 0);
+                            tc::umma_commit(&bars.pv_done[q]);
+                            if (t + 1 < tiles) {
+                                if (q == 0) ok = wait(&bars.k_full[done & 1], done >> 1);
+                                ok = ok && wait(&bars.pv_done[q], turn);          // P lies where the next S will
+                                if (ok) {
+                                    after_sync();
+                                    scores(q);
+                                }
                             }
                         }
-                    }
-                    if (ok) {
-                        tc::umma_commit(&bars.v_empty[now & 1]);
-                        if (t + 1 < tiles) tc::umma_commit(&bars.k_empty[done & 1]);
-                    }
-                }
-                if (!ok) {                                  // products under way end before tensor memory is given back
-                    tc::umma_commit(&bars.drain);
-                    tc::mbar_wait(&bars.drain, 0);
-                }
-            }
-            __syncwarp();
-            kv_tiles += tiles;
-            my_tiles += tiles;
-            if (halves == 2) second_tiles += tiles;
-            if (tiles > 0) ++q_items;
-        } else {
-            const int q = warp / 4, r = tid & 127;           // tile, row of it
-            const bool mine = q < halves;
-            const int row = min(item.m0 + q * kTileRows + r, item.m_end - 1);
-            const bool exists = item.m0 + q * kTileRows + r < item.m_end;
-            const int seq_row = row / B.group, head = h * B.group + row % B.group;
-            const Span k = span_of(item.s, seq_row, seq_row, a.causal, a.window);
-            float rs = 0.f;
-            if (tiles > 0 && mine) {
-                const long long q0 = (item.s.row0 + seq_row) * a.q_row + head * a.q_head;
-                float top = 0.f, f[16];
-                for (int d = 0; d < B.dim; d += 16) {
-                    load16(a.q, q0, d, B.dim, B.dtype, f);
-#pragma unroll
-                    for (int x = 0; x < 16; ++x) top = fmaxf(top, fabsf(f[x]));
-                }
-                const int e = top > 1e-30f && top <= 3e38f ? int(__float_as_uint(top) >> 23) - 126 - 12 : 0;
-                float down = __uint_as_float(uint32_t(127 - e) << 23);
-                rs = a.scale_log2 * __uint_as_float(uint32_t(127 + e) << 23) * k_unit;
-                if (rs < 0.f) { rs = -rs; down = -down; }    // the largest product is then the largest x
-                rs = fmaxf(rs, 1e-37f);                      // scores scaled by 0 are alike, hidden ones are not
-#pragma unroll 1
-                for (int d = 0; d < DP; d += 16) {
-                    load16(a.q, q0, d, B.dim, B.dtype, f);
-                    uint32_t y[8];
-#pragma unroll
-                    for (int x = 0; x < 8; ++x) y[x] = half2_bits(f[2 * x] * down, f[2 * x + 1] * down);
-                    unsigned char* to = smem + L::kQ + q * L::kTile + (d / 64) * L::kHalf + r * 128;
-                    const int c = d % 64 / 8;
-                    *reinterpret_cast<uint4*>(to + (c ^ (r & 7)) * 16) = make_uint4(y[0], y[1], y[2], y[3]);
-                    *reinterpret_cast<uint4*>(to + ((c + 1) ^ (r & 7)) * 16) = make_uint4(y[4], y[5], y[6], y[7]);
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            }
-            __syncwarp();
-            if (tiles > 0 && lane == 0) tc::mbar_arrive(&bars.q_full);
-
-            const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_at = tmem + lanes + q * kKeys, o_at = tmem + lanes + L::kO + q * DP;
-            float off = 0.f, bar_x = -INFINITY, l = 0.f;
-            for (int t = 0; mine && t < tiles; ++t) {
-                wait(&bars.s_full[q], my_tiles + t);
-                if (__any_sync(~0u, failed)) { failed = true; break; }
-                after_sync();
-                const int j0 = j_first + t * kKeys;
-                const bool edge = with_holes || j0 < item.inner_lo || j0 + kKeys > item.inner_hi;
-                // columns of 32 keys that the row does not attend become minus infinity
-                const auto hide = [&](uint32_t (&s)[32], int c) {
-                    const int lo = k.lo - j0 - c * 32, hi = k.hi - j0 - c * 32;
-#pragma unroll
-                    for (int x = 0; x < 32; ++x) if (x < lo || x >= hi) s[x] = 0xff800000u;
-                    if (with_holes) {
-#pragma unroll
-                        for (int g = 0; g < 2; ++g) {
-                            const int j = j0 + c * 32 + g * 16;
-                            if (j < item.keys.hi && page_of(B, item.b, j >> B.page_shift) < 0)
-#pragma unroll
-                                for (int x = 0; x < 16; ++x) s[g * 16 + x] = 0xff800000u;
+                        if (ok) {
+                            tc::umma_commit(&bars.v_empty[now & 1]);
+                            if (t + 1 < tiles) tc::umma_commit(&bars.k_empty[done & 1]);
                         }
                     }
-                };
-                float top = -INFINITY;
-#pragma unroll
-                for (int c = 0; c < kKeys / 32; ++c) {
-                    uint32_t s[32];
-                    tmem_load32(s, s_at + c * 32);
-                    tmem_loaded(s);
-                    if (edge) hide(s, c);
-                    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                    for (int x = 0; x < 32; ++x) m[x & 3] = fmaxf(m[x & 3], __uint_as_float(s[x]));
-                    top = fmaxf(top, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
-                }
-                top *= rs;
-                if (__any_sync(~0u, top > bar_x)) {
-                    const float old = bar_x - kHeadroom, now = fmaxf(top, old);
-                    float f = 1.f;
-                    if (now > -INFINITY) {
-                        f = exp2_fast(old - now);
-                        off = now - kLift;
-                        bar_x = now + kHeadroom;
-                    }
-                    l *= f;
-                    if (t > 0) {
-#pragma unroll 1
-                        for (int c = 0; c < DP / 32; ++c) {
-                            uint32_t o[32];
-                            tmem_load32(o, o_at + c * 32);
-                            tmem_loaded(o);
-#pragma unroll
-                            for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
-                            tc::tmem_st16(o_at + c * 32, reinterpret_cast<const uint32_t(&)[16]>(o[0]));
-                            tc::tmem_st16(o_at + c * 32 + 16, reinterpret_cast<const uint32_t(&)[16]>(o[16]));
-                        }
+                    if (!ok) {                                  // products under way end before tensor memory is given back
+                        tc::umma_commit(&bars.drain);
+                        tc::mbar_wait(&bars.drain, 0);
                     }
                 }
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int c = 0; c < kKeys / 32; ++c) {
-                    uint32_t s[32], w[16];
-                    tmem_load32(s, s_at + c * 32);
-                    tmem_loaded(s);
-                    if (edge) hide(s, c);
-#pragma unroll
-                    for (int x = 0; x < 32; x += 2) {
-                        const float u = exp2_fast(fmaf(__uint_as_float(s[x]), rs, -off)), v = exp2_fast(fmaf(__uint_as_float(s[x + 1]), rs, -off));
-                        sum[x & 2] += u;
-                        sum[(x & 2) + 1] += v;
-                        w[x / 2] = half2_bits(u, v);
-                    }
-                    tc::tmem_st16(s_at + c * 16, w);          // over columns that have been read
-                }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                tmem_stored();
-                before_sync();
                 __syncwarp();
-                if (lane == 0) tc::mbar_arrive(&bars.p_full[q]);
+                kv_tiles += tiles;
+                my_tiles += tiles;
+                if (halves == 2) second_tiles += tiles;
+                if (tiles > 0) ++q_items;
             }
-            if (mine && tiles > 0) {
-                wait(&bars.pv_done[q], my_tiles + tiles - 1);
-                if (__any_sync(~0u, failed)) failed = true;
-                after_sync();
-            }
-            asm volatile("bar.sync 1, 384;" ::: "memory");    // the conversion's notes of NaNs
-            const bool whole = item.c0 == 0 && item.c1 == item.cost;
-            if (mine && !failed) {
-                uint32_t nan[4] = {0, 0, 0, 0};
-                const int n = min(*(volatile int*)&nan_count, kNanKeys);
-                for (int i = 0; i < n; ++i) {
-                    const NanPiece* g = p.nans + (long long)blockIdx.x * kNanKeys + i;
-                    const int key = *(volatile const int*)&g->key;
-                    const uint32_t bits = *(volatile const uint16_t*)&g->bits, unit = *(volatile const uint16_t*)&g->unit;
-                    if (key >= k.lo && key < k.hi)
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) if (x == int(unit / 2)) nan[x] |= bits << (16 * (unit & 1));
-                }
-                float* const part = a.parts + ((long long)blockIdx.x * 2 + (item.c0 > 0 ? 0 : 1)) * L::kPart;
-                const int part_row = q * kTileRows + r;
-                const float m = bar_x - kHeadroom;
-#pragma unroll
-                for (int c = 0; c < DP / 32; ++c) {
-                    uint32_t o[32];
-                    if (tiles > 0) {
-                        tmem_load32(o, o_at + c * 32);
-                        tmem_loaded(o);
-                    } else {
-#pragma unroll
-                        for (int x = 0; x < 32; ++x) o[x] = 0;
-                    }
-                    if (!exists) continue;
-#pragma unroll
-                    for (int x = 0; x < 32; x += 4) {
-                        float4 v;
-                        v.x = nan[c] >> x & 1 ? NAN : __uint_as_float(o[x]) * v_unit;
-                        v.y = nan[c] >> (x + 1) & 1 ? NAN : __uint_as_float(o[x + 1]) * v_unit;
-                        v.z = nan[c] >> (x + 2) & 1 ? NAN : __uint_as_float(o[x + 2]) * v_unit;
-                        v.w = nan[c] >> (x + 3) & 1 ? NAN : __uint_as_float(o[x + 3]) * v_unit;
-                        if (whole) store_row(a, item.s.row0 + seq_row, head, c * 32 + x, v, m, l);
-                        else *reinterpret_cast<float4*>(part + part_row * DP + c * 32 + x) = v;
-                    }
-                }
-                if (!whole && exists) {
-                    part[kItemRows * DP + part_row] = m;
-                    part[kItemRows * DP + kItemRows + part_row] = l;
-                }
-                before_sync();
-            }
-            if (mine) my_tiles += tiles;
         }
-        if (warp >= kConvertWarp && warp < kCopyWarp) asm volatile("bar.sync 1, 384;" ::: "memory");
-        before_sync();
-        __syncthreads();
-        after_sync();
-        if (gave_up) break;
-        if (tid == 0) {
-            top_scale[0] = top_scale[1] = 0;
-            holes = nan_count = 0;
-            more_items = next_item(p, walk, item);
-        }
-        __syncthreads();
     }
     // a copy that nobody has waited for lands before the block ends
     if (warp == kCopyWarp && gave_up && my_tiles > 0) {
