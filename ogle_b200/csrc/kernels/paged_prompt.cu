@@ -9,8 +9,10 @@
 //   one thread    issues the products: S = Q K^T per tile, O += P V per tile, P taken from tensor memory
 //   2 x 4 warps   a row a thread: maximum, weights 2^(x - off), their sum; P in fp16 over S; O rescaled when a row's maximum
 //                 has grown by more than 2^8
-// While one tile of rows is being weighted, the other's products run. P lies over S in tensor memory (2 x 128 columns for S,
-// 2 x DP for O), so the next S of a tile is asked for once its P V is through.
+// A tile of keys is taken in two steps of 64. A tile of rows has two S of 64 columns in tensor memory (2 x 2 x 64, and 2 x DP
+// for O), so that the products of one step run while another is being weighted; P lies over its S, which is written again
+// once its P V is through. (With one S of 128 columns, scores, weights and sums of a tile came one after the other: 5000 cycles
+// a tile of keys where the products take 2048.)
 //
 // Work: items (sequence, tile of 256 rows, kv head) laid end to end by their tiles of keys, cut into one range a block; parts
 // of items that were cut go to the workspace and are joined as in the form for few rows (paged_attention.cu). The ranges'
@@ -23,6 +25,7 @@ namespace {
 using namespace paged;
 
 constexpr int kKeys = 128;                       // of a tile
+constexpr int kStep = 64;                        // of a step: half a tile
 constexpr int kTileRows = 128, kItemRows = 2 * kTileRows;
 constexpr int kItemCost = 3;                     // tiles that an item's beginning and end take as long as
 constexpr int kThreads = 16 * 32;                // 8 warps of rows, 4 of conversion, copies, products, and two that fill up their group
@@ -199,13 +202,6 @@ __device__ __forceinline__ void tmem_load16(uint32_t (&r)[16], uint32_t addr) {
           "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(addr) : "memory");
 }
-// Four loads of 32 columns and one wait.
-__device__ __forceinline__ void tmem_load128(uint32_t (&s)[4][32], uint32_t addr) {
-#pragma unroll
-    for (int c = 0; c < 4; ++c) tmem_load32(s[c], addr + c * 32);
-#pragma unroll
-    for (int c = 0; c < 4; ++c) tmem_loaded(s[c]);
-}
 __device__ __forceinline__ unsigned long long pair(float lo, float hi) {
     unsigned long long r;
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
@@ -254,7 +250,7 @@ __device__ __forceinline__ int stage_at(int r, int unit) {
 struct Bars {
     uint64_t k_came, k_taken, v_came, v_taken;   // the copied tiles
     uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
-    uint64_t q_full, s_full[2], p_full[2], pv_done[2], drain;
+    uint64_t q_full, s_full[2][2], p_full[2][2], pv_done[2][2], drain;   // [tile of rows][step & 1]
 };
 
 template <int DP>
@@ -281,7 +277,9 @@ paged_prompt_kernel(PromptArgs p, const __grid_constant__ CUtensorMap k_map, con
         for (int i = 0; i < 2; ++i) {
             tc::mbar_init(&bars.k_full[i], 4); tc::mbar_init(&bars.v_full[i], 4);
             tc::mbar_init(&bars.k_empty[i], 1); tc::mbar_init(&bars.v_empty[i], 1);
-            tc::mbar_init(&bars.s_full[i], 1); tc::mbar_init(&bars.p_full[i], 4); tc::mbar_init(&bars.pv_done[i], 1);
+            for (int j = 0; j < 2; ++j) {
+                tc::mbar_init(&bars.s_full[i][j], 1); tc::mbar_init(&bars.p_full[i][j], 4); tc::mbar_init(&bars.pv_done[i][j], 1);
+            }
         }
         tc::mbar_init(&bars.q_full, 8);
         tc::mbar_init(&bars.drain, 1);
@@ -310,7 +308,7 @@ paged_prompt_kernel(PromptArgs p, const __grid_constant__ CUtensorMap k_map, con
     const uint32_t limit = a.spin_limit;
     volatile int* const abort = &gave_up;
     // tiles that this thread's role has been through, whatever item they were of
-    uint32_t kv_tiles = 0, q_items = 0, my_tiles = 0, second_tiles = 0;
+    uint32_t kv_tiles = 0, q_items = 0, copies = 0, my_steps = 0, second_steps = 0;
     bool failed = false;
     const auto wait = [&](uint64_t* bar, uint32_t parity) {
         if (!failed && !tc::wait_turn(bar, parity & 1, abort, limit)) {
@@ -367,7 +365,7 @@ paged_prompt_kernel(PromptArgs p, const __grid_constant__ CUtensorMap k_map, con
     if (warp < kConvertWarp) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRowRegisters));
         const int q = warp / 4, r = tid & 127;           // tile, row of it
-        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_at = tmem + lanes + q * kKeys, o_at = tmem + lanes + L::kO + q * DP;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_at = tmem + lanes + q * 2 * kStep, o_at = tmem + lanes + L::kO + q * DP;
         for (bool more = more_items != 0; more; more = end_item()) {
             begin_item();
             const int h = item.h;
@@ -376,29 +374,46 @@ paged_prompt_kernel(PromptArgs p, const __grid_constant__ CUtensorMap k_map, con
             const int seq_row = row / B.group, head = h * B.group + row % B.group;
             const Span k = span_of(item.s, seq_row, seq_row, a.causal, a.window);
             if (tiles > 0 && mine) {
-                // queries of the warp's 32 rows, 16 values a lane: rows side by side are read together
-                constexpr int kLanes = DP / 16, kTogether = 32 / kLanes, kRounds = 32 / kTogether;
+                // queries of the warp's 32 rows, 16 values a lane: rows side by side are read together, half of them before the first is used
+                constexpr int kLanes = DP / 16, kTogether = 32 / kLanes, kRounds = 32 / kTogether, kAtOnce = kRounds / 2;
                 const int d = lane % kLanes * 16;
+                const long long mine_at = (item.s.row0 + seq_row) * a.q_row + head * a.q_head;
                 const bool back = a.scale_log2 < 0.f;        // the largest product is then the largest x
-#pragma unroll 2
-                for (int x = 0; x < kRounds; ++x) {
-                    const int at = (warp & 3) * 32 + x * kTogether + lane / kLanes, m = min(item.m0 + q * kTileRows + at, item.m_end - 1);
-                    float f[16], top = 0.f;
-                    load16(a.q, (item.s.row0 + m / B.group) * a.q_row + (h * B.group + m % B.group) * a.q_head, d, B.dim, B.dtype, f);
+#pragma unroll 1
+                for (int x0 = 0; x0 < kRounds; x0 += kAtOnce) {
+                    uint4 raw[kAtOnce][2];
 #pragma unroll
-                    for (int y = 0; y < 16; ++y) top = fmaxf(top, fabsf(f[y]));
+                    for (int x = 0; x < kAtOnce; ++x) {
+                        const long long from = __shfl_sync(~0u, mine_at, (x0 + x) * kTogether + lane / kLanes);
+                        const uint4* g = reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(a.q) + from + d);
+                        raw[x][0] = raw[x][1] = make_uint4(0, 0, 0, 0);
+                        if (d < B.dim) { raw[x][0] = g[0]; raw[x][1] = g[1]; }
+                    }
 #pragma unroll
-                    for (int y = 1; y < kLanes; y *= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, y));
-                    const int e = top > 1e-30f && top <= 3e38f ? int(__float_as_uint(top) >> 23) - 126 - 12 : 0;
-                    const float down = __uint_as_float(uint32_t(127 - e) << 23 | (back ? 0x80000000u : 0u));
-                    if (lane % kLanes == 0) row_scale[q][at] = __uint_as_float(uint32_t(127 + e) << 23);
-                    uint32_t y[8];
+                    for (int x = 0; x < kAtOnce; ++x) {
+                        const int at = (warp & 3) * 32 + (x0 + x) * kTogether + lane / kLanes;
+                        const uint32_t* w = reinterpret_cast<const uint32_t*>(raw[x]);
+                        float f[16], top = 0.f;
 #pragma unroll
-                    for (int z = 0; z < 8; ++z) y[z] = half2_bits(f[2 * z] * down, f[2 * z + 1] * down);
-                    unsigned char* to = smem + L::kQ + q * L::kTile + (d / 64) * L::kHalf + at * 128;
-                    const int c = d % 64 / 8;
-                    *reinterpret_cast<uint4*>(to + (c ^ (at & 7)) * 16) = make_uint4(y[0], y[1], y[2], y[3]);
-                    *reinterpret_cast<uint4*>(to + ((c + 1) ^ (at & 7)) * 16) = make_uint4(y[4], y[5], y[6], y[7]);
+                        for (int y = 0; y < 8; ++y) {
+                            const float2 g = B.dtype == OGLE_F16 ? __half22float2(*reinterpret_cast<const __half2*>(w + y)) : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(w + y));
+                            f[2 * y] = g.x;
+                            f[2 * y + 1] = g.y;
+                            top = fmaxf(top, fmaxf(fabsf(g.x), fabsf(g.y)));
+                        }
+#pragma unroll
+                        for (int y = 1; y < kLanes; y *= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, y));
+                        const int e = top > 1e-30f && top <= 3e38f ? int(__float_as_uint(top) >> 23) - 126 - 12 : 0;
+                        const float down = __uint_as_float(uint32_t(127 - e) << 23 | (back ? 0x80000000u : 0u));
+                        if (lane % kLanes == 0) row_scale[q][at] = __uint_as_float(uint32_t(127 + e) << 23);
+                        uint32_t y[8];
+#pragma unroll
+                        for (int z = 0; z < 8; ++z) y[z] = half2_bits(f[2 * z] * down, f[2 * z + 1] * down);
+                        unsigned char* to = smem + L::kQ + q * L::kTile + (d / 64) * L::kHalf + at * 128;
+                        const int c = d % 64 / 8;
+                        *reinterpret_cast<uint4*>(to + (c ^ (at & 7)) * 16) = make_uint4(y[0], y[1], y[2], y[3]);
+                        *reinterpret_cast<uint4*>(to + ((c + 1) ^ (at & 7)) * 16) = make_uint4(y[4], y[5], y[6], y[7]);
+                    }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             }
@@ -408,23 +423,27 @@ paged_prompt_kernel(PromptArgs p, const __grid_constant__ CUtensorMap k_map, con
             const float rs = mine && tiles > 0 ? fmaxf(fabsf(a.scale_log2) * row_scale[q][r] * k_unit, 1e-37f) : 0.f;
 
             float off = 0.f, bar_x = -INFINITY, l = 0.f;
-            for (int t = 0; mine && t < tiles; ++t) {
-                wait(&bars.s_full[q], my_tiles + t);
+            for (int u = 0; mine && u < 2 * tiles; ++u) {
+                const uint32_t turn = my_steps + u, sp_at = s_at + (turn & 1) * kStep;
+                wait(&bars.s_full[q][turn & 1], turn >> 1);
                 if (__any_sync(~0u, failed)) { failed = true; break; }
                 after_sync();
-                const int j0 = j_first + t * kKeys;
-                uint32_t s[4][32];
-                tmem_load128(s, s_at);
-                if (with_holes || j0 < item.inner_lo || j0 + kKeys > item.inner_hi) {
+                const int j0 = j_first + u * kStep;
+                uint32_t s[2][32];
+                tmem_load32(s[0], sp_at);
+                tmem_load32(s[1], sp_at + 32);
+                tmem_loaded(s[0]);
+                tmem_loaded(s[1]);
+                if (with_holes || j0 < item.inner_lo || j0 + kStep > item.inner_hi) {
                     // keys that the row does not attend
                     const int lo = k.lo - j0, hi = k.hi - j0;
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
+                    for (int c = 0; c < 2; ++c)
 #pragma unroll
                         for (int x = 0; x < 32; ++x) if (c * 32 + x < lo || c * 32 + x >= hi) s[c][x] = 0xff800000u;
                     if (with_holes) {
 #pragma unroll
-                        for (int g = 0; g < kKeys / kChunk; ++g) {
+                        for (int g = 0; g < kStep / kChunk; ++g) {
                             const int j = j0 + g * kChunk;
                             if (j < item.keys.hi && page_of(B, item.b, j >> B.page_shift) < 0)
 #pragma unroll
@@ -435,9 +454,9 @@ paged_prompt_kernel(PromptArgs p, const __grid_constant__ CUtensorMap k_map, con
                 float m[4];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    m[c] = __uint_as_float(s[c][0]);
+                    m[c] = __uint_as_float(s[c / 2][c % 2 * 16]);
 #pragma unroll
-                    for (int x = 1; x < 32; ++x) m[c] = fmaxf(m[c], __uint_as_float(s[c][x]));
+                    for (int x = 1; x < 16; ++x) m[c] = fmaxf(m[c], __uint_as_float(s[c / 2][c % 2 * 16 + x]));
                 }
                 const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * rs;
                 if (__any_sync(~0u, top > bar_x)) {
@@ -449,7 +468,10 @@ paged_prompt_kernel(PromptArgs p, const __grid_constant__ CUtensorMap k_map, con
                         bar_x = now + kHeadroom;
                     }
                     l *= f;
-                    if (t > 0) {
+                    if (u > 0) {
+                        wait(&bars.pv_done[q][(turn - 1) & 1], (turn - 1) >> 1);
+                        if (__any_sync(~0u, failed)) { failed = true; break; }
+                        after_sync();
 #pragma unroll 1
                         for (int c = 0; c < DP / 16; ++c) {
                             uint32_t o[16];
@@ -463,29 +485,30 @@ paged_prompt_kernel(PromptArgs p, const __grid_constant__ CUtensorMap k_map, con
                 const unsigned long long rs2 = pair(rs, rs), off2 = pair(-off, -off);
                 unsigned long long sum[2] = {0, 0};
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
+                for (int c = 0; c < 2; ++c) {
                     uint32_t w[16];
 #pragma unroll
                     for (int x = 0; x < 32; x += 2) {
-                        float u, v;
-                        unpair(fma2(pair(__uint_as_float(s[c][x]), __uint_as_float(s[c][x + 1])), rs2, off2), u, v);
-                        u = exp2_fast(u);
-                        v = exp2_fast(v);
-                        sum[x / 2 & 1] = add2(sum[x / 2 & 1], pair(u, v));
-                        w[x / 2] = half2_bits(u, v);
+                        float e, f;
+                        unpair(fma2(pair(__uint_as_float(s[c][x]), __uint_as_float(s[c][x + 1])), rs2, off2), e, f);
+                        e = exp2_fast(e);
+                        f = exp2_fast(f);
+                        sum[x / 2 & 1] = add2(sum[x / 2 & 1], pair(e, f));
+                        w[x / 2] = half2_bits(e, f);
                     }
-                    tc::tmem_st16(s_at + c * 16, w);          // over scores, all of which have been read
+                    tc::tmem_st16(sp_at + c * 16, w);          // over scores, all of which have been read
                 }
-                float u, v;
-                unpair(add2(sum[0], sum[1]), u, v);
-                l += u + v;
+                float e, f;
+                unpair(add2(sum[0], sum[1]), e, f);
+                l += e + f;
                 tmem_stored();
                 before_sync();
                 __syncwarp();
-                if (lane == 0) tc::mbar_arrive(&bars.p_full[q]);
+                if (lane == 0) tc::mbar_arrive(&bars.p_full[q][turn & 1]);
             }
             if (mine && tiles > 0) {
-                wait(&bars.pv_done[q], my_tiles + tiles - 1);
+                const uint32_t turn = my_steps + 2 * tiles - 1;
+                wait(&bars.pv_done[q][turn & 1], turn >> 1);
                 if (__any_sync(~0u, failed)) failed = true;
                 after_sync();
             }
@@ -540,15 +563,14 @@ paged_prompt_kernel(PromptArgs p, const __grid_constant__ CUtensorMap k_map, con
                 if (whole) {
                     __syncwarp();
                     constexpr int kPieces = DP / 8, kTogether = 32 / kPieces;
-                    const int piece = lane % kPieces;
+                    const int piece = lane % kPieces, n_rows = item.m_end - item.m0 - q * kTileRows - (warp & 3) * 32;
+                    const long long mine_at = (item.s.row0 + seq_row) * a.out_row + head * a.out_head;
 #pragma unroll 4
                     for (int x = 0; x < 32; x += kTogether) {
-                        const int at = x + lane / kPieces, m = item.m0 + q * kTileRows + (warp & 3) * 32 + at;
-                        if (m < item.m_end && piece * 8 < B.dim) {
-                            const uint4 z = *reinterpret_cast<const uint4*>(turn + at * (DP * 2) + (piece ^ (at & 7)) * 16);
-                            const long long y = (item.s.row0 + m / B.group) * a.out_row + (h * B.group + m % B.group) * a.out_head + piece * 8;
-                            *reinterpret_cast<uint4*>(static_cast<unsigned short*>(a.out) + y) = z;
-                        }
+                        const int at = x + lane / kPieces;
+                        const long long to = __shfl_sync(~0u, mine_at, at);
+                        const uint4 z = *reinterpret_cast<const uint4*>(turn + at * (DP * 2) + (piece ^ (at & 7)) * 16);
+                        if (at < n_rows && piece * 8 < B.dim) *reinterpret_cast<uint4*>(static_cast<unsigned short*>(a.out) + to + piece * 8) = z;
                     }
                     if (exists && a.lse)
                         a.lse[(long long)(item.s.row0 + seq_row) * B.q_heads + head] = l == 0.f ? -INFINITY : (bar_x - kHeadroom - kLift + log2f(l)) * 0.6931471805599453f;
@@ -558,7 +580,7 @@ paged_prompt_kernel(PromptArgs p, const __grid_constant__ CUtensorMap k_map, con
                     part[kItemRows] = l;
                 }
             }
-            if (mine) my_tiles += tiles;
+            if (mine) my_steps += 2 * tiles;
         }
     } else if (warp < kCopyWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvertRegisters));
@@ -664,57 +686,59 @@ paged_prompt_kernel(PromptArgs p, const __grid_constant__ CUtensorMap k_map, con
                         if (lane == 0) tc::mbar_expect_tx(came, L::kBytes);
                         __syncwarp();
                         if (lane < 8) copy_box(base + (v ? L::kStageV : L::kStageK) + lane * kChunk * DP, v ? &v_map : &k_map, tc::smem_u32(came), 0, token, h, now);
-                        my_tiles = kv_tiles * 2 + v + 1;                          // copies asked for
+                        copies = kv_tiles * 2 + v + 1;
                     }
                     ++kv_tiles;
                 }
             } else if (warp == kProductWarp) {
                 if (tiles > 0 && tc::elect_one()) {
                     constexpr uint32_t kF16 = (1u << 4) | ((uint32_t)(kTileRows >> 4) << 24);     // fp16 x fp16 into fp32, 128 rows
-                    constexpr uint32_t kScores = kF16 | ((uint32_t)(kKeys >> 3) << 17);
+                    constexpr uint32_t kScores = kF16 | ((uint32_t)(kStep >> 3) << 17);
                     constexpr uint32_t kSums = kF16 | (1u << 16) | ((uint32_t)(DP >> 3) << 17);   // values: elements side by side
-                    uint32_t done = kv_tiles;                   // tiles of keys whose products have been asked for
-                    const auto scores = [&](int q) {            // S = Q K^T of tile `done`'s keys
-                        const uint64_t qd = tc::umma_desc(base + L::kQ + q * L::kTile), kd = tc::umma_desc(base + L::kK + (done & 1) * L::kTile);
-    #pragma unroll
+                    const int steps = 2 * tiles;
+                    const auto turn_of = [&](int q, int u) { return (q ? second_steps : my_steps) + u; };
+                    const auto scores = [&](int q, int u) {     // S = Q K^T of step u
+                        const uint32_t turn = turn_of(q, u), tile = kv_tiles + u / 2;
+                        const uint64_t qd = tc::umma_desc(base + L::kQ + q * L::kTile), kd = tc::umma_desc(base + L::kK + (tile & 1) * L::kTile + (u & 1) * kStep * 128);
+#pragma unroll
                         for (int k = 0; k < DP / 16; ++k) {
                             const uint64_t o = (uint64_t)((k / 4) * (L::kHalf >> 4) + (k % 4) * 2);
-                            product(tmem + q * kKeys, qd + o, kd + o, kScores, k > 0);
+                            product(tmem + (q * 2 + (turn & 1)) * kStep, qd + o, kd + o, kScores, k > 0);
                         }
-                        tc::umma_commit(&bars.s_full[q]);
+                        tc::umma_commit(&bars.s_full[q][turn & 1]);
                     };
-                    bool ok = wait(&bars.q_full, q_items) && wait(&bars.k_full[done & 1], done >> 1);
+                    bool ok = wait(&bars.q_full, q_items) && wait(&bars.k_full[kv_tiles & 1], kv_tiles >> 1);
                     if (ok) {
                         after_sync();
-                        for (int q = 0; q < halves; ++q) scores(q);
-                        tc::umma_commit(&bars.k_empty[done & 1]);
+                        for (int u = 0; u < 2; ++u)
+                            for (int q = 0; q < halves; ++q) scores(q, u);
+                        tc::umma_commit(&bars.k_empty[kv_tiles & 1]);
                     }
-                    for (int t = 0; ok && t < tiles; ++t) {
-                        const uint32_t now = done++;            // values of `now`, keys of `done`
-                        ok = wait(&bars.v_full[now & 1], now >> 1);
+                    for (int u = 0; ok && u < steps; ++u) {
+                        const uint32_t now = kv_tiles + u / 2;      // tile of the step's values; the keys asked for are of the next
+                        if ((u & 1) == 0) ok = wait(&bars.v_full[now & 1], now >> 1);
+                        const uint32_t vbase = base + L::kV + (now & 1) * L::kTile + (u & 1) * kStep * 128;
                         for (int q = 0; ok && q < halves; ++q) {
-                            const uint32_t turn = (q ? second_tiles : my_tiles) + t;
-                            ok = wait(&bars.p_full[q], turn);
+                            const uint32_t turn = turn_of(q, u);
+                            ok = wait(&bars.p_full[q][turn & 1], turn >> 1);
                             if (!ok) break;
                             after_sync();
-                            const uint32_t vbase = base + L::kV + (now & 1) * L::kTile;
-    #pragma unroll
-                            for (int k = 0; k < kKeys / 16; ++k)
-                                product_tmem(tmem + L::kO + q * DP, tmem + q * kKeys + k * 8, desc_mn(vbase + k * 2048, L::kHalf), kSums, t > 0 || k > 0);
-                            tc::umma_commit(&bars.pv_done[q]);
-                            if (t + 1 < tiles) {
-                                if (q == 0) ok = wait(&bars.k_full[done & 1], done >> 1);
-                                ok = ok && wait(&bars.pv_done[q], turn);          // P lies where the next S will
-                                if (ok) {
-                                    after_sync();
-                                    scores(q);
-                                }
-                            }
+#pragma unroll
+                            for (int k = 0; k < kStep / 16; ++k)
+                                product_tmem(tmem + L::kO + q * DP, tmem + (q * 2 + (turn & 1)) * kStep + k * 8, desc_mn(vbase + k * 2048, L::kHalf), kSums, u > 0 || k > 0);
+                            tc::umma_commit(&bars.pv_done[q][turn & 1]);
                         }
-                        if (ok) {
-                            tc::umma_commit(&bars.v_empty[now & 1]);
-                            if (t + 1 < tiles) tc::umma_commit(&bars.k_empty[done & 1]);
+                        if (ok && (u & 1)) tc::umma_commit(&bars.v_empty[now & 1]);
+                        if (!ok || u + 2 >= steps) continue;
+                        if ((u & 1) == 0) ok = wait(&bars.k_full[(now + 1) & 1], (now + 1) >> 1);
+                        for (int q = 0; ok && q < halves; ++q) {
+                            const uint32_t turn = turn_of(q, u);
+                            ok = wait(&bars.pv_done[q][turn & 1], turn >> 1);     // P lies where the S will
+                            if (!ok) break;
+                            after_sync();
+                            scores(q, u + 2);
                         }
+                        if (ok && (u & 1)) tc::umma_commit(&bars.k_empty[(now + 1) & 1]);
                     }
                     if (!ok) {                                  // products under way end before tensor memory is given back
                         tc::umma_commit(&bars.drain);
@@ -723,15 +747,15 @@ paged_prompt_kernel(PromptArgs p, const __grid_constant__ CUtensorMap k_map, con
                 }
                 __syncwarp();
                 kv_tiles += tiles;
-                my_tiles += tiles;
-                if (halves == 2) second_tiles += tiles;
+                my_steps += 2 * tiles;
+                if (halves == 2) second_steps += 2 * tiles;
                 if (tiles > 0) ++q_items;
             }
         }
     }
     // a copy that nobody has waited for lands before the block ends
-    if (warp == kCopyWarp && gave_up && my_tiles > 0) {
-        const uint32_t last = my_tiles - 1;                    // copy `last`: keys and values in turn
+    if (warp == kCopyWarp && gave_up && copies > 0) {
+        const uint32_t last = copies - 1;                    // copy `last`: keys and values in turn
         tc::mbar_wait(last & 1 ? &bars.v_came : &bars.k_came, (last >> 1) & 1);
         if (last > 0) tc::mbar_wait(last & 1 ? &bars.k_came : &bars.v_came, ((last - 1) >> 1) & 1);
     }
