@@ -232,13 +232,36 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t next) {
     d |= (uint64_t)2 << 61;
     return d;
 }
-__device__ __forceinline__ void product(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+// The four products of 64 elements of the reduction, issued from one block of instructions: the descriptors of the later ones
+// are sums with constants, and the issuing thread does nothing in between. Queries by keys: 32 bytes on for each.
+__device__ __forceinline__ void products_scores(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.eq.b32 q, 0, 0;\n\t"
+        "add.s64 a1, %1, 2;\n\tadd.s64 b1, %2, 2;\n\t"
+        "add.s64 a2, %1, 4;\n\tadd.s64 b2, %2, 4;\n\t"
+        "add.s64 a3, %1, 6;\n\tadd.s64 b3, %2, 6;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, q;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, q;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, q;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
-__device__ __forceinline__ void product_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+// Weights (in tensor memory, 8 columns for 16 keys) by values: 16 tokens, 2048 bytes, on for each.
+__device__ __forceinline__ void products_sums(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b32 a1, a2, a3;\n\t.reg .b64 b1, b2, b3;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.eq.b32 q, 0, 0;\n\t"
+        "add.u32 a1, %1, 8;\n\tadd.s64 b1, %2, 128;\n\t"
+        "add.u32 a2, %1, 16;\n\tadd.s64 b2, %2, 256;\n\t"
+        "add.u32 a3, %1, 24;\n\tadd.s64 b3, %2, 384;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, q;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, q;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, q;\n\t}"
+        ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
 
 // Where 16 bytes, `unit` of row r, of the copied e4m3 tile lie: boxes of 16 rows, as the copies' swizzle puts them.
@@ -701,10 +724,8 @@ paged_prompt_kernel(PromptArgs p, const __grid_constant__ CUtensorMap k_map, con
                         const uint32_t turn = turn_of(q, u), tile = kv_tiles + u / 2;
                         const uint64_t qd = tc::umma_desc(base + L::kQ + q * L::kTile), kd = tc::umma_desc(base + L::kK + (tile & 1) * L::kTile + (u & 1) * kStep * 128);
 #pragma unroll
-                        for (int k = 0; k < DP / 16; ++k) {
-                            const uint64_t o = (uint64_t)((k / 4) * (L::kHalf >> 4) + (k % 4) * 2);
-                            product(tmem + (q * 2 + (turn & 1)) * kStep, qd + o, kd + o, kScores, k > 0);
-                        }
+                        for (int k = 0; k < DP / 64; ++k)
+                            products_scores(tmem + (q * 2 + (turn & 1)) * kStep, qd + k * (L::kHalf >> 4), kd + k * (L::kHalf >> 4), kScores, k);
                         tc::umma_commit(&bars.s_full[q][turn & 1]);
                     };
                     bool ok = wait(&bars.q_full, q_items) && wait(&bars.k_full[kv_tiles & 1], kv_tiles >> 1);
@@ -723,9 +744,7 @@ paged_prompt_kernel(PromptArgs p, const __grid_constant__ CUtensorMap k_map, con
                             ok = wait(&bars.p_full[q][turn & 1], turn >> 1);
                             if (!ok) break;
                             after_sync();
-#pragma unroll
-                            for (int k = 0; k < kStep / 16; ++k)
-                                product_tmem(tmem + L::kO + q * DP, tmem + (q * 2 + (turn & 1)) * kStep + k * 8, desc_mn(vbase + k * 2048, L::kHalf), kSums, u > 0 || k > 0);
+                            products_sums(tmem + L::kO + q * DP, tmem + (q * 2 + (turn & 1)) * kStep, desc_mn(vbase, L::kHalf), kSums, u);
                             tc::umma_commit(&bars.pv_done[q][turn & 1]);
                         }
                         if (ok && (u & 1)) tc::umma_commit(&bars.v_empty[now & 1]);
