@@ -564,11 +564,18 @@ paged_prompt_kernel(PromptArgs p, const __grid_constant__ CUtensorMap k_map, con
                     }
 #pragma unroll
                     for (int x = 0; x < 32; ++x) o[x] = nan[c] >> x & 1 ? 0x7fc00000u : __float_as_uint(__uint_as_float(o[x]) * inv);
-                    if (!whole) {
-                        float* const to = a.parts + ((long long)blockIdx.x * 2 + (item.c0 > 0 ? 0 : 1)) * L::kPart + (q * kTileRows + r) * DP + c * 32;
-                        if (exists)
+                    if (!whole) {                  // 128 bytes of each row
+                        __syncwarp();
 #pragma unroll
-                            for (int x = 0; x < 32; x += 4) *reinterpret_cast<uint4*>(to + x) = make_uint4(o[x], o[x + 1], o[x + 2], o[x + 3]);
+                        for (int x = 0; x < 8; ++x)
+                            *reinterpret_cast<uint4*>(turn + lane * 128 + (x ^ (lane & 7)) * 16) = make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+                        __syncwarp();
+                        float* const to = a.parts + ((long long)blockIdx.x * 2 + (item.c0 > 0 ? 0 : 1)) * L::kPart + (q * kTileRows + (warp & 3) * 32) * DP + c * 32;
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) {
+                            const int at = x * 4 + lane / 8;
+                            *reinterpret_cast<uint4*>(to + at * DP + (lane & 7) * 4) = *reinterpret_cast<const uint4*>(turn + at * 128 + ((lane & 7) ^ (at & 7)) * 16);
+                        }
                         continue;
                     }
 #pragma unroll
