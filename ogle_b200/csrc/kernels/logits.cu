@@ -1,8 +1,10 @@
 // Logits before a token is chosen: repeated-token penalties, sparse biases, grammar masks, in one pass.
 //
-// A block has a slice of one row's vocabulary. It counts the row's tokens that fall into its slice in shared memory (whole
-// numbers: their order does not matter) and notes for each the last bias named for it; then every logit is read and written
-// once, 16 bytes at a time where the row's address allows it.
+// A block has a range of one row's vocabulary. It writes every logit, masked, once - 16 bytes at a time where the row's address
+// allows it - and mends those that a token of the text or a bias names: tokens are counted in shared memory (whole numbers:
+// their order does not matter), the last bias named for a token is noted beside its count, and each such logit is computed
+// anew. A row has some hundred of them, not worth a look-up for each of the others (which took 17 of 25 instructions a logit:
+// 400 x 150000 93 us). Few tokens and biases go into a hash table at once; many are counted slice by slice of the range.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -12,9 +14,21 @@ namespace ogle {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr unsigned kSeen = 0x80000000u;          // the token is in the prompt; the other bits count it behind it
+constexpr int kSlice = 8192;                     // words of shared memory
+constexpr int kEntries = kSlice / 2, kMostHashed = kEntries * 3 / 4;      // of the table: a token and its word each
+constexpr int kText = 2048;                      // tokens of the text that are kept in shared memory
+constexpr unsigned kEmpty = ~0u;
+// A token's word in shared memory: how often it is behind the prompt (17 bits), the last bias named for it (13 bits, 0: none),
+// whether it is in the prompt. Rows with more tokens or biases than that go through half a slice at a time, with 31 bits to count
+// and a table of their own for biases.
+constexpr unsigned kSeen = 0x80000000u;
+constexpr int kBiasShift = 17;
+constexpr int kMaxTokens = (1 << kBiasShift) - 1, kMaxBiases = (1 << 13) - 1;
 
-struct LogitsArgs { OgleLogitsParams p; };
+struct LogitsArgs {
+    OgleLogitsParams p;
+    int range;                                   // tokens of a block
+};
 
 template <typename T> struct Vec { static constexpr int kN = 16 / sizeof(T); };
 
@@ -34,154 +48,197 @@ __device__ __forceinline__ void store_vec(To* p, const float (&x)[N]) {
 
 struct RowTerms { float repetition, presence, frequency; };
 
-__device__ __forceinline__ float adjusted(float x, unsigned count, int bias, const float* bias_value, bool allowed, const RowTerms& t) {
-    if (count) {
+// word: kSeen and the count alone; bias: the last one's number + 1, or 0.
+__device__ __forceinline__ float adjusted(float x, unsigned word, unsigned bias, const float* bias_value, const RowTerms& t) {
+    if (word) {
         x = x > 0.f ? __fdiv_rn(x, t.repetition) : __fmul_rn(x, t.repetition);
-        const unsigned n = count & ~kSeen;
+        const unsigned n = word & ~kSeen;
         if (n) x = __fsub_rn(__fsub_rn(x, __fmul_rn(t.frequency, float(n))), t.presence);
     }
-    if (bias) x = __fadd_rn(x, __ldg(bias_value + bias - 1));
-    return allowed ? x : -INFINITY;
+    return bias ? __fadd_rn(x, __ldg(bias_value + bias - 1)) : x;
 }
 
-// U: vectors of 16 bytes a thread has of the slice; they are on their way while the tokens are counted.
-template <typename Ti, typename To, int U>
-__global__ void __launch_bounds__(kThreads) adjust_logits_kernel(LogitsArgs a) {
-    constexpr int N = Vec<Ti>::kN, kSlice = kThreads * N * U;
-    extern __shared__ __align__(16) unsigned counts[];           // [kSlice], and as many last biases behind them
+// (Loops over tokens are not unrolled: they run once in a block's life, and fetching their instructions took longer than what they do - one
+// row of 32000: 16 us with all of them unrolled, 7 so.)
+template <typename Ti, typename To>
+__global__ void __launch_bounds__(kThreads, 4) adjust_logits_kernel(LogitsArgs a) {
+    constexpr int N = Vec<Ti>::kN, U = 4;
+    __shared__ __align__(16) unsigned words[kSlice];
+    __shared__ int text[kText];
+    __shared__ uint16_t taken[kMostHashed];
+    __shared__ int n_here, n_taken;
     const OgleLogitsParams& p = a.p;
     const int r = blockIdx.y, tid = threadIdx.x;
     const Ti* in = static_cast<const Ti*>(p.logits) + r * p.logits_stride;
     To* out = static_cast<To*>(p.out) + r * p.out_stride;
-    // the row begins `shift` elements behind a 16-byte boundary; a slice is whole vectors between such boundaries
+    // the row begins `shift` elements behind a 16-byte boundary; a range is whole vectors between such boundaries
     const int shift = int(reinterpret_cast<uintptr_t>(in) / sizeof(Ti)) & (N - 1);
     const bool vectors = (reinterpret_cast<uintptr_t>(in) % sizeof(Ti)) == 0 && ((reinterpret_cast<uintptr_t>(out) - shift * sizeof(To)) & 15) == 0;
-    const int s0 = blockIdx.x * kSlice - shift, s1 = min(s0 + kSlice, p.vocab), first = max(s0, 0);
-    if (first >= s1) return;
-    unsigned* const last_bias = counts + kSlice;
-    const bool biased = p.bias_token != nullptr;
+    const int begin = blockIdx.x * a.range - shift, end = min(begin + a.range, p.vocab), first = max(begin, 0);
     grid_dependency_trigger();
     grid_dependency_wait();
-    uint4 v[U];
-    if (vectors) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int t = s0 + (u * kThreads + tid) * N;
-            if (t >= 0 && t + N <= p.vocab) v[u] = *reinterpret_cast<const uint4*>(in + t);
-        }
-    }
-    const uint4 none = make_uint4(0, 0, 0, 0);
-#pragma unroll
-    for (int i = 0; i < N * U / 4; ++i) {
-        reinterpret_cast<uint4*>(counts)[i * kThreads + tid] = none;
-        if (biased) reinterpret_cast<uint4*>(last_bias)[i * kThreads + tid] = none;
-    }
-    __syncthreads();
-    const unsigned width = s1 - first, at0 = first - s0;
-    if (p.tokens) {
-        const int t0 = max(p.token_start[r], 0), n = min(p.token_start[r + 1], p.n_tokens) - t0, prompt = p.prompt_len ? p.prompt_len[r] : 0;
-        const int* tokens = p.tokens + t0;
-#pragma unroll 4
-        for (int i = tid; i < n; i += kThreads) {
-            const unsigned t = unsigned(__ldg(tokens + i) - first);
-            if (t < width) {
-                if (i < prompt) atomicOr(&counts[t + at0], kSeen);
-                else atomicAdd(&counts[t + at0], 1u);
-            }
-        }
-    }
-    const int bias0 = biased ? max(p.bias_start[r], 0) : 0;
-    if (biased) {
-        const int n = min(p.bias_start[r + 1], p.n_biases) - bias0;
-        for (int i = tid; i < n; i += kThreads) {
-            const unsigned t = unsigned(__ldg(p.bias_token + bias0 + i) - first);
-            if (t < width) atomicMax(&last_bias[t + at0], unsigned(i + 1));
-        }
-    }
-    const float* bias_value = biased ? p.bias_value + bias0 : nullptr;
-    const RowTerms terms = {p.repetition ? p.repetition[r] : 1.f, p.presence ? p.presence[r] : 0.f, p.frequency ? p.frequency[r] : 0.f};
     const unsigned* allowed = p.allowed ? p.allowed + r * p.allowed_stride : nullptr;
-    __syncthreads();
-    const auto one = [&](int t) {
-        const bool ok = !allowed || (__ldg(allowed + t / 32) >> (t % 32) & 1);
-        out[t] = To(adjusted(as_float(in[t]), counts[t - s0], biased ? int(last_bias[t - s0]) : 0, bias_value, ok, terms));
-    };
-    if (!vectors) {
-        for (int t = first + tid; t < s1; t += kThreads) one(t);
-        return;
+    const int last_word = (p.vocab - 1) / 32;
+    const int token0 = p.tokens ? max(p.token_start[r], 0) : 0, n_tokens = p.tokens ? min(p.token_start[r + 1], p.n_tokens) - token0 : 0;
+    const int bias0 = p.bias_token ? max(p.bias_start[r], 0) : 0, n_biases = p.bias_token ? min(p.bias_start[r + 1], p.n_biases) - bias0 : 0;
+    const bool named = n_tokens > 0 || n_biases > 0;
+    if (named) {
+#pragma unroll 4
+        for (int i = tid; i < min(n_tokens, kText); i += kThreads) text[i] = __ldg(p.tokens + token0 + i);
+        if (tid == 0) n_here = n_taken = 0;
     }
+    const auto allows = [&](int t) { return !allowed || (__ldg(allowed + t / 32) >> (t % 32) & 1); };
+
+    // every logit, masked (before the counting: where all blocks counted first, the memory had nothing to do meanwhile - 400 x 150000
+    // 80 us, 57 so)
+    int edge = first, edge_end = end;            // what is not whole vectors
+    if (vectors) {
+        for (int t0 = begin + tid * N; t0 < end; t0 += U * kThreads * N) {
+            uint4 v[U];
+            unsigned bits[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int t = s0 + (u * kThreads + tid) * N;
-        if (t >= s1) continue;
-        if (t < 0 || t + N > p.vocab) {          // a vector that hangs over an end of the row
-            for (int l = 0; l < N; ++l)
-                if (t + l >= 0 && t + l < s1) one(t + l);
-            continue;
-        }
-        const Ti* h = reinterpret_cast<const Ti*>(&v[u]);
-        unsigned bits = ~0u;
-        if (allowed) {
-            const int w = t / 32, s = t % 32;
-            bits = __ldg(allowed + w) >> s;
-            if (s + N > 32) bits |= __ldg(allowed + w + 1) << (32 - s);
-        }
-        float x[N];
-        unsigned c[N], any = 0;
+            for (int u = 0; u < U; ++u) {
+                const int t = t0 + u * kThreads * N;
+                if (t >= 0 && t + N <= end) v[u] = *reinterpret_cast<const uint4*>(in + t);
+            }
 #pragma unroll
-        for (int l = 0; l < N; ++l) x[l] = as_float(h[l]);
+            for (int u = 0; u < U; ++u) {        // two words whether or not the bits lie in both: no branch between the loads
+                const int t = min(max(t0 + u * kThreads * N, 0), p.vocab - 1), w = t / 32;
+                bits[u] = allowed ? __funnelshift_r(__ldg(allowed + w), __ldg(allowed + min(w + 1, last_word)), t) : ~0u;
+            }
 #pragma unroll
-        for (int l = 0; l < N; l += 4) {
-            const uint4 q = *reinterpret_cast<const uint4*>(counts + t - s0 + l);
-            c[l] = q.x; c[l + 1] = q.y; c[l + 2] = q.z; c[l + 3] = q.w;
-            any |= q.x | q.y | q.z | q.w;
-        }
-        // most vectors have no token of the text and no bias
-        if (any) {
+            for (int u = 0; u < U; ++u) {
+                const int t = t0 + u * kThreads * N;
+                if (t >= 0 && t + N <= end) {
+                    const Ti* h = reinterpret_cast<const Ti*>(&v[u]);
+                    float x[N];
 #pragma unroll
-            for (int l = 0; l < N; ++l) x[l] = adjusted(x[l], c[l], 0, nullptr, true, terms);
-        }
-        if (biased) {
-#pragma unroll
-            for (int l = 0; l < N; l += 4) {
-                const uint4 q = *reinterpret_cast<const uint4*>(last_bias + t - s0 + l);
-                if (q.x | q.y | q.z | q.w) {
-                    const unsigned i[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) if (i[k]) x[l + k] = __fadd_rn(x[l + k], __ldg(bias_value + i[k] - 1));
+                    for (int l = 0; l < N; ++l) x[l] = bits[u] >> l & 1 ? as_float(h[l]) : -INFINITY;
+                    store_vec<To, N>(out + t, x);
                 }
             }
         }
-#pragma unroll
-        for (int l = 0; l < N; ++l) x[l] = bits >> l & 1 ? x[l] : -INFINITY;
-        store_vec<To, N>(out + t, x);
+        edge_end = begin < 0 ? min(begin + N, end) : first;
     }
-}
+    for (int k = 0; k < 2; ++k) {                // its head, or all of it; its tail
+        for (int t = edge + tid; t < edge_end; t += kThreads) out[t] = To(allows(t) ? as_float(in[t]) : -INFINITY);
+        edge = vectors ? max(begin + (end - begin) / N * N, edge_end) : end;
+        edge_end = end;
+    }
+    if (!named) return;
 
-template <typename Ti, typename To, int U>
-cudaError_t launch(const LogitsArgs& a, cudaStream_t s) {
-    constexpr int kSlice = kThreads * Vec<Ti>::kN * U;
-    const size_t smem = size_t(kSlice) * 4 * (a.p.bias_token ? 2 : 1);
-    auto kernel = adjust_logits_kernel<Ti, To, U>;
-    if (smem > 48 * 1024) {
-        static std::atomic<uint64_t> sized{0};                   // devices whose limit of shared memory is raised
-        int device = 0;
-        cudaError_t e = cudaGetDevice(&device);
-        if (e != cudaSuccess) return e;
-        if (!(sized.load(std::memory_order_relaxed) >> (device & 63) & 1)) {
-            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSlice * 8);
-            if (e != cudaSuccess) return e;
-            sized.fetch_or(1ull << (device & 63), std::memory_order_relaxed);
+    const int prompt = p.tokens && p.prompt_len ? p.prompt_len[r] : 0;
+    const float* bias_value = p.bias_value + bias0;
+    const RowTerms terms = {p.repetition ? p.repetition[r] : 1.f, p.presence ? p.presence[r] : 0.f, p.frequency ? p.frequency[r] : 0.f};
+    // f(number, token), for biases first and then for the text's tokens: those in [s0, s0 + width)
+    const auto each = [&](bool biases, int s0, unsigned width, auto f) {
+        const int n = biases ? n_biases : n_tokens;
+#pragma unroll 1
+        for (int i = tid; i < n; i += kThreads) {
+            const int token = biases ? __ldg(p.bias_token + bias0 + i) : (i < kText ? text[i] : __ldg(p.tokens + token0 + i));
+            if (token >= 0 && unsigned(token - s0) < width) f(i, token);
         }
+    };
+    // (in place, `in` has the logit still: what the mask let through is as it was)
+    const auto mend = [&](int token, unsigned word, unsigned bias) {
+        const float x = as_float(in[token]);
+        if (allows(token)) out[token] = To(adjusted(x, word, bias, bias_value, terms));
+    };
+    const bool is_long = n_tokens > kMaxTokens || n_biases > kMaxBiases;
+    const unsigned range = end - first;
+    unsigned* const keys = words + kEntries;
+
+    // a hash table, where the text's tokens and biases that fall into the range are few
+    for (int i = tid; i < kEntries / 4; i += kThreads) {
+        reinterpret_cast<uint4*>(words)[i] = make_uint4(0, 0, 0, 0);
+        reinterpret_cast<uint4*>(keys)[i] = make_uint4(kEmpty, kEmpty, kEmpty, kEmpty);
     }
-    return launch_overlapped(kernel, dim3(div_up(a.p.vocab + Vec<Ti>::kN - 1, kSlice), a.p.rows), dim3(kThreads), smem, s, a);
+    __syncthreads();                             // all logits of the range are written, too
+    bool hashed = !is_long;
+    if (hashed && n_tokens + n_biases > kMostHashed) {
+        int mine = 0;
+        for (int k = 0; k < 2; ++k) each(k, first, range, [&](int, int) { ++mine; });
+        if (mine) atomicAdd(&n_here, mine);
+        __syncthreads();
+        hashed = n_here <= kMostHashed;
+        __syncthreads();
+    }
+    if (hashed) {
+        const auto entry = [&](int token) {      // its place in the table: at most three quarters are taken, so there is one
+            unsigned h = unsigned(token) * 2654435761u >> 20;
+            for (;;) {
+                const unsigned k = atomicCAS(&keys[h], kEmpty, unsigned(token));
+                if (k == kEmpty) {               // a warp's new entries go on the list together
+                    const unsigned with = __activemask(), lane = tid & 31, leader = __ffs(with) - 1;
+                    int at = 0;
+                    if (lane == leader) at = atomicAdd(&n_taken, __popc(with));
+                    at = __shfl_sync(with, at, leader);
+                    taken[at + __popc(with & ((1u << lane) - 1))] = uint16_t(h);
+                }
+                if (k == kEmpty || k == unsigned(token)) return h;
+                h = (h + 1) & (kEntries - 1);
+            }
+        };
+        static_assert(kEntries == 4096, "20 bits off a hash of 32");
+        // biases first: a word then has nothing else, and its largest value is the last of them
+        if (n_biases > 0) {
+            each(true, first, range, [&](int i, int token) { atomicMax(&words[entry(token)], unsigned(i + 1) << kBiasShift); });
+            __syncthreads();
+        }
+        each(false, first, range, [&](int i, int token) {
+            const unsigned h = entry(token);
+            if (i < prompt) atomicOr(&words[h], kSeen);
+            else atomicAdd(&words[h], 1u);
+        });
+        __syncthreads();
+#pragma unroll 1
+        for (int i = tid; i < n_taken; i += kThreads) {
+            const unsigned h = taken[i], w = words[h];
+            mend(int(keys[h]), w & (kSeen | kMaxTokens), w << 1 >> (kBiasShift + 1));
+        }
+        return;
+    }
+    // a word for each token of a slice, or two: counts and biases
+    const unsigned slice = is_long ? kSlice / 2 : kSlice, step = is_long ? 2 : 1;
+    for (int i = tid; i < kEntries / 4; i += kThreads) reinterpret_cast<uint4*>(keys)[i] = make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+    for (int s0 = first; s0 < end; s0 += slice) {
+        const unsigned width = min(int(slice), end - s0);
+        __syncthreads();                         // the words are 0
+        each(true, s0, width, [&](int i, int token) {
+            atomicMax(&words[(token - s0) * step + step - 1], is_long ? unsigned(i + 1) : unsigned(i + 1) << kBiasShift);
+        });
+        if (!is_long) __syncthreads();
+        each(false, s0, width, [&](int i, int token) {
+            if (i < prompt) atomicOr(&words[(token - s0) * step], kSeen);
+            else atomicAdd(&words[(token - s0) * step], 1u);
+        });
+        __syncthreads();
+        for (int k = 0; k < 2; ++k)              // the first to take a token's word out has the token
+            each(k, s0, width, [&](int, int token) {
+                if (is_long) {
+                    const unsigned long long w = atomicExch(reinterpret_cast<unsigned long long*>(words) + (token - s0), 0ull);
+                    if (w) mend(token, unsigned(w), unsigned(w >> 32));
+                } else {
+                    const unsigned w = atomicExch(&words[token - s0], 0u);
+                    if (w) mend(token, w & (kSeen | kMaxTokens), w << 1 >> (kBiasShift + 1));
+                }
+            });
+    }
 }
 
 template <typename Ti, typename To>
-cudaError_t launch(const LogitsArgs& a, cudaStream_t s) {
-    // Slices of four vectors a thread, which count the row's tokens a quarter as often, where they still fill the GPU.
-    const long blocks = (long)div_up(a.p.vocab, kThreads * Vec<Ti>::kN * 4) * a.p.rows;
-    return blocks >= 2 * kNumSMs ? launch<Ti, To, 4>(a, s) : launch<Ti, To, 1>(a, s);
+cudaError_t launch(LogitsArgs a, cudaStream_t s) {
+    constexpr int N = Vec<Ti>::kN, kPiece = kThreads * N;
+    // A block's range: whole pieces of a vector a thread. As many blocks to a row as one round of them (four to an SM) has
+    // for it; at least one for every 2000 tokens of a row's text, so that those of a range fit the hash table. (400 x 150000, a row a
+    // block: 16 pieces a block 71 us, so 56.)
+    const long pieces = div_up(a.p.vocab + N - 1, kPiece), text = div_up(long(a.p.n_tokens) + a.p.n_biases, a.p.rows);
+    long blocks = 4L * kNumSMs / a.p.rows;
+    if (blocks < div_up(text, 2000)) blocks = div_up(text, 2000);
+    const long each = div_up(pieces, blocks > 1 ? blocks : 1);
+    a.range = int(each * kPiece);
+    return launch_overlapped(adjust_logits_kernel<Ti, To>, dim3(div_up(pieces, each), a.p.rows), dim3(kThreads), 0, s, a);
 }
 
 }  // namespace
@@ -197,7 +254,7 @@ extern "C" int ogle_cuda_adjust_logits(const OgleLogitsParams* p, ogle_stream_t 
     if (!p->logits || !p->out || (p->tokens && !p->token_start) || (p->bias_token && (!p->bias_value || !p->bias_start))) return OGLE_ERR_INVALID;
     if (p->logits_stride < p->vocab || p->out_stride < p->vocab || (p->allowed && p->allowed_stride != 0 && p->allowed_stride < (p->vocab + 31) / 32)) return OGLE_ERR_INVALID;
     if (p->out == p->logits && (p->out_dtype != p->dtype || p->out_stride != p->logits_stride)) return OGLE_ERR_INVALID;
-    const LogitsArgs a = {*p};
+    const LogitsArgs a = {*p, 1};
     cudaError_t e;
     if (p->dtype == OGLE_F32) e = launch<float, float>(a, stream);
     else if (p->dtype == OGLE_F16) e = p->out_dtype == OGLE_F16 ? launch<__half, __half>(a, stream) : launch<__half, float>(a, stream);

@@ -487,6 +487,23 @@ def test_logits(rows, vocab, history, n_bias, masked, dtype, out_dtype):
     assert got.dtype == out_dtype and torch.equal(got.cpu(), want)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_logits_of_long_texts_and_bias_lists(dtype):
+    """Rows around the counts that a token's word holds: 131071 tokens, 8191 biases; a token said more often than that."""
+    rng = np.random.default_rng(5)
+    counts, vocab = [131071, 131072, 400000, 10, 0], 20000
+    x = torch.from_numpy((4 * rng.standard_normal((5, vocab))).astype(np.float32)).to(dtype)
+    starts = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    tokens = np.concatenate([np.full(131071, 7), np.full(131072, 8), (rng.random(400000) ** 8 * vocab), np.arange(10)]).astype(np.int32)
+    tokens[starts[2]:starts[2] + 200000] = 19999
+    prompt = np.array([0, 1, 1000, 3, 0], dtype=np.int32)
+    rep, pres, freq = np.full(5, 1.25, np.float32), np.full(5, 0.5, np.float32), np.array([1e-3, 1e-3, 1e-4, 1.0, 1.0], np.float32)
+    biases = [(rng.integers(0, vocab, n).astype(np.int32), rng.standard_normal(n).astype(np.float32)) for n in (8191, 3, 8192, 9000, 30000)]
+    case = (tokens, starts, prompt, rep, pres, freq, biases, None)
+    got = run_logits(x, *case, out_dtype=F32)
+    assert torch.equal(got.cpu(), torch.from_numpy(logits32(x.float().numpy(), *case)))
+
+
 def test_logits_steps_that_are_left_out():
     x, tokens, starts, prompt, rep, pres, freq, biases, allowed = logits_case(4, 3000, 100, 6, True, F32)
     full = (tokens, starts, prompt, rep, pres, freq, biases, allowed)
