@@ -131,7 +131,7 @@ __device__ __forceinline__ float finite_abs(float x) {
 }
 
 template <typename T, int W>
-__global__ void __launch_bounds__(kMaxThreads) paged_append_kernel(AppendArgs a) {
+__global__ void __launch_bounds__(kMaxThreads, 3) paged_append_kernel(AppendArgs a) {
     __shared__ int where[4];
     __shared__ float warp_max[kMaxThreads / 32];
     const Batch& B = a.b;
