@@ -542,3 +542,70 @@ def test_logits_between_unlike_strides():
 
 def test_nothing_waited_in_vain():
     assert _lib.cuda_lib().ogle_cuda_device_status() == 0
+
+
+# -------------------------------------------------------------------------------------------------------- example
+def whole_text_logits(model, text, prompt_len, caches, page_tokens, pages, answers):
+    """The example model's last logits from the whole text in 64 bits, over the keys and values that its cache holds."""
+    w = lambda t: t.cpu().double()  # noqa: E731
+    n, h, hk, d = len(text), model.q_heads, model.kv_heads, model.head_dim
+    x = w(model.embedding)[text]
+    table = w(model.rotary)[:n]
+    for layer, cache in enumerate(caches):
+        q = (x @ w(model.qkv[layer]).T).view(n, h + 2 * hk, d)[:, :h].clone()
+        c, s = table[:, None, :d // 2], table[:, None, d // 2:]
+        a, b = q[..., :d // 2].clone(), q[..., d // 2:].clone()
+        q[..., :d // 2], q[..., d // 2:] = a * c - b * s, b * c + a * s
+        k, v = (ref.cached(cache[i], cache[2 + i], torch.tensor(pages), n) for i in (0, 1))
+        o = torch.zeros(n, h, d, dtype=torch.float64)
+        hidden = torch.arange(n)[None] > torch.arange(n)[:, None]
+        if model.window:
+            hidden |= torch.arange(n)[None] <= torch.arange(n)[:, None] - model.window
+        for i in range(h):
+            p = torch.softmax((q[:, i] @ k[:, i // (h // hk)].T * d ** -0.5).masked_fill(hidden, -math.inf), 1)
+            o[:, i] = p @ v[:, i // (h // hk)]
+        x = x + o.reshape(n, -1) @ w(model.out[layer]).T
+    return x[-1] @ w(model.embedding).T
+
+
+@pytest.mark.parametrize("window", [0, 9])
+def test_example_answers(window):
+    """Prompts and single tokens through products, append, attention and logits: each step's logits are those of the whole text. (The
+    cache holds what was quantised on the way, so keys and values are taken from it.) Tolerance: fp32-grade products and sums
+    over two layers, 1e-4 of the largest logit."""
+    from ogle_b200 import lm_example
+    model = lm_example.Model(window=window)
+    g = torch.Generator().manual_seed(3)
+    prompts = [torch.randint(1, 1000, (n,), generator=g).tolist() for n in (5, 1, 40, 17)]
+    answers = lm_example.Answers(model, prompts, favoured=((7, 4.0), (31, -2.0)))
+    for _ in range(6):
+        texts = [list(t) for t in answers.texts]
+        got = answers.step().cpu().double()
+        for b, text in enumerate(texts):
+            want = whole_text_logits(model, text, len(prompts[b]), answers.caches, 16, answers.pages[b], answers)
+            seen, said = torch.tensor(sorted(set(text))), torch.bincount(torch.tensor(text[len(prompts[b]):] or [0]), minlength=1000).double()
+            if len(text) == len(prompts[b]):
+                said.zero_()
+            raw = float(want.abs().max())
+            want[seen] = torch.where(want[seen] > 0, want[seen] / np.float64(np.float32(1.3)), want[seen] * np.float64(np.float32(1.3)))
+            want -= said * np.float64(np.float32(0.2)) + (said > 0) * 0.5
+            want[7] += 4.0
+            want[31] -= 2.0
+            assert float(got[b, 0]) == -math.inf
+            assert float((got[b, 1:] - want[1:]).abs().max()) <= 1e-4 * raw
+    assert all(0 not in t[len(p):] for t, p in zip(answers.texts, prompts))
+
+
+def test_example_answers_do_not_depend_on_the_batch():
+    from ogle_b200 import lm_example
+    model = lm_example.Model()
+    g = torch.Generator().manual_seed(4)
+    prompts = [torch.randint(1, 1000, (n,), generator=g).tolist() for n in (3, 30, 12)]
+    together = lm_example.Answers(model, prompts)
+    for _ in range(8):
+        together.step()
+    for i, p in enumerate(prompts):
+        alone = lm_example.Answers(model, [p])
+        for _ in range(8):
+            alone.step()
+        assert alone.texts[0] == together.texts[i]
