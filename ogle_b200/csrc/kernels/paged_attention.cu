@@ -28,15 +28,16 @@ constexpr int kSegmentCost = 8;                  // tiles that a segment's begin
 template <int DP, int MT, bool kSplit>
 struct Form {
     static constexpr int kRows = MT * (kSplit ? 8 : 16);
-    static constexpr int kStages = DP == 64 ? 6 : (DP == 128 ? 4 : 3);
+    static constexpr int kStages = DP == 64 ? 5 : 3;
     static constexpr int kBoxBytes = kChunk * (DP == 64 ? 64 : 128);                // of one copy
     static constexpr int kBoxes = DP == 256 ? 2 : 1;                                // to a step's keys, or values
     static constexpr int kStageBytes = 2 * kChunk * DP;
     static constexpr int kRing = kWarps * kStages * kStageBytes;
     static constexpr int kJoin = kWarps * kRows * (DP + 4) * 4;
-    static constexpr int kSmem = (kRing > kJoin ? kRing : kJoin) + 1024;            // the ring begins on a swizzle's boundary
+    static constexpr int kQueries = (kRing > kJoin ? kRing : kJoin);                // behind both: the queries as A operands, a lane's 16 bytes a step
+    static constexpr int kSmem = kQueries + MT * (DP / 16) * 512 + 1024;            // the ring begins on a swizzle's boundary
     static constexpr int kPart = kRows * (DP + 2);      // floats of a part: values, then m, then sums
-    static constexpr int kBlocks = (DP == 64 ? 4 : (DP == 128 ? 3 : 2)) - (MT == 2 ? 1 : 0);   // that fit an SM at once
+    static constexpr int kBlocks = DP == 64 ? (MT == 1 ? 5 : 3) : (DP == 128 ? (MT == 1 ? 4 : 2) : 2);   // that fit an SM at once
 };
 
 // ---- the ranges
@@ -205,6 +206,7 @@ paged_attention_kernel(AttnArgs a, const __grid_constant__ CUtensorMap k_map, co
     __shared__ long long shared[10];
     __shared__ __align__(8) uint64_t bars[kWarps][F::kStages];
     __shared__ int gave_up, more_segments;
+    __shared__ float row_scale[kRows];
     __shared__ Walk walk;
     __shared__ Segment segment;
     unsigned char* const smem = dynamic + ((1024 - (tc::smem_u32(dynamic) & 1023)) & 1023);
@@ -272,44 +274,51 @@ paged_attention_kernel(AttnArgs a, const __grid_constant__ CUtensorMap k_map, co
             if (i < count) issue(i, p);
         }
 
-        // queries: this thread's parts of the rows it has
-        uint32_t Q[MT][KS][4];
-        float rs[MT][NR], off[MT][NR], bar_x[MT][NR], l[MT][NR];      // weight 2^(x - off); an x above bar_x moves both
+        // queries, once for all warps: in shared memory as the products take them (registers for them would leave room for a block less)
+        uint4* const queries = reinterpret_cast<uint4*>(smem + F::kQueries) + lane;
+        const float kDown = -3e38f;               // m of a row that has not met a key
+        float rs[MT][NR], noff[MT][NR], l[MT][NR];            // weight 2^(s rs + noff) of product s; noff = kLift - m
+#pragma unroll
+        for (int i = 0; i < MT * NR; ++i) {
+            const int mt = i / NR, r = i % NR;
+            if (i % kWarps != warp || segment.steps == 0) continue;     // steps 0: a range that has the segment's cost alone
+            // rows that are not there repeat the last
+            const int tile_row = mt * (kSplit ? 8 : 16) + r * 8 + r8, row = min(segment.m0 + tile_row, segment.m_end - 1);
+            const long long q0 = (segment.s.row0 + row / B.group) * a.q_row + (h * B.group + row % B.group) * a.q_head;
+            float f[DP / 4], top = 0.f;
+#pragma unroll
+            for (int u = 0; u < DP / 64; ++u) load16(a.q, q0, 16 * (c4 + 4 * u), B.dim, B.dtype, f + 16 * u);
+#pragma unroll
+            for (int x = 0; x < DP / 4; ++x) top = fmaxf(top, fabsf(f[x]));
+            top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+            // 2^e with |q| 2^-e below 2^12; an infinite or vanishing row stays as it is. A negative scale turns the queries' signs; scores
+            // scaled by 0 are alike, hidden ones are not
+            const int e = top > 1e-30f && top <= 3e38f ? int(__float_as_uint(top) >> 23) - 126 - 12 : 0;
+            const float down = __uint_as_float(uint32_t(127 - e) << 23 | (a.scale_log2 < 0.f ? 0x80000000u : 0u));
+            if (c4 == 0) row_scale[tile_row] = fmaxf(fabsf(a.scale_log2) * __uint_as_float(uint32_t(127 + e) << 23), 1e-37f);
+#pragma unroll
+            for (int x = 0; x < DP / 4; ++x) f[x] *= down;
+#pragma unroll
+            for (int t = 0; t < KS; ++t) {        // step t: word t % 4 of unit c4 + 4 (t / 4) - the order in which keys are read
+                const uint32_t u = half2_bits(f[4 * t], f[4 * t + 1]), v = half2_bits(f[4 * t + 2], f[4 * t + 3]);
+                uint4* const to = queries + (mt * KS + t) * 32;
+                if (kSplit) {
+                    *to = make_uint4(u, rest_bits(u, f[4 * t], f[4 * t + 1]), v, rest_bits(v, f[4 * t + 2], f[4 * t + 3]));
+                } else {
+                    reinterpret_cast<uint32_t*>(to)[r] = u;
+                    reinterpret_cast<uint32_t*>(to)[2 + r] = v;
+                }
+            }
+        }
+        __syncthreads();
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
-                // rows that are not there repeat the last
-                const int row = min(segment.m0 + mt * (kSplit ? 8 : 16) + r * 8 + r8, segment.m_end - 1);
-                const long long q0 = (segment.s.row0 + row / B.group) * a.q_row + (h * B.group + row % B.group) * a.q_head;
-                off[mt][r] = 0.f;
-                bar_x[mt][r] = -INFINITY;
+                noff[mt][r] = kLift - kDown;
                 l[mt][r] = 0.f;
-                rs[mt][r] = 0.f;
-                if (segment.steps == 0) continue; // a range that has the segment's cost alone
-                float f[DP / 4], top = 0.f;
-#pragma unroll
-                for (int u = 0; u < DP / 64; ++u) load16(a.q, q0, 16 * (c4 + 4 * u), B.dim, B.dtype, f + 16 * u);
-#pragma unroll
-                for (int x = 0; x < DP / 4; ++x) top = fmaxf(top, fabsf(f[x]));
-                top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-                // 2^e with |q| 2^-e below 2^12; an infinite or vanishing row stays as it is
-                const int e = top > 1e-30f && top <= 3e38f ? int(__float_as_uint(top) >> 23) - 126 - 12 : 0;
-                const float down = __uint_as_float(uint32_t(127 - e) << 23);
-                rs[mt][r] = a.scale_log2 * __uint_as_float(uint32_t(127 + e) << 23);
-#pragma unroll
-                for (int x = 0; x < DP / 4; ++x) f[x] *= down;
-#pragma unroll
-                for (int t = 0; t < KS; ++t) {    // step t: word t % 4 of unit c4 + 4 (t / 4) - the order in which keys are read
-                    const uint32_t u = half2_bits(f[4 * t], f[4 * t + 1]), v = half2_bits(f[4 * t + 2], f[4 * t + 3]);
-                    if (kSplit) {
-                        Q[mt][t][0] = u; Q[mt][t][1] = rest_bits(u, f[4 * t], f[4 * t + 1]);
-                        Q[mt][t][2] = v; Q[mt][t][3] = rest_bits(v, f[4 * t + 2], f[4 * t + 3]);
-                    } else {
-                        Q[mt][t][r] = u; Q[mt][t][2 + r] = v;
-                    }
-                }
+                rs[mt][r] = row_scale[mt * (kSplit ? 8 : 16) + r * 8 + r8];
             }
         float O[MT][NB][4];
 #pragma unroll
@@ -342,10 +351,12 @@ paged_attention_kernel(AttnArgs a, const __grid_constant__ CUtensorMap k_map, co
             }
             if (++get == F::kStages) { get = 0; parity ^= 1; }
             const int j0 = j_begin + (i * kWarps + warp) * kChunk;
-            const float k_scale = __shfl_sync(~0u, ks[0], i & 31), v_scale = __shfl_sync(~0u, vs[0], i & 31);
+            float k_scale = __shfl_sync(~0u, ks[0], i & 31);
+            const float v_scale = __shfl_sync(~0u, vs[0], i & 31);
             const bool edge = j0 < inner_lo || j0 + kChunk > inner_hi || k_scale == 0.f;
-            // x = q . k
-            float x[MT][2][NR * 2], S[2][MT][4];
+            if (k_scale == 0.f) k_scale = 1.f;    // no page: all is hidden below
+            // products of queries and keys; rows of parts are put together
+            float S[2][MT][4];
 #pragma unroll
             for (int nb = 0; nb < 2; ++nb)
 #pragma unroll
@@ -358,27 +369,27 @@ paged_attention_kernel(AttnArgs a, const __grid_constant__ CUtensorMap k_map, co
 #pragma unroll
                 for (int nb = 0; nb < 2; ++nb) w[nb] = *reinterpret_cast<const uint4*>(step + unit_at<DP>(nb * 8 + key_of<DP>(r8), c4 + 4 * u));
 #pragma unroll
-                for (int y = 0; y < 4; ++y)       // the two blocks in turn: neither waits for its own last product
+                for (int y = 0; y < 4; ++y) {     // the two blocks in turn: neither waits for its own last product
+                    uint32_t q[MT][4];
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) *reinterpret_cast<uint4*>(q[mt]) = queries[(mt * KS + 4 * u + y) * 32];
 #pragma unroll
                     for (int nb = 0; nb < 2; ++nb) {
                         uint32_t b0, b1;
                         paged::e4m3x4_to_half2(reinterpret_cast<const uint32_t*>(&w[nb])[y], b0, b1);
 #pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) mma(S[nb][mt], Q[mt][4 * u + y], b0, b1);
-                    }
-            }
-#pragma unroll
-            for (int nb = 0; nb < 2; ++nb)
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    if (kSplit) {
-                        x[mt][nb][0] = (S[nb][mt][0] + S[nb][mt][2]) * (rs[mt][0] * k_scale);
-                        x[mt][nb][1] = (S[nb][mt][1] + S[nb][mt][3]) * (rs[mt][0] * k_scale);
-                    } else {
-#pragma unroll
-                        for (int y = 0; y < 4; ++y) x[mt][nb][y % (2 * NR)] = S[nb][mt][y] * (rs[mt][(y / 2) % NR] * k_scale);
+                        for (int mt = 0; mt < MT; ++mt) mma(S[nb][mt], q[mt], b0, b1);
                     }
                 }
+            }
+            if (kSplit)
+#pragma unroll
+                for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+                        S[nb][mt][0] += S[nb][mt][2];
+                        S[nb][mt][1] += S[nb][mt][3];
+                    }
             if (edge) {
                 const bool no_page = __shfl_sync(~0u, page[0], i & 31) == nowhere;
 #pragma unroll
@@ -392,39 +403,59 @@ paged_attention_kernel(AttnArgs a, const __grid_constant__ CUtensorMap k_map, co
 #pragma unroll
                             for (int y = 0; y < 2; ++y) {
                                 const int j = j0 + nb * 8 + key_of<DP>(c4 * 2 + y);
-                                if (no_page || j < k.lo || j >= k.hi) x[mt][nb][2 * r + y] = -INFINITY;
+                                if (no_page || j < k.lo || j >= k.hi) S[nb][mt][2 * r + y] = -INFINITY;
                             }
                     }
             }
-            // a larger unit for a row's weights or for the values: rare
-            bool more = v_scale > vref;
+            // weights 2^(s rk + noff), times the values' scale against the largest met so far, as A operands of the second product
+            const float scale = v_scale == 0.f ? vref : v_scale;
+            float v_log = 0.f, v_back = 1.f;      // log2 of that ratio, and its inverse for the sums of weights
+            if (scale < vref) {
+                const float ratio = scale * vinv;
+                v_log = __log2f(ratio);
+                v_back = 1.f / ratio;
+            }
+            float e[MT][2][2 * NR], rk[MT][NR];
+            bool more = scale > vref;
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                for (int nb = 0; nb < 2; ++nb)
+                for (int r = 0; r < NR; ++r) {
+                    rk[mt][r] = rs[mt][r] * k_scale;
 #pragma unroll
-                    for (int y = 0; y < 2 * NR; ++y) more |= x[mt][nb][y] > bar_x[mt][y / 2];
+                    for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+                        for (int y = 0; y < 2; ++y) {
+                            e[mt][nb][2 * r + y] = fmaf(S[nb][mt][2 * r + y], rk[mt][r], noff[mt][r] + v_log);
+                            more |= e[mt][nb][2 * r + y] > kHeadroom + kLift + v_log;
+                        }
+                }
             if (__any_sync(~0u, more)) {
-                const float vnew = fmaxf(vref, v_scale), vratio = vref / vnew;
+                // a larger unit for a row's weights or for the values: rare
+                const float vnew = fmaxf(vref, scale), vratio = vref / vnew;
                 vref = vnew;
                 vinv = 1.f / vnew;
+                if (scale == vnew) { v_log = 0.f; v_back = 1.f; }
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
                     float f[NR];
 #pragma unroll
                     for (int r = 0; r < NR; ++r) {
-                        float top = fmaxf(fmaxf(x[mt][0][2 * r], x[mt][0][2 * r + 1]), fmaxf(x[mt][1][2 * r], x[mt][1][2 * r + 1]));
+                        const float* s0 = &S[0][mt][2 * r];
+                        const float* s1 = &S[1][mt][2 * r];
+                        float top = fmaxf(fmaxf(s0[0], s0[1]), fmaxf(s1[0], s1[1])) * rk[mt][r];
                         top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
                         top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-                        top = fmaxf(top, bar_x[mt][r] - kHeadroom);
-                        f[r] = 1.f;
-                        if (top > -INFINITY) {
-                            f[r] = exp2_fast(bar_x[mt][r] - kHeadroom - top);
-                            off[mt][r] = top - kLift;
-                            bar_x[mt][r] = top + kHeadroom;
-                        }
+                        const float m = kLift - noff[mt][r];
+                        top = fmaxf(top, m);
+                        f[r] = exp2_fast(m - top);
+                        noff[mt][r] = kLift - top;
                         l[mt][r] *= f[r];
                         f[r] *= vratio;
+#pragma unroll
+                        for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+                            for (int y = 0; y < 2; ++y) e[mt][nb][2 * r + y] = fmaf(S[nb][mt][2 * r + y], rk[mt][r], noff[mt][r] + v_log);
                     }
 #pragma unroll
                     for (int n = 0; n < NB; ++n)
@@ -432,30 +463,26 @@ paged_attention_kernel(AttnArgs a, const __grid_constant__ CUtensorMap k_map, co
                         for (int y = 0; y < 4; ++y) O[mt][n][y] *= f[(y / 2) % NR];
                 }
             }
-            // weights, and with the values' scale as A operands of the second product
-            const float v_unit = v_scale * vinv;
             uint32_t P[MT][4];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                for (int nb = 0; nb < 2; ++nb)
+                for (int r = 0; r < NR; ++r) {
+                    float sum = 0.f;
 #pragma unroll
-                    for (int r = 0; r < NR; ++r) {
-                        float p[2];
-#pragma unroll
-                        for (int y = 0; y < 2; ++y) {
-                            p[y] = exp2_fast(x[mt][nb][2 * r + y] - off[mt][r]);
-                            l[mt][r] += p[y];
-                            p[y] *= v_unit;
-                        }
-                        const uint32_t hi = half2_bits(p[0], p[1]);
+                    for (int nb = 0; nb < 2; ++nb) {
+                        const float p0 = exp2_fast(e[mt][nb][2 * r]), p1 = exp2_fast(e[mt][nb][2 * r + 1]);
+                        sum += p0 + p1;
+                        const uint32_t hi = half2_bits(p0, p1);
                         if (kSplit) {
                             P[mt][2 * nb] = hi;
-                            P[mt][2 * nb + 1] = rest_bits(hi, p[0], p[1]);
+                            P[mt][2 * nb + 1] = rest_bits(hi, p0, p1);
                         } else {
                             P[mt][2 * nb + r] = hi;
                         }
                     }
+                    l[mt][r] = fmaf(sum, v_back, l[mt][r]);
+                }
             // the step's values, two units (32 elements) at a time
             const auto values = [&](auto at_edge) {
                 constexpr bool kEdge = decltype(at_edge)::value;
@@ -467,8 +494,8 @@ paged_attention_kernel(AttnArgs a, const __grid_constant__ CUtensorMap k_map, co
                         for (int nb = 0; nb < 2; ++nb)
 #pragma unroll
                             for (int r = 0; r < 2; ++r) {
-                                const float* e = &x[mt][nb][2 * (r % NR)];
-                                seen[mt][2 * nb + r] = r >= NR ? 0u : (e[0] == -INFINITY ? 0u : 0x3c00u) | (e[1] == -INFINITY ? 0u : 0x3c000000u);
+                                const float* s = &S[nb][mt][2 * (r % NR)];
+                                seen[mt][2 * nb + r] = r >= NR ? 0u : (s[0] == -INFINITY ? 0u : 0x3c00u) | (s[1] == -INFINITY ? 0u : 0x3c000000u);
                             }
                 }
 #pragma unroll
@@ -540,7 +567,7 @@ paged_attention_kernel(AttnArgs a, const __grid_constant__ CUtensorMap k_map, co
                     v.x *= vref; v.y *= vref; v.z *= vref; v.w *= vref;
                     *reinterpret_cast<float4*>(row + u * 16 + c4 * 4) = v;
                 }
-                if (c4 == 0) { row[DP] = bar_x[mt][r] - kHeadroom; row[DP + 1] = sum; }
+                if (c4 == 0) { row[DP] = kLift - noff[mt][r]; row[DP + 1] = sum; }
             }
         __syncthreads();
         const bool whole = segment.c0 == 0 && segment.c1 == segment.cost;

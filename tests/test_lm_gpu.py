@@ -59,6 +59,16 @@ def test_attention_of_all_tokens(dtype):
         ref.check_attention(got, ref.attention64(q, batch, total, new, scale=0.3, causal=False, window=window), dtype)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("scale", [-0.2, 0.0])
+def test_attention_with_negative_and_vanishing_scales(scale, dtype):
+    new, past = [1, 3], [300, 20]
+    batch, total = ref.make_batch(new, past, 16, 2, 128)
+    q = rows_of(4, 8, 128, dtype)
+    got = lm.attention(q, scale=scale, **batch)
+    ref.check_attention(got, ref.attention64(q, batch, total, new, scale=scale), dtype)
+
+
 def test_sequences_without_tokens_or_rows():
     new, past = [1, 0, 1, 3, 0], [10, 5, 0, 100, 0]
     batch, total = ref.make_batch(new, past, 16, 2, 128)
