@@ -606,14 +606,11 @@ paged_attention_kernel(AttnArgs a, const __grid_constant__ CUtensorMap k_map, co
 }
 
 // Adds up the parts of segments that were cut, in the order of their ranges, and answers for sequences without a key. Block
-// (c, y) has segment c, or the one that begins in range c and goes on in the next; of its rows y, y + gridDim.y, ...:
-// kWarpsOfRow warps have a row, and each every so-many-th of its parts.
+// (c, y) has segment c, or the one that begins in range c and goes on in the next; of its rows y, y + gridDim.y, ... a warp has one.
 constexpr int kJoinWarps = 8;
-template <int DP, int kWarpsOfRow>
+template <int DP>
 __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(AttnArgs a, int ranges, int rows_of_tile) {
-    constexpr int kVecs = DP / 4, kPerLane = (kVecs + 31) / 32, kRowsAtOnce = kJoinWarps / kWarpsOfRow;
-    __shared__ float4 sums[kJoinWarps][kVecs];
-    __shared__ float weights[kJoinWarps];
+    constexpr int kVecs = DP / 4, kPerLane = (kVecs + 31) / 32;
     const Batch& B = a.b;
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, c = blockIdx.x;
     grid_dependency_trigger();
@@ -636,65 +633,126 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(AttnArgs a,
     const int part_floats = rows_of_tile * (DP + 2);
     const auto part = [&](int k) { return a.parts + ((long long)k * 2 + (k == cut.first ? 1 : 0)) * part_floats; };
     const auto none = [&](int k) { return cut.gaps && quotient(cut.total * k, ranges) == quotient(cut.total * (k + 1), ranges); };
-    for (int r0 = blockIdx.y * kRowsAtOnce; r0 < cut.rows; r0 += gridDim.y * kRowsAtOnce) {
-        const int r = r0 + warp / kWarpsOfRow;
+    for (int r = blockIdx.y * kJoinWarps + warp; r < cut.rows; r += gridDim.y * kJoinWarps) {
         float top = -INFINITY, sum = 0.f;
         float4 v[kPerLane];
 #pragma unroll
         for (int u = 0; u < kPerLane; ++u) v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (r < cut.rows) {
-            for (int k = cut.first + lane; k < cut.last; k += 32)
-                if (!none(k)) {
-                    const float* p = part(k) + rows_of_tile * DP + r;
-                    if (p[rows_of_tile] != 0.f) top = fmaxf(top, p[0]);
-                }
+        for (int k = cut.first + lane; k < cut.last; k += 32)
+            if (!none(k)) {
+                const float* p = part(k) + rows_of_tile * DP + r;
+                if (p[rows_of_tile] != 0.f) top = fmaxf(top, p[0]);
+            }
 #pragma unroll
-            for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+        for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
 #pragma unroll 4
-            for (int k = cut.first + warp % kWarpsOfRow; k < cut.last; k += kWarpsOfRow) {
-                if (none(k)) continue;
-                const float* p = part(k);
-                const float m = p[rows_of_tile * DP + r], l = p[rows_of_tile * DP + rows_of_tile + r];
-                const float f = l == 0.f ? 0.f : exp2_fast(m - top);    // a part without a weight has zeros
-                sum += l * f;
-#pragma unroll
-                for (int u = 0; u < kPerLane; ++u)
-                    if (u * 32 + lane < kVecs) {
-                        const float4 o = *reinterpret_cast<const float4*>(p + r * DP + (u * 32 + lane) * 4);
-                        v[u].x += o.x * f; v[u].y += o.y * f; v[u].z += o.z * f; v[u].w += o.w * f;
-                    }
-            }
-        }
-        if (kWarpsOfRow > 1) {
+        for (int k = cut.first; k < cut.last; ++k) {
+            if (none(k)) continue;
+            const float* p = part(k);
+            const float m = p[rows_of_tile * DP + r], l = p[rows_of_tile * DP + rows_of_tile + r];
+            const float f = l == 0.f ? 0.f : exp2_fast(m - top);    // a part without a weight has zeros
+            sum += l * f;
 #pragma unroll
             for (int u = 0; u < kPerLane; ++u)
-                if (u * 32 + lane < kVecs) sums[warp][u * 32 + lane] = v[u];
-            if (lane == 0) weights[warp] = sum;
-            __syncthreads();
-            sum = 0.f;
-#pragma unroll
-            for (int u = 0; u < kPerLane; ++u) {
-                v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (warp % kWarpsOfRow == 0 && u * 32 + lane < kVecs)
-#pragma unroll
-                    for (int w = 0; w < kWarpsOfRow; ++w) {
-                        const float4 q = sums[warp + w][u * 32 + lane];
-                        v[u].x += q.x; v[u].y += q.y; v[u].z += q.z; v[u].w += q.w;
-                    }
-            }
-            if (warp % kWarpsOfRow == 0)
-#pragma unroll
-                for (int w = 0; w < kWarpsOfRow; ++w) sum += weights[warp + w];
-            __syncthreads();
+                if (u * 32 + lane < kVecs) {
+                    const float4 o = *reinterpret_cast<const float4*>(p + r * DP + (u * 32 + lane) * 4);
+                    v[u].x += o.x * f; v[u].y += o.y * f; v[u].z += o.z * f; v[u].w += o.w * f;
+                }
         }
-        if (r < cut.rows && warp % kWarpsOfRow == 0) {
-            const int row = cut.m0 + r;
+        const int row = cut.m0 + r;
 #pragma unroll
-            for (int u = 0; u < kPerLane; ++u)
-                if (u * 32 + lane < kVecs)
-                    store_row(a, cut.row0 + row / B.group, cut.h * B.group + row % B.group, (u * 32 + lane) * 4, v[u], top, sum);
+        for (int u = 0; u < kPerLane; ++u)
+            if (u * 32 + lane < kVecs)
+                store_row(a, cut.row0 + row / B.group, cut.h * B.group + row % B.group, (u * 32 + lane) * 4, v[u], top, sum);
+    }
+}
+
+// The same for segments of many parts: a block has one row, looks at all its parts' maxima and sums at once, and its warps take
+// every sixteenth part each.
+constexpr int kManyWarps = 16, kMostRanges = 8 * kNumSMs;
+template <int DP>
+__global__ void __launch_bounds__(kManyWarps * 32) paged_join_many_kernel(AttnArgs a, int ranges, int rows_of_tile) {
+    constexpr int kVecs = DP / 4, kPerLane = (kVecs + 31) / 32;
+    __shared__ float factor[kMostRanges];
+    __shared__ float4 sums[kManyWarps][kVecs];
+    __shared__ float tops[kManyWarps], weights[kManyWarps];
+    const Batch& B = a.b;
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, c = blockIdx.x, r = blockIdx.y;
+    grid_dependency_trigger();
+    grid_dependency_wait();
+    // what nobody has written of: tiles of rows that the sequence does not have, sequences without a key
+    const Cut cut = a.cuts[c];
+    const Sequence s = few_sequence(a, c / (B.kv_heads * a.by_segment));
+    const int tiles = tiles_of(s, a.causal, a.window);
+    if (r == 0 && s.n > 0 && tiles == 0 && c % (B.kv_heads * a.by_segment) == 0)
+        for (int idx = tid; idx < s.n * B.q_heads; idx += blockDim.x)
+            for (int d = 0; d < B.dim; d += 4)
+                store_row(a, s.row0 + idx / B.q_heads, idx % B.q_heads, d, make_float4(0.f, 0.f, 0.f, 0.f), 0.f, 0.f);
+    if (c % a.by_segment >= row_tiles(B, s.n, rows_of_tile) || tiles == 0 || r >= cut.rows) return;
+    const int part_floats = rows_of_tile * (DP + 2), n = cut.last - cut.first;
+    const auto part = [&](int k) { return a.parts + ((long long)(cut.first + k) * 2 + (k == 0 ? 1 : 0)) * part_floats; };
+    const auto none = [&](int k) { return cut.gaps && quotient(cut.total * (cut.first + k), ranges) == quotient(cut.total * (cut.first + k + 1), ranges); };
+    constexpr int kMine = (kMostRanges + kManyWarps * 32 - 1) / (kManyWarps * 32);
+    float m[kMine], l[kMine], top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+        const int k = tid + i * kManyWarps * 32;
+        m[i] = l[i] = 0.f;
+        if (k < n && !none(k)) {
+            const float* p = part(k) + rows_of_tile * DP + r;
+            m[i] = p[0];
+            l[i] = p[rows_of_tile];
+            if (l[i] != 0.f) top = fmaxf(top, m[i]);
         }
     }
+#pragma unroll
+    for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+    if (lane == 0) tops[warp] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kManyWarps; ++w) top = fmaxf(top, tops[w]);
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+        const int k = tid + i * kManyWarps * 32;
+        const float f = l[i] == 0.f ? 0.f : exp2_fast(m[i] - top);       // a part without a weight has zeros, a range without a tile no part
+        if (k < n) factor[k] = l[i] == 0.f ? -1.f : f;
+        sum += l[i] * f;
+    }
+#pragma unroll
+    for (int d = 16; d; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
+    if (lane == 0) weights[warp] = sum;
+    __syncthreads();
+    float4 v[kPerLane];
+#pragma unroll
+    for (int u = 0; u < kPerLane; ++u) v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int k = warp; k < n; k += kManyWarps) {
+        const float f = factor[k];
+        if (f == -1.f) continue;
+        const float* p = part(k) + r * DP;
+#pragma unroll
+        for (int u = 0; u < kPerLane; ++u)
+            if (u * 32 + lane < kVecs) {
+                const float4 o = *reinterpret_cast<const float4*>(p + (u * 32 + lane) * 4);
+                v[u].x += o.x * f; v[u].y += o.y * f; v[u].z += o.z * f; v[u].w += o.w * f;
+            }
+    }
+#pragma unroll
+    for (int u = 0; u < kPerLane; ++u)
+        if (u * 32 + lane < kVecs) sums[warp][u * 32 + lane] = v[u];
+    __syncthreads();
+    if (tid >= kVecs) return;
+    sum = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kManyWarps; ++w) {
+        const float4 q = sums[w][tid];
+        sum += weights[w];
+        o.x += q.x; o.y += q.y; o.z += q.z; o.w += q.w;
+    }
+    const int row = cut.m0 + r;
+    store_row(a, cut.row0 + row / B.group, cut.h * B.group + row % B.group, tid * 4, o, top, sum);
 }
 
 // ---- host
@@ -775,15 +833,17 @@ bool cache_map(CUtensorMap* m, const Batch& b, const void* cache, int dp) {
 }
 
 int launch_join(const AttnArgs& a, int dp, bool many, int entries, int ranges, int tile_rows, int rows, cudaStream_t stream) {
-    const auto run = [&](auto kernel, int y) {
+    const auto run = [&](auto kernel, int y, int warps) {
         const cudaError_t e = launch_overlapped_if(overlapped_launches_enabled(true), kernel, dim3(unsigned(entries), unsigned(y)),
-                                                   dim3(kJoinWarps * 32), 0, stream, a, ranges, tile_rows);
+                                                   dim3(warps * 32), 0, stream, a, ranges, tile_rows);
         if (e != cudaSuccess) { set_last_error(e); (void)cudaGetLastError(); return int(OGLE_ERR_CUDA); }
         return finish_launch();
     };
-    if (dp == 64) return many ? run(paged_join_kernel<64, kJoinWarps>, rows) : run(paged_join_kernel<64, 1>, div_up(rows, kJoinWarps));
-    if (dp == 128) return many ? run(paged_join_kernel<128, kJoinWarps>, rows) : run(paged_join_kernel<128, 1>, div_up(rows, kJoinWarps));
-    return many ? run(paged_join_kernel<256, kJoinWarps>, rows) : run(paged_join_kernel<256, 1>, div_up(rows, kJoinWarps));
+    if (many) {
+        const auto kernel = dp == 64 ? paged_join_many_kernel<64> : (dp == 128 ? paged_join_many_kernel<128> : paged_join_many_kernel<256>);
+        return run(kernel, rows, kManyWarps);
+    }
+    return run(dp == 64 ? paged_join_kernel<64> : (dp == 128 ? paged_join_kernel<128> : paged_join_kernel<256>), div_up(rows, kJoinWarps), kJoinWarps);
 }
 
 }  // namespace paged
@@ -851,10 +911,10 @@ int ogle_cuda_paged_attention(const OglePagedBatch* batch, const OgleAttentionPa
         if (e != cudaSuccess) { set_last_error(e); (void)cudaGetLastError(); return OGLE_ERR_CUDA; }
         int rc = finish_launch();
         if (rc != OGLE_OK) return rc;
-        // one warp to a row, or eight where few segments are cut into many parts
+        // a warp to a row, or sixteen where few segments are cut into many parts
         const long long rows = (long long)(a.b.max_rows < a.b.n_rows ? a.b.max_rows : a.b.n_rows) * a.b.group;
         const int tile = int(rows < F::kRows ? (rows < 1 ? 1 : rows) : F::kRows);
-        const bool many = ranges > 4 * segments;
+        const bool many = ranges > 8 * segments;
         return launch_join(a, DP, many, a.by_segment ? int(segments < 1 ? 1 : segments) : ranges, ranges, F::kRows, tile, stream);
     });
 }
