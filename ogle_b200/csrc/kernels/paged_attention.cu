@@ -609,7 +609,7 @@ paged_attention_kernel(AttnArgs a, const __grid_constant__ CUtensorMap k_map, co
 // (c, y) has segment c, or the one that begins in range c and goes on in the next; of its rows y, y + gridDim.y, ... a warp has one.
 constexpr int kJoinWarps = 8;
 template <int DP>
-__global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(AttnArgs a, int ranges, int rows_of_tile) {
+__global__ void __launch_bounds__(kJoinWarps * 32, 6) paged_join_kernel(AttnArgs a, int ranges, int rows_of_tile) {
     constexpr int kVecs = DP / 4, kPerLane = (kVecs + 31) / 32;
     const Batch& B = a.b;
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, c = blockIdx.x;
@@ -645,7 +645,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(AttnArgs a,
             }
 #pragma unroll
         for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-#pragma unroll 4
+#pragma unroll 2
         for (int k = cut.first; k < cut.last; ++k) {
             if (none(k)) continue;
             const float* p = part(k);

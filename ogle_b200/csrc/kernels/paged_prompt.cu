@@ -2,17 +2,18 @@
 //
 // A block has 256 rows (row of the sequence x query head of the group) of one sequence and kv head, as two tiles of 128, and goes
 // through the keys 128 at a time:
-//   one warp      brings a tile of keys and of values, as 8-bit boxes of 16 tokens of a page, and looks up their scales
-//   four warps    turn them into fp16 operands: e4m3 is exact in fp16, and a page's scale relative to the largest of the item is
-//                 a power of two that is multiplied in on the way (exact down to 2^-15 of the largest; what lies below is
-//                 rounded to 2^-33 of the largest value), so that scores and weights know nothing of pages
+//   four warps    read a tile of keys and of values ahead into registers and turn them into fp16 operands: e4m3 is exact in fp16, and
+//                 a page's scale relative to the largest of the item is a power of two that is multiplied in on the way (exact
+//                 down to 2^-15 of the largest; what lies below is rounded to 2^-33 of the largest value), so that scores and
+//                 weights know nothing of pages
 //   one thread    issues the products: S = Q K^T per tile, O += P V per tile, P taken from tensor memory
 //   2 x 4 warps   a row a thread: maximum, weights 2^(x - off), their sum; P in fp16 over S; O rescaled when a row's maximum
 //                 has grown by more than 2^8
-// A tile of keys is taken in two steps of 64. A tile of rows has two S of 64 columns in tensor memory (2 x 2 x 64, and 2 x DP
-// for O), so that the products of one step run while another is being weighted; P lies over its S, which is written again
-// once its P V is through. (With one S of 128 columns, scores, weights and sums of a tile came one after the other: 5000 cycles
-// a tile of keys where the products take 2048.)
+// While one tile of rows is being weighted, the other's products run. Weights are handed over in two steps of 64 keys, so that the
+// first sums run while the second half is being weighted. P lies over S in tensor memory (2 x 128 columns for S, 2 x DP for O), so
+// the next S of a tile of rows is asked for once its P V is through.
+// Shared memory has the products' operands to deliver beside the conversion's traffic; two S of 64 keys a tile of rows, which
+// overlap more, read the queries twice as often and were slower.
 //
 // Work: items (sequence, tile of 256 rows, kv head) laid end to end by their tiles of keys, cut into one range a block; parts
 // of items that were cut go to the workspace and are joined as in the form for few rows (paged_attention.cu). The ranges'
@@ -27,11 +28,11 @@ using namespace paged;
 constexpr int kKeys = 128;                       // of a tile
 constexpr int kStep = 64;                        // of a step: half a tile
 constexpr int kTileRows = 128, kItemRows = 2 * kTileRows;
-constexpr int kItemCost = 3;                     // tiles that an item's beginning and end take as long as
-constexpr int kThreads = 16 * 32;                // 8 warps of rows, 4 of conversion, copies, products, and two that fill up their group
-// Registers of a thread: a row has its 128 scores in them. (2 x 184 + 96 + 48) x 128 = the 128 of 512 threads at launch.
-constexpr int kRowRegisters = 184, kConvertRegisters = 96, kIssueRegisters = 48;
-constexpr int kConvertWarp = 8, kCopyWarp = 12, kProductWarp = 13;
+constexpr int kItemCost = 10;                    // tiles that an item's beginning and end take as long as
+constexpr int kThreads = 16 * 32;                // 8 warps of rows, 4 of conversion, one for products and three that fill up its group
+// Registers of a thread: a row has its 128 scores in them. (2 x 176 + 112 + 48) x 128 = the 128 of 512 threads at launch.
+constexpr int kRowRegisters = 176, kConvertRegisters = 112, kIssueRegisters = 48;
+constexpr int kConvertWarp = 8, kProductWarp = 12;
 constexpr int kNanKeys = 8192;                   // pieces of 16 values with a NaN that an item's edges can have: 1024 keys x 8
 
 // A piece of 16 values of a token at an item's edge: which of them are NaN.
@@ -52,9 +53,8 @@ template <int DP>
 struct Layout {
     static constexpr int kHalf = kTileRows * 128;                 // 64 elements of 128 rows
     static constexpr int kTile = DP / 64 * kHalf;                 // a tile of fp16
-    static constexpr int kBytes = kKeys * DP;                     // of e4m3
-    static constexpr int kQ = 0, kK = kQ + 2 * kTile, kV = kK + 2 * kTile, kStageK = kV + 2 * kTile, kStageV = kStageK + kBytes;
-    static constexpr int kSmem = kStageV + kBytes + 1024;
+    static constexpr int kQ = 0, kK = kQ + 2 * kTile, kV = kK + 2 * kTile;
+    static constexpr int kSmem = kV + 2 * kTile + 1024;
     static constexpr int kPart = kItemRows * (DP + 2);
     static constexpr int kO = 256;                                // first column of O in tensor memory
 };
@@ -110,11 +110,11 @@ __global__ void __launch_bounds__(1024) paged_plan_kernel(AttnArgs a, int max_ti
             }
             if (pass == 1 && mine > 0) {
                 const long long begin = before + sum - mine, end = begin + mine;
-                for (int k = int((begin * ranges + total - 1) / total); k < ranges; ++k) {
-                    const long long x = total * k / ranges;
+                for (int k = int(quotient(begin * ranges + total - 1, total)); k < ranges; ++k) {
+                    const long long x = quotient(total * k, ranges);
                     if (x >= end) break;
-                    if (x >= begin && (k == ranges - 1 || x != total * (k + 1) / ranges))   // the last of ranges that begin alike has the tiles
-                        starts[k] = Start{b, rt, int((x - begin) / cost), int((x - begin) % cost)};
+                    if (x >= begin && (k == ranges - 1 || x != quotient(total * (k + 1), ranges)))   // the last of ranges that begin alike has the tiles
+                        starts[k] = Start{b, rt, int(x - begin) / cost, int(x - begin) % cost};
                 }
             }
             before += all;
@@ -264,21 +264,14 @@ __device__ __forceinline__ void products_sums(uint32_t d, uint32_t a, uint64_t b
         ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
 
-// Where 16 bytes, `unit` of row r, of the copied e4m3 tile lie: boxes of 16 rows, as the copies' swizzle puts them.
-template <int DP>
-__device__ __forceinline__ int stage_at(int r, int unit) {
-    return DP == 64 ? r * 64 + (unit ^ ((r >> 1) & 3)) * 16 : r * 128 + (unit ^ (r & 7)) * 16;
-}
-
 struct Bars {
-    uint64_t k_came, k_taken, v_came, v_taken;   // the copied tiles
     uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
-    uint64_t q_full, s_full[2][2], p_full[2][2], pv_done[2][2], drain;   // [tile of rows][step & 1]
+    uint64_t q_full, s_full[2], p_full[2][2], pv_done[2][2], drain;      // [tile of rows][step of the tile of keys]
 };
 
 template <int DP>
 __global__ void __launch_bounds__(kThreads, 1)
-paged_prompt_kernel(PromptArgs p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
+paged_prompt_kernel(PromptArgs p) {
     using L = Layout<DP>;
     extern __shared__ __align__(16) unsigned char dynamic[];
     __shared__ __align__(8) Bars bars;
@@ -286,7 +279,6 @@ paged_prompt_kernel(PromptArgs p, const __grid_constant__ CUtensorMap k_map, con
     __shared__ Item item;
     __shared__ uint32_t tmem_slot, top_scale[2];   // bits of the item's largest scales of keys and values
     __shared__ float row_scale[2][kTileRows];      // 2^e that a row's queries were divided by
-    __shared__ float ratio[2][8];                  // scales of the copied tile's 16-token groups, against those
     __shared__ int more_items, holes, nan_count;
     __shared__ volatile int gave_up;
     unsigned char* const smem = dynamic + ((1024 - (tc::smem_u32(dynamic) & 1023)) & 1023);
@@ -295,14 +287,11 @@ paged_prompt_kernel(PromptArgs p, const __grid_constant__ CUtensorMap k_map, con
     const Batch& B = a.b;
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     if (tid == 0) {
-        tc::mbar_init(&bars.k_came, 1); tc::mbar_init(&bars.v_came, 1);
-        tc::mbar_init(&bars.k_taken, 4); tc::mbar_init(&bars.v_taken, 4);
         for (int i = 0; i < 2; ++i) {
             tc::mbar_init(&bars.k_full[i], 4); tc::mbar_init(&bars.v_full[i], 4);
             tc::mbar_init(&bars.k_empty[i], 1); tc::mbar_init(&bars.v_empty[i], 1);
-            for (int j = 0; j < 2; ++j) {
-                tc::mbar_init(&bars.s_full[i][j], 1); tc::mbar_init(&bars.p_full[i][j], 4); tc::mbar_init(&bars.pv_done[i][j], 1);
-            }
+            tc::mbar_init(&bars.s_full[i], 1);
+            for (int j = 0; j < 2; ++j) { tc::mbar_init(&bars.p_full[i][j], 4); tc::mbar_init(&bars.pv_done[i][j], 1); }
         }
         tc::mbar_init(&bars.q_full, 8);
         tc::mbar_init(&bars.drain, 1);
@@ -331,7 +320,7 @@ paged_prompt_kernel(PromptArgs p, const __grid_constant__ CUtensorMap k_map, con
     const uint32_t limit = a.spin_limit;
     volatile int* const abort = &gave_up;
     // tiles that this thread's role has been through, whatever item they were of
-    uint32_t kv_tiles = 0, q_items = 0, copies = 0, my_steps = 0, second_steps = 0;
+    uint32_t kv_tiles = 0, q_items = 0, my_tiles = 0, second_tiles = 0;
     bool failed = false;
     const auto wait = [&](uint64_t* bar, uint32_t parity) {
         if (!failed && !tc::wait_turn(bar, parity & 1, abort, limit)) {
@@ -388,7 +377,7 @@ paged_prompt_kernel(PromptArgs p, const __grid_constant__ CUtensorMap k_map, con
     if (warp < kConvertWarp) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRowRegisters));
         const int q = warp / 4, r = tid & 127;           // tile, row of it
-        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_at = tmem + lanes + q * 2 * kStep, o_at = tmem + lanes + L::kO + q * DP;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_at = tmem + lanes + q * kKeys, o_at = tmem + lanes + L::kO + q * DP;
         for (bool more = more_items != 0; more; more = end_item()) {
             begin_item();
             const int h = item.h;
@@ -397,8 +386,8 @@ paged_prompt_kernel(PromptArgs p, const __grid_constant__ CUtensorMap k_map, con
             const int seq_row = row / B.group, head = h * B.group + row % B.group;
             const Span k = span_of(item.s, seq_row, seq_row, a.causal, a.window);
             if (tiles > 0 && mine) {
-                // queries of the warp's 32 rows, 16 values a lane: rows side by side are read together, half of them before the first is used
-                constexpr int kLanes = DP / 16, kTogether = 32 / kLanes, kRounds = 32 / kTogether, kAtOnce = kRounds / 2;
+                // queries of the warp's 32 rows, 16 values a lane: rows side by side are read together, all of them before the first is used
+                constexpr int kLanes = DP / 16, kTogether = 32 / kLanes, kRounds = 32 / kTogether, kAtOnce = kRounds < 8 ? kRounds : 8;
                 const int d = lane % kLanes * 16;
                 const long long mine_at = (item.s.row0 + seq_row) * a.q_row + head * a.q_head;
                 const bool back = a.scale_log2 < 0.f;        // the largest product is then the largest x
@@ -446,27 +435,27 @@ paged_prompt_kernel(PromptArgs p, const __grid_constant__ CUtensorMap k_map, con
             const float rs = mine && tiles > 0 ? fmaxf(fabsf(a.scale_log2) * row_scale[q][r] * k_unit, 1e-37f) : 0.f;
 
             float off = 0.f, bar_x = -INFINITY, l = 0.f;
-            for (int u = 0; mine && u < 2 * tiles; ++u) {
-                const uint32_t turn = my_steps + u, sp_at = s_at + (turn & 1) * kStep;
-                wait(&bars.s_full[q][turn & 1], turn >> 1);
+            for (int t = 0; mine && t < tiles; ++t) {
+                wait(&bars.s_full[q], my_tiles + t);
                 if (__any_sync(~0u, failed)) { failed = true; break; }
                 after_sync();
-                const int j0 = j_first + u * kStep;
-                uint32_t s[2][32];
-                tmem_load32(s[0], sp_at);
-                tmem_load32(s[1], sp_at + 32);
-                tmem_loaded(s[0]);
-                tmem_loaded(s[1]);
-                if (with_holes || j0 < item.inner_lo || j0 + kStep > item.inner_hi) {
+                const int j0 = j_first + t * kKeys;
+                const bool edge = with_holes || j0 < item.inner_lo || j0 + kKeys > item.inner_hi;
+                uint32_t s[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_load32(s[c], s_at + c * 32);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_loaded(s[c]);
+                if (edge) {
                     // keys that the row does not attend
                     const int lo = k.lo - j0, hi = k.hi - j0;
 #pragma unroll
-                    for (int c = 0; c < 2; ++c)
+                    for (int c = 0; c < 4; ++c)
 #pragma unroll
                         for (int x = 0; x < 32; ++x) if (c * 32 + x < lo || c * 32 + x >= hi) s[c][x] = 0xff800000u;
                     if (with_holes) {
 #pragma unroll
-                        for (int g = 0; g < kStep / kChunk; ++g) {
+                        for (int g = 0; g < kKeys / kChunk; ++g) {
                             const int j = j0 + g * kChunk;
                             if (j < item.keys.hi && page_of(B, item.b, j >> B.page_shift) < 0)
 #pragma unroll
@@ -477,9 +466,9 @@ paged_prompt_kernel(PromptArgs p, const __grid_constant__ CUtensorMap k_map, con
                 float m[4];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    m[c] = __uint_as_float(s[c / 2][c % 2 * 16]);
+                    m[c] = __uint_as_float(s[c][0]);
 #pragma unroll
-                    for (int x = 1; x < 16; ++x) m[c] = fmaxf(m[c], __uint_as_float(s[c / 2][c % 2 * 16 + x]));
+                    for (int x = 1; x < 32; ++x) m[c] = fmaxf(m[c], __uint_as_float(s[c][x]));
                 }
                 const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * rs;
                 if (__any_sync(~0u, top > bar_x)) {
@@ -491,10 +480,7 @@ paged_prompt_kernel(PromptArgs p, const __grid_constant__ CUtensorMap k_map, con
                         bar_x = now + kHeadroom;
                     }
                     l *= f;
-                    if (u > 0) {
-                        wait(&bars.pv_done[q][(turn - 1) & 1], (turn - 1) >> 1);
-                        if (__any_sync(~0u, failed)) { failed = true; break; }
-                        after_sync();
+                    if (t > 0) {
 #pragma unroll 1
                         for (int c = 0; c < DP / 16; ++c) {
                             uint32_t o[16];
@@ -508,7 +494,7 @@ paged_prompt_kernel(PromptArgs p, const __grid_constant__ CUtensorMap k_map, con
                 const unsigned long long rs2 = pair(rs, rs), off2 = pair(-off, -off);
                 unsigned long long sum[2] = {0, 0};
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
+                for (int c = 0; c < 4; ++c) {
                     uint32_t w[16];
 #pragma unroll
                     for (int x = 0; x < 32; x += 2) {
@@ -519,19 +505,20 @@ paged_prompt_kernel(PromptArgs p, const __grid_constant__ CUtensorMap k_map, con
                         sum[x / 2 & 1] = add2(sum[x / 2 & 1], pair(e, f));
                         w[x / 2] = half2_bits(e, f);
                     }
-                    tc::tmem_st16(sp_at + c * 16, w);          // over scores, all of which have been read
+                    tc::tmem_st16(s_at + c / 2 * kStep + c % 2 * 16, w);          // over scores, all of which have been read
+                    if (c & 1) {                          // a step's weights
+                        tmem_stored();
+                        before_sync();
+                        __syncwarp();
+                        if (lane == 0) tc::mbar_arrive(&bars.p_full[q][c / 2]);
+                    }
                 }
                 float e, f;
                 unpair(add2(sum[0], sum[1]), e, f);
                 l += e + f;
-                tmem_stored();
-                before_sync();
-                __syncwarp();
-                if (lane == 0) tc::mbar_arrive(&bars.p_full[q][turn & 1]);
             }
             if (mine && tiles > 0) {
-                const uint32_t turn = my_steps + 2 * tiles - 1;
-                wait(&bars.pv_done[q][turn & 1], turn >> 1);
+                wait(&bars.pv_done[q][1], my_tiles + tiles - 1);
                 if (__any_sync(~0u, failed)) failed = true;
                 after_sync();
             }
@@ -610,71 +597,106 @@ paged_prompt_kernel(PromptArgs p, const __grid_constant__ CUtensorMap k_map, con
                     part[kItemRows] = l;
                 }
             }
-            if (mine) my_steps += 2 * tiles;
+            if (mine) my_tiles += tiles;
         }
-    } else if (warp < kCopyWarp) {
+    } else if (warp < kProductWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvertRegisters));
-        // a piece is 16 values of a token; eight lanes that store together have two tokens' four pieces: different banks
+        // a piece is 16 values of a token; eight lanes that store together have two tokens' four pieces: different banks. A warp has 32
+        // tokens of a tile: two groups of 16, each in one page
+        constexpr int kHalves = DP / 64, kRounds = 4;
         const int piece = lane & 3, row8 = lane >> 2, cw = warp - kConvertWarp;
         for (bool more = more_items != 0; more; more = end_item()) {
             begin_item();
-            for (int t = 0; t < tiles && !failed; ++t) {
+            const int h = item.h, in_page = (1 << B.page_shift) - 1;
+            int page[2];                           // of the tile whose values are asked for next
+            float rk[2], rv[2];                    // scales of the tile that has been asked for, against the largest
+            uint4 k_raw[kRounds][kHalves], v_raw[kRounds][kHalves];
+            const auto look_up = [&](int t) {
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    const int j = j_first + t * kKeys + cw * 32 + g * kChunk;
+                    page[g] = t < tiles && j < item.keys.hi ? page_of(B, item.b, j >> B.page_shift) : -1;
+                }
+            };
+            const auto ask = [&](int t, const unsigned char* cache, const float* scales, float unit, uint4 (&raw)[kRounds][kHalves], float (&ratio)[2]) {
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    ratio[g] = 0.f;
+                    const int slot = (j_first + t * kKeys + cw * 32 + g * kChunk) & in_page;
+                    const unsigned char* from = cache + (long long)page[g] * B.page_stride + h * B.head_stride + (long long)(slot + row8) * B.token_stride + piece * 16;
+                    if (page[g] >= 0) ratio[g] = __ldg(scales + (long long)page[g] * B.kv_heads + h) / unit;
+#pragma unroll
+                    for (int x = 0; x < 2; ++x)
+#pragma unroll
+                        for (int half = 0; half < kHalves; ++half) {
+                            raw[g * 2 + x][half] = make_uint4(0, 0, 0, 0);
+                            if (page[g] >= 0 && half * 64 + piece * 16 < B.dim)
+                                raw[g * 2 + x][half] = __ldg(reinterpret_cast<const uint4*>(from + x * 8 * B.token_stride + half * 64));
+                        }
+                }
+            };
+            const auto store = [&](int j0, bool clean, unsigned char* to, const uint4 (&raw)[kRounds][kHalves], const float (&ratio)[2]) {
+#pragma unroll
+                for (int x = 0; x < kRounds; ++x) {
+                    const int r = cw * 32 + x * 8 + row8;
+                    const __half2 f = __float2half2_rn(ratio[x / 2]);
+#pragma unroll
+                    for (int half = 0; half < kHalves; ++half) {
+                        uint32_t y[8];
+                        const uint32_t w[4] = {raw[x][half].x, raw[x][half].y, raw[x][half].z, raw[x][half].w};
+#pragma unroll
+                        for (int z = 0; z < 4; ++z) e4m3x4_to_half2(w[z], y[2 * z], y[2 * z + 1]);
+                        if (clean) {
+                            // a NaN of a token that some row does not attend: out of the operand, its rows get it at the end
+                            uint32_t bits = 0;
+#pragma unroll
+                            for (int z = 0; z < 8; ++z) {
+                                const __half2 g = *reinterpret_cast<const __half2*>(&y[z]);
+                                const uint32_t n = __hneu2_mask(g, g);
+                                y[z] &= ~n;
+                                bits |= ((n & 1) | (n >> 30 & 2)) << (2 * z);
+                            }
+                            const int key = j0 + r;
+                            if (bits && key >= item.keys.lo && key < item.keys.hi) {
+                                const int at = atomicAdd(&nan_count, 1);
+                                if (at < kNanKeys) p.nans[(long long)blockIdx.x * kNanKeys + at] = NanPiece{key, uint16_t(bits), uint16_t(half * 4 + piece)};
+                            }
+                        }
+#pragma unroll
+                        for (int z = 0; z < 8; ++z) {
+                            const __half2 g = __hmul2(*reinterpret_cast<const __half2*>(&y[z]), f);
+                            y[z] = *reinterpret_cast<const uint32_t*>(&g);
+                        }
+                        unsigned char* row = to + half * L::kHalf + r * 128;
+                        *reinterpret_cast<uint4*>(row + ((2 * piece) ^ (r & 7)) * 16) = make_uint4(y[0], y[1], y[2], y[3]);
+                        *reinterpret_cast<uint4*>(row + ((2 * piece + 1) ^ (r & 7)) * 16) = make_uint4(y[4], y[5], y[6], y[7]);
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+            };
+            if (tiles > 0) {
+                look_up(0);
+                ask(0, B.k_cache, B.k_scale, k_unit, k_raw, rk);
+                ask(0, B.v_cache, B.v_scale, v_unit, v_raw, rv);
+                look_up(1);
+            }
+            for (int t = 0; t < tiles; ++t) {
                 const uint32_t st = kv_tiles & 1, use = kv_tiles >> 1;
                 const int j0 = j_first + t * kKeys;
                 const bool edge = j0 < item.inner_lo || j0 + kKeys > item.inner_hi;
-#pragma unroll 1
-                for (int v = 0; v < 2; ++v) {
-                    wait(v ? &bars.v_came : &bars.k_came, kv_tiles);
-                    wait(v ? &bars.v_empty[st] : &bars.k_empty[st], use + 1);
-                    if (__any_sync(~0u, failed)) { failed = true; break; }
-                    const unsigned char* from = smem + (v ? L::kStageV : L::kStageK);
-                    unsigned char* to = smem + (v ? L::kV : L::kK) + st * L::kTile;
-#pragma unroll 2
-                    for (int x = 0; x < kKeys / 32; ++x) {
-                        const int r = cw * 32 + x * 8 + row8;
-                        const __half2 f = __float2half2_rn(ratio[v][r / kChunk]);
-                        uint4 in[DP / 64];
-#pragma unroll
-                        for (int half = 0; half < DP / 64; ++half) in[half] = *reinterpret_cast<const uint4*>(from + stage_at<DP>(r, half * 4 + piece));
-#pragma unroll
-                        for (int half = 0; half < DP / 64; ++half) {
-                            uint32_t y[8];
-                            const uint32_t w[4] = {in[half].x, in[half].y, in[half].z, in[half].w};
-#pragma unroll
-                            for (int z = 0; z < 4; ++z) e4m3x4_to_half2(w[z], y[2 * z], y[2 * z + 1]);
-                            if (v && edge) {
-                                // a NaN of a token that some row does not attend: out of the operand, its rows get it at the end
-                                uint32_t bits = 0;
-#pragma unroll
-                                for (int z = 0; z < 8; ++z) {
-                                    const __half2 g = *reinterpret_cast<const __half2*>(&y[z]);
-                                    const uint32_t n = __hneu2_mask(g, g);
-                                    y[z] &= ~n;
-                                    bits |= ((n & 1) | (n >> 30 & 2)) << (2 * z);
-                                }
-                                const int key = j0 + r;
-                                if (bits && key >= item.keys.lo && key < item.keys.hi) {
-                                    const int at = atomicAdd(&nan_count, 1);
-                                    if (at < kNanKeys) p.nans[(long long)blockIdx.x * kNanKeys + at] = NanPiece{key, uint16_t(bits), uint16_t(half * 4 + piece)};
-                                }
-                            }
-#pragma unroll
-                            for (int z = 0; z < 8; ++z) {
-                                const __half2 g = __hmul2(*reinterpret_cast<const __half2*>(&y[z]), f);
-                                y[z] = *reinterpret_cast<const uint32_t*>(&g);
-                            }
-                            unsigned char* row = to + half * L::kHalf + r * 128;
-                            *reinterpret_cast<uint4*>(row + ((2 * piece) ^ (r & 7)) * 16) = make_uint4(y[0], y[1], y[2], y[3]);
-                            *reinterpret_cast<uint4*>(row + ((2 * piece + 1) ^ (r & 7)) * 16) = make_uint4(y[4], y[5], y[6], y[7]);
-                        }
-                    }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) {
-                        tc::mbar_arrive(v ? &bars.v_full[st] : &bars.k_full[st]);
-                        tc::mbar_arrive(v ? &bars.v_taken : &bars.k_taken);
-                    }
-                }
+                wait(&bars.k_empty[st], use + 1);
+                if (__any_sync(~0u, failed)) { failed = true; break; }
+                store(j0, false, smem + L::kK + st * L::kTile, k_raw, rk);
+                if (lane == 0) tc::mbar_arrive(&bars.k_full[st]);
+                ask(t + 1, B.k_cache, B.k_scale, k_unit, k_raw, rk);
+                wait(&bars.v_empty[st], use + 1);
+                if (__any_sync(~0u, failed)) { failed = true; break; }
+                if (edge) store(j0, true, smem + L::kV + st * L::kTile, v_raw, rv);
+                else store(j0, false, smem + L::kV + st * L::kTile, v_raw, rv);
+                if (lane == 0) tc::mbar_arrive(&bars.v_full[st]);
+                ask(t + 1, B.v_cache, B.v_scale, v_unit, v_raw, rv);
+                look_up(t + 2);
                 ++kv_tiles;
             }
             asm volatile("bar.sync 1, 384;" ::: "memory");
@@ -683,88 +705,47 @@ paged_prompt_kernel(PromptArgs p, const __grid_constant__ CUtensorMap k_map, con
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegisters));
         for (bool more = more_items != 0; more; more = end_item()) {
             begin_item();
-            const int h = item.h;
-            if (warp == kCopyWarp) {
-                // lane g has the 16 tokens of group g
-                const int nowhere = max(B.n_pages, 1), in_page = (1 << B.page_shift) - 1;
-                const auto look_up = [&](int t, int& page, float& rk, float& rv) {
-                    const int j = j_first + t * kKeys + (lane & 7) * kChunk;
-                    page = nowhere;
-                    rk = rv = 0.f;
-                    if (t >= tiles || j >= item.keys.hi) return;
-                    const int x = page_of(B, item.b, j >> B.page_shift);
-                    if (x < 0) return;
-                    page = x;
-                    const long long o = (long long)x * B.kv_heads + h;
-                    rk = __ldg(B.k_scale + o) / k_unit;
-                    rv = __ldg(B.v_scale + o) / v_unit;
-                };
-                int page;
-                float rk, rv;
-                look_up(0, page, rk, rv);
-                for (int t = 0; t < tiles && !failed; ++t) {
-                    const int token = (j_first + t * kKeys + (lane & 7) * kChunk) & in_page, now = page;
-                    const float now_k = rk, now_v = rv;
-                    look_up(t + 1, page, rk, rv);
-    #pragma unroll
-                    for (int v = 0; v < 2; ++v) {
-                        uint64_t* const came = v ? &bars.v_came : &bars.k_came;
-                        const bool free = wait(v ? &bars.v_taken : &bars.k_taken, kv_tiles + 1);
-                        if (__any_sync(~0u, !free)) { failed = true; break; }
-                        if (lane < 8) ratio[v][lane] = v ? now_v : now_k;
-                        __syncwarp();
-                        if (lane == 0) tc::mbar_expect_tx(came, L::kBytes);
-                        __syncwarp();
-                        if (lane < 8) copy_box(base + (v ? L::kStageV : L::kStageK) + lane * kChunk * DP, v ? &v_map : &k_map, tc::smem_u32(came), 0, token, h, now);
-                        copies = kv_tiles * 2 + v + 1;
-                    }
-                    ++kv_tiles;
-                }
-            } else if (warp == kProductWarp) {
+            if (warp == kProductWarp) {
                 if (tiles > 0 && tc::elect_one()) {
                     constexpr uint32_t kF16 = (1u << 4) | ((uint32_t)(kTileRows >> 4) << 24);     // fp16 x fp16 into fp32, 128 rows
-                    constexpr uint32_t kScores = kF16 | ((uint32_t)(kStep >> 3) << 17);
+                    constexpr uint32_t kScores = kF16 | ((uint32_t)(kKeys >> 3) << 17);
                     constexpr uint32_t kSums = kF16 | (1u << 16) | ((uint32_t)(DP >> 3) << 17);   // values: elements side by side
-                    const int steps = 2 * tiles;
-                    const auto turn_of = [&](int q, int u) { return (q ? second_steps : my_steps) + u; };
-                    const auto scores = [&](int q, int u) {     // S = Q K^T of step u
-                        const uint32_t turn = turn_of(q, u), tile = kv_tiles + u / 2;
-                        const uint64_t qd = tc::umma_desc(base + L::kQ + q * L::kTile), kd = tc::umma_desc(base + L::kK + (tile & 1) * L::kTile + (u & 1) * kStep * 128);
+                    const auto scores = [&](int q, int t) {     // S = Q K^T of tile t
+                        const uint64_t qd = tc::umma_desc(base + L::kQ + q * L::kTile), kd = tc::umma_desc(base + L::kK + ((kv_tiles + t) & 1) * L::kTile);
 #pragma unroll
-                        for (int k = 0; k < DP / 64; ++k)
-                            products_scores(tmem + (q * 2 + (turn & 1)) * kStep, qd + k * (L::kHalf >> 4), kd + k * (L::kHalf >> 4), kScores, k);
-                        tc::umma_commit(&bars.s_full[q][turn & 1]);
+                        for (int k = 0; k < DP / 64; ++k) products_scores(tmem + q * kKeys, qd + k * (L::kHalf >> 4), kd + k * (L::kHalf >> 4), kScores, k);
+                        tc::umma_commit(&bars.s_full[q]);
+                    };
+                    const auto sums = [&](int q, int t, int step) {     // O += P V of a step of tile t; false: its weights did not come
+                        if (!wait(&bars.p_full[q][step], (q ? second_tiles : my_tiles) + t)) return false;
+                        after_sync();
+                        products_sums(tmem + L::kO + q * DP, tmem + q * kKeys + step * kStep, desc_mn(base + L::kV + ((kv_tiles + t) & 1) * L::kTile + step * kStep * 128, L::kHalf),
+                                      kSums, t + step);
+                        tc::umma_commit(&bars.pv_done[q][step]);
+                        return true;
+                    };
+                    const auto next = [&](int q, int t) {               // the next S of a tile of rows lies where its P is read
+                        if (!wait(&bars.pv_done[q][1], (q ? second_tiles : my_tiles) + t)) return false;
+                        after_sync();
+                        scores(q, t + 1);
+                        return true;
                     };
                     bool ok = wait(&bars.q_full, q_items) && wait(&bars.k_full[kv_tiles & 1], kv_tiles >> 1);
                     if (ok) {
                         after_sync();
-                        for (int u = 0; u < 2; ++u)
-                            for (int q = 0; q < halves; ++q) scores(q, u);
+                        for (int q = 0; q < halves; ++q) scores(q, 0);
                         tc::umma_commit(&bars.k_empty[kv_tiles & 1]);
                     }
-                    for (int u = 0; ok && u < steps; ++u) {
-                        const uint32_t now = kv_tiles + u / 2;      // tile of the step's values; the keys asked for are of the next
-                        if ((u & 1) == 0) ok = wait(&bars.v_full[now & 1], now >> 1);
-                        const uint32_t vbase = base + L::kV + (now & 1) * L::kTile + (u & 1) * kStep * 128;
-                        for (int q = 0; ok && q < halves; ++q) {
-                            const uint32_t turn = turn_of(q, u);
-                            ok = wait(&bars.p_full[q][turn & 1], turn >> 1);
-                            if (!ok) break;
-                            after_sync();
-                            products_sums(tmem + L::kO + q * DP, tmem + (q * 2 + (turn & 1)) * kStep, desc_mn(vbase, L::kHalf), kSums, u);
-                            tc::umma_commit(&bars.pv_done[q][turn & 1]);
+                    for (int t = 0; ok && t < tiles; ++t) {
+                        const uint32_t now = kv_tiles + t;
+                        const bool last = t + 1 == tiles;
+                        ok = wait(&bars.v_full[now & 1], now >> 1) && sums(0, t, 0) && sums(0, t, 1);
+                        if (ok && !last) ok = wait(&bars.k_full[(now + 1) & 1], (now + 1) >> 1) && next(0, t);
+                        if (ok && halves == 2) ok = sums(1, t, 0) && sums(1, t, 1) && (last || next(1, t));
+                        if (ok) {
+                            tc::umma_commit(&bars.v_empty[now & 1]);
+                            if (!last) tc::umma_commit(&bars.k_empty[(now + 1) & 1]);
                         }
-                        if (ok && (u & 1)) tc::umma_commit(&bars.v_empty[now & 1]);
-                        if (!ok || u + 2 >= steps) continue;
-                        if ((u & 1) == 0) ok = wait(&bars.k_full[(now + 1) & 1], (now + 1) >> 1);
-                        for (int q = 0; ok && q < halves; ++q) {
-                            const uint32_t turn = turn_of(q, u);
-                            ok = wait(&bars.pv_done[q][turn & 1], turn >> 1);     // P lies where the S will
-                            if (!ok) break;
-                            after_sync();
-                            scores(q, u + 2);
-                        }
-                        if (ok && (u & 1)) tc::umma_commit(&bars.k_empty[(now + 1) & 1]);
                     }
                     if (!ok) {                                  // products under way end before tensor memory is given back
                         tc::umma_commit(&bars.drain);
@@ -773,17 +754,11 @@ paged_prompt_kernel(PromptArgs p, const __grid_constant__ CUtensorMap k_map, con
                 }
                 __syncwarp();
                 kv_tiles += tiles;
-                my_steps += 2 * tiles;
-                if (halves == 2) second_steps += 2 * tiles;
+                my_tiles += tiles;
+                if (halves == 2) second_tiles += tiles;
                 if (tiles > 0) ++q_items;
             }
         }
-    }
-    // a copy that nobody has waited for lands before the block ends
-    if (warp == kCopyWarp && gave_up && copies > 0) {
-        const uint32_t last = copies - 1;                    // copy `last`: keys and values in turn
-        tc::mbar_wait(last & 1 ? &bars.v_came : &bars.k_came, (last >> 1) & 1);
-        if (last > 0) tc::mbar_wait(last & 1 ? &bars.k_came : &bars.v_came, ((last - 1) >> 1) & 1);
     }
     before_sync();
     __syncthreads();
@@ -819,16 +794,11 @@ int launch_form(const OglePagedBatch* b, PromptArgs p, void* workspace, cudaStre
         e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
         if (e == cudaSuccess) sized.fetch_or(1ull << (device & 63), std::memory_order_relaxed);
     }
-    CUtensorMap k_map, v_map;
-    if (e == cudaSuccess && (!cache_map(&k_map, p.a.b, p.a.b.k_cache, DP) || !cache_map(&v_map, p.a.b, p.a.b.v_cache, DP))) {
-        set_last_error("paged_attention: no tensor map of the cache");
-        return OGLE_ERR_CUDA;
-    }
     if (e == cudaSuccess) e = launch_overlapped(paged_plan_kernel, dim3(1), dim3(1024), 0, stream, p.a, p.max_tiles, ranges, plan, starts);
     if (e != cudaSuccess) { set_last_error(e); (void)cudaGetLastError(); return OGLE_ERR_CUDA; }
     int rc = finish_launch();
     if (rc != OGLE_OK) return rc;
-    e = launch_overlapped_if(overlapped_launches_enabled(true), kernel, dim3(ranges), dim3(kThreads), L::kSmem, stream, p, k_map, v_map);
+    e = launch_overlapped_if(overlapped_launches_enabled(true), kernel, dim3(ranges), dim3(kThreads), L::kSmem, stream, p);
     if (e != cudaSuccess) { set_last_error(e); (void)cudaGetLastError(); return OGLE_ERR_CUDA; }
     rc = finish_launch();
     if (rc != OGLE_OK) return rc;
