@@ -8,6 +8,8 @@
 // Work: a segment is a tile of kRows rows (row of the sequence x query head of the group) of one sequence and kv head. All
 // segments' tiles of 64 keys, laid end to end, are cut into equal ranges, one for each block, whatever the sequences' lengths are. A segment
 // inside a block's range is finished there; parts of others go to the workspace, and paged_join_kernel adds them in order.
+// Where there are few segments, none of them long, the blocks of a cluster have one segment instead and add their parts
+// through each other's shared memory: one launch, no workspace.
 //
 // The products run on 16-bit operands: an e4m3 value is an fp16 exactly; queries are scaled by a power of two so that their
 // largest lies below 2^12 (11 bits of each, or 22 as two parts), weights lie below 2^15. kSplit keeps queries and weights as
@@ -197,9 +199,76 @@ __device__ __forceinline__ bool next_segment(const AttnArgs& a, Walk& w, Segment
     return false;
 }
 
+// One thread: the cluster's segment, and this block's share of its tiles; false where there is no such tile of rows.
+template <int kRows>
+__device__ __forceinline__ bool cluster_segment(const AttnArgs& a, Segment& g) {
+    const Batch& B = a.b;
+    const int c = blockIdx.x / a.cluster, rank = blockIdx.x % a.cluster, rt = c % a.by_segment;
+    g.b = c / (a.by_segment * B.kv_heads);
+    g.h = c / a.by_segment % B.kv_heads;
+    g.s = few_sequence(a, g.b);
+    g.m0 = rt * kRows;
+    if (g.m0 >= g.s.n * B.group) return false;
+    g.m_end = min(g.s.n * B.group, g.m0 + kRows);
+    const int first_row = g.m0 / B.group, last_row = (g.m_end - 1) / B.group;
+    g.keys = span_of(g.s, first_row, last_row, a.causal, a.window);
+    g.inner_lo = span_of(g.s, last_row, 0, a.causal, a.window).lo;
+    g.inner_hi = span_of(g.s, 0, first_row, a.causal, a.window).hi;
+    const int lo = g.keys.lo & ~(kChunk - 1), chunks = g.keys.hi > lo ? (g.keys.hi - lo + kChunk - 1) / kChunk : 0;
+    const int c0 = chunks * rank / a.cluster, c1 = chunks * (rank + 1) / a.cluster;
+    g.j_begin = lo + c0 * kChunk;
+    g.steps = c1 - c0;
+    g.c0 = g.c1 = g.cost = 0;
+    return true;
+}
+
+__device__ __forceinline__ float4 remote_load4(uint32_t addr, int rank) {
+    uint32_t r;
+    float4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(r) : "memory");
+    return v;
+}
+__device__ __forceinline__ float2 remote_load2(uint32_t addr, int rank) {
+    uint32_t r;
+    float2 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(r) : "memory");
+    return v;
+}
+__device__ __forceinline__ void cluster_meet() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+
+// Each block of the cluster has every so-many-th row and adds the blocks' parts in their order.
+template <int DP>
+__device__ __noinline__ void cluster_join(const AttnArgs& a, const Segment& g, const unsigned char* parts, const float2* sums, int rows) {
+    const int size = a.cluster, rank = blockIdx.x % size;
+#pragma unroll 1
+    for (int idx = threadIdx.x; idx < rows * (DP / 4); idx += kWarps * 32) {
+        const int r = idx / (DP / 4), d = idx % (DP / 4) * 4, row = g.m0 + r;
+        if (row >= g.m_end || r % size != rank) continue;
+        float top = -INFINITY, sum = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k = 0; k < size; ++k) {
+            const float2 q = remote_load2(tc::smem_u32(sums + r), k);
+            if (q.y != 0.f) top = fmaxf(top, q.x);
+        }
+        for (int k = 0; k < size; ++k) {
+            const float2 q = remote_load2(tc::smem_u32(sums + r), k);
+            if (q.y == 0.f) continue;
+            const float f = exp2_fast(q.x - top);
+            const float4 o = remote_load4(tc::smem_u32(parts) + (r * (DP + 4) + d) * 4, k);
+            sum += q.y * f;
+            v.x += o.x * f; v.y += o.y * f; v.z += o.z * f; v.w += o.w * f;
+        }
+        store_row(a, g.s.row0 + row / a.b.group, g.h * a.b.group + row % a.b.group, d, v, top, sum);
+    }
+}
+
 template <int DP, int MT, bool kSplit>
 __global__ void __launch_bounds__(kWarps * 32, (Form<DP, MT, kSplit>::kBlocks))
-paged_attention_kernel(AttnArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
+paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
     using F = Form<DP, MT, kSplit>;
     constexpr int kRows = F::kRows, NR = kSplit ? 1 : 2, KS = DP / 16, NB = DP / 8;
     extern __shared__ __align__(16) unsigned char dynamic[];
@@ -207,6 +276,7 @@ paged_attention_kernel(AttnArgs a, const __grid_constant__ CUtensorMap k_map, co
     __shared__ __align__(8) uint64_t bars[kWarps][F::kStages];
     __shared__ int gave_up, more_segments;
     __shared__ float row_scale[kRows];
+    __shared__ __align__(8) float2 block_sum[kRows];      // cluster: m and sum of weights of a row in this block
     __shared__ Walk walk;
     __shared__ Segment segment;
     unsigned char* const smem = dynamic + ((1024 - (tc::smem_u32(dynamic) & 1023)) & 1023);
@@ -219,13 +289,19 @@ paged_attention_kernel(AttnArgs a, const __grid_constant__ CUtensorMap k_map, co
     }
     grid_dependency_trigger();
     grid_dependency_wait();
-    const Place place = locate(a, kRows, blockIdx.x, gridDim.x, shared);    // its barriers: `bars` is set up
-    if (tid == 0) {
-        if (!a.by_segment) a.cuts[blockIdx.x].rows = 0;
-        walk = Walk{quotient(place.total * blockIdx.x, gridDim.x), place.first, quotient(place.total * (blockIdx.x + 1), gridDim.x), place.total, place.b, place.cost};
-        more_segments = place.b >= 0 && next_segment<kRows>(a, walk, segment);
+    if (a.cluster) {
+        if (tid == 0) more_segments = cluster_segment<kRows>(a, segment);
+        __syncthreads();
+        if (!more_segments) return;
+    } else {
+        const Place place = locate(a, kRows, blockIdx.x, gridDim.x, shared);
+        if (tid == 0) {
+            if (!a.by_segment) a.cuts[blockIdx.x].rows = 0;
+            walk = Walk{quotient(place.total * blockIdx.x, gridDim.x), place.first, quotient(place.total * (blockIdx.x + 1), gridDim.x), place.total, place.b, place.cost};
+            more_segments = place.b >= 0 && next_segment<kRows>(a, walk, segment);
+        }
+        __syncthreads();
     }
-    __syncthreads();
     const unsigned char* const my_ring = smem + warp * F::kStages * F::kStageBytes;
     const uint32_t ring = tc::smem_u32(my_ring), bar0 = tc::smem_u32(&bars[warp][0]);
     const int nowhere = max(B.n_pages, 1);
@@ -542,7 +618,7 @@ paged_attention_kernel(AttnArgs a, const __grid_constant__ CUtensorMap k_map, co
             if (n < count) issue(n, (n ^ i) >> 5 ? p1 : p0);
         }
         __syncthreads();                          // every warp is through with its ring: the parts take its place
-        if (gave_up) return;
+        if (gave_up && !a.cluster) return;
 
         // the warps' parts: values [kRows][DP + 4], then m and l
         float* const mine = reinterpret_cast<float*>(smem) + warp * kRows * (DP + 4);
@@ -590,12 +666,23 @@ paged_attention_kernel(AttnArgs a, const __grid_constant__ CUtensorMap k_map, co
                 sum += q[DP + 1] * f;
                 v.x += o.x * f; v.y += o.y * f; v.z += o.z * f; v.w += o.w * f;
             }
+            if (a.cluster) {                      // where the first warp's were: no other thread reads them
+                *reinterpret_cast<float4*>(smem + (r * (DP + 4) + d) * 4) = v;
+                if (d == 0) block_sum[r] = make_float2(top, sum);
+                continue;
+            }
             if (!whole) {
                 *reinterpret_cast<float4*>(part + r * DP + d) = v;
                 if (d == 0) { part[kRows * DP + r] = top; part[kRows * DP + kRows + r] = sum; }
                 continue;
             }
             store_row(a, segment.s.row0 + row / B.group, segment.h * B.group + row % B.group, d, v, top, sum);
+        }
+        if (a.cluster) {
+            cluster_meet();
+            if (!gave_up) cluster_join<DP>(a, segment, smem, block_sum, kRows);
+            cluster_meet();                       // nobody reads this block's part any more
+            return;
         }
         // the next segment's copies take the parts' place
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -789,6 +876,26 @@ auto with_form(const Choice& c, G g) {
                    : g(std::integral_constant<int, 256>(), std::integral_constant<int, 1>(), std::false_type());
 }
 
+// Tiles of rows that a sequence can have in this form, and segments of the whole call.
+long long row_tiles_of(const OglePagedBatch* b, int rows) {
+    long long most = (long long)(b->max_rows < b->n_rows ? b->max_rows : b->n_rows) * (b->q_heads / b->kv_heads);
+    if (few_limit(b) && most > kFewRows) most = kFewRows;
+    return (most + rows - 1) / rows;
+}
+// Blocks of a cluster that has one segment, or 0: ranges. A call over clusters saves the second launch and the search for ranges, about
+// 3 us, but takes as long as the longest sequence's share, and blocks that the clusters do not use stay idle. us over ranges / clusters,
+// one query row each, 32 query heads to 8 of 128 elements: one sequence of 700 tokens 10.8 / 9.4, of 4000 13.6 / 13.6, of 8000 15.1 /
+// 19.8; 4 of 2000 14.7 / 11.7, of 8000 23.1 / 22.7, of 16000 33.4 / 38.9; 16 of up to 4000 35.7 / 23.9, of up to 8000 35.4 / 38.2.
+// So the tiles of 64 keys that pay a block go from 6, where few blocks of the GPU are used, to about 30, where all are.
+int cluster_of(const OglePagedBatch* b, const OgleAttentionParams* p, int rows, int blocks) {
+    const long long segments = row_tiles_of(b, rows) * b->n_seqs * b->kv_heads, slots = kNumSMs * blocks;
+    if (segments < 1 || segments * 2 > slots) return 0;
+    const long long size = slots / segments < 8 ? slots / segments : 8;
+    long long keys = b->max_kv_len;
+    if (p->window > 0 && keys > (long long)p->window + b->max_rows) keys = (long long)p->window + b->max_rows;
+    return keys <= kTileKeys * size * (6 + 25 * segments * size / slots) ? int(size) : 0;
+}
+
 // Ranges: as many blocks as fit the GPU at once, and no more than there can be tiles.
 int ranges_of(const OglePagedBatch* b, int rows, int blocks) {
     const long long max_rows = b->max_rows < b->n_rows ? b->max_rows : b->n_rows;
@@ -807,10 +914,11 @@ int few_limit(const OglePagedBatch* b) {
 // Whether some sequence can have few rows, as far as the host knows.
 bool some_few(const OglePagedBatch* b) { return !few_limit(b) || (long long)b->n_seqs * b->max_rows != b->n_rows; }
 
-size_t few_workspace(const OglePagedBatch* b) {
+size_t few_workspace(const OglePagedBatch* b, const OgleAttentionParams* p) {
     if (!some_few(b)) return 0;
     return with_form(choose(b), [&](auto dp, auto mt, auto split) {
         using F = Form<decltype(dp)::value, decltype(mt)::value, decltype(split)::value>;
+        if (cluster_of(b, p, F::kRows, F::kBlocks)) return sizeof(Cut);   // not read: a caller without a workspace finds out at every size
         return size_t(ranges_of(b, F::kRows, F::kBlocks)) * (2 * F::kPart * sizeof(float) + sizeof(Cut));
     });
 }
@@ -857,7 +965,7 @@ size_t ogle_cuda_paged_attention_workspace_bytes(const OglePagedBatch* batch, co
     Batch b;
     if (!p || paged::translate(batch, b) != OGLE_OK || b.n_seqs == 0) return 0;
     // the forms run one after the other: what one has left there the other may overwrite
-    const size_t few = few_workspace(batch), prompts = few_limit(batch) ? prompt_workspace(batch) : 0;
+    const size_t few = few_workspace(batch, p), prompts = few_limit(batch) ? prompt_workspace(batch) : 0;
     return few > prompts ? few : prompts;
 }
 
@@ -891,9 +999,9 @@ int ogle_cuda_paged_attention(const OglePagedBatch* batch, const OgleAttentionPa
         using F = Form<DP, MT, kSplit>;
         const int ranges = ranges_of(batch, F::kRows, F::kBlocks);
         auto kernel = paged_attention_kernel<DP, MT, kSplit>;
-        const long long max_tiles = ((long long)(a.b.max_rows < a.b.n_rows ? a.b.max_rows : a.b.n_rows) * a.b.group + F::kRows - 1) / F::kRows;
-        const long long segments = max_tiles * a.b.n_seqs * a.b.kv_heads;
-        a.by_segment = segments < ranges ? int(max_tiles) : 0;
+        const long long max_tiles = row_tiles_of(batch, F::kRows), segments = max_tiles * a.b.n_seqs * a.b.kv_heads;
+        a.cluster = cluster_of(batch, p, F::kRows, F::kBlocks);
+        a.by_segment = a.cluster || segments < ranges ? int(max_tiles) : 0;
         a.cuts = reinterpret_cast<Cut*>(a.parts + size_t(ranges) * 2 * F::kPart);
         static std::atomic<uint64_t> sized{0};           // devices whose limit of shared memory is raised
         int device = 0;
@@ -907,10 +1015,25 @@ int ogle_cuda_paged_attention(const OglePagedBatch* batch, const OgleAttentionPa
             set_last_error("paged_attention: no tensor map of the cache");
             return OGLE_ERR_CUDA;
         }
-        if (e == cudaSuccess) e = launch_overlapped(kernel, dim3(ranges), dim3(kWarps * 32), F::kSmem, stream, a, k_map, v_map);
+        if (e == cudaSuccess) {
+            cudaLaunchAttribute attr[2];
+            attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            attr[0].val.programmaticStreamSerializationAllowed = overlapped_launches_enabled() ? 1 : 0;
+            attr[1].id = cudaLaunchAttributeClusterDimension;
+            attr[1].val.clusterDim.x = a.cluster ? a.cluster : 1;
+            attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(a.cluster ? unsigned(segments * a.cluster) : ranges);
+            cfg.blockDim = dim3(kWarps * 32);
+            cfg.dynamicSmemBytes = F::kSmem;
+            cfg.stream = stream;
+            cfg.attrs = attr;
+            cfg.numAttrs = a.cluster ? 2 : 1;
+            e = cudaLaunchKernelEx(&cfg, kernel, a, k_map, v_map);
+        }
         if (e != cudaSuccess) { set_last_error(e); (void)cudaGetLastError(); return OGLE_ERR_CUDA; }
         int rc = finish_launch();
-        if (rc != OGLE_OK) return rc;
+        if (rc != OGLE_OK || a.cluster) return rc;
         // a warp to a row, or sixteen where few segments are cut into many parts
         const long long rows = (long long)(a.b.max_rows < a.b.n_rows ? a.b.max_rows : a.b.n_rows) * a.b.group;
         const int tile = int(rows < F::kRows ? (rows < 1 ? 1 : rows) : F::kRows);

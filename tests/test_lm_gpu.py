@@ -619,3 +619,81 @@ def test_example_answers_do_not_depend_on_the_batch():
         for _ in range(8):
             alone.step()
         assert alone.texts[0] == together.texts[i]
+
+
+def widened(batch):
+    """The same batch under a bound of a million tokens: the attention cuts it into ranges, where short bounds have a cluster of blocks a
+    tile of rows."""
+    table, page = batch["block_table"], batch["cache"][0].shape[2]
+    wide = torch.full((table.shape[0], (1 << 20) // page), -1, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    return {**batch, "block_table": wide, "max_kv_len": 1 << 20}
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("case", range(len(CASES)))
+def test_attention_under_a_wide_bound(case, dtype):
+    new, past, page, heads, kv_heads, dim, window = CASES[case]
+    batch, total = ref.make_batch(new, past, page, kv_heads, dim, seed=case)
+    q = rows_of(sum(new), heads, dim, dtype)
+    got = lm.attention(q, window=window, **widened(batch))
+    ref.check_attention(got, ref.attention64(q, batch, total, new, window=window), dtype)
+    got = lm.attention(q, **widened(batch))
+    ref.check_attention(got, ref.attention64(q, batch, total, new), dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_of_many_sequences_in_windows(dtype):
+    """More tiles of rows than the GPU has blocks for clusters."""
+    new, past = [1 + b % 3 for b in range(210)], [(37 * b) % 300 for b in range(210)]
+    batch, total = ref.make_batch(new, past, 16, 2, 64, seed=4)
+    q = rows_of(sum(new), 4, 64, dtype)
+    for window in (0, 33):
+        got = lm.attention(q, window=window, **batch)
+        ref.check_attention(got, ref.attention64(q, batch, total, new, window=window), dtype)
+
+
+def test_missing_pages_and_empty_sequences_under_a_wide_bound():
+    new, past = [1, 0, 1, 3, 2], [10, 5, 0, 100, 300]
+    batch, total = ref.make_batch(new, past, 16, 2, 128)
+    batch["block_table"][4, 3] = -1
+    q = rows_of(7, 8, 128, F32)
+    batch["kv_len"][0] = 0
+    batch["kv_len"][3] = 2                                       # of three rows the first stands before the text
+    short, wide = lm.attention(q, **batch), lm.attention(q, **widened(batch))
+    top = float(batch["cache"][1].float().nan_to_num().abs().amax((0, 1, 2, 3)) * batch["cache"][3].max())
+    assert torch.equal(torch.isinf(short[1]), torch.isinf(wide[1])) and bool(torch.isinf(wide[1][0]).all())
+    assert bool((wide[0][0] == 0).all()) and bool((wide[0][2] == 0).all())
+    assert float((short[0] - wide[0]).abs().max()) <= 2 * ref.LIMIT[F32] * top
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_nan_under_a_wide_bound(dtype):
+    new, past = [6, 1], [30, 100]
+    batch, total = ref.make_batch(new, past, 16, 2, 64, seed=3)
+    at = int(batch["block_table"][0, 2])
+    batch["cache"][1].view(torch.uint8)[at, 0, 1, 5] = 0xff     # token 33 of sequence 0: its rows 3.. attend it
+    q = rows_of(7, 4, 64, dtype)
+    for b in (batch, widened(batch)):
+        out, lse = lm.attention(q, **b)
+        hit = torch.zeros(out.shape, dtype=torch.bool, device="cuda")
+        hit[3:6, 0:2, 5] = True
+        assert torch.equal(torch.isnan(out), hit) and bool(torch.isfinite(lse).all())
+
+
+@pytest.mark.parametrize("wide", [False, True])
+def test_both_forms_report_a_wait_that_runs_out(wide):
+    batch, total = ref.make_batch([1, 2], [700, 90], 16, 2, 128)
+    q = rows_of(3, 8, 128, BF16)
+    lib = _lib.cuda_lib()
+    want = lm.attention(q, **(widened(batch) if wide else batch))
+    lib.ogle_cuda_set_wait_limit(0)
+    try:
+        lm.attention(q, **(widened(batch) if wide else batch))
+        torch.cuda.synchronize()
+        assert lib.ogle_cuda_device_status() != 0
+    finally:
+        lib.ogle_cuda_set_wait_limit(-1)
+        lib.ogle_cuda_clear_device_status()
+    again = lm.attention(q, **(widened(batch) if wide else batch))
+    assert torch.equal(again[0], want[0]) and torch.equal(again[1], want[1])
