@@ -4,7 +4,8 @@
 // allows it - and mends those that a token of the text or a bias names: tokens are counted in shared memory (whole numbers:
 // their order does not matter), the last bias named for a token is noted beside its count, and each such logit is computed
 // anew. A row has some hundred of them, not worth a look-up for each of the others (which took 17 of 25 instructions a logit:
-// 400 x 150000 93 us). Few tokens and biases go into a hash table at once; many are counted slice by slice of the range.
+// 400 x 150000 93 us). Few tokens and biases go into a hash table at once; where they turn out to be too many for it, they are counted
+// slice by slice of the range.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -66,7 +67,7 @@ __global__ void __launch_bounds__(kThreads, 4) adjust_logits_kernel(LogitsArgs a
     __shared__ __align__(16) unsigned words[kSlice];
     __shared__ int text[kText];
     __shared__ uint16_t taken[kMostHashed];
-    __shared__ int n_here, n_taken;
+    __shared__ int n_taken;
     const OgleLogitsParams& p = a.p;
     const int r = blockIdx.y, tid = threadIdx.x;
     const Ti* in = static_cast<const Ti*>(p.logits) + r * p.logits_stride;
@@ -85,7 +86,7 @@ __global__ void __launch_bounds__(kThreads, 4) adjust_logits_kernel(LogitsArgs a
     if (named) {
 #pragma unroll 4
         for (int i = tid; i < min(n_tokens, kText); i += kThreads) text[i] = __ldg(p.tokens + token0 + i);
-        if (tid == 0) n_here = n_taken = 0;
+        if (tid == 0) n_taken = 0;
     }
     const auto allows = [&](int t) { return !allowed || (__ldg(allowed + t / 32) >> (t % 32) & 1); };
 
@@ -130,7 +131,8 @@ __global__ void __launch_bounds__(kThreads, 4) adjust_logits_kernel(LogitsArgs a
     const int prompt = p.tokens && p.prompt_len ? p.prompt_len[r] : 0;
     const float* bias_value = p.bias_value + bias0;
     const RowTerms terms = {p.repetition ? p.repetition[r] : 1.f, p.presence ? p.presence[r] : 0.f, p.frequency ? p.frequency[r] : 0.f};
-    // f(number, token), for biases first and then for the text's tokens: those in [s0, s0 + width)
+    // f(number, token), for biases or for the text's tokens: those in [s0, s0 + width). (Collecting them first, until a warp's lanes have one
+    // each, took 1 us from 64 x 128001 with texts of 4000 and added 3 to 400 x 150000, whose blocks have whole rows.)
     const auto each = [&](bool biases, int s0, unsigned width, auto f) {
         const int n = biases ? n_biases : n_tokens;
 #pragma unroll 1
@@ -154,17 +156,10 @@ __global__ void __launch_bounds__(kThreads, 4) adjust_logits_kernel(LogitsArgs a
         reinterpret_cast<uint4*>(keys)[i] = make_uint4(kEmpty, kEmpty, kEmpty, kEmpty);
     }
     __syncthreads();                             // all logits of the range are written, too
-    bool hashed = !is_long;
-    if (hashed && n_tokens + n_biases > kMostHashed) {
-        int mine = 0;
-        for (int k = 0; k < 2; ++k) each(k, first, range, [&](int, int) { ++mine; });
-        if (mine) atomicAdd(&n_here, mine);
-        __syncthreads();
-        hashed = n_here <= kMostHashed;
-        __syncthreads();
-    }
-    if (hashed) {
-        const auto entry = [&](int token) {      // its place in the table: at most three quarters are taken, so there is one
+    if (!is_long) {
+        // Its place in the table. Three quarters of it are for use; where more tokens come than that, no thread begins another, and
+        // what was in hand - one a thread - finds a place still.
+        const auto entry = [&](int token) {
             unsigned h = unsigned(token) * 2654435761u >> 20;
             for (;;) {
                 const unsigned k = atomicCAS(&keys[h], kEmpty, unsigned(token));
@@ -173,30 +168,38 @@ __global__ void __launch_bounds__(kThreads, 4) adjust_logits_kernel(LogitsArgs a
                     int at = 0;
                     if (lane == leader) at = atomicAdd(&n_taken, __popc(with));
                     at = __shfl_sync(with, at, leader);
-                    taken[at + __popc(with & ((1u << lane) - 1))] = uint16_t(h);
+                    at += __popc(with & ((1u << lane) - 1));
+                    if (at < kMostHashed) taken[at] = uint16_t(h);
                 }
                 if (k == kEmpty || k == unsigned(token)) return h;
                 h = (h + 1) & (kEntries - 1);
             }
         };
-        static_assert(kEntries == 4096, "20 bits off a hash of 32");
+        static_assert(kEntries == 4096 && kMostHashed + kThreads < kEntries, "20 bits off a hash of 32");
+        const auto full = [&] { return *static_cast<volatile int*>(&n_taken) > kMostHashed; };
         // biases first: a word then has nothing else, and its largest value is the last of them
         if (n_biases > 0) {
-            each(true, first, range, [&](int i, int token) { atomicMax(&words[entry(token)], unsigned(i + 1) << kBiasShift); });
+            each(true, first, range, [&](int i, int token) {
+                if (!full()) atomicMax(&words[entry(token)], unsigned(i + 1) << kBiasShift);
+            });
             __syncthreads();
         }
         each(false, first, range, [&](int i, int token) {
+            if (full()) return;
             const unsigned h = entry(token);
             if (i < prompt) atomicOr(&words[h], kSeen);
             else atomicAdd(&words[h], 1u);
         });
         __syncthreads();
+        if (n_taken <= kMostHashed) {
 #pragma unroll 1
-        for (int i = tid; i < n_taken; i += kThreads) {
-            const unsigned h = taken[i], w = words[h];
-            mend(int(keys[h]), w & (kSeen | kMaxTokens), w << 1 >> (kBiasShift + 1));
+            for (int i = tid; i < n_taken; i += kThreads) {
+                const unsigned h = taken[i], w = words[h];
+                mend(int(keys[h]), w & (kSeen | kMaxTokens), w << 1 >> (kBiasShift + 1));
+            }
+            return;
         }
-        return;
+        for (int i = tid; i < kEntries / 4; i += kThreads) reinterpret_cast<uint4*>(words)[i] = make_uint4(0, 0, 0, 0);
     }
     // a word for each token of a slice, or two: counts and biases
     const unsigned slice = is_long ? kSlice / 2 : kSlice, step = is_long ? 2 : 1;
