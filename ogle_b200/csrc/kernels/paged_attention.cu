@@ -1018,7 +1018,8 @@ int ogle_cuda_paged_attention(const OglePagedBatch* batch, const OgleAttentionPa
         if (e == cudaSuccess) {
             cudaLaunchAttribute attr[2];
             attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-            attr[0].val.programmaticStreamSerializationAllowed = overlapped_launches_enabled() ? 1 : 0;
+            // behind the prompt form's launches it is this call's own affair
+            attr[0].val.programmaticStreamSerializationAllowed = overlapped_launches_enabled(a.few_limit > 0) ? 1 : 0;
             attr[1].id = cudaLaunchAttributeClusterDimension;
             attr[1].val.clusterDim.x = a.cluster ? a.cluster : 1;
             attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;

@@ -766,8 +766,7 @@ paged_prompt_kernel(PromptArgs p) {
     if (warp == kProductWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
 }
 
-// Blocks: one to an SM, and no more than there can be tiles.
-int prompt_ranges(const OglePagedBatch* b) { return kNumSMs; }
+constexpr int kPromptRanges = kNumSMs;           // a block to an SM; what has no tile has no range
 long long prompt_tiles(const OglePagedBatch* b) {
     const long long rows = b->max_rows < b->n_rows ? b->max_rows : b->n_rows;
     return (rows * (b->q_heads / b->kv_heads) + kItemRows - 1) / kItemRows;
@@ -777,7 +776,7 @@ size_t up16(size_t n) { return (n + 15) & ~size_t(15); }
 template <int DP>
 int launch_form(const OglePagedBatch* b, PromptArgs p, void* workspace, cudaStream_t stream) {
     using L = Layout<DP>;
-    const int ranges = prompt_ranges(b);
+    constexpr int ranges = kPromptRanges;
     unsigned char* w = static_cast<unsigned char*>(workspace);
     p.a.parts = reinterpret_cast<float*>(w); w += up16(size_t(ranges) * 2 * L::kPart * sizeof(float));
     p.a.cuts = reinterpret_cast<Cut*>(w); w += up16(ranges * sizeof(Cut));
@@ -811,7 +810,7 @@ int launch_form(const OglePagedBatch* b, PromptArgs p, void* workspace, cudaStre
 namespace paged {
 
 size_t prompt_workspace(const OglePagedBatch* b) {
-    const int ranges = prompt_ranges(b);
+    constexpr int ranges = kPromptRanges;
     const size_t part = b->head_dim <= 64 ? Layout<64>::kPart : Layout<128>::kPart;
     return up16(size_t(ranges) * 2 * part * sizeof(float)) + up16(ranges * sizeof(Cut)) + sizeof(Plan) + ranges * sizeof(Start) +
            size_t(ranges) * kNanKeys * sizeof(NanPiece);
