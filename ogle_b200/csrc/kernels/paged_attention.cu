@@ -882,18 +882,63 @@ long long row_tiles_of(const OglePagedBatch* b, int rows) {
     if (few_limit(b) && most > kFewRows) most = kFewRows;
     return (most + rows - 1) / rows;
 }
+// Raises the kernel's limit of shared memory, once for each device.
+template <int DP, int MT, bool kSplit>
+cudaError_t prepare() {
+    static std::atomic<uint64_t> sized{0};
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e == cudaSuccess && !(sized.load(std::memory_order_relaxed) >> (device & 63) & 1)) {
+        e = cudaFuncSetAttribute(paged_attention_kernel<DP, MT, kSplit>, cudaFuncAttributeMaxDynamicSharedMemorySize, Form<DP, MT, kSplit>::kSmem);
+        if (e == cudaSuccess) sized.fetch_or(1ull << (device & 63), std::memory_order_relaxed);
+    }
+    return e;
+}
+
+// Clusters of so many blocks that the GPU runs at once. Asked once: every B200 gives the same answer.
+template <int DP, int MT, bool kSplit>
+int most_clusters(int size) {
+    static std::atomic<int> known[9] = {};            // one more than the number
+    int n = known[size].load(std::memory_order_relaxed);
+    if (n == 0) {
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = size;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(size);
+        cfg.blockDim = dim3(kWarps * 32);
+        cfg.dynamicSmemBytes = Form<DP, MT, kSplit>::kSmem;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        if (prepare<DP, MT, kSplit>() != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, paged_attention_kernel<DP, MT, kSplit>, &cfg) != cudaSuccess) {
+            (void)cudaGetLastError();
+            return 0;
+        }
+        known[size].store(++n, std::memory_order_relaxed);
+    }
+    return n - 1;
+}
+
 // Blocks of a cluster that has one segment, or 0: ranges. A call over clusters saves the second launch and the search for ranges, about
 // 3 us, but takes as long as the longest sequence's share, and blocks that the clusters do not use stay idle. us over ranges / clusters,
 // one query row each, 32 query heads to 8 of 128 elements: one sequence of 700 tokens 10.8 / 9.4, of 4000 13.6 / 13.6, of 8000 15.1 /
 // 19.8; 4 of 2000 14.7 / 11.7, of 8000 23.1 / 22.7, of 16000 33.4 / 38.9; 16 of up to 4000 35.7 / 23.9, of up to 8000 35.4 / 38.2.
 // So the tiles of 64 keys that pay a block go from 6, where few blocks of the GPU are used, to about 30, where all are.
-int cluster_of(const OglePagedBatch* b, const OgleAttentionParams* p, int rows, int blocks) {
-    const long long segments = row_tiles_of(b, rows) * b->n_seqs * b->kv_heads, slots = kNumSMs * blocks;
+// A cluster has to fit into a part of the GPU with all its blocks, so the sizes are those of which the runtime says that all run at once:
+// 96 clusters of 3 with 256 elements, two blocks an SM, do not (288 of 296 slots: 24 drafts over 4096 tokens 85 us, 70 in ranges).
+template <int DP, int MT, bool kSplit>
+int cluster_of(const OglePagedBatch* b, const OgleAttentionParams* p) {
+    using F = Form<DP, MT, kSplit>;
+    constexpr long long slots = kNumSMs * F::kBlocks;
+    const long long segments = row_tiles_of(b, F::kRows) * b->n_seqs * b->kv_heads;
     if (segments < 1 || segments * 2 > slots) return 0;
-    const long long size = slots / segments < 8 ? slots / segments : 8;
+    int size = slots / segments < 8 ? int(slots / segments) : 8;
+    while (size > 1 && most_clusters<DP, MT, kSplit>(size) < segments) --size;
+    if (size < 2) return 0;
     long long keys = b->max_kv_len;
     if (p->window > 0 && keys > (long long)p->window + b->max_rows) keys = (long long)p->window + b->max_rows;
-    return keys <= kTileKeys * size * (6 + 25 * segments * size / slots) ? int(size) : 0;
+    return keys <= kTileKeys * size * (6 + 25 * segments * size / slots) ? size : 0;
 }
 
 // Ranges: as many blocks as fit the GPU at once, and no more than there can be tiles.
@@ -918,7 +963,8 @@ size_t few_workspace(const OglePagedBatch* b, const OgleAttentionParams* p) {
     if (!some_few(b)) return 0;
     return with_form(choose(b), [&](auto dp, auto mt, auto split) {
         using F = Form<decltype(dp)::value, decltype(mt)::value, decltype(split)::value>;
-        if (cluster_of(b, p, F::kRows, F::kBlocks)) return sizeof(Cut);   // not read: a caller without a workspace finds out at every size
+        // with clusters it is not read, but a caller without a workspace finds out at every size
+        if (cluster_of<decltype(dp)::value, decltype(mt)::value, decltype(split)::value>(b, p)) return sizeof(Cut);
         return size_t(ranges_of(b, F::kRows, F::kBlocks)) * (2 * F::kPart * sizeof(float) + sizeof(Cut));
     });
 }
@@ -1000,16 +1046,10 @@ int ogle_cuda_paged_attention(const OglePagedBatch* batch, const OgleAttentionPa
         const int ranges = ranges_of(batch, F::kRows, F::kBlocks);
         auto kernel = paged_attention_kernel<DP, MT, kSplit>;
         const long long max_tiles = row_tiles_of(batch, F::kRows), segments = max_tiles * a.b.n_seqs * a.b.kv_heads;
-        a.cluster = cluster_of(batch, p, F::kRows, F::kBlocks);
+        a.cluster = cluster_of<DP, MT, kSplit>(batch, p);
         a.by_segment = a.cluster || segments < ranges ? int(max_tiles) : 0;
         a.cuts = reinterpret_cast<Cut*>(a.parts + size_t(ranges) * 2 * F::kPart);
-        static std::atomic<uint64_t> sized{0};           // devices whose limit of shared memory is raised
-        int device = 0;
-        cudaError_t e = cudaGetDevice(&device);
-        if (e == cudaSuccess && !(sized.load(std::memory_order_relaxed) >> (device & 63) & 1)) {
-            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
-            if (e == cudaSuccess) sized.fetch_or(1ull << (device & 63), std::memory_order_relaxed);
-        }
+        cudaError_t e = prepare<DP, MT, kSplit>();
         CUtensorMap k_map, v_map;
         if (e == cudaSuccess && (!cache_map(&k_map, a.b, a.b.k_cache, DP) || !cache_map(&v_map, a.b, a.b.v_cache, DP))) {
             set_last_error("paged_attention: no tensor map of the cache");
