@@ -67,7 +67,8 @@ const char* ogle_cuda_last_error(void);
 int ogle_cuda_device_status(void);
 int ogle_cuda_clear_device_status(void);
 /* The raw status word: which wait gave up (1 producer, 2 MMA issuer, 3 operand split,
- * 4 epilogue, 5 accumulator hand-back; 6 depthwise, 8 direct stem or fp32 contraction); 0 when none did. Synchronises the
+ * 4 epilogue, 5 accumulator hand-back; 6 depthwise, 8 direct stem or fp32 contraction,
+ * 9 paged attention); 0 when none did. Synchronises the
  * device. */
 int ogle_cuda_device_status_detail(void);
 /* Programmatic dependent launches for the kernels launched after this call (process-wide): each kernel's
@@ -75,7 +76,8 @@ int ogle_cuda_device_status_detail(void);
  * on the stream drains; every kernel waits for its predecessor's results before its first global access. Pays
  * when the launches are short (5 % at one image per step, 1-4 % up to 16), costs 1-2 % when they are long: the
  * runtime turns it on for sessions whose tensors hold less than 1 GB. The environment variable OGLE_PDL (0/1), when set, overrides it.
- * ogle_cuda_gemm_ws overlaps its product with its own packing pass whatever is set here; OGLE_PDL=0 keeps those apart too.
+ * ogle_cuda_gemm_ws overlaps its product with its own packing pass whatever is set here, ogle_cuda_paged_attention
+ * its second launch and those that follow; OGLE_PDL=0 keeps those apart too.
  * Captured CUDA graphs keep what was in force when they were captured. */
 int ogle_cuda_set_overlapped_launches(int on);
 
@@ -93,7 +95,7 @@ typedef struct {
 int ogle_cuda_last_contraction(OgleContraction* out);
 
 /* How many times a role of the tensor-core kernels polls for its turn before it gives up, or, for its operands, a thread
- * of the fp32 contraction by the copy engine or a warp of the direct RGB stem, for the launches that follow on any stream
+ * of the fp32 contraction by the copy engine, a warp of the direct RGB stem or of paged attention, for the launches that follow on any stream
  * (process-wide). polls < 0 restores the default (2^22,
  * tens of milliseconds); 0 makes every such wait give up at once. It exists to exercise the
  * give-up path without a fault: a launch whose waits run out writes no valid output, sets the

@@ -3,6 +3,10 @@
 // A block has one page of one sequence and either one head of the keys, one of the values, or a few heads of the queries: the
 // page's scale depends on all rows that come to it, and nothing else does, so no block waits for another and no sum has an
 // order to depend on. The rows' values stay in registers between the maximum and the rounding.
+//
+// Bound by memory where prompts are appended: 26000 rows of 32 + 2 x 8 heads of 128 in bf16, 855 MB, 188 us, 70 % of what a copy
+// reaches (three blocks an SM, 80 registers a thread; two blocks 221 us). Single tokens are bound by latency - row, maximum, page: 5 us
+// on the device for 1 or 96 of them, 14 us a call.
 #include <type_traits>
 
 #include "paged.cuh"
@@ -333,7 +337,8 @@ extern "C" int ogle_cuda_kv_append(const OglePagedBatch* batch, const OgleAppend
     long pages = B.max_rows == 1 ? B.n_seqs : (long)(B.n_rows >> B.page_shift) + 2L * B.n_seqs;
     if (B.max_rows > 1 && pages > B.n_rows) pages = B.n_rows;
     const int tokens = B.max_rows < (1 << B.page_shift) ? B.max_rows : 1 << B.page_shift;
-    // 16 bytes of 16-bit values at a time where the rotated part is whole pieces of that
+    // 16 bytes of 16-bit values at a time where the rotated part is whole pieces of that (the 26000 rows: 221 us so, 338 by 8 bytes, when
+    // both had their first form)
     const bool wide = dt != OGLE_F32 && a.rotary_dim % 16 == 0;
     const int pieces = B.dim / (wide ? 16 : 8), hold = kHoldValues / (wide ? 16 : 8);
     int threads = (div_up(tokens, hold) * pieces + 31) / 32 * 32;

@@ -11,6 +11,11 @@
 // Where there are few segments, none of them long, the blocks of a cluster have one segment instead and add their parts
 // through each other's shared memory: one launch, no workspace.
 //
+// Measured: 64 sequences of up to 8000 tokens, 32 query heads to 8 of 128, 570 MB: 111 us, 79 % of what a copy reaches. 3 sequences
+// of up to 200000 tokens, 16 query heads to one: 52 us, 3.9 TB/s with the join - 500 instructions a step of 16 keys, each warp
+// waiting 2 of 8 cycles for the one before (four blocks an SM, the queries in shared memory; three, in registers: 56). What is short is bound
+// by latency: one sequence of 700 tokens takes 9 us on the device.
+//
 // The products run on 16-bit operands: an e4m3 value is an fp16 exactly; queries are scaled by a power of two so that their
 // largest lies below 2^12 (11 bits of each, or 22 as two parts), weights lie below 2^15. kSplit keeps queries and weights as
 // two parts, the high ones in rows 0-7 of the multiply and the low ones in rows 8-15: an accumulator's two halves of a row are
@@ -26,7 +31,7 @@ using namespace paged;
 
 constexpr int kWarps = 4;
 constexpr int kTileKeys = kWarps * kChunk;
-constexpr int kSegmentCost = 8;                  // tiles that a segment's beginning and end take as long as
+constexpr int kSegmentCost = 8;                  // tiles that a segment's beginning and end take as long as (64 sequences: 0 139 us, 2 124, 8 114)
 template <int DP, int MT, bool kSplit>
 struct Form {
     static constexpr int kRows = MT * (kSplit ? 8 : 16);

@@ -13,7 +13,10 @@
 // first sums run while the second half is being weighted. P lies over S in tensor memory (2 x 128 columns for S, 2 x DP for O), so
 // the next S of a tile of rows is asked for once its P V is through.
 // Shared memory has the products' operands to deliver beside the conversion's traffic; two S of 64 keys a tile of rows, which
-// overlap more, read the queries twice as often and were slower.
+// overlap more, read the queries twice as often and were slower (3.2 us a tile of keys, so 2.1: 1150 TFLOP/s where texts are long). The
+// tensor cores and the exponentials each need half of that; taking a quarter of the exponentials off the special function units, by a
+// polynomial, made it slower. Six prompts of 2000 rows over 2500 earlier tokens: 358 us, 500 TFLOP/s - an item's beginning and end
+// (queries, the first scores, the last sums, results: 10 us) take as long as its tiles there.
 //
 // Work: items (sequence, tile of 256 rows, kv head) laid end to end by their tiles of keys, cut into one range a block; parts
 // of items that were cut go to the workspace and are joined as in the form for few rows (paged_attention.cu). The ranges'
@@ -28,7 +31,7 @@ using namespace paged;
 constexpr int kKeys = 128;                       // of a tile
 constexpr int kStep = 64;                        // of a step: half a tile
 constexpr int kTileRows = 128, kItemRows = 2 * kTileRows;
-constexpr int kItemCost = 10;                    // tiles that an item's beginning and end take as long as
+constexpr int kItemCost = 10;                    // tiles that an item's beginning and end take as long as: 20000 cycles, a tile 2000 to 4000
 constexpr int kThreads = 16 * 32;                // 8 warps of rows, 4 of conversion, one for products and three that fill up its group
 // Registers of a thread: a row has its 128 scores in them. (2 x 176 + 112 + 48) x 128 = the 128 of 512 threads at launch.
 constexpr int kRowRegisters = 176, kConvertRegisters = 112, kIssueRegisters = 48;

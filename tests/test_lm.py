@@ -1,5 +1,6 @@
 """The language-model operators' checks of their arguments: no GPU needed."""
 import ctypes as C
+import os
 
 import pytest
 import torch
@@ -132,3 +133,26 @@ def test_rotary_table():
     angle = 7 * 100.0 ** (-i / 8)
     assert torch.allclose(t[7].double(), torch.cat([angle.cos(), angle.sin()]), atol=1e-7)
     assert torch.equal(t[0], torch.cat([torch.ones(8), torch.zeros(8)]))
+
+
+def test_structures_lie_as_the_header_says(tmp_path):
+    """Offsets and sizes of the ctypes mirrors, and so of the packed bytes, against the compiler's."""
+    import shutil
+    import subprocess
+    compiler = shutil.which("g++")
+    if not compiler:
+        pytest.skip("no g++")
+    mirrors = {"OglePagedBatch": _lib.PagedBatch, "OgleAppendParams": _lib.AppendParams, "OgleAttentionParams": _lib.AttentionParams,
+               "OgleLogitsParams": _lib.LogitsParams}
+    lines = ["#include <cstddef>", '#include "ogle_cuda.h"']
+    for name, mirror in mirrors.items():
+        lines.append(f"static_assert(sizeof({name}) == {C.sizeof(mirror)}, \"\");")
+        lines += [f"static_assert(offsetof({name}, {f}) == {getattr(mirror, f).offset}, \"\");" for f, _ in mirror._fields_]
+    source = tmp_path / "layout.cc"
+    source.write_text("\n".join(lines) + "\n")
+    include = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+    done = subprocess.run([compiler, "-std=c++17", "-fsyntax-only", "-I", include, str(source)], capture_output=True, text=True)
+    assert done.returncode == 0, done.stderr
+    packed = _lib.packer(_lib.AttentionParams).pack(1, 2, 3, 4, 5, 6, 7, 0.5, 1, 9, 0)
+    back = _lib.AttentionParams.from_buffer_copy(packed)
+    assert (back.q, back.out, back.lse, back.q_row, back.out_head, back.scale, back.causal, back.window) == (1, 2, 3, 4, 7, 0.5, 1, 9)
