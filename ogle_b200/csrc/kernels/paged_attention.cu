@@ -900,7 +900,7 @@ cudaError_t prepare() {
     return e;
 }
 
-// Clusters of so many blocks that the GPU runs at once. Asked once: every B200 gives the same answer.
+// Clusters of so many blocks that the GPU runs at once. Asked once for all devices: two of them may differ by a few, which costs time at most.
 template <int DP, int MT, bool kSplit>
 int most_clusters(int size) {
     static std::atomic<int> known[9] = {};            // one more than the number

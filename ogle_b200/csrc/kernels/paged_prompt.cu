@@ -41,8 +41,8 @@ constexpr int kNanKeys = 8192;                   // pieces of 16 values with a N
 // A piece of 16 values of a token at an item's edge: which of them are NaN.
 struct NanPiece { int key; uint16_t bits, unit; };
 
-struct Start { int b, rt, h, off; };             // where a range begins: sequence, tile of rows, kv head, what of the item lies before; b -1: it is empty
-struct Plan { long long total; int unused[2]; };
+struct Start { int b, rt, h, off; };             // where a range begins: sequence, tile of rows, kv head, what of the item lies before; b -1: nowhere
+struct Plan { long long total; int ranges, cost; };   // what all items count; ranges that it is cut into; what an item's ends count of it
 
 struct PromptArgs {
     AttnArgs a;
@@ -74,63 +74,93 @@ __device__ __forceinline__ Span item_span(const AttnArgs& a, const Sequence& s, 
     const int m0 = rt * kItemRows, m_end = min(s.n * a.b.group, m0 + kItemRows);
     return span_of(s, m0 / a.b.group, (m_end - 1) / a.b.group, a.causal, a.window);
 }
-// What tile rt of a sequence's rows counts, for each kv head; 0 where there is none, or no key for the whole sequence.
-__device__ __forceinline__ int item_cost(const AttnArgs& a, const Sequence& s, int rt) {
-    if (s.n <= 0 || rt >= row_tiles(a.b, s.n, kItemRows)) return 0;
+// Tiles of keys of tile rt of a sequence's rows; -1 where there is no such item, or no key for the whole sequence.
+__device__ __forceinline__ int item_tiles(const AttnArgs& a, const Sequence& s, int rt) {
+    if (s.n <= 0 || rt >= row_tiles(a.b, s.n, kItemRows)) return -1;
     const Span all = span_of(s, 0, s.n - 1, a.causal, a.window);
-    return all.hi > all.lo ? key_tiles(item_span(a, s, rt)) + kItemCost : 0;
+    return all.hi > all.lo ? key_tiles(item_span(a, s, rt)) : -1;
 }
 
-// One block: sums all items and writes down where each range begins.
+// One block: sums all items, and each range's thread looks up which of them it begins in. An item's ends count as kItemCost tiles, but as
+// a quarter of a range at most (and 1 at least: an item whose rows attend nothing is somebody's, too), so that short ranges are not
+// spent on them.
 __global__ void __launch_bounds__(1024) paged_plan_kernel(AttnArgs a, int max_tiles, int ranges, Plan* plan, Start* starts) {
-    __shared__ long long sums[32];
+    __shared__ long long sums[2][32], ends[1024];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const long long n = (long long)a.b.n_seqs * max_tiles;
     grid_dependency_trigger();
     grid_dependency_wait();
-    for (int k = tid; k < ranges; k += 1024) starts[k].b = -1;
-    long long total = 0;
-    for (int pass = 0; pass < 2; ++pass) {
-        long long before = 0;
-        for (long long i0 = 0; i0 < n; i0 += 1024) {
-            const long long i = i0 + tid;
-            const int b = int(quotient(i, max_tiles)), rt = int(i - (long long)b * max_tiles);
-            const int cost = i < n ? item_cost(a, prompt_sequence(a, b), rt) : 0;
-            const long long mine = (long long)cost * a.b.kv_heads;
-            long long sum = mine;
+    const auto tiles_at = [&](long long i, int& b, int& rt) {
+        b = int(quotient(i, max_tiles));
+        rt = int(i - (long long)b * max_tiles);
+        return i < n ? item_tiles(a, prompt_sequence(a, b), rt) : -1;
+    };
+    long long tiles = 0, items = 0;
+    for (long long i = tid; i < n; i += 1024) {
+        int b, rt;
+        const int t = tiles_at(i, b, rt);
+        if (t >= 0) { tiles += t; ++items; }
+    }
 #pragma unroll
-            for (int d = 1; d < 32; d *= 2) {
-                const long long u = __shfl_up_sync(~0u, sum, d);
-                if (lane >= d) sum += u;
-            }
-            __syncthreads();
-            if (lane == 31) sums[warp] = sum;
-            __syncthreads();
-            long long all = 0;
-            for (int w = 0; w < 32; ++w) {
-                if (w < warp) sum += sums[w];
-                all += sums[w];
-            }
-            if (pass == 1 && mine > 0) {
-                const long long begin = before + sum - mine, end = begin + mine;
-                for (int k = int(quotient(begin * ranges + total - 1, total)); k < ranges; ++k) {
-                    const long long x = quotient(total * k, ranges);
-                    if (x >= end) break;
-                    if (x >= begin && (k == ranges - 1 || x != quotient(total * (k + 1), ranges)))   // the last of ranges that begin alike has the tiles
-                        starts[k] = Start{b, rt, int(x - begin) / cost, int(x - begin) % cost};
-                }
-            }
-            before += all;
+    for (int d = 16; d; d /= 2) {
+        tiles += __shfl_xor_sync(~0u, tiles, d);
+        items += __shfl_xor_sync(~0u, items, d);
+    }
+    if (lane == 0) { sums[0][warp] = tiles; sums[1][warp] = items; }
+    __syncthreads();
+    tiles = sums[0][lane];
+    items = sums[1][lane];
+#pragma unroll
+    for (int d = 16; d; d /= 2) {
+        tiles += __shfl_xor_sync(~0u, tiles, d);
+        items += __shfl_xor_sync(~0u, items, d);
+    }
+    const int heads = a.b.kv_heads, cost = int(max(1LL, min((long long)kItemCost, quotient(tiles * heads, 4LL * ranges))));
+    const long long total = (tiles + items * cost) * heads;
+    const int used = int(min((long long)ranges, total));
+    if (tid == 0) *plan = Plan{total, used, cost};
+    const long long at = tid < used ? quotient(total * tid, used) : -1;    // a thread to a range: there are no more than threads
+    if (tid < ranges && tid >= used) starts[tid].b = -1;
+    long long before = 0;
+    for (long long i0 = 0; i0 < n; i0 += 1024) {
+        int b, rt;
+        const int t = tiles_at(i0 + tid, b, rt);
+        long long sum = t < 0 ? 0 : (long long)(t + cost) * heads;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const long long u = __shfl_up_sync(~0u, sum, d);
+            if (lane >= d) sum += u;
         }
-        total = before;
-        if (pass == 0 && tid == 0) plan->total = total;
-        if (total == 0) break;
         __syncthreads();
+        if (lane == 31) sums[0][warp] = sum;
+        __syncthreads();
+        long long all = sums[0][lane];
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const long long u = __shfl_up_sync(~0u, all, d);
+            if (lane >= d) all += u;
+        }
+        const long long ahead = __shfl_sync(~0u, all, max(warp - 1, 0));
+        all = __shfl_sync(~0u, all, 31);
+        ends[tid] = before + sum + (warp > 0 ? ahead : 0);
+        __syncthreads();
+        if (at >= before && at < before + all) {
+            int lo = 0, hi = 1023;                 // the first item that ends behind the range's beginning
+            while (lo < hi) {
+                const int mid = (lo + hi) / 2;
+                if (ends[mid] > at) hi = mid;
+                else lo = mid + 1;
+            }
+            const int c = tiles_at(i0 + lo, b, rt) + cost;
+            const long long x = at - (ends[lo] - (long long)c * heads), h = quotient(x, c);
+            starts[tid] = Start{b, rt, int(h), int(x - h * c)};
+        }
+        before += all;
     }
 }
 
 // A block's place in its range, and the item that it has.
-struct Walk { long long at, end, total; int b, rt, h, off; };
+struct Walk { long long at, end, total; int ranges, cost, b, rt, h, off; };
 struct Item {
     Sequence s;
     int b, h, m0, m_end;
@@ -145,8 +175,9 @@ __device__ __forceinline__ bool next_item(const PromptArgs& p, Walk& w, Item& g)
     const Batch& B = a.b;
     while (w.at < w.end && w.b < B.n_seqs) {
         g.s = prompt_sequence(a, w.b);
-        g.cost = item_cost(a, g.s, w.rt);
-        if (g.cost == 0) {
+        const int tiles = item_tiles(a, g.s, w.rt);
+        g.cost = tiles + w.cost;
+        if (tiles < 0) {
             w.rt = w.h = w.off = 0;
             ++w.b;
             continue;
@@ -160,13 +191,13 @@ __device__ __forceinline__ bool next_item(const PromptArgs& p, Walk& w, Item& g)
         g.inner_hi = span_of(g.s, 0, g.m0 / B.group, a.causal, a.window).hi;
         g.c0 = w.off;
         g.c1 = int(min((long long)g.cost, w.off + (w.end - w.at)));
-        const int t0 = max(g.c0 - kItemCost, 0), t1 = max(g.c1 - kItemCost, 0);
+        const int t0 = max(g.c0 - w.cost, 0), t1 = max(g.c1 - w.cost, 0);
         g.j0 = (g.keys.lo & ~(kChunk - 1)) + t0 * kKeys;
         g.tiles = t1 - t0;
         if (g.c0 == 0 && g.c1 < g.cost) {
             const long long item_end = w.at + g.cost;
-            const int last = min(int(quotient(item_end * gridDim.x + w.total - 1, w.total)), int(gridDim.x));
-            a.cuts[blockIdx.x] = Cut{g.m_end - g.m0, g.s.row0, g.h, g.m0, int(blockIdx.x), last, w.total < gridDim.x, 0, w.total};
+            const int last = min(int(quotient(item_end * w.ranges + w.total - 1, w.total)), w.ranges);
+            a.cuts[blockIdx.x] = Cut{g.m_end - g.m0, g.s.row0, g.h, g.m0, int(blockIdx.x), last, 0, 0, w.total};
         }
         w.at += g.c1 - g.c0;
         w.off = 0;
@@ -312,9 +343,13 @@ paged_prompt_kernel(PromptArgs p) {
     if (tid == 0) {
         a.cuts[blockIdx.x].rows = 0;
         const Start s = p.starts[blockIdx.x];
-        const long long total = p.plan->total;
-        walk = Walk{quotient(total * blockIdx.x, gridDim.x), quotient(total * (blockIdx.x + 1), gridDim.x), total, s.b, s.rt, s.h, s.off};
-        more_items = s.b >= 0 && next_item(p, walk, item);
+        const Plan plan = *p.plan;
+        more_items = 0;
+        if (s.b >= 0) {                            // else: no such range
+            walk = Walk{quotient(plan.total * blockIdx.x, plan.ranges), quotient(plan.total * (blockIdx.x + 1), plan.ranges), plan.total,
+                        plan.ranges, plan.cost, s.b, s.rt, s.h, s.off};
+            more_items = next_item(p, walk, item);
+        }
     }
     before_sync();
     __syncthreads();
@@ -769,7 +804,7 @@ paged_prompt_kernel(PromptArgs p) {
     if (warp == kProductWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
 }
 
-constexpr int kPromptRanges = kNumSMs;           // a block to an SM; what has no tile has no range
+constexpr int kPromptRanges = kNumSMs;           // at most: a block to an SM
 long long prompt_tiles(const OglePagedBatch* b) {
     const long long rows = b->max_rows < b->n_rows ? b->max_rows : b->n_rows;
     return (rows * (b->q_heads / b->kv_heads) + kItemRows - 1) / kItemRows;
