@@ -850,13 +850,13 @@ __global__ void __launch_bounds__(kManyWarps * 32) paged_join_many_kernel(AttnAr
 // ---- host
 struct Choice { int dp, mt; bool split; };
 
-constexpr int kFewRows = 64;
 int few_limit(const OglePagedBatch* b);
 
 Choice choose(const OglePagedBatch* b) {
     Choice c;
     long long rows = (long long)(b->max_rows < b->n_rows ? b->max_rows : b->n_rows) * (b->q_heads / b->kv_heads);
-    if (few_limit(b) && rows > kFewRows) rows = kFewRows;
+    const int limit = few_limit(b);
+    if (limit && rows > limit) rows = limit;
     c.dp = b->head_dim <= 64 ? 64 : (b->head_dim <= 128 ? 128 : 256);
     c.split = b->dtype == OGLE_F32 || rows <= 8;
     c.mt = c.dp == 256 || rows <= (c.split ? 8 : 16) ? 1 : 2;
@@ -884,7 +884,8 @@ auto with_form(const Choice& c, G g) {
 // Tiles of rows that a sequence can have in this form, and segments of the whole call.
 long long row_tiles_of(const OglePagedBatch* b, int rows) {
     long long most = (long long)(b->max_rows < b->n_rows ? b->max_rows : b->n_rows) * (b->q_heads / b->kv_heads);
-    if (few_limit(b) && most > kFewRows) most = kFewRows;
+    const int limit = few_limit(b);
+    if (limit && most > limit) most = limit;
     return (most + rows - 1) / rows;
 }
 // Raises the kernel's limit of shared memory, once for each device.
@@ -956,10 +957,16 @@ int ranges_of(const OglePagedBatch* b, int rows, int blocks) {
 }
 
 // Rows x query heads of a group above which a sequence is the prompt form's, or 0: every sequence is taken here. The prompt form reads a
-// key once for 256 rows, where this one reads it for 16 or 32, and needs about 64 of them to be the faster.
+// key once for 256 rows, where this one reads it for 16 or 32, but has three launches and the tensor cores' latencies to begin and end
+// with. us here / there, 32 query heads to 8 of 128 elements: 64 and 80 rows of 8 sequences over 20000 tokens 174 / 187 and 249 / 188,
+// over 3000 46 / 56 and 58 / 57; 128 rows of 32 sequences over 300 70 / 63; of one sequence, 128 rows over 20000 58 / 56, 256 over 3000
+// 32 / 42, over 300 21 / 31. So 64 rows, and more where the call has few keys to go through.
 int few_limit(const OglePagedBatch* b) {
+    if (b->dtype == OGLE_F32 || b->head_dim > 128) return 0;
     const long long rows = (long long)(b->max_rows < b->n_rows ? b->max_rows : b->n_rows) * (b->q_heads / b->kv_heads);
-    return b->dtype != OGLE_F32 && b->head_dim <= 128 && rows > kFewRows ? kFewRows : 0;
+    const long long keys = (long long)b->n_seqs * b->kv_heads * b->max_kv_len * (b->head_dim <= 64 ? 64 : 128) / 128;
+    const long long limit = 64 + 5000000 / (keys > 5000 ? keys : 5000);
+    return rows > limit ? int(limit) : 0;
 }
 // Whether some sequence can have few rows, as far as the host knows.
 bool some_few(const OglePagedBatch* b) { return !few_limit(b) || (long long)b->n_seqs * b->max_rows != b->n_rows; }

@@ -697,3 +697,53 @@ def test_both_forms_report_a_wait_that_runs_out(wide):
         lib.ogle_cuda_clear_device_status()
     again = lm.attention(q, **(widened(batch) if wide else batch))
     assert torch.equal(again[0], want[0]) and torch.equal(again[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("case", range(len(PROMPTS)))
+def test_attention_of_prompts_under_a_wide_bound(case, dtype):
+    """The tensor cores' form, which short calls do without."""
+    new, past, page, heads, kv_heads, dim, window = PROMPTS[case]
+    batch, total = ref.make_batch(new, past, page, kv_heads, dim, seed=100 + case)
+    q = rows_of(sum(new), heads, dim, dtype)
+    for causal in (True, False):
+        got = lm.attention(q, window=window, causal=causal, **widened(batch))
+        ref.check_attention(got, ref.attention64(q, batch, total, new, window=window, causal=causal), dtype)
+
+
+@pytest.mark.parametrize("rows", [150, 300])
+def test_nan_and_missing_pages_in_prompts_under_a_wide_bound(rows):
+    new, past = [rows, 200], [30, 100]
+    batch, total = ref.make_batch(new, past, 16, 2, 64, seed=3)
+    q = rows_of(sum(new), 4, 64, BF16)
+    clean = lm.attention(q, window=70, **widened(batch))
+    ref.check_attention(clean, ref.attention64(q, batch, total, new, window=70), BF16)
+    at = int(batch["block_table"][0, 5])
+    batch["cache"][1].view(torch.uint8)[at, 1, 4, 33] = 0x7f    # token 84 of sequence 0: rows 54..123 attend it
+    out, lse = lm.attention(q, window=70, **widened(batch))
+    hit = torch.zeros(out.shape, dtype=torch.bool, device="cuda")
+    hit[54:124, 2:4, 33] = True
+    assert torch.equal(torch.isnan(out), hit) and bool(torch.isfinite(lse).all())
+    batch["block_table"][0, 5] = -1                             # nobody attends its 16 tokens, nor the NaN
+    for b in (batch, widened(batch)):
+        gone = lm.attention(q, window=70, **b)
+        assert bool(torch.isfinite(gone[0]).all())
+    few, many = lm.attention(q, window=70, **batch), gone
+    top = float(batch["cache"][1].float().nan_to_num().abs().max() * batch["cache"][3].max())
+    assert bool(((few[0].float() - many[0].float()).abs() <= 2 * ref.LIMIT[BF16] * top + 2 * ref.half_step(few[0].float(), BF16)).all())
+    assert torch.allclose(few[1], many[1], rtol=2e-5, atol=2e-5)
+
+
+def test_prompts_longer_than_their_text_under_a_wide_bound():
+    """The device says that a sequence has fewer tokens than rows: the first rows stand before the text."""
+    batch, total = ref.make_batch([400, 300], [0, 50], 64, 2, 128)
+    q = rows_of(700, 8, 128, F16)
+    batch["kv_len"][0] = 90
+    for b in (batch, widened(batch)):
+        out, lse = lm.attention(q, **b)
+        assert bool((out[:310] == 0).all()) and bool(torch.isinf(lse[:310]).all())
+        assert bool(torch.isfinite(lse[310:]).all())
+        only = {**b, "row_start": torch.tensor([0, 90, 390], dtype=torch.int32, device="cuda"), "max_rows": 300}
+        same = lm.attention(q[310:], **only)
+        limit = 2 * ref.LIMIT[F16] * float(batch["cache"][1].float().nan_to_num().abs().max() * batch["cache"][3].max()) + 2 * ref.half_step(same[0].float(), F16)
+        assert bool(((out[310:].float() - same[0].float()).abs() <= limit).all())
