@@ -473,7 +473,9 @@ int ogle_cuda_kv_append(const OglePagedBatch* batch, const OgleAppendParams* p, 
  * not reach it, whatever its bytes are. Scores, statistics and sums are in fp32; for fp32 activations the queries and weights enter
  * the products as two 16-bit parts.
  * The caller lends `workspace` (>= ogle_cuda_paged_attention_workspace_bytes, 16-byte aligned); nothing in it has to be
- * cleared, and it may be reused once the stream has passed the call. Strides in elements, multiples of 16 bytes. */
+ * cleared, and it may be reused once the stream has passed the call. Where no more than OGLE_ATTENTION_NO_WORKSPACE bytes are asked
+ * for, nothing is read or written there. Strides in elements, multiples of 16 bytes. */
+#define OGLE_ATTENTION_NO_WORKSPACE 64
 typedef struct {
     const void* q;
     void* out;

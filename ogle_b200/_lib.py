@@ -14,6 +14,7 @@ RT_LIB_PATH = os.path.join(_HERE, "libogle_rt.so")
 OGLE_MAX_CONCAT_INPUTS = 16
 
 MATH_FP32, MATH_TF32, MATH_TF32X3 = 0, 1, 2
+ATTENTION_NO_WORKSPACE = 64
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 ACT_NONE, ACT_CLIP, ACT_RELU = 0, 1, 2
 

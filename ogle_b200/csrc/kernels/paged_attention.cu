@@ -975,7 +975,8 @@ size_t few_workspace(const OglePagedBatch* b, const OgleAttentionParams* p) {
     if (!some_few(b)) return 0;
     return with_form(choose(b), [&](auto dp, auto mt, auto split) {
         using F = Form<decltype(dp)::value, decltype(mt)::value, decltype(split)::value>;
-        // with clusters it is not read, but a caller without a workspace finds out at every size
+        // with clusters it is not touched, but a caller without a workspace finds out at every size
+        static_assert(sizeof(Cut) <= OGLE_ATTENTION_NO_WORKSPACE && 2 * F::kPart * sizeof(float) > OGLE_ATTENTION_NO_WORKSPACE, "");
         if (cluster_of<decltype(dp)::value, decltype(mt)::value, decltype(split)::value>(b, p)) return sizeof(Cut);
         return size_t(ranges_of(b, F::kRows, F::kBlocks)) * (2 * F::kPart * sizeof(float) + sizeof(Cut));
     });
