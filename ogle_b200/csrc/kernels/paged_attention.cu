@@ -11,7 +11,7 @@
 // Where there are few segments, none of them long, the blocks of a cluster have one segment instead and add their parts
 // through each other's shared memory: one launch, no workspace.
 //
-// Measured: 64 sequences of up to 8000 tokens, 32 query heads to 8 of 128, 570 MB: 111 us, 79 % of what a copy reaches. 3 sequences
+// Measured: 64 sequences of up to 8000 tokens, 32 query heads to 8 of 128, 570 MB: 111 to 119 us, 74 to 79 % of what a copy reaches. 3 sequences
 // of up to 200000 tokens, 16 query heads to one: 52 us, 3.9 TB/s with the join - 500 instructions a step of 16 keys, each warp
 // waiting 2 of 8 cycles for the one before (four blocks an SM, the queries in shared memory; three, in registers: 56). What is short is bound
 // by latency: one sequence of 700 tokens takes 9 us on the device.
