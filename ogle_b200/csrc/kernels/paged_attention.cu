@@ -359,7 +359,8 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
         uint4* const queries = reinterpret_cast<uint4*>(smem + F::kQueries) + lane;
         const float kDown = -3e38f;               // m of a row that has not met a key
         float rs[MT][NR], noff[MT][NR], l[MT][NR];            // weight 2^(s rs + noff) of product s; noff = kLift - m
-#pragma unroll
+        // (one copy of the code: it runs once a segment, and fetching a second took longer than running it - drafts of 5 rows 62 us, so 58)
+#pragma unroll 1
         for (int i = 0; i < MT * NR; ++i) {
             const int mt = i / NR, r = i % NR;
             if (i % kWarps != warp || segment.steps == 0) continue;     // steps 0: a range that has the segment's cost alone
@@ -964,9 +965,9 @@ int ranges_of(const OglePagedBatch* b, int rows, int blocks) {
 int few_limit(const OglePagedBatch* b) {
     if (b->dtype == OGLE_F32 || b->head_dim > 128) return 0;
     const long long rows = (long long)(b->max_rows < b->n_rows ? b->max_rows : b->n_rows) * (b->q_heads / b->kv_heads);
-    const long long keys = (long long)b->n_seqs * b->kv_heads * b->max_kv_len * (b->head_dim <= 64 ? 64 : 128) / 128;
-    const long long limit = 64 + 5000000 / (keys > 5000 ? keys : 5000);
-    return rows > limit ? int(limit) : 0;
+    const double keys = double(b->n_seqs) * b->kv_heads * b->max_kv_len * (b->head_dim <= 64 ? 0.5 : 1.0);
+    const int limit = 64 + int(5e6 / (keys > 5e3 ? keys : 5e3));
+    return rows > limit ? limit : 0;
 }
 // Whether some sequence can have few rows, as far as the host knows.
 bool some_few(const OglePagedBatch* b) { return !few_limit(b) || (long long)b->n_seqs * b->max_rows != b->n_rows; }
