@@ -15,7 +15,7 @@
 // Shared memory has the products' operands to deliver beside the conversion's traffic; two S of 64 keys a tile of rows, which
 // overlap more, read the queries twice as often and were slower (3.2 us a tile of keys, so 2.1: 1150 TFLOP/s where texts are long). The
 // tensor cores and the exponentials each need half of that; taking a quarter of the exponentials off the special function units, by a
-// polynomial, made it slower. Six prompts of 2000 rows over 2500 earlier tokens: 358 us, 500 TFLOP/s - an item's beginning and end
+// polynomial, made it slower. Six prompts of 2000 rows over 2500 earlier tokens: 339 us, 525 TFLOP/s - an item's beginning and end
 // (queries, the first scores, the last sums, results: 10 us) take as long as its tiles there.
 //
 // Work: items (sequence, tile of 256 rows, kv head) laid end to end by their tiles of keys, cut into one range a block; parts
@@ -424,8 +424,10 @@ paged_prompt_kernel(PromptArgs p) {
             const int seq_row = row / B.group, head = h * B.group + row % B.group;
             const Span k = span_of(item.s, seq_row, seq_row, a.causal, a.window);
             if (tiles > 0 && mine) {
-                // queries of the warp's 32 rows, 16 values a lane: rows side by side are read together, all of them before the first is used
-                constexpr int kLanes = DP / 16, kTogether = 32 / kLanes, kRounds = 32 / kTogether, kAtOnce = kRounds < 8 ? kRounds : 8;
+                // queries of the warp's 32 rows, 16 values a lane: rows side by side are read together, two rounds before the first is used (what
+                // runs once an item is short code: with all eight rounds, and the results' four parts below, unrolled, its instructions took
+                // longer to fetch - six prompts 359 us, so 339)
+                constexpr int kLanes = DP / 16, kTogether = 32 / kLanes, kRounds = 32 / kTogether, kAtOnce = kRounds < 2 ? kRounds : 2;
                 const int d = lane % kLanes * 16;
                 const long long mine_at = (item.s.row0 + seq_row) * a.q_row + head * a.q_head;
                 const bool back = a.scale_log2 < 0.f;        // the largest product is then the largest x
@@ -577,8 +579,9 @@ paged_prompt_kernel(PromptArgs p) {
                 // whole lines: 64 bytes of each of its rows at a time, pieces of 16 bytes turned by the row.
                 unsigned char* const turn = smem + L::kQ + q * L::kTile + (warp & 3) * 32 * (DP * 2);
                 const float inv = !whole ? v_unit : (l == 0.f ? 0.f : v_unit / l);
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < DP / 32; ++c) {
+                    const uint32_t bad = c & 2 ? (c & 1 ? nan[3] : nan[2]) : (c & 1 ? nan[1] : nan[0]);
                     uint32_t o[32];
                     if (tiles > 0) {
                         tmem_load32(o, o_at + c * 32);
@@ -588,7 +591,7 @@ paged_prompt_kernel(PromptArgs p) {
                         for (int x = 0; x < 32; ++x) o[x] = 0;
                     }
 #pragma unroll
-                    for (int x = 0; x < 32; ++x) o[x] = nan[c] >> x & 1 ? 0x7fc00000u : __float_as_uint(__uint_as_float(o[x]) * inv);
+                    for (int x = 0; x < 32; ++x) o[x] = bad >> x & 1 ? 0x7fc00000u : __float_as_uint(__uint_as_float(o[x]) * inv);
                     if (!whole) {                  // 128 bytes of each row
                         __syncwarp();
 #pragma unroll
