@@ -15,7 +15,7 @@
 // Shared memory has the products' operands to deliver beside the conversion's traffic; two S of 64 keys a tile of rows, which
 // overlap more, read the queries twice as often and were slower (3.2 us a tile of keys, so 2.1: 1150 TFLOP/s where texts are long). The
 // tensor cores and the exponentials each need half of that; taking a quarter of the exponentials off the special function units, by a
-// polynomial, made it slower. Six prompts of 2000 rows over 2500 earlier tokens: 339 us, 525 TFLOP/s - an item's beginning and end
+// polynomial, made it slower. Six prompts of 2000 rows over 2500 earlier tokens: 331 us, 538 TFLOP/s - an item's beginning and end
 // (queries, the first scores, the last sums, results: 10 us) take as long as its tiles there.
 //
 // Work: items (sequence, tile of 256 rows, kv head) laid end to end by their tiles of keys, cut into one range a block; parts
@@ -426,7 +426,7 @@ paged_prompt_kernel(PromptArgs p) {
             if (tiles > 0 && mine) {
                 // queries of the warp's 32 rows, 16 values a lane: rows side by side are read together, two rounds before the first is used (what
                 // runs once an item is short code: with all eight rounds, and the results' four parts below, unrolled, its instructions took
-                // longer to fetch - six prompts 359 us, so 339)
+                // longer to fetch - six prompts 359 us, so 331)
                 constexpr int kLanes = DP / 16, kTogether = 32 / kLanes, kRounds = 32 / kTogether, kAtOnce = kRounds < 2 ? kRounds : 2;
                 const int d = lane % kLanes * 16;
                 const long long mine_at = (item.s.row0 + seq_row) * a.q_row + head * a.q_head;
@@ -623,7 +623,7 @@ paged_prompt_kernel(PromptArgs p) {
                     constexpr int kPieces = DP / 8, kTogether = 32 / kPieces;
                     const int piece = lane % kPieces, n_rows = item.m_end - item.m0 - q * kTileRows - (warp & 3) * 32;
                     const long long mine_at = (item.s.row0 + seq_row) * a.out_row + head * a.out_head;
-#pragma unroll 4
+#pragma unroll 2
                     for (int x = 0; x < 32; x += kTogether) {
                         const int at = x + lane / kPieces;
                         const long long to = __shfl_sync(~0u, mine_at, at);
