@@ -78,6 +78,8 @@ __global__ void __launch_bounds__(kThreads, 4) adjust_logits_kernel(LogitsArgs a
     const int begin = blockIdx.x * a.range - shift, end = min(begin + a.range, p.vocab), first = max(begin, 0);
     grid_dependency_trigger();
     grid_dependency_wait();
+    // The grid has pieces for the row that begins farthest behind its boundary: of another row the last block may be past the vocabulary.
+    if (begin >= end) return;
     const unsigned* allowed = p.allowed ? p.allowed + r * p.allowed_stride : nullptr;
     const int last_word = (p.vocab - 1) / 32;
     const int token0 = p.tokens ? max(p.token_start[r], 0) : 0, n_tokens = p.tokens ? min(p.token_start[r + 1], p.n_tokens) - token0 : 0;

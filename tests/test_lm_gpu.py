@@ -747,3 +747,33 @@ def test_prompts_longer_than_their_text_under_a_wide_bound():
         same = lm.attention(q[310:], **only)
         limit = 2 * ref.LIMIT[F16] * float(batch["cache"][1].float().nan_to_num().abs().max() * batch["cache"][3].max()) + 2 * ref.half_step(same[0].float(), F16)
         assert bool(((out[310:].float() - same[0].float()).abs() <= limit).all())
+
+
+def logits_in_place(view, tokens, starts, prompt, rep, pres, freq, biases, allowed):
+    d = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+    bs = np.concatenate([[0], np.cumsum([len(b[0]) for b in biases])]).astype(np.int32)
+    return lm.adjust_logits(view, d(tokens), d(starts), d(prompt), d(rep), d(pres), d(freq), d(np.concatenate([b[0] for b in biases])),
+                            d(np.concatenate([b[1] for b in biases])), d(bs), d(allowed), out=view)
+
+
+@pytest.mark.parametrize("vocab", [1021, 1022, 1023, 2042, 2045, 8190, 32767])
+@pytest.mark.parametrize("rows", [1, 3])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_logits_of_vocabularies_just_below_whole_pieces(vocab, rows, dtype):
+    """A row that begins on a 16-byte boundary needs a block less than one that does not: penalties are applied once, in place too, tokens far
+    outside the vocabulary are ignored, and nothing behind a row is touched."""
+    x, tokens, starts, prompt, rep, pres, freq, biases, allowed = logits_case(rows, vocab, 600, 9, True, dtype, seed=vocab + rows)
+    rng = np.random.default_rng(rows)
+    out_of = rng.random(len(tokens)) < 0.3
+    tokens[out_of] = vocab + (rng.random(int(out_of.sum())) * 3000).astype(np.int32)
+    case = (tokens, starts, prompt, rep, pres, freq, biases, allowed)
+    want = torch.from_numpy(logits32(x.float().numpy(), *case)).to(dtype)
+    wide = torch.full((rows + 1, vocab // 8 * 8 + 4096), 9.0, dtype=dtype, device="cuda")      # rows on boundaries
+    for offset in (0, 1):
+        wide.fill_(9.0)
+        view = wide[:rows, offset:offset + vocab]
+        view.copy_(x)
+        got = logits_in_place(view, *case)
+        assert got.data_ptr() == view.data_ptr() and torch.equal(got.cpu(), want)
+        assert bool((wide[:, :offset] == 9).all()) and bool((wide[:rows, offset + vocab:] == 9).all()) and bool((wide[rows] == 9).all())
+    assert torch.equal(run_logits(x, *case).cpu(), want)
