@@ -624,7 +624,12 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
             if (n < count) issue(n, (n ^ i) >> 5 ? p1 : p0);
         }
         __syncthreads();                          // every warp is through with its ring: the parts take its place
-        if (gave_up && !a.cluster) return;
+        if (gave_up && !a.cluster) {
+            // the segments that the rest of the range begins get their notes all the same: the join follows whatever stands there
+            if (tid == 0 && a.by_segment)
+                while (next_segment<kRows>(a, walk, segment)) {}
+            return;
+        }
 
         // the warps' parts: values [kRows][DP + 4], then m and l
         float* const mine = reinterpret_cast<float*>(smem) + warp * kRows * (DP + 4);

@@ -777,3 +777,40 @@ def test_logits_of_vocabularies_just_below_whole_pieces(vocab, rows, dtype):
         assert got.data_ptr() == view.data_ptr() and torch.equal(got.cpu(), want)
         assert bool((wide[:, :offset] == 9).all()) and bool((wide[:rows, offset + vocab:] == 9).all()) and bool((wide[rows] == 9).all())
     assert torch.equal(run_logits(x, *case).cpu(), want)
+
+
+def attention_through_c(q, batch, out, lse, fill):
+    """lm.attention by way of the C entry point, in a workspace whose every byte is `fill`. Returns the workspace's size."""
+    rows, heads, dim = q.shape
+    lib = _lib.cuda_lib()
+    b = lm._batch(batch["cache"], batch["block_table"], batch["kv_len"], batch["max_kv_len"], batch["row_start"], batch["max_rows"], rows, heads, q.dtype)
+    p = lm._ATTENTION(q.data_ptr(), out.data_ptr(), lse.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1), dim ** -0.5, 1, 0, 0)
+    n = lib.ogle_cuda_paged_attention_workspace_bytes(b, p)
+    workspace = torch.full((n,), fill, dtype=torch.uint8, device="cuda")
+    assert lib.ogle_cuda_paged_attention(b, p, workspace.data_ptr(), n, lm._stream()) == 0
+    return n
+
+
+@pytest.mark.parametrize("past,kv_heads", [([30000] + [10] * 19, 8), ([100000, 9, 9], 1), ([40000] + [30] * 90, 8)])
+def test_a_block_that_gives_up_leaves_segments_behind_it(past, kv_heads):
+    """Ranges that have several segments, in a workspace of arbitrary bytes: the call ends, reports itself and stores nothing outside its rows."""
+    n = len(past)
+    batch, total = ref.make_batch([1] * n, past, 64, kv_heads, 64)
+    q = rows_of(n, 2 * kv_heads, 64, BF16)
+    want = lm.attention(q, **batch)
+    wide, lse = torch.full((n + 2, 2 * kv_heads, 64), 5.0, dtype=BF16, device="cuda"), torch.full((n + 2, 2 * kv_heads), 5.0, device="cuda")
+    out, lib = wide[1:n + 1], _lib.cuda_lib()
+    assert attention_through_c(q, batch, out, lse[1:n + 1], 0x7f) > _lib.ATTENTION_NO_WORKSPACE      # ranges, no clusters
+    assert torch.equal(out, want[0]) and torch.equal(lse[1:n + 1], want[1])
+    lib.ogle_cuda_set_wait_limit(0)
+    try:
+        attention_through_c(q, batch, out, lse[1:n + 1], 0x7f)
+        torch.cuda.synchronize()
+        assert lib.ogle_cuda_device_status() == -6 and lib.ogle_cuda_device_status_detail() == 9
+    finally:
+        lib.ogle_cuda_set_wait_limit(-1)
+        lib.ogle_cuda_clear_device_status()
+    for t in (wide, lse):
+        assert bool((t[0] == 5).all()) and bool((t[n + 1] == 5).all())
+    again = lm.attention(q, **batch)
+    assert torch.equal(again[0], want[0]) and torch.equal(again[1], want[1])
