@@ -1045,6 +1045,7 @@ int ogle_cuda_paged_attention(const OglePagedBatch* batch, const OgleAttentionPa
     if (!paged::strides_ok(p->q, p->q_row, p->q_head, batch->dtype) || !paged::strides_ok(p->out, p->out_row, p->out_head, batch->dtype) || !aligned16(workspace))
         return OGLE_ERR_ALIGNMENT;
     if (workspace_bytes < ogle_cuda_paged_attention_workspace_bytes(batch, p)) return OGLE_ERR_INVALID;
+    if (a.b.max_rows == 0) return OGLE_OK;       // no row of any sequence counts: there would be no segment to launch for
     a.q = p->q; a.out = p->out; a.lse = p->lse;
     a.q_row = p->q_row; a.q_head = p->q_head; a.out_row = p->out_row; a.out_head = p->out_head;
     a.scale_log2 = p->scale * 1.4426950408889634f;

@@ -814,3 +814,15 @@ def test_a_block_that_gives_up_leaves_segments_behind_it(past, kv_heads):
         assert bool((t[0] == 5).all()) and bool((t[n + 1] == 5).all())
     again = lm.attention(q, **batch)
     assert torch.equal(again[0], want[0]) and torch.equal(again[1], want[1])
+
+
+def test_a_bound_of_no_rows_leaves_everything_as_it_is():
+    batch, total = ref.make_batch([2, 1], [30, 400], 16, 2, 64)
+    batch["max_rows"] = 0
+    q = rows_of(3, 4, 64, BF16)
+    out, before = torch.full_like(q, 5.0), [t.clone() for t in batch["cache"]]
+    assert lm.attention(q, out=out, **batch)[0] is out
+    lm.append(q[:, :2], q[:, 2:], q=q, out=out, **batch)
+    torch.cuda.synchronize()
+    assert bool((out == 5).all()) and _lib.cuda_lib().ogle_cuda_device_status() == 0
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(batch["cache"], before))
