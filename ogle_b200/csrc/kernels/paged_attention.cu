@@ -287,11 +287,11 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
     unsigned char* const smem = dynamic + ((1024 - (tc::smem_u32(dynamic) & 1023)) & 1023);
     const Batch& B = a.b;
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, c4 = lane & 3, r8 = lane >> 2;
-    if (tid < kWarps * F::kStages) tc::mbar_init(&bars[0][0] + tid, 1);
-    if (tid == 0) {
-        gave_up = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if (tid < kWarps * F::kStages) {
+        tc::mbar_init(&bars[0][0] + tid, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");       // by each thread that has initialised one
     }
+    if (tid == 0) gave_up = 0;
     grid_dependency_trigger();
     grid_dependency_wait();
     if (a.cluster) {

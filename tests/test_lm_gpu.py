@@ -826,3 +826,18 @@ def test_a_bound_of_no_rows_leaves_everything_as_it_is():
     torch.cuda.synchronize()
     assert bool((out == 5).all()) and _lib.cuda_lib().ogle_cuda_device_status() == 0
     assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(batch["cache"], before))
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_first_copies_of_many_short_blocks(dim):
+    """Blocks that ask for copies as soon as they have begun, in both kinds of division, again and again: the same bits every time."""
+    n = 60
+    batch, total = ref.make_batch([1] * n, [(53 * b) % 130 for b in range(n)], 16, 4, dim, seed=dim)
+    q = rows_of(n, 8, dim, BF16)
+    for b in (batch, widened(batch)):
+        want = lm.attention(q, **b)
+        ref.check_attention(want, ref.attention64(q, b, total, [1] * n), BF16)
+        for _ in range(50):
+            got = lm.attention(q, **b)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert _lib.cuda_lib().ogle_cuda_device_status() == 0
