@@ -974,7 +974,7 @@ int few_limit(const OglePagedBatch* b) {
     const int limit = 64 + int(5e6 / (keys > 5e3 ? keys : 5e3));
     return rows > limit ? limit : 0;
 }
-// Whether some sequence can have few rows, as far as the host knows.
+// Whether to launch the form for few rows, too: not where n_rows is max_rows of every sequence.
 bool some_few(const OglePagedBatch* b) { return !few_limit(b) || (long long)b->n_seqs * b->max_rows != b->n_rows; }
 
 size_t few_workspace(const OglePagedBatch* b, const OgleAttentionParams* p) {
@@ -1054,10 +1054,14 @@ int ogle_cuda_paged_attention(const OglePagedBatch* batch, const OgleAttentionPa
     a.spin_limit = tc::role_wait_limit();
     a.error = error_flag_ptr();
     if (!a.error) return OGLE_ERR_CUDA;
-    a.few_limit = few_limit(batch);
-    if (a.few_limit) {
+    const int limit = few_limit(batch);
+    if (limit) {
+        // where the host sees no sequence of few rows, the prompt form takes those that the device has all the same: row_start may hold fewer
+        // rows than n_rows
+        const bool few = some_few(batch);
+        a.few_limit = few ? limit : 0;
         rc = launch_prompts(batch, a, workspace, stream);
-        if (rc != OGLE_OK || !some_few(batch)) return rc;
+        if (rc != OGLE_OK || !few) return rc;
     }
     return with_form(choose(batch), [&](auto dp, auto mt, auto split) -> int {
         constexpr int DP = decltype(dp)::value, MT = decltype(mt)::value;

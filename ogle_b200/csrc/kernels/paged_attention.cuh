@@ -22,7 +22,7 @@ struct AttnArgs {
     int causal, window;
     float* parts;                                // [ranges][2][kRows] x (DP + 2)
     struct Cut* cuts;                            // [ranges]
-    int few_limit;                               // sequences of more rows x query heads of a group are the prompt form's
+    int few_limit;                               // sequences of more rows x query heads of a group are the prompt form's; 0: all are one form's
     int by_segment;                              // tiles of rows a sequence can have, where cuts are kept by segment; else 0
     int cluster;                                 // blocks of a cluster that has one segment, or 0: ranges
     uint32_t spin_limit;

@@ -841,3 +841,42 @@ def test_first_copies_of_many_short_blocks(dim):
             got = lm.attention(q, **b)
             assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     assert _lib.cuda_lib().ogle_cuda_device_status() == 0
+
+
+def poisoned_memory(*like):
+    """Memory of these sizes handed back to the allocator full of NaN: what the next call's results take is not what was right before."""
+    held = [torch.full_like(t, math.nan) for t in like for _ in range(2)]
+    del held
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_prompts_shorter_than_their_bound(dim, dtype):
+    """As many rows as sequences x max_rows, but fewer of them in row_start: sequences of a few rows in a padded batch are answered, too."""
+    bound, batches = 700, ([3, 700], [1, 1], [0, 60], [700, 0], [699, 5])
+    for new in batches:
+        batch, total = ref.make_batch(new, [400, 900], 64, 2, dim, seed=sum(new))
+        batch["max_rows"], n = bound, sum(new)
+        q = rows_of(2 * bound, 4, dim, dtype)
+        poisoned_memory(q)
+        out, lse = lm.attention(q, **batch)
+        ref.check_attention((out[:n], lse[:n]), ref.attention64(q[:n], batch, total, new), dtype)
+
+
+def test_a_captured_prompt_replayed_with_other_rows():
+    """A step captured for a prompt of 1024 rows, replayed with rows and lengths of other steps."""
+    rows, heads, page = 1024, 8, 64
+    batch, total = ref.make_batch([rows], [3000], page, 2, 128, seed=9)
+    q = rows_of(rows, heads, 128, BF16)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = lm.attention(q, **batch)
+    for n, past in ((1024, 3000), (3, 3000), (40, 17), (500, 0), (1, 4023)):
+        batch["row_start"].copy_(torch.tensor([0, n], dtype=torch.int32))
+        batch["kv_len"].fill_(past + n)
+        out.fill_(math.nan)
+        lse.fill_(math.nan)
+        graph.replay()
+        torch.cuda.synchronize()
+        ref.check_attention((out[:n], lse[:n]), ref.attention64(q[:n], batch, [past + n], [n]), BF16)
+        assert bool(torch.isnan(lse[n:]).all())                  # rows behind row_start's last are nobody's
