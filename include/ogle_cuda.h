@@ -431,7 +431,8 @@ typedef enum { OGLE_F32 = 0, OGLE_F16 = 1, OGLE_BF16 = 2 } OgleDataType;
  * Rows: sequence b has rows row_start[b] .. row_start[b + 1] of the call's q, k, v and out, the last of the kv_len[b] tokens
  * it has once they are appended: row i of n stands at position kv_len[b] - n + i. row_start NULL: one row a sequence.
  * The host gives bounds of what the device holds, so that nothing waits for it: max_rows (rows of a sequence) and
- * max_kv_len; rows and tokens beyond them are ignored. */
+ * max_kv_len. Rows of a sequence behind its first max_rows are ignored, and tokens from position max_kv_len on: neither stored nor
+ * attended; the others keep the positions that kv_len and row_start give them. Rows that no sequence has are ignored too. */
 typedef struct {
     int n_seqs, n_rows;            /* sequences; rows of all of them */
     int max_rows, max_kv_len;

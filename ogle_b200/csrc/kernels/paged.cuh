@@ -58,17 +58,21 @@ inline bool strides_ok(const void* p, long long row, long long head, int dtype) 
     return aligned16(p) && (row * size) % 16 == 0 && (head * size) % 16 == 0;
 }
 
-// One sequence: rows [row0, row0 + n) of the call, the last n of its len tokens.
-struct Sequence { int row0, n, len; };
+// One sequence: rows [row0, row0 + n) of the call, of which the first stands at position `first` (below 0: before the text), and len tokens.
+struct Sequence { int row0, n, len, first; };
 
-// What the device holds, cut to the bounds that the host gave: nothing outside the buffers is named whatever is in it.
+// What the device holds, cut to the bounds that the host gave: nothing outside the buffers is named whatever is in it. Rows keep the
+// positions that the whole counts give them.
 __device__ __forceinline__ Sequence sequence(const Batch& a, int b) {
     Sequence s;
     s.row0 = a.row_start ? a.row_start[b] : b;
     const int end = a.row_start ? a.row_start[b + 1] : b + 1;
-    s.len = min(max(a.kv_len[b], 0), a.max_kv_len);
+    s.len = max(a.kv_len[b], 0);
     s.row0 = min(max(s.row0, 0), a.n_rows);
-    s.n = min(min(max(end, s.row0), a.n_rows) - s.row0, a.max_rows);
+    s.n = min(max(end, s.row0), a.n_rows) - s.row0;
+    s.first = s.len - s.n;
+    s.len = min(s.len, a.max_kv_len);
+    s.n = min(s.n, a.max_rows);
     return s;
 }
 

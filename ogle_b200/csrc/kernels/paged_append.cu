@@ -151,8 +151,8 @@ __global__ void __launch_bounds__(kMaxThreads, 3) paged_append_kernel(AppendArgs
                 int pages = 0;
                 if (b0 + tid < B.n_seqs) {
                     const paged::Sequence s = paged::sequence(B, b0 + tid);
-                    const int p0 = max(s.len - s.n, 0);
-                    pages = s.n > 0 && s.len > 0 ? ((s.len - 1) >> B.page_shift) - (p0 >> B.page_shift) + 1 : 0;
+                    const int p0 = max(s.first, 0), p1 = min(s.first + s.n, s.len);
+                    pages = p1 > p0 ? ((p1 - 1) >> B.page_shift) - (p0 >> B.page_shift) + 1 : 0;
                 }
                 int sum = pages;
 #pragma unroll
@@ -178,11 +178,11 @@ __global__ void __launch_bounds__(kMaxThreads, 3) paged_append_kernel(AppendArgs
         if (b < 0) return;
     }
     const paged::Sequence s = paged::sequence(B, b);
-    if (s.n <= 0 || s.len <= 0) return;
-    const int begin = max(s.len - s.n, 0);                       // the first new token
+    const int begin = max(s.first, 0), end = min(s.first + s.n, s.len);          // the new tokens
+    if (end <= begin) return;
     const int block = (begin >> B.page_shift) + nth;             // of the sequence's blocks of tokens
-    const int t0 = max(begin, block << B.page_shift), t1 = min(s.len, (block + 1) << B.page_shift);
-    const int row0 = s.row0 + s.n - s.len;                       // row of token t: row0 + t
+    const int t0 = max(begin, block << B.page_shift), t1 = min(end, (block + 1) << B.page_shift);
+    const int row0 = s.row0 - s.first;                           // row of token t: row0 + t
     // a thread has one piece of every `stride`-th token
     const int pieces = B.dim / (2 * W), half = a.rotary_dim / 2, stride = int(blockDim.x) / pieces, my_piece = tid % pieces;
     const int my_t = tid / pieces < stride ? t0 + tid / pieces : t1;

@@ -49,8 +49,8 @@ __device__ __forceinline__ int row_tiles(const Batch& a, int n, int rows) { retu
 struct Span { int lo, hi; };
 __device__ __forceinline__ Span span_of(const paged::Sequence& s, int first_row, int last_row, int causal, int window) {
     Span k;
-    k.hi = causal ? min(s.len, s.len - s.n + last_row + 1) : s.len;
-    k.lo = window > 0 ? max(0, s.len - s.n + first_row - window + 1) : 0;
+    k.hi = causal ? min(s.len, s.first + last_row + 1) : s.len;
+    k.lo = window > 0 ? max(0, s.first + first_row - window + 1) : 0;
     k.hi = max(k.hi, 0);
     return k;
 }

@@ -880,3 +880,60 @@ def test_a_captured_prompt_replayed_with_other_rows():
         torch.cuda.synchronize()
         ref.check_attention((out[:n], lse[:n]), ref.attention64(q[:n], batch, [past + n], [n]), BF16)
         assert bool(torch.isnan(lse[n:]).all())                  # rows behind row_start's last are nobody's
+
+
+def rows64(q, batch, b, first, last, length, window=0, causal=True):
+    """(out, lse, largest |v|) of rows q at positions first.. of sequence b, over the tokens below `last`, of `length` in the cache."""
+    k, v = (ref.cached(batch["cache"][i], batch["cache"][2 + i], batch["block_table"][b], length)[:last] for i in (0, 1))
+    n, heads, dim = q.shape
+    pos, j = first + torch.arange(n)[:, None], torch.arange(last)[None]
+    hidden = (j > pos) & causal | (j <= pos - window) & (window > 0)
+    out, lse = torch.zeros(n, heads, dim, dtype=torch.float64), torch.zeros(n, heads, dtype=torch.float64)
+    for h in range(heads):
+        kh = h // (heads // k.shape[1])
+        s = (q[:, h].cpu().double() @ k[:, kh].T * dim ** -0.5).masked_fill(hidden, -math.inf)
+        lse[:, h] = torch.logsumexp(s, 1)
+        out[:, h] = torch.softmax(s, 1).nan_to_num() @ v[:, kh]
+    return out, lse, float(v.abs().max())
+
+
+@pytest.mark.parametrize("new,past,max_rows,max_kv_len", [([5], [40], 3, 45), ([5, 1], [40, 90], 5, 60), ([4, 9], [100, 30], 2, 90),
+                                                          ([900], [300], 600, 1200), ([900, 50], [300, 2000], 900, 1000)])
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_rows_and_tokens_beyond_the_bounds(new, past, max_rows, max_kv_len, dtype):
+    """They are left out; those that are left keep their positions."""
+    batch, total = ref.make_batch(new, past, 16, 2, 64, seed=max_kv_len)
+    batch.update(max_rows=max_rows, max_kv_len=max_kv_len)
+    q = rows_of(sum(new), 4, 64, dtype)
+    for window, causal in ((0, True), (37, True), (37, False)):
+        out, lse = lm.attention(q, window=window, causal=causal, **batch)
+        row = 0
+        for b, n in enumerate(new):
+            m = min(n, max_rows)
+            want = rows64(q[row:row + m], batch, b, past[b], min(total[b], max_kv_len), total[b], window, causal)
+            ref.check_attention((out[row:row + m], lse[row:row + m]), want, dtype)
+            row += n
+
+
+@pytest.mark.parametrize("new,past,max_rows,max_kv_len", [([5], [40], 3, 45), ([5, 1], [40, 90], 5, 60), ([4, 40], [100, 30], 35, 62)])
+def test_append_of_rows_beyond_the_bounds(new, past, max_rows, max_kv_len):
+    """As an append of the rows within the bounds alone."""
+    rows = sum(new)
+    qkv = rows_of(rows, 8, 64, F32, amplitude=2.0)
+    q, k, v = qkv[:, :4], qkv[:, 4:6], qkv[:, 6:]
+    table = lm.rotary_table(max(n + p for n, p in zip(new, past)), 64)
+    batch, total = ref.make_batch(new, past, 16, 2, 64)
+    before = [t.clone() for t in batch["cache"]]
+    out = torch.full((rows, 4, 64), 5.0, device="cuda")
+    lm.append(k, v, q=q, rotary=table, out=out, **{**batch, "max_rows": max_rows, "max_kv_len": max_kv_len})
+    keep = [max(0, min(n, max_rows, max_kv_len - p)) for n, p in zip(new, past)]
+    at = torch.tensor([sum(new[:b]) + i for b, m in enumerate(keep) for i in range(m)])
+    ends = [p + m if m else 0 for p, m in zip(past, keep)]
+    positions = torch.tensor([p + i for p, m in zip(past, keep) for i in range(m)])
+    for i, x in ((0, ref.rotated32(k.cpu()[at], table.cpu(), positions, False)), (1, v.cpu()[at])):
+        want = ref.append32(x, before[i], before[2 + i], batch["block_table"].cpu(), keep, ends)
+        assert torch.equal(batch["cache"][2 + i].cpu(), want[1]) and ref.same_bytes(batch["cache"][i], want[0])
+    assert torch.equal(out.cpu()[at], ref.rotated32(q.cpu()[at], table.cpu(), positions, False))
+    left = torch.ones(rows, dtype=torch.bool)
+    left[at] = False
+    assert bool((out.cpu()[left] == 5).all())
