@@ -50,7 +50,7 @@ struct Span { int lo, hi; };
 __device__ __forceinline__ Span span_of(const paged::Sequence& s, int first_row, int last_row, int causal, int window) {
     Span k;
     k.hi = causal ? min(s.len, s.first + last_row + 1) : s.len;
-    k.lo = window > 0 ? max(0, s.first + first_row - window + 1) : 0;
+    k.lo = window > 0 ? max(0, max(s.first + first_row, 0) - window + 1) : 0;        // any window: the difference of two that are not negative
     k.hi = max(k.hi, 0);
     return k;
 }

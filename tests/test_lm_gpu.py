@@ -937,3 +937,16 @@ def test_append_of_rows_beyond_the_bounds(new, past, max_rows, max_kv_len):
     left = torch.ones(rows, dtype=torch.bool)
     left[at] = False
     assert bool((out.cpu()[left] == 5).all())
+
+
+@pytest.mark.parametrize("rows", [20, 1100])
+def test_the_longest_window(rows):
+    """A window of 2^31 - 1 is none, for rows that stand before the text, too (not causal: they attend all of it)."""
+    batch, total = ref.make_batch([rows], [0], 64, 2, 64)
+    q = rows_of(rows, 4, 64, BF16)
+    batch["kv_len"].fill_(12)
+    for causal in (True, False):
+        want = lm.attention(q, causal=causal, **batch)
+        got = lm.attention(q, causal=causal, window=2 ** 31 - 1, **batch)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        assert bool(torch.isinf(want[1][:rows - 12]).all()) == causal
