@@ -374,11 +374,10 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
             for (int x = 0; x < DP / 4; ++x) top = fmaxf(top, fabsf(f[x]));
             top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
             top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-            // 2^e with |q| 2^-e below 2^12; an infinite or vanishing row stays as it is. A negative scale turns the queries' signs; scores
-            // scaled by 0 are alike, hidden ones are not
+            // 2^e with |q| 2^-e below 2^12; an infinite or vanishing row stays as it is. A negative scale turns the queries' signs
             const int e = top > 1e-30f && top <= 3e38f ? int(__float_as_uint(top) >> 23) - 126 - 12 : 0;
             const float down = __uint_as_float(uint32_t(127 - e) << 23 | (a.scale_log2 < 0.f ? 0x80000000u : 0u));
-            if (c4 == 0) row_scale[tile_row] = fmaxf(fabsf(a.scale_log2) * __uint_as_float(uint32_t(127 + e) << 23), 1e-37f);
+            if (c4 == 0) row_scale[tile_row] = fabsf(a.scale_log2) * __uint_as_float(uint32_t(127 + e) << 23);
 #pragma unroll
             for (int x = 0; x < DP / 4; ++x) f[x] *= down;
 #pragma unroll
@@ -503,7 +502,7 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                 for (int r = 0; r < NR; ++r) {
-                    rk[mt][r] = rs[mt][r] * k_scale;
+                    rk[mt][r] = fmaxf(rs[mt][r] * k_scale, 1e-37f);    // never 0: a hidden key's minus infinity has to stay one
 #pragma unroll
                     for (int nb = 0; nb < 2; ++nb)
 #pragma unroll

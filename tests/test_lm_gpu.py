@@ -950,3 +950,16 @@ def test_the_longest_window(rows):
         got = lm.attention(q, causal=causal, window=2 ** 31 - 1, **batch)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
         assert bool(torch.isinf(want[1][:rows - 12]).all()) == causal
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("new", [[1, 3], [90, 200]])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_scores_that_vanish_against_hidden_ones(dtype, new, wide):
+    """Scores whose factor is below the smallest fp32 number are 0; those of hidden keys are minus infinity all the same."""
+    batch, total = ref.make_batch(new, [50, 20], 16, 2, 64)
+    batch["cache"][2].mul_(2.0 ** -60)
+    q = rows_of(sum(new), 4, 64, dtype, amplitude=1e-18)
+    for scale in (0.0, 1e-20, -1e-20):
+        got = lm.attention(q, scale=scale, **(widened(batch) if wide else batch))
+        ref.check_attention(got, ref.attention64(q, batch, total, new, scale=scale), dtype)
