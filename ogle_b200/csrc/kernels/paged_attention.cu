@@ -358,7 +358,10 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
         // queries, once for all warps: in shared memory as the products take them (registers for them would leave room for a block less)
         uint4* const queries = reinterpret_cast<uint4*>(smem + F::kQueries) + lane;
         const float kDown = -3e38f;               // m of a row that has not met a key
-        float rs[MT][NR], noff[MT][NR], l[MT][NR];            // weight 2^(s rs + noff) of product s; noff = kLift - m
+        // weight w = 2^(s rs + noff) of product s; noff = kLift - m. Sums of weights are of w; the values' sums O are of w 2^(log2 scale + up),
+        // so that the row's largest w x scale, not its largest w, lies near 2^kLift: what a page's scale is to other rows, or to a key that
+        // hardly counts, takes no bits from this row's weights
+        float rs[MT][NR], noff[MT][NR], up[MT][NR], l[MT][NR];
         // (one copy of the code: it runs once a segment, and fetching a second took longer than running it - drafts of 5 rows 62 us, so 58)
 #pragma unroll 1
         for (int i = 0; i < MT * NR; ++i) {
@@ -398,6 +401,7 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
                 noff[mt][r] = kLift - kDown;
+                up[mt][r] = 0.f;
                 l[mt][r] = 0.f;
                 rs[mt][r] = row_scale[mt * (kSplit ? 8 : 16) + r * 8 + r8];
             }
@@ -408,7 +412,6 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
             for (int n = 0; n < NB; ++n)
 #pragma unroll
                 for (int x = 0; x < 4; ++x) O[mt][n][x] = 0.f;
-        float vref = 1.1754944e-38f, vinv = 8.507059e37f;     // the unit of O, the largest value scale met; 1 / vref
 
         for (int i = 0; i < count; ++i) {
             if ((i & 31) == 0 && i > 0) {
@@ -488,35 +491,26 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
                             }
                     }
             }
-            // weights 2^(s rk + noff), times the values' scale against the largest met so far, as A operands of the second product
-            const float scale = v_scale == 0.f ? vref : v_scale;
-            float v_log = 0.f, v_back = 1.f;      // log2 of that ratio, and its inverse for the sums of weights
-            if (scale < vref) {
-                const float ratio = scale * vinv;
-                v_log = __log2f(ratio);
-                v_back = 1.f / ratio;
-            }
+            // weights 2^(s rk + noff), and times the values' scale as A operands of the second product
+            const float v_log = v_scale > 0.f ? float(int(__float_as_uint(v_scale) >> 23) - 127) : -INFINITY;     // a power of two, or no value
             float e[MT][2][2 * NR], rk[MT][NR];
-            bool more = scale > vref;
+            bool more = false;
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                 for (int r = 0; r < NR; ++r) {
                     rk[mt][r] = fmaxf(rs[mt][r] * k_scale, 1e-37f);    // never 0: a hidden key's minus infinity has to stay one
+                    const float most = kHeadroom + kLift - fmaxf(v_log + up[mt][r], 0.f);      // of w, and of w x scale
 #pragma unroll
                     for (int nb = 0; nb < 2; ++nb)
 #pragma unroll
                         for (int y = 0; y < 2; ++y) {
-                            e[mt][nb][2 * r + y] = fmaf(S[nb][mt][2 * r + y], rk[mt][r], noff[mt][r] + v_log);
-                            more |= e[mt][nb][2 * r + y] > kHeadroom + kLift + v_log;
+                            e[mt][nb][2 * r + y] = fmaf(S[nb][mt][2 * r + y], rk[mt][r], noff[mt][r]);
+                            more |= e[mt][nb][2 * r + y] > most;
                         }
                 }
             if (__any_sync(~0u, more)) {
-                // a larger unit for a row's weights or for the values: rare
-                const float vnew = fmaxf(vref, scale), vratio = vref / vnew;
-                vref = vnew;
-                vinv = 1.f / vnew;
-                if (scale == vnew) { v_log = 0.f; v_back = 1.f; }
+                // a larger unit for a row's weights or for its values: rare
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
                     float f[NR];
@@ -528,15 +522,17 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
                         top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
                         top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
                         const float m = kLift - noff[mt][r];
-                        top = fmaxf(top, m);
-                        f[r] = exp2_fast(m - top);
-                        noff[mt][r] = kLift - top;
-                        l[mt][r] *= f[r];
-                        f[r] *= vratio;
+                        const float now = fmaxf(top, m), move = m - now;
+                        // m - log2 of the largest w x scale: smaller with this step's, or as much larger as m
+                        const float high = fminf(up[mt][r] - move, now - top - v_log);
+                        f[r] = exp2_fast(move + (high - up[mt][r]));
+                        up[mt][r] = high;
+                        noff[mt][r] = kLift - now;
+                        l[mt][r] *= exp2_fast(move);
 #pragma unroll
                         for (int nb = 0; nb < 2; ++nb)
 #pragma unroll
-                            for (int y = 0; y < 2; ++y) e[mt][nb][2 * r + y] = fmaf(S[nb][mt][2 * r + y], rk[mt][r], noff[mt][r] + v_log);
+                            for (int y = 0; y < 2; ++y) e[mt][nb][2 * r + y] = fmaf(S[nb][mt][2 * r + y], rk[mt][r], noff[mt][r]);
                     }
 #pragma unroll
                     for (int n = 0; n < NB; ++n)
@@ -549,11 +545,13 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                 for (int r = 0; r < NR; ++r) {
-                    float sum = 0.f;
+                    const float by = exp2_fast(fminf(v_log + up[mt][r], 126.f));    // beyond that w is 0
 #pragma unroll
                     for (int nb = 0; nb < 2; ++nb) {
-                        const float p0 = exp2_fast(e[mt][nb][2 * r]), p1 = exp2_fast(e[mt][nb][2 * r + 1]);
-                        sum += p0 + p1;
+                        float p0 = exp2_fast(e[mt][nb][2 * r]), p1 = exp2_fast(e[mt][nb][2 * r + 1]);
+                        l[mt][r] += p0 + p1;
+                        p0 *= by;
+                        p1 *= by;
                         const uint32_t hi = half2_bits(p0, p1);
                         if (kSplit) {
                             P[mt][2 * nb] = hi;
@@ -562,7 +560,6 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
                             P[mt][2 * nb + r] = hi;
                         }
                     }
-                    l[mt][r] = fmaf(sum, v_back, l[mt][r]);
                 }
             // the step's values, two units (32 elements) at a time
             const auto values = [&](auto at_edge) {
@@ -639,6 +636,7 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
                 float sum = l[mt][r];
                 sum += __shfl_xor_sync(~0u, sum, 1);
                 sum += __shfl_xor_sync(~0u, sum, 2);
+                const float unit = exp2_fast(-up[mt][r]);
                 float* row = mine + (mt * (kSplit ? 8 : 16) + r * 8 + r8) * (DP + 4);
 #pragma unroll
                 for (int u = 0; u < DP / 16; ++u) {
@@ -650,7 +648,7 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
                         v.x = O[mt][2 * u][2 * r]; v.y = O[mt][2 * u + 1][2 * r];
                         v.z = O[mt][2 * u][2 * r + 1]; v.w = O[mt][2 * u + 1][2 * r + 1];
                     }
-                    v.x *= vref; v.y *= vref; v.z *= vref; v.w *= vref;
+                    v.x *= unit; v.y *= unit; v.z *= unit; v.w *= unit;
                     *reinterpret_cast<float4*>(row + u * 16 + c4 * 4) = v;
                 }
                 if (c4 == 0) { row[DP] = kLift - noff[mt][r]; row[DP + 1] = sum; }

@@ -963,3 +963,69 @@ def test_scores_that_vanish_against_hidden_ones(dtype, new, wide):
     for scale in (0.0, 1e-20, -1e-20):
         got = lm.attention(q, scale=scale, **(widened(batch) if wide else batch))
         ref.check_attention(got, ref.attention64(q, batch, total, new, scale=scale), dtype)
+
+
+def check_each(got, q, batch, total, new, dtype, window=0):
+    """Against 64 bits, each element within what its own weights and values allow: LIMIT of the sum of |weight x value| - not of the largest value
+    in the cache -, 2^-20 of the largest sum of |q k| for scores above 30, the result's rounding, and for each key a smallest fp16 number, 2^-25, against the row's largest weight x scale, which stands
+    for at least 2^7; a value is at most 448 scales: 448 x 2^-32 < 2^-23 of it."""
+    out, lse = (t.double() for t in got)
+    heads, row, page = q.shape[1], 0, batch["cache"][0].shape[2]
+    group = heads // batch["cache"][0].shape[1]
+    for b, n in enumerate(new):
+        at = batch["block_table"][b, :-(-total[b] // page)].long()
+
+        def tokens(cache, scale):                               # [heads][tokens][...] of the sequence
+            x = cache.view(torch.uint8)[at].view(ref.E4M3).double() * scale[at].double()[..., None, None]
+            return x.transpose(0, 1).flatten(1, 2)[:, :total[b]].repeat_interleave(group, 0)
+
+        k, v = (tokens(batch["cache"][i], batch["cache"][2 + i]) for i in (0, 1))
+        scales = batch["cache"][3][at].double().T.repeat_interleave(page, 1)[:, :total[b]].repeat_interleave(group, 0)
+        pos, j = torch.arange(total[b] - n, total[b], device="cuda")[:, None], torch.arange(total[b], device="cuda")[None]
+        hidden = (j > pos) | (j <= pos - window) & (window > 0)
+        x = q[row:row + n].double().transpose(0, 1) * q.shape[2] ** -0.5
+        s = (x @ k.transpose(1, 2)).masked_fill(hidden, -math.inf)
+        size = (x.abs() @ k.abs().transpose(1, 2)).masked_fill(hidden, 0).amax(2, keepdim=True)
+        p = torch.softmax(s, 2)
+        want, sums = p @ v, p @ v.abs()
+        step = ref.half_step(want, dtype).clamp(min=2.0 ** -25 if dtype == F16 else 0.0)
+        limit = (ref.LIMIT[dtype] + 2.0 ** -20 * size) * sums + step + total[b] * 2.0 ** -23 * (p * scales[:, None]).amax(2, keepdim=True)
+        over = ((out[row:row + n].transpose(0, 1) - want).abs() / limit).amax()
+        assert float(over) <= 1, (b, float(over))
+        assert float((lse[row:row + n].T - torch.logsumexp(s, 2)).abs().max()) <= 2e-5 * max(1.0, float(s.masked_fill(hidden, 0).abs().max()))
+        row += n
+
+
+SPREADS = [
+    # new rows, earlier tokens, page, q heads, kv heads, dim, window: some calls of so many keys that a block goes through several pages
+    ([1] * 40, [1500 + 37 * b for b in range(40)], 16, 8, 4, 64, 0),
+    ([5] * 30, [900 + 50 * b for b in range(30)], 32, 16, 8, 128, 700),
+    ([3, 16] * 12, [1300 + 60 * b for b in range(24)], 16, 12, 4, 256, 0),
+    ([2] * 48, [1000] * 48, 16, 32, 2, 128, 0),
+    ([5, 12], [43, 200], 16, 8, 4, 128, 50),                    # rows in a window that others of the tile have left
+]
+
+
+def outliers(batch, total, apart):
+    """Every eighth page of a sequence of several, the first among them, has values 2^apart as large and keys against which queries that are
+    positive score far below all others."""
+    k, v, ks, vs = batch["cache"]
+    page = k.shape[2]
+    for b, t in enumerate(total):
+        for i in range(0, -(-t // page), 8) if t > page else ():
+            at = int(batch["block_table"][b, i])
+            vs[at] *= 2.0 ** apart
+            k.view(torch.uint8)[at] |= 0x80
+
+
+@pytest.mark.parametrize("apart", [12, 24, 40])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("case", range(len(SPREADS)))
+def test_pages_of_values_far_apart(case, dtype, apart):
+    """Large values that a row does not attend, or hardly, leave the small ones that it does attend as they are."""
+    new, past, page, heads, kv_heads, dim, window = SPREADS[case]
+    batch, total = ref.make_batch(new, past, page, kv_heads, dim, seed=200 + case)
+    outliers(batch, total, apart)
+    q = rows_of(sum(new), heads, dim, dtype, amplitude=8.0).abs()
+    for b in (batch, widened(batch)):
+        check_each(lm.attention(q, window=window, **b), q, b, total, new, dtype, window)
