@@ -424,7 +424,7 @@ typedef enum { OGLE_F32 = 0, OGLE_F16 = 1, OGLE_BF16 = 2 } OgleDataType;
 /* A batch of sequences and the cache their keys and values lie in.
  * Cache: e4m3 bytes, page p, key/value head h, token t of the page, element d at
  * p * page_stride + h * head_stride + t * token_stride + d (bytes; the same for keys and values; multiples of 16). One scale
- * for each page and head, a power of two: value = e4m3 * scale[p * kv_heads + h].
+ * for each page and head, a power of two, or 0: value = e4m3 * scale[p * kv_heads + h].
  * Token j of sequence b lies in page block_table[b * table_stride + j / page_tokens]. A page of a sequence that is
  * appended to belongs to that sequence alone; full pages may be shared. An entry outside [0, n_pages) names no page:
  * nothing is stored there, and its tokens are not attended.
@@ -452,9 +452,9 @@ typedef struct {
  * Rotation of a pair (x1, x2) by row `position` of the table: (x1 c - x2 s, x2 c + x1 s), in fp32, with c = rotary[position][i],
  * s = rotary[position][rotary_dim / 2 + i]; the pairs are (x[i], x[i + rotary_dim / 2]), or neighbours with `interleaved`. Elements
  * from rotary_dim on stay as they are; rotary NULL rotates nothing.
- * A page's scale is the smallest power of two with |x| <= 448 scale for what it has taken since its first slot was last
- * written; where a row needs a larger one, what is in the page is moved by the exponent. An infinity is stored as the largest
- * value, a NaN as NaN; neither counts for the scale.
+ * A page's scale is the smallest power of two, but 2^-120 at least, with |x| <= 448 scale for what it has taken since its first slot
+ * was last written, and 0 while that has been zeros alone; where a row needs a larger one, what is in the page is moved by the
+ * exponent. An infinity is stored as the largest value, a NaN as NaN; neither counts for the scale.
  * q may be NULL (nothing to rotate); q_out may be q. Strides in elements, multiples of 16 bytes, elements side by side. */
 typedef struct {
     const void *k, *v, *q;

@@ -263,9 +263,8 @@ __global__ void __launch_bounds__(kMaxThreads, 3) paged_append_kernel(AppendArgs
     } else {
         __syncwarp();
     }
-    float now = fmaxf(old, top > 0.f ? scale_for(top) : 0.f);
-    if (now <= 0.f) now = 1.f;
-    const float inverse = 1.f / now;                             // a power of two: exact
+    const float now = fmaxf(old, top > 0.f ? scale_for(top) : 0.f);      // 0: nothing but zeros so far (and infinities and NaN)
+    const float inverse = now > 0.f ? 1.f / now : 1.f;           // a power of two: exact
 
     auto store = [&](int t, const float (&z)[2 * W]) {
         unsigned char* y = out + (long long)(t & (page_tokens - 1)) * B.token_stride;
@@ -289,7 +288,7 @@ __global__ void __launch_bounds__(kMaxThreads, 3) paged_append_kernel(AppendArgs
         load_piece<T, W>(x0 + (row0 + t) * x_row, p, a.rotary + (long long)t * rotary_dim, half, inter, z);
         store(t, z);
     }
-    if (slot0 > 0 && old < now) {                                // what the page has already moves to the new scale
+    if (slot0 > 0 && 0.f < old && old < now) {                   // what the page has already moves to the new scale (under 0 it has no size)
         const float ratio = old * inverse;
         const int words = B.dim / 4, slots = page_tokens - (t1 - t0);
         for (int i = tid; i < slots * words; i += blockDim.x) {
@@ -301,7 +300,7 @@ __global__ void __launch_bounds__(kMaxThreads, 3) paged_append_kernel(AppendArgs
             *w = paged::e4m3x2(fl.x * ratio, fl.y * ratio) | paged::e4m3x2(fh.x * ratio, fh.y * ratio) << 16;
         }
     }
-    if (tid == 0 && old != now) *scale = now;
+    if (tid == 0 && (slot0 == 0 || old != now)) *scale = now;
 }
 
 }  // namespace

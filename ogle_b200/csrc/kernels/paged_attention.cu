@@ -435,10 +435,8 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
             }
             if (++get == F::kStages) { get = 0; parity ^= 1; }
             const int j0 = j_begin + (i * kWarps + warp) * kChunk;
-            float k_scale = __shfl_sync(~0u, ks[0], i & 31);
-            const float v_scale = __shfl_sync(~0u, vs[0], i & 31);
-            const bool edge = j0 < inner_lo || j0 + kChunk > inner_hi || k_scale == 0.f;
-            if (k_scale == 0.f) k_scale = 1.f;    // no page: all is hidden below
+            const float k_scale = __shfl_sync(~0u, ks[0], i & 31), v_scale = __shfl_sync(~0u, vs[0], i & 31);
+            const bool edge = j0 < inner_lo || j0 + kChunk > inner_hi || k_scale == 0.f;       // 0: no page, or one of zeros
             // products of queries and keys; rows of parts are put together
             float S[2][MT][4];
 #pragma unroll
@@ -499,7 +497,7 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                 for (int r = 0; r < NR; ++r) {
-                    rk[mt][r] = fmaxf(rs[mt][r] * k_scale, 1e-37f);    // never 0: a hidden key's minus infinity has to stay one
+                    rk[mt][r] = fmaxf(rs[mt][r] * k_scale, 1e-37f);    // never 0: a hidden key's minus infinity stays one
                     const float most = kHeadroom + kLift - fmaxf(v_log + up[mt][r], 0.f);      // of w, and of w x scale
 #pragma unroll
                     for (int nb = 0; nb < 2; ++nb)

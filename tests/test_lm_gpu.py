@@ -968,7 +968,7 @@ def test_scores_that_vanish_against_hidden_ones(dtype, new, wide):
 def check_each(got, q, batch, total, new, dtype, window=0):
     """Against 64 bits, each element within what its own weights and values allow: LIMIT of the sum of |weight x value| - not of the largest value
     in the cache -, 2^-20 of the largest sum of |q k| for scores above 30, the result's rounding, and for each key a smallest fp16 number, 2^-25, against the row's largest weight x scale, which stands
-    for at least 2^7; a value is at most 448 scales: 448 x 2^-32 < 2^-23 of it."""
+    for at least 2^7; a value is at most 448 scales: 448 x 2^-32 < 2^-23 of it. Weights are fp32 numbers: below 2^-126 of the row's largest they are 0."""
     out, lse = (t.double() for t in got)
     heads, row, page = q.shape[1], 0, batch["cache"][0].shape[2]
     group = heads // batch["cache"][0].shape[1]
@@ -988,7 +988,7 @@ def check_each(got, q, batch, total, new, dtype, window=0):
         size = (x.abs() @ k.abs().transpose(1, 2)).masked_fill(hidden, 0).amax(2, keepdim=True)
         p = torch.softmax(s, 2)
         want, sums = p @ v, p @ v.abs()
-        step = ref.half_step(want, dtype).clamp(min=2.0 ** -25 if dtype == F16 else 0.0)
+        step = ref.half_step(want, dtype).clamp(min=2.0 ** -25 if dtype == F16 else 2.0 ** -149) + total[b] * 2.0 ** -117 * scales.amax(1)[:, None, None]
         limit = (ref.LIMIT[dtype] + 2.0 ** -20 * size) * sums + step + total[b] * 2.0 ** -23 * (p * scales[:, None]).amax(2, keepdim=True)
         over = ((out[row:row + n].transpose(0, 1) - want).abs() / limit).amax()
         assert float(over) <= 1, (b, float(over))
@@ -1029,3 +1029,76 @@ def test_pages_of_values_far_apart(case, dtype, apart):
     q = rows_of(sum(new), heads, dim, dtype, amplitude=8.0).abs()
     for b in (batch, widened(batch)):
         check_each(lm.attention(q, window=window, **b), q, b, total, new, dtype, window)
+
+
+def append_rows(cache, table, x, start, together):
+    """Rows x [n, heads, dim] as keys and values of one sequence from position `start` on, in calls of so many rows."""
+    n, page = len(x), cache[0].shape[2]
+    for i in range(0, n, together):
+        part = x[i:i + together].cuda()
+        m = len(part)
+        lm.append(part, part, cache, table, torch.tensor([start + i + m], dtype=torch.int32, device="cuda"), table.shape[1] * page,
+                  row_start=torch.tensor([0, m], dtype=torch.int32, device="cuda"), max_rows=m)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("together", [1, 3, 20])
+def test_pages_that_begin_with_zeros(together, dtype):
+    """Zeros ask for no scale: it is 0 until the head has another value, and then what that needs, also in a page used before."""
+    page, heads, dim = 16, 3, 64
+    x = torch.zeros(20, heads, dim)
+    g = torch.Generator().manual_seed(2)
+    x[5:, 0] = 1e-3 * torch.randn(15, dim, generator=g)          # zeros, then small values
+    x[7, 1, 3], x[8, 1, 4] = 1e-30, -0.0                         # one value alone
+    x = x.to(dtype)                                              # the last head: zeros
+    cache = lm.new_cache(3, heads, page, dim)
+    for s in cache[2:]:
+        s.fill_(1024.0)                                          # what an earlier text has left
+    table = torch.tensor([[2, 0]], dtype=torch.int32, device="cuda")
+    append_rows(cache, table, x, 0, together)
+    for c, s in ((cache[0], cache[2]), (cache[1], cache[3])):
+        for at, first, end in ((2, 0, 16), (0, 16, 20)):
+            top = x[first:end].float().abs().amax((0, 2))
+            want = torch.where(top > 0, ref.scale_for(top), torch.zeros(()))
+            assert torch.equal(s[at].cpu(), want)
+        got, want = ref.cached(c, s, table[0], 20), x.double()
+        scale = s.cpu().double()[[2] * 16 + [0] * 4][..., None]
+        # half a step of e4m3 at the final scale, and as much where the scale has grown since (the value was rounded twice)
+        assert bool(((got - want).abs() <= torch.maximum(want.abs() * 2.0 ** -3, scale * 2.0 ** -9)).all())
+        assert bool((got[:, 2] == 0).all()) and bool((got[:5] == 0).all())
+
+
+def test_infinities_and_nan_before_the_first_value():
+    """They ask for no scale either: an infinity is the largest value that the scale has once there is one, a NaN stays one."""
+    page, heads, dim = 16, 2, 64
+    x = torch.zeros(6, heads, dim)
+    x[1, 0, 0], x[1, 0, 1], x[2, 0, 2] = math.inf, -math.inf, math.nan
+    x[3, 0, 5] = 0.01
+    x[4, 1, 7] = math.inf
+    for together in (1, 6):
+        cache = lm.new_cache(1, heads, page, dim)
+        append_rows(cache, torch.zeros(1, 1, dtype=torch.int32, device="cuda"), x, 0, together)
+        scale = float(ref.scale_for(torch.tensor(0.01)))
+        assert torch.equal(cache[2].cpu(), torch.tensor([[scale, 0.0]]))
+        got = cache[0].cpu().float()
+        assert float(got[0, 0, 1, 0]) == 448 and float(got[0, 0, 1, 1]) == -448 and math.isnan(float(got[0, 0, 2, 2]))
+        assert abs(float(got[0, 0, 3, 5]) * scale - 0.01) <= 0.01 * 2.0 ** -4
+        assert float(got[0, 1, 4, 7]) == 448
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("new,heads,dtype", [([1, 4], 8, F32), ([1, 4], 8, BF16), ([300, 260], 8, F32)])
+def test_attention_over_pages_of_zeros(dtype, new, heads, wide):
+    """Keys and values of scale 0 are zeros - scores of 0, no part in the result - and take no bits from small values beside them. What
+    their bytes are does not matter (an infinity stored before any value is 448)."""
+    batch, total = ref.make_batch(new, [200, 30], 16, 2, 64, seed=5)
+    k, v, ks, vs = batch["cache"]
+    vs.mul_(2.0 ** -30)
+    for b, t in enumerate(total):
+        for i in range(0, t // 16, 2):
+            at = int(batch["block_table"][b, i])
+            (ks if i % 4 else vs)[at] = 0.0
+            k.view(torch.uint8)[at, :, 3] = v.view(torch.uint8)[at, :, 5] = 0x7e        # 448
+    q = rows_of(sum(new), heads, 64, dtype)
+    b = widened(batch) if wide else batch
+    check_each(lm.attention(q, **b), q, b, total, new, dtype)
