@@ -4,8 +4,8 @@
 // through the keys 128 at a time:
 //   four warps    read a tile of keys and of values ahead into registers and turn them into fp16 operands: e4m3 is exact in fp16, and
 //                 a page's scale relative to the largest of the item is a power of two that is multiplied in on the way (exact
-//                 down to 2^-15 of the largest; what lies below is rounded to 2^-33 of the largest value), so that scores and
-//                 weights know nothing of pages
+//                 down to 2^-15 of the largest), so that scores and weights know nothing of pages. Where an item's pages lie
+//                 further apart, bytes alone are converted and the rows multiply by their pages' scales (see `apart`)
 //   one thread    issues the products: S = Q K^T per tile, O += P V per tile, P taken from tensor memory
 //   2 x 4 warps   a row a thread: maximum, weights 2^(x - off), their sum; P in fp16 over S; O rescaled when a row's maximum
 //                 has grown by more than 2^8
@@ -36,6 +36,10 @@ constexpr int kThreads = 16 * 32;                // 8 warps of rows, 4 of conver
 // Registers of a thread: a row has its 128 scores in them. (2 x 176 + 112 + 48) x 128 = the 128 of 512 threads at launch.
 constexpr int kRowRegisters = 176, kConvertRegisters = 112, kIssueRegisters = 48;
 constexpr int kConvertWarp = 8, kProductWarp = 12;
+// Spread, as a power of two, up to which an item's scales are multiplied into its operands. Keys: all are exact fp16 numbers then. Values, too,
+// but weights end at 2^-25 against a largest of 2^7 at least, and one that counts as 0 loses 2^-32 of a value 2^8 times the row's: 2^12 of
+// them lose 2^-12, as much as a weight's own rounding.
+constexpr int kKeySpread = 15, kValueSpread = 8;
 constexpr int kNanKeys = 8192;                   // pieces of 16 values with a NaN that an item's edges can have: 1024 keys x 8
 
 // A piece of 16 values of a token at an item's edge: which of them are NaN.
@@ -303,17 +307,112 @@ struct Bars {
     uint64_t q_full, s_full[2], p_full[2][2], pv_done[2][2], drain;      // [tile of rows][step of the tile of keys]
 };
 
+// A row's scores and weights where the item's pages lie apart, for all its tiles; false where scores did not come.
+// Scores are read twice, 32 at a time: this runs rarely, and needs few registers so. x = s rk is rounded before `off` is taken
+// away - the row's largest x comes to kLift however large it is -, and O is of w 2^(log2 scale + up), with the row's largest w x scale
+// near 2^kLift (as in the form for few rows).
+struct RowState { float off, up, l; };
+template <int DP>
+__device__ __noinline__ bool rows_apart(const AttnArgs& a, const Item& item, Bars& bars, volatile int* abort, int q, Span k, float rs, int j_first, int tiles,
+                                        uint32_t my_tiles, uint32_t s_at, uint32_t o_at, RowState& state) {
+    float off = -3e38f, up = 0.f, l = 0.f;
+    const Batch& B = a.b;
+    const int lane = threadIdx.x % 32, h = item.h;
+    for (int t = 0; t < tiles; ++t) {
+        const bool came = tc::wait_turn(&bars.s_full[q], (my_tiles + t) & 1, abort, a.spin_limit);
+        if (!__all_sync(~0u, came)) {
+            if (!came && !*abort) {
+                *abort = 1;
+                tc::record_error(a.error, kGaveUp);
+            }
+            return false;
+        }
+        after_sync();
+        // factors of the tile's eight chunks, a lane each; no page: no key
+        const int j0 = j_first + t * kKeys, j = j0 + (lane & 7) * kChunk, page = j < item.keys.hi ? page_of(B, item.b, j >> B.page_shift) : -1;
+        const float ks = page >= 0 ? __ldg(B.k_scale + (long long)page * B.kv_heads + h) : -1.f;
+        const float vs = page >= 0 ? __ldg(B.v_scale + (long long)page * B.kv_heads + h) : 0.f;
+        const float v_log = vs > 0.f ? float(int(__float_as_uint(vs) >> 23) - 127) : -INFINITY;
+        const auto read = [&](int c, uint32_t (&s)[32]) {
+            tmem_load32(s, s_at + c * 32);
+            tmem_loaded(s);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                const int key = j0 + c * 32 + i;
+                const float k_scale = __shfl_sync(~0u, ks, c * 2 + i / kChunk);
+                const float x = __fmul_rn(__uint_as_float(s[i]), fmaxf(rs * k_scale, 1e-37f));
+                s[i] = key < k.lo || key >= k.hi || k_scale < 0.f ? 0xff800000u : __float_as_uint(x);
+            }
+        };
+        float x[kKeys / kChunk], top = -INFINITY, high = INFINITY;       // of each chunk the largest
+        bool more = false;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            uint32_t s[32];
+            read(c, s);
+#pragma unroll
+            for (int g = 2 * c; g < 2 * c + 2; ++g) {
+                x[g] = __uint_as_float(s[g % 2 * kChunk]);
+#pragma unroll
+                for (int i = 1; i < kChunk; ++i) x[g] = fmaxf(x[g], __uint_as_float(s[g % 2 * kChunk + i]));
+                top = fmaxf(top, x[g]);
+                more |= x[g] - off + fmaxf(__shfl_sync(~0u, v_log, g) + up, 0.f) > kHeadroom + kLift;
+            }
+        }
+        if (__any_sync(~0u, more)) {
+            const float now = fmaxf(off, top - kLift), move = off - now;
+#pragma unroll
+            for (int g = 0; g < kKeys / kChunk; ++g) high = fminf(high, kLift - (x[g] - now) - __shfl_sync(~0u, v_log, g));
+            high = fminf(high, up - move);
+            const float f = exp2_fast(move + (high - up));
+            if (t > 0)
+#pragma unroll 1
+                for (int c = 0; c < DP / 16; ++c) {
+                    uint32_t o[16];
+                    tmem_load16(o, o_at + c * 16);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                    tc::tmem_st16(o_at + c * 16, o);
+                }
+            l *= exp2_fast(move);
+            off = now;
+            up = high;
+        }
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+            uint32_t s[32], w[16];
+            read(c, s);
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+                const float by = exp2_fast(fminf(__shfl_sync(~0u, v_log, c * 2 + i / kChunk) + up, 126.f));
+                const float e = exp2_fast(__uint_as_float(s[i]) - off), f = exp2_fast(__uint_as_float(s[i + 1]) - off);
+                l += e + f;
+                w[i / 2] = half2_bits(e * by, f * by);
+            }
+            tc::tmem_st16(s_at + c / 2 * kStep + c % 2 * 16, w);
+            if (c & 1) {
+                tmem_stored();
+                before_sync();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&bars.p_full[q][c / 2]);
+            }
+        }
+    }
+    state = RowState{off, up, l};
+    return true;
+}
+
 template <int DP>
 __global__ void __launch_bounds__(kThreads, 1)
-paged_prompt_kernel(PromptArgs p) {
+paged_prompt_kernel(const __grid_constant__ PromptArgs p) {
     using L = Layout<DP>;
     extern __shared__ __align__(16) unsigned char dynamic[];
     __shared__ __align__(8) Bars bars;
     __shared__ Walk walk;
     __shared__ Item item;
-    __shared__ uint32_t tmem_slot, top_scale[2];   // bits of the item's largest scales of keys and values
+    __shared__ uint32_t tmem_slot, top_scale[2], low_scale[2];    // bits of the item's largest and smallest scales of keys and values
     __shared__ float row_scale[2][kTileRows];      // 2^e that a row's queries were divided by
-    __shared__ int more_items, holes, nan_count;
+    __shared__ int more_items, odd_pages, nan_count;
     __shared__ volatile int gave_up;
     unsigned char* const smem = dynamic + ((1024 - (tc::smem_u32(dynamic) & 1023)) & 1023);
     const uint32_t base = tc::smem_u32(smem);
@@ -332,7 +431,8 @@ paged_prompt_kernel(PromptArgs p) {
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         gave_up = 0;
         top_scale[0] = top_scale[1] = 0;
-        holes = nan_count = 0;
+        low_scale[0] = low_scale[1] = ~0u;
+        odd_pages = nan_count = 0;
     }
     if (warp == kProductWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(&tmem_slot)), "r"(512u));
@@ -375,28 +475,38 @@ paged_prompt_kernel(PromptArgs p) {
     int j_first = 0, tiles = 0, halves = 0;        // first key, tiles of keys, tiles of rows that exist
     float k_unit = 1.f, v_unit = 1.f;              // the largest scales
     bool with_holes = false;                       // some of its tokens have no page
+    // Its pages' scales lie too far apart for operands relative to the largest, or some of its values are zeros throughout (a row that
+    // attends little else would keep nothing of the rest): operands are bytes, rows know of pages
+    bool apart = false;
     const auto begin_item = [&]() {
         j_first = item.j0;
         tiles = item.tiles;
         const int j_last = min(item.keys.hi, j_first + tiles * kKeys);
         if (tiles > 0) {
-            uint32_t top_k = 0, top_v = 0, hole = 0;
+            uint32_t top_k = 0, top_v = 0, low_k = ~0u, low_v = ~0u;
+            int odd = 0;
             for (int i = (j_first >> B.page_shift) + tid; i <= (j_last - 1) >> B.page_shift; i += kThreads) {
                 const int page = page_of(B, item.b, i);
-                if (page < 0) { hole = 1; continue; }
+                if (page < 0) { odd |= 1; continue; }
                 const long long o = (long long)page * B.kv_heads + item.h;
-                top_k = max(top_k, __float_as_uint(__ldg(B.k_scale + o)) & 0x7fffffffu);
-                top_v = max(top_v, __float_as_uint(__ldg(B.v_scale + o)) & 0x7fffffffu);
+                const uint32_t k = __float_as_uint(__ldg(B.k_scale + o)) & 0x7fffffffu, v = __float_as_uint(__ldg(B.v_scale + o)) & 0x7fffffffu;
+                top_k = max(top_k, k);
+                top_v = max(top_v, v);
+                low_k = min(low_k, k ? k : ~0u);
+                low_v = min(low_v, v ? v : ~0u);
+                if (v == 0) odd |= 2;
             }
-            if (top_k) atomicMax(&top_scale[0], top_k);
-            if (top_v) atomicMax(&top_scale[1], top_v);
-            if (hole) atomicOr(&holes, 1);
+            if (top_k) { atomicMax(&top_scale[0], top_k); atomicMin(&low_scale[0], low_k); }
+            if (top_v) { atomicMax(&top_scale[1], top_v); atomicMin(&low_scale[1], low_v); }
+            if (odd) atomicOr(&odd_pages, odd);
         }
         __syncthreads();
-        k_unit = top_scale[0] ? __uint_as_float(top_scale[0]) : 1.f;
-        v_unit = top_scale[1] ? __uint_as_float(top_scale[1]) : 1.f;
+        const auto spread = [&](int i) { return top_scale[i] ? int(top_scale[i] >> 23) - int(low_scale[i] >> 23) : 0; };
+        apart = spread(0) > kKeySpread || spread(1) > kValueSpread || (odd_pages & 2);
+        k_unit = top_scale[0] && !apart ? __uint_as_float(top_scale[0]) : 1.f;
+        v_unit = top_scale[1] && !apart ? __uint_as_float(top_scale[1]) : 1.f;
         halves = item.m_end - item.m0 > kTileRows ? 2 : 1;
-        with_holes = holes != 0;
+        with_holes = odd_pages & 1;
     };
     const auto end_item = [&]() {                  // false: no item is left, or a wait has run out
         before_sync();
@@ -405,7 +515,8 @@ paged_prompt_kernel(PromptArgs p) {
         if (gave_up) return false;
         if (tid == 0) {
             top_scale[0] = top_scale[1] = 0;
-            holes = nan_count = 0;
+            low_scale[0] = low_scale[1] = ~0u;
+            odd_pages = nan_count = 0;
             more_items = next_item(p, walk, item);
         }
         __syncthreads();
@@ -474,8 +585,8 @@ paged_prompt_kernel(PromptArgs p) {
             // scores scaled by 0 are alike, hidden ones are not
             const float rs = mine && tiles > 0 ? fmaxf(fabsf(a.scale_log2) * row_scale[q][r] * k_unit, 1e-37f) : 0.f;
 
-            float off = 0.f, bar_x = -INFINITY, l = 0.f;
-            for (int t = 0; mine && t < tiles; ++t) {
+            float off = 0.f, bar_x = -INFINITY, l = 0.f, up = 0.f;
+            for (int t = 0; mine && !apart && t < tiles; ++t) {
                 wait(&bars.s_full[q], my_tiles + t);
                 if (__any_sync(~0u, failed)) { failed = true; break; }
                 after_sync();
@@ -557,6 +668,13 @@ paged_prompt_kernel(PromptArgs p) {
                 unpair(add2(sum[0], sum[1]), e, f);
                 l += e + f;
             }
+            if (mine && apart && tiles > 0) {
+                RowState state = {-3e38f, 0.f, 0.f};
+                if (!failed && !rows_apart<DP>(a, item, bars, abort, q, k, rs, j_first, tiles, my_tiles, s_at, o_at, state)) failed = true;
+                bar_x = state.off + (kLift + kHeadroom);
+                up = state.up;
+                l = state.l;
+            }
             if (mine && tiles > 0) {
                 wait(&bars.pv_done[q][1], my_tiles + tiles - 1);
                 if (__any_sync(~0u, failed)) failed = true;
@@ -578,7 +696,9 @@ paged_prompt_kernel(PromptArgs p) {
                 // A row is a thread's; its values go through shared memory - where the tile's queries were - so that a warp stores
                 // whole lines: 64 bytes of each of its rows at a time, pieces of 16 bytes turned by the row.
                 unsigned char* const turn = smem + L::kQ + q * L::kTile + (warp & 3) * 32 * (DP * 2);
-                const float inv = !whole ? v_unit : (l == 0.f ? 0.f : v_unit / l);
+                // of O; in two factors where it can be near the smallest fp32 number
+                const float unit = apart ? exp2_fast(-0.5f * up) : v_unit, more = apart ? unit : 1.f;
+                const float inv = !whole ? unit : (l == 0.f ? 0.f : unit / l);
 #pragma unroll 1
                 for (int c = 0; c < DP / 32; ++c) {
                     const uint32_t bad = c & 2 ? (c & 1 ? nan[3] : nan[2]) : (c & 1 ? nan[1] : nan[0]);
@@ -591,7 +711,7 @@ paged_prompt_kernel(PromptArgs p) {
                         for (int x = 0; x < 32; ++x) o[x] = 0;
                     }
 #pragma unroll
-                    for (int x = 0; x < 32; ++x) o[x] = bad >> x & 1 ? 0x7fc00000u : __float_as_uint(__uint_as_float(o[x]) * inv);
+                    for (int x = 0; x < 32; ++x) o[x] = bad >> x & 1 ? 0x7fc00000u : __float_as_uint(__uint_as_float(o[x]) * more * inv);
                     if (!whole) {                  // 128 bytes of each row
                         __syncwarp();
 #pragma unroll
@@ -649,6 +769,7 @@ paged_prompt_kernel(PromptArgs p) {
         for (bool more = more_items != 0; more; more = end_item()) {
             begin_item();
             const int h = item.h, in_page = (1 << B.page_shift) - 1;
+            const float k_inverse = apart ? 1.7014118e38f : 1.f / k_unit, v_inverse = apart ? 1.7014118e38f : 1.f / v_unit;
             int page[2];                           // of the tile whose values are asked for next
             float rk[2], rv[2];                    // scales of the tile that has been asked for, against the largest
             uint4 k_raw[kRounds][kHalves], v_raw[kRounds][kHalves];
@@ -659,13 +780,16 @@ paged_prompt_kernel(PromptArgs p) {
                     page[g] = t < tiles && j < item.keys.hi ? page_of(B, item.b, j >> B.page_shift) : -1;
                 }
             };
-            const auto ask = [&](int t, const unsigned char* cache, const float* scales, float unit, uint4 (&raw)[kRounds][kHalves], float (&ratio)[2]) {
+            const auto ask = [&](int t, const unsigned char* cache, const float* scales, float inverse, uint4 (&raw)[kRounds][kHalves], float (&ratio)[2]) {
 #pragma unroll
                 for (int g = 0; g < 2; ++g) {
                     ratio[g] = 0.f;
                     const int slot = (j_first + t * kKeys + cw * 32 + g * kChunk) & in_page;
                     const unsigned char* from = cache + (long long)page[g] * B.page_stride + h * B.head_stride + (long long)(slot + row8) * B.token_stride + piece * 16;
-                    if (page[g] >= 0) ratio[g] = __ldg(scales + (long long)page[g] * B.kv_heads + h) / unit;
+                    if (page[g] >= 0) {
+                        const float scale = __ldg(scales + (long long)page[g] * B.kv_heads + h);
+                        ratio[g] = fminf(scale * inverse, 1.f);       // (apart: 1, or 0)
+                    }
 #pragma unroll
                     for (int x = 0; x < 2; ++x)
 #pragma unroll
@@ -718,8 +842,8 @@ paged_prompt_kernel(PromptArgs p) {
             };
             if (tiles > 0) {
                 look_up(0);
-                ask(0, B.k_cache, B.k_scale, k_unit, k_raw, rk);
-                ask(0, B.v_cache, B.v_scale, v_unit, v_raw, rv);
+                ask(0, B.k_cache, B.k_scale, k_inverse, k_raw, rk);
+                ask(0, B.v_cache, B.v_scale, v_inverse, v_raw, rv);
                 look_up(1);
             }
             for (int t = 0; t < tiles; ++t) {
@@ -730,13 +854,13 @@ paged_prompt_kernel(PromptArgs p) {
                 if (__any_sync(~0u, failed)) { failed = true; break; }
                 store(j0, false, smem + L::kK + st * L::kTile, k_raw, rk);
                 if (lane == 0) tc::mbar_arrive(&bars.k_full[st]);
-                ask(t + 1, B.k_cache, B.k_scale, k_unit, k_raw, rk);
+                ask(t + 1, B.k_cache, B.k_scale, k_inverse, k_raw, rk);
                 wait(&bars.v_empty[st], use + 1);
                 if (__any_sync(~0u, failed)) { failed = true; break; }
                 if (edge) store(j0, true, smem + L::kV + st * L::kTile, v_raw, rv);
                 else store(j0, false, smem + L::kV + st * L::kTile, v_raw, rv);
                 if (lane == 0) tc::mbar_arrive(&bars.v_full[st]);
-                ask(t + 1, B.v_cache, B.v_scale, v_unit, v_raw, rv);
+                ask(t + 1, B.v_cache, B.v_scale, v_inverse, v_raw, rv);
                 look_up(t + 2);
                 ++kv_tiles;
             }

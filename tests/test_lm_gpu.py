@@ -965,8 +965,8 @@ def test_scores_that_vanish_against_hidden_ones(dtype, new, wide):
         ref.check_attention(got, ref.attention64(q, batch, total, new, scale=scale), dtype)
 
 
-def check_each(got, q, batch, total, new, dtype, window=0):
-    """Against 64 bits, each element within what its own weights and values allow: LIMIT of the sum of |weight x value| - not of the largest value
+def check_each(got, q, batch, total, new, dtype, window=0, factor=1.0):
+    """Against 64 bits (scores times `factor`), each element within what its own weights and values allow: LIMIT of the sum of |weight x value| - not of the largest value
     in the cache -, 2^-20 of the largest sum of |q k| for scores above 30, the result's rounding, and for each key a smallest fp16 number, 2^-25, against the row's largest weight x scale, which stands
     for at least 2^7; a value is at most 448 scales: 448 x 2^-32 < 2^-23 of it. Weights are fp32 numbers: below 2^-126 of the row's largest they are 0."""
     out, lse = (t.double() for t in got)
@@ -983,14 +983,17 @@ def check_each(got, q, batch, total, new, dtype, window=0):
         scales = batch["cache"][3][at].double().T.repeat_interleave(page, 1)[:, :total[b]].repeat_interleave(group, 0)
         pos, j = torch.arange(total[b] - n, total[b], device="cuda")[:, None], torch.arange(total[b], device="cuda")[None]
         hidden = (j > pos) | (j <= pos - window) & (window > 0)
-        x = q[row:row + n].double().transpose(0, 1) * q.shape[2] ** -0.5
+        x = q[row:row + n].double().transpose(0, 1) * (factor * q.shape[2] ** -0.5)
         s = (x @ k.transpose(1, 2)).masked_fill(hidden, -math.inf)
         size = (x.abs() @ k.abs().transpose(1, 2)).masked_fill(hidden, 0).amax(2, keepdim=True)
         p = torch.softmax(s, 2)
         want, sums = p @ v, p @ v.abs()
-        step = ref.half_step(want, dtype).clamp(min=2.0 ** -25 if dtype == F16 else 2.0 ** -149) + total[b] * 2.0 ** -117 * scales.amax(1)[:, None, None]
+        step = ref.half_step(want, dtype).clamp(min={F32: 2.0 ** -149, F16: 2.0 ** -25, BF16: 2.0 ** -134}[dtype]) + total[b] * 2.0 ** -117 * scales.amax(1)[:, None, None]
         limit = (ref.LIMIT[dtype] + 2.0 ** -20 * size) * sums + step + total[b] * 2.0 ** -23 * (p * scales[:, None]).amax(2, keepdim=True)
-        over = ((out[row:row + n].transpose(0, 1) - want).abs() / limit).amax()
+        over = (out[row:row + n].transpose(0, 1) - want).abs() / limit
+        if dtype == F16:                                         # beyond the type's largest number: an infinity
+            over = over.masked_fill((want.abs() + limit >= 65504) & (out[row:row + n].transpose(0, 1).abs() >= 65504), 0)
+        over = over.amax()
         assert float(over) <= 1, (b, float(over))
         assert float((lse[row:row + n].T - torch.logsumexp(s, 2)).abs().max()) <= 2e-5 * max(1.0, float(s.masked_fill(hidden, 0).abs().max()))
         row += n
@@ -1087,7 +1090,7 @@ def test_infinities_and_nan_before_the_first_value():
 
 
 @pytest.mark.parametrize("wide", [False, True])
-@pytest.mark.parametrize("new,heads,dtype", [([1, 4], 8, F32), ([1, 4], 8, BF16), ([300, 260], 8, F32)])
+@pytest.mark.parametrize("new,heads,dtype", [([1, 4], 8, F32), ([1, 4], 8, BF16), ([300, 260], 8, F32), ([300, 260], 8, BF16), ([300, 260], 8, F16)])
 def test_attention_over_pages_of_zeros(dtype, new, heads, wide):
     """Keys and values of scale 0 are zeros - scores of 0, no part in the result - and take no bits from small values beside them. What
     their bytes are does not matter (an infinity stored before any value is 448)."""
@@ -1102,3 +1105,63 @@ def test_attention_over_pages_of_zeros(dtype, new, heads, wide):
     q = rows_of(sum(new), heads, 64, dtype)
     b = widened(batch) if wide else batch
     check_each(lm.attention(q, **b), q, b, total, new, dtype)
+
+
+SPREAD_PROMPTS = [
+    # new rows, earlier tokens, page, q heads, kv heads, dim, window: all of more rows than the form for few rows takes
+    ([700, 900], [300, 0], 16, 8, 2, 64, 0),
+    ([520], [2000], 64, 4, 1, 128, 0),                          # few items: cut into parts
+    ([1100, 600], [100, 900], 32, 6, 2, 80, 300),
+    ([300] * 12, [170 * b for b in range(12)], 16, 16, 2, 128, 0),
+]
+
+
+@pytest.mark.parametrize("apart", [6, 12, 24, 40])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("case", range(len(SPREAD_PROMPTS)))
+def test_prompts_over_pages_of_values_far_apart(case, dtype, apart):
+    new, past, page, heads, kv_heads, dim, window = SPREAD_PROMPTS[case]
+    batch, total = ref.make_batch(new, past, page, kv_heads, dim, seed=300 + case)
+    outliers(batch, total, apart)
+    q = rows_of(sum(new), heads, dim, dtype, amplitude=8.0).abs()
+    for b in (batch, widened(batch)):
+        check_each(lm.attention(q, window=window, **b), q, b, total, new, dtype, window)
+
+
+@pytest.mark.parametrize("which,apart", [(2, 20), (3, 20), (3, 30)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("case", range(len(SPREAD_PROMPTS)))
+def test_prompts_before_keys_or_values_of_another_size(case, dtype, which, apart):
+    """Keys or values of the text's last pages 2^apart as large: rows before them are as without them, small as theirs are."""
+    new, past, page, heads, kv_heads, dim, window = SPREAD_PROMPTS[case]
+    batch, total = ref.make_batch(new, past, page, kv_heads, dim, seed=400 + case)
+    batch["cache"][which].mul_(2.0 ** -apart)
+    for b, t in enumerate(total):
+        for i in range(max(0, t // page - 3), -(-t // page)):
+            batch["cache"][which][int(batch["block_table"][b, i])] *= 2.0 ** apart
+    if which == 3 and dtype == F16:
+        batch["cache"][3].mul_(2.0 ** 8)                        # fp16 results end at 2^-24 and at 65504
+    q = rows_of(sum(new), heads, dim, dtype, amplitude=4.0)
+    if which == 2:
+        q *= 2.0 ** 4
+    for b in (batch, widened(batch)):
+        check_each(lm.attention(q, window=window, scale=2.0 ** (apart - 4) * dim ** -0.5 if which == 2 else None, **b), q, b, total, new, dtype, window,
+                   2.0 ** (apart - 4) if which == 2 else 1.0)
+
+
+@pytest.mark.parametrize("gap", [20, 55, 62, 66])
+@pytest.mark.parametrize("rows,dtype", [(600, BF16), (600, F16)])
+def test_values_beside_a_key_of_all_weight_and_no_value(rows, dtype, gap):
+    """One key, of a page whose values are zeros, has nearly all of the weight; what the others add is near the smallest fp32 numbers."""
+    batch, total = ref.make_batch([rows], [200], 16, 2, 64, seed=6)
+    k, v, ks, vs = batch["cache"]
+    k.view(torch.uint8).zero_()
+    ks.fill_(1.0)
+    vs.mul_(2.0 ** -30)
+    at = int(batch["block_table"][0, 2])
+    vs[at] = 0.0
+    k.view(torch.uint8)[at, :, 5] = 0x38                         # 1
+    q = torch.full((rows, 4, 64), 1.0, dtype=dtype, device="cuda")
+    factor = gap / 64 * 8
+    for b in (batch, widened(batch)):
+        check_each(lm.attention(q, scale=factor / 8, **b), q, b, total, [rows], dtype, 0, factor)
