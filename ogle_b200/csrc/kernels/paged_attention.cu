@@ -634,7 +634,7 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
                 float sum = l[mt][r];
                 sum += __shfl_xor_sync(~0u, sum, 1);
                 sum += __shfl_xor_sync(~0u, sum, 2);
-                const float unit = exp2_fast(-up[mt][r]);
+                const float unit = exp2_fast(-0.5f * up[mt][r]);        // applied twice: its square can be below the smallest fp32 number
                 float* row = mine + (mt * (kSplit ? 8 : 16) + r * 8 + r8) * (DP + 4);
 #pragma unroll
                 for (int u = 0; u < DP / 16; ++u) {
@@ -646,7 +646,7 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
                         v.x = O[mt][2 * u][2 * r]; v.y = O[mt][2 * u + 1][2 * r];
                         v.z = O[mt][2 * u][2 * r + 1]; v.w = O[mt][2 * u + 1][2 * r + 1];
                     }
-                    v.x *= unit; v.y *= unit; v.z *= unit; v.w *= unit;
+                    v.x = v.x * unit * unit; v.y = v.y * unit * unit; v.z = v.z * unit * unit; v.w = v.w * unit * unit;
                     *reinterpret_cast<float4*>(row + u * 16 + c4 * 4) = v;
                 }
                 if (c4 == 0) { row[DP] = kLift - noff[mt][r]; row[DP + 1] = sum; }

@@ -1150,18 +1150,20 @@ def test_prompts_before_keys_or_values_of_another_size(case, dtype, which, apart
 
 
 @pytest.mark.parametrize("gap", [20, 55, 62, 66])
-@pytest.mark.parametrize("rows,dtype", [(600, BF16), (600, F16)])
-def test_values_beside_a_key_of_all_weight_and_no_value(rows, dtype, gap):
+@pytest.mark.parametrize("rows,seqs,dtype", [(600, 1, BF16), (600, 1, F16), (1, 1, F32), (1, 48, F32), (1, 48, BF16), (5, 48, F16), (5, 48, BF16), (40, 12, F32)])
+def test_values_beside_a_key_of_all_weight_and_no_value(rows, seqs, dtype, gap):
     """One key, of a page whose values are zeros, has nearly all of the weight; what the others add is near the smallest fp32 numbers."""
-    batch, total = ref.make_batch([rows], [200], 16, 2, 64, seed=6)
+    new = [rows] * seqs
+    batch, total = ref.make_batch(new, [200 + 1200 * (seqs > 1)] * seqs, 16, 2, 64, seed=6)
     k, v, ks, vs = batch["cache"]
     k.view(torch.uint8).zero_()
     ks.fill_(1.0)
     vs.mul_(2.0 ** -30)
-    at = int(batch["block_table"][0, 2])
-    vs[at] = 0.0
-    k.view(torch.uint8)[at, :, 5] = 0x38                         # 1
-    q = torch.full((rows, 4, 64), 1.0, dtype=dtype, device="cuda")
+    for b in range(seqs):
+        at = int(batch["block_table"][b, 2])
+        vs[at] = 0.0
+        k.view(torch.uint8)[at, :, 5] = 0x38                     # 1
+    q = torch.full((sum(new), 4, 64), 1.0, dtype=dtype, device="cuda")
     factor = gap / 64 * 8
     for b in (batch, widened(batch)):
-        check_each(lm.attention(q, scale=factor / 8, **b), q, b, total, [rows], dtype, 0, factor)
+        check_each(lm.attention(q, scale=factor / 8, **b), q, b, total, new, dtype, 0, factor)
