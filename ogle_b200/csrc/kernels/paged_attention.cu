@@ -358,7 +358,8 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
         // queries, once for all warps: in shared memory as the products take them (registers for them would leave room for a block less)
         uint4* const queries = reinterpret_cast<uint4*>(smem + F::kQueries) + lane;
         const float kDown = -3e38f;               // m of a row that has not met a key
-        // weight w = 2^(s rs + noff) of product s; noff = kLift - m. Sums of weights are of w; the values' sums O are of w 2^(log2 scale + up),
+        // weight w = 2^(s rs + noff) of product s; noff = kLift - m. (The product is rounded before the sum: so is m, and the largest x of a row comes
+        // near kLift however large it is, where a fused sum would be off by what m was rounded by.) Sums of weights are of w; the values' sums O are of w 2^(log2 scale + up),
         // so that the row's largest w x scale, not its largest w, lies near 2^kLift: what a page's scale is to other rows, or to a key that
         // hardly counts, takes no bits from this row's weights
         float rs[MT][NR], noff[MT][NR], up[MT][NR], l[MT][NR];
@@ -501,11 +502,11 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
                     const float most = kHeadroom + kLift - fmaxf(v_log + up[mt][r], 0.f);      // of w, and of w x scale
 #pragma unroll
                     for (int nb = 0; nb < 2; ++nb)
-#pragma unroll
-                        for (int y = 0; y < 2; ++y) {
-                            e[mt][nb][2 * r + y] = fmaf(S[nb][mt][2 * r + y], rk[mt][r], noff[mt][r]);
-                            more |= e[mt][nb][2 * r + y] > most;
-                        }
+                    {
+                        float* const x = &e[mt][nb][2 * r];
+                        unpair(add2(mul2(pair(S[nb][mt][2 * r], S[nb][mt][2 * r + 1]), pair(rk[mt][r], rk[mt][r])), pair(noff[mt][r], noff[mt][r])), x[0], x[1]);
+                        more |= x[0] > most || x[1] > most;
+                    }
                 }
             if (__any_sync(~0u, more)) {
                 // a larger unit for a row's weights or for its values: rare
@@ -516,21 +517,20 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
                     for (int r = 0; r < NR; ++r) {
                         const float* s0 = &S[0][mt][2 * r];
                         const float* s1 = &S[1][mt][2 * r];
-                        float top = fmaxf(fmaxf(s0[0], s0[1]), fmaxf(s1[0], s1[1])) * rk[mt][r];
+                        float top = __fmul_rn(fmaxf(fmaxf(s0[0], s0[1]), fmaxf(s1[0], s1[1])), rk[mt][r]);
                         top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
                         top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-                        const float m = kLift - noff[mt][r];
-                        const float now = fmaxf(top, m), move = m - now;
-                        // m - log2 of the largest w x scale: smaller with this step's, or as much larger as m
-                        const float high = fminf(up[mt][r] - move, now - top - v_log);
+                        const float now = fminf(noff[mt][r], kLift - top), move = now - noff[mt][r];
+                        // what brings the largest w x scale to kLift: less with this step's, or as much more as m
+                        const float high = fminf(up[mt][r] - move, kLift - (top + now) - v_log);
                         f[r] = exp2_fast(move + (high - up[mt][r]));
                         up[mt][r] = high;
-                        noff[mt][r] = kLift - now;
+                        noff[mt][r] = now;
                         l[mt][r] *= exp2_fast(move);
 #pragma unroll
                         for (int nb = 0; nb < 2; ++nb)
 #pragma unroll
-                            for (int y = 0; y < 2; ++y) e[mt][nb][2 * r + y] = fmaf(S[nb][mt][2 * r + y], rk[mt][r], noff[mt][r]);
+                            for (int y = 0; y < 2; ++y) e[mt][nb][2 * r + y] = __fadd_rn(__fmul_rn(S[nb][mt][2 * r + y], rk[mt][r]), noff[mt][r]);
                     }
 #pragma unroll
                     for (int n = 0; n < NB; ++n)

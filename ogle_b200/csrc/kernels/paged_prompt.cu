@@ -40,6 +40,7 @@ constexpr int kConvertWarp = 8, kProductWarp = 12;
 // but weights end at 2^-25 against a largest of 2^7 at least, and one that counts as 0 loses 2^-32 of a value 2^8 times the row's: 2^12 of
 // them lose 2^-12, as much as a weight's own rounding.
 constexpr int kKeySpread = 15, kValueSpread = 8;
+constexpr float kLargeScore = 4194304.f;         // 2^22: larger ones leave the fused sums
 constexpr int kNanKeys = 8192;                   // pieces of 16 values with a NaN that an item's edges can have: 1024 keys x 8
 
 // A piece of 16 values of a token at an item's edge: which of them are NaN.
@@ -240,22 +241,6 @@ __device__ __forceinline__ void tmem_load16(uint32_t (&r)[16], uint32_t addr) {
           "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(addr) : "memory");
 }
-__device__ __forceinline__ unsigned long long pair(float lo, float hi) {
-    unsigned long long r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-__device__ __forceinline__ void unpair(unsigned long long v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
-__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
-    unsigned long long r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
-    unsigned long long r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
 __device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -307,18 +292,19 @@ struct Bars {
     uint64_t q_full, s_full[2], p_full[2][2], pv_done[2][2], drain;      // [tile of rows][step of the tile of keys]
 };
 
-// A row's scores and weights where the item's pages lie apart, for all its tiles; false where scores did not come.
+// A row's scores and weights where the item's pages lie apart, or scores are too large for the fused sums of the first loop, for its tiles
+// from `state.tile` on; false where scores did not come.
 // Scores are read twice, 32 at a time: this runs rarely, and needs few registers so. x = s rk is rounded before `off` is taken
 // away - the row's largest x comes to kLift however large it is -, and O is of w 2^(log2 scale + up), with the row's largest w x scale
 // near 2^kLift (as in the form for few rows).
-struct RowState { float off, up, l; };
+struct RowState { int tile; float off, up, l; };
 template <int DP>
-__device__ __noinline__ bool rows_apart(const AttnArgs& a, const Item& item, Bars& bars, volatile int* abort, int q, Span k, float rs, int j_first, int tiles,
+__device__ __noinline__ bool rows_apart(const AttnArgs& a, const Item& item, Bars& bars, volatile int* abort, int q, Span k, float rs, bool apart, int j_first, int tiles,
                                         uint32_t my_tiles, uint32_t s_at, uint32_t o_at, RowState& state) {
-    float off = -3e38f, up = 0.f, l = 0.f;
+    float off = state.off, up = state.up, l = state.l;
     const Batch& B = a.b;
     const int lane = threadIdx.x % 32, h = item.h;
-    for (int t = 0; t < tiles; ++t) {
+    for (int t = state.tile; t < tiles; ++t) {
         const bool came = tc::wait_turn(&bars.s_full[q], (my_tiles + t) & 1, abort, a.spin_limit);
         if (!__all_sync(~0u, came)) {
             if (!came && !*abort) {
@@ -330,8 +316,8 @@ __device__ __noinline__ bool rows_apart(const AttnArgs& a, const Item& item, Bar
         after_sync();
         // factors of the tile's eight chunks, a lane each; no page: no key
         const int j0 = j_first + t * kKeys, j = j0 + (lane & 7) * kChunk, page = j < item.keys.hi ? page_of(B, item.b, j >> B.page_shift) : -1;
-        const float ks = page >= 0 ? __ldg(B.k_scale + (long long)page * B.kv_heads + h) : -1.f;
-        const float vs = page >= 0 ? __ldg(B.v_scale + (long long)page * B.kv_heads + h) : 0.f;
+        const float ks = page < 0 ? -1.f : (apart ? __ldg(B.k_scale + (long long)page * B.kv_heads + h) : 1.f);
+        const float vs = page < 0 ? 0.f : (apart ? __ldg(B.v_scale + (long long)page * B.kv_heads + h) : 1.f);
         const float v_log = vs > 0.f ? float(int(__float_as_uint(vs) >> 23) - 127) : -INFINITY;
         const auto read = [&](int c, uint32_t (&s)[32]) {
             tmem_load32(s, s_at + c * 32);
@@ -398,7 +384,7 @@ __device__ __noinline__ bool rows_apart(const AttnArgs& a, const Item& item, Bar
             }
         }
     }
-    state = RowState{off, up, l};
+    state = RowState{tiles, off, up, l};
     return true;
 }
 
@@ -586,7 +572,8 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs p) {
             const float rs = mine && tiles > 0 ? fmaxf(fabsf(a.scale_log2) * row_scale[q][r] * k_unit, 1e-37f) : 0.f;
 
             float off = 0.f, bar_x = -INFINITY, l = 0.f, up = 0.f;
-            for (int t = 0; mine && !apart && t < tiles; ++t) {
+            int t = 0;
+            for (; mine && !apart && t < tiles; ++t) {
                 wait(&bars.s_full[q], my_tiles + t);
                 if (__any_sync(~0u, failed)) { failed = true; break; }
                 after_sync();
@@ -624,6 +611,8 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs p) {
                 const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * rs;
                 if (__any_sync(~0u, top > bar_x)) {
                     const float old = bar_x - kHeadroom, now = fmaxf(top, old);
+                    // fp32 numbers lie up to 1/4 apart below this, and further where weights would notice: the other loop's
+                    if (__any_sync(~0u, top > kLargeScore || top < -kLargeScore && top > -INFINITY)) break;
                     float f = 1.f;
                     if (now > -INFINITY) {
                         f = exp2_fast(old - now);
@@ -668,9 +657,9 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs p) {
                 unpair(add2(sum[0], sum[1]), e, f);
                 l += e + f;
             }
-            if (mine && apart && tiles > 0) {
-                RowState state = {-3e38f, 0.f, 0.f};
-                if (!failed && !rows_apart<DP>(a, item, bars, abort, q, k, rs, j_first, tiles, my_tiles, s_at, o_at, state)) failed = true;
+            if (mine && t < tiles && !failed) {
+                RowState state = {t, bar_x > -INFINITY ? off : -3e38f, 0.f, l};
+                if (!rows_apart<DP>(a, item, bars, abort, q, k, rs, apart, j_first, tiles, my_tiles, s_at, o_at, state)) failed = true;
                 bar_x = state.off + (kLift + kHeadroom);
                 up = state.up;
                 l = state.l;
@@ -697,7 +686,7 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs p) {
                 // whole lines: 64 bytes of each of its rows at a time, pieces of 16 bytes turned by the row.
                 unsigned char* const turn = smem + L::kQ + q * L::kTile + (warp & 3) * 32 * (DP * 2);
                 // of O; in two factors where it can be near the smallest fp32 number
-                const float unit = apart ? exp2_fast(-0.5f * up) : v_unit, more = apart ? unit : 1.f;
+                const float more = exp2_fast(-0.5f * up), unit = more * v_unit;
                 const float inv = !whole ? unit : (l == 0.f ? 0.f : unit / l);
 #pragma unroll 1
                 for (int c = 0; c < DP / 32; ++c) {

@@ -1128,7 +1128,7 @@ def test_prompts_over_pages_of_values_far_apart(case, dtype, apart):
         check_each(lm.attention(q, window=window, **b), q, b, total, new, dtype, window)
 
 
-@pytest.mark.parametrize("which,apart", [(2, 20), (3, 20), (3, 30)])
+@pytest.mark.parametrize("which,apart", [(2, 20), (2, 30), (3, 20), (3, 30)])
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("case", range(len(SPREAD_PROMPTS)))
 def test_prompts_before_keys_or_values_of_another_size(case, dtype, which, apart):
@@ -1167,3 +1167,14 @@ def test_values_beside_a_key_of_all_weight_and_no_value(rows, seqs, dtype, gap):
     factor = gap / 64 * 8
     for b in (batch, widened(batch)):
         check_each(lm.attention(q, scale=factor / 8, **b), q, b, total, new, dtype, 0, factor)
+
+
+@pytest.mark.parametrize("factor", [1e3, 1e6, 1e9, -1e9])
+@pytest.mark.parametrize("new,past,window", [([1] * 24, [1200] * 24, 0), ([1, 3], [40, 700], 0), ([7] * 12, [900] * 12, 500), ([600, 300], [0, 900], 0), ([530], [3000], 700)])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_scores_of_any_size(new, past, window, factor, dtype):
+    """Where fp32 scores lie further apart than weights reach, the largest still has a weight, and no weight is infinite."""
+    batch, total = ref.make_batch(new, past, 16, 2, 64, seed=len(new))
+    q = rows_of(sum(new), 4, 64, dtype, amplitude=4.0)
+    for b in (batch, widened(batch)):
+        check_each(lm.attention(q, scale=factor / 8, window=window, **b), q, b, total, new, dtype, window, factor)
