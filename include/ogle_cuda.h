@@ -455,7 +455,8 @@ typedef struct {
  * A page's scale is the smallest power of two, but 2^-120 at least, with |x| <= 448 scale for what it has taken since its first slot
  * was last written, and 0 while that has been zeros alone; where a row needs a larger one, what is in the page is moved by the
  * exponent. An infinity is stored as the largest value, a NaN as NaN; neither counts for the scale.
- * q may be NULL (nothing to rotate); q_out may be q. Strides in elements, multiples of 16 bytes, elements side by side. */
+ * q may be NULL (nothing to rotate); q_out may be q. A row that stands before the text (kv_len is less than the sequence's rows) has
+ * q_out 0. Strides in elements, multiples of 16 bytes, elements side by side. */
 typedef struct {
     const void *k, *v, *q;
     void* q_out;

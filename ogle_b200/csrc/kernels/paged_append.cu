@@ -4,7 +4,7 @@
 // page's scale depends on all rows that come to it, and nothing else does, so no block waits for another and no sum has an
 // order to depend on. The rows' values stay in registers between the maximum and the rounding.
 //
-// Bound by memory where prompts are appended: 26000 rows of 32 + 2 x 8 heads of 128 in bf16, 855 MB, 188 us, 70 % of what a copy
+// Bound by memory where prompts are appended: 26000 rows of 32 + 2 x 8 heads of 128 in bf16, 855 MB, 190 us, 69 % of what a copy
 // reaches (three blocks an SM, 80 registers a thread; two blocks 221 us). Single tokens are bound by latency - row, maximum, page: 5 us
 // on the device for 1 or 96 of them, 14 us a call.
 #include <type_traits>
@@ -134,6 +134,15 @@ __device__ __forceinline__ float finite_abs(float x) {
     return a <= 3.402823466e38f ? a : 0.f;
 }
 
+// Zeros in `vecs` x 16 bytes of each head of the rows. (Out of line and behind all else, and still 1.6 us of the 26000 rows' 190: it takes
+// registers.)
+__device__ __noinline__ void clear_rows(void* out, long long row_bytes, long long head_bytes, int rows, int heads, int vecs) {
+    for (int i = threadIdx.x; i < rows * heads * vecs; i += blockDim.x) {
+        const int row = i / (heads * vecs), h = i / vecs % heads;
+        *reinterpret_cast<uint4*>(static_cast<unsigned char*>(out) + row * row_bytes + h * head_bytes + i % vecs * 16) = make_uint4(0, 0, 0, 0);
+    }
+}
+
 template <typename T, int W>
 __global__ void __launch_bounds__(kMaxThreads, 3) paged_append_kernel(AppendArgs a) {
     __shared__ int where[4];
@@ -152,7 +161,7 @@ __global__ void __launch_bounds__(kMaxThreads, 3) paged_append_kernel(AppendArgs
                 if (b0 + tid < B.n_seqs) {
                     const paged::Sequence s = paged::sequence(B, b0 + tid);
                     const int p0 = max(s.first, 0), p1 = min(s.first + s.n, s.len);
-                    pages = p1 > p0 ? ((p1 - 1) >> B.page_shift) - (p0 >> B.page_shift) + 1 : 0;
+                    pages = p1 > p0 ? ((p1 - 1) >> B.page_shift) - (p0 >> B.page_shift) + 1 : (s.n > 0 && s.first < 0);
                 }
                 int sum = pages;
 #pragma unroll
@@ -179,7 +188,8 @@ __global__ void __launch_bounds__(kMaxThreads, 3) paged_append_kernel(AppendArgs
     }
     const paged::Sequence s = paged::sequence(B, b);
     const int begin = max(s.first, 0), end = min(s.first + s.n, s.len);          // the new tokens
-    if (end <= begin) return;
+    const bool clears = s.first < 0 && nth == 0 && int(blockIdx.y) >= 2 * B.kv_heads;    // rows before the text: their queries are 0
+    if (end <= begin && !clears) return;
     const int block = (begin >> B.page_shift) + nth;             // of the sequence's blocks of tokens
     const int t0 = max(begin, block << B.page_shift), t1 = min(end, (block + 1) << B.page_shift);
     const int row0 = s.row0 - s.first;                           // row of token t: row0 + t
@@ -220,6 +230,11 @@ __global__ void __launch_bounds__(kMaxThreads, 3) paged_append_kernel(AppendArgs
                     store_values<T, W>(y0 + h * a.qo_head + p.at, x);
                     store_values<T, W>(y0 + h * a.qo_head + p.at2, x + W);
                 }
+        }
+        if (clears) {
+            const paged::Sequence before = paged::sequence(B, b);
+            clear_rows(static_cast<T*>(a.q_out) + before.row0 * a.qo_row + h0 * a.qo_head, a.qo_row * sizeof(T), a.qo_head * sizeof(T),
+                       min(before.n, -before.first), heads, B.dim * sizeof(T) / 16);
         }
         return;
     }

@@ -1178,3 +1178,23 @@ def test_scores_of_any_size(new, past, window, factor, dtype):
     q = rows_of(sum(new), 4, 64, dtype, amplitude=4.0)
     for b in (batch, widened(batch)):
         check_each(lm.attention(q, scale=factor / 8, window=window, **b), q, b, total, new, dtype, window, factor)
+
+
+@pytest.mark.parametrize("new,kv_len", [([4, 1, 30], [2, 0, 40]), ([1, 1, 1], [0, 5, 0]), ([40, 3], [0, 3])])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rotary", [0, 64])
+def test_queries_of_rows_that_stand_before_the_text(new, kv_len, dtype, rotary):
+    """The device says that a sequence has fewer tokens than rows: such rows' queries are 0, as the attention's results for them are."""
+    batch, total = ref.make_batch(new, [100] * len(new), 16, 2, 64)
+    batch["kv_len"].copy_(torch.tensor(kv_len, dtype=torch.int32))
+    rows = sum(new)
+    qkv = rows_of(rows, 10, 64, dtype)
+    q, k, v = qkv[:, :6], qkv[:, 6:8], qkv[:, 8:]
+    table = lm.rotary_table(200, rotary) if rotary else None
+    positions = torch.tensor([t - n + i for n, t in zip(new, kv_len) for i in range(n)])
+    want = ref.rotated32(q.cpu(), table.cpu(), positions.clamp(min=0), False) if rotary else q.cpu().float()
+    want[positions < 0] = 0
+    poisoned_memory(torch.empty(rows, 6, 64, dtype=dtype, device="cuda"))
+    assert torch.equal(lm.append(k, v, q=q, rotary=table, **batch).cpu(), want.to(dtype))
+    in_place = q.clone()
+    assert torch.equal(lm.append(k, v, q=in_place, out=in_place, rotary=table, **batch).cpu(), want.to(dtype))
