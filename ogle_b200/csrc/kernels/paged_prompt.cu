@@ -901,10 +901,6 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs p) {
                             if (!last) tc::umma_commit(&bars.k_empty[(now + 1) & 1]);
                         }
                     }
-                    if (!ok) {                                  // products under way end before tensor memory is given back
-                        tc::umma_commit(&bars.drain);
-                        tc::mbar_wait(&bars.drain, 0);
-                    }
                 }
                 __syncwarp();
                 kv_tiles += tiles;
@@ -914,6 +910,13 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs p) {
             }
         }
     }
+    // Products under way end before tensor memory is given back, whichever role gave up (the rows wait for the last ones otherwise). The
+    // thread elected is the one that issued them: for one mask it is always the same.
+    if (gave_up && warp == kProductWarp && tc::elect_one()) {
+        tc::umma_commit(&bars.drain);
+        tc::mbar_wait(&bars.drain, 0);
+    }
+    __syncwarp();
     before_sync();
     __syncthreads();
     after_sync();

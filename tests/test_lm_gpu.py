@@ -1198,3 +1198,41 @@ def test_queries_of_rows_that_stand_before_the_text(new, kv_len, dtype, rotary):
     assert torch.equal(lm.append(k, v, q=q, rotary=table, **batch).cpu(), want.to(dtype))
     in_place = q.clone()
     assert torch.equal(lm.append(k, v, q=in_place, out=in_place, rotary=table, **batch).cpu(), want.to(dtype))
+
+
+def takes_the_prompt_form(q, batch):
+    """The tensor cores' form asks for two parts of 256 rows for each of 148 blocks, more than the other form ever does."""
+    rows, heads, dim = q.shape
+    b = lm._batch(batch["cache"], batch["block_table"], batch["kv_len"], batch["max_kv_len"], batch["row_start"], batch["max_rows"], rows, heads, q.dtype)
+    p = lm._ATTENTION(q.data_ptr(), q.data_ptr(), 0, q.stride(0), q.stride(1), q.stride(0), q.stride(1), 1.0, 1, 0, 0)
+    return _lib.cuda_lib().ogle_cuda_paged_attention_workspace_bytes(b, p) >= 148 * 2 * 256 * ((64 if dim <= 64 else 128) + 2) * 4
+
+
+@pytest.mark.parametrize("limit", [0, 1, 40])
+@pytest.mark.parametrize("new,past,apart", [([300], [200], 0), ([700, 130], [0, 900], 0), ([150] * 9, [2000] * 9, 0), ([700, 130], [200, 900], 30)])
+def test_prompt_form_reports_a_wait_that_runs_out(new, past, apart, limit):
+    """Whichever role's wait it is: the call ends, stores nothing outside its rows, and the next one is right."""
+    batch, total = ref.make_batch(new, past, 16, 2, 64)
+    if apart:
+        outliers(batch, total, apart)
+    n = sum(new)
+    q, b = rows_of(n, 4, 64, BF16), widened(batch)
+    assert takes_the_prompt_form(q, b)
+    want, lib = lm.attention(q, **b), _lib.cuda_lib()
+    wide, lse = torch.full((n + 2, 4, 64), 5.0, dtype=BF16, device="cuda"), torch.full((n + 2, 4), 5.0, device="cuda")
+    lib.ogle_cuda_set_wait_limit(limit)
+    try:
+        attention_through_c(q, b, wide[1:n + 1], lse[1:n + 1], 0x7f)
+        torch.cuda.synchronize()
+        status, detail = lib.ogle_cuda_device_status(), lib.ogle_cuda_device_status_detail()
+    finally:
+        lib.ogle_cuda_set_wait_limit(-1)
+        lib.ogle_cuda_clear_device_status()
+    if limit == 0 or status:                                     # (a few polls may be enough: each waits a while)
+        assert status == -6 and detail == 9
+    else:
+        assert torch.equal(wide[1:n + 1], want[0]) and torch.equal(lse[1:n + 1], want[1])
+    for t in (wide, lse):
+        assert bool((t[0] == 5).all()) and bool((t[n + 1] == 5).all())
+    again = lm.attention(q, **b)
+    assert torch.equal(again[0], want[0]) and torch.equal(again[1], want[1]) and lib.ogle_cuda_device_status() == 0
