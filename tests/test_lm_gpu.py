@@ -1208,6 +1208,88 @@ def takes_the_prompt_form(q, batch):
     return _lib.cuda_lib().ogle_cuda_paged_attention_workspace_bytes(b, p) >= 148 * 2 * 256 * ((64 if dim <= 64 else 128) + 2) * 4
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_the_limit_between_the_forms(dtype, dim):
+    """The most rows that the form for few rows takes, and one more."""
+    for wide in (False, True):
+        forms, limit = [], 0
+        for rows in (60, 4000):
+            batch, _ = ref.make_batch([rows], [0], 64, 1, dim)
+            forms.append(takes_the_prompt_form(rows_of(rows, 1, dim, dtype), widened(batch) if wide else batch))
+        assert forms == [False, True]
+        low, high = 60, 4000
+        while high - low > 1:
+            rows = (low + high) // 2
+            batch, _ = ref.make_batch([rows], [0], 64, 1, dim)
+            if takes_the_prompt_form(rows_of(rows, 1, dim, dtype), widened(batch) if wide else batch):
+                high = rows
+            else:
+                low = rows
+        for rows in (low, high):
+            batch, total = ref.make_batch([rows], [0], 64, 1, dim)
+            q = rows_of(rows, 1, dim, dtype)
+            b = widened(batch) if wide else batch
+            assert takes_the_prompt_form(q, b) == (rows == high)
+            ref.check_attention(lm.attention(q, **b), ref.attention64(q, batch, total, [rows]), dtype)
+
+
+@pytest.mark.parametrize("scale", [0.2, -0.1, 0.0])
+@pytest.mark.parametrize("causal,window", [(True, 0), (False, 50), (True, 70)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_prompt_form_with_negative_and_vanishing_scales(dtype, causal, window, scale):
+    new, past = [300, 90], [40, 700]
+    batch, total = ref.make_batch(new, past, 16, 2, 80)
+    q, b = rows_of(sum(new), 4, 80, dtype), widened(batch)
+    assert takes_the_prompt_form(q, b)
+    got = lm.attention(q, causal=causal, window=window, scale=scale, **b)
+    ref.check_attention(got, ref.attention64(q, batch, total, new, scale=scale, causal=causal, window=window), dtype)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_prompt_form_with_nan_among_keys_and_values(dtype):
+    new, past = [150, 300], [30, 100]
+    batch, total = ref.make_batch(new, past, 16, 2, 64, seed=3)
+    q, b = rows_of(sum(new), 4, 64, dtype), widened(batch)
+    assert takes_the_prompt_form(q, b)
+    clean = lm.attention(q, window=70, **b)
+
+    def put(cache, b, token, head, element):
+        cache.view(torch.uint8)[int(batch["block_table"][b, token // 16]), head, token % 16, element] = 0x7f
+
+    put(batch["cache"][1], 0, 60, 0, 5)        # rows 30..99 of sequence 0
+    put(batch["cache"][1], 0, 60, 0, 40)
+    put(batch["cache"][0], 0, 120, 1, 0)       # rows 90..
+    put(batch["cache"][1], 1, 399, 1, 63)      # its last row alone
+    out, lse = lm.attention(q, window=70, **b)
+    hit = torch.zeros(out.shape, dtype=torch.bool, device="cuda")
+    hit[30:100, 0:2, 5] = hit[30:100, 0:2, 40] = True
+    hit[90:150, 2:4] = True
+    hit[449, 2:4, 63] = True
+    assert torch.equal(torch.isnan(out), hit)
+    top = float(batch["cache"][1].float().nan_to_num().abs().max() * batch["cache"][3].max())
+    assert bool(((out[~hit] - clean[0][~hit]).abs() <= 2 * ref.LIMIT[dtype] * top + 2 * ref.half_step(clean[0][~hit].float(), dtype)).all())
+    keys_hit = torch.zeros(lse.shape, dtype=torch.bool, device="cuda")
+    keys_hit[90:150, 2:4] = True
+    assert torch.equal(torch.isnan(lse), keys_hit) and torch.allclose(lse[~keys_hit], clean[1][~keys_hit], rtol=2e-5, atol=2e-5)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_prompt_form_over_missing_pages(dtype):
+    """Rows whose every token has lost its page, and rows with some left: as the form for few rows has them."""
+    batch, total = ref.make_batch([200], [0], 16, 1, 64)
+    q = rows_of(200, 2, 64, dtype)
+    batch["block_table"][0, 0] = batch["block_table"][0, 5] = -1
+    b = widened(batch)
+    assert takes_the_prompt_form(q, b) and not takes_the_prompt_form(q, batch)
+    out, lse = lm.attention(q, **b)
+    assert bool((out[:16] == 0).all()) and bool((lse[:16] == -math.inf).all())
+    few = lm.attention(q, **batch)
+    top = float(batch["cache"][1].float().nan_to_num().abs().max() * batch["cache"][3].max())
+    assert bool(((out.float() - few[0].float()).abs() <= 2 * ref.LIMIT[dtype] * top + 2 * ref.half_step(few[0].float(), dtype)).all())
+    assert torch.allclose(lse[16:], few[1][16:], rtol=2e-5, atol=2e-5)
+
+
 @pytest.mark.parametrize("limit", [0, 1, 40])
 @pytest.mark.parametrize("new,past,apart", [([300], [200], 0), ([700, 130], [0, 900], 0), ([150] * 9, [2000] * 9, 0), ([700, 130], [200, 900], 30)])
 def test_prompt_form_reports_a_wait_that_runs_out(new, past, apart, limit):
