@@ -472,8 +472,11 @@ int ogle_cuda_kv_append(const OglePagedBatch* batch, const OgleAppendParams* p, 
 /* out[row][h] = sum_j softmax_j(scale q.k_j) v_j over the tokens j < kv_len of the row's sequence - with `causal` those up to the
  * row's own position, with window > 0 those after position - window. lse (may be NULL), [n_rows][q_heads]: the natural logarithm
  * of the sum of exponentials. A row without a token has out 0 and lse minus infinity. A token that a row does not attend does
- * not reach it, whatever its bytes are. Scores, statistics and sums are in fp32; for fp32 activations the queries and weights enter
- * the products as two 16-bit parts.
+ * not reach it, whatever its bytes are and however large its page's scales. Scores, statistics and sums are in fp32. Queries and
+ * weights enter the products in fewer bits: as two 16-bit parts, 22 bits, for fp32 activations, and for 16-bit ones where no sequence can
+ * have more than 8 rows x query heads of a kv head (max_rows); else as one, 11 bits, which a query of such a type has anyway. Of a
+ * weight times its value's scale, what lies below 2^-24 of the row's largest such product may be lost; a weight below 2^-126 of the
+ * row's largest is 0.
  * The caller lends `workspace` (>= ogle_cuda_paged_attention_workspace_bytes, 16-byte aligned); nothing in it has to be
  * cleared, and it may be reused once the stream has passed the call. Where no more than OGLE_ATTENTION_NO_WORKSPACE bytes are asked
  * for, nothing is read or written there. Strides in elements, multiples of 16 bytes. */

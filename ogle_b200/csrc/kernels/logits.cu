@@ -237,7 +237,9 @@ cudaError_t launch(LogitsArgs a, cudaStream_t s) {
     constexpr int N = Vec<Ti>::kN, kPiece = kThreads * N;
     // A block's range: whole pieces of a vector a thread. As many blocks to a row as one round of them (four to an SM) has
     // for it; at least one for every 2000 tokens of a row's text, so that those of a range fit the hash table. (400 x 150000, a row a
-    // block: 16 pieces a block 71 us, so 56.)
+    // block: 16 pieces a block 71 us, so 56. One for every 500 / 1000 / 2000 / 4000 / without, us: 400 x 150000, texts of up to 8000,
+    // 194 / 226 / 283 / 397 / 610; 150 x 50000, 16000, 165 / 122 / 162 / 204 / 230; 64 x 128001, 40000, 346 / 357 / 326 / 417 / 417;
+    // 592 x 32000, 2500, 54 / 50 / 48 / 48 / 48; 400 x 150000, 2000, 64 / 74 / 71 / 71 / 71.)
     const long pieces = div_up(a.p.vocab + N - 1, kPiece), text = div_up(long(a.p.n_tokens) + a.p.n_biases, a.p.rows);
     long blocks = 4L * kNumSMs / a.p.rows;
     if (blocks < div_up(text, 2000)) blocks = div_up(text, 2000);

@@ -11,8 +11,8 @@
 // Where there are few segments, none of them long, the blocks of a cluster have one segment instead and add their parts
 // through each other's shared memory: one launch, no workspace.
 //
-// Measured: 64 sequences of up to 8000 tokens, 32 query heads to 8 of 128, 570 MB: 111 to 119 us, 74 to 79 % of what a copy reaches. 3 sequences
-// of up to 200000 tokens, 16 query heads to one: 52 us, 3.9 TB/s with the join - 500 instructions a step of 16 keys, each warp
+// Measured: 64 sequences of up to 8000 tokens, 32 query heads to 8 of 128, 570 MB: 112 to 118 us, 74 to 78 % of what a copy reaches. 3 sequences
+// of up to 200000 tokens, 16 query heads to one: 51 us, 3.9 TB/s with the join - 500 instructions a step of 16 keys, each warp
 // waiting 2 of 8 cycles for the one before (four blocks an SM, the queries in shared memory; three, in registers: 56). What is short is bound
 // by latency: one sequence of 700 tokens takes 9 us on the device.
 //
@@ -363,7 +363,7 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
         // so that the row's largest w x scale, not its largest w, lies near 2^kLift: what a page's scale is to other rows, or to a key that
         // hardly counts, takes no bits from this row's weights
         float rs[MT][NR], noff[MT][NR], up[MT][NR], l[MT][NR];
-        // (one copy of the code: it runs once a segment, and fetching a second took longer than running it - drafts of 5 rows 62 us, so 58)
+        // (one copy of the code: it runs once a segment, and fetching a second took longer than running it - drafts of 5 rows 62 us, so 60)
 #pragma unroll 1
         for (int i = 0; i < MT * NR; ++i) {
             const int mt = i / NR, r = i % NR;
@@ -933,7 +933,9 @@ int most_clusters(int size) {
 // 19.8; 4 of 2000 14.7 / 11.7, of 8000 23.1 / 22.7, of 16000 33.4 / 38.9; 16 of up to 4000 35.7 / 23.9, of up to 8000 35.4 / 38.2.
 // So the tiles of 64 keys that pay a block go from 6, where few blocks of the GPU are used, to about 30, where all are.
 // A cluster has to fit into a part of the GPU with all its blocks, so the sizes are those of which the runtime says that all run at once:
-// 96 clusters of 3 with 256 elements, two blocks an SM, do not (288 of 296 slots: 24 drafts over 4096 tokens 85 us, 70 in ranges).
+// of 96 clusters of 3 with 256 elements, two blocks an SM, 93 do (288 of 296 slots): 24 drafts of 5 over 4096 tokens each 83 us, 58 in ranges,
+// and over 1000 40, 29 in clusters of 2. Where lengths differ the last three come as the shortest end - up to 20000 tokens in a window of
+// 4096 59 us, 61 in ranges; one row each over up to 2000 26, 29 in clusters of 2 -, but lengths are the device's.
 template <int DP, int MT, bool kSplit>
 int cluster_of(const OglePagedBatch* b, const OgleAttentionParams* p) {
     using F = Form<DP, MT, kSplit>;
@@ -962,6 +964,9 @@ int ranges_of(const OglePagedBatch* b, int rows, int blocks) {
 // with. us here / there, 32 query heads to 8 of 128 elements: 64 and 80 rows of 8 sequences over 20000 tokens 174 / 187 and 249 / 188,
 // over 3000 46 / 56 and 58 / 57; 128 rows of 32 sequences over 300 70 / 63; of one sequence, 128 rows over 20000 58 / 56, 256 over 3000
 // 32 / 42, over 300 21 / 31. So 64 rows, and more where the call has few keys to go through.
+// fp32 and heads above 128 stay here whatever their rows are, far from what the tensor cores could do: six prompts of about 2000 rows over about
+// 2500 tokens, 32 query heads to 8, take 1896 us in fp32 (94 TFLOP/s; heads of 64 1103), 2336 in bf16 with heads of 256. The prompt form holds one
+// fp16 part of queries and weights, and sums of two tiles of 256 columns would fill the tensor memory that the scores need.
 int few_limit(const OglePagedBatch* b) {
     if (b->dtype == OGLE_F32 || b->head_dim > 128) return 0;
     const long long rows = (long long)(b->max_rows < b->n_rows ? b->max_rows : b->n_rows) * (b->q_heads / b->kv_heads);
@@ -1097,6 +1102,8 @@ int ogle_cuda_paged_attention(const OglePagedBatch* batch, const OgleAttentionPa
         // a warp to a row, or sixteen where few segments are cut into many parts
         const long long rows = (long long)(a.b.max_rows < a.b.n_rows ? a.b.max_rows : a.b.n_rows) * a.b.group;
         const int tile = int(rows < F::kRows ? (rows < 1 ? 1 : rows) : F::kRows);
+        // us by warps / by sixteen a row: one segment of 100000 keys 273 / 28, 32 of 60000 78 / 66, 72 of 60000 107 / 100, 96 of
+        // 40000 99 / 94, 144 of 30000 105 / 104, 288 of 16000 99 / 102; of 16 rows each, 40 of 60000 81 / 72, 80 of 30000 73 / 73
         const bool many = ranges > 8 * segments;
         return launch_join(a, DP, many, a.by_segment ? int(segments < 1 ? 1 : segments) : ranges, ranges, F::kRows, tile, stream);
     });

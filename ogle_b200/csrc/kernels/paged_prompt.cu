@@ -5,7 +5,8 @@
 //   four warps    read a tile of keys and of values ahead into registers and turn them into fp16 operands: e4m3 is exact in fp16, and
 //                 a page's scale relative to the largest of the item is a power of two that is multiplied in on the way (exact
 //                 down to 2^-15 of the largest), so that scores and weights know nothing of pages. Where an item's pages lie
-//                 further apart, bytes alone are converted and the rows multiply by their pages' scales (see `apart`)
+//                 further apart, bytes alone are converted and the rows multiply by their pages' scales (see `apart`; the
+//                 prompts below take 715 us then)
 //   one thread    issues the products: S = Q K^T per tile, O += P V per tile, P taken from tensor memory
 //   2 x 4 warps   a row a thread: maximum, weights 2^(x - off), their sum; P in fp16 over S; O rescaled when a row's maximum
 //                 has grown by more than 2^8
@@ -13,9 +14,9 @@
 // first sums run while the second half is being weighted. P lies over S in tensor memory (2 x 128 columns for S, 2 x DP for O), so
 // the next S of a tile of rows is asked for once its P V is through.
 // Shared memory has the products' operands to deliver beside the conversion's traffic; two S of 64 keys a tile of rows, which
-// overlap more, read the queries twice as often and were slower (3.2 us a tile of keys, so 2.1: 1150 TFLOP/s where texts are long). The
-// tensor cores and the exponentials each need half of that; taking a quarter of the exponentials off the special function units, by a
-// polynomial, made it slower. Six prompts of 2000 rows over 2500 earlier tokens: 331 us, 538 TFLOP/s - an item's beginning and end
+// overlap more, read the queries twice as often and were slower (3.2 us a tile of keys, so 2.1). The tensor pipe and the special
+// function units are each busy for half of the time where texts are long (2048 rows over 30000 tokens: 1011 us, 1029 TFLOP/s, 51 % both
+// by the counters); taking a quarter of the exponentials off the latter, by a polynomial, made it slower. Six prompts of 2000 rows over 2500 earlier tokens: 326 us, 546 TFLOP/s - an item's beginning and end
 // (queries, the first scores, the last sums, results: 10 us) take as long as its tiles there.
 //
 // Work: items (sequence, tile of 256 rows, kv head) laid end to end by their tiles of keys, cut into one range a block; parts

@@ -3,12 +3,15 @@ in 8 bits, attention over that cache, and the adjustment of logits before a toke
 on torch CUDA tensors; torch is used for device memory and the current stream only.
 
 The cache is four tensors (k, v, k_scale, v_scale): k and v float8_e4m3fn [pages, kv heads, page tokens, head dim] (any strides
-that keep a token's elements side by side and 16-byte boundaries), one float32 scale for each page and kv head. `new_cache` makes
-one; a page may be anywhere in it. Sequence b's token j lies in page block_table[b, j // page tokens].
+that keep a token's elements side by side and 16-byte boundaries), one float32 scale for each page and kv head, a power of two, or 0
+where append has met nothing but zeros in the page. `new_cache` makes one; a page may be anywhere in it. Sequence b's token j lies in
+page block_table[b, j // page tokens].
 
 Rows are the new tokens of all sequences, one sequence behind the other: sequence b has rows row_start[b]..row_start[b + 1], the
 last of the kv_len[b] tokens that it has once they are appended. Without row_start every sequence has one row. max_kv_len and
-max_rows are the host's bounds of what kv_len and row_start hold on the device: nothing here waits for the device.
+max_rows are the host's bounds of what kv_len and row_start hold on the device: nothing here waits for the device. Rows of a sequence
+behind its first max_rows, rows that no sequence has (a padded batch), and tokens from max_kv_len on are ignored: a result made here
+holds what was in memory there.
 """
 import torch
 
@@ -86,7 +89,7 @@ def append(k, v, cache, block_table, kv_len, max_kv_len, row_start=None, max_row
     """Stores the rows' keys and values k, v [rows, kv heads, head dim] in the cache, quantised to e4m3 with a power-of-two
     scale for each page and head (ogle_cuda_kv_append). rotary [positions, rotary dim] (see rotary_table; None: no rotation)
     rotates k and q by the rows' positions on the way, in pairs half the rotary dim apart or, interleaved, of neighbours.
-    Returns the rotated q (into `out`, which may be q itself), or None without q."""
+    Returns the rotated q (into `out`, which may be q itself; 0 for rows that stand before the text), or None without q."""
     rows, dtype = k.shape[0], k.dtype
     heads, dim = cache[0].shape[1], cache[0].shape[3]
     q_heads = heads if q is None else q.shape[1]
