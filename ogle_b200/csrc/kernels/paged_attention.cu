@@ -358,10 +358,10 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
         // queries, once for all warps: in shared memory as the products take them (registers for them would leave room for a block less)
         uint4* const queries = reinterpret_cast<uint4*>(smem + F::kQueries) + lane;
         const float kDown = -3e38f;               // m of a row that has not met a key
-        // weight w = 2^(s rs + noff) of product s; noff = kLift - m. (The product is rounded before the sum: so is m, and the largest x of a row comes
-        // near kLift however large it is, where a fused sum would be off by what m was rounded by.) Sums of weights are of w; the values' sums O are of w 2^(log2 scale + up),
-        // so that the row's largest w x scale, not its largest w, lies near 2^kLift: what a page's scale is to other rows, or to a key that
-        // hardly counts, takes no bits from this row's weights
+        // weight w = 2^(s rs + noff) of product s; noff = kLift - m. (The product is rounded before the sum: so is m, and the largest x of a
+        // row comes near kLift however large it is, where a fused sum would be off by what m was rounded by.) Sums of weights are of w; the
+        // values' sums O are of w 2^(log2 scale + up), so that the row's largest w x scale, not its largest w, lies near 2^kLift: what a page's
+        // scale is to other rows, or to a key that hardly counts, takes no bits from this row's weights
         float rs[MT][NR], noff[MT][NR], up[MT][NR], l[MT][NR];
         // (one copy of the code: it runs once a segment, and fetching a second took longer than running it - drafts of 5 rows 62 us, so 60)
 #pragma unroll 1
