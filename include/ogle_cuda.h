@@ -521,6 +521,97 @@ typedef struct {
 } OgleLogitsParams;
 int ogle_cuda_adjust_logits(const OgleLogitsParams* p, ogle_stream_t stream);
 
+/* ------------------------------------------- searching over the paged cache */
+/* The best continuations of a group of texts (the beams of a search) over all its beams and tokens. Row g * beams + b is beam b of group
+ * g; its token t has the total
+ *   scores[row] + x_t - log sum_u exp(x_u),    x = logits[row]
+ * in 64 bits, where a NaN logit counts as minus infinity and plus infinity as the largest number of the logits' type. A logit of minus
+ * infinity is no continuation; a beam whose score is not finite has none. scores NULL: 0 for all.
+ * Of each group the `count` largest totals, in falling order, equal ones by beam and then by token, go to out_score (rounded to fp32),
+ * out_beam and out_token [n_groups][count]; behind the last there are minus infinity, -1, -1. Of these the first `beams` whose token is
+ * none of ends[0 .. n_ends) go on: next_row (the parent's row, g * beams + out_beam), next_token and next_score [n_groups][beams], filled
+ * up with -1, -1, minus infinity. (With end tokens a count of 2 * beams is enough for all to go on.)
+ * Exponentials are of fp32, but those of the largest logits, and sums of 64 bits: the logarithm of a row's sum is within 2^-22 of its
+ * value, most often within 2^-26. `workspace`: as above; what is in it need not outlive the call. */
+typedef struct {
+    int n_groups, beams, vocab, count;     /* count at most 128 */
+    int dtype;                             /* OgleDataType of the logits */
+    int n_ends;                            /* at most 1024 */
+    long long logits_stride;
+    const void* logits;
+    const float* scores;
+    const int* ends;
+    float* out_score;
+    int *out_beam, *out_token;
+    int *next_row, *next_token;
+    float* next_score;
+} OgleBeamParams;
+size_t ogle_cuda_beam_step_workspace_bytes(const OgleBeamParams* p);
+int ogle_cuda_beam_step(const OgleBeamParams* p, void* workspace, size_t workspace_bytes, ogle_stream_t stream);
+
+/* The block tables of the texts that go on, from those of the texts there were. New text i goes on from sequence parent[i] (-1, or any
+ * number that is no sequence: from nothing) and is about to have tokens[i] more (tokens NULL: new_tokens each). Of its parent's
+ * kv_len tokens
+ *   full pages are shared;
+ *   a last page that is not full stays with the first text that goes on from that parent, if refs says that nobody else has it; any other
+ *   gets a page of its own, and copies[i] = (old page, new page, tokens in it) says what ogle_cuda_copy_pages has to bring there,
+ * and pages are added until all its tokens have one. Entry i of copies is (-1, -1, 0) where there is nothing to copy. new_len[i] is the
+ * length with the new tokens; entries of the new table behind the last page are -1. A block without a page (-1) in the parent's row
+ * stays one; blocks from new_blocks on have no place in the table.
+ * refs[page] counts the table entries that name a page, other tables' too; 0: free. new_refs has the counts after the old table's rows are
+ * gone and the new ones are there, so that texts that end (no new one goes on from them) or were cut (kv_len is less than what the row has
+ * pages for) give theirs back. Requests are served in the order of texts and blocks, the k-th with the k-th lowest page that is free in
+ * refs; what a call frees the next can have. Where they run out the entry is -1.
+ * state[0]: pages free in new_refs; state[1]: requests that found none. With any, the old table and refs are still good: the call can
+ * be made again with fewer texts. New arrays must not overlap the old ones. Lengths below 0 count as 0. */
+typedef struct {
+    int n_old, n_new;
+    int old_blocks, new_blocks;            /* columns */
+    int page_tokens, n_pages;
+    int new_tokens, reserved;
+    long long old_stride, new_stride;
+    const int *table, *kv_len;             /* [n_old][old_blocks], [n_old] */
+    const int *parent, *tokens;            /* [n_new] */
+    const int* refs;                       /* [n_pages] */
+    int *new_table, *new_len, *new_refs;
+    int* copies;                           /* [n_new][3] */
+    int* state;                            /* [2] */
+} OgleAdvanceParams;
+size_t ogle_cuda_advance_pages_workspace_bytes(const OgleAdvanceParams* p);
+int ogle_cuda_advance_pages(const OgleAdvanceParams* p, void* workspace, size_t workspace_bytes, ogle_stream_t stream);
+
+/* Used pages to the front of the pool. With U pages in use (refs not 0), the k-th used page from U on moves to the k-th free one below
+ * U, for the first n_copies of them: copies[k] = (page, new page, page_tokens), the rest (-1, -1, 0). The new table names the new pages
+ * (new_table may be table), new_refs has their counts (it may not be refs). state[0]: U; state[1]: moves that are left. What is in the pages is
+ * ogle_cuda_copy_pages' to move. */
+typedef struct {
+    int n_seqs, blocks;
+    int page_tokens, n_pages, n_copies, reserved;
+    long long table_stride, new_stride;
+    const int *table, *refs;
+    int *new_table, *new_refs, *copies, *state;
+} OgleCompactParams;
+size_t ogle_cuda_compact_pages_workspace_bytes(const OgleCompactParams* p);
+int ogle_cuda_compact_pages(const OgleCompactParams* p, void* workspace, size_t workspace_bytes, ogle_stream_t stream);
+
+/* For each (source page, destination page, tokens) of copies, in every layer's cache: the first `tokens` tokens of all heads, keys and
+ * values, and the page's scales - and bounds, where the layer has them. The other slots of the destination stay as they are. An entry that names a
+ * page outside the cache is left out. No page may be the destination of two entries, or of one and the source of another.
+ * Layers have their pages in the same strides (see OglePagedBatch). */
+typedef struct {
+    void *k, *v;
+    float *k_scale, *v_scale;              /* [n_pages][kv_heads] */
+    signed char* bounds;                   /* [n_pages][kv_heads][2][head_dim], or NULL */
+    float* bounds_scale;                   /* [n_pages][kv_heads] */
+} OglePageTensors;
+typedef struct {
+    int n_copies, n_layers;
+    int kv_heads, head_dim, page_tokens, n_pages;
+    long long page_stride, head_stride, token_stride;
+    const int* copies;
+} OgleCopyPagesParams;
+int ogle_cuda_copy_pages(const OgleCopyPagesParams* p, const OglePageTensors* layers_host_array, ogle_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

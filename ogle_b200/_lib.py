@@ -102,6 +102,46 @@ class LogitsParams(C.Structure):
     ]
 
 
+class BeamParams(C.Structure):
+    _fields_ = [
+        ("n_groups", C.c_int), ("beams", C.c_int), ("vocab", C.c_int), ("count", C.c_int), ("dtype", C.c_int), ("n_ends", C.c_int),
+        ("logits_stride", C.c_longlong), ("logits", C.c_void_p), ("scores", C.c_void_p), ("ends", C.c_void_p),
+        ("out_score", C.c_void_p), ("out_beam", C.c_void_p), ("out_token", C.c_void_p),
+        ("next_row", C.c_void_p), ("next_token", C.c_void_p), ("next_score", C.c_void_p),
+    ]
+
+
+class AdvanceParams(C.Structure):
+    _fields_ = [
+        ("n_old", C.c_int), ("n_new", C.c_int), ("old_blocks", C.c_int), ("new_blocks", C.c_int),
+        ("page_tokens", C.c_int), ("n_pages", C.c_int), ("new_tokens", C.c_int), ("reserved", C.c_int),
+        ("old_stride", C.c_longlong), ("new_stride", C.c_longlong),
+        ("table", C.c_void_p), ("kv_len", C.c_void_p), ("parent", C.c_void_p), ("tokens", C.c_void_p), ("refs", C.c_void_p),
+        ("new_table", C.c_void_p), ("new_len", C.c_void_p), ("new_refs", C.c_void_p), ("copies", C.c_void_p), ("state", C.c_void_p),
+    ]
+
+
+class CompactParams(C.Structure):
+    _fields_ = [
+        ("n_seqs", C.c_int), ("blocks", C.c_int), ("page_tokens", C.c_int), ("n_pages", C.c_int), ("n_copies", C.c_int), ("reserved", C.c_int),
+        ("table_stride", C.c_longlong), ("new_stride", C.c_longlong),
+        ("table", C.c_void_p), ("refs", C.c_void_p), ("new_table", C.c_void_p), ("new_refs", C.c_void_p),
+        ("copies", C.c_void_p), ("state", C.c_void_p),
+    ]
+
+
+class PageTensors(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("bounds", C.c_void_p), ("bounds_scale", C.c_void_p)]
+
+
+class CopyPagesParams(C.Structure):
+    _fields_ = [
+        ("n_copies", C.c_int), ("n_layers", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int), ("page_tokens", C.c_int), ("n_pages", C.c_int),
+        ("page_stride", C.c_longlong), ("head_stride", C.c_longlong), ("token_stride", C.c_longlong), ("copies", C.c_void_p),
+    ]
+
+
 def packer(structure):
     """struct.Struct that writes all fields of a ctypes structure of ints, floats and addresses: a quarter of the time that filling in the
     structure takes (22 fields: 0.3 us against 1.3). An address that is missing is 0."""
@@ -167,6 +207,13 @@ CUDA_SYMBOLS = {
     "ogle_cuda_paged_attention_workspace_bytes": (C.c_size_t, [_vp, _vp]),
     "ogle_cuda_paged_attention": (C.c_int, [_vp, _vp, _vp, C.c_size_t, _vp]),
     "ogle_cuda_adjust_logits": (C.c_int, [_vp, _vp]),
+    "ogle_cuda_beam_step_workspace_bytes": (C.c_size_t, [_vp]),
+    "ogle_cuda_beam_step": (C.c_int, [_vp, _vp, C.c_size_t, _vp]),
+    "ogle_cuda_advance_pages_workspace_bytes": (C.c_size_t, [_vp]),
+    "ogle_cuda_advance_pages": (C.c_int, [_vp, _vp, C.c_size_t, _vp]),
+    "ogle_cuda_compact_pages_workspace_bytes": (C.c_size_t, [_vp]),
+    "ogle_cuda_compact_pages": (C.c_int, [_vp, _vp, C.c_size_t, _vp]),
+    "ogle_cuda_copy_pages": (C.c_int, [_vp, _vp, _vp]),
     "ogle_cuda_ssd_decode_detect": (C.c_int, [C.POINTER(DetectParams), _vp, _vp, _vp, C.POINTER(C.c_float)] + [_vp] * 6),
 }
 

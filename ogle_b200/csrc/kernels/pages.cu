@@ -1,0 +1,621 @@
+// The pages of the paged cache between two steps: who has which, copies of those that two texts would write to, compaction.
+//
+// References are counted: refs[page] is how often tables name the page, 0 where it is free. Every result is determined by its inputs -
+// the k-th page asked for is the k-th lowest free one - so nothing depends on which block comes first, and atomics add whole numbers.
+//
+// What there is to read and write is small (64 x 8 sequences of 40 blocks and 8000 pages: 230 KB), so the launches are what it costs:
+// one that looks at all pages and all sequences side by side, and one that writes. A bit for each free page and a count for each
+// 1024 of them lead from a request's number to its page in one binary search and one warp's look at 32 words.
+#include "common.cuh"
+
+namespace ogle {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kChunkPages = kThreads * 4;        // pages that a block looks at at a time
+constexpr int kMostChunks = 1024;
+constexpr int kMostPages = 1 << 26;
+
+// Pages in chunks: one count for each, one bit for each page.
+struct Pool {
+    int n_pages, chunk, chunks;                  // pages of a chunk: a multiple of kChunkPages
+    unsigned* bits;
+    int* counts;
+};
+
+struct AdvanceArgs {
+    OgleAdvanceParams p;
+    Pool pool;                                   // of the free pages
+    int *children, *first_child;                 // of each old sequence: texts that go on from it; the first of them
+    int* base;                                   // of each new one: requests of those before it; then all of them
+    int page_shift;
+};
+
+__device__ __forceinline__ bool is_page(int page, int n_pages) { return (unsigned)page < (unsigned)n_pages; }
+
+// A block's part of the pool: bits and count of the pages for which `wanted` holds, the counts copied on the way.
+template <typename F>
+__device__ __forceinline__ void scan_chunk(const Pool& pool, int chunk, const int* refs, int* out, F wanted) {
+    __shared__ int sums[kThreads / 32];
+    const int tid = threadIdx.x, first = chunk * pool.chunk, end = min(first + pool.chunk, pool.n_pages);
+    int mine = 0;
+    for (int p0 = first; p0 < end; p0 += kChunkPages) {
+        int r[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int p = p0 + u * kThreads + tid;
+            r[u] = p < end ? __ldg(refs + p) : 1;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int p = p0 + u * kThreads + tid;
+            const unsigned b = __ballot_sync(~0u, p < end && wanted(r[u]));
+            if (p < end) out[p] = r[u];
+            if ((tid & 31) == 0 && p < end) {
+                pool.bits[p / 32] = b;
+                mine += __popc(b);
+            }
+        }
+    }
+    if ((tid & 31) == 0) sums[tid / 32] = mine;
+    __syncthreads();
+    if (tid == 0) {
+        int all = 0;
+#pragma unroll
+        for (int w = 0; w < kThreads / 32; ++w) all += sums[w];
+        pool.counts[chunk] = all;
+    }
+}
+
+// Exclusive sums of the chunks' counts, in shared memory, and their total. A whole block of 32 * kWarps threads.
+template <int kWarps>
+__device__ __forceinline__ int sum_chunks(const Pool& pool, int* before) {
+    __shared__ int sums[kWarps];
+    const int tid = threadIdx.x, lane = tid & 31, per = (pool.chunks + kWarps * 32 - 1) / (kWarps * 32);
+    int mine = 0;
+    for (int i = 0; i < per; ++i) {
+        const int c = tid * per + i;
+        if (c < pool.chunks) mine += pool.counts[c];
+    }
+    int sum = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const int o = __shfl_up_sync(~0u, sum, d);
+        if (lane >= d) sum += o;
+    }
+    if (lane == 31) sums[tid / 32] = sum;
+    __syncthreads();
+    int total = 0, at = sum - mine;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < tid / 32) at += sums[w];
+        total += sums[w];
+    }
+    for (int i = 0; i < per; ++i) {
+        const int c = tid * per + i;
+        if (c < pool.chunks) {
+            before[c] = at;
+            at += pool.counts[c];
+        }
+    }
+    __syncthreads();
+    return total;
+}
+
+// The k-th page whose bit is set, of more than k: a warp's work.
+__device__ __forceinline__ int kth_page(const Pool& pool, const int* before, int k) {
+    int lo = 0, hi = pool.chunks;                // the last chunk that begins at or before k
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (before[mid] <= k) lo = mid;
+        else hi = mid;
+    }
+    const int lane = threadIdx.x & 31, words = (pool.n_pages + 31) / 32;
+    int left = k - before[lo];
+    for (int w0 = lo * (pool.chunk / 32); w0 < words; w0 += 32) {
+        const unsigned b = w0 + lane < words ? pool.bits[w0 + lane] : 0u;
+        int sum = __popc(b);
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const int o = __shfl_up_sync(~0u, sum, d);
+            if (lane >= d) sum += o;
+        }
+        const int n = __popc(b);
+        const unsigned here = __ballot_sync(~0u, left < sum);
+        if (here) {
+            const int l = __ffs(here) - 1;
+            int page = -1;
+            if (lane == l) page = (w0 + lane) * 32 + __fns(b, 0, left - (sum - n) + 1);
+            return __shfl_sync(~0u, page, l);
+        }
+        left -= __shfl_sync(~0u, sum, 31);
+    }
+    return -1;
+}
+
+// What becomes of a new text's blocks.
+struct Text {
+    int parent, length, full;                    // blocks [0, full) are shared with the parent
+    int half;                                    // the parent's page of the block that is half full, -1: none
+    bool half_full, keeps;                       // there is such a block; its page goes on with this text
+    int first_wanted, end;                       // blocks that ask for a page
+};
+
+__device__ __forceinline__ Text text_of(const AdvanceArgs& a, int i) {
+    const OgleAdvanceParams& p = a.p;
+    Text t;
+    t.parent = __ldg(p.parent + i);
+    if ((unsigned)t.parent >= (unsigned)p.n_old) t.parent = -1;
+    t.length = t.parent >= 0 ? max(__ldg(p.kv_len + t.parent), 0) : 0;
+    const int more = max(p.tokens ? __ldg(p.tokens + i) : p.new_tokens, 0), part = t.length & ((1 << a.page_shift) - 1);
+    t.full = t.length >> a.page_shift;
+    t.half_full = part > 0;
+    t.half = -1;
+    t.keeps = false;
+    if (t.half_full && t.full < p.old_blocks && t.full < p.new_blocks) {
+        const int page = __ldg(p.table + t.parent * p.old_stride + t.full);
+        if (is_page(page, p.n_pages)) {
+            t.half = page;
+            t.keeps = __ldg(p.refs + page) == 1 && __ldcg(a.first_child + t.parent) == i;
+        }
+    }
+    t.first_wanted = t.full + (t.half_full && (t.half < 0 || t.keeps));
+    const long long blocks = ((long long)t.length + more + (1 << a.page_shift) - 1) >> a.page_shift;
+    t.end = int(min(blocks, (long long)p.new_blocks));
+    t.first_wanted = min(t.first_wanted, t.end);
+    return t;
+}
+
+// Blocks [0, chunks): the pool. The last block: the sequences.
+__global__ void __launch_bounds__(kThreads) advance_plan_kernel(AdvanceArgs a) {
+    const OgleAdvanceParams& p = a.p;
+    const int tid = threadIdx.x, lane = tid & 31;
+    grid_dependency_trigger();
+    grid_dependency_wait();
+    if (int(blockIdx.x) < a.pool.chunks) {
+        scan_chunk(a.pool, blockIdx.x, p.refs, p.new_refs, [](int r) { return r == 0; });
+        return;
+    }
+    if (tid < 2) p.state[tid] = 0;
+    for (int i = tid; i < p.n_old; i += kThreads) {
+        a.children[i] = 0;
+        a.first_child[i] = 0x7fffffff;
+    }
+    __syncthreads();
+    for (int i = tid; i < p.n_new; i += kThreads) {
+        const int parent = __ldg(p.parent + i);
+        if ((unsigned)parent < (unsigned)p.n_old) {
+            atomicAdd(a.children + parent, 1);
+            atomicMin(a.first_child + parent, i);
+        }
+    }
+    __syncthreads();
+    __shared__ int sums[kThreads / 32];
+    int before = 0;
+    for (int i0 = 0; i0 < p.n_new; i0 += kThreads) {
+        const int i = i0 + tid;
+        int wanted = 0;
+        if (i < p.n_new) {
+            const Text t = text_of(a, i);
+            wanted = t.end - t.first_wanted;
+        }
+        int sum = wanted;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const int o = __shfl_up_sync(~0u, sum, d);
+            if (lane >= d) sum += o;
+        }
+        if (lane == 31) sums[tid / 32] = sum;
+        __syncthreads();
+        int all = 0;
+#pragma unroll
+        for (int w = 0; w < kThreads / 32; ++w) {
+            if (w < tid / 32) sum += sums[w];
+            all += sums[w];
+        }
+        if (i < p.n_new) a.base[i] = before + sum - wanted;
+        before += all;
+        __syncthreads();
+    }
+    if (tid == 0) a.base[p.n_new] = before;
+}
+
+// Block i: the table's row of new text i, and what the old sequence i gives back.
+constexpr int kRowWarps = 4;
+__global__ void __launch_bounds__(kRowWarps * 32) advance_rows_kernel(AdvanceArgs a) {
+    __shared__ int before[kMostChunks];
+    __shared__ int freed;
+    const OgleAdvanceParams& p = a.p;
+    const int tid = threadIdx.x, i = blockIdx.x;
+    if (tid == 0) freed = 0;
+    grid_dependency_trigger();
+    grid_dependency_wait();
+    if (i < p.n_new) {
+        const Text t = text_of(a, i);
+        const int base = __ldcg(a.base + i), wanted = t.end - t.first_wanted;
+        int free_pages = 0;
+        if (wanted > 0 || i == 0) free_pages = sum_chunks<kRowWarps>(a.pool, before);
+        int* row = p.new_table + i * p.new_stride;
+        for (int c = tid; c < p.new_blocks; c += kRowWarps * 32) {
+            int page = -1;
+            if (t.parent >= 0 && c < p.old_blocks && (c < t.full || c == t.full && t.keeps)) page = __ldg(p.table + t.parent * p.old_stride + c);
+            if (c < t.first_wanted || c >= t.end) row[c] = page;
+        }
+        for (int k = tid / 32; k < wanted; k += kRowWarps) {
+            const int page = base + k < free_pages ? kth_page(a.pool, before, base + k) : -1;
+            if ((tid & 31) == 0) {
+                row[t.first_wanted + k] = page;
+                if (page >= 0) atomicAdd(p.new_refs + page, 1);
+            }
+            if (k == 0 && (tid & 31) == 0) {
+                const bool copied = t.half >= 0 && !t.keeps && page >= 0;
+                p.copies[3 * i] = copied ? t.half : -1;
+                p.copies[3 * i + 1] = copied ? page : -1;
+                p.copies[3 * i + 2] = copied ? t.length & ((1 << a.page_shift) - 1) : 0;
+            }
+        }
+        if (tid == 0) {
+            if (wanted <= 0) { p.copies[3 * i] = p.copies[3 * i + 1] = -1; p.copies[3 * i + 2] = 0; }
+            p.new_len[i] = t.length + max(p.tokens ? __ldg(p.tokens + i) : p.new_tokens, 0);
+            if (i == 0) {
+                const int all = __ldcg(a.base + p.n_new), granted = min(all, free_pages);
+                atomicAdd(p.state, free_pages - granted);
+                atomicAdd(p.state + 1, all - granted);
+            }
+        }
+    }
+    if (i < p.n_old) {
+        const int children = __ldcg(a.children + i), length = max(__ldg(p.kv_len + i), 0), full = length >> a.page_shift;
+        const bool half_full = (length & ((1 << a.page_shift) - 1)) > 0;
+        int mine = 0;
+        for (int c = tid; c < p.old_blocks; c += kRowWarps * 32) {
+            const int page = __ldg(p.table + i * p.old_stride + c);
+            if (!is_page(page, p.n_pages)) continue;
+            int n = 0;                           // of the new texts that name it here
+            if (c < p.new_blocks) {
+                if (c < full) n = children;
+                else if (c == full && half_full) n = children > 0 && __ldg(p.refs + page) == 1;
+            }
+            if (n != 1) mine += atomicAdd(p.new_refs + page, n - 1) + n - 1 == 0;
+        }
+        __syncthreads();
+        if (mine) atomicAdd(&freed, mine);
+        __syncthreads();
+        if (tid == 0 && freed) atomicAdd(p.state, freed);
+    }
+    if (i == 0 && p.n_new == 0 && tid < 32) {    // nobody above has counted the free pages
+        int n = 0;
+        for (int c = tid; c < a.pool.chunks; c += 32) n += a.pool.counts[c];
+#pragma unroll
+        for (int d = 16; d; d /= 2) n += __shfl_xor_sync(~0u, n, d);
+        if (tid == 0) atomicAdd(p.state, n);
+    }
+}
+
+// ---- compaction
+struct CompactArgs {
+    OgleCompactParams p;
+    Pool pool;                                   // of the used pages
+    int* rank;                                   // of a used page behind the border: its number among those
+    int* used;                                   // the border: pages in use
+};
+
+__global__ void __launch_bounds__(kThreads) compact_scan_kernel(CompactArgs a) {
+    grid_dependency_trigger();
+    grid_dependency_wait();
+    scan_chunk(a.pool, blockIdx.x, a.p.refs, a.p.new_refs, [](int r) { return r != 0; });
+}
+
+// Pages in use below `page`: the sums of the chunks before it, and of the words before it in its chunk. A warp's work.
+__device__ __forceinline__ int used_below(const Pool& pool, const int* before, int total, int page) {
+    const int lane = threadIdx.x & 31;
+    if (page >= pool.n_pages) return total;
+    const int chunk = page / pool.chunk;
+    int n = 0;
+    for (int w = chunk * (pool.chunk / 32) + lane; w <= page / 32; w += 32) {
+        const unsigned b = pool.bits[w];
+        n += __popc(w < page / 32 ? b : b & ((1u << (page & 31)) - 1));
+    }
+#pragma unroll
+    for (int d = 16; d; d /= 2) n += __shfl_xor_sync(~0u, n, d);
+    return before[chunk] + n;
+}
+
+// The k-th used page behind the border and the k-th free one before it get copy k.
+__global__ void __launch_bounds__(kThreads) compact_pair_kernel(CompactArgs a) {
+    __shared__ int before[kMostChunks];
+    __shared__ int below_border;
+    const OgleCompactParams& p = a.p;
+    const Pool& pool = a.pool;
+    const int tid = threadIdx.x, lane = tid & 31;
+    grid_dependency_trigger();
+    grid_dependency_wait();
+    const int used = sum_chunks<kThreads / 32>(pool, before);
+    if (tid < 32) {
+        const int n = used_below(pool, before, used, used);
+        if (tid == 0) below_border = n;
+    }
+    __syncthreads();
+    const int moves = used - below_border;       // used behind the border, and free before it
+    if (blockIdx.x == 0) {
+        if (tid == 0) {
+            *a.used = used;
+            p.state[0] = used;
+            p.state[1] = moves - min(moves, p.n_copies);
+        }
+        for (int k = moves + tid; k < p.n_copies; k += kThreads) {
+            p.copies[3 * k] = p.copies[3 * k + 1] = -1;
+            p.copies[3 * k + 2] = 0;
+        }
+    }
+    const int first = blockIdx.x * pool.chunk, end = min(first + pool.chunk, pool.n_pages);
+    int sum = before[blockIdx.x];                // used pages below the warp's word, kept by each warp for itself
+    const int words = (end - first + 31) / 32;
+    for (int w0 = 0; w0 < words; w0 += 32) {     // 32 words: every warp sums them, each then has every eighth
+        const unsigned b = w0 + lane < words ? pool.bits[first / 32 + w0 + lane] : 0u;
+        int in = __popc(b);
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const int o = __shfl_up_sync(~0u, in, d);
+            if (lane >= d) in += o;
+        }
+        const int ex = in - __popc(b);
+        for (int w = tid / 32; w < 32; w += kThreads / 32) {
+            const unsigned word = __shfl_sync(~0u, b, w);
+            const int page = first + (w0 + w) * 32 + lane, n = sum + __shfl_sync(~0u, ex, w) + __popc(word & ((1u << lane) - 1));
+            if (page >= end) continue;
+            const bool is_used = word >> lane & 1;
+            if (is_used && page >= used) {
+                const int k = n - below_border;
+                a.rank[page] = k;
+                if (k < p.n_copies) {
+                    p.copies[3 * k] = page;
+                    p.copies[3 * k + 2] = p.page_tokens;
+                }
+            } else if (!is_used && page < used) {
+                const int k = page - n;
+                if (k < p.n_copies) p.copies[3 * k + 1] = page;
+            }
+        }
+        sum += __shfl_sync(~0u, in, 31);
+    }
+}
+
+__global__ void __launch_bounds__(kThreads) compact_table_kernel(CompactArgs a) {
+    const OgleCompactParams& p = a.p;
+    grid_dependency_trigger();
+    grid_dependency_wait();
+    const int used = *a.used;
+    const long long entries = (long long)p.n_seqs * p.blocks, all = entries + p.n_copies;
+    for (long long i = blockIdx.x * (long long)kThreads + threadIdx.x; i < all; i += (long long)gridDim.x * kThreads) {
+        if (i < entries) {
+            const int row = int(i / p.blocks), c = int(i % p.blocks);
+            int page = p.table[row * p.table_stride + c];        // (not a read-only load: new_table may be table)
+            if (is_page(page, p.n_pages) && page >= used && __ldg(p.refs + page) != 0) {
+                const int k = a.rank[page];
+                if (k < p.n_copies) page = p.copies[3 * k + 1];
+            }
+            p.new_table[row * p.new_stride + c] = page;
+        } else {
+            const int k = int(i - entries), src = p.copies[3 * k], dst = p.copies[3 * k + 1];
+            if (src >= 0) {
+                p.new_refs[dst] = __ldg(p.refs + src);
+                p.new_refs[src] = 0;
+            }
+        }
+    }
+}
+
+// ---- copies
+constexpr int kMostLayers = 64;                  // of a launch
+constexpr int kUnit = 4096;                      // bytes that a warp copies at a time: 8 x 16 a lane
+struct CopyArgs {
+    int n_copies, n_layers, kv_heads, dim, page_tokens, n_pages;
+    long long page_stride, head_stride, token_stride;
+    const int* copies;
+    int unit_rows, units;                        // rows (a token of a head) of a unit; units of a page
+    int packed;                                  // a page's bytes lie in one piece
+    OglePageTensors layer[kMostLayers];
+};
+
+// A warp has a unit of one page's keys or values in one layer; that of the page's first unit its scales, too. A unit's loads are under way
+// together, and the units of an SM's warps: 96 KB and more.
+__global__ void __launch_bounds__(kThreads) copy_pages_kernel(const __grid_constant__ CopyArgs a) {
+    const int lane = threadIdx.x & 31;
+    grid_dependency_trigger();
+    grid_dependency_wait();
+    const long long all = (long long)a.n_copies * a.n_layers * 2 * a.units, step = (long long)gridDim.x * (kThreads / 32);
+    for (long long u = (long long)blockIdx.x * (kThreads / 32) + threadIdx.x / 32; u < all; u += step) {
+        // neighbours in a block: the units of a page, then keys and values, then layers, so that a copy's entry is read from near
+        const int unit = int(u % a.units);
+        const long long rest = u / a.units;
+        const int kind = int(rest & 1), layer = int((rest >> 1) % a.n_layers), c = int((rest >> 1) / a.n_layers);
+        const int src = __ldg(a.copies + 3 * c), dst = __ldg(a.copies + 3 * c + 1), tokens = min(__ldg(a.copies + 3 * c + 2), a.page_tokens);
+        if ((unsigned)src >= (unsigned)a.n_pages || (unsigned)dst >= (unsigned)a.n_pages || src == dst) continue;
+        const OglePageTensors& t = a.layer[layer];
+        unsigned char* const base = static_cast<unsigned char*>(kind ? t.v : t.k);
+        const unsigned char* const from = base + src * a.page_stride;
+        unsigned char* const to = base + dst * a.page_stride;
+        if (unit == 0) {
+            float* const scale = kind ? t.v_scale : t.k_scale;
+            for (int h = lane; h < a.kv_heads; h += 32) scale[(long long)dst * a.kv_heads + h] = scale[(long long)src * a.kv_heads + h];
+            if (kind == 0 && t.bounds) {
+                const long long bytes = 2LL * a.kv_heads * a.dim;
+                const uint4* const f = reinterpret_cast<const uint4*>(t.bounds + src * bytes);
+                uint4* const g = reinterpret_cast<uint4*>(t.bounds + dst * bytes);
+                for (int i = lane; i < bytes / 16; i += 32) g[i] = f[i];
+                for (int h = lane; h < a.kv_heads; h += 32)
+                    t.bounds_scale[(long long)dst * a.kv_heads + h] = t.bounds_scale[(long long)src * a.kv_heads + h];
+            }
+        }
+        if (tokens <= 0) continue;
+        const int vecs = a.dim / 16, rows = min(a.kv_heads * tokens - unit * a.unit_rows, a.unit_rows), n = rows * vecs;
+        if (n <= 0) continue;
+        const bool whole = a.packed && tokens == a.page_tokens;
+        // quotients by reciprocals: of i below 256 x 16 exactly, of rows (2^22 at most) within one
+        const float by_vecs = 1.f / float(vecs), by_tokens = 1.f / float(tokens);
+        const auto offset = [&](int i) {
+            if (whole) return (long long)unit * a.unit_rows * a.dim + i * 16LL;
+            const int r = int((float(i) + 0.5f) * by_vecs), row = unit * a.unit_rows + r;
+            int h = int((float(row) + 0.5f) * by_tokens), t = row - h * tokens;
+            if (t < 0) { --h; t += tokens; }
+            if (t >= tokens) { ++h; t -= tokens; }
+            return h * a.head_stride + t * a.token_stride + (i - r * vecs) * 16LL;
+        };
+        constexpr int U = 8;
+        for (int i0 = lane; i0 < n; i0 += 32 * U) {
+            uint4 v[U];
+#pragma unroll
+            for (int x = 0; x < U; ++x)
+                if (i0 + x * 32 < n) v[x] = *reinterpret_cast<const uint4*>(from + offset(i0 + x * 32));
+#pragma unroll
+            for (int x = 0; x < U; ++x)
+                if (i0 + x * 32 < n) *reinterpret_cast<uint4*>(to + offset(i0 + x * 32)) = v[x];
+        }
+    }
+}
+
+Pool pool_of(int n_pages) {
+    Pool pool = {};
+    pool.n_pages = n_pages;
+    pool.chunk = kChunkPages;
+    while (div_up(n_pages, pool.chunk) > kMostChunks) pool.chunk *= 2;
+    pool.chunks = div_up(n_pages, pool.chunk);
+    return pool;
+}
+size_t pool_words(const Pool& pool) { return size_t(pool.n_pages + 31) / 32 + pool.chunks; }
+bool page_size_ok(int tokens) { return tokens >= 16 && tokens <= 1024 && (tokens & (tokens - 1)) == 0; }
+int failed(cudaError_t e) {
+    set_last_error(e);
+    (void)cudaGetLastError();
+    return OGLE_ERR_CUDA;
+}
+
+int check_advance(const OgleAdvanceParams* p) {
+    if (!p || p->n_old < 0 || p->n_new < 0 || p->old_blocks < 0 || p->new_blocks < 0 || p->n_pages < 0 || !page_size_ok(p->page_tokens)) return OGLE_ERR_INVALID;
+    if (p->n_pages > kMostPages || p->n_old > (1 << 24) || p->n_new > (1 << 24) || p->new_blocks > (1 << 24) || p->old_blocks > (1 << 24)) return OGLE_ERR_UNSUPPORTED;
+    if ((long long)p->n_new * p->new_blocks >= (1LL << 31)) return OGLE_ERR_UNSUPPORTED;      // requests are counted in 32 bits
+    if ((p->n_old > 1 && p->old_stride < p->old_blocks) || (p->n_new > 1 && p->new_stride < p->new_blocks)) return OGLE_ERR_INVALID;
+    return OGLE_OK;
+}
+int check_compact(const OgleCompactParams* p) {
+    if (!p || p->n_seqs < 0 || p->blocks < 0 || p->n_pages < 0 || p->n_copies < 0 || !page_size_ok(p->page_tokens)) return OGLE_ERR_INVALID;
+    if (p->n_pages > kMostPages) return OGLE_ERR_UNSUPPORTED;
+    if (p->n_seqs > 1 && (p->table_stride < p->blocks || p->new_stride < p->blocks)) return OGLE_ERR_INVALID;
+    return OGLE_OK;
+}
+
+}  // namespace
+}  // namespace ogle
+
+using namespace ogle;
+
+extern "C" {
+
+size_t ogle_cuda_advance_pages_workspace_bytes(const OgleAdvanceParams* p) {
+    if (check_advance(p) != OGLE_OK) return 0;
+    return (pool_words(pool_of(p->n_pages)) + 2 * size_t(p->n_old) + p->n_new + 1) * 4;
+}
+
+int ogle_cuda_advance_pages(const OgleAdvanceParams* p, void* workspace, size_t workspace_bytes, ogle_stream_t stream) {
+    const int rc = check_advance(p);
+    if (rc != OGLE_OK) return rc;
+    if (!p->state || (p->n_pages > 0 && (!p->refs || !p->new_refs)) || (p->n_old > 0 && (!p->table || !p->kv_len)) ||
+        (p->n_new > 0 && (!p->parent || !p->new_table || !p->new_len || !p->copies)) || !workspace)
+        return OGLE_ERR_INVALID;
+    // the rows of several texts read the row of one
+    if ((p->n_pages > 0 && p->refs == p->new_refs) || (p->n_new > 0 && (p->table == p->new_table || p->kv_len == p->new_len))) return OGLE_ERR_INVALID;
+    if (workspace_bytes < ogle_cuda_advance_pages_workspace_bytes(p)) return OGLE_ERR_INVALID;
+    if (reinterpret_cast<uintptr_t>(workspace) & 3) return OGLE_ERR_ALIGNMENT;
+    AdvanceArgs a = {};
+    a.p = *p;
+    a.pool = pool_of(p->n_pages);
+    a.pool.bits = static_cast<unsigned*>(workspace);
+    a.pool.counts = reinterpret_cast<int*>(a.pool.bits + (p->n_pages + 31) / 32);
+    a.children = a.pool.counts + a.pool.chunks;
+    a.first_child = a.children + p->n_old;
+    a.base = a.first_child + p->n_old;
+    a.page_shift = 4;
+    while ((1 << a.page_shift) < p->page_tokens) ++a.page_shift;
+    cudaError_t e = launch_overlapped(advance_plan_kernel, dim3(a.pool.chunks + 1), dim3(kThreads), 0, stream, a);
+    if (e != cudaSuccess) return failed(e);
+    const int done = finish_launch();
+    if (done != OGLE_OK) return done;
+    const int rows = p->n_new > p->n_old ? p->n_new : p->n_old;
+    e = launch_overlapped_if(overlapped_launches_enabled(true), advance_rows_kernel, dim3(rows < 1 ? 1 : rows), dim3(kRowWarps * 32), 0, stream, a);
+    return e == cudaSuccess ? finish_launch() : failed(e);
+}
+
+size_t ogle_cuda_compact_pages_workspace_bytes(const OgleCompactParams* p) {
+    if (check_compact(p) != OGLE_OK) return 0;
+    return (pool_words(pool_of(p->n_pages)) + size_t(p->n_pages) + 1) * 4;
+}
+
+int ogle_cuda_compact_pages(const OgleCompactParams* p, void* workspace, size_t workspace_bytes, ogle_stream_t stream) {
+    const int rc = check_compact(p);
+    if (rc != OGLE_OK) return rc;
+    const bool table = p->n_seqs > 0 && p->blocks > 0;
+    if (!p->state || (p->n_pages > 0 && (!p->refs || !p->new_refs)) || (table && (!p->table || !p->new_table)) || (p->n_copies > 0 && !p->copies) || !workspace)
+        return OGLE_ERR_INVALID;
+    if (p->n_pages > 0 && p->refs == p->new_refs) return OGLE_ERR_INVALID;
+    if (workspace_bytes < ogle_cuda_compact_pages_workspace_bytes(p)) return OGLE_ERR_INVALID;
+    if (reinterpret_cast<uintptr_t>(workspace) & 3) return OGLE_ERR_ALIGNMENT;
+    CompactArgs a = {};
+    a.p = *p;
+    a.pool = pool_of(p->n_pages);
+    a.pool.bits = static_cast<unsigned*>(workspace);
+    a.pool.counts = reinterpret_cast<int*>(a.pool.bits + (p->n_pages + 31) / 32);
+    a.rank = a.pool.counts + a.pool.chunks;
+    a.used = a.rank + p->n_pages;
+    const bool overlapped = overlapped_launches_enabled(true);
+    cudaError_t e = cudaSuccess;
+    int done = OGLE_OK;
+    if (p->n_pages > 0) {
+        e = launch_overlapped(compact_scan_kernel, dim3(a.pool.chunks), dim3(kThreads), 0, stream, a);
+        if (e != cudaSuccess) return failed(e);
+        done = finish_launch();
+        if (done != OGLE_OK) return done;
+    }
+    e = launch_overlapped_if(overlapped && p->n_pages > 0, compact_pair_kernel, dim3(a.pool.chunks > 0 ? a.pool.chunks : 1), dim3(kThreads), 0, stream, a);
+    if (e != cudaSuccess) return failed(e);
+    done = finish_launch();
+    const long items = (table ? (long)p->n_seqs * p->blocks : 0) + p->n_copies;
+    if (done != OGLE_OK || items == 0) return done;
+    if (!table) a.p.n_seqs = a.p.blocks = 0;
+    e = launch_overlapped_if(overlapped, compact_table_kernel, dim3(grid_for(items, kThreads)), dim3(kThreads), 0, stream, a);
+    return e == cudaSuccess ? finish_launch() : failed(e);
+}
+
+int ogle_cuda_copy_pages(const OgleCopyPagesParams* p, const OglePageTensors* layers_host_array, ogle_stream_t stream) {
+    if (!p || p->n_copies < 0 || p->n_layers < 0 || p->n_pages < 0 || p->kv_heads < 1 || p->kv_heads > 4096 || !page_size_ok(p->page_tokens)) return OGLE_ERR_INVALID;
+    if (p->head_dim < 16 || p->head_dim % 16 != 0) return OGLE_ERR_INVALID;
+    if (p->head_dim > 256) return OGLE_ERR_UNSUPPORTED;
+    if ((p->page_stride | p->head_stride | p->token_stride) & 15) return OGLE_ERR_ALIGNMENT;
+    if (p->page_stride < 1 || p->head_stride < 1 || p->token_stride < p->head_dim) return OGLE_ERR_INVALID;
+    if (p->n_copies == 0 || p->n_layers == 0 || p->n_pages == 0) return OGLE_OK;
+    if (!p->copies || !layers_host_array) return OGLE_ERR_INVALID;
+    for (int l = 0; l < p->n_layers; ++l) {
+        const OglePageTensors& t = layers_host_array[l];
+        if (!t.k || !t.v || !t.k_scale || !t.v_scale || (t.bounds && !t.bounds_scale)) return OGLE_ERR_INVALID;
+        if (!aligned16(t.k) || !aligned16(t.v) || !aligned16(t.bounds)) return OGLE_ERR_ALIGNMENT;
+    }
+    CopyArgs a;
+    a.n_copies = p->n_copies; a.kv_heads = p->kv_heads; a.dim = p->head_dim; a.page_tokens = p->page_tokens; a.n_pages = p->n_pages;
+    a.page_stride = p->page_stride; a.head_stride = p->head_stride; a.token_stride = p->token_stride;
+    a.copies = p->copies;
+    a.unit_rows = kUnit / p->head_dim;
+    a.units = div_up((long)p->kv_heads * p->page_tokens, a.unit_rows);
+    a.packed = p->token_stride == p->head_dim && p->head_stride == p->token_stride * p->page_tokens;
+    for (int first = 0; first < p->n_layers; first += kMostLayers) {
+        a.n_layers = p->n_layers - first < kMostLayers ? p->n_layers - first : kMostLayers;
+        for (int l = 0; l < a.n_layers; ++l) a.layer[l] = layers_host_array[first + l];
+        const long warps = (long)a.n_copies * a.n_layers * 2 * a.units;
+        const cudaError_t e = launch_overlapped(copy_pages_kernel, dim3(grid_for(warps * 32, kThreads)), dim3(kThreads), 0, stream, a);
+        if (e != cudaSuccess) return failed(e);
+        const int rc = finish_launch();
+        if (rc != OGLE_OK) return rc;
+    }
+    return OGLE_OK;
+}
+
+}  // extern "C"

@@ -22,6 +22,9 @@ from .ops import _stream
 _DTYPE = {torch.float32: _lib.DTYPE_F32, torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
 _PAGED_BATCH, _APPEND = _lib.packer(_lib.PagedBatch).pack, _lib.packer(_lib.AppendParams).pack
 _ATTENTION, _LOGITS = _lib.packer(_lib.AttentionParams).pack, _lib.packer(_lib.LogitsParams).pack
+_BEAM, _ADVANCE = _lib.packer(_lib.BeamParams).pack, _lib.packer(_lib.AdvanceParams).pack
+_COMPACT, _COPY_PAGES = _lib.packer(_lib.CompactParams).pack, _lib.packer(_lib.CopyPagesParams).pack
+_PAGE_TENSORS = _lib.packer(_lib.PageTensors).pack
 _I32, _F32, _E4M3 = torch.int32, torch.float32, torch.float8_e4m3fn
 
 
@@ -181,3 +184,111 @@ def adjust_logits(logits, tokens=None, token_start=None, prompt_len=None, repeti
                 _vector(bias_start, _I32, rows + 1, "bias_start"), allowed.data_ptr() if allowed is not None else 0)
     check(_lib.cuda_lib().ogle_cuda_adjust_logits(p, _stream()), "adjust_logits")
     return out
+
+
+def _table(t, name):
+    """(sequences, blocks, row stride) of a block table."""
+    shape, stride = t.shape, t.stride()
+    if t.dtype != _I32 or not t.is_cuda or len(shape) != 2 or stride[1] != 1 and shape[1] > 1:
+        raise ValueError(f"{name}: expected an int32 CUDA tensor [sequences, blocks]")
+    return shape[0], shape[1], stride[0] if shape[0] > 1 else shape[1]
+
+
+def beam_step(logits, scores, beams, count, ends=None):
+    """The best continuations of each group of `beams` rows of logits [groups * beams, vocab] (ogle_cuda_beam_step): by the rows' scores
+    (float32 [groups * beams]: the logarithm of what each text has come to; not finite: no such text; None: 0) plus the logarithm of the
+    token's probability. Returns (score, beam, token) of the `count` best, [groups, count], in falling order, equal ones by beam and
+    token, behind the last -inf, -1, -1; and (next_row, next_token, next_score) [groups * beams]: the first `beams` of these whose token is not
+    among `ends` (int32), as advance_pages takes them - the row that each goes on from, or -1."""
+    if logits.dim() != 2 or not logits.is_cuda or logits.dtype not in _DTYPE or logits.stride(1) != 1 and logits.shape[1] > 1:
+        raise ValueError("logits: expected a CUDA tensor [rows, vocab] in float32, float16 or bfloat16, a row's elements side by side")
+    rows, vocab = logits.shape
+    if beams < 1 or rows % beams != 0:
+        raise ValueError(f"{rows} rows are no whole groups of {beams} beams")
+    groups = rows // beams
+    score, next_score = logits.new_empty(groups, count, dtype=_F32), logits.new_empty(rows, dtype=_F32)
+    found, following = logits.new_empty(2, groups, count, dtype=_I32), logits.new_empty(2, rows, dtype=_I32)
+    beam, token = found.unbind(0)
+    next_row, next_token = following.unbind(0)
+    p = _BEAM(groups, beams, vocab, count, _DTYPE[logits.dtype], ends.numel() if ends is not None else 0, logits.stride(0) if rows > 1 else vocab,
+              logits.data_ptr(), _vector(scores, _F32, rows, "scores"), _vector(ends, _I32, None, "ends"), score.data_ptr(), beam.data_ptr(),
+              token.data_ptr(), next_row.data_ptr(), next_token.data_ptr(), next_score.data_ptr())
+    lib = _lib.cuda_lib()
+    n = lib.ogle_cuda_beam_step_workspace_bytes(p)
+    workspace = logits.new_empty(max(n, 16), dtype=torch.uint8)
+    check(lib.ogle_cuda_beam_step(p, workspace.data_ptr(), n, _stream()), "beam_step")
+    return score, beam, token, next_row, next_token, next_score
+
+
+def advance_pages(block_table, kv_len, parent, new, refs, page_tokens, blocks=None):
+    """Block table of the texts that go on (ogle_cuda_advance_pages). Text i goes on from sequence parent[i] of block_table and kv_len (-1: from
+    nothing) and is about to have new[i] more tokens (int32, or one number for all): it shares the parent's full pages, keeps or copies the last
+    one and gets what else its tokens need. refs int32 [pages]: how many table entries name each page. Sequences that no text goes on from
+    are gone. Nothing is changed in place. Returns (table [texts, blocks], kv_len with the new tokens, refs, copies int32 [texts, 3] for
+    copy_pages, state): state[0] pages are free for the next call, state[1] requests found none (an entry of -1: take the old table
+    again, with fewer texts). blocks: columns of the new table, as the old one where None."""
+    seqs, old_blocks, stride = _table(block_table, "block_table")
+    n, pages = parent.numel(), refs.numel()
+    blocks = old_blocks if blocks is None else blocks
+    # one allocation for all five
+    out = refs.new_empty(n * (blocks + 4) + pages + 2)
+    at = out.data_ptr()
+    tokens = new if isinstance(new, torch.Tensor) else None
+    p = _ADVANCE(seqs, n, old_blocks, blocks, page_tokens, pages, 0 if tokens is not None else new, 0, stride, blocks, block_table.data_ptr(),
+                 _vector(kv_len, _I32, seqs, "kv_len"), _vector(parent, _I32, n, "parent"), _vector(tokens, _I32, n, "new"),
+                 _vector(refs, _I32, pages, "refs"), at, at + 4 * n * blocks, at + 4 * n * (blocks + 4), at + 4 * n * (blocks + 1),
+                 at + 4 * (n * (blocks + 4) + pages))
+    lib = _lib.cuda_lib()
+    size = lib.ogle_cuda_advance_pages_workspace_bytes(p)
+    workspace = refs.new_empty(size // 4 + 1)
+    check(lib.ogle_cuda_advance_pages(p, workspace.data_ptr(), size, _stream()), "advance_pages")
+    table, length, copies, new_refs, state = out.split([n * blocks, n, 3 * n, pages, 2])
+    return table.view(n, blocks), length, new_refs, copies.view(n, 3), state
+
+
+def compact_pages(block_table, refs, most, page_tokens):
+    """Moves used pages to the front of the pool (ogle_cuda_compact_pages), `most` of them at most. Nothing is changed in place. Returns
+    (table, refs, copies int32 [most, 3] for copy_pages, state): state[0] pages are in use, state[1] moves are left for another call."""
+    seqs, blocks, stride = _table(block_table, "block_table")
+    pages = refs.numel()
+    out = refs.new_empty(seqs * blocks + pages + 3 * most + 2)
+    at = out.data_ptr()
+    p = _COMPACT(seqs, blocks, page_tokens, pages, most, 0, stride, blocks, block_table.data_ptr(), _vector(refs, _I32, pages, "refs"), at,
+                 at + 4 * seqs * blocks, at + 4 * (seqs * blocks + pages), at + 4 * (seqs * blocks + pages + 3 * most))
+    lib = _lib.cuda_lib()
+    size = lib.ogle_cuda_compact_pages_workspace_bytes(p)
+    workspace = refs.new_empty(size // 4 + 1)
+    check(lib.ogle_cuda_compact_pages(p, workspace.data_ptr(), size, _stream()), "compact_pages")
+    table, new_refs, copies, state = out.split([seqs * blocks, pages, 3 * most, 2])
+    return table.view(seqs, blocks), new_refs, copies.view(most, 3), state
+
+
+def copy_pages(caches, copies, bounds=None):
+    """For each (page, new page, tokens) of copies, int32 [n, 3], the first tokens of the page's keys and values and its scales in each of
+    the caches (ogle_cuda_copy_pages), in place; bounds, where there are some, go along: one pair (see new_bounds) for each cache."""
+    if not caches:
+        return
+    k0 = caches[0][0]
+    shape, stride = k0.shape, k0.stride()
+    if len(shape) != 4 or stride[3] != 1:
+        raise ValueError("caches: expected keys and values [pages, kv heads, page tokens, head dim], the elements of a token side by side")
+    pages, heads, page_tokens, dim = shape
+    layers = []
+    for i, (k, v, k_scale, v_scale) in enumerate(caches):
+        if k.dtype != _E4M3 or v.dtype != _E4M3 or not k.is_cuda or not v.is_cuda or k.shape != shape or v.shape != shape or k.stride() != stride or v.stride() != stride:
+            raise ValueError("caches: expected float8_e4m3fn CUDA tensors of the same shape and strides for all keys and values")
+        b = (0, 0) if bounds is None else _bounds(bounds[i], pages, heads, dim)
+        layers.append(_PAGE_TENSORS(k.data_ptr(), v.data_ptr(), _vector(k_scale, _F32, pages * heads, "k_scale"),
+                                    _vector(v_scale, _F32, pages * heads, "v_scale"), *b))
+    if copies.dim() != 2 or copies.shape[1] != 3:
+        raise ValueError("copies: expected [n, 3]")
+    p = _COPY_PAGES(copies.shape[0], len(layers), heads, dim, page_tokens, pages, stride[0], stride[1], stride[2], _vector(copies, _I32, None, "copies"))
+    check(_lib.cuda_lib().ogle_cuda_copy_pages(p, b"".join(layers), _stream()), "copy_pages")
+
+
+def _bounds(bounds, pages, heads, dim):
+    """Addresses of a cache's bounds."""
+    lo_hi, scale = bounds
+    if lo_hi.shape != (pages, heads, 2, dim):
+        raise ValueError(f"bounds: expected int8 [{pages}, {heads}, 2, {dim}]")
+    return _vector(lo_hi, torch.int8, None, "bounds"), _vector(scale, _F32, pages * heads, "the bounds' scale")
