@@ -612,6 +612,46 @@ typedef struct {
 } OgleCopyPagesParams;
 int ogle_cuda_copy_pages(const OgleCopyPagesParams* p, const OglePageTensors* layers_host_array, ogle_stream_t stream);
 
+/* ---------------------------------- attention over chosen pages of the cache */
+/* Bounds of the keys of every page that a row of the batch was appended to: bounds [n_pages][kv_heads][2][head_dim], the least and the
+ * largest of the page's keys in every element as whole numbers, rounded away from each other, and their unit bounds_scale [n_pages]
+ * [kv_heads]: value = bounds * bounds_scale. The unit is the page's scale times the smallest power of two t with |e4m3| <= 127 t. Of a page
+ * those of its slots count that hold tokens of the sequence (positions below kv_len); a NaN does not count. To be called behind
+ * ogle_cuda_kv_append, with its batch; pages that it does not touch keep their bounds. */
+int ogle_cuda_page_bounds(const OglePagedBatch* batch, signed char* bounds, float* bounds_scale, ogle_stream_t stream);
+
+/* For each row and kv head the `count` pages that its query heads attend, as blocks of the row's sequence (position / page_tokens):
+ *   blocks [0, first) and the row's own block with the last - 1 before it, always (first + last at most count, last at least 1);
+ *   of the others up to the row's own those with the largest scores, equal ones from the lowest.
+ * chosen[row][head][0 .. count), rising, filled up with -1; a block without a page is never among them. Score of a page: the largest
+ * over the head's group of query heads of
+ *   sum_d (q_d > 0 ? q_d hi_d : q_d lo_d) * bounds_scale
+ * where q are the row's queries as whole numbers, q / s rounded to the nearest (even) and cut at +-127, s the smallest power of two with
+ * |q| <= 127 s over the group's heads (infinities and NaN count as 0). All of it is exact in fp32. For attention whose scale is positive. */
+typedef struct {
+    const void* q;
+    long long q_row, q_head;
+    const signed char* bounds;
+    const float* bounds_scale;
+    int* chosen;
+    long long chosen_row, chosen_head;     /* strides */
+    int count, first, last, reserved;
+} OgleChooseParams;
+size_t ogle_cuda_choose_pages_workspace_bytes(const OglePagedBatch* batch, const OgleChooseParams* p);
+int ogle_cuda_choose_pages(const OglePagedBatch* batch, const OgleChooseParams* p, void* workspace, size_t workspace_bytes, ogle_stream_t stream);
+
+/* ogle_cuda_paged_attention over chosen pages alone: a row's query heads of kv head h attend the tokens up to its position of the blocks
+ * chosen[row][h][0 .. count), rising and filled up with -1 as ogle_cuda_choose_pages leaves them. p->causal is 1 and p->window 0. Results,
+ * precision and workspace as there; a row that no block was chosen for has out 0 and lse minus infinity. */
+typedef struct {
+    const int* chosen;
+    long long chosen_row, chosen_head;
+    int count, reserved;
+} OgleChosenPages;
+size_t ogle_cuda_sparse_attention_workspace_bytes(const OglePagedBatch* batch, const OgleAttentionParams* p, const OgleChosenPages* c);
+int ogle_cuda_sparse_attention(const OglePagedBatch* batch, const OgleAttentionParams* p, const OgleChosenPages* c, void* workspace,
+                               size_t workspace_bytes, ogle_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -162,6 +162,9 @@ struct Segment {
     int j_begin, steps;                           // the range's keys in steps
     Span keys;                                    // that some row attends
     int inner_lo, inner_hi;                       // that every row attends
+    const int* blocks;                            // chosen pages: of the one row, or ...
+    const int2* list;                             // ... of the tile's rows
+    int first_row, entries;
 };
 
 // One thread: the next segment of the range; false where there is none.
@@ -205,7 +208,7 @@ __device__ __forceinline__ bool next_segment(const AttnArgs& a, Walk& w, Segment
 }
 
 // One thread: the cluster's segment, and this block's share of its tiles; false where there is no such tile of rows.
-template <int kRows>
+template <int kRows, bool kChosen>
 __device__ __forceinline__ bool cluster_segment(const AttnArgs& a, Segment& g) {
     const Batch& B = a.b;
     const int c = blockIdx.x / a.cluster, rank = blockIdx.x % a.cluster, rt = c % a.by_segment;
@@ -219,7 +222,18 @@ __device__ __forceinline__ bool cluster_segment(const AttnArgs& a, Segment& g) {
     g.keys = span_of(g.s, first_row, last_row, a.causal, a.window);
     g.inner_lo = span_of(g.s, last_row, 0, a.causal, a.window).lo;
     g.inner_hi = span_of(g.s, 0, first_row, a.causal, a.window).hi;
-    const int lo = g.keys.lo & ~(kChunk - 1), chunks = g.keys.hi > lo ? (g.keys.hi - lo + kChunk - 1) / kChunk : 0;
+    int lo = g.keys.lo & ~(kChunk - 1), chunks = g.keys.hi > lo ? (g.keys.hi - lo + kChunk - 1) / kChunk : 0;
+    if constexpr (kChosen) {
+        // keys by their place in the list of pages
+        g.first_row = first_row;
+        g.list = a.lists ? a.lists + (long long)c * a.list_stride : nullptr;
+        g.blocks = a.chosen + (g.s.row0 + first_row) * a.chosen_row + g.h * a.chosen_head;
+        // (a row's choice may be shorter still: what is behind its end names no page)
+        g.entries = a.lists ? a.list_len[c] : min(a.count, g.keys.hi > 0 ? ((g.keys.hi - 1) >> B.page_shift) + 1 : 0);
+        lo = 0;
+        chunks = g.entries << B.page_shift >> 4;
+        static_assert(kChunk == 16, "");
+    }
     const int c0 = chunks * rank / a.cluster, c1 = chunks * (rank + 1) / a.cluster;
     g.j_begin = lo + c0 * kChunk;
     g.steps = c1 - c0;
@@ -271,7 +285,9 @@ __device__ __noinline__ void cluster_join(const AttnArgs& a, const Segment& g, c
     }
 }
 
-template <int DP, int MT, bool kSplit>
+// kChosen: over the pages that rows have chosen, a segment to a cluster (of one block or more). A place in the segment's list of pages
+// stands for a key until it is looked up.
+template <int DP, int MT, bool kSplit, bool kChosen>
 __global__ void __launch_bounds__(kWarps * 32, (Form<DP, MT, kSplit>::kBlocks))
 paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
     using F = Form<DP, MT, kSplit>;
@@ -294,8 +310,8 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
     if (tid == 0) gave_up = 0;
     grid_dependency_trigger();
     grid_dependency_wait();
-    if (a.cluster) {
-        if (tid == 0) more_segments = cluster_segment<kRows>(a, segment);
+    if (kChosen || a.cluster) {
+        if (tid == 0) more_segments = cluster_segment<kRows, kChosen>(a, segment);
         __syncthreads();
         if (!more_segments) return;
     } else {
@@ -322,9 +338,31 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
         // pages and scales of the warp's next 32 steps, a lane each; the 32 behind them are on their way
         int page[2] = {nowhere, nowhere};         // where there is no page: the copies find themselves outside and bring zeros
         float ks[2] = {0.f, 0.f}, vs[2] = {0.f, 0.f};
+        const int in_page = (1 << B.page_shift) - 1;
+        int start[2] = {0, 0};                    // chosen pages: a step's first key
+        unsigned seen_by[2] = {0u, 0u};           // and the rows that have chosen its page
         const auto look_up = [&](int which, int i) {
             int p = -1;
-            if (i < count) p = paged::page_of(B, segment.b, (j_begin + (i * kWarps + warp) * kChunk) >> B.page_shift);
+            if (i < count) {
+                const int at = j_begin + (i * kWarps + warp) * kChunk;
+                int block = at >> B.page_shift;
+                if constexpr (kChosen) {
+                    seen_by[which] = ~0u;
+                    if (segment.list) {
+                        const int2 e = segment.list[block];
+                        block = e.x;
+                        seen_by[which] = unsigned(e.y);
+                    } else {
+                        block = __ldg(segment.blocks + block);
+                    }
+                    // none, or one behind the text
+                    if (block < 0 || block > (segment.s.len - 1) >> B.page_shift) block = -1;
+                    start[which] = block < 0 ? 0 : (block << B.page_shift) + (at & in_page);
+                    if (block >= 0) p = paged::page_of(B, segment.b, block);
+                } else {
+                    p = paged::page_of(B, segment.b, block);
+                }
+            }
             page[which] = p >= 0 ? p : nowhere;
             ks[which] = vs[which] = 0.f;
             if (p >= 0) {
@@ -335,7 +373,6 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
         };
         look_up(0, lane);
         look_up(1, 32 + lane);
-        const int in_page = (1 << B.page_shift) - 1;
         const auto issue = [&](int i, int p) {    // step i, whose page is p
             if (lane == 0) {
                 const uint32_t dst = ring + put * F::kStageBytes, bar = bar0 + put * 8;
@@ -417,6 +454,7 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
         for (int i = 0; i < count; ++i) {
             if ((i & 31) == 0 && i > 0) {
                 page[0] = page[1]; ks[0] = ks[1]; vs[0] = vs[1];
+                if constexpr (kChosen) { start[0] = start[1]; seen_by[0] = seen_by[1]; }
                 look_up(1, i + 32 + lane);
             }
             const unsigned char* const step = my_ring + get * F::kStageBytes;
@@ -435,9 +473,10 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
                 break;
             }
             if (++get == F::kStages) { get = 0; parity ^= 1; }
-            const int j0 = j_begin + (i * kWarps + warp) * kChunk;
+            const int j0 = kChosen ? __shfl_sync(~0u, start[0], i & 31) : j_begin + (i * kWarps + warp) * kChunk;
+            const unsigned rows_here = kChosen ? __shfl_sync(~0u, seen_by[0], i & 31) : ~0u;
             const float k_scale = __shfl_sync(~0u, ks[0], i & 31), v_scale = __shfl_sync(~0u, vs[0], i & 31);
-            const bool edge = j0 < inner_lo || j0 + kChunk > inner_hi || k_scale == 0.f;       // 0: no page, or one of zeros
+            const bool edge = j0 < inner_lo || j0 + kChunk > inner_hi || k_scale == 0.f || rows_here != ~0u;       // 0: no page, or one of zeros
             // products of queries and keys; rows of parts are put together
             float S[2][MT][4];
 #pragma unroll
@@ -480,7 +519,8 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
 #pragma unroll
                     for (int r = 0; r < NR; ++r) {
                         const int row = min(segment.m0 + mt * (kSplit ? 8 : 16) + r * 8 + r8, segment.m_end - 1) / B.group;
-                        const Span k = span_of(segment.s, row, row, a.causal, a.window);
+                        Span k = span_of(segment.s, row, row, a.causal, a.window);
+                        if (kChosen && !(rows_here >> (row - segment.first_row) & 1)) k.hi = 0;
 #pragma unroll
                         for (int nb = 0; nb < 2; ++nb)
 #pragma unroll
@@ -618,7 +658,7 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
             if (n < count) issue(n, (n ^ i) >> 5 ? p1 : p0);
         }
         __syncthreads();                          // every warp is through with its ring: the parts take its place
-        if (gave_up && !a.cluster) {
+        if (!kChosen && gave_up && !a.cluster) {
             // the segments that the rest of the range begins get their notes all the same: the join follows whatever stands there
             if (tid == 0 && a.by_segment)
                 while (next_segment<kRows>(a, walk, segment)) {}
@@ -672,7 +712,7 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
                 sum += q[DP + 1] * f;
                 v.x += o.x * f; v.y += o.y * f; v.z += o.z * f; v.w += o.w * f;
             }
-            if (a.cluster) {                      // where the first warp's were: no other thread reads them
+            if (kChosen || a.cluster) {           // where the first warp's were: no other thread reads them
                 *reinterpret_cast<float4*>(smem + (r * (DP + 4) + d) * 4) = v;
                 if (d == 0) block_sum[r] = make_float2(top, sum);
                 continue;
@@ -684,7 +724,7 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
             }
             store_row(a, segment.s.row0 + row / B.group, segment.h * B.group + row % B.group, d, v, top, sum);
         }
-        if (a.cluster) {
+        if (kChosen || a.cluster) {
             cluster_meet();
             if (!gave_up) cluster_join<DP>(a, segment, smem, block_sum, kRows);
             cluster_meet();                       // nobody reads this block's part any more
@@ -848,6 +888,39 @@ __global__ void __launch_bounds__(kManyWarps * 32) paged_join_many_kernel(AttnAr
     store_row(a, cut.row0 + row / B.group, cut.h * B.group + row % B.group, tid * 4, o, top, sum);
 }
 
+// The pages that some row of a tile has chosen, in order, with the rows that have: a warp to a segment, a lane to a row, whose choices rise.
+constexpr int kMergeWarps = 4;
+__global__ void __launch_bounds__(kMergeWarps * 32) merge_choices_kernel(AttnArgs a, int tile_rows, int segments) {
+    const Batch& B = a.b;
+    const int lane = threadIdx.x & 31, c = blockIdx.x * kMergeWarps + threadIdx.x / 32;
+    grid_dependency_trigger();
+    grid_dependency_wait();
+    if (c >= segments) return;
+    const int b = c / (a.by_segment * B.kv_heads), h = c / a.by_segment % B.kv_heads, m0 = c % a.by_segment * tile_rows;
+    const Sequence s = sequence(B, b);
+    const int m_end = min(s.n * B.group, m0 + tile_rows), first_row = m0 / B.group, rows = m0 < m_end ? (m_end - 1) / B.group - first_row + 1 : 0;
+    const int* const mine = a.chosen + (s.row0 + first_row + min(lane, max(rows - 1, 0))) * a.chosen_row + h * a.chosen_head;
+    constexpr int kNone = 0x7fffffff;
+    const auto at = [&](int i) {
+        const int v = lane < rows && i < a.count ? __ldg(mine + i) : -1;
+        return v < 0 ? kNone : v;
+    };
+    int head = at(0), next = at(1), i = 1, n = 0;
+    int2* const list = a.lists + (long long)c * a.list_stride;
+    for (;;) {
+        const int least = __reduce_min_sync(~0u, head);
+        if (least == kNone || n >= a.list_stride) break;
+        const unsigned who = __ballot_sync(~0u, head == least);
+        if (lane == 0) list[n] = make_int2(least, int(who));
+        ++n;
+        if (who >> lane & 1) {
+            head = next;
+            next = at(++i);
+        }
+    }
+    if (lane == 0) a.list_len[c] = n;
+}
+
 // ---- host
 struct Choice { int dp, mt; bool split; };
 
@@ -889,14 +962,18 @@ long long row_tiles_of(const OglePagedBatch* b, int rows) {
     if (limit && most > limit) most = limit;
     return (most + rows - 1) / rows;
 }
+long long row_tiles_of_all(const OglePagedBatch* b, int rows) {
+    const long long most = (long long)(b->max_rows < b->n_rows ? b->max_rows : b->n_rows) * (b->q_heads / b->kv_heads);
+    return (most + rows - 1) / rows;
+}
 // Raises the kernel's limit of shared memory, once for each device.
-template <int DP, int MT, bool kSplit>
+template <int DP, int MT, bool kSplit, bool kChosen = false>
 cudaError_t prepare() {
     static std::atomic<uint64_t> sized{0};
     int device = 0;
     cudaError_t e = cudaGetDevice(&device);
     if (e == cudaSuccess && !(sized.load(std::memory_order_relaxed) >> (device & 63) & 1)) {
-        e = cudaFuncSetAttribute(paged_attention_kernel<DP, MT, kSplit>, cudaFuncAttributeMaxDynamicSharedMemorySize, Form<DP, MT, kSplit>::kSmem);
+        e = cudaFuncSetAttribute(paged_attention_kernel<DP, MT, kSplit, kChosen>, cudaFuncAttributeMaxDynamicSharedMemorySize, Form<DP, MT, kSplit>::kSmem);
         if (e == cudaSuccess) sized.fetch_or(1ull << (device & 63), std::memory_order_relaxed);
     }
     return e;
@@ -918,7 +995,7 @@ int most_clusters(int size) {
         cfg.dynamicSmemBytes = Form<DP, MT, kSplit>::kSmem;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        if (prepare<DP, MT, kSplit>() != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, paged_attention_kernel<DP, MT, kSplit>, &cfg) != cudaSuccess) {
+        if (prepare<DP, MT, kSplit>() != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, paged_attention_kernel<DP, MT, kSplit, false>, &cfg) != cudaSuccess) {
             (void)cudaGetLastError();
             return 0;
         }
@@ -986,6 +1063,34 @@ size_t few_workspace(const OglePagedBatch* b, const OgleAttentionParams* p) {
         if (cluster_of<decltype(dp)::value, decltype(mt)::value, decltype(split)::value>(b, p)) return sizeof(Cut);
         return size_t(ranges_of(b, F::kRows, F::kBlocks)) * (2 * F::kPart * sizeof(float) + sizeof(Cut));
     });
+}
+
+// Rows that a tile can have a part of.
+int rows_in_tile(const OglePagedBatch* b, int tile_rows) {
+    const int group = b->q_heads / b->kv_heads;
+    return (tile_rows + group - 2) / group + 1;
+}
+// Attention over chosen pages: segments, and what is kept of the tiles' lists where several rows share a tile.
+struct ChosenShape { long long segments; int tiles, list_stride; size_t lists; };
+ChosenShape chosen_shape(const OglePagedBatch* b, int tile_rows, int count) {
+    ChosenShape c;
+    c.tiles = int(row_tiles_of_all(b, tile_rows));
+    c.segments = (long long)c.tiles * b->n_seqs * b->kv_heads;
+    const int rows = b->max_rows < b->n_rows ? b->max_rows : b->n_rows, in_tile = rows_in_tile(b, tile_rows);
+    c.list_stride = (in_tile < rows ? in_tile : rows) * count;
+    c.lists = rows > 1 ? size_t(c.segments) * (c.list_stride * sizeof(int2) + sizeof(int)) : 0;
+    return c;
+}
+// Blocks to a segment. What is longest is the number of rounds of blocks, each as long as its share of the segment's tiles of 64 keys and
+// what a segment's beginning, end and join are worth.
+int chosen_cluster(const ChosenShape& c, long long tiles, int slots) {
+    int best = 1;
+    double least = 0;
+    for (int size = 1; size <= 8; ++size) {
+        const double rounds = double((c.segments * size + slots - 1) / slots), cost = rounds * (double((tiles + size - 1) / size) + kSegmentCost + (size > 1 ? 2 : 0));
+        if (size == 1 || cost < least) { best = size; least = cost; }
+    }
+    return best;
 }
 
 }  // namespace
@@ -1068,7 +1173,7 @@ int ogle_cuda_paged_attention(const OglePagedBatch* batch, const OgleAttentionPa
         constexpr bool kSplit = decltype(split)::value;
         using F = Form<DP, MT, kSplit>;
         const int ranges = ranges_of(batch, F::kRows, F::kBlocks);
-        auto kernel = paged_attention_kernel<DP, MT, kSplit>;
+        auto kernel = paged_attention_kernel<DP, MT, kSplit, false>;
         const long long max_tiles = row_tiles_of(batch, F::kRows), segments = max_tiles * a.b.n_seqs * a.b.kv_heads;
         a.cluster = cluster_of<DP, MT, kSplit>(batch, p);
         a.by_segment = a.cluster || segments < ranges ? int(max_tiles) : 0;
@@ -1106,6 +1211,88 @@ int ogle_cuda_paged_attention(const OglePagedBatch* batch, const OgleAttentionPa
         // 40000 99 / 94, 144 of 30000 105 / 104, 288 of 16000 99 / 102; of 16 rows each, 40 of 60000 81 / 72, 80 of 30000 73 / 73
         const bool many = ranges > 8 * segments;
         return launch_join(a, DP, many, a.by_segment ? int(segments < 1 ? 1 : segments) : ranges, ranges, F::kRows, tile, stream);
+    });
+}
+
+size_t ogle_cuda_sparse_attention_workspace_bytes(const OglePagedBatch* batch, const OgleAttentionParams* p, const OgleChosenPages* c) {
+    Batch b;
+    if (!p || !c || c->count < 1 || paged::translate(batch, b) != OGLE_OK || b.n_seqs == 0 || b.max_rows == 0) return 0;
+    return with_form(choose(batch), [&](auto dp, auto mt, auto split) {
+        using F = Form<decltype(dp)::value, decltype(mt)::value, decltype(split)::value>;
+        return chosen_shape(batch, F::kRows, c->count).lists;
+    });
+}
+
+int ogle_cuda_sparse_attention(const OglePagedBatch* batch, const OgleAttentionParams* p, const OgleChosenPages* c, void* workspace,
+                               size_t workspace_bytes, ogle_stream_t stream) {
+    AttnArgs a = {};
+    int rc = paged::translate(batch, a.b);
+    if (rc != OGLE_OK) return rc;
+    if (!p || !c || p->causal != 1 || p->window != 0 || c->count < 1) return OGLE_ERR_INVALID;
+    if (a.b.n_seqs == 0) return OGLE_OK;
+    if (!p->q || !p->out || !c->chosen || c->chosen_row < c->count || c->chosen_head < c->count) return OGLE_ERR_INVALID;
+    if (!paged::strides_ok(p->q, p->q_row, p->q_head, batch->dtype) || !paged::strides_ok(p->out, p->out_row, p->out_head, batch->dtype) || !aligned16(workspace))
+        return OGLE_ERR_ALIGNMENT;
+    // a tile's keys are counted in 32 bits
+    if ((long long)c->count * batch->page_tokens * 33 >= (1LL << 31)) return OGLE_ERR_UNSUPPORTED;
+    if (a.b.max_rows == 0) return OGLE_OK;
+    const size_t needed = ogle_cuda_sparse_attention_workspace_bytes(batch, p, c);
+    if (needed > 0 && (!workspace || workspace_bytes < needed)) return OGLE_ERR_INVALID;
+    a.q = p->q; a.out = p->out; a.lse = p->lse;
+    a.q_row = p->q_row; a.q_head = p->q_head; a.out_row = p->out_row; a.out_head = p->out_head;
+    a.scale_log2 = p->scale * 1.4426950408889634f;
+    a.causal = 1;
+    a.spin_limit = tc::role_wait_limit();
+    a.error = error_flag_ptr();
+    if (!a.error) return OGLE_ERR_CUDA;
+    a.chosen = c->chosen; a.chosen_row = c->chosen_row; a.chosen_head = c->chosen_head; a.count = c->count;
+    return with_form(choose(batch), [&](auto dp, auto mt, auto split) -> int {
+        constexpr int DP = decltype(dp)::value, MT = decltype(mt)::value;
+        constexpr bool kSplit = decltype(split)::value;
+        using F = Form<DP, MT, kSplit>;
+        const ChosenShape shape = chosen_shape(batch, F::kRows, c->count);
+        const long long pages = ((long long)a.b.max_kv_len + batch->page_tokens - 1) / batch->page_tokens;
+        const long long tiles = ((c->count < pages ? c->count : pages) * batch->page_tokens + kTileKeys - 1) / kTileKeys;
+        a.by_segment = shape.tiles;
+        a.cluster = chosen_cluster(shape, tiles, kNumSMs * F::kBlocks);
+        if (shape.segments * a.cluster >= (1LL << 31)) return OGLE_ERR_UNSUPPORTED;
+        cudaError_t e = prepare<DP, MT, kSplit, true>();
+        CUtensorMap k_map, v_map;
+        if (e == cudaSuccess && (!cache_map(&k_map, a.b, a.b.k_cache, DP) || !cache_map(&v_map, a.b, a.b.v_cache, DP))) {
+            set_last_error("sparse_attention: no tensor map of the cache");
+            return OGLE_ERR_CUDA;
+        }
+        if (e == cudaSuccess && shape.lists) {
+            a.list_stride = shape.list_stride;
+            a.lists = static_cast<int2*>(workspace);
+            a.list_len = reinterpret_cast<int*>(a.lists + size_t(shape.segments) * shape.list_stride);
+            e = launch_overlapped(merge_choices_kernel, dim3(unsigned((shape.segments + kMergeWarps - 1) / kMergeWarps)), dim3(kMergeWarps * 32), 0, stream, a,
+                                  F::kRows, int(shape.segments));
+            if (e == cudaSuccess) {
+                const int done = finish_launch();
+                if (done != OGLE_OK) return done;
+            }
+        }
+        if (e == cudaSuccess) {
+            cudaLaunchAttribute attr[2];
+            attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            // behind the lists' launch it is this call's own affair
+            attr[0].val.programmaticStreamSerializationAllowed = overlapped_launches_enabled(shape.lists > 0) ? 1 : 0;
+            attr[1].id = cudaLaunchAttributeClusterDimension;
+            attr[1].val.clusterDim.x = a.cluster;
+            attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(unsigned(shape.segments * a.cluster));
+            cfg.blockDim = dim3(kWarps * 32);
+            cfg.dynamicSmemBytes = F::kSmem;
+            cfg.stream = stream;
+            cfg.attrs = attr;
+            cfg.numAttrs = 2;
+            auto kernel = paged_attention_kernel<DP, MT, kSplit, true>;
+            e = cudaLaunchKernelEx(&cfg, kernel, a, k_map, v_map);
+        }
+        if (e != cudaSuccess) { set_last_error(e); (void)cudaGetLastError(); return OGLE_ERR_CUDA; }
+        return finish_launch();
     });
 }
 

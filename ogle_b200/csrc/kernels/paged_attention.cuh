@@ -27,6 +27,13 @@ struct AttnArgs {
     int cluster;                                 // blocks of a cluster that has one segment, or 0: ranges
     uint32_t spin_limit;
     int* error;
+    // attention over chosen pages: the blocks of a row's choice, or, where a tile can have several rows, of the tile's - a block and the
+    // rows of the tile that have chosen it, lists of list_stride entries, list_len of them in use
+    const int* chosen;
+    long long chosen_row, chosen_head;
+    int count, list_stride;
+    int2* lists;
+    int* list_len;
 };
 
 // What the join needs of a segment that was cut. rows 0: it was not. Kept by segment where there are fewer segments than

@@ -1,0 +1,491 @@
+// Which pages of the cache a query attends: bounds of the pages' keys, a score of every page for every query, the best of them.
+//
+// A page's bounds are the least and the largest key in every element, as whole numbers below 128 times a power of two of the page. A
+// query is whole numbers below 128 as well (and a power of two that all pages share), so the largest product that any key within the bounds
+// could have with it is a sum of products of whole numbers below 2^24: it does not depend on how it is summed, and two
+// implementations of the score agree in every bit. The sum is a product of 8-bit matrices - the query's positive elements with the upper
+// bounds, its negative ones with the lower - for which the cache's layout is the multiply's: a page is a column.
+//
+// Bound by what is launched and looked up where texts are ordinary (64 texts of up to 8000 tokens: 14 MB), by the bounds' bytes else.
+#include "paged.cuh"
+
+namespace ogle {
+namespace {
+
+using paged::Batch;
+
+// ---- bounds
+struct BoundsArgs {
+    Batch b;
+    signed char* bounds;
+    float* scale;
+    int per_seq;                                 // pages that a sequence can have appended to
+};
+
+// The smallest power of two t with amax <= 127 t, from the bits (1 for 0).
+__device__ __forceinline__ float unit_for(float amax) {
+    const uint32_t u = __float_as_uint(amax);
+    const int e = int(u >> 23) - 126 - 7 + ((u & 0x7fffffu) > 0x7e0000u ? 1 : 0);      // amax = f 2^(e + 7), f in [0.5, 1); 127 = 0.9921875 * 2^7
+    return amax > 0.f ? __uint_as_float(uint32_t(max(e, -120) + 127) << 23) : 1.f;
+}
+
+constexpr int kBoundThreads = 128;
+
+// A block has one page and head: a thread 16 elements of every so-many-th key.
+__global__ void __launch_bounds__(kBoundThreads) page_bounds_kernel(BoundsArgs a) {
+    __shared__ __half2 lowest[kBoundThreads * 8], highest[kBoundThreads * 8];
+    __shared__ float tops[kBoundThreads / 32];
+    const Batch& B = a.b;
+    const int tid = threadIdx.x, h = blockIdx.y, b = blockIdx.x / a.per_seq, nth = blockIdx.x % a.per_seq;
+    grid_dependency_trigger();
+    grid_dependency_wait();
+    const paged::Sequence s = paged::sequence(B, b);
+    const int begin = max(s.first, 0), end = min(s.first + s.n, s.len), block = (begin >> B.page_shift) + nth;
+    if (end <= begin || block > (end - 1) >> B.page_shift) return;
+    const int page = paged::page_of(B, b, block);
+    if (page < 0) return;
+    const int tokens = min(s.len - (block << B.page_shift), 1 << B.page_shift), cols = B.dim / 16, lanes = kBoundThreads / cols;
+    const int col = tid % cols, first = tid / cols;
+    const unsigned char* const keys = B.k_cache + page * B.page_stride + h * B.head_stride + col * 16;
+    const float inf = INFINITY;
+    __half2 lo[8], hi[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        lo[i] = __float2half2_rn(inf);
+        hi[i] = __float2half2_rn(-inf);
+    }
+    if (first < lanes) {
+#pragma unroll 4
+        for (int t = first; t < tokens; t += lanes) {
+            const uint4 v = *reinterpret_cast<const uint4*>(keys + t * B.token_stride);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t x, y;
+                paged::e4m3x4_to_half2(w[i], x, y);
+                const __half2 p = *reinterpret_cast<const __half2*>(&x), q = *reinterpret_cast<const __half2*>(&y);
+                lo[2 * i] = __hmin2(lo[2 * i], p);         // (of a number and a NaN, the number)
+                hi[2 * i] = __hmax2(hi[2 * i], p);
+                lo[2 * i + 1] = __hmin2(lo[2 * i + 1], q);
+                hi[2 * i + 1] = __hmax2(hi[2 * i + 1], q);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            lowest[first * (cols * 8) + col * 8 + i] = lo[i];
+            highest[first * (cols * 8) + col * 8 + i] = hi[i];
+        }
+    }
+    __syncthreads();
+    // pair `tid` of the elements
+    const int pairs = B.dim / 2;
+    float l[2] = {0.f, 0.f}, u[2] = {0.f, 0.f}, top = 0.f;
+    if (tid < pairs) {
+        __half2 least = lowest[tid], most = highest[tid];
+        for (int i = 1; i < lanes; ++i) {
+            least = __hmin2(least, lowest[i * pairs + tid]);
+            most = __hmax2(most, highest[i * pairs + tid]);
+        }
+        const float2 f = __half22float2(least), g = __half22float2(most);
+        if (f.x <= g.x) { l[0] = f.x; u[0] = g.x; }        // else: nothing but NaN
+        if (f.y <= g.y) { l[1] = f.y; u[1] = g.y; }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) top = fmaxf(top, fmaxf(fabsf(l[i]), fabsf(u[i])));
+    }
+#pragma unroll
+    for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+    if ((tid & 31) == 0) tops[tid / 32] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kBoundThreads / 32; ++w) top = fmaxf(top, tops[w]);
+    const float unit = unit_for(top), by = 1.f / unit;
+    const long long at = (long long)page * B.kv_heads + h;
+    if (tid < pairs) {
+        signed char* const out = a.bounds + at * 2 * B.dim + tid * 2;
+        *reinterpret_cast<char2*>(out) = make_char2((signed char)floorf(l[0] * by), (signed char)floorf(l[1] * by));
+        *reinterpret_cast<char2*>(out + B.dim) = make_char2((signed char)ceilf(u[0] * by), (signed char)ceilf(u[1] * by));
+    }
+    if (tid == 0) a.scale[at] = unit * B.k_scale[at];
+}
+
+// ---- scores
+struct ChooseArgs {
+    Batch b;
+    const void* q;
+    long long q_row, q_head;
+    const signed char* bounds;
+    const float* scale;
+    int* chosen;
+    long long chosen_row, chosen_head;
+    int count, first, last;
+    unsigned* keys;                              // [rows][kv heads][stride]
+    long long stride;
+    int row0, rows;                              // rows of this launch
+    int tiles, chunks;                           // tiles of rows that a sequence can have; chunks of pages
+};
+
+constexpr int kScoreWarps = 4;
+constexpr int kStepPages = 8;
+constexpr int kChunkPages = kScoreWarps * kStepPages * 8;        // of a block
+constexpr unsigned kAlways = ~0u;
+
+__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// A page's score as a number that orders the same way: 0 for what is not chosen, 1 for what has no size.
+__device__ __forceinline__ unsigned ordered_score(float x) {
+    x += 0.f;
+    if (x != x) return 1u;
+    const uint32_t u = __float_as_uint(x);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// Rows of a tile: as many as have their query heads of a group in the 16 rows of a multiply, at least one.
+__device__ __forceinline__ int rows_of_tile(int group) { return group >= 16 ? 1 : 16 / group; }
+
+// A block has a tile of rows of one sequence, one kv head and a chunk of pages. The queries lie in shared memory as the multiply takes
+// them: of 64 bytes of a head's elements, lane c4 of four has bytes [16 c4, 16 c4 + 16) - the order in which pages are read -, the
+// lower bounds' first, then the upper bounds'.
+__global__ void __launch_bounds__(kScoreWarps * 32) choose_score_kernel(ChooseArgs a) {
+    extern __shared__ __align__(16) unsigned char queries[];
+    __shared__ int tile_score[kScoreWarps][16][kStepPages + 1];
+    __shared__ float tops[kScoreWarps], step_unit[kScoreWarps][kStepPages];
+    __shared__ int step_page[kScoreWarps][kStepPages];
+    const Batch& B = a.b;
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, c4 = lane & 3, r8 = lane >> 2;
+    grid_dependency_trigger();
+    grid_dependency_wait();
+    const int chunk = blockIdx.x % a.chunks, rest = blockIdx.x / a.chunks, h = rest % B.kv_heads, tile = rest / B.kv_heads % a.tiles, b = rest / B.kv_heads / a.tiles;
+    const paged::Sequence s = paged::sequence(B, b);
+    const int per = rows_of_tile(B.group);
+    // rows of the tile that belong to this launch
+    const int r0 = max(tile * per, a.row0 - s.row0), r1 = min(min(tile * per + per, s.n), a.row0 + a.rows - s.row0);
+    if (r0 >= r1) return;
+    const int last_place = s.first + r1 - 1;
+    const int blocks = min(last_place, s.len - 1) >= 0 ? (min(last_place, s.len - 1) >> B.page_shift) + 1 : 0;
+    const int first_page = chunk * kChunkPages, end_page = min(first_page + kChunkPages, blocks);
+    if (first_page >= blocks) return;
+    const int n_rows = r1 - r0, heads = n_rows * B.group, m_tiles = (heads + 15) / 16;
+    const int words = (B.dim + 63) / 64;         // of 64 elements
+
+    // the queries' whole numbers: a row's heads share a unit
+    for (int r = 0; r < n_rows; ++r) {
+        const long long q0 = (long long)(s.row0 + r0 + r) * a.q_row + (long long)h * B.group * a.q_head;
+        float top = 0.f;
+        for (int i = tid; i < B.group * B.dim; i += kScoreWarps * 32) {
+            const float x = fabsf(paged::to_float(a.q, q0 + i / B.dim * a.q_head + i % B.dim, B.dtype));
+            if (x <= 3.402823466e38f) top = fmaxf(top, x);
+        }
+#pragma unroll
+        for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+        __syncthreads();
+        if (lane == 0) tops[warp] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kScoreWarps; ++w) top = fmaxf(top, tops[w]);
+        const float by = 1.f / unit_for(top);
+        for (int i = tid; i < B.group * words * 64; i += kScoreWarps * 32) {
+            const int g = i / (words * 64), d = i % (words * 64);
+            int x = 0;
+            if (d < B.dim) {
+                float f = paged::to_float(a.q, q0 + g * a.q_head + d, B.dtype);
+                if (!(fabsf(f) <= 3.402823466e38f)) f = 0.f;
+                x = min(max(__float2int_rn(f * by), -127), 127);
+            }
+            // element d: word d / 64 of lane (d % 64) / 16; its 16 bytes are two steps' operands, 8 bytes each
+            const int m = r * B.group + g, mt = m / 16, row = m % 16, w = d / 64, c = d % 64 / 16, byte = d % 16;
+            // (a lane's words of a step: row r8 bytes 0-3, row r8 + 8 the same, row r8 bytes 4-7, row r8 + 8 the same)
+            const int at = ((mt * 2 * words + w) * 2 + byte / 8) * 512 + ((row & 7) * 4 + c) * 16 + (byte % 8 / 4) * 8 + (row / 8) * 4 + byte % 4;
+            queries[at] = (unsigned char)(signed char)min(x, 0);
+            queries[at + words * 2 * 512] = (unsigned char)(signed char)max(x, 0);
+        }
+    }
+    // rows of the last multiply that are not there
+    for (int i = tid + heads; i < m_tiles * 16; i += kScoreWarps * 32) {
+        const int mt = i / 16, row = i % 16;
+        for (int w = 0; w < 2 * words * 2; ++w)
+            for (int c = 0; c < 4; ++c) {
+                unsigned* const p = reinterpret_cast<unsigned*>(queries + (mt * 2 * words * 2 + w) * 512 + ((row & 7) * 4 + c) * 16 + (row / 8) * 4);
+                p[0] = 0;
+                p[2] = 0;
+            }
+    }
+    __syncthreads();
+
+    const int bytes = 2 * B.dim;
+    for (int p0 = first_page + warp * kStepPages; p0 < end_page; p0 += kScoreWarps * kStepPages) {
+        const int block = p0 + r8;               // this lane's page: a column of the multiply
+        const int page = block < end_page ? paged::page_of(B, b, block) : -1;
+        const signed char* const mine = a.bounds + ((long long)max(page, 0) * B.kv_heads + h) * bytes;
+        const float unit = page >= 0 ? __ldg(a.scale + (long long)page * B.kv_heads + h) : 0.f;
+        if (c4 == 0) { step_page[warp][r8] = page; step_unit[warp][r8] = unit; }
+        uint4 v[8];                              // words of the lower, then of the upper bounds
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+            for (int side = 0; side < 2; ++side) {
+                const int d = w * 64 + c4 * 16;
+                v[2 * w + side] = w < words && d < B.dim && page >= 0 ? __ldg(reinterpret_cast<const uint4*>(mine + side * B.dim + d)) : make_uint4(0, 0, 0, 0);
+            }
+        for (int mt = 0; mt < m_tiles; ++mt) {
+            int c[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+                if (w < words)
+#pragma unroll
+                    for (int side = 0; side < 2; ++side) {
+                        const uint4* const q = reinterpret_cast<const uint4*>(queries) + ((mt * 2 + side) * words + w) * 2 * 32 + lane;
+                        const uint4 x = q[0], y = q[32], z = v[2 * w + side];
+                        mma_s8(c, x.x, x.y, x.z, x.w, z.x, z.y);
+                        mma_s8(c, y.x, y.y, y.z, y.w, z.z, z.w);
+                    }
+            tile_score[warp][r8][c4 * 2] = c[0];
+            tile_score[warp][r8][c4 * 2 + 1] = c[1];
+            tile_score[warp][r8 + 8][c4 * 2] = c[2];
+            tile_score[warp][r8 + 8][c4 * 2 + 1] = c[3];
+            __syncwarp();
+            // the best of a row's heads: of a whole row, or of 16 of its heads more
+            for (int i = lane; i < n_rows * kStepPages; i += 32) {
+                const int r = i / kStepPages, n = i % kStepPages;
+                const int from = B.group <= 16 ? r * B.group : 0, to = B.group <= 16 ? from + B.group : min(16, B.group - mt * 16);
+                int best = tile_score[warp][from][n];
+                for (int g = from + 1; g < to; ++g) best = max(best, tile_score[warp][g][n]);
+                const int place = s.first + r0 + r, blk = p0 + n;
+                const int own = min(place, s.len - 1) >> B.page_shift;
+                if (blk >= end_page) continue;
+                unsigned key = 0;
+                if (step_page[warp][n] >= 0 && place >= 0 && blk <= own)
+                    key = blk < a.first || blk > own - a.last ? kAlways : ordered_score(float(best) * step_unit[warp][n]);
+                unsigned* const to_key = a.keys + ((long long)(s.row0 + r0 + r - a.row0) * B.kv_heads + h) * a.stride + blk;
+                *to_key = mt > 0 ? max(*to_key, key) : key;
+            }
+            __syncwarp();
+        }
+    }
+}
+
+// ---- the best
+constexpr int kPickThreads = 256, kBins = 2048;
+constexpr int kHeld = 8192;                      // keys that a block holds in shared memory
+
+// A block has one row and kv head. Few pages: each key's rank. Else the count-th largest key by its digits, 11, 11 and 10 bits; then each
+// thread has a piece of the pages, so that what is chosen comes out in order.
+__global__ void __launch_bounds__(kPickThreads) choose_pick_kernel(ChooseArgs a) {
+    extern __shared__ __align__(16) unsigned held[];
+    __shared__ int bins[kBins];
+    __shared__ int sums[2][kPickThreads / 32];
+    __shared__ unsigned digit;
+    __shared__ int above;
+    const Batch& B = a.b;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid / 32;
+    grid_dependency_trigger();
+    grid_dependency_wait();
+    const int h = blockIdx.x % B.kv_heads, rest = blockIdx.x / B.kv_heads, r = rest % B.max_rows, b = rest / B.max_rows;
+    const paged::Sequence s = paged::sequence(B, b);
+    const int row = s.row0 + r;
+    if (r >= s.n || row < a.row0 || row >= a.row0 + a.rows) return;
+    int* const out = a.chosen + row * a.chosen_row + h * a.chosen_head;
+    const int place = s.first + r, top = min(place, s.len - 1), n = top >= 0 ? (top >> B.page_shift) + 1 : 0;
+    const unsigned* const keys = a.keys + ((long long)(row - a.row0) * B.kv_heads + h) * a.stride;
+    const bool holds = n <= kHeld;
+    if (holds) {
+        for (int i = tid; i < n; i += kPickThreads) held[i] = keys[i];
+        if (tid < 4 && n + tid < (n + 3) / 4 * 4) held[n + tid] = 0;
+        __syncthreads();
+    }
+    const auto key = [&](int i) { return holds ? held[i] : keys[i]; };
+    unsigned border = 0;                         // what is above it is chosen, and `equal` of those that are the border
+    int equal = 0, per = (n + kPickThreads - 1) / kPickThreads;
+    if (n <= kPickThreads) {
+        const unsigned mine = tid < n ? held[tid] : 0u;
+        int rank = 0;
+        for (int j = 0; j < n; j += 4) {
+            const uint4 k = *reinterpret_cast<const uint4*>(held + j);
+            rank += (k.x > mine || k.x == mine && j < tid) + (k.y > mine || k.y == mine && j + 1 < tid) +
+                    (k.z > mine || k.z == mine && j + 2 < tid) + (k.w > mine || k.w == mine && j + 3 < tid);
+        }
+        const unsigned who = __ballot_sync(~0u, mine && rank < a.count);
+        if (lane == 0) sums[0][warp] = __popc(who);
+        __syncthreads();
+        int at = __popc(who & ((1u << lane) - 1)), all = 0;
+#pragma unroll
+        for (int w = 0; w < kPickThreads / 32; ++w) {
+            if (w < warp) at += sums[0][w];
+            all += sums[0][w];
+        }
+        if (who >> lane & 1) out[at] = tid;
+        for (int i = all + tid; i < a.count; i += kPickThreads) out[i] = -1;
+        return;
+    }
+    int need = a.count;
+    unsigned known = 0;                          // the border's upper digits, and which bits these are
+    unsigned mask = 0;
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), size = pass == 2 ? 1024 : 2048;
+        for (int i = tid; i < kBins; i += kPickThreads) bins[i] = 0;
+        if (tid == 0) { digit = 0; above = 0; }
+        __syncthreads();
+        for (int i = tid; i < n; i += kPickThreads) {
+            const unsigned k = key(i);
+            if ((k & mask) == known) atomicAdd(bins + (k >> shift & (size - 1)), 1);
+        }
+        __syncthreads();
+        // from the largest digit down: thread t has bins [size - 8 (t + 1), size - 8 t)
+        const int from = size - 8 * (tid + 1);
+        int mine = 0;
+        if (from >= 0)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) mine += bins[from + i];
+        int sum = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const int o = __shfl_up_sync(~0u, sum, d);
+            if (lane >= d) sum += o;
+        }
+        if (lane == 31) sums[0][warp] = sum;
+        __syncthreads();
+        for (int w = 0; w < warp; ++w) sum += sums[0][w];
+        if (sum >= need && sum - mine < need) {  // one thread, where there are as many keys
+            int before = sum - mine;
+            for (int i = 7; i >= 0; --i) {
+                if (before + bins[from + i] >= need) { digit = unsigned(from + i); above = before; break; }
+                before += bins[from + i];
+            }
+        }
+        __syncthreads();
+        need -= above;
+        known |= digit << shift;
+        mask |= unsigned(size - 1) << shift;
+        __syncthreads();
+    }
+    border = known;
+    equal = border ? need : 0;
+    // pieces of an odd number of keys: a warp's threads read from different banks
+    per |= 1;
+    const int i0 = min(tid * per, n), i1 = min(i0 + per, n);
+    int more = 0, same = 0;
+    for (int i = i0; i < i1; ++i) {
+        const unsigned k = key(i);
+        more += k > border;
+        same += k == border;
+    }
+    int m = more, e = same;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const int o = __shfl_up_sync(~0u, m, d), q = __shfl_up_sync(~0u, e, d);
+        if (lane >= d) { m += o; e += q; }
+    }
+    if (lane == 31) { sums[0][warp] = m; sums[1][warp] = e; }
+    __syncthreads();
+    int all_more = 0, all_same = 0;
+#pragma unroll
+    for (int w = 0; w < kPickThreads / 32; ++w) {
+        if (w < warp) { m += sums[0][w]; e += sums[1][w]; }
+        all_more += sums[0][w];
+        all_same += sums[1][w];
+    }
+    int before_more = m - more, before_same = e - same;
+    for (int i = i0; i < i1; ++i) {
+        const unsigned k = key(i);
+        if (k > border || k == border && before_same < equal) out[before_more + min(before_same, equal)] = i;
+        before_more += k > border;
+        before_same += k == border;
+    }
+    for (int i = all_more + min(all_same, equal) + tid; i < a.count; i += kPickThreads) out[i] = -1;
+}
+
+constexpr long long kMostKeys = 64ll << 20;      // of a launch: 256 MB
+
+long long key_stride(const Batch& b) { return b.max_kv_len > 0 ? ((b.max_kv_len - 1) >> b.page_shift) + 1 : 1; }
+long long rows_at_once(const Batch& b) {
+    const long long n = kMostKeys / (key_stride(b) * b.kv_heads);
+    return n < 1 ? 1 : (n < b.n_rows ? n : b.n_rows);
+}
+int failed(cudaError_t e) {
+    set_last_error(e);
+    (void)cudaGetLastError();
+    return OGLE_ERR_CUDA;
+}
+
+}  // namespace
+}  // namespace ogle
+
+using namespace ogle;
+
+extern "C" {
+
+int ogle_cuda_page_bounds(const OglePagedBatch* batch, signed char* bounds, float* bounds_scale, ogle_stream_t stream) {
+    BoundsArgs a = {};
+    const int rc = paged::translate(batch, a.b);
+    if (rc != OGLE_OK) return rc;
+    if (a.b.n_seqs == 0) return OGLE_OK;
+    if (!bounds || !bounds_scale) return OGLE_ERR_INVALID;
+    if (!aligned16(bounds)) return OGLE_ERR_ALIGNMENT;
+    if (a.b.max_rows == 0 || a.b.max_kv_len == 0) return OGLE_OK;
+    a.bounds = bounds;
+    a.scale = bounds_scale;
+    const long long rows = a.b.max_rows < a.b.n_rows ? a.b.max_rows : a.b.n_rows;
+    a.per_seq = rows == 1 ? 1 : int((rows + (1 << a.b.page_shift) - 2) >> a.b.page_shift) + 1;
+    if ((long long)a.per_seq * a.b.n_seqs >= (1LL << 31)) return OGLE_ERR_UNSUPPORTED;
+    const cudaError_t e = launch_overlapped(page_bounds_kernel, dim3(a.per_seq * a.b.n_seqs, a.b.kv_heads), dim3(kBoundThreads), 0, stream, a);
+    return e == cudaSuccess ? finish_launch() : failed(e);
+}
+
+size_t ogle_cuda_choose_pages_workspace_bytes(const OglePagedBatch* batch, const OgleChooseParams* p) {
+    Batch b;
+    if (!p || paged::translate(batch, b) != OGLE_OK || b.n_seqs == 0 || b.max_rows == 0 || b.max_kv_len == 0) return 0;
+    return size_t(rows_at_once(b) * b.kv_heads * key_stride(b)) * sizeof(unsigned);
+}
+
+int ogle_cuda_choose_pages(const OglePagedBatch* batch, const OgleChooseParams* p, void* workspace, size_t workspace_bytes, ogle_stream_t stream) {
+    ChooseArgs a = {};
+    const int rc = paged::translate(batch, a.b);
+    if (rc != OGLE_OK) return rc;
+    if (!p || p->count < 1 || p->first < 0 || p->last < 1 || p->first > p->count || p->last > p->count - p->first) return OGLE_ERR_INVALID;
+    Batch& B = a.b;
+    if (B.n_seqs == 0) return OGLE_OK;
+    if (!p->q || !p->bounds || !p->bounds_scale || !p->chosen) return OGLE_ERR_INVALID;
+    if (p->chosen_head < p->count || p->chosen_row < p->count) return OGLE_ERR_INVALID;
+    if (!paged::strides_ok(p->q, p->q_row, p->q_head, batch->dtype) || !aligned16(p->bounds)) return OGLE_ERR_ALIGNMENT;
+    if (B.group > 256) return OGLE_ERR_UNSUPPORTED;
+    if (B.max_rows == 0) return OGLE_OK;
+    // (with a bound of no tokens every choice is empty, and nothing is read or written there)
+    if (B.max_kv_len > 0 && (!workspace || workspace_bytes < ogle_cuda_choose_pages_workspace_bytes(batch, p))) return OGLE_ERR_INVALID;
+    if (reinterpret_cast<uintptr_t>(workspace) & 3) return OGLE_ERR_ALIGNMENT;
+    a.q = p->q; a.q_row = p->q_row; a.q_head = p->q_head;
+    a.bounds = p->bounds; a.scale = p->bounds_scale;
+    a.chosen = p->chosen; a.chosen_row = p->chosen_row; a.chosen_head = p->chosen_head;
+    a.count = p->count; a.first = p->first; a.last = p->last;
+    a.keys = static_cast<unsigned*>(workspace);
+    a.stride = key_stride(B);
+    if (B.max_rows > B.n_rows) B.max_rows = B.n_rows;
+    const int per = B.group >= 16 ? 1 : 16 / B.group;
+    a.tiles = div_up(B.max_rows, per);
+    a.chunks = div_up(a.stride, kChunkPages);
+    const long long blocks = (long long)B.n_seqs * a.tiles * B.kv_heads * a.chunks, picks = (long long)B.n_seqs * B.max_rows * B.kv_heads;
+    if (blocks >= (1LL << 31) || picks >= (1LL << 31)) return OGLE_ERR_UNSUPPORTED;
+    const size_t queries = size_t(div_up(per * B.group, 16)) * 2 * div_up(B.dim, 64) * 1024, held = size_t(a.stride < kHeld ? div_up(a.stride, 4) * 4 : kHeld) * 4;
+    if (queries > (48u << 10) - 4096) {
+        const cudaError_t e = cudaFuncSetAttribute(choose_score_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(queries));
+        if (e != cudaSuccess) return failed(e);
+    }
+    const long long at_once = rows_at_once(B);
+    for (long long row0 = 0; row0 < B.n_rows; row0 += at_once) {
+        a.row0 = int(row0);
+        a.rows = int(B.n_rows - row0 < at_once ? B.n_rows - row0 : at_once);
+        cudaError_t e = launch_overlapped(choose_score_kernel, dim3(unsigned(blocks)), dim3(kScoreWarps * 32), queries, stream, a);
+        if (e != cudaSuccess) return failed(e);
+        int done = finish_launch();
+        if (done != OGLE_OK) return done;
+        e = launch_overlapped_if(overlapped_launches_enabled(true), choose_pick_kernel, dim3(unsigned(picks)), dim3(kPickThreads), held, stream, a);
+        if (e != cudaSuccess) return failed(e);
+        done = finish_launch();
+        if (done != OGLE_OK) return done;
+    }
+    return OGLE_OK;
+}
+
+}  // extern "C"

@@ -24,6 +24,7 @@ _PAGED_BATCH, _APPEND = _lib.packer(_lib.PagedBatch).pack, _lib.packer(_lib.Appe
 _ATTENTION, _LOGITS = _lib.packer(_lib.AttentionParams).pack, _lib.packer(_lib.LogitsParams).pack
 _BEAM, _ADVANCE = _lib.packer(_lib.BeamParams).pack, _lib.packer(_lib.AdvanceParams).pack
 _COMPACT, _COPY_PAGES = _lib.packer(_lib.CompactParams).pack, _lib.packer(_lib.CopyPagesParams).pack
+_CHOOSE, _CHOSEN = _lib.packer(_lib.ChooseParams).pack, _lib.packer(_lib.ChosenPages).pack
 _PAGE_TENSORS = _lib.packer(_lib.PageTensors).pack
 _I32, _F32, _E4M3 = torch.int32, torch.float32, torch.float8_e4m3fn
 
@@ -292,3 +293,67 @@ def _bounds(bounds, pages, heads, dim):
     if lo_hi.shape != (pages, heads, 2, dim):
         raise ValueError(f"bounds: expected int8 [{pages}, {heads}, 2, {dim}]")
     return _vector(lo_hi, torch.int8, None, "bounds"), _vector(scale, _F32, pages * heads, "the bounds' scale")
+
+
+def new_bounds(cache):
+    """Room for the bounds of a cache's pages: (int8 [pages, kv heads, 2, head dim], float32 [pages, kv heads])."""
+    pages, heads, _, dim = cache[0].shape
+    return (torch.zeros(pages, heads, 2, dim, dtype=torch.int8, device=cache[0].device), torch.zeros(pages, heads, dtype=_F32, device=cache[0].device))
+
+
+def page_bounds(cache, bounds, block_table, kv_len, max_kv_len, row_start=None, max_rows=1):
+    """Bounds of the keys in every page that the batch's rows were appended to (ogle_cuda_page_bounds), in place: behind `append`, with its
+    batch. choose_pages needs them of all pages that a row may choose."""
+    pages, heads, _, dim = cache[0].shape
+    # any count of rows that row_start stays below will do, as any type
+    rows = block_table.shape[0] * (1 if row_start is None else max_rows)
+    b = _batch(cache, block_table, kv_len, max_kv_len, row_start, max_rows, rows, heads, torch.bfloat16)
+    check(_lib.cuda_lib().ogle_cuda_page_bounds(b, *_bounds(bounds, pages, heads, dim), _stream()), "page_bounds")
+
+
+def choose_pages(q, cache, bounds, block_table, kv_len, max_kv_len, row_start=None, max_rows=1, count=16, first=1, last=1):
+    """The `count` pages that each row of q [rows, heads, head dim] attends (ogle_cuda_choose_pages), for each kv head as blocks of the row's
+    sequence: the `first` ones, the row's own with the last - 1 before it, and of the others those whose keys, going by their bounds, can have
+    the largest product with one of the head's queries. Returns int32 [rows, kv heads, count], rising, filled up with -1."""
+    if q.dim() != 3:
+        raise ValueError("q: expected [rows, heads, head dim]")
+    pages, kv_heads, _, dim = cache[0].shape
+    rows, heads, _ = q.shape
+    b = _batch(cache, block_table, kv_len, max_kv_len, row_start, max_rows, rows, heads, q.dtype)
+    chosen = q.new_empty(rows, kv_heads, max(count, 0), dtype=_I32)
+    p = _CHOOSE(*_rows(q, q.dtype, rows, heads, dim, "q"), *_bounds(bounds, pages, kv_heads, dim), chosen.data_ptr(), kv_heads * count, count,
+                count, first, last, 0)
+    lib = _lib.cuda_lib()
+    n = lib.ogle_cuda_choose_pages_workspace_bytes(b, p)
+    workspace = q.new_empty(max(n, 16), dtype=torch.uint8)
+    check(lib.ogle_cuda_choose_pages(b, p, workspace.data_ptr(), n, _stream()), "choose_pages")
+    return chosen
+
+
+def sparse_attention(q, cache, chosen, block_table, kv_len, max_kv_len, row_start=None, max_rows=1, scale=None, out=None):
+    """Softmax attention of q [rows, heads, head dim] over the tokens, up to the row's own, of the pages that choose_pages has chosen for the
+    row and kv head (ogle_cuda_sparse_attention). chosen: int32 [rows, kv heads, count], rising, filled up with -1. Returns (out, lse) as
+    `attention` does."""
+    dtype = q.dtype
+    if q.dim() != 3:
+        raise ValueError("q: expected [rows, heads, head dim]")
+    rows, heads, dim = q.shape
+    kv_heads = cache[0].shape[1]
+    b = _batch(cache, block_table, kv_len, max_kv_len, row_start, max_rows, rows, heads, dtype)
+    pq = _rows(q, dtype, rows, heads, cache[0].shape[3], "q")
+    if chosen.dim() != 3 or chosen.dtype != _I32 or not chosen.is_cuda or chosen.shape[0] != rows or chosen.shape[1] != kv_heads or chosen.stride(2) != 1 and chosen.shape[2] > 1:
+        raise ValueError(f"chosen: expected an int32 CUDA tensor [{rows}, {kv_heads}, count], a choice's entries side by side")
+    if out is None:
+        out = q.new_empty(rows, heads, dim)
+        po = out.data_ptr(), heads * dim, dim
+    else:
+        po = _rows(out, dtype, rows, heads, dim, "out")
+    lse = q.new_empty(rows, heads, dtype=_F32)
+    p = _ATTENTION(pq[0], po[0], lse.data_ptr(), pq[1], pq[2], po[1], po[2], dim ** -0.5 if scale is None else scale, 1, 0, 0)
+    count = chosen.shape[2]
+    c = _CHOSEN(chosen.data_ptr(), chosen.stride(0) if rows > 1 else kv_heads * count, chosen.stride(1) if kv_heads > 1 else count, count, 0)
+    lib = _lib.cuda_lib()
+    n = lib.ogle_cuda_sparse_attention_workspace_bytes(b, p, c)
+    workspace = q.new_empty(n, dtype=torch.uint8) if n else None
+    check(lib.ogle_cuda_sparse_attention(b, p, c, workspace.data_ptr() if n else 0, n, _stream()), "sparse_attention")
+    return out, lse
