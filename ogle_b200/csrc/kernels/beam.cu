@@ -337,7 +337,7 @@ constexpr int kPickThreads = 512, kPickWarps = kPickThreads / 32, kPicked = 1024
 constexpr int kMostBeams = 1024;
 
 __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamArgs a) {
-    extern __shared__ double2 beam_terms[];                        // of each beam: m, and score - log sum exp(x - m)
+    extern __shared__ double2 beam_terms[];                        // of each beam: its largest logit m, and log sum exp(x - m)
     __shared__ Total found[kPicked];
     __shared__ Total best[kMostCount];
     __shared__ double warp_value[kPickWarps];
@@ -353,7 +353,10 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamArgs a) {
     for (int b = warp; b < p.beams; b += kPickWarps) {
         const unsigned char* const mine = parts + (size_t)b * a.ranges * stride;
         float top = -INFINITY;
-        for (int r = lane; r < a.ranges; r += 32) top = fmaxf(top, reinterpret_cast<const Part*>(mine + r * stride)->m);
+        for (int r = lane; r < a.ranges; r += 32) {
+            const Key k = *reinterpret_cast<const Key*>(mine + r * stride + sizeof(Part));
+            if (k) top = fmaxf(top, logit_of(k));
+        }
 #pragma unroll
         for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
         double sum = 0.;
@@ -363,10 +366,30 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamArgs a) {
         }
 #pragma unroll
         for (int d = 16; d; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
-        if (lane == 0) {
-            const double score = p.scores ? (double)p.scores[g * p.beams + b] : 0.;
-            beam_terms[b] = make_double2(top, sum > 0. ? score - log(sum) : 0.);       // no sum: no kept logit either
-        }
+        if (lane == 0) beam_terms[b] = make_double2(top, sum > 0. ? log(sum) : 0.);    // no sum: no kept logit either
+    }
+    __syncthreads();
+    // Two beams of the same logits differ in the last bits of their sums where their rows lie differently to 16 bytes. They count as the same,
+    // so that their totals are equal and come in the beams' order; so does what is as near by chance.
+    constexpr int kMine = (kMostBeams + kPickThreads - 1) / kPickThreads;
+    double minus[kMine];
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+        const int b = tid + i * kPickThreads;
+        if (b >= p.beams) break;
+        const double2 term = beam_terms[b];
+        minus[i] = term.y;
+        for (int o = 0; o < b; ++o)
+            if (beam_terms[o].x == term.x && fabs(beam_terms[o].y - term.y) <= 0x1p-22) {
+                minus[i] = beam_terms[o].y;
+                break;
+            }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+        const int b = tid + i * kPickThreads;
+        if (b < p.beams) beam_terms[b].y = (p.scores ? (double)p.scores[g * p.beams + b] : 0.) - minus[i];
     }
     __syncthreads();
     const int lists = p.beams * a.ranges, all = lists * p.count;

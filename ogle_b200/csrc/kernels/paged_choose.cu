@@ -22,12 +22,14 @@ struct BoundsArgs {
     int per_seq;                                 // pages that a sequence can have appended to
 };
 
-// The smallest power of two t with amax <= 127 t, from the bits (1 for 0).
-__device__ __forceinline__ float unit_for(float amax) {
-    const uint32_t u = __float_as_uint(amax);
-    const int e = int(u >> 23) - 126 - 7 + ((u & 0x7fffffu) > 0x7e0000u ? 1 : 0);      // amax = f 2^(e + 7), f in [0.5, 1); 127 = 0.9921875 * 2^7
-    return amax > 0.f ? __uint_as_float(uint32_t(max(e, -120) + 127) << 23) : 1.f;
+// The exponent of the smallest power of two t with amax <= 127 t, from the bits (0 for 0).
+__device__ __forceinline__ int unit_exponent(float amax) {
+    if (amax == 0.f) return 0;
+    const bool small = amax < 0x1p-100f;
+    const uint32_t u = __float_as_uint(small ? amax * 0x1p60f : amax);
+    return int(u >> 23) - 126 - 7 - (small ? 60 : 0) + ((u & 0x7fffffu) > 0x7e0000u ? 1 : 0);     // amax = f 2^(e + 7), f in [0.5, 1); 127 = 0.9921875 * 2^7
 }
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(uint32_t(e + 127) << 23); }
 
 constexpr int kBoundThreads = 128;
 
@@ -98,7 +100,8 @@ __global__ void __launch_bounds__(kBoundThreads) page_bounds_kernel(BoundsArgs a
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kBoundThreads / 32; ++w) top = fmaxf(top, tops[w]);
-    const float unit = unit_for(top), by = 1.f / unit;
+    const int exponent = unit_exponent(top);     // of e4m3 values: -15 to 2
+    const float unit = power_of_two(exponent), by = power_of_two(-exponent);
     const long long at = (long long)page * B.kv_heads + h;
     if (tid < pairs) {
         signed char* const out = a.bounds + at * 2 * B.dim + tid * 2;
@@ -185,14 +188,15 @@ __global__ void __launch_bounds__(kScoreWarps * 32) choose_score_kernel(ChooseAr
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < kScoreWarps; ++w) top = fmaxf(top, tops[w]);
-        const float by = 1.f / unit_for(top);
+        const int exponent = unit_exponent(top), half = -exponent / 2;
+        const float by = power_of_two(half), by_rest = power_of_two(-exponent - half);     // their product can be above the largest number
         for (int i = tid; i < B.group * words * 64; i += kScoreWarps * 32) {
             const int g = i / (words * 64), d = i % (words * 64);
             int x = 0;
             if (d < B.dim) {
                 float f = paged::to_float(a.q, q0 + g * a.q_head + d, B.dtype);
                 if (!(fabsf(f) <= 3.402823466e38f)) f = 0.f;
-                x = min(max(__float2int_rn(f * by), -127), 127);
+                x = min(max(__float2int_rn(f * by * by_rest), -127), 127);
             }
             // element d: word d / 64 of lane (d % 64) / 16; its 16 bytes are two steps' operands, 8 bytes each
             const int m = r * B.group + g, mt = m / 16, row = m % 16, w = d / 64, c = d % 64 / 16, byte = d % 16;
