@@ -13,6 +13,7 @@
 #include <cuda_fp16.h>
 
 #include "common.cuh"
+#include "pairs.cuh"
 
 namespace ogle {
 namespace {
@@ -21,9 +22,10 @@ constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kVecs = 4;                         // of 16 bytes, a thread's share of a batch
 constexpr int kMostCount = 128, kMostEnds = 1024;
 constexpr int kKept = 1024;                      // logits that a block keeps at most ...
-constexpr int kRankAt = 512;                     // ... and how many of them are ranked at the end of a batch
+constexpr int kRankAt = kThreads;                // ... and how many of them are ranked at the end of a batch: one a thread
 constexpr float kLargest = 3.402823466e38f;
-static_assert(kRankAt + kMostCount <= kKept, "what the slow way adds to the kept");
+constexpr float kSpread = 40.f;                  // of x above m: sums stay below 2^58 of 2^127
+static_assert(kRankAt + kMostCount <= kKept && kMostCount * 2 <= kKept, "what the slow way adds to the kept");
 
 // A logit and its token in one number: the larger logit is the larger number, of equal ones the lower token. 0: none.
 typedef unsigned long long Key;
@@ -49,89 +51,168 @@ struct BeamArgs {
     unsigned char* parts;
 };
 
-template <typename T> struct Vec { static constexpr int kN = 16 / sizeof(T); };
-template <typename T> __device__ __forceinline__ float largest_of();
-template <> __device__ __forceinline__ float largest_of<float>() { return kLargest; }
-template <> __device__ __forceinline__ float largest_of<__half>() { return 65504.f; }
-template <> __device__ __forceinline__ float largest_of<__nv_bfloat16>() { return 3.38953139e38f; }
+// 16 bytes of logits.
+template <typename T> struct Vec;
+template <> struct Vec<float> {
+    static constexpr int kN = 4;
+    static constexpr float kMost = kLargest;
+    static constexpr uint32_t kNothing = 0xff800000u;              // minus infinity
+    static __device__ __forceinline__ float at(const uint4& v, int l) { return __uint_as_float(reinterpret_cast<const uint32_t*>(&v)[l]); }
+    static __device__ __forceinline__ float largest(const uint4& v) {      // NaN where one is
+        float r = __uint_as_float(v.x);
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(r) : "f"(__uint_as_float(v.y)));
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(r) : "f"(__uint_as_float(v.z)));
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(r) : "f"(__uint_as_float(v.w)));
+        return r;
+    }
+};
+template <> struct Vec<__half> {
+    static constexpr int kN = 8;
+    static constexpr float kMost = 65504.f;
+    static constexpr uint32_t kNothing = 0xfc00fc00u;
+    static __device__ __forceinline__ float at(const uint4& v, int l) { return __half2float(reinterpret_cast<const __half*>(&v)[l]); }
+    static __device__ __forceinline__ float largest(const uint4& v) {
+        const __half2* h = reinterpret_cast<const __half2*>(&v);
+        const __half2 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+        return __half2float(__hmax_nan(__low2half(m), __high2half(m)));
+    }
+};
+template <> struct Vec<__nv_bfloat16> {
+    static constexpr int kN = 8;
+    static constexpr float kMost = 3.38953139e38f;
+    static constexpr uint32_t kNothing = 0xff80ff80u;
+    static __device__ __forceinline__ float at(const uint4& v, int l) {
+        const uint32_t w = reinterpret_cast<const uint32_t*>(&v)[l / 2];
+        return __uint_as_float(l % 2 ? w & 0xffff0000u : w << 16);
+    }
+    static __device__ __forceinline__ float largest(const uint4& v) {
+        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+        const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+        return __bfloat162float(__hmax_nan(__low2bfloat16(m), __high2bfloat16(m)));
+    }
+};
 
-template <typename T>
-__device__ __forceinline__ void unpack(const uint4& v, float (&x)[Vec<T>::kN]) {
-    const T* h = reinterpret_cast<const T*>(&v);
-#pragma unroll
-    for (int l = 0; l < Vec<T>::kN; ++l) x[l] = float(h[l]);
+// exp(x - m) of two logits as the sums have it.
+constexpr float kLog2e = 1.442695022f, kLog2eRest = 1.925963033e-8f;
+__device__ __forceinline__ unsigned long long exponents(float x, float y, unsigned long long minus_m) {
+    const unsigned long long d = add2(pair(x, y), minus_m);
+    return fma2(d, pair(kLog2eRest, kLog2eRest), mul2(d, pair(kLog2e, kLog2e)));
 }
-__device__ __forceinline__ float max_nan(float a, float b) {       // NaN where one is
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
-// exp(x - m) as the sums have it.
 __device__ __forceinline__ float weight(float x, float m) {
-    const float d = x - m, t = fmaf(d, 1.925963033e-8f, d * 1.442695022f);
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(t));
-    return y;
+    float t, u;
+    unpair(exponents(x, x, pair(-m, -m)), t, u);
+    return exp2_fast(t);
 }
 
 // The kept logits in order: keys[0 .. n) become the `count` largest of them, falling; returns how many there are. All threads.
 __device__ __noinline__ int rank_kept(Key* keys, int n, int count, int* scratch) {
     const int tid = threadIdx.x;
-    Key mine[kKept / kThreads];
-    int rank[kKept / kThreads];
+    constexpr int kMine = kKept / kThreads;
+    Key mine[kMine];
+    int rank[kMine];
     int there = 0;
     __syncthreads();
     if (tid == 0) *scratch = 0;
+    if (tid == 1 && n % 2 == 1) keys[n] = 0ull;
 #pragma unroll
-    for (int i = 0; i < kKept / kThreads; ++i) {
+    for (int i = 0; i < kMine; ++i) {
         mine[i] = tid + i * kThreads < n ? keys[tid + i * kThreads] : 0ull;
         rank[i] = 0;
         there += mine[i] != 0;
     }
     __syncthreads();
+    const ulonglong2* const two = reinterpret_cast<const ulonglong2*>(keys);
     if (n <= kThreads) {
 #pragma unroll 4
-        for (int j = 0; j < n; ++j) rank[0] += keys[j] > mine[0];
+        for (int j = 0; j < n; j += 2) {
+            const ulonglong2 k = two[j / 2];
+            rank[0] += (k.x > mine[0]) + (k.y > mine[0]);
+        }
     } else {
-        for (int j = 0; j < n; ++j) {
-            const Key k = keys[j];
+#pragma unroll 1
+        for (int j = 0; j < n; j += 2) {
+            const ulonglong2 k = two[j / 2];
 #pragma unroll
-            for (int i = 0; i < kKept / kThreads; ++i) rank[i] += k > mine[i];
+            for (int i = 0; i < kMine; ++i) rank[i] += (k.x > mine[i]) + (k.y > mine[i]);
         }
     }
     if (there) atomicAdd(scratch, there);
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kKept / kThreads; ++i)
+    for (int i = 0; i < kMine; ++i)
         if (mine[i] && rank[i] < count) keys[rank[i]] = mine[i];
     const int all = min(*scratch, count);
     __syncthreads();
     return all;
 }
 
-// The largest key that `count` keys of the batch reach, 0 where there are fewer: bit by bit. For batches most of which pass the border - many
-// equal logits, or a rising row. All threads; `f` counts a thread's keys from a given one on.
-template <typename F>
-__device__ __forceinline__ Key border_of_batch(int count, int* sums, F f) {
+// Calls f(logit, token) for this thread's share of a batch, from memory: for what is rare.
+template <typename T, typename F>
+__device__ __forceinline__ void each_of_batch(const T* in, int t0, int end, F f) {
+    constexpr int N = Vec<T>::kN;
+#pragma unroll 1
+    for (int i = 0; i < kVecs * N; ++i) {
+        const int t = t0 + (i / N * kThreads + threadIdx.x) * N + i % N;
+        if (t >= 0 && t < end) {
+            const float x = float(in[t]);
+            if (x > -INFINITY) f(fminf(x, Vec<T>::kMost), t);      // (not of a NaN)
+        }
+    }
+}
+
+// This thread's share of a batch that has a NaN, an infinity or logits far above m.
+template <typename T>
+__device__ __noinline__ Part rare_sum(const T* in, int t0, int end, double sum, float m) {
+    float top = m;
+    each_of_batch(in, t0, end, [&](float x, int) { top = fmaxf(top, x); });
+    if (top - m > kSpread) {
+        sum *= exp((double)m - (double)top);
+        m = top;
+    }
+    float s = 0.f;
+    each_of_batch(in, t0, end, [&](float x, int) { s += weight(x, m); });
+    return Part{sum + (double)s, m, 0};
+}
+
+// More has passed the border in the batch at t0 than there is room for - many equal logits, or a rising row: what came before it in order, then
+// the `count` best of the batch, whose border is found bit by bit. Returns how many are kept. All threads.
+template <typename T>
+__device__ __noinline__ int keep_best_of_batch(const T* in, int t0, int end, Key* kept, int* n_kept, int count, int* scratch, int* sums) {
+    const int tid = threadIdx.x;
+    for (int i = tid; i < kKept; i += kThreads)
+        if (token_of(kept[i]) >= t0) kept[i] = 0ull;
+    const int n = rank_kept(kept, kKept, count, scratch);
+    if (tid == 0) *n_kept = n;
     Key border = 0;
 #pragma unroll 1
     for (int bit = 63; bit >= 0; --bit) {
         const Key next = border | 1ull << bit;
-        const int n = __reduce_add_sync(~0u, f(next));
+        int c = 0;
+        each_of_batch(in, t0, end, [&](float x, int t) { c += key_of(x, t) >= next; });
+        c = __reduce_add_sync(~0u, c);
         __syncthreads();
-        if ((threadIdx.x & 31) == 0) sums[threadIdx.x / 32] = n;
+        if ((tid & 31) == 0) sums[tid / 32] = c;
         __syncthreads();
         int all = 0;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) all += sums[w];
         if (all >= count) border = next;
     }
-    return border;
+    each_of_batch(in, t0, end, [&](float x, int t) {               // (fewer than count in the batch: all that there are)
+        const Key k = key_of(x, t);
+        if (k >= border) {
+            const int at = atomicAdd(n_kept, 1);
+            if (at < kKept) kept[at] = k;
+        }
+    });
+    __syncthreads();
+    return *n_kept;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 3) beam_rows_kernel(BeamArgs a) {
-    constexpr int N = Vec<T>::kN, kBatch = kThreads * kVecs * N;
+__global__ void __launch_bounds__(kThreads, 4) beam_rows_kernel(BeamArgs a) {
+    using V = Vec<T>;
+    constexpr int N = V::kN, kBatch = kThreads * kVecs * N;
     __shared__ __align__(16) Key kept[kKept];
     __shared__ int n_kept, scratch, sums[kWarps];
     __shared__ float warp_m[kWarps];
@@ -153,12 +234,11 @@ __global__ void __launch_bounds__(kThreads, 3) beam_rows_kernel(BeamArgs a) {
         for (int i = tid; i < p.count; i += kThreads) reinterpret_cast<Key*>(out + sizeof(Part))[i] = 0ull;
         return;
     }
-    const uint32_t nothing = sizeof(T) == 4 ? 0xff800000u : (largest_of<T>() < 1e5f ? 0xfc00fc00u : 0xff80ff80u);      // minus infinity
     const auto load = [&](int t0, uint4 (&v)[kVecs]) {
 #pragma unroll
         for (int u = 0; u < kVecs; ++u) {
             const int t = t0 + (u * kThreads + tid) * N;
-            v[u] = make_uint4(nothing, nothing, nothing, nothing);
+            v[u] = make_uint4(V::kNothing, V::kNothing, V::kNothing, V::kNothing);
             if (t >= 0 && t + N <= end) {
                 v[u] = __ldcs(reinterpret_cast<const uint4*>(in + t));
             } else if (t + N > 0 && t < end) {                     // the row's ends
@@ -169,130 +249,94 @@ __global__ void __launch_bounds__(kThreads, 3) beam_rows_kernel(BeamArgs a) {
         }
     };
 
-    const int of_warp = (p.count + kWarps - 1) / kWarps;
     uint4 v[kVecs];
     load(begin, v);
-    float m = 0.f, m0 = 0.f, border = -INFINITY;
+    // The first batch's largest logits of all threads: m, and a border that `count` logits reach.
+    float m = -kLargest, border;
+    {
+        float top = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < kVecs; ++u) {
+            const float x = V::largest(v[u]);
+            if (x == x) {
+                top = fmaxf(top, x);
+            } else {
+#pragma unroll
+                for (int l = 0; l < N; ++l) top = fmaxf(top, V::at(v[u], l));
+            }
+        }
+        uint32_t mine = ordered(fminf(top, V::kMost) + 0.f), best = 0, nth = 0;
+        for (int i = 0; i < (p.count + kWarps - 1) / kWarps; ++i) {
+            nth = __reduce_max_sync(~0u, mine);
+            if (i == 0) best = nth;
+            const unsigned who = __ballot_sync(~0u, mine == nth);
+            if (lane == __ffs(who) - 1) mine = 0;
+        }
+        if (lane == 0) {
+            warp_m[tid / 32] = unordered(best);
+            warp_border[tid / 32] = nth;
+        }
+        __syncthreads();
+        uint32_t least = ~0u;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            m = fmaxf(m, warp_m[w]);
+            least = min(least, warp_border[w]);
+        }
+        border = unordered(least);                                 // a logit of minus infinity never passes, whatever the border
+    }
+    const float m0 = m;
     double sum = 0.;
 #pragma unroll 1
     for (int t0 = begin; t0 < end; t0 += kBatch) {
+        const bool first = t0 == begin;
         uint4 next[kVecs];
         if (t0 + kBatch < end) load(t0 + kBatch, next);
-        const auto largest = [&] {
-            float top = -INFINITY;
-#pragma unroll
-            for (int u = 0; u < kVecs; ++u) {
-                float x[N];
-                unpack<T>(v[u], x);
-#pragma unroll
-                for (int l = 0; l < N; ++l) top = max_nan(top, x[l]);
-            }
-            return top;
-        };
-        float top = largest();
-        if (!(top <= kLargest)) {                                  // a NaN or an infinity: rare
-#pragma unroll
-            for (int u = 0; u < kVecs; ++u) {
-                T* const h = reinterpret_cast<T*>(&v[u]);
-#pragma unroll
-                for (int l = 0; l < N; ++l) {
-                    const float x = float(h[l]);
-                    if (x != x) h[l] = T(-INFINITY);
-                    else if (x > kLargest) h[l] = T(largest_of<T>());
-                }
-            }
-            top = largest();
-        }
-        const bool first = t0 == begin;
-        if (first) {
-            uint32_t mine = ordered(top + 0.f), best = 0, nth = 0;
-            for (int i = 0; i < of_warp; ++i) {
-                nth = __reduce_max_sync(~0u, mine);
-                if (i == 0) best = nth;
-                const unsigned who = __ballot_sync(~0u, mine == nth);
-                if (lane == __ffs(who) - 1) mine = 0;
-            }
-            if (lane == 0) {
-                warp_m[tid / 32] = unordered(best);
-                warp_border[tid / 32] = of_warp <= 32 ? nth : 0;
-            }
-            __syncthreads();
-            uint32_t least = ~0u;
-            m = -kLargest;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                m = fmaxf(m, warp_m[w]);
-                least = min(least, warp_border[w]);
-            }
-            m0 = m;
-            // (below: a logit of minus infinity never passes)
-            border = least > ordered(-INFINITY) ? unordered(least) : -INFINITY;
-        }
-        if (top - m > 40.f) {                                      // sums stay below 2^58 of 2^127
-            sum *= exp((double)m - (double)top);
-            m = top;
-        }
-        float s[kVecs];
+        float top[kVecs];
+        unsigned long long s = 0ull;
+        const unsigned long long minus_m = pair(-m, -m);
 #pragma unroll
         for (int u = 0; u < kVecs; ++u) {
-            float x[N];
-            unpack<T>(v[u], x);
-            s[u] = 0.f;
+            top[u] = V::largest(v[u]);
 #pragma unroll
-            for (int l = 0; l < N; ++l) s[u] += weight(x[l], m);
+            for (int l = 0; l < N; l += 2) {
+                float e, f;
+                unpair(exponents(V::at(v[u], l), V::at(v[u], l + 1), minus_m), e, f);
+                s = add2(s, pair(exp2_fast(e), exp2_fast(f)));
+            }
         }
-        sum += (double)((s[0] + s[1]) + (s[2] + s[3]));
+        bool fine = true;
+#pragma unroll
+        for (int u = 0; u < kVecs; ++u) fine &= top[u] <= fminf(m + kSpread, V::kMost);
+        if (fine) {
+            float e, f;
+            unpair(s, e, f);
+            sum += (double)(e + f);
+        } else {
+            const Part part = rare_sum(in, t0, end, sum, m);
+            sum = part.sum;
+            m = part.m;
+        }
         bool full = false;
         // of a later batch what equals the border comes behind `count` that do and are of lower tokens
-        const auto passes = [&](float x) { return x > border || first && x == border && x > -INFINITY; };
-        if (passes(top)) {
 #pragma unroll
-            for (int u = 0; u < kVecs; ++u) {
-                float x[N];
-                unpack<T>(v[u], x);
+        for (int u = 0; u < kVecs; ++u)
+            if (!(top[u] < border || !first && top[u] == border)) {      // (or a NaN among them)
 #pragma unroll
-                for (int l = 0; l < N; ++l)
-                    if (passes(x[l])) {
+                for (int l = 0; l < N; ++l) {
+                    const float x = V::at(v[u], l);
+                    if ((x > border || first && x == border) && x > -INFINITY) {
                         const int at = atomicAdd(&n_kept, 1);
-                        if (at < kKept) kept[at] = key_of(x[l], t0 + (u * kThreads + tid) * N + l);
+                        if (at < kKept) kept[at] = key_of(fminf(x, V::kMost), t0 + (u * kThreads + tid) * N + l);
                         full |= at >= kRankAt;
                     }
+                }
             }
-        }
-        if (__syncthreads_or(full)) {
+        // the first batch's border is a guess: the next one is as high as can be
+        if (__syncthreads_or(full || first)) {
             int n = n_kept;
-            const bool lost = n > kKept;
-            if (lost) {
-                // the batch again: what came before it, then as many of it as can count
-                for (int i = tid; i < kKept; i += kThreads)
-                    if (token_of(kept[i]) >= t0) kept[i] = 0ull;
-                n = rank_kept(kept, kKept, p.count, &scratch);
-                if (tid == 0) n_kept = n;
-                const auto each = [&](auto f) {
-#pragma unroll
-                    for (int u = 0; u < kVecs; ++u) {
-                        float x[N];
-                        unpack<T>(v[u], x);
-#pragma unroll
-                        for (int l = 0; l < N; ++l) f(key_of(x[l], t0 + (u * kThreads + tid) * N + l));
-                    }
-                };
-                const Key from = border_of_batch(p.count, sums, [&](Key k) {
-                    int c = 0;
-                    each([&](Key mine) { c += mine >= k; });
-                    return c;
-                });
-                each([&](Key mine) {
-                    // (fewer than count in the batch: all that there are)
-                    if (mine != 0 && mine >= from) {
-                        const int at = atomicAdd(&n_kept, 1);
-                        if (at < kKept) kept[at] = mine;
-                    }
-                });
-                __syncthreads();
-                n = n_kept;
-            }
-            n = rank_kept(kept, min(n, kKept), p.count, &scratch);
+            if (n > kKept) n = keep_best_of_batch(in, t0, end, kept, &n_kept, p.count, &scratch, sums);
+            n = rank_kept(kept, n, p.count, &scratch);
             if (tid == 0) n_kept = n;
             if (n == p.count) border = logit_of(kept[n - 1]);
             __syncthreads();
@@ -330,18 +374,24 @@ __global__ void __launch_bounds__(kThreads, 3) beam_rows_kernel(BeamArgs a) {
 }
 
 // ---- the groups
-struct Total { double value; unsigned long long at; };             // at: beam * vocab + token
+// A total as a whole number of the same order, and where it comes from: beam * vocab + token, the lower the better.
+struct __align__(16) Total { unsigned long long value, at; };
+__device__ __forceinline__ unsigned long long ordered(double x) {
+    const unsigned long long u = __double_as_longlong(x + 0.);
+    return u >> 63 ? ~u : u | 1ull << 63;
+}
+__device__ __forceinline__ double unordered(unsigned long long u) { return __longlong_as_double(u >> 63 ? u & ~(1ull << 63) : ~u); }
 __device__ __forceinline__ bool better(const Total& x, const Total& y) { return x.value > y.value || x.value == y.value && x.at < y.at; }
 
 constexpr int kPickThreads = 512, kPickWarps = kPickThreads / 32, kPicked = 1024;
 constexpr int kMostBeams = 1024;
 
 __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamArgs a) {
-    extern __shared__ double2 beam_terms[];                        // of each beam: its largest logit m, and log sum exp(x - m)
+    extern __shared__ double2 beam_terms[];                        // of each beam: its largest logit m, and log sum exp(x - m); then score minus that
     __shared__ Total found[kPicked];
     __shared__ Total best[kMostCount];
-    __shared__ double warp_value[kPickWarps];
-    __shared__ unsigned long long warp_at[kPickWarps];
+    __shared__ unsigned warp_border[kPickWarps];
+    __shared__ Total warp_best[kPickWarps];
     __shared__ int n_found;
     const OgleBeamParams& p = a.p;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid / 32, g = blockIdx.x;
@@ -350,18 +400,29 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamArgs a) {
     grid_dependency_trigger();
     grid_dependency_wait();
     const unsigned char* const parts = a.parts + (size_t)g * p.beams * a.ranges * stride;
+    const int lists = p.beams * a.ranges, all = lists * p.count;
+    // Candidate i is the (i / lists)-th of list i % lists: the lists' best come first, and neighbours are of different lists.
+    const auto key_at = [&](int i, int& list) {
+        const int place = i / lists;
+        list = i - place * lists;
+        return reinterpret_cast<const Key*>(parts + list * stride + sizeof(Part))[place];
+    };
+    int my_list = 0;
+    const Key my_key = tid < all ? key_at(tid, my_list) : 0ull;    // under way while the sums are added
     for (int b = warp; b < p.beams; b += kPickWarps) {
         const unsigned char* const mine = parts + (size_t)b * a.ranges * stride;
         float top = -INFINITY;
+        Part part = {0., -INFINITY, 0};
         for (int r = lane; r < a.ranges; r += 32) {
             const Key k = *reinterpret_cast<const Key*>(mine + r * stride + sizeof(Part));
+            if (r == lane) part = *reinterpret_cast<const Part*>(mine + r * stride);
             if (k) top = fmaxf(top, logit_of(k));
         }
 #pragma unroll
         for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
         double sum = 0.;
         for (int r = lane; r < a.ranges; r += 32) {
-            const Part part = *reinterpret_cast<const Part*>(mine + r * stride);
+            if (r != lane) part = *reinterpret_cast<const Part*>(mine + r * stride);
             if (part.sum > 0.) sum += part.sum * exp((double)part.m - (double)top);
         }
 #pragma unroll
@@ -392,42 +453,45 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamArgs a) {
         if (b < p.beams) beam_terms[b].y = (p.scores ? (double)p.scores[g * p.beams + b] : 0.) - minus[i];
     }
     __syncthreads();
-    const int lists = p.beams * a.ranges, all = lists * p.count;
-    const auto total = [&](int i, Total& t) {                      // candidate i; false where there is none
-        const int list = i / p.count, b = list / a.ranges;
-        const Key k = reinterpret_cast<const Key*>(parts + list * stride + sizeof(Part))[i - list * p.count];
-        if (!k) return false;
+    const auto total = [&](Key k, int list) {
+        const int b = list / a.ranges;
         const double2 term = beam_terms[b];
-        t.value = term.y + ((double)logit_of(k) - term.x);
-        t.at = (unsigned long long)b * p.vocab + token_of(k);
-        return true;
+        return Total{ordered(term.y + ((double)logit_of(k) - term.x)), (unsigned long long)b * p.vocab + token_of(k)};
     };
-    // a border that `count` of them reach, from the threads' own best as above
-    double border = -INFINITY;
-    if (all > kPickThreads) {
-        double mine = -INFINITY;
-        Total t;
-        for (int i = tid; i < all; i += kPickThreads)
-            if (total(i, t)) mine = fmax(mine, t.value);
-        double nth = -INFINITY;
-        for (int i = 0; i < (p.count + kPickWarps - 1) / kPickWarps; ++i) {
-            nth = mine;
-#pragma unroll
-            for (int d = 16; d; d /= 2) nth = fmax(nth, __shfl_xor_sync(~0u, nth, d));
-            const unsigned who = __ballot_sync(~0u, mine == nth);
-            if (lane == __ffs(who) - 1) mine = -INFINITY;
+    // A border that `count` of them reach, by the upper half of the totals' bits: the count-th of the threads' best in some warp; of more than
+    // a warp, the (count / 16)-th in each, the least of them.
+    const Total my_total = my_key ? total(my_key, my_list) : Total{0ull, ~0ull};
+    unsigned border = 0;
+    if (all > 32) {
+        unsigned long long top = my_total.value;
+        for (int i = tid + kPickThreads; i < all; i += kPickThreads) {
+            int list;
+            const Key k = key_at(i, list);
+            if (k) top = max(top, total(k, list).value);
         }
-        if (lane == 0) warp_value[warp] = nth;
+        unsigned mine = unsigned(top >> 32), nth = 0;
+        const int of_warp = p.count <= 32 ? p.count : (p.count + kPickWarps - 1) / kPickWarps;
+        for (int i = 0; i < of_warp; ++i) {
+            nth = __reduce_max_sync(~0u, mine);
+            const unsigned who = __ballot_sync(~0u, mine == nth);
+            if (lane == __ffs(who) - 1) mine = 0;
+        }
+        if (lane == 0) warp_border[warp] = nth;
         __syncthreads();
-        border = warp_value[0];
-        for (int w = 1; w < kPickWarps; ++w) border = fmin(border, warp_value[w]);
+        border = warp_border[0];
+        for (int w = 1; w < kPickWarps; ++w) border = p.count <= 32 ? max(border, warp_border[w]) : min(border, warp_border[w]);
     }
-    for (int i = tid; i < all; i += kPickThreads) {
-        Total t;
-        if (total(i, t) && t.value >= border) {
+    const auto offer = [&](const Total& t) {
+        if (unsigned(t.value >> 32) >= border) {
             const int at = atomicAdd(&n_found, 1);
             if (at < kPicked) found[at] = t;
         }
+    };
+    if (my_key) offer(my_total);
+    for (int i = tid + kPickThreads; i < all; i += kPickThreads) {
+        int list;
+        const Key k = key_at(i, list);
+        if (k) offer(total(k, list));
     }
     __syncthreads();
     int n = n_found;
@@ -435,29 +499,33 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamArgs a) {
         for (int i = tid; i < n; i += kPickThreads) {
             const Total mine = found[i];
             int rank = 0;
+#pragma unroll 4
             for (int j = 0; j < n; ++j) rank += better(found[j], mine);
             if (rank < p.count) best[rank] = mine;
         }
         n = min(n, p.count);
     } else {
-        // too many equal ones: the best, the best of the rest, ...
-        Total last = {INFINITY, 0ull};
+        // too many alike: the best, the best of the rest, ...
+        Total last = {~0ull, 0ull};
         for (int k = 0; k < p.count; ++k) {
-            Total mine = {-INFINITY, ~0ull}, t;
-            for (int i = tid; i < all; i += kPickThreads)
-                if (total(i, t) && better(last, t) && better(t, mine)) mine = t;
+            Total mine = {0ull, ~0ull};
+            for (int i = tid; i < all; i += kPickThreads) {
+                int list;
+                const Key key = key_at(i, list);
+                if (!key) continue;
+                const Total t = total(key, list);
+                if (better(last, t) && better(t, mine)) mine = t;
+            }
 #pragma unroll
             for (int d = 16; d; d /= 2) {
                 const Total o = {__shfl_xor_sync(~0u, mine.value, d), __shfl_xor_sync(~0u, mine.at, d)};
                 if (better(o, mine)) mine = o;
             }
-            if (lane == 0) { warp_value[warp] = mine.value; warp_at[warp] = mine.at; }
+            if (lane == 0) warp_best[warp] = mine;
             __syncthreads();
-            last = Total{warp_value[0], warp_at[0]};
-            for (int w = 1; w < kPickWarps; ++w) {
-                const Total o = {warp_value[w], warp_at[w]};
-                if (better(o, last)) last = o;
-            }
+            last = warp_best[0];
+            for (int w = 1; w < kPickWarps; ++w)
+                if (better(warp_best[w], last)) last = warp_best[w];
             __syncthreads();
             if (tid == 0) best[k] = last;
         }
@@ -466,7 +534,7 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamArgs a) {
     __syncthreads();
     for (int i = tid; i < p.count; i += kPickThreads) {
         const bool there = i < n;
-        p.out_score[(size_t)g * p.count + i] = there ? float(best[i].value) : -INFINITY;
+        p.out_score[(size_t)g * p.count + i] = there ? float(unordered(best[i].value)) : -INFINITY;
         p.out_beam[(size_t)g * p.count + i] = there ? int(best[i].at / p.vocab) : -1;
         p.out_token[(size_t)g * p.count + i] = there ? int(best[i].at % p.vocab) : -1;
     }
@@ -487,7 +555,7 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamArgs a) {
             if (goes_on && at < p.beams) {
                 p.next_row[(size_t)g * p.beams + at] = g * p.beams + beam;
                 p.next_token[(size_t)g * p.beams + at] = token;
-                p.next_score[(size_t)g * p.beams + at] = float(best[i].value);
+                p.next_score[(size_t)g * p.beams + at] = float(unordered(best[i].value));
             }
             next += __popc(who);
         }
@@ -509,7 +577,7 @@ int check(const OgleBeamParams* p) {
 void split(const OgleBeamParams* p, int& range, int& ranges) {
     const int n = p->dtype == OGLE_F32 ? 4 : 8, batch = kThreads * kVecs * n;
     const long batches = div_up((long)p->vocab + n - 1, batch), rows = (long)p->n_groups * p->beams;
-    long blocks = rows > 0 ? 3L * kNumSMs / rows : 1;
+    long blocks = rows > 0 ? 4L * kNumSMs / rows : 1;
     if (blocks < 1) blocks = 1;
     const long each = batches > 0 ? div_up(batches, blocks) : 1;
     range = int(each * batch);

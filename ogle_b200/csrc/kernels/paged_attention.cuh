@@ -1,6 +1,7 @@
 // What the forms of attention over the paged cache share.
 #pragma once
 #include "paged.cuh"
+#include "pairs.cuh"
 #include "tc_common.cuh"
 #include "tma_host.h"
 
@@ -75,34 +76,6 @@ __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
 __device__ __forceinline__ uint32_t rest_bits(uint32_t rounded, float lo, float hi) {
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&rounded));
     return half2_bits(lo - f.x, hi - f.y);
-}
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// Two fp32 numbers at a time.
-__device__ __forceinline__ unsigned long long pair(float lo, float hi) {
-    unsigned long long r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-__device__ __forceinline__ void unpair(unsigned long long v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
-__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
-    unsigned long long r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
-    unsigned long long r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
-    unsigned long long r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
 }
 
 // Four values of a row of the result from its weighted sum v, its m and its sum of weights; with the first four, its lse.
