@@ -24,6 +24,7 @@ constexpr int kMostCount = 128, kMostEnds = 1024;
 constexpr int kKept = 1024;                      // logits that a block keeps at most ...
 constexpr int kRankAt = kThreads;                // ... and how many of them are ranked at the end of a batch: one a thread
 constexpr float kLargest = 3.402823466e38f;
+constexpr int kGroup = 4;                        // batches between two looks at what has been kept, at most
 constexpr float kSpread = 40.f;                  // of x above m: sums stay below 2^58 of 2^127
 static_assert(kRankAt + kMostCount <= kKept && kMostCount * 2 <= kKept, "what the slow way adds to the kept");
 
@@ -41,8 +42,8 @@ __device__ __forceinline__ Key key_of(float x, int token) {
 __device__ __forceinline__ float logit_of(Key k) { return unordered(uint32_t(k >> 32)); }
 __device__ __forceinline__ int token_of(Key k) { return int(~uint32_t(k)); }
 
-// What a block leaves behind, followed by its `count` best in falling order (0: none).
-struct __align__(16) Part { double sum; float m; int unused; };
+// What a block leaves behind - a sum of exp(x - m) -, followed by its `count` best in falling order (0: none).
+struct __align__(16) Part { double sum, m; };
 __host__ __device__ inline size_t part_bytes(int count) { return sizeof(Part) + ((size_t)count + 1) / 2 * 16; }
 
 struct BeamArgs {
@@ -58,6 +59,9 @@ template <> struct Vec<float> {
     static constexpr float kMost = kLargest;
     static constexpr uint32_t kNothing = 0xff800000u;              // minus infinity
     static __device__ __forceinline__ float at(const uint4& v, int l) { return __uint_as_float(reinterpret_cast<const uint32_t*>(&v)[l]); }
+    static __device__ __forceinline__ float at_any(const uint4& v, int l) {       // l known at run time alone
+        return __uint_as_float(l & 2 ? (l & 1 ? v.w : v.z) : (l & 1 ? v.y : v.x));
+    }
     static __device__ __forceinline__ float largest(const uint4& v) {      // NaN where one is
         float r = __uint_as_float(v.x);
         asm("max.NaN.f32 %0, %0, %1;" : "+f"(r) : "f"(__uint_as_float(v.y)));
@@ -71,6 +75,10 @@ template <> struct Vec<__half> {
     static constexpr float kMost = 65504.f;
     static constexpr uint32_t kNothing = 0xfc00fc00u;
     static __device__ __forceinline__ float at(const uint4& v, int l) { return __half2float(reinterpret_cast<const __half*>(&v)[l]); }
+    static __device__ __forceinline__ float at_any(const uint4& v, int l) {
+        const uint32_t w = l & 4 ? (l & 2 ? v.w : v.z) : (l & 2 ? v.y : v.x), h = l & 1 ? w >> 16 : w & 0xffffu;
+        return __half2float(__ushort_as_half((unsigned short)h));
+    }
     static __device__ __forceinline__ float largest(const uint4& v) {
         const __half2* h = reinterpret_cast<const __half2*>(&v);
         const __half2 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
@@ -85,6 +93,10 @@ template <> struct Vec<__nv_bfloat16> {
         const uint32_t w = reinterpret_cast<const uint32_t*>(&v)[l / 2];
         return __uint_as_float(l % 2 ? w & 0xffff0000u : w << 16);
     }
+    static __device__ __forceinline__ float at_any(const uint4& v, int l) {
+        const uint32_t w = l & 4 ? (l & 2 ? v.w : v.z) : (l & 2 ? v.y : v.x), h = l & 1 ? w >> 16 : w & 0xffffu;
+        return __uint_as_float(h << 16);
+    }
     static __device__ __forceinline__ float largest(const uint4& v) {
         const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
         const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
@@ -92,17 +104,10 @@ template <> struct Vec<__nv_bfloat16> {
     }
 };
 
-// exp(x - m) of two logits as the sums have it.
-constexpr float kLog2e = 1.442695022f, kLog2eRest = 1.925963033e-8f;
-__device__ __forceinline__ unsigned long long exponents(float x, float y, unsigned long long minus_m) {
-    const unsigned long long d = add2(pair(x, y), minus_m);
-    return fma2(d, pair(kLog2eRest, kLog2eRest), mul2(d, pair(kLog2e, kLog2e)));
-}
-__device__ __forceinline__ float weight(float x, float m) {
-    float t, u;
-    unpair(exponents(x, x, pair(-m, -m)), t, u);
-    return exp2_fast(t);
-}
+// exp(x - m) as the sums have it: 2^(x log2(e) - c) in one rounding of the exponent, which is small where the weight is large. c is an fp32
+// number, m what it stands for; log2(e) in fp32 makes a weight wrong by 2^-26 of its distance from m.
+constexpr float kLog2e = 1.442695022f;
+__device__ __forceinline__ float weight(float x, float c) { return exp2_fast(fmaf(x, kLog2e, -c)); }
 
 // The kept logits in order: keys[0 .. n) become the `count` largest of them, falling; returns how many there are. All threads.
 __device__ __noinline__ int rank_kept(Key* keys, int n, int count, int* scratch) {
@@ -123,6 +128,7 @@ __device__ __noinline__ int rank_kept(Key* keys, int n, int count, int* scratch)
     __syncthreads();
     const ulonglong2* const two = reinterpret_cast<const ulonglong2*>(keys);
     if (n <= kThreads) {
+        if (mine[0])
 #pragma unroll 4
         for (int j = 0; j < n; j += 2) {
             const ulonglong2 k = two[j / 2];
@@ -146,38 +152,45 @@ __device__ __noinline__ int rank_kept(Key* keys, int n, int count, int* scratch)
     return all;
 }
 
-// Calls f(logit, token) for this thread's share of a batch, from memory: for what is rare.
+// Calls f(logit, token) for this thread's share of the logits from t0 to end, from memory: for what is rare.
 template <typename T, typename F>
-__device__ __forceinline__ void each_of_batch(const T* in, int t0, int end, F f) {
+__device__ __forceinline__ void each_of(const T* in, int t0, int end, F f) {
     constexpr int N = Vec<T>::kN;
 #pragma unroll 1
-    for (int i = 0; i < kVecs * N; ++i) {
-        const int t = t0 + (i / N * kThreads + threadIdx.x) * N + i % N;
-        if (t >= 0 && t < end) {
+    for (int t1 = t0 + threadIdx.x * N; t1 < end; t1 += kThreads * N)
+#pragma unroll 1
+        for (int t = max(t1, 0); t < min(t1 + N, end); ++t) {
             const float x = float(in[t]);
             if (x > -INFINITY) f(fminf(x, Vec<T>::kMost), t);      // (not of a NaN)
         }
-    }
 }
 
-// This thread's share of a batch that has a NaN, an infinity or logits far above m.
+// A thread's sum of exp(x - m). Logits up to fine_to are added by weight(x, c); above 10^6, where c would not stand for any number near m, none is.
+struct Sum { double sum, m; float c, fine_to; };
+__device__ __forceinline__ void refer_to(Sum& s, float m, float most) {
+    const bool fine = fabsf(m) < 1e6f;
+    s.c = fine ? m * kLog2e : 0.f;
+    s.m = fine ? (double)s.c / (double)kLog2e : (double)m;
+    s.fine_to = fine ? fminf(float(s.m) + kSpread, most) : -INFINITY;
+}
+// This thread's share of a batch that has a NaN, an infinity or logits far above m, or whose m is far from 0.
 template <typename T>
-__device__ __noinline__ Part rare_sum(const T* in, int t0, int end, double sum, float m) {
-    float top = m;
-    each_of_batch(in, t0, end, [&](float x, int) { top = fmaxf(top, x); });
-    if (top - m > kSpread) {
-        sum *= exp((double)m - (double)top);
-        m = top;
+__device__ __noinline__ Sum rare_sum(const T* in, int t0, int end, Sum s) {
+    float top = -kLargest;
+    each_of(in, t0, end, [&](float x, int) { top = fmaxf(top, x); });
+    if ((double)top - s.m > kSpread) {
+        const double before = s.m;
+        refer_to(s, top, Vec<T>::kMost);
+        s.sum *= exp(before - s.m);
     }
-    float s = 0.f;
-    each_of_batch(in, t0, end, [&](float x, int) { s += weight(x, m); });
-    return Part{sum + (double)s, m, 0};
+    each_of(in, t0, end, [&](float x, int) { s.sum += exp((double)x - s.m); });
+    return s;
 }
 
-// More has passed the border in the batch at t0 than there is room for - many equal logits, or a rising row: what came before it in order, then
-// the `count` best of the batch, whose border is found bit by bit. Returns how many are kept. All threads.
+// More has passed the border in the batches from t0 to end than there is room for - many equal logits, or a rising row: what came before them
+// in order, then the `count` best of them, whose border is found bit by bit. Returns how many are kept. All threads.
 template <typename T>
-__device__ __noinline__ int keep_best_of_batch(const T* in, int t0, int end, Key* kept, int* n_kept, int count, int* scratch, int* sums) {
+__device__ __noinline__ int keep_best(const T* in, int t0, int end, Key* kept, int* n_kept, int count, int* scratch, int* sums) {
     const int tid = threadIdx.x;
     for (int i = tid; i < kKept; i += kThreads)
         if (token_of(kept[i]) >= t0) kept[i] = 0ull;
@@ -188,7 +201,7 @@ __device__ __noinline__ int keep_best_of_batch(const T* in, int t0, int end, Key
     for (int bit = 63; bit >= 0; --bit) {
         const Key next = border | 1ull << bit;
         int c = 0;
-        each_of_batch(in, t0, end, [&](float x, int t) { c += key_of(x, t) >= next; });
+        each_of(in, t0, end, [&](float x, int t) { c += key_of(x, t) >= next; });
         c = __reduce_add_sync(~0u, c);
         __syncthreads();
         if ((tid & 31) == 0) sums[tid / 32] = c;
@@ -198,7 +211,7 @@ __device__ __noinline__ int keep_best_of_batch(const T* in, int t0, int end, Key
         for (int w = 0; w < kWarps; ++w) all += sums[w];
         if (all >= count) border = next;
     }
-    each_of_batch(in, t0, end, [&](float x, int t) {               // (fewer than count in the batch: all that there are)
+    each_of(in, t0, end, [&](float x, int t) {                     // (fewer than count of them: all that there are)
         const Key k = key_of(x, t);
         if (k >= border) {
             const int at = atomicAdd(n_kept, 1);
@@ -210,12 +223,12 @@ __device__ __noinline__ int keep_best_of_batch(const T* in, int t0, int end, Key
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 4) beam_rows_kernel(BeamArgs a) {
+__global__ void __launch_bounds__(kThreads, 3) beam_rows_kernel(BeamArgs a) {
     using V = Vec<T>;
     constexpr int N = V::kN, kBatch = kThreads * kVecs * N;
     __shared__ __align__(16) Key kept[kKept];
     __shared__ int n_kept, scratch, sums[kWarps];
-    __shared__ float warp_m[kWarps];
+    __shared__ double warp_m[kWarps];
     __shared__ uint32_t warp_border[kWarps];
     __shared__ double warp_sum[kWarps];
     const OgleBeamParams& p = a.p;
@@ -230,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, 4) beam_rows_kernel(BeamArgs a) {
     const int begin = blockIdx.x * a.range - shift, end = min(begin + a.range, p.vocab);
     const float score = p.scores ? p.scores[row] : 0.f;
     if (begin >= end || !(fabsf(score) <= kLargest)) {             // behind the row's end, or of a beam that is none
-        if (tid == 0) *reinterpret_cast<Part*>(out) = Part{0., -INFINITY, 0};
+        if (tid == 0) *reinterpret_cast<Part*>(out) = Part{0., 0.};
         for (int i = tid; i < p.count; i += kThreads) reinterpret_cast<Key*>(out + sizeof(Part))[i] = 0ull;
         return;
     }
@@ -252,8 +265,11 @@ __global__ void __launch_bounds__(kThreads, 4) beam_rows_kernel(BeamArgs a) {
     uint4 v[kVecs];
     load(begin, v);
     // The first batch's largest logits of all threads: m, and a border that `count` logits reach.
-    float m = -kLargest, border;
+    float limit;                                                   // what is above it is kept
+    Sum sum;
+    sum.sum = 0.;
     {
+        float m = -kLargest;
         float top = -INFINITY;
 #pragma unroll
         for (int u = 0; u < kVecs; ++u) {
@@ -273,102 +289,106 @@ __global__ void __launch_bounds__(kThreads, 4) beam_rows_kernel(BeamArgs a) {
             if (lane == __ffs(who) - 1) mine = 0;
         }
         if (lane == 0) {
-            warp_m[tid / 32] = unordered(best);
+            warp_m[tid / 32] = (double)unordered(best);
             warp_border[tid / 32] = nth;
         }
         __syncthreads();
         uint32_t least = ~0u;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-            m = fmaxf(m, warp_m[w]);
+            m = fmaxf(m, float(warp_m[w]));
             least = min(least, warp_border[w]);
         }
-        border = unordered(least);                                 // a logit of minus infinity never passes, whatever the border
+        // the number below it (below 0 comes -0, which is not less)
+        limit = least > ordered(-INFINITY) ? unordered(least - (least == 0x80000000u ? 2 : 1)) : -INFINITY;
+        refer_to(sum, m, V::kMost);
     }
-    const float m0 = m;
-    double sum = 0.;
+    const double m0 = sum.m;
+    int group_begin = begin, n = 0;
+    bool full = false;
 #pragma unroll 1
-    for (int t0 = begin; t0 < end; t0 += kBatch) {
-        const bool first = t0 == begin;
+    for (int t0 = begin, batch = 0; t0 < end; t0 += kBatch, ++batch) {
         uint4 next[kVecs];
-        if (t0 + kBatch < end) load(t0 + kBatch, next);
+        const bool last = t0 + kBatch >= end;
+        if (!last) load(t0 + kBatch, next);
         float top[kVecs];
         unsigned long long s = 0ull;
-        const unsigned long long minus_m = pair(-m, -m);
+        const unsigned long long log2e = pair(kLog2e, kLog2e), minus_c = pair(-sum.c, -sum.c);
+        bool fine = true;
 #pragma unroll
         for (int u = 0; u < kVecs; ++u) {
             top[u] = V::largest(v[u]);
+            fine &= top[u] <= sum.fine_to;
 #pragma unroll
             for (int l = 0; l < N; l += 2) {
                 float e, f;
-                unpair(exponents(V::at(v[u], l), V::at(v[u], l + 1), minus_m), e, f);
+                unpair(fma2(pair(V::at(v[u], l), V::at(v[u], l + 1)), log2e, minus_c), e, f);
                 s = add2(s, pair(exp2_fast(e), exp2_fast(f)));
             }
         }
-        bool fine = true;
-#pragma unroll
-        for (int u = 0; u < kVecs; ++u) fine &= top[u] <= fminf(m + kSpread, V::kMost);
         if (fine) {
             float e, f;
             unpair(s, e, f);
-            sum += (double)(e + f);
+            sum.sum += (double)(e + f);
         } else {
-            const Part part = rare_sum(in, t0, end, sum, m);
-            sum = part.sum;
-            m = part.m;
+            sum = rare_sum(in, t0, min(t0 + kBatch, end), sum);
         }
-        bool full = false;
-        // of a later batch what equals the border comes behind `count` that do and are of lower tokens
 #pragma unroll
         for (int u = 0; u < kVecs; ++u)
-            if (!(top[u] < border || !first && top[u] == border)) {      // (or a NaN among them)
+            if (!(top[u] <= limit)) {                              // (or a NaN among them)
+                unsigned who = 0;
 #pragma unroll
-                for (int l = 0; l < N; ++l) {
-                    const float x = V::at(v[u], l);
-                    if ((x > border || first && x == border) && x > -INFINITY) {
-                        const int at = atomicAdd(&n_kept, 1);
-                        if (at < kKept) kept[at] = key_of(fminf(x, V::kMost), t0 + (u * kThreads + tid) * N + l);
-                        full |= at >= kRankAt;
-                    }
+                for (int l = 0; l < N; ++l) who |= unsigned(V::at(v[u], l) > limit) << l;
+                while (who) {                                      // most often one
+                    const int l = __ffs(who) - 1;
+                    who &= who - 1;
+                    const int at = atomicAdd(&n_kept, 1);
+                    if (at < kKept) kept[at] = key_of(fminf(V::at_any(v[u], l), V::kMost), t0 + (u * kThreads + tid) * N + l);
+                    full |= at >= kRankAt;
                 }
             }
-        // the first batch's border is a guess: the next one is as high as can be
-        if (__syncthreads_or(full || first)) {
-            int n = n_kept;
-            if (n > kKept) n = keep_best_of_batch(in, t0, end, kept, &n_kept, p.count, &scratch, sums);
-            n = rank_kept(kept, n, p.count, &scratch);
-            if (tid == 0) n_kept = n;
-            if (n == p.count) border = logit_of(kept[n - 1]);
-            __syncthreads();
+        // The first batch's border is a guess: the next one is as high as can be. It is raised when there is twice as much to go by, and as often
+        // as there is much to rank.
+        const bool raise = (batch & (batch + 1)) == 0 || last;
+        if (raise || batch % kGroup == 0) {
+            if (__syncthreads_or(full || raise)) {
+                n = n_kept;
+                if (n > kKept) n = keep_best(in, group_begin, min(t0 + kBatch, end), kept, &n_kept, p.count, &scratch, sums);
+                n = rank_kept(kept, n, p.count, &scratch);
+                if (tid == 0) n_kept = n;
+                // what equals the border later comes behind `count` that do, whose tokens are lower
+                limit = n == p.count ? logit_of(kept[n - 1]) : -INFINITY;
+                __syncthreads();
+            }
+            group_begin = t0 + kBatch;
+            full = false;
         }
 #pragma unroll
         for (int u = 0; u < kVecs; ++u) v[u] = next[u];
     }
 
-    __syncthreads();
-    const int n = rank_kept(kept, n_kept, p.count, &scratch);
     // the kept logits' part of the sum in 64 bits, where all threads have the same m
-    const bool same = __syncthreads_and(m == m0);
+    const bool same = __syncthreads_and(sum.m == m0 && sum.fine_to > -INFINITY);
     if (same && tid < n) {
         const float x = logit_of(kept[tid]);
-        sum += exp((double)x - (double)m) - (double)weight(x, m);
+        sum.sum += exp((double)x - sum.m) - (double)weight(x, sum.c);
     }
-    float top = m;
+    double top = sum.m;
 #pragma unroll
-    for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+    for (int d = 16; d; d /= 2) top = fmax(top, __shfl_xor_sync(~0u, top, d));
     if (lane == 0) warp_m[tid / 32] = top;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, warp_m[w]);
-    if (top != m) sum *= exp((double)m - (double)top);
+    for (int w = 0; w < kWarps; ++w) top = fmax(top, warp_m[w]);
+    if (top != sum.m) sum.sum *= exp(sum.m - top);
 #pragma unroll
-    for (int d = 16; d; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
-    if (lane == 0) warp_sum[tid / 32] = sum;
+    for (int d = 16; d; d /= 2) sum.sum += __shfl_xor_sync(~0u, sum.sum, d);
+    if (lane == 0) warp_sum[tid / 32] = sum.sum;
     __syncthreads();
     if (tid == 0) {
-        sum = 0.;
-        for (int w = 0; w < kWarps; ++w) sum += warp_sum[w];
-        *reinterpret_cast<Part*>(out) = Part{sum, top, 0};
+        double all = 0.;
+        for (int w = 0; w < kWarps; ++w) all += warp_sum[w];
+        *reinterpret_cast<Part*>(out) = Part{all, top};
     }
     for (int i = tid; i < p.count; i += kThreads) reinterpret_cast<Key*>(out + sizeof(Part))[i] = i < n ? kept[i] : 0ull;
 }
@@ -412,7 +432,7 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamArgs a) {
     for (int b = warp; b < p.beams; b += kPickWarps) {
         const unsigned char* const mine = parts + (size_t)b * a.ranges * stride;
         float top = -INFINITY;
-        Part part = {0., -INFINITY, 0};
+        Part part = {0., 0.};
         for (int r = lane; r < a.ranges; r += 32) {
             const Key k = *reinterpret_cast<const Key*>(mine + r * stride + sizeof(Part));
             if (r == lane) part = *reinterpret_cast<const Part*>(mine + r * stride);
@@ -423,7 +443,7 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamArgs a) {
         double sum = 0.;
         for (int r = lane; r < a.ranges; r += 32) {
             if (r != lane) part = *reinterpret_cast<const Part*>(mine + r * stride);
-            if (part.sum > 0.) sum += part.sum * exp((double)part.m - (double)top);
+            if (part.sum > 0.) sum += part.sum * exp(part.m - (double)top);
         }
 #pragma unroll
         for (int d = 16; d; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
@@ -577,7 +597,7 @@ int check(const OgleBeamParams* p) {
 void split(const OgleBeamParams* p, int& range, int& ranges) {
     const int n = p->dtype == OGLE_F32 ? 4 : 8, batch = kThreads * kVecs * n;
     const long batches = div_up((long)p->vocab + n - 1, batch), rows = (long)p->n_groups * p->beams;
-    long blocks = rows > 0 ? 4L * kNumSMs / rows : 1;
+    long blocks = rows > 0 ? 3L * kNumSMs / rows : 1;
     if (blocks < 1) blocks = 1;
     const long each = batches > 0 ? div_up(batches, blocks) : 1;
     range = int(each * batch);
