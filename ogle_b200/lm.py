@@ -207,18 +207,20 @@ def beam_step(logits, scores, beams, count, ends=None):
     if beams < 1 or rows % beams != 0:
         raise ValueError(f"{rows} rows are no whole groups of {beams} beams")
     groups = rows // beams
-    score, next_score = logits.new_empty(groups, count, dtype=_F32), logits.new_empty(rows, dtype=_F32)
-    found, following = logits.new_empty(2, groups, count, dtype=_I32), logits.new_empty(2, rows, dtype=_I32)
-    beam, token = found.unbind(0)
-    next_row, next_token = following.unbind(0)
+    # one allocation for all six (a view is 1.1 us, an allocation 1.5)
+    n = groups * count
+    out = logits.new_empty(3 * (n + rows), dtype=_I32)
+    at = out.data_ptr()
     p = _BEAM(groups, beams, vocab, count, _DTYPE[logits.dtype], ends.numel() if ends is not None else 0, logits.stride(0) if rows > 1 else vocab,
-              logits.data_ptr(), _vector(scores, _F32, rows, "scores"), _vector(ends, _I32, None, "ends"), score.data_ptr(), beam.data_ptr(),
-              token.data_ptr(), next_row.data_ptr(), next_token.data_ptr(), next_score.data_ptr())
+              logits.data_ptr(), _vector(scores, _F32, rows, "scores"), _vector(ends, _I32, None, "ends"), at, at + 4 * n, at + 8 * n,
+              at + 12 * n, at + 12 * n + 4 * rows, at + 12 * n + 8 * rows)
     lib = _lib.cuda_lib()
-    n = lib.ogle_cuda_beam_step_workspace_bytes(p)
-    workspace = logits.new_empty(max(n, 16), dtype=torch.uint8)
-    check(lib.ogle_cuda_beam_step(p, workspace.data_ptr(), n, _stream()), "beam_step")
-    return score, beam, token, next_row, next_token, next_score
+    size = lib.ogle_cuda_beam_step_workspace_bytes(p)
+    workspace = logits.new_empty(max(size, 16), dtype=torch.uint8)
+    check(lib.ogle_cuda_beam_step(p, workspace.data_ptr(), size, _stream()), "beam_step")
+    shape, stride, out32 = (groups, count), (count, 1), out.view(_F32)
+    return (out32.as_strided(shape, stride), out.as_strided(shape, stride, n), out.as_strided(shape, stride, 2 * n),
+            out.as_strided((rows,), (1,), 3 * n), out.as_strided((rows,), (1,), 3 * n + rows), out32.as_strided((rows,), (1,), 3 * n + 2 * rows))
 
 
 def advance_pages(block_table, kv_len, parent, new, refs, page_tokens, blocks=None):
@@ -243,8 +245,9 @@ def advance_pages(block_table, kv_len, parent, new, refs, page_tokens, blocks=No
     size = lib.ogle_cuda_advance_pages_workspace_bytes(p)
     workspace = refs.new_empty(size // 4 + 1)
     check(lib.ogle_cuda_advance_pages(p, workspace.data_ptr(), size, _stream()), "advance_pages")
-    table, length, copies, new_refs, state = out.split([n * blocks, n, 3 * n, pages, 2])
-    return table.view(n, blocks), length, new_refs, copies.view(n, 3), state
+    at = n * blocks
+    return (out.as_strided((n, blocks), (blocks, 1)), out.as_strided((n,), (1,), at), out.as_strided((pages,), (1,), at + 4 * n),
+            out.as_strided((n, 3), (3, 1), at + n), out.as_strided((2,), (1,), at + 4 * n + pages))
 
 
 def compact_pages(block_table, refs, most, page_tokens):
@@ -260,8 +263,9 @@ def compact_pages(block_table, refs, most, page_tokens):
     size = lib.ogle_cuda_compact_pages_workspace_bytes(p)
     workspace = refs.new_empty(size // 4 + 1)
     check(lib.ogle_cuda_compact_pages(p, workspace.data_ptr(), size, _stream()), "compact_pages")
-    table, new_refs, copies, state = out.split([seqs * blocks, pages, 3 * most, 2])
-    return table.view(seqs, blocks), new_refs, copies.view(most, 3), state
+    at = seqs * blocks
+    return (out.as_strided((seqs, blocks), (blocks, 1)), out.as_strided((pages,), (1,), at), out.as_strided((most, 3), (3, 1), at + pages),
+            out.as_strided((2,), (1,), at + pages + 3 * most))
 
 
 def copy_pages(caches, copies, bounds=None):
