@@ -407,53 +407,116 @@ __global__ void __launch_bounds__(kThreads) compact_table_kernel(CompactArgs a) 
 }
 
 // ---- copies
+// A window of copies is shared out among the blocks (., y): each adds up how many units its copies have - many have nothing to copy, others a
+// token or a page -, and its warps take every so-many-th unit. (A warp to every unit that there could be: 512 texts with 200 copies of
+// half a page in four layers, 107 MB, 30 us; 16 so.)
 constexpr int kMostLayers = 64;                  // of a launch
-constexpr int kUnit = 4096;                      // bytes that a warp copies at a time: 8 x 16 a lane
+constexpr int kWindow = 1024;                    // copies that a block looks over
 struct CopyArgs {
     int n_copies, n_layers, kv_heads, dim, page_tokens, n_pages;
     long long page_stride, head_stride, token_stride;
     const int* copies;
-    int unit_rows, units;                        // rows (a token of a head) of a unit; units of a page
+    int unit_rows;                               // rows (a token of a head) of a unit
     int packed;                                  // a page's bytes lie in one piece
     OglePageTensors layer[kMostLayers];
 };
+struct Entry { int src, dst, tokens; };
+__device__ __forceinline__ Entry entry_at(const CopyArgs& a, int c) {
+    const int* const e = a.copies + 3LL * c;
+    Entry x = {__ldg(e), __ldg(e + 1), min(max(__ldg(e + 2), 0), a.page_tokens)};
+    if (!is_page(x.src, a.n_pages) || !is_page(x.dst, a.n_pages) || x.src == x.dst) x.src = -1;
+    return x;
+}
 
-// A warp has a unit of one page's keys or values in one layer; that of the page's first unit its scales, too. A unit's loads are under way
-// together, and the units of an SM's warps: 96 KB and more.
-__global__ void __launch_bounds__(kThreads) copy_pages_kernel(const __grid_constant__ CopyArgs a) {
-    const int lane = threadIdx.x & 31;
+// The window's copies; first[i]: units of those before the i-th; returns all copies'. A whole block of kN threads.
+template <int kN, typename F>
+__device__ __forceinline__ int sum_units(const CopyArgs& a, int* first, Entry* entries, F units) {
+    __shared__ int sums[kN / 32];
+    constexpr int kMine = kWindow / kN;
+    const int tid = threadIdx.x, lane = tid & 31, c0 = blockIdx.y * kWindow, n = min(kWindow, a.n_copies - c0);
+    int mine[kMine], all_mine = 0;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {            // (neighbours read neighbours: thread t has entries t, t + kN, ...)
+        const int c = i * kN + tid;
+        mine[i] = 0;
+        if (c < n) {
+            const Entry e = entry_at(a, c0 + c);
+            entries[c] = e;
+            if (e.src >= 0) mine[i] = units(e);
+        }
+        first[c] = mine[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+        mine[i] = first[tid * kMine + i];
+        all_mine += mine[i];
+    }
+    int sum = all_mine;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const int o = __shfl_up_sync(~0u, sum, d);
+        if (lane >= d) sum += o;
+    }
+    if (lane == 31) sums[tid / 32] = sum;
+    __syncthreads();
+    int total = 0;
+#pragma unroll
+    for (int w = 0; w < kN / 32; ++w) {
+        if (w < tid / 32) sum += sums[w];
+        total += sums[w];
+    }
+    int at = sum - all_mine;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+        first[tid * kMine + i] = at;
+        at += mine[i];
+    }
+    __syncthreads();
+    return total;
+}
+__device__ __forceinline__ int copy_of(const int* first, int unit) {       // the last copy that begins at or before it
+    int lo = 0, hi = kWindow;
+#pragma unroll 1
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (first[mid] <= unit) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// A warp has a unit of one page's keys or values in one layer, by loads and stores of 16 bytes; that of a page's first unit takes its scales,
+// too. 8192 pages of 3 KB in four layers, 403 MB: 72 us, 85 % of what a copy reaches. (Runs of up to 4 KB through shared memory by the copy
+// engine, 48 of an SM under way: 80 us; half a unit loaded while the last one is stored: no gain from 64 registers on.)
+constexpr int kUnit = 4096;                      // bytes of a unit: 8 x 16 a lane
+constexpr int kCopyBlocks = 4;                   // that fit an SM at once
+__global__ void __launch_bounds__(kThreads, kCopyBlocks) copy_pages_kernel(const __grid_constant__ CopyArgs a) {
+    __shared__ int first[kWindow];
+    __shared__ Entry entries[kWindow];
+    const int tid = threadIdx.x, lane = tid & 31;
     grid_dependency_trigger();
     grid_dependency_wait();
-    const long long all = (long long)a.n_copies * a.n_layers * 2 * a.units, step = (long long)gridDim.x * (kThreads / 32);
-    for (long long u = (long long)blockIdx.x * (kThreads / 32) + threadIdx.x / 32; u < all; u += step) {
-        // neighbours in a block: the units of a page, then keys and values, then layers, so that a copy's entry is read from near
-        const int unit = int(u % a.units);
-        const long long rest = u / a.units;
-        const int kind = int(rest & 1), layer = int((rest >> 1) % a.n_layers), c = int((rest >> 1) / a.n_layers);
-        const int src = __ldg(a.copies + 3 * c), dst = __ldg(a.copies + 3 * c + 1), tokens = min(__ldg(a.copies + 3 * c + 2), a.page_tokens);
-        if ((unsigned)src >= (unsigned)a.n_pages || (unsigned)dst >= (unsigned)a.n_pages || src == dst) continue;
-        const OglePageTensors& t = a.layer[layer];
+    const int total = sum_units<kThreads>(a, first, entries, [&](const Entry& e) { return max((a.kv_heads * e.tokens + a.unit_rows - 1) / a.unit_rows, 1); });
+    const int all = total * a.n_layers * 2, step = gridDim.x * (kThreads / 32), vecs = a.dim / 16;
+    const float by_vecs = 1.f / float(vecs);
+    for (int u = blockIdx.x * (kThreads / 32) + tid / 32; u < all; u += step) {
+        const int which = u / total, kind = which & 1, of = u - which * total;
+        const int c = copy_of(first, of);
+        const Entry e = entries[c];
+        const int src = e.src, dst = e.dst, tokens = e.tokens, unit = of - first[c];
+        const OglePageTensors& t = a.layer[which >> 1];
         unsigned char* const base = static_cast<unsigned char*>(kind ? t.v : t.k);
         const unsigned char* const from = base + src * a.page_stride;
         unsigned char* const to = base + dst * a.page_stride;
-        if (unit == 0) {
-            float* const scale = kind ? t.v_scale : t.k_scale;
-            for (int h = lane; h < a.kv_heads; h += 32) scale[(long long)dst * a.kv_heads + h] = scale[(long long)src * a.kv_heads + h];
-            if (kind == 0 && t.bounds) {
-                const long long bytes = 2LL * a.kv_heads * a.dim;
-                const uint4* const f = reinterpret_cast<const uint4*>(t.bounds + src * bytes);
-                uint4* const g = reinterpret_cast<uint4*>(t.bounds + dst * bytes);
-                for (int i = lane; i < bytes / 16; i += 32) g[i] = f[i];
-                for (int h = lane; h < a.kv_heads; h += 32)
-                    t.bounds_scale[(long long)dst * a.kv_heads + h] = t.bounds_scale[(long long)src * a.kv_heads + h];
-            }
-        }
-        if (tokens <= 0) continue;
-        const int vecs = a.dim / 16, rows = min(a.kv_heads * tokens - unit * a.unit_rows, a.unit_rows), n = rows * vecs;
-        if (n <= 0) continue;
+        // a head's scale to a lane, under way with the rest
+        float* const scales = kind ? t.v_scale : t.k_scale;
+        float scale = 0.f;
+        if (unit == 0 && lane < a.kv_heads) scale = scales[(long long)src * a.kv_heads + lane];
+        const int rows = min(a.kv_heads * tokens - unit * a.unit_rows, a.unit_rows), n_vecs = rows * vecs;
         const bool whole = a.packed && tokens == a.page_tokens;
         // quotients by reciprocals: of i below 256 x 16 exactly, of rows (2^22 at most) within one
-        const float by_vecs = 1.f / float(vecs), by_tokens = 1.f / float(tokens);
+        const float by_tokens = 1.f / float(max(tokens, 1));
         const auto offset = [&](int i) {
             if (whole) return (long long)unit * a.unit_rows * a.dim + i * 16LL;
             const int r = int((float(i) + 0.5f) * by_vecs), row = unit * a.unit_rows + r;
@@ -463,14 +526,24 @@ __global__ void __launch_bounds__(kThreads) copy_pages_kernel(const __grid_const
             return h * a.head_stride + t * a.token_stride + (i - r * vecs) * 16LL;
         };
         constexpr int U = 8;
-        for (int i0 = lane; i0 < n; i0 += 32 * U) {
+        for (int i0 = lane; i0 < n_vecs; i0 += 32 * U) {
             uint4 v[U];
 #pragma unroll
             for (int x = 0; x < U; ++x)
-                if (i0 + x * 32 < n) v[x] = *reinterpret_cast<const uint4*>(from + offset(i0 + x * 32));
+                if (i0 + x * 32 < n_vecs) v[x] = *reinterpret_cast<const uint4*>(from + offset(i0 + x * 32));
 #pragma unroll
             for (int x = 0; x < U; ++x)
-                if (i0 + x * 32 < n) *reinterpret_cast<uint4*>(to + offset(i0 + x * 32)) = v[x];
+                if (i0 + x * 32 < n_vecs) *reinterpret_cast<uint4*>(to + offset(i0 + x * 32)) = v[x];
+        }
+        if (unit > 0) continue;
+        if (lane < a.kv_heads) scales[(long long)dst * a.kv_heads + lane] = scale;
+        for (int h = lane + 32; h < a.kv_heads; h += 32) scales[(long long)dst * a.kv_heads + h] = scales[(long long)src * a.kv_heads + h];
+        if (kind == 0 && t.bounds) {
+            const long long bytes = 2LL * a.kv_heads * a.dim;
+            const uint4* const f = reinterpret_cast<const uint4*>(t.bounds + src * bytes);
+            uint4* const g = reinterpret_cast<uint4*>(t.bounds + dst * bytes);
+            for (int i = lane; i < bytes / 16; i += 32) g[i] = f[i];
+            for (int h = lane; h < a.kv_heads; h += 32) t.bounds_scale[(long long)dst * a.kv_heads + h] = t.bounds_scale[(long long)src * a.kv_heads + h];
         }
     }
 }
@@ -604,13 +677,19 @@ int ogle_cuda_copy_pages(const OgleCopyPagesParams* p, const OglePageTensors* la
     a.page_stride = p->page_stride; a.head_stride = p->head_stride; a.token_stride = p->token_stride;
     a.copies = p->copies;
     a.unit_rows = kUnit / p->head_dim;
-    a.units = div_up((long)p->kv_heads * p->page_tokens, a.unit_rows);
     a.packed = p->token_stride == p->head_dim && p->head_stride == p->token_stride * p->page_tokens;
+    const long most_units = div_up((long)p->kv_heads * p->page_tokens, a.unit_rows);
+    // a window's units are counted in 32 bits, its windows in a grid's second dimension
+    if (most_units * kWindow * kMostLayers * 2 >= (1L << 31) || p->n_copies > 65535 * kWindow) return OGLE_ERR_UNSUPPORTED;
     for (int first = 0; first < p->n_layers; first += kMostLayers) {
         a.n_layers = p->n_layers - first < kMostLayers ? p->n_layers - first : kMostLayers;
         for (int l = 0; l < a.n_layers; ++l) a.layer[l] = layers_host_array[first + l];
-        const long warps = (long)a.n_copies * a.n_layers * 2 * a.units;
-        const cudaError_t e = launch_overlapped(copy_pages_kernel, dim3(grid_for(warps * 32, kThreads)), dim3(kThreads), 0, stream, a);
+        // one round of blocks for all windows
+        const long windows = div_up(p->n_copies, kWindow), units = (long)(p->n_copies < kWindow ? p->n_copies : kWindow) * a.n_layers * 2 * most_units;
+        const long at_once = div_up(kNumSMs * kCopyBlocks, windows);
+        long blocks = div_up(units, kThreads / 32);
+        if (blocks > at_once) blocks = at_once;
+        const cudaError_t e = launch_overlapped(copy_pages_kernel, dim3((unsigned)blocks, (unsigned)windows), dim3(kThreads), 0, stream, a);
         if (e != cudaSuccess) return failed(e);
         const int rc = finish_launch();
         if (rc != OGLE_OK) return rc;
