@@ -165,6 +165,7 @@ struct Segment {
     const int* blocks;                            // chosen pages: of the one row, or ...
     const int2* list;                             // ... of the tile's rows
     int first_row, entries;
+    unsigned all_rows;                            // bits of the tile's rows
 };
 
 // One thread: the next segment of the range; false where there is none.
@@ -226,6 +227,7 @@ __device__ __forceinline__ bool cluster_segment(const AttnArgs& a, Segment& g) {
     if constexpr (kChosen) {
         // keys by their place in the list of pages
         g.first_row = first_row;
+        g.all_rows = ~0u >> (31 - (last_row - first_row));
         g.list = a.lists ? a.lists + (long long)c * a.list_stride : nullptr;
         g.blocks = a.chosen + (g.s.row0 + first_row) * a.chosen_row + g.h * a.chosen_head;
         // (a row's choice may be shorter still: what is behind its end names no page)
@@ -340,14 +342,14 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
         float ks[2] = {0.f, 0.f}, vs[2] = {0.f, 0.f};
         const int in_page = (1 << B.page_shift) - 1;
         int start[2] = {0, 0};                    // chosen pages: a step's first key
-        unsigned seen_by[2] = {0u, 0u};           // and the rows that have chosen its page
+        unsigned seen_by[2] = {0u, 0u};           // and the rows that have chosen its page; none where there is no page
         const auto look_up = [&](int which, int i) {
             int p = -1;
             if (i < count) {
                 const int at = j_begin + (i * kWarps + warp) * kChunk;
                 int block = at >> B.page_shift;
                 if constexpr (kChosen) {
-                    seen_by[which] = ~0u;
+                    seen_by[which] = segment.all_rows;
                     if (segment.list) {
                         const int2 e = segment.list[block];
                         block = e.x;
@@ -359,6 +361,7 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
                     if (block < 0 || block > (segment.s.len - 1) >> B.page_shift) block = -1;
                     start[which] = block < 0 ? 0 : (block << B.page_shift) + (at & in_page);
                     if (block >= 0) p = paged::page_of(B, segment.b, block);
+                    if (p < 0) seen_by[which] = 0u;
                 } else {
                     p = paged::page_of(B, segment.b, block);
                 }
@@ -451,6 +454,19 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
 #pragma unroll
                 for (int x = 0; x < 4; ++x) O[mt][n][x] = 0.f;
 
+        // chosen pages: of this lane's rows, the number in the tile and the first key that is hidden
+        int row_bit[MT][NR], row_hi[MT][NR];
+        if constexpr (kChosen) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int r = 0; r < NR; ++r) {
+                    const int row = min(segment.m0 + mt * (kSplit ? 8 : 16) + r * 8 + r8, segment.m_end - 1) / B.group;
+                    row_bit[mt][r] = row - segment.first_row;
+                    row_hi[mt][r] = span_of(segment.s, row, row, 1, 0).hi;
+                }
+        }
+
         for (int i = 0; i < count; ++i) {
             if ((i & 31) == 0 && i > 0) {
                 page[0] = page[1]; ks[0] = ks[1]; vs[0] = vs[1];
@@ -474,9 +490,9 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
             }
             if (++get == F::kStages) { get = 0; parity ^= 1; }
             const int j0 = kChosen ? __shfl_sync(~0u, start[0], i & 31) : j_begin + (i * kWarps + warp) * kChunk;
-            const unsigned rows_here = kChosen ? __shfl_sync(~0u, seen_by[0], i & 31) : ~0u;
+            const unsigned rows_here = kChosen ? __shfl_sync(~0u, seen_by[0], i & 31) : 0u;
             const float k_scale = __shfl_sync(~0u, ks[0], i & 31), v_scale = __shfl_sync(~0u, vs[0], i & 31);
-            const bool edge = j0 < inner_lo || j0 + kChunk > inner_hi || k_scale == 0.f || rows_here != ~0u;       // 0: no page, or one of zeros
+            const bool edge = j0 < inner_lo || j0 + kChunk > inner_hi || k_scale == 0.f || kChosen && rows_here != segment.all_rows;       // 0: no page, or one of zeros
             // products of queries and keys; rows of parts are put together
             float S[2][MT][4];
 #pragma unroll
@@ -512,15 +528,26 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
                         S[nb][mt][0] += S[nb][mt][2];
                         S[nb][mt][1] += S[nb][mt][3];
                     }
-            if (edge) {
+            if (kChosen && edge) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int r = 0; r < NR; ++r) {
+                        const int end = rows_here >> row_bit[mt][r] & 1 ? row_hi[mt][r] - j0 : 0;
+#pragma unroll
+                        for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+                            for (int y = 0; y < 2; ++y)
+                                if (nb * 8 + key_of<DP>(c4 * 2 + y) >= end) S[nb][mt][2 * r + y] = -INFINITY;
+                    }
+            } else if (edge) {
                 const bool no_page = __shfl_sync(~0u, page[0], i & 31) == nowhere;
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                     for (int r = 0; r < NR; ++r) {
                         const int row = min(segment.m0 + mt * (kSplit ? 8 : 16) + r * 8 + r8, segment.m_end - 1) / B.group;
-                        Span k = span_of(segment.s, row, row, a.causal, a.window);
-                        if (kChosen && !(rows_here >> (row - segment.first_row) & 1)) k.hi = 0;
+                        const Span k = span_of(segment.s, row, row, a.causal, a.window);
 #pragma unroll
                         for (int nb = 0; nb < 2; ++nb)
 #pragma unroll
@@ -618,6 +645,14 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
                 for (int u = 0; u < DP / 32; ++u) {
                     uint32_t w[4];
                     ldmatrix_trans(w, at_v + unit_at<DP>(value_row, 2 * u + (lane >> 4)));
+                    bool look = kEdge;            // for NaNs
+                    if constexpr (kEdge && kChosen) {
+                        // most steps are some row's edge: a byte is a NaN where all its lower bits are set
+                        uint32_t set = 0;
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) set |= (w[y] & 0x7f7f7f7fu) + 0x01010101u;
+                        look = __any_sync(~0u, (set & 0x80808080u) != 0);
+                    }
                     uint32_t v[4][2];
 #pragma unroll
                     for (int y = 0; y < 4; ++y)   // (a key, the next) of the even element, then of the odd one
@@ -627,7 +662,7 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
 #pragma unroll
                         for (int odd = 0; odd < 2; ++odd) {
                             uint32_t b0 = v[2 * y][odd], b1 = v[2 * y + 1][odd];
-                            if (kEdge) {
+                            if (look) {
                                 // a row that does not attend a key has weight 0 for it, and 0 x NaN would still be NaN: NaNs are
                                 // taken out, and counted for the rows that do attend them
                                 const __half2 h0 = *reinterpret_cast<const __half2*>(&b0), h1 = *reinterpret_cast<const __half2*>(&b1);
