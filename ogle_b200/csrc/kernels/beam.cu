@@ -3,11 +3,12 @@
 // One pass over the logits: a block has a range of one row, in batches of 4 x 16 bytes a thread. It sums exp(x - m) for some m near the
 // largest logit and keeps, in shared memory, the logits that may be among its best: those above a border that `count` of them
 // are known to reach. The first border comes from the threads' own maxima: in each of the 8 warps the (count / 8)-th largest, the least of
-// them. Whenever more than a few hundred have gathered, they are ranked and the count-th is the new border. A second, small launch
-// adds the ranges' sums and picks a group's best of the ranges' lists.
+// them. After 1, 2, 4, 8, ... batches what has been kept is ranked, and the count-th is the new border. A second, small launch
+// adds the ranges' sums and picks a group's best of the ranges' lists. What the first has no room or no numbers for - rising rows, NaN,
+// infinities, logits beyond 10^6 - it leaves to the second, which goes over such a range again.
 //
 // Which of two beams' tokens comes first hangs on the logarithms of their sums, to all bits that are left. So the totals are
-// of 64 bits, and the sums nearly: x - m times log2(e) in two parts, exponentials in fp32 - but those of the kept logits, which are most of a
+// of 64 bits, and the sums nearly: exponents in one rounding, exponentials in fp32 - but those of the kept logits, which are most of a
 // peaked row's sum, are put right in 64 bits at the end -, a batch's sum of a thread in fp32, all others in 64.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -22,11 +23,11 @@ constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kVecs = 4;                         // of 16 bytes, a thread's share of a batch
 constexpr int kMostCount = 128, kMostEnds = 1024;
 constexpr int kKept = 1024;                      // logits that a block keeps at most ...
-constexpr int kRankAt = kThreads;                // ... and how many of them are ranked at the end of a batch: one a thread
+constexpr int kRankAt = kThreads;                // ... and how many of them are ranked, once there are more: one a thread
+constexpr int kLook = 8;                         // batches between two looks at that, at most
 constexpr float kLargest = 3.402823466e38f;
-constexpr int kGroup = 4;                        // batches between two looks at what has been kept, at most
 constexpr float kSpread = 40.f;                  // of x above m: sums stay below 2^58 of 2^127
-static_assert(kRankAt + kMostCount <= kKept && kMostCount * 2 <= kKept, "what the slow way adds to the kept");
+constexpr float kTame = 1e6f;                    // logits beyond it are left to the second launch: fp32 has no exponent for x log2(e) - c there
 
 // A logit and its token in one number: the larger logit is the larger number, of equal ones the lower token. 0: none.
 typedef unsigned long long Key;
@@ -42,8 +43,10 @@ __device__ __forceinline__ Key key_of(float x, int token) {
 __device__ __forceinline__ float logit_of(Key k) { return unordered(uint32_t(k >> 32)); }
 __device__ __forceinline__ int token_of(Key k) { return int(~uint32_t(k)); }
 
-// What a block leaves behind - a sum of exp(x - m) -, followed by its `count` best in falling order (0: none).
+// What a block leaves behind - a sum of exp(x - m), or kAgain: the range is to be gone over again -, followed by its `count` best in falling
+// order (0: none).
 struct __align__(16) Part { double sum, m; };
+constexpr double kAgain = -1.;
 __host__ __device__ inline size_t part_bytes(int count) { return sizeof(Part) + ((size_t)count + 1) / 2 * 16; }
 
 struct BeamArgs {
@@ -104,122 +107,60 @@ template <> struct Vec<__nv_bfloat16> {
     }
 };
 
+__device__ __forceinline__ float max_nan(float x, float y) {       // NaN where one is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+    return r;
+}
+// The logits of range r: the row begins `shift` elements behind a 16-byte boundary; a range is whole vectors between such boundaries.
+template <typename T>
+__device__ __forceinline__ void range_of(const BeamArgs& a, const T* row, int r, int& begin, int& end) {
+    const int shift = int(reinterpret_cast<uintptr_t>(row) / sizeof(T)) & (Vec<T>::kN - 1);
+    begin = r * a.range - shift;
+    end = min(begin + a.range, a.p.vocab);
+}
+
 // exp(x - m) as the sums have it: 2^(x log2(e) - c) in one rounding of the exponent, which is small where the weight is large. c is an fp32
 // number, m what it stands for; log2(e) in fp32 makes a weight wrong by 2^-26 of its distance from m.
 constexpr float kLog2e = 1.442695022f;
 __device__ __forceinline__ float weight(float x, float c) { return exp2_fast(fmaf(x, kLog2e, -c)); }
 
-// The kept logits in order: keys[0 .. n) become the `count` largest of them, falling; returns how many there are. All threads.
-__device__ __noinline__ int rank_kept(Key* keys, int n, int count, int* scratch) {
+// The kept logits in order: keys[0 .. n) become the `count` largest of them, falling; returns how many there are. All threads; what has been
+// written to keys is there, and so is the result.
+__device__ __forceinline__ int rank_kept(Key* keys, int n, int count) {
     const int tid = threadIdx.x;
     constexpr int kMine = kKept / kThreads;
     Key mine[kMine];
     int rank[kMine];
-    int there = 0;
-    __syncthreads();
-    if (tid == 0) *scratch = 0;
-    if (tid == 1 && n % 2 == 1) keys[n] = 0ull;
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
         mine[i] = tid + i * kThreads < n ? keys[tid + i * kThreads] : 0ull;
         rank[i] = 0;
-        there += mine[i] != 0;
     }
-    __syncthreads();
-    const ulonglong2* const two = reinterpret_cast<const ulonglong2*>(keys);
     if (n <= kThreads) {
-        if (mine[0])
+        if (mine[0]) {
+            const ulonglong2* const two = reinterpret_cast<const ulonglong2*>(keys);
 #pragma unroll 4
-        for (int j = 0; j < n; j += 2) {
-            const ulonglong2 k = two[j / 2];
-            rank[0] += (k.x > mine[0]) + (k.y > mine[0]);
+            for (int j = 0; j + 1 < n; j += 2) {
+                const ulonglong2 k = two[j / 2];
+                rank[0] += (k.x > mine[0]) + (k.y > mine[0]);
+            }
+            if (n & 1) rank[0] += keys[n - 1] > mine[0];
         }
     } else {
 #pragma unroll 1
-        for (int j = 0; j < n; j += 2) {
-            const ulonglong2 k = two[j / 2];
+        for (int j = 0; j < n; ++j) {
+            const Key k = keys[j];
 #pragma unroll
-            for (int i = 0; i < kMine; ++i) rank[i] += (k.x > mine[i]) + (k.y > mine[i]);
+            for (int i = 0; i < kMine; ++i) rank[i] += k > mine[i];
         }
     }
-    if (there) atomicAdd(scratch, there);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kMine; ++i)
         if (mine[i] && rank[i] < count) keys[rank[i]] = mine[i];
-    const int all = min(*scratch, count);
     __syncthreads();
-    return all;
-}
-
-// Calls f(logit, token) for this thread's share of the logits from t0 to end, from memory: for what is rare.
-template <typename T, typename F>
-__device__ __forceinline__ void each_of(const T* in, int t0, int end, F f) {
-    constexpr int N = Vec<T>::kN;
-#pragma unroll 1
-    for (int t1 = t0 + threadIdx.x * N; t1 < end; t1 += kThreads * N)
-#pragma unroll 1
-        for (int t = max(t1, 0); t < min(t1 + N, end); ++t) {
-            const float x = float(in[t]);
-            if (x > -INFINITY) f(fminf(x, Vec<T>::kMost), t);      // (not of a NaN)
-        }
-}
-
-// A thread's sum of exp(x - m). Logits up to fine_to are added by weight(x, c); above 10^6, where c would not stand for any number near m, none is.
-struct Sum { double sum, m; float c, fine_to; };
-__device__ __forceinline__ void refer_to(Sum& s, float m, float most) {
-    const bool fine = fabsf(m) < 1e6f;
-    s.c = fine ? m * kLog2e : 0.f;
-    s.m = fine ? (double)s.c / (double)kLog2e : (double)m;
-    s.fine_to = fine ? fminf(float(s.m) + kSpread, most) : -INFINITY;
-}
-// This thread's share of a batch that has a NaN, an infinity or logits far above m, or whose m is far from 0.
-template <typename T>
-__device__ __noinline__ Sum rare_sum(const T* in, int t0, int end, Sum s) {
-    float top = -kLargest;
-    each_of(in, t0, end, [&](float x, int) { top = fmaxf(top, x); });
-    if ((double)top - s.m > kSpread) {
-        const double before = s.m;
-        refer_to(s, top, Vec<T>::kMost);
-        s.sum *= exp(before - s.m);
-    }
-    each_of(in, t0, end, [&](float x, int) { s.sum += exp((double)x - s.m); });
-    return s;
-}
-
-// More has passed the border in the batches from t0 to end than there is room for - many equal logits, or a rising row: what came before them
-// in order, then the `count` best of them, whose border is found bit by bit. Returns how many are kept. All threads.
-template <typename T>
-__device__ __noinline__ int keep_best(const T* in, int t0, int end, Key* kept, int* n_kept, int count, int* scratch, int* sums) {
-    const int tid = threadIdx.x;
-    for (int i = tid; i < kKept; i += kThreads)
-        if (token_of(kept[i]) >= t0) kept[i] = 0ull;
-    const int n = rank_kept(kept, kKept, count, scratch);
-    if (tid == 0) *n_kept = n;
-    Key border = 0;
-#pragma unroll 1
-    for (int bit = 63; bit >= 0; --bit) {
-        const Key next = border | 1ull << bit;
-        int c = 0;
-        each_of(in, t0, end, [&](float x, int t) { c += key_of(x, t) >= next; });
-        c = __reduce_add_sync(~0u, c);
-        __syncthreads();
-        if ((tid & 31) == 0) sums[tid / 32] = c;
-        __syncthreads();
-        int all = 0;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) all += sums[w];
-        if (all >= count) border = next;
-    }
-    each_of(in, t0, end, [&](float x, int t) {                     // (fewer than count of them: all that there are)
-        const Key k = key_of(x, t);
-        if (k >= border) {
-            const int at = atomicAdd(n_kept, 1);
-            if (at < kKept) kept[at] = k;
-        }
-    });
-    __syncthreads();
-    return *n_kept;
+    return min(n, count);
 }
 
 template <typename T>
@@ -227,10 +168,9 @@ __global__ void __launch_bounds__(kThreads, 3) beam_rows_kernel(BeamArgs a) {
     using V = Vec<T>;
     constexpr int N = V::kN, kBatch = kThreads * kVecs * N;
     __shared__ __align__(16) Key kept[kKept];
-    __shared__ int n_kept, scratch, sums[kWarps];
-    __shared__ double warp_m[kWarps];
+    __shared__ int n_kept, first_equal;
+    __shared__ double warp_m[kWarps], warp_sum[kWarps];
     __shared__ uint32_t warp_border[kWarps];
-    __shared__ double warp_sum[kWarps];
     const OgleBeamParams& p = a.p;
     const int tid = threadIdx.x, lane = tid & 31, row = blockIdx.y;
     if (tid == 0) n_kept = 0;
@@ -238,15 +178,8 @@ __global__ void __launch_bounds__(kThreads, 3) beam_rows_kernel(BeamArgs a) {
     grid_dependency_wait();
     unsigned char* const out = a.parts + ((size_t)row * a.ranges + blockIdx.x) * part_bytes(p.count);
     const T* const in = static_cast<const T*>(p.logits) + row * p.logits_stride;
-    // the row begins `shift` elements behind a 16-byte boundary; a range is whole vectors between such boundaries
-    const int shift = int(reinterpret_cast<uintptr_t>(in) / sizeof(T)) & (N - 1);
-    const int begin = blockIdx.x * a.range - shift, end = min(begin + a.range, p.vocab);
-    const float score = p.scores ? p.scores[row] : 0.f;
-    if (begin >= end || !(fabsf(score) <= kLargest)) {             // behind the row's end, or of a beam that is none
-        if (tid == 0) *reinterpret_cast<Part*>(out) = Part{0., 0.};
-        for (int i = tid; i < p.count; i += kThreads) reinterpret_cast<Key*>(out + sizeof(Part))[i] = 0ull;
-        return;
-    }
+    int begin, end;
+    range_of<T>(a, in, blockIdx.x, begin, end);
     const auto load = [&](int t0, uint4 (&v)[kVecs]) {
 #pragma unroll
         for (int u = 0; u < kVecs; ++u) {
@@ -261,27 +194,28 @@ __global__ void __launch_bounds__(kThreads, 3) beam_rows_kernel(BeamArgs a) {
             }
         }
     };
-
+    const float score = p.scores ? p.scores[row] : 0.f;
     uint4 v[kVecs];
-    load(begin, v);
-    // The first batch's largest logits of all threads: m, and a border that `count` logits reach.
-    float limit;                                                   // what is above it is kept
-    Sum sum;
-    sum.sum = 0.;
+    if (begin < end) load(begin, v);             // (under way while the score is)
+    if (begin >= end || !(fabsf(score) <= kLargest)) {             // behind the row's end, or of a beam that is none
+        if (tid == 0) *reinterpret_cast<Part*>(out) = Part{0., 0.};
+        for (int i = tid; i < p.count; i += kThreads) reinterpret_cast<Key*>(out + sizeof(Part))[i] = 0ull;
+        return;
+    }
+
+    // The first batch's largest logits of all threads: m, and a border that `count` logits reach. (A NaN is the largest, and its range is gone
+    // over again.)
+    float c, fine_to, limit;                                       // weights are 2^(x log2(e) - c), for logits up to fine_to; what is above limit is kept
+    const auto refer_to = [&](float m) {
+        c = m > -kTame ? m * kLog2e : 0.f;                         // (else nothing but a mask's lowest so far: it has no weight)
+        fine_to = m > -kTame ? fminf(m + kSpread, kTame) : -kTame;
+    };
+    uint32_t border = ~0u;
     {
-        float m = -kLargest;
-        float top = -INFINITY;
+        float top = V::largest(v[0]);
 #pragma unroll
-        for (int u = 0; u < kVecs; ++u) {
-            const float x = V::largest(v[u]);
-            if (x == x) {
-                top = fmaxf(top, x);
-            } else {
-#pragma unroll
-                for (int l = 0; l < N; ++l) top = fmaxf(top, V::at(v[u], l));
-            }
-        }
-        uint32_t mine = ordered(fminf(top, V::kMost) + 0.f), best = 0, nth = 0;
+        for (int u = 1; u < kVecs; ++u) top = max_nan(top, V::largest(v[u]));
+        uint32_t mine = ordered(top + 0.f), best = 0, nth = 0;
         for (int i = 0; i < (p.count + kWarps - 1) / kWarps; ++i) {
             nth = __reduce_max_sync(~0u, mine);
             if (i == 0) best = nth;
@@ -293,102 +227,140 @@ __global__ void __launch_bounds__(kThreads, 3) beam_rows_kernel(BeamArgs a) {
             warp_border[tid / 32] = nth;
         }
         __syncthreads();
-        uint32_t least = ~0u;
+        double m = -kLargest;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-            m = fmaxf(m, float(warp_m[w]));
-            least = min(least, warp_border[w]);
+            m = fmax(m, warp_m[w]);
+            border = min(border, warp_border[w]);
         }
-        // the number below it (below 0 comes -0, which is not less)
-        limit = least > ordered(-INFINITY) ? unordered(least - (least == 0x80000000u ? 2 : 1)) : -INFINITY;
-        refer_to(sum, m, V::kMost);
+        // the number below the border (below 0 comes -0, which is not less)
+        limit = border > ordered(-INFINITY) ? unordered(border - (border == 0x80000000u ? 2 : 1)) : -INFINITY;
+        refer_to(fminf(float(m), V::kMost));
     }
-    const double m0 = sum.m;
-    int group_begin = begin, n = 0;
-    bool full = false;
+    const float c0 = c;
+    double sum = 0.;
+    int n = 0;
+    bool full = false, again = false;
 #pragma unroll 1
     for (int t0 = begin, batch = 0; t0 < end; t0 += kBatch, ++batch) {
         uint4 next[kVecs];
         const bool last = t0 + kBatch >= end;
         if (!last) load(t0 + kBatch, next);
-        float top[kVecs];
-        unsigned long long s = 0ull;
-        const unsigned long long log2e = pair(kLog2e, kLog2e), minus_c = pair(-sum.c, -sum.c);
-        bool fine = true;
+        float top[kVecs], most;
 #pragma unroll
         for (int u = 0; u < kVecs; ++u) {
             top[u] = V::largest(v[u]);
-            fine &= top[u] <= sum.fine_to;
+            most = u == 0 ? top[0] : max_nan(most, top[u]);
+        }
+        if (!(most <= fine_to)) {                                  // far above m, or a NaN: rare
+            if (most <= kTame) {
+                const float before = c;
+                refer_to(most);
+                sum *= exp2((double)before - (double)c);
+            } else {
+                again = true;
+            }
+        }
+        unsigned long long s = 0ull;
+        const unsigned long long log2e = pair(kLog2e, kLog2e), minus_c = pair(-c, -c);
+#pragma unroll
+        for (int u = 0; u < kVecs; ++u)
 #pragma unroll
             for (int l = 0; l < N; l += 2) {
                 float e, f;
                 unpair(fma2(pair(V::at(v[u], l), V::at(v[u], l + 1)), log2e, minus_c), e, f);
                 s = add2(s, pair(exp2_fast(e), exp2_fast(f)));
             }
-        }
-        if (fine) {
-            float e, f;
-            unpair(s, e, f);
-            sum.sum += (double)(e + f);
-        } else {
-            sum = rare_sum(in, t0, min(t0 + kBatch, end), sum);
-        }
+        float e, f;
+        unpair(s, e, f);
+        sum += (double)(e + f);
+        // Kept: what is above the limit. (The second time round - of the first batch, most of which equals the border - of those that equal it
+        // the first 256 tokens', where there are enough of them.)
+        const auto keep = [&](int below) {
 #pragma unroll
-        for (int u = 0; u < kVecs; ++u)
-            if (!(top[u] <= limit)) {                              // (or a NaN among them)
-                unsigned who = 0;
+            for (int u = 0; u < kVecs; ++u)
+                if (top[u] > limit) {
+                    unsigned who = 0;
 #pragma unroll
-                for (int l = 0; l < N; ++l) who |= unsigned(V::at(v[u], l) > limit) << l;
-                while (who) {                                      // most often one
-                    const int l = __ffs(who) - 1;
-                    who &= who - 1;
-                    const int at = atomicAdd(&n_kept, 1);
-                    if (at < kKept) kept[at] = key_of(fminf(V::at_any(v[u], l), V::kMost), t0 + (u * kThreads + tid) * N + l);
-                    full |= at >= kRankAt;
+                    for (int l = 0; l < N; ++l) who |= unsigned(V::at(v[u], l) > limit) << l;
+                    while (who) {                                  // most often one
+                        const int l = __ffs(who) - 1, token = t0 + (u * kThreads + tid) * N + l;
+                        who &= who - 1;
+                        const float x = V::at_any(v[u], l);
+                        if (token >= below && ordered(x + 0.f) == border) continue;
+                        const int at = atomicAdd(&n_kept, 1);
+                        if (at < kKept) kept[at] = key_of(x, token);
+                        full |= at >= kRankAt;
+                    }
                 }
-            }
-        // The first batch's border is a guess: the next one is as high as can be. It is raised when there is twice as much to go by, and as often
-        // as there is much to rank.
+        };
+        keep(0x7fffffff);
+        // The first batch's border is a guess: the next one is as high as can be. It is raised when there is twice as much to go by.
         const bool raise = (batch & (batch + 1)) == 0 || last;
-        if (raise || batch % kGroup == 0) {
+        if (raise || batch % kLook == 0) {
             if (__syncthreads_or(full || raise)) {
                 n = n_kept;
-                if (n > kKept) n = keep_best(in, group_begin, min(t0 + kBatch, end), kept, &n_kept, p.count, &scratch, sums);
-                n = rank_kept(kept, n, p.count, &scratch);
+                if (n > kKept && batch == 0) {
+                    // many equal logits: what 256 tokens have of the border or more
+                    const int below = begin + kThreads * N / 8;
+                    __syncthreads();
+                    if (tid == 0) n_kept = first_equal = 0;
+                    __syncthreads();
+                    if (tid < kThreads / 8) {
+                        int mine = 0;
+#pragma unroll
+                        for (int l = 0; l < N; ++l) mine += V::at(v[0], l) > limit;
+                        atomicAdd(&first_equal, mine);
+                    }
+                    __syncthreads();
+                    keep(first_equal >= p.count ? below : 0x7fffffff);
+                    __syncthreads();
+                    n = n_kept;
+                }
+                if (n > kKept) {                                   // no room: the range is gone over again
+                    again = true;
+                    limit = INFINITY;
+                    n = 0;
+                } else {
+                    n = rank_kept(kept, n, p.count);
+                    // what equals the border later comes behind `count` that do, whose tokens are lower
+                    if (limit < INFINITY) limit = n == p.count ? logit_of(kept[n - 1]) : -INFINITY;
+                }
                 if (tid == 0) n_kept = n;
-                // what equals the border later comes behind `count` that do, whose tokens are lower
-                limit = n == p.count ? logit_of(kept[n - 1]) : -INFINITY;
                 __syncthreads();
             }
-            group_begin = t0 + kBatch;
             full = false;
         }
 #pragma unroll
         for (int u = 0; u < kVecs; ++u) v[u] = next[u];
     }
 
-    // the kept logits' part of the sum in 64 bits, where all threads have the same m
-    const bool same = __syncthreads_and(sum.m == m0 && sum.fine_to > -INFINITY);
-    if (same && tid < n) {
-        const float x = logit_of(kept[tid]);
-        sum.sum += exp((double)x - sum.m) - (double)weight(x, sum.c);
+    // the kept logits' part of the sum in 64 bits, where all threads have the same c
+    const double inverse = 1. / (double)kLog2e;
+    const bool same = __syncthreads_and(c == c0);
+    double top = (double)c * inverse;
+    if (same) {
+        if (tid < n) {
+            const float x = logit_of(kept[tid]);
+            sum += exp((double)x - top) - (double)weight(x, c);
+        }
+    } else {
+#pragma unroll
+        for (int d = 16; d; d /= 2) top = fmax(top, __shfl_xor_sync(~0u, top, d));
+        if (lane == 0) warp_m[tid / 32] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = fmax(top, warp_m[w]);
+        sum *= exp((double)c * inverse - top);
     }
-    double top = sum.m;
 #pragma unroll
-    for (int d = 16; d; d /= 2) top = fmax(top, __shfl_xor_sync(~0u, top, d));
-    if (lane == 0) warp_m[tid / 32] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = fmax(top, warp_m[w]);
-    if (top != sum.m) sum.sum *= exp(sum.m - top);
-#pragma unroll
-    for (int d = 16; d; d /= 2) sum.sum += __shfl_xor_sync(~0u, sum.sum, d);
-    if (lane == 0) warp_sum[tid / 32] = sum.sum;
-    __syncthreads();
+    for (int d = 16; d; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
+    if (lane == 0) warp_sum[tid / 32] = sum;
+    const bool redo = __syncthreads_or(again);
     if (tid == 0) {
         double all = 0.;
         for (int w = 0; w < kWarps; ++w) all += warp_sum[w];
-        *reinterpret_cast<Part*>(out) = Part{all, top};
+        *reinterpret_cast<Part*>(out) = Part{redo ? kAgain : all, top};
     }
     for (int i = tid; i < p.count; i += kThreads) reinterpret_cast<Key*>(out + sizeof(Part))[i] = i < n ? kept[i] : 0ull;
 }
@@ -406,6 +378,98 @@ __device__ __forceinline__ bool better(const Total& x, const Total& y) { return 
 constexpr int kPickThreads = 512, kPickWarps = kPickThreads / 32, kPicked = 1024;
 constexpr int kMostBeams = 1024;
 
+// Goes over a range again, whatever its logits are: their sum in 64 bits; the count-th largest bit by bit, what is above it, and of those that
+// equal it the first. All threads; `found` is theirs to use.
+template <typename T>
+__device__ __noinline__ void again(const BeamArgs& a, const T* row, int r, unsigned char* out, Total* found) {
+    __shared__ double sums[kPickWarps];
+    __shared__ int counts[2][kPickWarps];
+    __shared__ int n_found, before[kPickWarps];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid / 32, count = a.p.count;
+    int begin, end;
+    range_of(a, row, r, begin, end);
+    begin = max(begin, 0);
+    const auto at = [&](int t) {                                   // minus infinity for a NaN
+        const float x = float(row[t]);
+        return x == x ? fminf(x, Vec<T>::kMost) + 0.f : -INFINITY;
+    };
+    float top = -INFINITY;
+#pragma unroll 8
+    for (int t = begin + tid; t < end; t += kPickThreads) top = fmaxf(top, at(t));
+#pragma unroll
+    for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+    __syncthreads();
+    if (lane == 0) sums[warp] = (double)top;
+    __syncthreads();
+    for (int w = 0; w < kPickWarps; ++w) top = fmaxf(top, float(sums[w]));
+    __syncthreads();
+    double sum = 0.;
+    if (top > -INFINITY)
+#pragma unroll 4
+        for (int t = begin + tid; t < end; t += kPickThreads) sum += exp((double)at(t) - (double)top);
+#pragma unroll
+    for (int d = 16; d; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
+    if (lane == 0) sums[warp] = sum;
+    uint32_t border = 0;
+    int more = 0;                                                  // above the border
+    for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t next = border | 1u << bit;
+        int c = 0;
+#pragma unroll 8
+        for (int t = begin + tid; t < end; t += kPickThreads) {
+            const float x = at(t);
+            c += x > -INFINITY && ordered(x) >= next;
+        }
+        c = __reduce_add_sync(~0u, c);
+        if (lane == 0) counts[bit & 1][warp] = c;
+        __syncthreads();
+        int all = 0;
+        for (int w = 0; w < kPickWarps; ++w) all += counts[bit & 1][w];
+        if (all >= count) border = next;
+        else more = all;                                           // (the last one that is too high: the next number above the border)
+    }
+    // in the tokens' order, so that the first come first; at most count of them
+    Key* const keys = reinterpret_cast<Key*>(found);
+    if (tid == 0) n_found = 0;
+    int equal = border ? count - more : 0;
+    if (border == 0) equal = 0;
+    __syncthreads();
+    for (int t0 = begin; t0 < end; t0 += kPickThreads) {
+        const int t = t0 + tid;
+        const float x = t < end ? at(t) : -INFINITY;
+        const uint32_t mine = x > -INFINITY ? ordered(x) : 0u;
+        const bool is = border && mine == border;
+        const unsigned who = __ballot_sync(~0u, is);
+        if (lane == 0) before[warp] = __popc(who);
+        __syncthreads();
+        int place = __popc(who & ((1u << lane) - 1)), all = 0;
+        for (int w = 0; w < kPickWarps; ++w) {
+            if (w < warp) place += before[w];
+            all += before[w];
+        }
+        if (mine > border || is && place < equal) keys[atomicAdd(&n_found, 1)] = key_of(x, t);
+        equal = max(equal - all, 0);
+        __syncthreads();
+    }
+    const int n = n_found;
+    for (int i = tid; i < count; i += kPickThreads) {
+        Key mine = 0ull;
+        int rank = i;
+        if (i < n) {
+            mine = keys[i];
+            rank = 0;
+            for (int j = 0; j < n; ++j) rank += keys[j] > mine;
+        }
+        reinterpret_cast<Key*>(out + sizeof(Part))[rank] = mine;
+    }
+    if (tid == 0) {
+        sum = 0.;
+        for (int w = 0; w < kPickWarps; ++w) sum += sums[w];
+        *reinterpret_cast<Part*>(out) = Part{sum, top > -INFINITY ? (double)top : 0.};
+    }
+    __syncthreads();
+}
+
 __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamArgs a) {
     extern __shared__ double2 beam_terms[];                        // of each beam: its largest logit m, and log sum exp(x - m); then score minus that
     __shared__ Total found[kPicked];
@@ -419,7 +483,7 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamArgs a) {
     if (tid == 0) n_found = 0;
     grid_dependency_trigger();
     grid_dependency_wait();
-    const unsigned char* const parts = a.parts + (size_t)g * p.beams * a.ranges * stride;
+    unsigned char* const parts = a.parts + (size_t)g * p.beams * a.ranges * stride;
     const int lists = p.beams * a.ranges, all = lists * p.count;
     // Candidate i is the (i / lists)-th of list i % lists: the lists' best come first, and neighbours are of different lists.
     const auto key_at = [&](int i, int& list) {
@@ -428,28 +492,46 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamArgs a) {
         return reinterpret_cast<const Key*>(parts + list * stride + sizeof(Part))[place];
     };
     int my_list = 0;
-    const Key my_key = tid < all ? key_at(tid, my_list) : 0ull;    // under way while the sums are added
-    for (int b = warp; b < p.beams; b += kPickWarps) {
-        const unsigned char* const mine = parts + (size_t)b * a.ranges * stride;
-        float top = -INFINITY;
-        Part part = {0., 0.};
-        for (int r = lane; r < a.ranges; r += 32) {
-            const Key k = *reinterpret_cast<const Key*>(mine + r * stride + sizeof(Part));
-            if (r == lane) part = *reinterpret_cast<const Part*>(mine + r * stride);
-            if (k) top = fmaxf(top, logit_of(k));
-        }
+    Key my_key = tid < all ? key_at(tid, my_list) : 0ull;          // under way while the sums are added
+    for (int round = 0; round < 2; ++round) {
+        bool redo = false;
+        for (int b = warp; b < p.beams; b += kPickWarps) {
+            const unsigned char* const mine = parts + (size_t)b * a.ranges * stride;
+            float top = -INFINITY;
+            Part part = {0., 0.};
+            for (int r = lane; r < a.ranges; r += 32) {
+                const Key k = *reinterpret_cast<const Key*>(mine + r * stride + sizeof(Part));
+                if (r == lane) part = *reinterpret_cast<const Part*>(mine + r * stride);
+                if (k) top = fmaxf(top, logit_of(k));
+            }
 #pragma unroll
-        for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-        double sum = 0.;
-        for (int r = lane; r < a.ranges; r += 32) {
-            if (r != lane) part = *reinterpret_cast<const Part*>(mine + r * stride);
-            if (part.sum > 0.) sum += part.sum * exp(part.m - (double)top);
-        }
+            for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+            double sum = 0.;
+            for (int r = lane; r < a.ranges; r += 32) {
+                if (r != lane) part = *reinterpret_cast<const Part*>(mine + r * stride);
+                if (part.sum > 0.) sum += part.sum * exp(part.m - (double)top);
+                redo |= part.sum < 0.;
+            }
 #pragma unroll
-        for (int d = 16; d; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
-        if (lane == 0) beam_terms[b] = make_double2(top, sum > 0. ? log(sum) : 0.);    // no sum: no kept logit either
+            for (int d = 16; d; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
+            redo |= sum == 0. && top > -INFINITY;                  // nothing but a mask's lowest
+            if (lane == 0) beam_terms[b] = make_double2(top, sum > 0. ? log(sum) : (top > -INFINITY ? NAN : 0.));
+        }
+        if (!__syncthreads_or(redo) || round > 0) break;
+        for (int list = 0; list < lists; ++list) {
+            const int b = list / a.ranges;
+            unsigned char* const part = parts + list * stride;
+            const double sum = reinterpret_cast<const Part*>(part)->sum;
+            if (sum < 0. || isnan(beam_terms[b].y)) {              // of a beam without any weight, all ranges
+                const size_t row = (size_t)(g * p.beams + b) * p.logits_stride;
+                if (p.dtype == OGLE_F32) again(a, static_cast<const float*>(p.logits) + row, list - b * a.ranges, part, found);
+                else if (p.dtype == OGLE_F16) again(a, static_cast<const __half*>(p.logits) + row, list - b * a.ranges, part, found);
+                else again(a, static_cast<const __nv_bfloat16*>(p.logits) + row, list - b * a.ranges, part, found);
+            }
+        }
+        __syncthreads();
+        my_key = tid < all ? key_at(tid, my_list) : 0ull;
     }
-    __syncthreads();
     // Two beams of the same logits differ in the last bits of their sums where their rows lie differently to 16 bytes. They count as the same,
     // so that their totals are equal and come in the beams' order; so does what is as near by chance.
     constexpr int kMine = (kMostBeams + kPickThreads - 1) / kPickThreads;

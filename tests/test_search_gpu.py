@@ -88,6 +88,34 @@ def test_beam_step_of_values_that_are_not_finite(dtype):
     assert bool((got[1][2] == -1).all()) and bool((got[3][8:] == -1).all())      # a group without a text
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("vocab", [8000, 30001])
+def test_beam_step_of_logits_behind_a_mask_and_far_apart(vocab, dtype):
+    """Masked for thousands of tokens, then logits of any size; steps upwards by more than an exponential holds; nothing but the lowest."""
+    lowest = torch.finfo(dtype).min
+    g = torch.Generator().manual_seed(9)
+    x = torch.randn(12, vocab, generator=g)
+    x[0, :vocab - 100] = lowest
+    x[1, :vocab - 100] = -math.inf
+    x[2, :vocab - 100] = lowest
+    x[2, vocab - 100:] -= 100
+    x[3, :vocab // 2] = lowest
+    x[3, vocab // 2:] -= 1000
+    x[4] += 50 * (torch.arange(vocab) // (vocab // 7)).float()
+    x[5] -= 50 * (torch.arange(vocab) // (vocab // 7)).float()
+    x[6] = lowest
+    x[7] = lowest
+    x[7, 3] = -20000
+    x[8] *= 10000
+    x[9] = -30000 if dtype == F16 else -2e6
+    x[10] = -30000 if dtype == F16 else -2e6
+    x[10, vocab - 5:] = -0.9e6 if dtype != F16 else -29000
+    x[11] = 65000 if dtype == F16 else 3e7
+    x = x.to(dtype).cuda()
+    scores = -torch.rand(12, generator=g).cuda()
+    ref.check_beam_step(lm.beam_step(x, scores, 1, 6), ref.beam_step(x, scores, 1, 6))
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("shift,stride", [(0, 5003), (1, 5004), (3, 5001), (5, 5008), (7, 6000)])
 def test_beam_step_of_rows_at_any_address(shift, stride, dtype):
