@@ -261,18 +261,19 @@ __global__ void __launch_bounds__(kThreads, 3) beam_rows_kernel(BeamArgs a) {
                 again = true;
             }
         }
-        unsigned long long s = 0ull;
+        unsigned long long s[kVecs];                               // (a sum to a vector: none waits for another)
         const unsigned long long log2e = pair(kLog2e, kLog2e), minus_c = pair(-c, -c);
 #pragma unroll
-        for (int u = 0; u < kVecs; ++u)
+        for (int l = 0; l < N; l += 2)
 #pragma unroll
-            for (int l = 0; l < N; l += 2) {
+            for (int u = 0; u < kVecs; ++u) {
                 float e, f;
                 unpair(fma2(pair(V::at(v[u], l), V::at(v[u], l + 1)), log2e, minus_c), e, f);
-                s = add2(s, pair(exp2_fast(e), exp2_fast(f)));
+                const unsigned long long w = pair(exp2_fast(e), exp2_fast(f));
+                s[u] = l == 0 ? w : add2(s[u], w);
             }
         float e, f;
-        unpair(s, e, f);
+        unpair(add2(add2(s[0], s[1]), add2(s[2], s[3])), e, f);
         sum += (double)(e + f);
         // Kept: what is above the limit. (The second time round - of the first batch, most of which equals the border - of those that equal it
         // the first 256 tokens', where there are enough of them.)
