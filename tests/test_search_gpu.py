@@ -8,7 +8,7 @@ import torch
 
 import lm_checks
 import search_checks as ref
-from ogle_b200 import _lib, lm
+from ogle_b200 import _lib, lm, lm_example
 
 pytestmark = pytest.mark.gpu
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
@@ -641,6 +641,72 @@ def test_two_searches_at_once_on_two_streams():
         torch.cuda.synchronize()
         for a, b in zip(alone, got):
             assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def prompts_of(lengths, vocab, seed=3):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randint(1, vocab, (n,), generator=g).tolist() for n in lengths]
+
+
+def check_pages(search):
+    """The counts are what the table says, and no page that a text writes to is another's."""
+    table, refs, page = search.table.tolist(), search.refs.tolist(), search.page_tokens
+    assert refs == counts([table], len(refs))
+    for row, n in zip(table, search.kv_len.tolist()):
+        assert all(p >= 0 for p in row[:-(-n // page)]) and all(p == -1 for p in row[-(-n // page):])
+        if n % page:
+            assert refs[row[n // page]] == 1
+
+
+@pytest.mark.parametrize("chosen", [0, 3])
+def test_search_scores_are_those_of_the_whole_texts(chosen):
+    """The score of every text that a search has found is the sum of its tokens' log probabilities when it is read as one prompt; and no text of
+    the same length that its step could have had instead scores higher than what was kept."""
+    model = lm_example.Model(layers=2, chosen=chosen)
+    search = lm_example.Search(model, prompts_of([37, 5, 64], model.vocab), 4, pages=120, ends=(7, 11), steps=25)
+    for step in range(20):
+        search.step()
+        check_pages(search)
+        if step % 6 == 5:
+            while int(search.compact(5)[1]):
+                pass
+            check_pages(search)
+    left, ended = search.texts()
+    assert all(len(t) == 4 for t in left)
+    texts = [(g, score, text) for kind in (left, ended) for g, found in enumerate(kind) for score, text in found]
+    for g, score, text in texts:
+        prompt = search.prompts[g]
+        whole = lm_example.Search(model, [prompt + text], 1, pages=40, steps=1)      # fills a cache of its own
+        rows = len(prompt) + len(text)
+        batch = dict(block_table=whole.table, kv_len=whole.kv_len, max_kv_len=whole.most, row_start=ints([0, rows]), max_rows=rows)
+        x = model.rows(torch.tensor(prompt + text).cuda(), whole.caches, batch, whole.bounds)
+        logits = torch.log_softmax(model.logits(x).double(), 1)
+        at = torch.arange(len(prompt) - 1, rows - 1, device="cuda")
+        want = float(logits[at, torch.tensor(text).cuda()].sum())
+        # A value that was stored under a smaller scale first may be another one of the 8-bit numbers, rounded twice, and pages are chosen by them.
+        # What this looks for - a page that is another text's, a copy that was not made - moves a score by units.
+        assert abs(score - want) <= 0.05 * len(text), (score, want)
+
+
+def test_search_with_one_beam_takes_the_likeliest_tokens():
+    model = lm_example.Model(layers=1)
+    prompts = prompts_of([20, 3, 33], model.vocab)
+    search = lm_example.Search(model, prompts, 1, steps=30)
+    answers = lm_example.Answers(model, prompts, repetition=1.0, presence=0.0, frequency=0.0, forbidden=())
+    for _ in range(15):
+        search.step()
+    for _ in range(16):
+        answers.step()
+    assert [found[0][1] for found in search.texts()[0]] == [t[n:] for t, n in zip(answers.texts, answers.prompt_len)]
+
+
+def test_search_without_enough_pages_says_so():
+    model = lm_example.Model(layers=1)
+    search = lm_example.Search(model, prompts_of([30, 30], model.vocab), 4, pages=9, steps=30)
+    for _ in range(20):
+        search.step()
+    with pytest.raises(RuntimeError):
+        search.texts()
 
 
 def test_nothing_waited_in_vain():
