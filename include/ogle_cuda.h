@@ -532,7 +532,8 @@ int ogle_cuda_adjust_logits(const OgleLogitsParams* p, ogle_stream_t stream);
  * none of ends[0 .. n_ends) go on: next_row (the parent's row, g * beams + out_beam), next_token and next_score [n_groups][beams], filled
  * up with -1, -1, minus infinity. (With end tokens a count of 2 * beams is enough for all to go on.)
  * Exponentials are of fp32, but those of the largest logits, and sums of 64 bits: the logarithm of a row's sum is within 2^-22 of its
- * value, most often within 2^-26. `workspace`: as above; what is in it need not outlive the call. */
+ * value, most often within 2^-24. Beams of the same largest logit whose logarithms are as near to each other count as having the same sum.
+ * n_groups * beams is 65535 at most. `workspace`: as above; what is in it need not outlive the call. */
 typedef struct {
     int n_groups, beams, vocab, count;     /* count at most 128 */
     int dtype;                             /* OgleDataType of the logits */
@@ -627,7 +628,8 @@ int ogle_cuda_page_bounds(const OglePagedBatch* batch, signed char* bounds, floa
  * over the head's group of query heads of
  *   sum_d (q_d > 0 ? q_d hi_d : q_d lo_d) * bounds_scale
  * where q are the row's queries as whole numbers, q / s rounded to the nearest (even) and cut at +-127, s the smallest power of two with
- * |q| <= 127 s over the group's heads (infinities and NaN count as 0). All of it is exact in fp32. For attention whose scale is positive. */
+ * |q| <= 127 s over the group's heads (infinities and NaN count as 0). All of it is exact in fp32. For attention whose scale is positive,
+ * and up to 256 query heads to a kv head. `workspace`: 16-byte aligned; nothing in it has to be cleared or kept. */
 typedef struct {
     const void* q;
     long long q_row, q_head;

@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) advance_rows_kernel(AdvanceArg
         }
         if (tid == 0) {
             if (wanted <= 0) { p.copies[3 * i] = p.copies[3 * i + 1] = -1; p.copies[3 * i + 2] = 0; }
-            p.new_len[i] = t.length + max(p.tokens ? __ldg(p.tokens + i) : p.new_tokens, 0);
+            p.new_len[i] = int(min((long long)t.length + max(p.tokens ? __ldg(p.tokens + i) : p.new_tokens, 0), 0x7fffffffLL));
             if (i == 0) {
                 const int all = __ldcg(a.base + p.n_new), granted = min(all, free_pages);
                 atomicAdd(p.state, free_pages - granted);

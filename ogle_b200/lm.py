@@ -187,6 +187,14 @@ def adjust_logits(logits, tokens=None, token_start=None, prompt_len=None, repeti
     return out
 
 
+def _here(t):
+    """The current stream, which is the one of t's device: a call does not go to another."""
+    device = t.get_device()
+    if device != torch.cuda.current_device():
+        raise ValueError(f"tensors of device {device}, but the current one is {torch.cuda.current_device()}")
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
 def _table(t, name):
     """(sequences, blocks, row stride) of a block table."""
     shape, stride = t.shape, t.stride()
@@ -217,7 +225,7 @@ def beam_step(logits, scores, beams, count, ends=None):
     lib = _lib.cuda_lib()
     size = lib.ogle_cuda_beam_step_workspace_bytes(p)
     workspace = logits.new_empty(max(size, 16), dtype=torch.uint8)
-    check(lib.ogle_cuda_beam_step(p, workspace.data_ptr(), size, _stream()), "beam_step")
+    check(lib.ogle_cuda_beam_step(p, workspace.data_ptr(), size, _here(logits)), "beam_step")
     shape, stride, out32 = (groups, count), (count, 1), out.view(_F32)
     return (out32.as_strided(shape, stride), out.as_strided(shape, stride, n), out.as_strided(shape, stride, 2 * n),
             out.as_strided((rows,), (1,), 3 * n), out.as_strided((rows,), (1,), 3 * n + rows), out32.as_strided((rows,), (1,), 3 * n + 2 * rows))
@@ -244,7 +252,7 @@ def advance_pages(block_table, kv_len, parent, new, refs, page_tokens, blocks=No
     lib = _lib.cuda_lib()
     size = lib.ogle_cuda_advance_pages_workspace_bytes(p)
     workspace = refs.new_empty(size // 4 + 1)
-    check(lib.ogle_cuda_advance_pages(p, workspace.data_ptr(), size, _stream()), "advance_pages")
+    check(lib.ogle_cuda_advance_pages(p, workspace.data_ptr(), size, _here(refs)), "advance_pages")
     at = n * blocks
     return (out.as_strided((n, blocks), (blocks, 1)), out.as_strided((n,), (1,), at), out.as_strided((pages,), (1,), at + 4 * n),
             out.as_strided((n, 3), (3, 1), at + n), out.as_strided((2,), (1,), at + 4 * n + pages))
@@ -262,7 +270,7 @@ def compact_pages(block_table, refs, most, page_tokens):
     lib = _lib.cuda_lib()
     size = lib.ogle_cuda_compact_pages_workspace_bytes(p)
     workspace = refs.new_empty(size // 4 + 1)
-    check(lib.ogle_cuda_compact_pages(p, workspace.data_ptr(), size, _stream()), "compact_pages")
+    check(lib.ogle_cuda_compact_pages(p, workspace.data_ptr(), size, _here(refs)), "compact_pages")
     at = seqs * blocks
     return (out.as_strided((seqs, blocks), (blocks, 1)), out.as_strided((pages,), (1,), at), out.as_strided((most, 3), (3, 1), at + pages),
             out.as_strided((2,), (1,), at + pages + 3 * most))
@@ -288,7 +296,7 @@ def copy_pages(caches, copies, bounds=None):
     if copies.dim() != 2 or copies.shape[1] != 3:
         raise ValueError("copies: expected [n, 3]")
     p = _COPY_PAGES(copies.shape[0], len(layers), heads, dim, page_tokens, pages, stride[0], stride[1], stride[2], _vector(copies, _I32, None, "copies"))
-    check(_lib.cuda_lib().ogle_cuda_copy_pages(p, b"".join(layers), _stream()), "copy_pages")
+    check(_lib.cuda_lib().ogle_cuda_copy_pages(p, b"".join(layers), _here(k0)), "copy_pages")
 
 
 def _bounds(bounds, pages, heads, dim):
@@ -309,10 +317,10 @@ def page_bounds(cache, bounds, block_table, kv_len, max_kv_len, row_start=None, 
     """Bounds of the keys in every page that the batch's rows were appended to (ogle_cuda_page_bounds), in place: behind `append`, with its
     batch. choose_pages needs them of all pages that a row may choose."""
     pages, heads, _, dim = cache[0].shape
-    # any count of rows that row_start stays below will do, as any type
-    rows = block_table.shape[0] * (1 if row_start is None else max_rows)
+    # rows are not looked at: of their number a bound will do, and any type
+    rows = block_table.shape[0] if row_start is None else min(block_table.shape[0] * max_rows, (1 << 30) // heads)
     b = _batch(cache, block_table, kv_len, max_kv_len, row_start, max_rows, rows, heads, torch.bfloat16)
-    check(_lib.cuda_lib().ogle_cuda_page_bounds(b, *_bounds(bounds, pages, heads, dim), _stream()), "page_bounds")
+    check(_lib.cuda_lib().ogle_cuda_page_bounds(b, *_bounds(bounds, pages, heads, dim), _here(cache[0])), "page_bounds")
 
 
 def choose_pages(q, cache, bounds, block_table, kv_len, max_kv_len, row_start=None, max_rows=1, count=16, first=1, last=1):
@@ -330,7 +338,7 @@ def choose_pages(q, cache, bounds, block_table, kv_len, max_kv_len, row_start=No
     lib = _lib.cuda_lib()
     n = lib.ogle_cuda_choose_pages_workspace_bytes(b, p)
     workspace = q.new_empty(max(n, 16), dtype=torch.uint8)
-    check(lib.ogle_cuda_choose_pages(b, p, workspace.data_ptr(), n, _stream()), "choose_pages")
+    check(lib.ogle_cuda_choose_pages(b, p, workspace.data_ptr(), n, _here(q)), "choose_pages")
     return chosen
 
 
@@ -359,5 +367,5 @@ def sparse_attention(q, cache, chosen, block_table, kv_len, max_kv_len, row_star
     lib = _lib.cuda_lib()
     n = lib.ogle_cuda_sparse_attention_workspace_bytes(b, p, c)
     workspace = q.new_empty(n, dtype=torch.uint8) if n else None
-    check(lib.ogle_cuda_sparse_attention(b, p, c, workspace.data_ptr() if n else 0, n, _stream()), "sparse_attention")
+    check(lib.ogle_cuda_sparse_attention(b, p, c, workspace.data_ptr() if n else 0, n, _here(q)), "sparse_attention")
     return out, lse

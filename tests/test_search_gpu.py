@@ -29,7 +29,7 @@ def beam_case(groups, beams, vocab, dtype, seed=0, spread=2.0):
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("groups,beams,vocab,count", [
     (1, 1, 1, 1), (1, 4, 7, 8), (3, 2, 255, 4), (2, 3, 4095, 6), (1, 4, 4097, 8), (5, 1, 8192, 2), (2, 5, 8193, 10), (1, 4, 32000, 8),
-    (40, 4, 2001, 8), (3, 8, 50001, 16), (1, 16, 150000, 32), (1, 100, 997, 128), (2, 2, 20, 128), (70, 8, 9001, 16), (1, 2, 129, 64)])
+    (40, 4, 2001, 8), (2, 1024, 301, 128), (3, 8, 50001, 16), (1, 16, 150000, 32), (1, 100, 997, 128), (2, 2, 20, 128), (70, 8, 9001, 16), (1, 2, 129, 64)])
 def test_beam_step(groups, beams, vocab, count, dtype):
     x, scores = beam_case(groups, beams, vocab, dtype)
     ends = [int(x[0].float().argmax()), vocab // 2]
@@ -382,6 +382,7 @@ CHOICES = [
     ([2, 1], [400, 30], 16, 40, 2, 48, 3, 1, 1),              # twenty heads to one
     ([1, 5], [6000, 5000], 16, 4, 4, 64, 64, 1, 1),           # more than 256 pages
     ([2], [2000], 16, 120, 1, 96, 12, 1, 1),
+    ([1, 2], [700, 90], 16, 256, 1, 256, 5, 1, 1),
     ([1], [140000], 16, 2, 1, 16, 96, 1, 1),                  # more than 8192 pages
 ]
 
@@ -707,6 +708,40 @@ def test_search_without_enough_pages_says_so():
         search.step()
     with pytest.raises(RuntimeError):
         search.texts()
+
+
+def test_tensors_of_another_device_than_the_current_one_are_refused(monkeypatch):
+    batch, total = lm_checks.make_batch([1, 1], [50, 20], 16, 2, 64)
+    cache, rest = batch["cache"], batch_only(batch)
+    bounds, q, one = lm.new_bounds(cache), torch.randn(2, 4, 64).cuda(), ints([1, 1])
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    for call in (lambda: lm.beam_step(torch.zeros(2, 9, device="cuda:0"), None, 2, 4), lambda: lm.advance_pages(rest["block_table"], rest["kv_len"], one, 1, one, 16),
+                 lambda: lm.compact_pages(rest["block_table"], one, 4, 16), lambda: lm.copy_pages([cache], torch.zeros(1, 3, dtype=torch.int32, device="cuda:0")),
+                 lambda: lm.page_bounds(cache, bounds, **rest), lambda: lm.choose_pages(q, cache, bounds, **rest),
+                 lambda: lm.sparse_attention(q, cache, torch.zeros(2, 2, 4, dtype=torch.int32, device="cuda:0"), **rest)):
+        with pytest.raises(ValueError):
+            call()
+
+
+def test_bounds_under_bounds_that_are_far_too_wide():
+    """max_rows and max_kv_len say more than 2^30 rows x heads; a batch of few rows of many possible ones."""
+    new, past = [5, 1, 0], [40, 700, 3]
+    batch, total = lm_checks.make_batch(new, past, 16, 2, 64)
+    want, got = lm.new_bounds(batch["cache"]), lm.new_bounds(batch["cache"])
+    lm.page_bounds(batch["cache"], want, **batch_only(batch))
+    wide = batch_only(batch)
+    wide["block_table"] = torch.cat([wide["block_table"], torch.full((3, 5000), -1, dtype=torch.int32, device="cuda")], 1)
+    wide["max_rows"], wide["max_kv_len"] = 400000, 80000
+    lm.page_bounds(batch["cache"], got, **wide)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    q = torch.randn(sum(new), 4, 64, generator=torch.Generator().manual_seed(1)).cuda()
+    bounds = with_bounds(batch, total)
+    narrow = lm.choose_pages(q, batch["cache"], bounds, count=5, **batch_only(batch))
+    wide["max_rows"] = 40
+    assert torch.equal(narrow, lm.choose_pages(q, batch["cache"], bounds, count=5, **wide))
+    a, b = lm.sparse_attention(q, batch["cache"], narrow, **batch_only(batch)), lm.sparse_attention(q, batch["cache"], narrow, **wide)
+    lm_checks.check_attention(a, ref.sparse64(q, batch, total, new, narrow), F32)
+    lm_checks.check_attention(b, ref.sparse64(q, batch, total, new, narrow), F32)
 
 
 def test_nothing_waited_in_vain():
