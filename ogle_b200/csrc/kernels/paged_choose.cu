@@ -127,7 +127,7 @@ struct ChooseArgs {
     int tiles, chunks, chunk_pages;              // tiles of rows that a sequence can have; chunks of pages
 };
 
-constexpr int kScoreWarps = 4;
+constexpr int kWarps = 4;
 constexpr int kStepPages = 8;
 constexpr int kMostSteps = 8;                    // of a warp
 constexpr unsigned kAlways = ~0u;
@@ -172,10 +172,18 @@ __device__ __forceinline__ void load8(const void* q, long long at, int dtype, fl
 // them: of 64 bytes of a head's elements, lane c4 of four has bytes [16 c4, 16 c4 + 16) - the order in which pages are read -, the
 // lower bounds' first, then the upper bounds'. A warp's pages are looked up at once, before anything else, and the bounds of its next
 // eight pages are under way while it multiplies.
+// kFew: rows of few pages, whose keys stay in shared memory and are picked from at once.
+constexpr int kRanked = 256;                     // keys whose ranks are counted one against all
+constexpr int kFewRows = 4, kFewWarps = kRanked / 32;
+__device__ __forceinline__ void pick_by_rank(const unsigned* ranked, int* sums, int n, int* out, int count);
+
+template <int kScoreWarps, bool kFew>
 __global__ void __launch_bounds__(kScoreWarps * 32) choose_score_kernel(ChooseArgs a) {
     extern __shared__ __align__(16) unsigned char queries[];
     __shared__ int tile_score[kScoreWarps][16][kStepPages + 1];
     __shared__ unsigned tops[16];
+    __shared__ __align__(16) unsigned ranked[kFew ? kFewRows : 1][kRanked];
+    __shared__ int sums[kScoreWarps];
     const Batch& B = a.b;
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, c4 = lane & 3, r8 = lane >> 2;
     if (tid < 16) tops[tid] = 0;
@@ -189,7 +197,7 @@ __global__ void __launch_bounds__(kScoreWarps * 32) choose_score_kernel(ChooseAr
     if (r0 >= r1) return;
     const int last_place = min(s.first + r1 - 1, s.len - 1), blocks = last_place >= 0 ? (last_place >> B.page_shift) + 1 : 0;
     const int first_page = chunk * a.chunk_pages, end_page = min(first_page + a.chunk_pages, blocks);
-    if (first_page >= blocks) return;
+    if (!kFew && first_page >= blocks) return;
     // lane l: page l % 8 of the warp's steps l / 8 and l / 8 + 4, ... (a chunk has kMostSteps of them at most)
     int page[kMostSteps / 4];
     float unit[kMostSteps / 4];
@@ -293,16 +301,51 @@ __global__ void __launch_bounds__(kScoreWarps * 32) choose_score_kernel(ChooseAr
                 const int place = s.first + r0 + r, own = min(place, s.len - 1) >> B.page_shift;
                 unsigned key = 0;
                 if (pg >= 0 && place >= 0 && blk <= own) key = blk < a.first || blk > own - a.last ? kAlways : ordered_score(float(best) * u);
-                unsigned* const to_key = a.keys + ((long long)(s.row0 + r0 + r - a.row0) * B.kv_heads + h) * a.stride + blk;
+                unsigned* const to_key = kFew ? ranked[kFew ? r : 0] + blk : a.keys + ((long long)(s.row0 + r0 + r - a.row0) * B.kv_heads + h) * a.stride + blk;
                 *to_key = mt > 0 ? max(*to_key, key) : key;
             }
             __syncwarp();
         }
     }
+    if constexpr (kFew) {
+        static_assert(kScoreWarps == kFewWarps && kMostSteps * kStepPages * kFewWarps >= kRanked, "a thread to a key, all pages in a chunk");
+        __syncthreads();
+        for (int r = 0; r < n_rows; ++r) {
+            const int place = min(s.first + r0 + r, s.len - 1), n = place >= 0 ? (place >> B.page_shift) + 1 : 0, row = s.row0 + r0 + r;
+            // behind the row's own page there are zeros up to whole fours
+            if (tid >= n && tid < (n + 3) / 4 * 4) ranked[r][tid] = 0;
+            __syncthreads();
+            pick_by_rank(ranked[r], sums, n, a.chosen + row * a.chosen_row + h * a.chosen_head, a.count);
+            __syncthreads();
+        }
+    }
 }
 
 // ---- the best
-constexpr int kRanked = 256;                     // keys whose ranks are counted one against all
+// Of at most kRanked keys, each one's rank. A block of as many threads or more; sums: a number to a warp.
+__device__ __forceinline__ void pick_by_rank(const unsigned* ranked, int* sums, int n, int* out, int count) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid / 32;
+    const unsigned mine = tid < n ? ranked[tid] : 0u;
+    int rank = 0;
+    if (mine)
+#pragma unroll 4
+        for (int j = 0; j < n; j += 4) {
+            const uint4 k = *reinterpret_cast<const uint4*>(ranked + j);
+            rank += (k.x > mine || k.x == mine && j < tid) + (k.y > mine || k.y == mine && j + 1 < tid) +
+                    (k.z > mine || k.z == mine && j + 2 < tid) + (k.w > mine || k.w == mine && j + 3 < tid);
+        }
+    const unsigned who = __ballot_sync(~0u, mine && rank < count);
+    if (lane == 0) sums[warp] = __popc(who);
+    __syncthreads();
+    int at = __popc(who & ((1u << lane) - 1)), all = 0;
+    for (int w = 0; w < int(blockDim.x) / 32; ++w) {
+        if (w < warp) at += sums[w];
+        all += sums[w];
+    }
+    if (who >> lane & 1) out[at] = tid;
+    for (int i = all + tid; i < count; i += int(blockDim.x)) out[i] = -1;
+}
+
 constexpr int kHeld = 8;                         // keys that a thread holds
 constexpr int kMostThreads = 1024;
 
@@ -326,25 +369,7 @@ __global__ void __launch_bounds__(kMostThreads) choose_pick_kernel(ChooseArgs a)
     if (n <= kRanked) {
         if (tid < kRanked) ranked[tid] = tid < n ? keys[tid] : 0u;
         __syncthreads();
-        const unsigned mine = tid < kRanked ? ranked[tid] : 0u;
-        int rank = 0;
-        if (mine)
-#pragma unroll 4
-            for (int j = 0; j < n; j += 4) {
-                const uint4 k = *reinterpret_cast<const uint4*>(ranked + j);
-                rank += (k.x > mine || k.x == mine && j < tid) + (k.y > mine || k.y == mine && j + 1 < tid) +
-                        (k.z > mine || k.z == mine && j + 2 < tid) + (k.w > mine || k.w == mine && j + 3 < tid);
-            }
-        const unsigned who = __ballot_sync(~0u, mine && rank < a.count);
-        if (lane == 0) sums[0][warp][0] = __popc(who);
-        __syncthreads();
-        int at = __popc(who & ((1u << lane) - 1)), all = 0;
-        for (int w = 0; w < warps; ++w) {
-            if (w < warp) at += sums[0][w][0];
-            all += sums[0][w][0];
-        }
-        if (who >> lane & 1) out[at] = tid;
-        for (int i = all + tid; i < a.count; i += threads) out[i] = -1;
+        pick_by_rank(ranked, &sums[0][0][0], n, out, a.count);
         return;
     }
     // a thread's pages [i0, i1): kHeld of them in registers, or, of more, whole fours in memory
@@ -421,6 +446,13 @@ long long rows_at_once(const Batch& b) {
     const long long n = kMostKeys / (key_stride(b) * b.kv_heads);
     return n < 1 ? 1 : (n < b.n_rows ? n : b.n_rows);
 }
+int tile_rows(const Batch& b) {
+    const int per = b.group >= 16 ? 1 : 16 / b.group, rows = b.max_rows < b.n_rows ? b.max_rows : b.n_rows;
+    return per < rows ? per : rows;
+}
+size_t query_bytes(const Batch& b) { return size_t(div_up(tile_rows(b) * b.group, 16)) * 2 * div_up(b.dim, 64) * 1024; }
+// Few pages, and few rows to a block: one launch.
+bool few_form(const Batch& b) { return key_stride(b) <= kRanked && tile_rows(b) <= kFewRows && query_bytes(b) <= (32u << 10); }
 int failed(cudaError_t e) {
     set_last_error(e);
     (void)cudaGetLastError();
@@ -453,7 +485,7 @@ int ogle_cuda_page_bounds(const OglePagedBatch* batch, signed char* bounds, floa
 
 size_t ogle_cuda_choose_pages_workspace_bytes(const OglePagedBatch* batch, const OgleChooseParams* p) {
     Batch b;
-    if (!p || paged::translate(batch, b) != OGLE_OK || b.n_seqs == 0 || b.max_rows == 0 || b.max_kv_len == 0) return 0;
+    if (!p || paged::translate(batch, b) != OGLE_OK || b.n_seqs == 0 || b.max_rows == 0 || b.max_kv_len == 0 || few_form(b)) return 0;
     return size_t(rows_at_once(b) * b.kv_heads * key_stride(b)) * sizeof(unsigned);
 }
 
@@ -469,8 +501,8 @@ int ogle_cuda_choose_pages(const OglePagedBatch* batch, const OgleChooseParams* 
     if (!paged::strides_ok(p->q, p->q_row, p->q_head, batch->dtype) || !aligned16(p->bounds)) return OGLE_ERR_ALIGNMENT;
     if (B.group > 256) return OGLE_ERR_UNSUPPORTED;
     if (B.max_rows == 0) return OGLE_OK;
-    // (with a bound of no tokens every choice is empty, and nothing is read or written there)
-    if (B.max_kv_len > 0 && (!workspace || workspace_bytes < ogle_cuda_choose_pages_workspace_bytes(batch, p))) return OGLE_ERR_INVALID;
+    const size_t needed = ogle_cuda_choose_pages_workspace_bytes(batch, p);
+    if (needed > 0 && (!workspace || workspace_bytes < needed)) return OGLE_ERR_INVALID;
     if (!aligned16(workspace)) return OGLE_ERR_ALIGNMENT;
     a.q = p->q; a.q_row = p->q_row; a.q_head = p->q_head;
     a.bounds = p->bounds; a.scale = p->bounds_scale;
@@ -482,6 +514,7 @@ int ogle_cuda_choose_pages(const OglePagedBatch* batch, const OgleChooseParams* 
     const int per = B.group >= 16 ? 1 : 16 / B.group;
     a.tiles = div_up(B.max_rows, per);
     // A chunk is one to eight steps of a block: as many as leave the GPU four blocks an SM.
+    constexpr int kScoreWarps = kWarps;
     const long long tiles = (long long)B.n_seqs * a.tiles * B.kv_heads, steps = div_up(a.stride, kScoreWarps * kStepPages);
     long long each = tiles * steps / (4 * kNumSMs);
     each = each < 1 ? 1 : (each > kMostSteps ? kMostSteps : each);
@@ -489,18 +522,27 @@ int ogle_cuda_choose_pages(const OglePagedBatch* batch, const OgleChooseParams* 
     a.chunks = div_up(a.stride, a.chunk_pages);
     const long long blocks = (long long)B.n_seqs * a.tiles * B.kv_heads * a.chunks, picks = (long long)B.n_seqs * B.max_rows * B.kv_heads;
     if (blocks >= (1LL << 31) || picks >= (1LL << 31)) return OGLE_ERR_UNSUPPORTED;
-    const size_t queries = size_t(div_up(per * B.group, 16)) * 2 * div_up(B.dim, 64) * 1024;
+    const size_t queries = query_bytes(B);
     int threads = div_up(a.stride, kHeld * 32) * 32;
     threads = threads < kRanked ? kRanked : (threads > kMostThreads ? kMostThreads : threads);
-    if (queries > (48u << 10) - 4096) {
-        const cudaError_t e = cudaFuncSetAttribute(choose_score_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(queries));
+    if (few_form(B)) {
+        if (tiles >= (1LL << 31)) return OGLE_ERR_UNSUPPORTED;
+        a.rows = B.n_rows;
+        a.chunks = 1;
+        a.chunk_pages = kRanked;
+        const cudaError_t e = launch_overlapped(choose_score_kernel<kFewWarps, true>, dim3(unsigned(tiles)), dim3(kFewWarps * 32), queries, stream, a);
+        return e == cudaSuccess ? finish_launch() : failed(e);
+    }
+    const auto score = choose_score_kernel<kWarps, false>;
+    if (queries > (44u << 10)) {
+        const cudaError_t e = cudaFuncSetAttribute(score, cudaFuncAttributeMaxDynamicSharedMemorySize, int(queries));
         if (e != cudaSuccess) return failed(e);
     }
     const long long at_once = rows_at_once(B);
     for (long long row0 = 0; row0 < B.n_rows; row0 += at_once) {
         a.row0 = int(row0);
         a.rows = int(B.n_rows - row0 < at_once ? B.n_rows - row0 : at_once);
-        cudaError_t e = launch_overlapped(choose_score_kernel, dim3(unsigned(blocks)), dim3(kScoreWarps * 32), queries, stream, a);
+        cudaError_t e = launch_overlapped(score, dim3(unsigned(blocks)), dim3(kScoreWarps * 32), queries, stream, a);
         if (e != cudaSuccess) return failed(e);
         int done = finish_launch();
         if (done != OGLE_OK) return done;

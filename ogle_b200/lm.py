@@ -337,8 +337,8 @@ def choose_pages(q, cache, bounds, block_table, kv_len, max_kv_len, row_start=No
                 count, first, last, 0)
     lib = _lib.cuda_lib()
     n = lib.ogle_cuda_choose_pages_workspace_bytes(b, p)
-    workspace = q.new_empty(max(n, 16), dtype=torch.uint8)
-    check(lib.ogle_cuda_choose_pages(b, p, workspace.data_ptr(), n, _here(q)), "choose_pages")
+    workspace = q.new_empty(n, dtype=torch.uint8) if n else None
+    check(lib.ogle_cuda_choose_pages(b, p, workspace.data_ptr() if n else 0, n, _here(q)), "choose_pages")
     return chosen
 
 

@@ -43,7 +43,8 @@ def test_workspaces_are_asked_for():
     assert lib.ogle_cuda_beam_step_workspace_bytes(C.byref(filled(_lib.BeamParams))) == 0
     assert lib.ogle_cuda_advance_pages_workspace_bytes(C.byref(filled(_lib.AdvanceParams, page_tokens=16))) > 0
     assert lib.ogle_cuda_compact_pages_workspace_bytes(C.byref(filled(_lib.CompactParams, page_tokens=16))) > 0
-    assert lib.ogle_cuda_choose_pages_workspace_bytes(C.byref(batch()), C.byref(filled(_lib.ChooseParams, count=4))) >= 2 * 2 * 7 * 4
+    many = batch(max_kv_len=16000, table_stride=1000)
+    assert lib.ogle_cuda_choose_pages_workspace_bytes(C.byref(many), C.byref(filled(_lib.ChooseParams, count=4))) >= 2 * 2 * 1000 * 4
     for call in ("beam_step", "advance_pages", "compact_pages"):
         assert getattr(lib, f"ogle_cuda_{call}")(None, None, 0, None) == INVALID
 
@@ -104,7 +105,10 @@ def choose(b=None, workspace=SOMEWHERE, size=1 << 40, **more):
     (dict(chosen_head=7), INVALID), (dict(chosen_row=7), INVALID), (dict(q_row=513), ALIGNMENT), (dict(bounds=SOMEWHERE + 8), ALIGNMENT),
     (dict(workspace=None), INVALID), (dict(size=100), INVALID), (dict(workspace=SOMEWHERE + 2), ALIGNMENT)])
 def test_choose_refusals(more, status):
-    assert choose(**more) == status
+    many = batch(max_kv_len=16000, table_stride=1000)
+    assert choose(many, **more) == status
+    if "workspace" not in more and "size" not in more:
+        assert choose(**more) == status
     assert choose(batch(n_seqs=-1)) == INVALID
     assert choose(batch(q_heads=514, kv_heads=2)) == UNSUPPORTED
 

@@ -165,7 +165,8 @@ def counts(tables, pages, held=()):
     return refs
 
 
-@pytest.mark.parametrize("page,pages,seqs,blocks", [(16, 40, 5, 6), (64, 3000, 60, 20), (32, 1025, 33, 7), (16, 70, 1, 30)])
+@pytest.mark.parametrize("page,pages,seqs,blocks", [(16, 40, 5, 6), (64, 3000, 60, 20), (32, 1025, 33, 7), (16, 70, 1, 30), (16, 8192, 24, 40), (16, 8193, 24, 40),
+                                                    (32, 6000, 25, 9)])
 def test_pages_of_texts_that_grow_fork_end_and_are_cut(page, pages, seqs, blocks):
     r = random.Random(pages)
     refs = [0] * pages
@@ -237,7 +238,8 @@ def test_advance_of_nothing():
     assert got[0].tolist() == [[0, 1, -1], [2, 3, -1]] and got[4].tolist() == [1, 0]
 
 
-@pytest.mark.parametrize("pages,seqs,blocks,most", [(50, 4, 5, 100), (50, 4, 5, 3), (2100, 30, 40, 500), (2100, 30, 40, 0), (1024, 1, 1, 5), (3, 1, 3, 3)])
+@pytest.mark.parametrize("pages,seqs,blocks,most", [(50, 4, 5, 100), (50, 4, 5, 3), (2100, 30, 40, 500), (2100, 30, 40, 0), (1024, 1, 1, 5), (3, 1, 3, 3),
+                                                    (8192, 20, 300, 2000), (8193, 20, 300, 2000), (5000, 110, 300, 900)])
 @pytest.mark.parametrize("used", [0.0, 0.3, 0.9, 1.0])
 def test_compact(pages, seqs, blocks, most, used):
     r = random.Random(pages + most)
@@ -382,6 +384,9 @@ CHOICES = [
     ([2, 1], [400, 30], 16, 40, 2, 48, 3, 1, 1),              # twenty heads to one
     ([1, 5], [6000, 5000], 16, 4, 4, 64, 64, 1, 1),           # more than 256 pages
     ([2], [2000], 16, 120, 1, 96, 12, 1, 1),
+    ([1, 1, 1], [4080, 4064, 4095], 16, 8, 2, 64, 100, 1, 1),        # 256 pages, one less, one more
+    ([2, 4, 1], [300, 1000, 7], 16, 20, 1, 80, 9, 1, 1),      # a row to a tile, few pages
+    ([4, 4], [500, 200], 64, 4, 1, 128, 3, 1, 1),             # four rows to a tile
     ([1, 2], [700, 90], 16, 256, 1, 256, 5, 1, 1),
     ([1], [140000], 16, 2, 1, 16, 96, 1, 1),                  # more than 8192 pages
 ]
