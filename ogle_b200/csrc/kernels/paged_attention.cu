@@ -693,6 +693,7 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
             if (n < count) issue(n, (n ^ i) >> 5 ? p1 : p0);
         }
         __syncthreads();                          // every warp is through with its ring: the parts take its place
+        if (kChosen && gave_up && a.cluster <= 1) return;
         if (!kChosen && gave_up && !a.cluster) {
             // the segments that the rest of the range begins get their notes all the same: the join follows whatever stands there
             if (tid == 0 && a.by_segment)
@@ -747,7 +748,7 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
                 sum += q[DP + 1] * f;
                 v.x += o.x * f; v.y += o.y * f; v.z += o.z * f; v.w += o.w * f;
             }
-            if (kChosen || a.cluster) {           // where the first warp's were: no other thread reads them
+            if (a.cluster > 1) {                  // where the first warp's were: no other thread reads them
                 *reinterpret_cast<float4*>(smem + (r * (DP + 4) + d) * 4) = v;
                 if (d == 0) block_sum[r] = make_float2(top, sum);
                 continue;
@@ -759,12 +760,13 @@ paged_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant
             }
             store_row(a, segment.s.row0 + row / B.group, segment.h * B.group + row % B.group, d, v, top, sum);
         }
-        if (kChosen || a.cluster) {
+        if (a.cluster > 1) {
             cluster_meet();
             if (!gave_up) cluster_join<DP>(a, segment, smem, block_sum, kRows);
             cluster_meet();                       // nobody reads this block's part any more
             return;
         }
+        if (kChosen) return;
         // the next segment's copies take the parts' place
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncthreads();
