@@ -2,8 +2,8 @@
 //
 // One pass over the logits: a block has a range of one row, in batches of 4 x 16 bytes a thread. It sums exp(x - m) for some m near the
 // largest logit and keeps, in shared memory, the logits that may be among its best: those above a border that `count` of them
-// are known to reach. The first border comes from the threads' own maxima: in each of the 8 warps the (count / 8)-th largest, the least of
-// them. After 1, 2, 4, 8, ... batches what has been kept is ranked, and the count-th is the new border. A second, small launch
+// are known to reach. The first border comes from the threads' own maxima: in each of the 8 warps the (count / 8)-th largest, where all
+// have logits, the least of them. After 1, 2, 4, 8, ... batches what has been kept is ranked, and the count-th is the new border. A second, small launch
 // adds the ranges' sums and picks a group's best of the ranges' lists. What the first has no room or no numbers for - rising rows, NaN,
 // infinities, logits beyond 10^6 - it leaves to the second, which goes over such a range again.
 //
@@ -171,6 +171,7 @@ __global__ void __launch_bounds__(kThreads, 3) beam_rows_kernel(BeamArgs a) {
     __shared__ int n_kept, first_equal;
     __shared__ double warp_m[kWarps], warp_sum[kWarps];
     __shared__ uint32_t warp_border[kWarps];
+    __shared__ int warp_have[kWarps];
     const OgleBeamParams& p = a.p;
     const int tid = threadIdx.x, lane = tid & 31, row = blockIdx.y;
     if (tid == 0) n_kept = 0;
@@ -215,8 +216,21 @@ __global__ void __launch_bounds__(kThreads, 3) beam_rows_kernel(BeamArgs a) {
         float top = V::largest(v[0]);
 #pragma unroll
         for (int u = 1; u < kVecs; ++u) top = max_nan(top, V::largest(v[u]));
-        uint32_t mine = ordered(top + 0.f), best = 0, nth = 0;
-        for (int i = 0; i < (p.count + kWarps - 1) / kWarps; ++i) {
+        // The k-th largest of each warp, or of all its threads that have a logit: with the least such k of which that is `count` threads.
+        const uint32_t nothing = ordered(-INFINITY);
+        uint32_t mine = ordered(top + 0.f), nth = 0;
+        const int have = __popc(__ballot_sync(~0u, mine > nothing));
+        if (lane == 0) warp_have[tid / 32] = have;
+        __syncthreads();
+        int k = 0, all = 0;
+        while (k < 32 && all < p.count) {
+            ++k;
+            all = 0;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) all += min(warp_have[w], k);
+        }
+        uint32_t best = nothing;
+        for (int i = 0; i < min(k, have); ++i) {
             nth = __reduce_max_sync(~0u, mine);
             if (i == 0) best = nth;
             const unsigned who = __ballot_sync(~0u, mine == nth);
@@ -224,7 +238,7 @@ __global__ void __launch_bounds__(kThreads, 3) beam_rows_kernel(BeamArgs a) {
         }
         if (lane == 0) {
             warp_m[tid / 32] = (double)unordered(best);
-            warp_border[tid / 32] = nth;
+            warp_border[tid / 32] = have > 0 ? nth : ~0u;
         }
         __syncthreads();
         double m = -kLargest;
@@ -234,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, 3) beam_rows_kernel(BeamArgs a) {
             border = min(border, warp_border[w]);
         }
         // the number below the border (below 0 comes -0, which is not less)
-        limit = border > ordered(-INFINITY) ? unordered(border - (border == 0x80000000u ? 2 : 1)) : -INFINITY;
+        limit = all >= p.count ? unordered(border - (border == 0x80000000u ? 2 : 1)) : -INFINITY;
         refer_to(fminf(float(m), V::kMost));
     }
     const float c0 = c;
@@ -561,41 +575,42 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamArgs a) {
         const double2 term = beam_terms[b];
         return Total{ordered(term.y + ((double)logit_of(k) - term.x)), (unsigned long long)b * p.vocab + token_of(k)};
     };
-    // A border that `count` of them reach, by the upper half of the totals' bits: the count-th of the threads' best in some warp; of more than
-    // a warp, the (count / 16)-th in each, the least of them.
+    // A border that `count` of them reach, by the upper half of the totals' bits: the count-th of the threads', among which the lists' best are,
+    // bit by bit; or, where the threads have them all and a low border costs little, that of some warp's. (One request of four beams over
+    // 32000 tokens, 256 candidates: 11.2 us on the device with the first, 9.6 with the second.)
     const Total my_total = my_key ? total(my_key, my_list) : Total{0ull, ~0ull};
+    const unsigned upper = unsigned(my_total.value >> 32);
     unsigned border = 0;
-    if (all > 32) {
-        unsigned long long top = my_total.value;
-        for (int i = tid + kPickThreads; i < all; i += kPickThreads) {
-            int list;
-            const Key k = key_at(i, list);
-            if (k) top = max(top, total(k, list).value);
-        }
-        unsigned mine = unsigned(top >> 32), nth = 0;
-        const int of_warp = p.count <= 32 ? p.count : (p.count + kPickWarps - 1) / kPickWarps;
-        for (int i = 0; i < of_warp; ++i) {
+    if (all > kPickThreads || p.count > 16) {
+#pragma unroll 1
+        for (unsigned bit = 1u << 31; bit; bit >>= 1)
+            if (__syncthreads_count(upper >= (border | bit)) >= p.count) border |= bit;
+    } else if (all > 32) {
+        unsigned mine = upper, nth = 0;
+        for (int i = 0; i < p.count; ++i) {
             nth = __reduce_max_sync(~0u, mine);
             const unsigned who = __ballot_sync(~0u, mine == nth);
             if (lane == __ffs(who) - 1) mine = 0;
         }
         if (lane == 0) warp_border[warp] = nth;
         __syncthreads();
-        border = warp_border[0];
-        for (int w = 1; w < kPickWarps; ++w) border = p.count <= 32 ? max(border, warp_border[w]) : min(border, warp_border[w]);
+        for (int w = 0; w < kPickWarps; ++w) border = max(border, warp_border[w]);
     }
     const auto offer = [&](const Total& t) {
-        if (unsigned(t.value >> 32) >= border) {
+        const bool in = unsigned(t.value >> 32) >= border;
+        if (in) {
             const int at = atomicAdd(&n_found, 1);
             if (at < kPicked) found[at] = t;
         }
+        return in;
     };
     if (my_key) offer(my_total);
-    for (int i = tid + kPickThreads; i < all; i += kPickThreads) {
-        int list;
-        const Key k = key_at(i, list);
-        if (k) offer(total(k, list));
-    }
+    // what the threads have not looked at yet, a list to a thread: it falls, and ends where it has fallen below the border
+    for (int list = tid; list < lists && all > kPickThreads; list += kPickThreads)
+        for (int place = list < kPickThreads ? (kPickThreads - list + lists - 1) / lists : 0; place < p.count; ++place) {
+            const Key k = reinterpret_cast<const Key*>(parts + list * stride + sizeof(Part))[place];
+            if (!k || !offer(total(k, list))) break;
+        }
     __syncthreads();
     int n = n_found;
     if (n <= kPicked) {

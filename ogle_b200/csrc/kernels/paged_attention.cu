@@ -216,9 +216,10 @@ __device__ __forceinline__ bool cluster_segment(const AttnArgs& a, Segment& g) {
     g.b = c / (a.by_segment * B.kv_heads);
     g.h = c / a.by_segment % B.kv_heads;
     g.s = few_sequence(a, g.b);
-    g.m0 = rt * kRows;
+    const int tile_rows = kChosen ? a.tile_rows : kRows;
+    g.m0 = rt * tile_rows;
     if (g.m0 >= g.s.n * B.group) return false;
-    g.m_end = min(g.s.n * B.group, g.m0 + kRows);
+    g.m_end = min(g.s.n * B.group, g.m0 + tile_rows);
     const int first_row = g.m0 / B.group, last_row = (g.m_end - 1) / B.group;
     g.keys = span_of(g.s, first_row, last_row, a.causal, a.window);
     g.inner_lo = span_of(g.s, last_row, 0, a.causal, a.window).lo;
@@ -1131,31 +1132,40 @@ size_t few_workspace(const OglePagedBatch* b, const OgleAttentionParams* p) {
     });
 }
 
-// Rows that a tile can have a part of.
-int rows_in_tile(const OglePagedBatch* b, int tile_rows) {
-    const int group = b->q_heads / b->kv_heads;
-    return (tile_rows + group - 2) / group + 1;
-}
-// Attention over chosen pages: segments, and what is kept of the tiles' lists where several rows share a tile.
-struct ChosenShape { long long segments; int tiles, list_stride; size_t lists; };
-ChosenShape chosen_shape(const OglePagedBatch* b, int tile_rows, int count) {
-    ChosenShape c;
-    c.tiles = int(row_tiles_of_all(b, tile_rows));
-    c.segments = (long long)c.tiles * b->n_seqs * b->kv_heads;
-    const int rows = b->max_rows < b->n_rows ? b->max_rows : b->n_rows, in_tile = rows_in_tile(b, tile_rows);
-    c.list_stride = (in_tile < rows ? in_tile : rows) * count;
-    c.lists = rows > 1 ? size_t(c.segments) * (c.list_stride * sizeof(int2) + sizeof(int)) : 0;
-    return c;
-}
-// Blocks to a segment. What is longest is the number of rounds of blocks, each as long as its share of the segment's tiles of 64 keys and
-// what a segment's beginning, end and join are worth.
-int chosen_cluster(const ChosenShape& c, long long tiles, int slots) {
-    int best = 1;
+// Attention over chosen pages: rows of a tile, segments, blocks to a segment, and what is kept of the tiles' lists where several rows share a
+// tile.
+struct ChosenShape { long long segments; int tile_rows, tiles, cluster, list_stride; size_t lists; };
+// What is longest is the number of rounds of blocks, each as long as its share of the segment's tiles of 64 keys and what a segment's
+// beginning, end and join are worth. r rows are taken to choose r^0.45 times the pages of one (neighbours that share half: 4 rows 46 pages
+// of 24 each, 8 rows 60), so that few rows with many pages are spread over more blocks than one tile of them could use.
+ChosenShape chosen_shape(const OglePagedBatch* b, int most_rows, int slots, int count) {
+    const int group = b->q_heads / b->kv_heads, rows = b->max_rows < b->n_rows ? b->max_rows : b->n_rows;
+    const long long pages = ((long long)b->max_kv_len + b->page_tokens - 1) / b->page_tokens;
+    ChosenShape best = {};
     double least = 0;
-    for (int size = 1; size <= 8; ++size) {
-        const double rounds = double((c.segments * size + slots - 1) / slots), cost = rounds * (double((tiles + size - 1) / size) + kSegmentCost + (size > 1 ? 2 : 0));
-        if (size == 1 || cost < least) { best = size; least = cost; }
+    double union_of = 1;                          // r^0.45 for r = 1, 2, 4, ...
+    for (int r = 1; ; r *= 2, union_of *= 1.366) {
+        if (r > 1 && (r * group > most_rows || r / 2 >= rows)) break;
+        const int tile_rows = r * group < most_rows ? r * group : most_rows;
+        ChosenShape c = {};
+        c.tile_rows = tile_rows;
+        c.tiles = int(row_tiles_of_all(b, tile_rows));
+        c.segments = (long long)c.tiles * b->n_seqs * b->kv_heads;
+        const double wanted = count * union_of < double(pages) ? count * union_of : double(pages), tiles = wanted * b->page_tokens / kTileKeys;
+        for (int size = 1; size <= 8; ++size) {
+            const double rounds = double((c.segments * size + slots - 1) / slots), cost = rounds * (tiles / size + kSegmentCost + (size > 1 ? 2 : 0));
+            if (least == 0 || cost < least) {
+                best = c;
+                best.cluster = size;
+                least = cost;
+            }
+        }
     }
+    int in_tile = (best.tile_rows + group - 2) / group + 1;        // rows that a tile can have a part of
+    if (best.tile_rows % group == 0) in_tile = best.tile_rows / group;
+    best.list_stride = (in_tile < rows ? in_tile : rows) * count;
+    // (one row to every tile, none cut: its choice is the list)
+    best.lists = rows > 1 && in_tile > 1 ? size_t(best.segments) * (best.list_stride * sizeof(int2) + sizeof(int)) : 0;
     return best;
 }
 
@@ -1285,7 +1295,7 @@ size_t ogle_cuda_sparse_attention_workspace_bytes(const OglePagedBatch* batch, c
     if (!p || !c || c->count < 1 || paged::translate(batch, b) != OGLE_OK || b.n_seqs == 0 || b.max_rows == 0) return 0;
     return with_form(choose_sparse(batch), [&](auto dp, auto mt, auto split) {
         using F = Form<decltype(dp)::value, decltype(mt)::value, decltype(split)::value>;
-        return chosen_shape(batch, F::kRows, c->count).lists;
+        return chosen_shape(batch, F::kRows, kNumSMs * F::kBlocks, c->count).lists;
     });
 }
 
@@ -1316,11 +1326,10 @@ int ogle_cuda_sparse_attention(const OglePagedBatch* batch, const OgleAttentionP
         constexpr int DP = decltype(dp)::value, MT = decltype(mt)::value;
         constexpr bool kSplit = decltype(split)::value;
         using F = Form<DP, MT, kSplit>;
-        const ChosenShape shape = chosen_shape(batch, F::kRows, c->count);
-        const long long pages = ((long long)a.b.max_kv_len + batch->page_tokens - 1) / batch->page_tokens;
-        const long long tiles = ((c->count < pages ? c->count : pages) * batch->page_tokens + kTileKeys - 1) / kTileKeys;
+        const ChosenShape shape = chosen_shape(batch, F::kRows, kNumSMs * F::kBlocks, c->count);
+        a.tile_rows = shape.tile_rows;
         a.by_segment = shape.tiles;
-        a.cluster = chosen_cluster(shape, tiles, kNumSMs * F::kBlocks);
+        a.cluster = shape.cluster;
         if (shape.segments * a.cluster >= (1LL << 31)) return OGLE_ERR_UNSUPPORTED;
         cudaError_t e = prepare<DP, MT, kSplit, true>();
         CUtensorMap k_map, v_map;
@@ -1333,7 +1342,7 @@ int ogle_cuda_sparse_attention(const OglePagedBatch* batch, const OgleAttentionP
             a.lists = static_cast<int2*>(workspace);
             a.list_len = reinterpret_cast<int*>(a.lists + size_t(shape.segments) * shape.list_stride);
             e = launch_overlapped(merge_choices_kernel, dim3(unsigned((shape.segments + kMergeWarps - 1) / kMergeWarps)), dim3(kMergeWarps * 32), 0, stream, a,
-                                  F::kRows, int(shape.segments));
+                                  shape.tile_rows, int(shape.segments));
             if (e == cudaSuccess) {
                 const int done = finish_launch();
                 if (done != OGLE_OK) return done;

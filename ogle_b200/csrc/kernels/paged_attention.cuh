@@ -32,7 +32,7 @@ struct AttnArgs {
     // rows of the tile that have chosen it, lists of list_stride entries, list_len of them in use
     const int* chosen;
     long long chosen_row, chosen_head;
-    int count, list_stride;
+    int count, list_stride, tile_rows;           // tile_rows: rows x query heads of a group in a tile
     int2* lists;
     int* list_len;
 };

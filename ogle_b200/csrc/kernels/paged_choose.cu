@@ -174,7 +174,7 @@ __device__ __forceinline__ void load8(const void* q, long long at, int dtype, fl
 // eight pages are under way while it multiplies.
 // kFew: rows of few pages, whose keys stay in shared memory and are picked from at once.
 constexpr int kRanked = 256;                     // keys whose ranks are counted one against all
-constexpr int kFewRows = 4, kFewWarps = kRanked / 32;
+constexpr int kFewRows = 4;
 __device__ __forceinline__ void pick_by_rank(const unsigned* ranked, int* sums, int n, int* out, int count);
 
 template <int kScoreWarps, bool kFew>
@@ -308,42 +308,46 @@ __global__ void __launch_bounds__(kScoreWarps * 32) choose_score_kernel(ChooseAr
         }
     }
     if constexpr (kFew) {
-        static_assert(kScoreWarps == kFewWarps && kMostSteps * kStepPages * kFewWarps >= kRanked, "a thread to a key, all pages in a chunk");
+        static_assert(kMostSteps * kStepPages * kScoreWarps >= kRanked, "all pages in a chunk");
         __syncthreads();
         for (int r = 0; r < n_rows; ++r) {
             const int place = min(s.first + r0 + r, s.len - 1), n = place >= 0 ? (place >> B.page_shift) + 1 : 0, row = s.row0 + r0 + r;
             // behind the row's own page there are zeros up to whole fours
-            if (tid >= n && tid < (n + 3) / 4 * 4) ranked[r][tid] = 0;
+            if (tid < 4 && n + tid < (n + 3) / 4 * 4) ranked[r][n + tid] = 0;
             __syncthreads();
             pick_by_rank(ranked[r], sums, n, a.chosen + row * a.chosen_row + h * a.chosen_head, a.count);
-            __syncthreads();
         }
     }
 }
 
 // ---- the best
-// Of at most kRanked keys, each one's rank. A block of as many threads or more; sums: a number to a warp.
+// Of at most kRanked keys, each one's rank. A block's work; sums: a number to a warp.
 __device__ __forceinline__ void pick_by_rank(const unsigned* ranked, int* sums, int n, int* out, int count) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid / 32;
-    const unsigned mine = tid < n ? ranked[tid] : 0u;
-    int rank = 0;
-    if (mine)
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid / 32, threads = blockDim.x;
+    int before = 0;
+    for (int i0 = 0; i0 < n; i0 += threads) {
+        const int i = i0 + tid;
+        const unsigned mine = i < n ? ranked[i] : 0u;
+        int rank = 0;
+        if (mine)
 #pragma unroll 4
-        for (int j = 0; j < n; j += 4) {
-            const uint4 k = *reinterpret_cast<const uint4*>(ranked + j);
-            rank += (k.x > mine || k.x == mine && j < tid) + (k.y > mine || k.y == mine && j + 1 < tid) +
-                    (k.z > mine || k.z == mine && j + 2 < tid) + (k.w > mine || k.w == mine && j + 3 < tid);
+            for (int j = 0; j < n; j += 4) {
+                const uint4 k = *reinterpret_cast<const uint4*>(ranked + j);
+                rank += (k.x > mine || k.x == mine && j < i) + (k.y > mine || k.y == mine && j + 1 < i) +
+                        (k.z > mine || k.z == mine && j + 2 < i) + (k.w > mine || k.w == mine && j + 3 < i);
+            }
+        const unsigned who = __ballot_sync(~0u, mine && rank < count);
+        if (lane == 0) sums[warp] = __popc(who);
+        __syncthreads();
+        int at = before + __popc(who & ((1u << lane) - 1));
+        for (int w = 0; w < threads / 32; ++w) {
+            if (w < warp) at += sums[w];
+            before += sums[w];
         }
-    const unsigned who = __ballot_sync(~0u, mine && rank < count);
-    if (lane == 0) sums[warp] = __popc(who);
-    __syncthreads();
-    int at = __popc(who & ((1u << lane) - 1)), all = 0;
-    for (int w = 0; w < int(blockDim.x) / 32; ++w) {
-        if (w < warp) at += sums[w];
-        all += sums[w];
+        if (who >> lane & 1) out[at] = i;
+        __syncthreads();
     }
-    if (who >> lane & 1) out[at] = tid;
-    for (int i = all + tid; i < count; i += int(blockDim.x)) out[i] = -1;
+    for (int i = before + tid; i < count; i += threads) out[i] = -1;
 }
 
 constexpr int kHeld = 8;                         // keys that a thread holds
@@ -530,7 +534,7 @@ int ogle_cuda_choose_pages(const OglePagedBatch* batch, const OgleChooseParams* 
         a.rows = B.n_rows;
         a.chunks = 1;
         a.chunk_pages = kRanked;
-        const cudaError_t e = launch_overlapped(choose_score_kernel<kFewWarps, true>, dim3(unsigned(tiles)), dim3(kFewWarps * 32), queries, stream, a);
+        const cudaError_t e = launch_overlapped(choose_score_kernel<kWarps, true>, dim3(unsigned(tiles)), dim3(kWarps * 32), queries, stream, a);
         return e == cudaSuccess ? finish_launch() : failed(e);
     }
     const auto score = choose_score_kernel<kWarps, false>;

@@ -125,9 +125,10 @@ def sparse(b=None, workspace=SOMEWHERE, size=1 << 40, choice={}, **more):
     (dict(workspace=SOMEWHERE + 2), ALIGNMENT), (dict(choice=dict(count=1 << 23, chosen_row=1 << 24, chosen_head=1 << 23)), UNSUPPORTED)])
 def test_sparse_refusals(more, status):
     assert sparse(**more) == status
-    # several rows to a sequence: lists
-    assert sparse(batch(n_rows=8, max_rows=4, row_start=SOMEWHERE), workspace=None) == INVALID
-    assert sparse(batch(n_rows=8, max_rows=4, row_start=SOMEWHERE), size=64) == INVALID
+    # several rows to a tile: lists
+    many = batch(n_rows=8000, max_rows=4000, row_start=SOMEWHERE)
+    assert sparse(many, workspace=None) == INVALID
+    assert sparse(many, size=64) == INVALID
     lib = _lib.cuda_lib()
     assert lib.ogle_cuda_sparse_attention(None, None, None, None, 0, None) == INVALID
     assert lib.ogle_cuda_page_bounds(C.byref(batch()), None, SOMEWHERE, None) == INVALID

@@ -38,6 +38,16 @@ def test_beam_step(groups, beams, vocab, count, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("vocab", [500, 1030, 1500, 2047, 8192 + 1100, 4096 + 1300])
+@pytest.mark.parametrize("beams,count", [(1, 1), (4, 40), (2, 128)])
+def test_beam_step_of_batches_that_few_threads_have(beams, count, vocab, dtype):
+    x, scores = beam_case(2, beams, vocab, dtype, seed=6)
+    ref.check_beam_step(lm.beam_step(x, scores, beams, count), ref.beam_step(x, scores, beams, count))
+    x[:, vocab // 9:] = -math.inf
+    ref.check_beam_step(lm.beam_step(x, scores, beams, count), ref.beam_step(x, scores, beams, count))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("vocab", [300, 8192, 70001])
 @pytest.mark.parametrize("kind", ["equal", "rising", "falling", "lowest", "few", "two values"])
 def test_beam_step_of_logits_in_order_and_alike(kind, vocab, dtype):
