@@ -3,9 +3,14 @@
 // One pass over the logits: a block has a range of one row, in batches of 4 x 16 bytes a thread. It sums exp(x - m) for some m near the
 // largest logit and keeps, in shared memory, the logits that may be among its best: those above a border that `count` of them
 // are known to reach. The first border comes from the threads' own maxima: in each of the 8 warps the (count / 8)-th largest, where all
-// have logits, the least of them. After 1, 2, 4, 8, ... batches what has been kept is ranked, and the count-th is the new border. A second, small launch
-// adds the ranges' sums and picks a group's best of the ranges' lists. What the first has no room or no numbers for - rising rows, NaN,
-// infinities, logits beyond 10^6 - it leaves to the second, which goes over such a range again.
+// have logits, the least of them. After 1, 2, 4, 8, ... batches what has been kept is ranked, and the count-th is the new border. A second,
+// small launch adds the ranges' sums and picks a group's best of the ranges' lists. What the first has no room or no numbers for - rising
+// rows, NaN, infinities, logits beyond 10^6 - it leaves to the second, which goes over such a range again (a row of 128000 in some 0.5 ms).
+//
+// Measured: 48 x 8 rows of 128001 in bf16, 98 MB, 16 best: 35 us for the rows, 2.8 TB/s (43 % of a copy), and 5 for the rest. 10 instructions a
+// logit, and 24 warps an SM that wait for one another's: neither memory nor the exponentials (43 % of their unit) are the bound. One
+// request of 4 x 32000 in fp32 takes 10 us on the device, 5 for each launch. (Everything kept at once ranked anew in each batch:
+// 128 us; a call of the rare cases' code from the first launch, whose registers it then took: 80.)
 //
 // Which of two beams' tokens comes first hangs on the logarithms of their sums, to all bits that are left. So the totals are
 // of 64 bits, and the sums nearly: exponents in one rounding, exponentials in fp32 - but those of the kept logits, which are most of a
@@ -336,6 +341,7 @@ __global__ void __launch_bounds__(kThreads, 3) beam_rows_kernel(BeamArgs a) {
                     again = true;
                     limit = INFINITY;
                     n = 0;
+                    __syncthreads();                               // everybody has seen the number
                 } else {
                     n = rank_kept(kept, n, p.count);
                     // what equals the border later comes behind `count` that do, whose tokens are lower
