@@ -1,7 +1,8 @@
 /* ogle_cuda.h - C ABI of the B200 (sm_100a) backend for the OGLE graph runtime's
  * data-parallel hot path: conv2d family with fused bias/BN/activation, gemm,
  * pooling, elementwise, concat, layout conversion and the SSD box decoder and
- * post-process; and the operators of a language model's decoding step.
+ * post-process; and the operators of a language model's decoding step, of beam search over its paged cache, and of attention over
+ * chosen pages of it.
  *
  * The reference runtime (kl456123/OGLE) has no foreign-function interface: each
  * operator's Kernel::Compute binds OpenGL textures and draws. Every entry point
@@ -584,7 +585,7 @@ int ogle_cuda_advance_pages(const OgleAdvanceParams* p, void* workspace, size_t 
 /* Used pages to the front of the pool. With U pages in use (refs not 0), the k-th used page from U on moves to the k-th free one below
  * U, for the first n_copies of them: copies[k] = (page, new page, page_tokens), the rest (-1, -1, 0). The new table names the new pages
  * (new_table may be table), new_refs has their counts (it may not be refs). state[0]: U; state[1]: moves that are left. What is in the pages is
- * ogle_cuda_copy_pages' to move. */
+ * ogle_cuda_copy_pages' to move. Whatever names a page that moves has to be in this table. */
 typedef struct {
     int n_seqs, blocks;
     int page_tokens, n_pages, n_copies, reserved;

@@ -6,7 +6,9 @@
 // implementations of the score agree in every bit. The sum is a product of 8-bit matrices - the query's positive elements with the upper
 // bounds, its negative ones with the lower - for which the cache's layout is the multiply's: a page is a column.
 //
-// Bound by what is launched and looked up where texts are ordinary (64 texts of up to 8000 tokens: 14 MB), by the bounds' bytes else.
+// Bound by latency: sequence, table, page, bounds, one look-up behind the other. 64 texts of up to 8000 tokens, pages of 64, 32 query heads to 8
+// of 128: 7 us for the bounds of the new tokens' pages (4 MB) and 9 for scores and choice (10 MB). Twelve drafts over up to 150000 tokens, pages of 32:
+// 5, 9 for the scores and 9 for the choice.
 #include "paged.cuh"
 
 namespace ogle {

@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) advance_rows_kernel(AdvanceArg
     grid_dependency_wait();
     advance_row<kRowWarps>(a, blockIdx.x);
 }
-// Both, by a cluster of kFewChunks blocks. (4 texts, 400 pages: 11 us on the device in two launches, 8 so.)
+// Both, by a cluster of kFewChunks blocks: a launch less, 2 us of the host's 18 for a call with 4 texts, and on the device 7 us instead of 8.
 __global__ void __launch_bounds__(kThreads) advance_few_kernel(AdvanceArgs a) {
     const int rank = blockIdx.x, rows = max(max(a.p.n_new, a.p.n_old), 1);
     grid_dependency_trigger();
@@ -440,7 +440,7 @@ __global__ void __launch_bounds__(kThreads) compact_table_kernel(CompactArgs a) 
     grid_dependency_wait();
     rename_pages(a);
 }
-// All three, by a cluster of kFewChunks blocks.
+// All three, by a cluster of kFewChunks blocks: 7 us on the device, as in three launches, and 14 us of the host's instead of 18.
 constexpr int kFewItems = 1 << 15;               // of the table and of the copies
 __global__ void __launch_bounds__(kThreads) compact_few_kernel(CompactArgs a) {
     const int rank = blockIdx.x;
@@ -456,7 +456,7 @@ __global__ void __launch_bounds__(kThreads) compact_few_kernel(CompactArgs a) {
 // ---- copies
 // A window of copies is shared out among the blocks (., y): each adds up how many units its copies have - many have nothing to copy, others a
 // token or a page -, and its warps take every so-many-th unit. (A warp to every unit that there could be: 512 texts with 200 copies of
-// half a page in four layers, 107 MB, 30 us; 16 so.)
+// half a page in four layers, 107 MB: 35 us, 20 so.)
 constexpr int kMostLayers = 64;                  // of a launch
 constexpr int kWindow = 1024;                    // copies that a block looks over
 struct CopyArgs {
@@ -534,8 +534,8 @@ __device__ __forceinline__ int copy_of(const int* first, int unit) {       // th
 }
 
 // A warp has a unit of one page's keys or values in one layer, by loads and stores of 16 bytes; that of a page's first unit takes its scales,
-// too. 8192 pages of 3 KB in four layers, 403 MB: 72 us, 85 % of what a copy reaches. (Runs of up to 4 KB through shared memory by the copy
-// engine, 48 of an SM under way: 80 us; half a unit loaded while the last one is stored: no gain from 64 registers on.)
+// too. 8192 pages of 3 KB in four layers, 403 MB: 76 us, 81 % of what a copy reaches. (Runs of up to 4 KB through shared memory by the copy
+// engine, 48 of an SM under way: 80 to 100; half a unit loaded while the last one is stored, in 64 registers: 150.)
 constexpr int kUnit = 4096;                      // bytes of a unit: 8 x 16 a lane
 constexpr int kCopyBlocks = 4;                   // that fit an SM at once
 __global__ void __launch_bounds__(kThreads, kCopyBlocks) copy_pages_kernel(const __grid_constant__ CopyArgs a) {

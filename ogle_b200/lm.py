@@ -1,6 +1,7 @@
 """The operators of a language model's decoding step (include/ogle_cuda.h): keys and values appended to a paged cache held
-in 8 bits, attention over that cache, and the adjustment of logits before a token is chosen. One function per entry point,
-on torch CUDA tensors; torch is used for device memory and the current stream only.
+in 8 bits, attention over that cache or over pages of it that a score chooses, the adjustment of logits before a token is chosen, the step of
+a beam search and the pages' management behind it. One function per entry point, on torch CUDA tensors; torch is used for device
+memory and the current stream only.
 
 The cache is four tensors (k, v, k_scale, v_scale): k and v float8_e4m3fn [pages, kv heads, page tokens, head dim] (any strides
 that keep a token's elements side by side and 16-byte boundaries), one float32 scale for each page and kv head, a power of two, or 0
@@ -12,6 +13,13 @@ last of the kv_len[b] tokens that it has once they are appended. Without row_sta
 max_rows are the host's bounds of what kv_len and row_start hold on the device: nothing here waits for the device. Rows of a sequence
 behind its first max_rows, rows that no sequence has (a padded batch), and tokens from max_kv_len on are ignored: a result made here
 holds what was in memory there.
+
+Pages are managed on the device: refs, int32 [pages], counts the table entries that name each page, 0 where it is free. advance_pages makes
+the block table of the texts that go on from another one (forked, grown, cut, ended, new), copy_pages copies what two of them would
+write to, compact_pages moves used pages to the front. None of them changes its inputs but the caches.
+
+Attention over few pages: page_bounds keeps bounds of every page's keys (new_bounds), choose_pages picks for each row and kv head the pages
+whose keys can have the largest products with its queries, sparse_attention attends those.
 """
 import torch
 
