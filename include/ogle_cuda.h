@@ -599,7 +599,7 @@ int ogle_cuda_compact_pages(const OgleCompactParams* p, void* workspace, size_t 
 /* For each (source page, destination page, tokens) of copies, in every layer's cache: the first `tokens` tokens of all heads, keys and
  * values, and the page's scales - and bounds, where the layer has them. The other slots of the destination stay as they are. An entry that names a
  * page outside the cache is left out. No page may be the destination of two entries, or of one and the source of another.
- * Layers have their pages in the same strides (see OglePagedBatch). */
+ * Layers have their pages in the same strides (see OglePagedBatch); from a page's first byte to its last there are less than 2^36. */
 typedef struct {
     void *k, *v;
     float *k_scale, *v_scale;              /* [n_pages][kv_heads] */

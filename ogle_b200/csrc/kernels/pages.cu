@@ -456,7 +456,7 @@ __global__ void __launch_bounds__(kThreads) compact_few_kernel(CompactArgs a) {
 // ---- copies
 // A window of copies is shared out among the blocks (., y): each adds up how many units its copies have - many have nothing to copy, others a
 // token or a page -, and its warps take every so-many-th unit. (A warp to every unit that there could be: 512 texts with 200 copies of
-// half a page in four layers, 107 MB: 35 us, 20 so.)
+// half a page in four layers, 107 MB: 35 us, 14 so.)
 constexpr int kMostLayers = 64;                  // of a launch
 constexpr int kWindow = 1024;                    // copies that a block looks over
 struct CopyArgs {
@@ -534,10 +534,10 @@ __device__ __forceinline__ int copy_of(const int* first, int unit) {       // th
 }
 
 // A warp has a unit of one page's keys or values in one layer, by loads and stores of 16 bytes; that of a page's first unit takes its scales,
-// too. 8192 pages of 3 KB in four layers, 403 MB: 76 us, 81 % of what a copy reaches. (Runs of up to 4 KB through shared memory by the copy
+// too. 8192 pages of 3 KB in four layers, 403 MB: 71 us, 87 % of what a copy reaches. (Runs of up to 4 KB through shared memory by the copy
 // engine, 48 of an SM under way: 80 to 100; half a unit loaded while the last one is stored, in 64 registers: 150.)
 constexpr int kUnit = 4096;                      // bytes of a unit: 8 x 16 a lane
-constexpr int kCopyBlocks = 4;                   // that fit an SM at once
+constexpr int kCopyBlocks = 2;                   // that fit an SM at once (three, in 85 registers, keep a unit's places in memory: 100 us)
 __global__ void __launch_bounds__(kThreads, kCopyBlocks) copy_pages_kernel(const __grid_constant__ CopyArgs a) {
     __shared__ int first[kWindow];
     __shared__ Entry entries[kWindow];
@@ -562,25 +562,39 @@ __global__ void __launch_bounds__(kThreads, kCopyBlocks) copy_pages_kernel(const
         if (unit == 0 && lane < a.kv_heads) scale = scales[(long long)src * a.kv_heads + lane];
         const int rows = min(a.kv_heads * tokens - unit * a.unit_rows, a.unit_rows), n_vecs = rows * vecs;
         const bool whole = a.packed && tokens == a.page_tokens;
-        // quotients by reciprocals: of i below 256 x 16 exactly, of rows (2^22 at most) within one
-        const float by_tokens = 1.f / float(max(tokens, 1));
-        const auto offset = [&](int i) {
-            if (whole) return (long long)unit * a.unit_rows * a.dim + i * 16LL;
-            const int r = int((float(i) + 0.5f) * by_vecs), row = unit * a.unit_rows + r;
-            int h = int((float(row) + 0.5f) * by_tokens), t = row - h * tokens;
-            if (t < 0) { --h; t += tokens; }
-            if (t >= tokens) { ++h; t -= tokens; }
-            return h * a.head_stride + t * a.token_stride + (i - r * vecs) * 16LL;
-        };
-        constexpr int U = 8;
-        for (int i0 = lane; i0 < n_vecs; i0 += 32 * U) {
+        // places in the page, in 16 bytes
+        constexpr int U = kUnit / 512;
+        const uint4* const in = reinterpret_cast<const uint4*>(from);
+        uint4* const out = reinterpret_cast<uint4*>(to);
+        if (whole) {
+            const uint4* const mine = in + (size_t)unit * a.unit_rows * vecs + lane;
+            uint4* const yours = out + (size_t)unit * a.unit_rows * vecs + lane;
             uint4 v[U];
 #pragma unroll
             for (int x = 0; x < U; ++x)
-                if (i0 + x * 32 < n_vecs) v[x] = *reinterpret_cast<const uint4*>(from + offset(i0 + x * 32));
+                if (x * 32 + lane < n_vecs) v[x] = mine[x * 32];
 #pragma unroll
             for (int x = 0; x < U; ++x)
-                if (i0 + x * 32 < n_vecs) *reinterpret_cast<uint4*>(to + offset(i0 + x * 32)) = v[x];
+                if (x * 32 + lane < n_vecs) yours[x * 32] = v[x];
+        } else {
+            // quotients by reciprocals: of i below 256 exactly, of rows (2^22 at most) within one
+            const float by_tokens = 1.f / float(max(tokens, 1));
+            const uint32_t per_head = uint32_t(a.head_stride >> 4), per_token = uint32_t(a.token_stride >> 4);
+            uint32_t at[U];
+            uint4 v[U];
+#pragma unroll
+            for (int x = 0; x < U; ++x) {
+                const int i = x * 32 + lane;
+                const int r = int((float(i) + 0.5f) * by_vecs), row = unit * a.unit_rows + r;
+                int h = int((float(row) + 0.5f) * by_tokens), t = row - h * tokens;
+                if (t < 0) { --h; t += tokens; }
+                if (t >= tokens) { ++h; t -= tokens; }
+                at[x] = h * per_head + t * per_token + (i - r * vecs);
+                if (i < n_vecs) v[x] = in[at[x]];
+            }
+#pragma unroll
+            for (int x = 0; x < U; ++x)
+                if (x * 32 + lane < n_vecs) out[at[x]] = v[x];
         }
         if (unit > 0) continue;
         if (lane < a.kv_heads) scales[(long long)dst * a.kv_heads + lane] = scale;
@@ -752,6 +766,8 @@ int ogle_cuda_copy_pages(const OgleCopyPagesParams* p, const OglePageTensors* la
     a.copies = p->copies;
     a.unit_rows = kUnit / p->head_dim;
     a.packed = p->token_stride == p->head_dim && p->head_stride == p->token_stride * p->page_tokens;
+    // places in a page are counted in 32 bits, in 16 bytes each
+    if ((p->kv_heads - 1) * (p->head_stride >> 4) + (p->page_tokens - 1) * (p->token_stride >> 4) >= (1LL << 32) - 16) return OGLE_ERR_UNSUPPORTED;
     const long most_units = div_up((long)p->kv_heads * p->page_tokens, a.unit_rows);
     // a window's units are counted in 32 bits, its windows in a grid's second dimension
     if (most_units * kWindow * kMostLayers * 2 >= (1L << 31) || p->n_copies > 65535 * kWindow) return OGLE_ERR_UNSUPPORTED;
@@ -760,7 +776,7 @@ int ogle_cuda_copy_pages(const OgleCopyPagesParams* p, const OglePageTensors* la
         for (int l = 0; l < a.n_layers; ++l) a.layer[l] = layers_host_array[first + l];
         // one round of blocks for all windows
         const long windows = div_up(p->n_copies, kWindow), units = (long)(p->n_copies < kWindow ? p->n_copies : kWindow) * a.n_layers * 2 * most_units;
-        const long at_once = div_up(kNumSMs * kCopyBlocks, windows);
+        const long at_once = windows < kNumSMs * kCopyBlocks ? kNumSMs * kCopyBlocks / windows : 1;
         long blocks = div_up(units, kThreads / 32);
         if (blocks > at_once) blocks = at_once;
         const cudaError_t e = launch_overlapped(copy_pages_kernel, dim3((unsigned)blocks, (unsigned)windows), dim3(kThreads), 0, stream, a);

@@ -87,7 +87,7 @@ COPY = dict(n_copies=3, n_layers=1, kv_heads=2, head_dim=64, page_tokens=16, n_p
 @pytest.mark.parametrize("more,layer,status", [
     (dict(n_copies=-1), {}, INVALID), (dict(n_layers=-1), {}, INVALID), (dict(kv_heads=0), {}, INVALID), (dict(head_dim=24), {}, INVALID),
     (dict(head_dim=272), {}, UNSUPPORTED), (dict(page_tokens=17), {}, INVALID), (dict(page_stride=2056), {}, ALIGNMENT), (dict(token_stride=48), {}, INVALID),
-    (dict(copies=None), {}, INVALID), ({}, dict(k=None), INVALID), ({}, dict(v_scale=None), INVALID), ({}, dict(bounds_scale=None), INVALID),
+    (dict(head_stride=1 << 37), {}, UNSUPPORTED), (dict(copies=None), {}, INVALID), ({}, dict(k=None), INVALID), ({}, dict(v_scale=None), INVALID), ({}, dict(bounds_scale=None), INVALID),
     ({}, dict(v=SOMEWHERE + 4), ALIGNMENT), ({}, dict(bounds=SOMEWHERE + 8), ALIGNMENT), (dict(n_copies=0), {}, OK), (dict(n_layers=0), {}, OK)])
 def test_copy_refusals(more, layer, status):
     p, t = filled(_lib.CopyPagesParams, **{**COPY, **more}), filled(_lib.PageTensors, **layer)
