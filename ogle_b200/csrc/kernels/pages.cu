@@ -652,7 +652,7 @@ int check_advance(const OgleAdvanceParams* p) {
 }
 int check_compact(const OgleCompactParams* p) {
     if (!p || p->n_seqs < 0 || p->blocks < 0 || p->n_pages < 0 || p->n_copies < 0 || !page_size_ok(p->page_tokens)) return OGLE_ERR_INVALID;
-    if (p->n_pages > kMostPages) return OGLE_ERR_UNSUPPORTED;
+    if (p->n_pages > kMostPages || p->n_copies > (1 << 28)) return OGLE_ERR_UNSUPPORTED;
     if (p->n_seqs > 1 && (p->table_stride < p->blocks || p->new_stride < p->blocks)) return OGLE_ERR_INVALID;
     return OGLE_OK;
 }

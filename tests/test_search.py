@@ -72,7 +72,7 @@ def test_advance_refusals(more, status):
 @pytest.mark.parametrize("more,status", [
     (dict(n_seqs=-1), INVALID), (dict(n_copies=-1), INVALID), (dict(page_tokens=0), INVALID), (dict(table_stride=3), INVALID), (dict(refs=None), INVALID),
     (dict(copies=None), INVALID), (dict(new_table=None), INVALID), (dict(state=None), INVALID), (dict(new_refs=SOMEWHERE), INVALID),
-    (dict(n_pages=(1 << 26) + 1), UNSUPPORTED)])
+    (dict(n_pages=(1 << 26) + 1), UNSUPPORTED), (dict(n_copies=(1 << 28) + 1), UNSUPPORTED)])
 def test_compact_refusals(more, status):
     p = filled(_lib.CompactParams, **{**dict(n_seqs=2, blocks=4, page_tokens=16, n_pages=10, n_copies=5, table_stride=4, new_stride=4, new_refs=2 * SOMEWHERE), **more})
     lib = _lib.cuda_lib()

@@ -725,6 +725,41 @@ def test_search_without_enough_pages_says_so():
         search.texts()
 
 
+def test_offsets_beyond_32_bits():
+    """Pages more than 2 GB apart: bounds, choice, attention and copies as over a packed cache."""
+    new, past = [1, 5], [70, 40]
+    batch, total = lm_checks.make_batch(new, past, 16, 2, 64)
+    k, v, ks, vs = batch["cache"]
+    apart, pages = (1 << 31) + 4096, k.shape[0]
+    assert pages <= 12
+    room = torch.empty(apart * (pages - 1) + 4096, dtype=torch.uint8, device="cuda")
+    far = [room[i * 2048:].as_strided(k.shape, (apart, 1024, 64, 1)).view(torch.float8_e4m3fn) for i in range(2)]
+    for a, b in zip(far, (k, v)):
+        a.view(torch.uint8).copy_(b.view(torch.uint8))
+    cache, rest = (*far, ks, vs), batch_only(batch)
+    bounds = with_bounds(batch, total)
+    got = lm.new_bounds(cache)
+    start = ints([0, total[0], sum(total)])
+    lm.page_bounds(cache, got, rest["block_table"], rest["kv_len"], rest["max_kv_len"], row_start=start, max_rows=max(total))
+    assert torch.equal(got[0], bounds[0]) and torch.equal(got[1], bounds[1])
+    q = torch.randn(6, 4, 64, generator=torch.Generator().manual_seed(1)).cuda()
+    chosen = lm.choose_pages(q, cache, bounds, count=3, **rest)
+    lm_checks.check_attention(lm.sparse_attention(q, cache, chosen, **rest), ref.sparse64(q, batch, total, new, chosen), F32)
+    copies = ints([(0, pages - 1, 16), (1, pages - 2, 5)])
+    lm.copy_pages([cache], copies, bounds=[bounds])
+    lm.copy_pages([(k, v, ks.clone(), vs.clone())], copies)
+    for a, b in zip(far, (k, v)):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_beam_step_of_nothing(dtype):
+    got = lm.beam_step(torch.empty(4, 0, dtype=dtype, device="cuda"), None, 2, 3)
+    assert got[0].shape == (2, 3) and bool((got[1] == -1).all()) and got[3].tolist() == [-1] * 4 and bool((got[5] == -math.inf).all())
+    got = lm.beam_step(torch.empty(0, 10, dtype=dtype, device="cuda"), None, 2, 3)
+    assert got[0].shape == (0, 3) and got[3].shape == (0,)
+
+
 def test_tensors_of_another_device_than_the_current_one_are_refused(monkeypatch):
     batch, total = lm_checks.make_batch([1, 1], [50, 20], 16, 2, 64)
     cache, rest = batch["cache"], batch_only(batch)
