@@ -544,6 +544,20 @@ def test_what_is_not_chosen_does_not_reach_a_row(dtype, new):
     assert bool((got[0][rows - 1] == 0).all()) and bool((got[1][rows - 1] == -math.inf).all())
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("new", [[1] * 80, [6] * 30])
+def test_nan_among_many_pages(new, dtype):
+    """More steps of a warp than it looks up at once; a few texts have NaN among the values of pages that they, or some of their rows, chose."""
+    page, kv_heads = 64, 8
+    batch, total = lm_checks.make_batch(new, [4000] * len(new), page, kv_heads, 16)
+    q = torch.randn(sum(new), 16, 16, generator=torch.Generator().manual_seed(1)).to(dtype).cuda()
+    chosen = random_choice(new, total, page, kv_heads, 50, seed=4)
+    v, table = batch["cache"][1].view(torch.uint8), batch["block_table"].tolist()
+    for b, c, token, element in ((0, 3, 5, 2), (2, 40, 63, 0), (2, 41, 0, 15), (7, 62, 1, 9)):
+        v[table[b][c], :, token, element] = 0x7f
+    lm_checks.check_attention(lm.sparse_attention(q, batch["cache"], chosen, **batch_only(batch)), ref.sparse64(q, batch, total, new, chosen), dtype)
+
+
 def test_rows_that_stand_before_the_text_or_are_nobodys():
     batch, total = lm_checks.make_batch([4, 1, 2], [60, 0, 200], 16, 2, 64)
     batch["kv_len"][0] = 2
