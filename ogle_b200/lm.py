@@ -203,6 +203,21 @@ def _here(t):
     return torch._C._cuda_getCurrentRawStream(device)
 
 
+#: A workspace of up to so many bytes lies behind a call's results, in their allocation; a larger one goes back when the call is made.
+_SMALL = 1 << 16
+
+
+def _results(like, ints, workspace):
+    """int32 results of a call and its workspace: (tensor of the results and what is behind them, their address, the workspace's, what holds it)."""
+    if workspace <= _SMALL:
+        first = (ints + 3) // 4 * 4
+        out = like.new_empty(first + (workspace + 3) // 4, dtype=_I32)
+        at = out.data_ptr()
+        return out, at, at + 4 * first, out
+    out, held = like.new_empty(ints, dtype=_I32), like.new_empty(workspace, dtype=torch.uint8)
+    return out, out.data_ptr(), held.data_ptr(), held
+
+
 def _table(t, name):
     """(sequences, blocks, row stride) of a block table."""
     shape, stride = t.shape, t.stride()
@@ -225,15 +240,13 @@ def beam_step(logits, scores, beams, count, ends=None):
     groups = rows // beams
     # one allocation for all six (a view is 1.1 us, an allocation 1.5)
     n = groups * count
-    out = logits.new_empty(3 * (n + rows), dtype=_I32)
-    at = out.data_ptr()
-    p = _BEAM(groups, beams, vocab, count, _DTYPE[logits.dtype], ends.numel() if ends is not None else 0, logits.stride(0) if rows > 1 else vocab,
-              logits.data_ptr(), _vector(scores, _F32, rows, "scores"), _vector(ends, _I32, None, "ends"), at, at + 4 * n, at + 8 * n,
-              at + 12 * n, at + 12 * n + 4 * rows, at + 12 * n + 8 * rows)
     lib = _lib.cuda_lib()
-    size = lib.ogle_cuda_beam_step_workspace_bytes(p)
-    workspace = logits.new_empty(max(size, 16), dtype=torch.uint8)
-    check(lib.ogle_cuda_beam_step(p, workspace.data_ptr(), size, _here(logits)), "beam_step")
+    given = (groups, beams, vocab, count, _DTYPE[logits.dtype], ends.numel() if ends is not None else 0, logits.stride(0) if rows > 1 else vocab,
+             logits.data_ptr(), _vector(scores, _F32, rows, "scores"), _vector(ends, _I32, None, "ends"))
+    size = lib.ogle_cuda_beam_step_workspace_bytes(_BEAM(*given, 0, 0, 0, 0, 0, 0))
+    out, at, workspace, held = _results(logits, 3 * (n + max(rows, 1)), size)
+    p = _BEAM(*given, at, at + 4 * n, at + 8 * n, at + 12 * n, at + 12 * n + 4 * rows, at + 12 * n + 8 * rows)
+    check(lib.ogle_cuda_beam_step(p, workspace, size, _here(logits)), "beam_step")
     shape, stride, out32 = (groups, count), (count, 1), out.view(_F32)
     return (out32.as_strided(shape, stride), out.as_strided(shape, stride, n), out.as_strided(shape, stride, 2 * n),
             out.as_strided((rows,), (1,), 3 * n), out.as_strided((rows,), (1,), 3 * n + rows), out32.as_strided((rows,), (1,), 3 * n + 2 * rows))
@@ -249,18 +262,14 @@ def advance_pages(block_table, kv_len, parent, new, refs, page_tokens, blocks=No
     seqs, old_blocks, stride = _table(block_table, "block_table")
     n, pages = parent.numel(), refs.numel()
     blocks = old_blocks if blocks is None else blocks
-    # one allocation for all five
-    out = refs.new_empty(n * (blocks + 4) + pages + 2)
-    at = out.data_ptr()
     tokens = new if isinstance(new, torch.Tensor) else None
-    p = _ADVANCE(seqs, n, old_blocks, blocks, page_tokens, pages, 0 if tokens is not None else new, 0, stride, blocks, block_table.data_ptr(),
-                 _vector(kv_len, _I32, seqs, "kv_len"), _vector(parent, _I32, n, "parent"), _vector(tokens, _I32, n, "new"),
-                 _vector(refs, _I32, pages, "refs"), at, at + 4 * n * blocks, at + 4 * n * (blocks + 4), at + 4 * n * (blocks + 1),
-                 at + 4 * (n * (blocks + 4) + pages))
     lib = _lib.cuda_lib()
-    size = lib.ogle_cuda_advance_pages_workspace_bytes(p)
-    workspace = refs.new_empty(size // 4 + 1)
-    check(lib.ogle_cuda_advance_pages(p, workspace.data_ptr(), size, _here(refs)), "advance_pages")
+    given = (seqs, n, old_blocks, blocks, page_tokens, pages, 0 if tokens is not None else new, 0, stride, blocks, block_table.data_ptr(),
+             _vector(kv_len, _I32, seqs, "kv_len"), _vector(parent, _I32, n, "parent"), _vector(tokens, _I32, n, "new"), _vector(refs, _I32, pages, "refs"))
+    size = lib.ogle_cuda_advance_pages_workspace_bytes(_ADVANCE(*given, 0, 0, 0, 0, 0))
+    out, at, workspace, held = _results(refs, n * (blocks + 4) + pages + 2, size)      # one allocation for all five
+    p = _ADVANCE(*given, at, at + 4 * n * blocks, at + 4 * n * (blocks + 4), at + 4 * n * (blocks + 1), at + 4 * (n * (blocks + 4) + pages))
+    check(lib.ogle_cuda_advance_pages(p, workspace, size, _here(refs)), "advance_pages")
     at = n * blocks
     return (out.as_strided((n, blocks), (blocks, 1)), out.as_strided((n,), (1,), at), out.as_strided((pages,), (1,), at + 4 * n),
             out.as_strided((n, 3), (3, 1), at + n), out.as_strided((2,), (1,), at + 4 * n + pages))
@@ -271,14 +280,12 @@ def compact_pages(block_table, refs, most, page_tokens):
     (table, refs, copies int32 [most, 3] for copy_pages, state): state[0] pages are in use, state[1] moves are left for another call."""
     seqs, blocks, stride = _table(block_table, "block_table")
     pages = refs.numel()
-    out = refs.new_empty(seqs * blocks + pages + 3 * most + 2)
-    at = out.data_ptr()
-    p = _COMPACT(seqs, blocks, page_tokens, pages, most, 0, stride, blocks, block_table.data_ptr(), _vector(refs, _I32, pages, "refs"), at,
-                 at + 4 * seqs * blocks, at + 4 * (seqs * blocks + pages), at + 4 * (seqs * blocks + pages + 3 * most))
     lib = _lib.cuda_lib()
-    size = lib.ogle_cuda_compact_pages_workspace_bytes(p)
-    workspace = refs.new_empty(size // 4 + 1)
-    check(lib.ogle_cuda_compact_pages(p, workspace.data_ptr(), size, _here(refs)), "compact_pages")
+    given = (seqs, blocks, page_tokens, pages, most, 0, stride, blocks, block_table.data_ptr(), _vector(refs, _I32, pages, "refs"))
+    size = lib.ogle_cuda_compact_pages_workspace_bytes(_COMPACT(*given, 0, 0, 0, 0))
+    out, at, workspace, held = _results(refs, seqs * blocks + pages + 3 * max(most, 0) + 2, size)
+    p = _COMPACT(*given, at, at + 4 * seqs * blocks, at + 4 * (seqs * blocks + pages), at + 4 * (seqs * blocks + pages + 3 * most))
+    check(lib.ogle_cuda_compact_pages(p, workspace, size, _here(refs)), "compact_pages")
     at = seqs * blocks
     return (out.as_strided((seqs, blocks), (blocks, 1)), out.as_strided((pages,), (1,), at), out.as_strided((most, 3), (3, 1), at + pages),
             out.as_strided((2,), (1,), at + pages + 3 * most))
@@ -373,7 +380,7 @@ def sparse_attention(q, cache, chosen, block_table, kv_len, max_kv_len, row_star
     count = chosen.shape[2]
     c = _CHOSEN(chosen.data_ptr(), chosen.stride(0) if rows > 1 else kv_heads * count, chosen.stride(1) if kv_heads > 1 else count, count, 0)
     lib = _lib.cuda_lib()
-    n = lib.ogle_cuda_sparse_attention_workspace_bytes(b, p, c)
+    n = lib.ogle_cuda_sparse_attention_workspace_bytes(b, p, c) if row_start is not None and max_rows > 1 else 0       # of single rows none
     workspace = q.new_empty(n, dtype=torch.uint8) if n else None
     check(lib.ogle_cuda_sparse_attention(b, p, c, workspace.data_ptr() if n else 0, n, _here(q)), "sparse_attention")
     return out, lse
