@@ -221,18 +221,27 @@ __global__ void __launch_bounds__(kThreads, 3) beam_rows_kernel(BeamArgs a) {
         float top = V::largest(v[0]);
 #pragma unroll
         for (int u = 1; u < kVecs; ++u) top = max_nan(top, V::largest(v[u]));
-        // The k-th largest of each warp, or of all its threads that have a logit: with the least such k of which that is `count` threads.
+        // The k-th largest of each warp, or of all its threads that have a logit: with the least such k of which that is `count` threads. A short row
+        // ends in a warp most of whose threads have none, and whose largest says little: where the other warps suffice it is left
+        // out. (Of 1289 logits such a warp's border lets up to all pass: 22 to 31 us, 5 without it.)
         const uint32_t nothing = ordered(-INFINITY);
         uint32_t mine = ordered(top + 0.f), nth = 0;
         const int have = __popc(__ballot_sync(~0u, mine > nothing));
         if (lane == 0) warp_have[tid / 32] = have;
         __syncthreads();
-        int k = 0, all = 0;
-        while (k < 32 && all < p.count) {
-            ++k;
+        int k = 0, all = 0, least = 0;                              // least: threads that have logits, in a warp that counts
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) least = max(least, (warp_have[w] + 1) / 2);
+        while (all < p.count) {
+            if (k == 32) {
+                if (least <= 1) break;
+                least = 1;
+            } else {
+                ++k;
+            }
             all = 0;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) all += min(warp_have[w], k);
+            for (int w = 0; w < kWarps; ++w) all += warp_have[w] >= least ? min(warp_have[w], k) : 0;
         }
         uint32_t best = nothing;
         for (int i = 0; i < min(k, have); ++i) {
@@ -243,7 +252,7 @@ __global__ void __launch_bounds__(kThreads, 3) beam_rows_kernel(BeamArgs a) {
         }
         if (lane == 0) {
             warp_m[tid / 32] = (double)unordered(best);
-            warp_border[tid / 32] = have > 0 ? nth : ~0u;
+            warp_border[tid / 32] = have > 0 && have >= least ? nth : ~0u;
         }
         __syncthreads();
         double m = -kLargest;

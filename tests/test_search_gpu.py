@@ -48,6 +48,17 @@ def test_beam_step_of_batches_that_few_threads_have(beams, count, vocab, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("vocab", [261, 515, 769, 1289, 2040])
+@pytest.mark.parametrize("end", [-20.0, 0.0, 20.0])
+def test_beam_step_of_rows_that_end_in_a_warp_with_few_logits(end, vocab, dtype):
+    """The row's last few logits the least, ordinary or the largest; counts that the other warps' threads reach, and that they do not."""
+    x, scores = beam_case(3, 3, vocab, dtype, seed=8)
+    x[:, vocab - 5:] += end
+    for count in (1, 6, 16, 33, 65, 128):
+        ref.check_beam_step(lm.beam_step(x, scores, 3, count), ref.beam_step(x, scores, 3, count))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("vocab", [300, 8192, 70001])
 @pytest.mark.parametrize("kind", ["equal", "rising", "falling", "lowest", "few", "two values"])
 def test_beam_step_of_logits_in_order_and_alike(kind, vocab, dtype):
