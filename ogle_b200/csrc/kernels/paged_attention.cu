@@ -1155,6 +1155,9 @@ struct ChosenShape { long long segments; int tile_rows, tiles, cluster, list_str
 // What is longest is the number of rounds of blocks, each as long as its share of the segment's tiles of 64 keys and what a segment's
 // beginning, end and join are worth. r rows are taken to choose r^0.45 times the pages of one (neighbours that share half: 4 rows 46 pages
 // of 24 each, 8 rows 60), so that few rows with many pages are spread over more blocks than one tile of them could use.
+// A cluster lies in one part of the chip, so that larger ones leave places over: of the 296 to 740, clusters of 3 to 5 can have 94 %, of 6 91,
+// of 7 87 and of 8 89 at the least, by the runtime's count. (80 segments of 33 pages, 592 places: in clusters of 7, which do not all fit, 26
+// to 30 us, of 6 16 to 23; 40 of 9 pages, 296 places: 20 and 11.)
 ChosenShape chosen_shape(const OglePagedBatch* b, int most_rows, int slots, int count) {
     const int group = b->q_heads / b->kv_heads, rows = b->max_rows < b->n_rows ? b->max_rows : b->n_rows;
     const long long pages = ((long long)b->max_kv_len + b->page_tokens - 1) / b->page_tokens;
@@ -1170,7 +1173,8 @@ ChosenShape chosen_shape(const OglePagedBatch* b, int most_rows, int slots, int 
         c.segments = (long long)c.tiles * b->n_seqs * b->kv_heads;
         const double wanted = count * union_of < double(pages) ? count * union_of : double(pages), tiles = wanted * b->page_tokens / kTileKeys;
         for (int size = 1; size <= 8; ++size) {
-            const double rounds = double((c.segments * size + slots - 1) / slots), cost = rounds * (tiles / size + kSegmentCost + (size > 1 ? 2 : 0));
+            const long long fit = (long long)slots * (size <= 2 ? 100 : size <= 5 ? 94 : size == 6 ? 91 : 87) / 100;
+            const double rounds = double((c.segments * size + fit - 1) / fit), cost = rounds * (tiles / size + kSegmentCost + (size > 1 ? 2 : 0));
             if (least == 0 || cost < least) {
                 best = c;
                 best.cluster = size;

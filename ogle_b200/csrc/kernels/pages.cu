@@ -460,7 +460,7 @@ __global__ void __launch_bounds__(kThreads) compact_few_kernel(CompactArgs a) {
 constexpr int kMostLayers = 64;                  // of a launch
 constexpr int kWindow = 1024;                    // copies that a block looks over, most
 constexpr int kDeal = 8;                         // copies next to each other in a window: the windows are dealt them in turn, as lists often end early
-                                                 // (733 moves of 128 KB in four layers in a list for 3921: 120 us, 68 so)
+                                                 // (733 moves of 128 KB in four layers in a list for 3921: 120 us, 65 so)
 struct CopyArgs {
     int n_copies, n_layers, kv_heads, dim, page_tokens, n_pages;
     long long page_stride, head_stride, token_stride;
