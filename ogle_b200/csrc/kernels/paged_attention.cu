@@ -1050,7 +1050,8 @@ long long row_tiles_of_all(const OglePagedBatch* b, int rows) {
     const long long most = (long long)(b->max_rows < b->n_rows ? b->max_rows : b->n_rows) * (b->q_heads / b->kv_heads);
     return (most + rows - 1) / rows;
 }
-// Raises the kernel's limit of shared memory, once for each device.
+constexpr int kMostCluster = 16;                  // over chosen pages; 8 are what any GPU can have
+// Raises the kernel's limits of shared memory and of a cluster's blocks, once for each device.
 template <int DP, int MT, bool kSplit, bool kChosen = false>
 cudaError_t prepare() {
     static std::atomic<uint64_t> sized{0};
@@ -1058,15 +1059,16 @@ cudaError_t prepare() {
     cudaError_t e = cudaGetDevice(&device);
     if (e == cudaSuccess && !(sized.load(std::memory_order_relaxed) >> (device & 63) & 1)) {
         e = cudaFuncSetAttribute(paged_attention_kernel<DP, MT, kSplit, kChosen>, cudaFuncAttributeMaxDynamicSharedMemorySize, Form<DP, MT, kSplit>::kSmem);
+        if (kChosen && e == cudaSuccess) e = cudaFuncSetAttribute(paged_attention_kernel<DP, MT, kSplit, kChosen>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e == cudaSuccess) sized.fetch_or(1ull << (device & 63), std::memory_order_relaxed);
     }
     return e;
 }
 
 // Clusters of so many blocks that the GPU runs at once. Asked once for all devices: two of them may differ by a few, which costs time at most.
-template <int DP, int MT, bool kSplit>
+template <int DP, int MT, bool kSplit, bool kChosen = false>
 int most_clusters(int size) {
-    static std::atomic<int> known[9] = {};            // one more than the number
+    static std::atomic<int> known[kMostCluster + 1] = {};      // one more than the number
     int n = known[size].load(std::memory_order_relaxed);
     if (n == 0) {
         cudaLaunchAttribute attr[1];
@@ -1079,7 +1081,7 @@ int most_clusters(int size) {
         cfg.dynamicSmemBytes = Form<DP, MT, kSplit>::kSmem;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        if (prepare<DP, MT, kSplit>() != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, paged_attention_kernel<DP, MT, kSplit, false>, &cfg) != cudaSuccess) {
+        if (prepare<DP, MT, kSplit, kChosen>() != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, paged_attention_kernel<DP, MT, kSplit, kChosen>, &cfg) != cudaSuccess) {
             (void)cudaGetLastError();
             return 0;
         }
@@ -1151,14 +1153,16 @@ size_t few_workspace(const OglePagedBatch* b, const OgleAttentionParams* p) {
 
 // Attention over chosen pages: rows of a tile, segments, blocks to a segment, and what is kept of the tiles' lists where several rows share a
 // tile.
-struct ChosenShape { long long segments; int tile_rows, tiles, cluster, list_stride; size_t lists; };
+struct ChosenShape { long long segments; int tile_rows, tiles, in_tile, cluster, list_stride; size_t lists; };      // in_tile: rows that one can have a part of
+constexpr int kListsCost = 7;                    // tiles that the lists' launch takes as long as (a tile 0.7 us)
 // What is longest is the number of rounds of blocks, each as long as its share of the segment's tiles of 64 keys and what a segment's
 // beginning, end and join are worth. r rows are taken to choose r^0.45 times the pages of one (neighbours that share half: 4 rows 46 pages
 // of 24 each, 8 rows 60), so that few rows with many pages are spread over more blocks than one tile of them could use.
-// A cluster lies in one part of the chip, so that larger ones leave places over: of the 296 to 740, clusters of 3 to 5 can have 94 %, of 6 91,
-// of 7 87 and of 8 89 at the least, by the runtime's count. (80 segments of 33 pages, 592 places: in clusters of 7, which do not all fit, 26
-// to 30 us, of 6 16 to 23; 40 of 9 pages, 296 places: 20 and 11.)
-ChosenShape chosen_shape(const OglePagedBatch* b, int most_rows, int slots, int count) {
+// A cluster lies in one part of the chip, so that large ones leave places over; the runtime says how many run at once: of 592 places clusters
+// of 3 have 561, of 7 546. (80 segments of 33 pages: in clusters of 7, which do not all fit, 26 to 30 us, of 6 16 to 23; 40 of 9
+// pages and 296 places: 20 and 11. Clusters of 16, 8: 4 segments of 79 pages of 128 17 and 24 us, 8 of 64 pages of 64 13 and 14.5.)
+template <typename MostClusters>
+ChosenShape chosen_shape(const OglePagedBatch* b, int most_rows, int slots, int count, MostClusters most_clusters) {
     const int group = b->q_heads / b->kv_heads, rows = b->max_rows < b->n_rows ? b->max_rows : b->n_rows;
     const long long pages = ((long long)b->max_kv_len + b->page_tokens - 1) / b->page_tokens;
     ChosenShape best = {};
@@ -1171,10 +1175,14 @@ ChosenShape chosen_shape(const OglePagedBatch* b, int most_rows, int slots, int 
         c.tile_rows = tile_rows;
         c.tiles = int(row_tiles_of_all(b, tile_rows));
         c.segments = (long long)c.tiles * b->n_seqs * b->kv_heads;
+        c.in_tile = rows <= 1 ? 1 : tile_rows % group == 0 ? tile_rows / group : (tile_rows + group - 2) / group + 1;
         const double wanted = count * union_of < double(pages) ? count * union_of : double(pages), tiles = wanted * b->page_tokens / kTileKeys;
-        for (int size = 1; size <= 8; ++size) {
-            const long long fit = (long long)slots * (size <= 2 ? 100 : size <= 5 ? 94 : size == 6 ? 91 : 87) / 100;
-            const double rounds = double((c.segments * size + fit - 1) / fit), cost = rounds * (tiles / size + kSegmentCost + (size > 1 ? 2 : 0));
+        for (int size = 1; size <= kMostCluster; size += size < 8 ? 1 : 8) {
+            long long fit = size == 1 ? slots : (long long)most_clusters(size) * size;
+            if (fit == 0 && size > 8) break;
+            if (fit == 0) fit = slots;            // (nothing to ask)
+            const double rounds = double((c.segments * size + fit - 1) / fit);
+            const double cost = rounds * (tiles / size + kSegmentCost + (size > 8 ? 4 : size > 1 ? 2 : 0)) + (c.in_tile > 1 ? kListsCost : 0);
             if (least == 0 || cost < least) {
                 best = c;
                 best.cluster = size;
@@ -1182,11 +1190,9 @@ ChosenShape chosen_shape(const OglePagedBatch* b, int most_rows, int slots, int 
             }
         }
     }
-    int in_tile = (best.tile_rows + group - 2) / group + 1;        // rows that a tile can have a part of
-    if (best.tile_rows % group == 0) in_tile = best.tile_rows / group;
-    best.list_stride = (in_tile < rows ? in_tile : rows) * count;
+    best.list_stride = (best.in_tile < rows ? best.in_tile : rows) * count;
     // (one row to every tile, none cut: its choice is the list)
-    best.lists = rows > 1 && in_tile > 1 ? size_t(best.segments) * (best.list_stride * sizeof(int2) + sizeof(int)) : 0;
+    best.lists = best.in_tile > 1 ? size_t(best.segments) * (best.list_stride * sizeof(int2) + sizeof(int)) : 0;
     return best;
 }
 
@@ -1315,8 +1321,9 @@ size_t ogle_cuda_sparse_attention_workspace_bytes(const OglePagedBatch* batch, c
     Batch b;
     if (!p || !c || c->count < 1 || paged::translate(batch, b) != OGLE_OK || b.n_seqs == 0 || b.max_rows == 0) return 0;
     return with_form(choose_sparse(batch), [&](auto dp, auto mt, auto split) {
-        using F = Form<decltype(dp)::value, decltype(mt)::value, decltype(split)::value>;
-        return chosen_shape(batch, F::kRows, kNumSMs * F::kBlocks, c->count).lists;
+        constexpr int DP = decltype(dp)::value, MT = decltype(mt)::value;
+        using F = Form<DP, MT, decltype(split)::value>;
+        return chosen_shape(batch, F::kRows, kNumSMs * F::kBlocks, c->count, most_clusters<DP, MT, decltype(split)::value, true>).lists;
     });
 }
 
@@ -1347,7 +1354,7 @@ int ogle_cuda_sparse_attention(const OglePagedBatch* batch, const OgleAttentionP
         constexpr int DP = decltype(dp)::value, MT = decltype(mt)::value;
         constexpr bool kSplit = decltype(split)::value;
         using F = Form<DP, MT, kSplit>;
-        const ChosenShape shape = chosen_shape(batch, F::kRows, kNumSMs * F::kBlocks, c->count);
+        const ChosenShape shape = chosen_shape(batch, F::kRows, kNumSMs * F::kBlocks, c->count, most_clusters<DP, MT, kSplit, true>);
         a.tile_rows = shape.tile_rows;
         a.by_segment = shape.tiles;
         a.cluster = shape.cluster;

@@ -516,6 +516,18 @@ def test_sparse_attention(case, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("new,past,page,heads,kv_heads,dim,count", [
+    ([1], [12000], 128, 16, 4, 96, 79), ([1, 1, 1], [9000, 77, 0], 64, 16, 1, 128, 90), ([1], [5000], 64, 4, 2, 256, 60),
+    ([1, 1], [7000, 6500], 128, 16, 4, 64, 47), ([3, 1], [8000, 8000], 64, 20, 2, 64, 64), ([4, 2], [6000, 30], 32, 8, 1, 128, 100)])
+def test_sparse_attention_of_few_rows_over_many_pages(new, past, page, heads, kv_heads, dim, count, dtype):
+    batch, total = lm_checks.make_batch(new, past, page, kv_heads, dim, seed=21)
+    q = torch.randn(sum(new), heads, dim, generator=torch.Generator().manual_seed(22)).to(dtype).cuda()
+    chosen = random_choice(new, total, page, kv_heads, count, seed=23)
+    got = lm.sparse_attention(q, batch["cache"], chosen, **batch_only(batch))
+    lm_checks.check_attention(got, ref.sparse64(q, batch, total, new, chosen), dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 def test_sparse_attention_over_all_pages_is_attention(dtype):
     new, past, page = [1, 4, 30], [900, 333, 20], 16
     batch, total = lm_checks.make_batch(new, past, page, 2, 64)
