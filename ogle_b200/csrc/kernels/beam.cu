@@ -33,6 +33,7 @@ constexpr int kLook = 8;                         // batches between two looks at
 constexpr float kLargest = 3.402823466e38f;
 constexpr float kSpread = 40.f;                  // of x above m: sums stay below 2^58 of 2^127
 constexpr float kTame = 1e6f;                    // logits beyond it are left to the second launch: fp32 has no exponent for x log2(e) - c there
+constexpr float kNear = 100.f;                   // what is further below a row's largest logit has no part in its sum: 2^30 of exp(-100) are 2^-114
 
 // A logit and its token in one number: the larger logit is the larger number, of equal ones the lower token. 0: none.
 typedef unsigned long long Key;
@@ -49,9 +50,11 @@ __device__ __forceinline__ float logit_of(Key k) { return unordered(uint32_t(k >
 __device__ __forceinline__ int token_of(Key k) { return int(~uint32_t(k)); }
 
 // What a block leaves behind - a sum of exp(x - m), or kAgain: the range is to be gone over again -, followed by its `count` best in falling
-// order (0: none).
+// order (0: none). The sum of logits that are all -kTame or less is left at 0.
 struct __align__(16) Part { double sum, m; };
 constexpr double kAgain = -1.;
+// Whether a range's sum is wanting: beside a row's largest logit `top`, with `best` the range's first key.
+__device__ __forceinline__ bool sum_is_wanting(double sum, Key best, float top) { return !(sum >= 0.) || sum == 0. && best && logit_of(best) >= top - kNear; }
 __host__ __device__ inline size_t part_bytes(int count) { return sizeof(Part) + ((size_t)count + 1) / 2 * 16; }
 
 struct BeamArgs {
@@ -213,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, 3) beam_rows_kernel(BeamArgs a) {
     // over again.)
     float c, fine_to, limit;                                       // weights are 2^(x log2(e) - c), for logits up to fine_to; what is above limit is kept
     const auto refer_to = [&](float m) {
-        c = m > -kTame ? m * kLog2e : 0.f;                         // (else nothing but a mask's lowest so far: it has no weight)
+        c = m > -kTame ? m * kLog2e : INFINITY;                    // (else nothing but a mask's lowest so far: no weight, no reference, a sum of 0)
         fine_to = m > -kTame ? fminf(m + kSpread, kTame) : -kTame;
     };
     uint32_t border = ~0u;
@@ -284,7 +287,7 @@ __global__ void __launch_bounds__(kThreads, 3) beam_rows_kernel(BeamArgs a) {
             if (most <= kTame) {
                 const float before = c;
                 refer_to(most);
-                sum *= exp2((double)before - (double)c);
+                sum = before < INFINITY ? sum * exp2((double)before - (double)c) : 0.;
             } else {
                 again = true;
             }
@@ -365,12 +368,17 @@ __global__ void __launch_bounds__(kThreads, 3) beam_rows_kernel(BeamArgs a) {
         for (int u = 0; u < kVecs; ++u) v[u] = next[u];
     }
 
+    // logits just above -kTame: those below it, whose weight was taken for 0, would count beside them
+    if (n > 0) {
+        const float best = logit_of(kept[0]);
+        again |= best > -kTame && best < kNear - kTame;
+    }
     // the kept logits' part of the sum in 64 bits, where all threads have the same c
     const double inverse = 1. / (double)kLog2e;
     const bool same = __syncthreads_and(c == c0);
-    double top = (double)c * inverse;
+    double top = c < INFINITY ? (double)c * inverse : -INFINITY;
     if (same) {
-        if (tid < n) {
+        if (tid < n && c < INFINITY) {
             const float x = logit_of(kept[tid]);
             sum += exp((double)x - top) - (double)weight(x, c);
         }
@@ -381,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 3) beam_rows_kernel(BeamArgs a) {
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) top = fmax(top, warp_m[w]);
-        sum *= exp((double)c * inverse - top);
+        sum = c < INFINITY ? sum * exp((double)c * inverse - top) : 0.;
     }
 #pragma unroll
     for (int d = 16; d; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
@@ -390,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, 3) beam_rows_kernel(BeamArgs a) {
     if (tid == 0) {
         double all = 0.;
         for (int w = 0; w < kWarps; ++w) all += warp_sum[w];
-        *reinterpret_cast<Part*>(out) = Part{redo ? kAgain : all, top};
+        *reinterpret_cast<Part*>(out) = Part{redo ? kAgain : all, top > -INFINITY ? top : 0.};
     }
     for (int i = tid; i < p.count; i += kThreads) reinterpret_cast<Key*>(out + sizeof(Part))[i] = i < n ? kept[i] : 0ull;
 }
@@ -540,19 +548,17 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamArgs a) {
             for (int r = lane; r < a.ranges; r += 32) {
                 if (r != lane) part = *reinterpret_cast<const Part*>(mine + r * stride);
                 if (part.sum > 0.) sum += part.sum * exp(part.m - (double)top);
-                redo |= part.sum < 0.;
+                else redo |= sum_is_wanting(part.sum, *reinterpret_cast<const Key*>(mine + r * stride + sizeof(Part)), top);
             }
 #pragma unroll
             for (int d = 16; d; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
-            redo |= sum == 0. && top > -INFINITY;                  // nothing but a mask's lowest
-            if (lane == 0) beam_terms[b] = make_double2(top, sum > 0. ? log(sum) : (top > -INFINITY ? NAN : 0.));
+            if (lane == 0) beam_terms[b] = make_double2(top, sum > 0. ? log(sum) : 0.);
         }
         if (!__syncthreads_or(redo) || round > 0) break;
         for (int list = 0; list < lists; ++list) {
             const int b = list / a.ranges;
             unsigned char* const part = parts + list * stride;
-            const double sum = reinterpret_cast<const Part*>(part)->sum;
-            if (sum < 0. || isnan(beam_terms[b].y)) {              // of a beam without any weight, all ranges
+            if (sum_is_wanting(reinterpret_cast<const Part*>(part)->sum, *reinterpret_cast<const Key*>(part + sizeof(Part)), float(beam_terms[b].x))) {
                 const size_t row = (size_t)(g * p.beams + b) * p.logits_stride;
                 if (p.dtype == OGLE_F32) again(a, static_cast<const float*>(p.logits) + row, list - b * a.ranges, part, found);
                 else if (p.dtype == OGLE_F16) again(a, static_cast<const __half*>(p.logits) + row, list - b * a.ranges, part, found);
