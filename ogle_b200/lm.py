@@ -332,8 +332,8 @@ def page_bounds(cache, bounds, block_table, kv_len, max_kv_len, row_start=None, 
     """Bounds of the keys in every page that the batch's rows were appended to (ogle_cuda_page_bounds), in place: behind `append`, with its
     batch. choose_pages needs them of all pages that a row may choose."""
     pages, heads, _, dim = cache[0].shape
-    # rows are not looked at: of their number a bound will do, and any type
-    rows = block_table.shape[0] if row_start is None else min(block_table.shape[0] * max_rows, (1 << 30) // heads)
+    # rows are not looked at, but row_start is cut to their number: any that a batch could have, and any type
+    rows = block_table.shape[0] if row_start is None else (1 << 30) // heads
     b = _batch(cache, block_table, kv_len, max_kv_len, row_start, max_rows, rows, heads, torch.bfloat16)
     check(_lib.cuda_lib().ogle_cuda_page_bounds(b, *_bounds(bounds, pages, heads, dim), _here(cache[0])), "page_bounds")
 

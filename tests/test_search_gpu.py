@@ -833,3 +833,61 @@ def test_bounds_under_bounds_that_are_far_too_wide():
 
 def test_nothing_waited_in_vain():
     assert _lib.cuda_lib().ogle_cuda_device_status() == 0
+
+
+# ------------------------------------------------------------------------------------------------------ batches of other shapes
+def check_bounds(batch, total, new, most, bounds, row_start):
+    """The bounds of the pages that the first `most` rows of each sequence were appended to, and of no other."""
+    k, _, ks, _ = batch["cache"]
+    page = k.shape[2]
+    lm.page_bounds(batch["cache"], bounds, batch["block_table"], batch["kv_len"], batch["max_kv_len"], row_start=row_start, max_rows=most)
+    touched = set()
+    for b, n in enumerate(new):
+        begin = total[b] - n
+        for c in range(begin // page, (begin + min(n, most) - 1) // page + 1) if n else ():
+            at = int(batch["block_table"][b, c])
+            touched.add(at)
+            lo_hi, unit = ref.page_bounds(k.cpu(), ks.cpu(), at, min(page, total[b] - c * page))
+            assert torch.equal(bounds[0][at].cpu().double(), lo_hi) and torch.equal(bounds[1][at].cpu().double(), unit), (b, c)
+    rest = [p for p in range(k.shape[0]) if p not in touched]
+    assert bool((bounds[0][rest] == 77).all())
+
+
+@pytest.mark.parametrize("new,past,most,before", [
+    ([1, 1, 1, 1], [40, 15, 16, 0], 1, 8),                   # rows that no sequence has, before the first
+    ([5, 1, 20], [30, 100, 0], 20, 1000),
+    ([100, 1], [3, 50], 10, 0),                              # more rows than max_rows
+    ([33, 40, 2, 0, 17], [0, 16, 31, 9, 200], 16, 0),
+    ([70, 70], [10, 300], 33, 5)])
+def test_bounds_of_batches_whose_rows_lie_anywhere(new, past, most, before):
+    batch, total = lm_checks.make_batch(new, past, 16, 2, 64)
+    bounds = lm.new_bounds(batch["cache"])
+    bounds[0].fill_(77)
+    check_bounds(batch, total, new, most, bounds, batch["row_start"] + before)
+
+
+def test_choices_behind_append_of_more_rows_than_count():
+    """append and page_bounds with one batch that begins behind rows which nobody has, and whose sequences have more rows than max_rows; the pages that got
+    large keys are then the next token's choice."""
+    new, past, page, most, before = [90, 1, 70], [100, 200, 500], 16, 12, 6
+    batch, total = lm_checks.make_batch(new, past, page, 2, 64)
+    bounds = with_bounds(batch, total)
+    g = torch.Generator().manual_seed(1)
+    k, v = (torch.randn(before + sum(new), 2, 64, generator=g).cuda() for _ in range(2))
+    call = dict(batch_only(batch), row_start=batch["row_start"] + before, max_rows=most)
+    lm.append(30 * k, v, batch["cache"], **call)
+    lm.page_bounds(batch["cache"], bounds, **call)
+    q = torch.randn(3, 4, 64, generator=g).cuda()
+    chosen = lm.choose_pages(q, batch["cache"], bounds, batch["block_table"], batch["kv_len"], batch["max_kv_len"], count=4).cpu()
+    keys, scales, table = batch["cache"][0].cpu(), batch["cache"][2].cpu(), batch["block_table"].cpu()
+    for b in range(3):
+        own, pages = (total[b] - 1) // page, table[b].tolist()
+        for h in range(2):
+            lo_hi, unit = torch.zeros(keys.shape[0], 2, 64), torch.zeros(keys.shape[0], dtype=torch.float64)
+            for c in range(own + 1):
+                found, size = ref.page_bounds(keys, scales, pages[c], min(page, total[b] - c * page))
+                lo_hi[pages[c]], unit[pages[c]] = found[h].float(), size[h]
+            want = ref.choose_row(q[b, 2 * h:2 * h + 2].cpu(), lo_hi, unit, table[b], own, 4, 1, 1)
+            assert chosen[b, h].tolist() == want, (b, h)
+            if new[b] > most:
+                assert past[b] // page + 1 in want or past[b] // page in want
