@@ -532,8 +532,9 @@ int ogle_cuda_adjust_logits(const OgleLogitsParams* p, ogle_stream_t stream);
  * out_beam and out_token [n_groups][count]; behind the last there are minus infinity, -1, -1. Of these the first `beams` whose token is
  * none of ends[0 .. n_ends) go on: next_row (the parent's row, g * beams + out_beam), next_token and next_score [n_groups][beams], filled
  * up with -1, -1, minus infinity. (With end tokens a count of 2 * beams is enough for all to go on.)
- * Exponentials are of fp32, but those of the largest logits, and sums of 64 bits: the logarithm of a row's sum is within 2^-22 of its
- * value, most often within 2^-24. Beams of the same largest logit whose logarithms are as near to each other count as having the same sum.
+ * Exponentials are of fp32, but those of most rows' largest logits, and sums of 64 bits: the logarithm of a row's sum is within 2^-19 of
+ * its value - that far off where thousands of equal logits far below the largest make up most of it -, most often within 2^-23. Beams of the
+ * same largest logit whose logarithms are within 2^-18 of each other count as having the same sum.
  * n_groups * beams is 65535 at most. `workspace`: as above; what is in it need not outlive the call. */
 typedef struct {
     int n_groups, beams, vocab, count;     /* count at most 128 */

@@ -14,7 +14,8 @@
 //
 // Which of two beams' tokens comes first hangs on the logarithms of their sums, to all bits that are left. So the totals are
 // of 64 bits, and the sums nearly: exponents in one rounding, exponentials in fp32 - but those of the kept logits, which are most of a
-// peaked row's sum, are put right in 64 bits at the end -, a batch's sum of a thread in fp32, all others in 64.
+// peaked row's sum, are put right in 64 bits at the end, unless a later batch rose far above the first -, a batch's sum of a thread in fp32, all
+// others in 64.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -31,7 +32,7 @@ constexpr int kKept = 1024;                      // logits that a block keeps at
 constexpr int kRankAt = kThreads;                // ... and how many of them are ranked, once there are more: one a thread
 constexpr int kLook = 8;                         // batches between two looks at that, at most
 constexpr float kLargest = 3.402823466e38f;
-constexpr float kSpread = 40.f;                  // of x above m: sums stay below 2^58 of 2^127
+constexpr float kSpread = 1.375f;                // of x above m: exponents stay below 2, and are rounded by 2^-24
 constexpr float kTame = 1e6f;                    // logits beyond it are left to the second launch: fp32 has no exponent for x log2(e) - c there
 constexpr float kNear = 100.f;                   // what is further below a row's largest logit has no part in its sum: 2^30 of exp(-100) are 2^-114
 
@@ -129,7 +130,9 @@ __device__ __forceinline__ void range_of(const BeamArgs& a, const T* row, int r,
 }
 
 // exp(x - m) as the sums have it: 2^(x log2(e) - c) in one rounding of the exponent, which is small where the weight is large. c is an fp32
-// number, m what it stands for; log2(e) in fp32 makes a weight wrong by 2^-26 of its distance from m.
+// number, m what it stands for; log2(e) in fp32 makes a weight wrong by 2^-26 of its distance from m. What a sum is off by is at most
+// 2^-19 of it: 2^-20 ln 2 where nearly all of it comes of alike logits 11 to 22 below m, all rounded alike, 2^-26 of that distance, 2^-22
+// for the exponentials and six roundings of 2^-24 in fp32. The roundings of logits that differ do so too, and cancel.
 constexpr float kLog2e = 1.442695022f;
 __device__ __forceinline__ float weight(float x, float c) { return exp2_fast(fmaf(x, kLog2e, -c)); }
 
@@ -568,8 +571,8 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamArgs a) {
         __syncthreads();
         my_key = tid < all ? key_at(tid, my_list) : 0ull;
     }
-    // Two beams of the same logits differ in the last bits of their sums where their rows lie differently to 16 bytes. They count as the same,
-    // so that their totals are equal and come in the beams' order; so does what is as near by chance.
+    // Two beams of the same logits differ in their sums' errors, twice 2^-19 at most, where their rows lie differently to 16 bytes. They count as
+    // the same, so that their totals are equal and come in the beams' order; so does what is as near by chance.
     constexpr int kMine = (kMostBeams + kPickThreads - 1) / kPickThreads;
     double minus[kMine];
 #pragma unroll
@@ -579,7 +582,7 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamArgs a) {
         const double2 term = beam_terms[b];
         minus[i] = term.y;
         for (int o = 0; o < b; ++o)
-            if (beam_terms[o].x == term.x && fabs(beam_terms[o].y - term.y) <= 0x1p-22) {
+            if (beam_terms[o].x == term.x && fabs(beam_terms[o].y - term.y) <= 0x1p-18) {
                 minus[i] = beam_terms[o].y;
                 break;
             }
