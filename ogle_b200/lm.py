@@ -229,8 +229,8 @@ def _table(t, name):
 def beam_step(logits, scores, beams, count, ends=None):
     """The best continuations of each group of `beams` rows of logits [groups * beams, vocab] (ogle_cuda_beam_step): by the rows' scores
     (float32 [groups * beams]: the logarithm of what each text has come to; not finite: no such text; None: 0) plus the logarithm of the
-    token's probability. Returns (score, beam, token) of the `count` best, [groups, count], in falling order, equal ones by beam and
-    token, behind the last -inf, -1, -1; and (next_row, next_token, next_score) [groups * beams]: the first `beams` of these whose token is not
+    token's probability. Returns (score, beam, token) of the `count` best, [groups, count], in falling order, equal ones by beam,
+    logit and token, behind the last -inf, -1, -1; and (next_row, next_token, next_score) [groups * beams]: the first `beams` of these whose token is not
     among `ends` (int32), as advance_pages takes them - the row that each goes on from, or -1."""
     if logits.dim() != 2 or not logits.is_cuda or logits.dtype not in _DTYPE or logits.stride(1) != 1 and logits.shape[1] > 1:
         raise ValueError("logits: expected a CUDA tensor [rows, vocab] in float32, float16 or bfloat16, a row's elements side by side")

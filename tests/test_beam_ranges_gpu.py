@@ -188,3 +188,19 @@ def test_beams_alike_whose_batches_are_not(edge, rest, dtype):
         assert torch.equal(got[i].cpu().long(), want[i].long()), i
     for i in (0, 5):
         assert bool(((got[i].cpu().double() - want[i]).abs() <= 2.0 ** -19 + want[i].abs() * 2.0 ** -24).all())
+
+
+# ------------------------------------------------------------------------------------------------------ totals that 64 bits cannot tell apart
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,vocab", [(1, 300), (3, 70001), (120, 70001)])
+def test_a_beams_order_is_its_logits(rows, vocab, dtype):
+    """Beside an infinite logit (the largest number), or a score as large, all other totals of a beam are the same number."""
+    x = torch.randn(rows, vocab, generator=torch.Generator().manual_seed(4))
+    x[:, vocab // 3] = math.inf
+    x = x.to(dtype).cuda()
+    check(lm.beam_step(x, None, 1, 8), ref.beam_step(x, None, 1, 8))
+    x[:, vocab // 3] = 0
+    scores = torch.full((rows,), -1e30).cuda()
+    check(lm.beam_step(x, scores, 1, 128), ref.beam_step(x, scores, 1, 128))
+    if rows % 3 == 0:
+        check(lm.beam_step(x, scores, 3, 128), ref.beam_step(x, scores, 3, 128))
