@@ -113,6 +113,9 @@ class Answers:
         return logits
 
 
+MOST_COUNT = 128                                # continuations that lm.beam_step finds for a group
+
+
 class Search:
     """Beam search over the answers to prompts: `beams` texts of each, whose pages, scores and parents stay on the device."""
 
@@ -132,10 +135,15 @@ class Search:
                      max_rows=max(lengths))
         x = model.rows(torch.tensor([t for p in prompts for t in p]).cuda(), self.caches, batch, self.bounds)
         x = x[torch.tensor([s - 1 for s in starts[1:]]).cuda()]
-        # the best tokens behind each prompt are the first beams
-        score, _, token, *_ = lm.beam_step(model.logits(x), None, 1, beams)
-        row = torch.arange(len(prompts), dtype=torch.int32).repeat_interleave(beams).cuda()
-        self.next = torch.where(token.view(-1) >= 0, row, -1), token.reshape(-1), score.reshape(-1)
+        # the best tokens behind each prompt that are no end token are the first beams
+        self.first = score, _, token = lm.beam_step(model.logits(x), None, 1, min(beams + len(ends), MOST_COUNT))[:3]
+        goes_on = token >= 0
+        if self.ends is not None:
+            goes_on &= ~(token[..., None] == self.ends).any(-1)
+        place = torch.where(goes_on, goes_on.cumsum(1) - 1, beams).clamp(max=beams)       # those behind the last beam have one place
+        row = torch.arange(len(prompts), dtype=torch.int32).cuda()[:, None].expand_as(token)
+        self.next = tuple(v.new_full((len(prompts), beams + 1), nothing).scatter(1, place, v)[:, :beams].flatten().contiguous()
+                          for v, nothing in ((row, -1), (token, -1), (score, -float("inf"))))
         self.found, self.taken = [], [self.next]
 
     def _advance(self, row, new):
@@ -178,7 +186,7 @@ class Search:
         for i, (row, score) in enumerate(zip(taken[-1][0], taken[-1][2])):
             if row >= 0:
                 left[i // self.beams].append((score, tokens(len(taken) - 1, i)))
-        ended = [[] for _ in self.prompts]
+        ended = [[(s, [t]) for s, t in zip(*found) if t in ends] for found in zip(self.first[0].tolist(), self.first[2].tolist())]
         for step, found in enumerate(self.found):
             score, beam, token = (t.tolist() for t in found)
             for g in range(len(self.prompts)):

@@ -891,3 +891,19 @@ def test_choices_behind_append_of_more_rows_than_count():
             assert chosen[b, h].tolist() == want, (b, h)
             if new[b] > most:
                 assert past[b] // page + 1 in want or past[b] // page in want
+
+
+# ------------------------------------------------------------------------------------------------------ the example's ends
+def test_search_ends_texts_at_their_first_token():
+    model = lm_example.Model(layers=1)
+    prompts, beams = prompts_of([20, 3], model.vocab), 3
+    plain = lm_example.Search(model, prompts, beams, steps=4)
+    first, score = (t.view(2, beams)[:, 0].tolist() for t in plain.next[1:])
+    search = lm_example.Search(model, prompts, beams, ends=sorted(set(first)), steps=4)
+    for _ in range(4):
+        search.step()
+    left, ended = search.texts()
+    for g in range(2):
+        assert any(text == [first[g]] and abs(s - score[g]) < 1e-5 for s, text in ended[g])
+        assert len(left[g]) == beams and all(not set(text) & set(first) for _, text in left[g])
+        assert all(text[-1] in first and not set(text[:-1]) & set(first) for _, text in ended[g])
