@@ -124,7 +124,10 @@ class Search:
         self.caches = model.new_caches(pages, page_tokens)
         self.bounds = model.new_bounds(self.caches)
         self.most = max(len(p) for p in prompts) + steps          # tokens of a text
-        self.ends = torch.tensor(list(ends), dtype=torch.int32).cuda() if ends else None
+        ends = sorted(set(ends))
+        self.ends = torch.tensor(ends, dtype=torch.int32).cuda() if ends else None
+        # each beam may have all end tokens among the best
+        self.count = min(beams * max(2, 1 + len(ends)), MOST_COUNT)
         none = torch.full((1, -(-self.most // page_tokens)), -1, dtype=torch.int32).cuda()
         lengths = [len(p) for p in prompts]
         self.refs = torch.zeros(pages, dtype=torch.int32).cuda()
@@ -157,7 +160,7 @@ class Search:
         self._advance(row, (row >= 0).int())
         batch = dict(block_table=self.table, kv_len=self.kv_len, max_kv_len=self.most)
         x = self.model.rows(token.clamp(min=0).long(), self.caches, batch, self.bounds)
-        found = lm.beam_step(self.model.logits(x), score, self.beams, 2 * self.beams, ends=self.ends)
+        found = lm.beam_step(self.model.logits(x), score, self.beams, self.count, ends=self.ends)
         self.found.append(found[:3])
         self.next = found[3:]
         self.taken.append(self.next)

@@ -907,3 +907,13 @@ def test_search_ends_texts_at_their_first_token():
         assert any(text == [first[g]] and abs(s - score[g]) < 1e-5 for s, text in ended[g])
         assert len(left[g]) == beams and all(not set(text) & set(first) for _, text in left[g])
         assert all(text[-1] in first and not set(text[:-1]) & set(first) for _, text in ended[g])
+
+
+def test_search_with_many_end_tokens_keeps_its_beams():
+    model = lm_example.Model(layers=1)
+    search = lm_example.Search(model, prompts_of([20, 3, 9], model.vocab), 2, ends=range(0, model.vocab, 2), steps=12)
+    for _ in range(12):
+        search.step()
+    left, ended = search.texts()
+    assert all(len(found) == 2 for found in left) and all(t % 2 for found in left for _, text in found for t in text)
+    assert all(text[-1] % 2 == 0 and all(t % 2 for t in text[:-1]) for found in ended for _, text in found)
