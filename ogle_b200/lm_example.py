@@ -120,7 +120,7 @@ class Search:
     """Beam search over the answers to prompts: `beams` texts of each, whose pages, scores and parents stay on the device."""
 
     def __init__(self, model, prompts, beams, page_tokens=16, pages=512, ends=(), steps=100):
-        self.model, self.beams, self.page_tokens, self.prompts = model, beams, page_tokens, [list(p) for p in prompts]
+        self.model, self.beams, self.page_tokens, self.prompts, self.steps = model, beams, page_tokens, [list(p) for p in prompts], steps
         self.caches = model.new_caches(pages, page_tokens)
         self.bounds = model.new_bounds(self.caches)
         self.most = max(len(p) for p in prompts) + steps          # tokens of a text
@@ -155,7 +155,9 @@ class Search:
         self.missing = self.missing + state[1]
 
     def step(self):
-        """Appends the chosen tokens and chooses the next ones."""
+        """Appends the chosen tokens and chooses the next ones, `steps` times at most: the tables have no room for more."""
+        if len(self.found) == self.steps:
+            raise ValueError(f"the search was made for {self.steps} steps")
         row, token, score = self.next
         self._advance(row, (row >= 0).int())
         batch = dict(block_table=self.table, kv_len=self.kv_len, max_kv_len=self.most)

@@ -917,3 +917,14 @@ def test_search_with_many_end_tokens_keeps_its_beams():
     left, ended = search.texts()
     assert all(len(found) == 2 for found in left) and all(t % 2 for found in left for _, text in found for t in text)
     assert all(text[-1] % 2 == 0 and all(t % 2 for t in text[:-1]) for found in ended for _, text in found)
+
+
+def test_search_refuses_a_step_too_many():
+    model = lm_example.Model(layers=1)
+    search = lm_example.Search(model, prompts_of([20, 3], model.vocab), 2, steps=5)
+    for _ in range(5):
+        search.step()
+    before = search.texts()
+    with pytest.raises(ValueError):
+        search.step()
+    assert search.texts() == before
