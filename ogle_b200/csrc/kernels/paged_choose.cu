@@ -9,6 +9,8 @@
 // Bound by latency: sequence, table, page, bounds, one look-up behind the other. 64 texts of up to 8000 tokens, pages of 64, 32 query heads to 8
 // of 128: 7 us for the bounds of the new tokens' pages (4 MB) and 9 for scores and choice (10 MB). Twelve drafts over up to 150000 tokens, pages of 32:
 // 5, 9 for the scores and 9 for the choice.
+#include <atomic>
+
 #include "paged.cuh"
 
 namespace ogle {
@@ -459,6 +461,20 @@ int tile_rows(const Batch& b) {
 size_t query_bytes(const Batch& b) { return size_t(div_up(tile_rows(b) * b.group, 16)) * 2 * div_up(b.dim, 64) * 1024; }
 // Few pages, and few rows to a block: one launch.
 bool few_form(const Batch& b) { return key_stride(b) <= kRanked && tile_rows(b) <= kFewRows && query_bytes(b) <= (32u << 10); }
+// Raises the kernel's limit of shared memory to what the largest group of heads takes, once for each device: another thread's call may be between its
+// own raise and its launch.
+constexpr int kMostGroup = 256, kMostQueries = kMostGroup / 16 * 2 * 4 * 1024;
+template <typename Kernel>
+cudaError_t allow_queries(Kernel kernel) {
+    static std::atomic<uint64_t> sized{0};
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e == cudaSuccess && !(sized.load(std::memory_order_relaxed) >> (device & 63) & 1)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostQueries);
+        if (e == cudaSuccess) sized.fetch_or(1ull << (device & 63), std::memory_order_relaxed);
+    }
+    return e;
+}
 int failed(cudaError_t e) {
     set_last_error(e);
     (void)cudaGetLastError();
@@ -505,7 +521,7 @@ int ogle_cuda_choose_pages(const OglePagedBatch* batch, const OgleChooseParams* 
     if (!p->q || !p->bounds || !p->bounds_scale || !p->chosen) return OGLE_ERR_INVALID;
     if (p->chosen_head < p->count || p->chosen_row < p->count) return OGLE_ERR_INVALID;
     if (!paged::strides_ok(p->q, p->q_row, p->q_head, batch->dtype) || !aligned16(p->bounds)) return OGLE_ERR_ALIGNMENT;
-    if (B.group > 256) return OGLE_ERR_UNSUPPORTED;
+    if (B.group > kMostGroup) return OGLE_ERR_UNSUPPORTED;
     if (B.max_rows == 0) return OGLE_OK;
     const size_t needed = ogle_cuda_choose_pages_workspace_bytes(batch, p);
     if (needed > 0 && (!workspace || workspace_bytes < needed)) return OGLE_ERR_INVALID;
@@ -541,7 +557,7 @@ int ogle_cuda_choose_pages(const OglePagedBatch* batch, const OgleChooseParams* 
     }
     const auto score = choose_score_kernel<kWarps, false>;
     if (queries > (44u << 10)) {
-        const cudaError_t e = cudaFuncSetAttribute(score, cudaFuncAttributeMaxDynamicSharedMemorySize, int(queries));
+        const cudaError_t e = allow_queries(score);
         if (e != cudaSuccess) return failed(e);
     }
     const long long at_once = rows_at_once(B);

@@ -928,3 +928,34 @@ def test_search_refuses_a_step_too_many():
     with pytest.raises(ValueError):
         search.step()
     assert search.texts() == before
+
+
+# ------------------------------------------------------------------------------------------------------ several callers
+def test_choices_of_two_threads_with_queries_of_different_sizes():
+    """Two host threads, each on a stream of its own, whose queries take 64 and 128 KB of shared memory."""
+    import threading
+    calls, failed = [], []
+    for group, seed in ((128, 1), (256, 2)):
+        batch, total = lm_checks.make_batch([1, 1], [5000, 300], 16, 1, 256, seed=seed)
+        bounds = with_bounds(batch, total)
+        q = torch.randn(2, group, 256, generator=torch.Generator().manual_seed(seed)).cuda()
+        calls.append(lambda q=q, batch=batch, bounds=bounds: lm.choose_pages(q, batch["cache"], bounds, count=5, **batch_only(batch)))
+    alone = [c() for c in calls]
+    torch.cuda.synchronize()
+
+    def many(call, want):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                got = [call() for _ in range(400)]
+            stream.synchronize()
+            assert all(torch.equal(g, want) for g in got)
+        except Exception as e:
+            failed.append(e)
+
+    threads = [threading.Thread(target=many, args=a) for a in zip(calls, alone)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
