@@ -51,19 +51,19 @@ def rotary_table(positions, rotary_dim, base=10000.0, device="cuda"):
     return torch.cat([angle.cos(), angle.sin()], 1).to(_F32).to(device)
 
 
-def _vector(t, dtype, n, name):
-    """Address of a contiguous vector of n values (any number, n None)."""
+def _vector(t, dtype, n, name, here=None):
+    """Address of a contiguous vector of n values (any number, n None), on device `here` (any, None)."""
     if t is None:
         return 0
-    if t.dtype != dtype or not t.is_cuda or not t.is_contiguous() or (n is not None and t.numel() != n):
-        raise ValueError(f"{name}: expected a contiguous {dtype} CUDA tensor" + (f" of {n} values" if n is not None else ""))
+    if t.dtype != dtype or (not t.is_cuda if here is None else t.get_device() != here) or not t.is_contiguous() or (n is not None and t.numel() != n):
+        raise ValueError(f"{name}: expected a contiguous {dtype} CUDA tensor" + (f" of {n} values" if n is not None else "") + (f" on device {here}" if here is not None else ""))
     return t.data_ptr()
 
 
-def _rows(t, dtype, rows, heads, dim, name):
+def _rows(t, dtype, rows, heads, dim, name, here=None):
     """(address, row stride, head stride) of activations [rows, heads, dim]."""
-    if t.dtype != dtype or not t.is_cuda or t.dim() != 3:
-        raise ValueError(f"{name}: expected a {dtype} CUDA tensor [rows, heads, head dim]")
+    if t.dtype != dtype or (not t.is_cuda if here is None else t.get_device() != here) or t.dim() != 3:
+        raise ValueError(f"{name}: expected a {dtype} CUDA tensor [rows, heads, head dim]" + (f" on device {here}" if here is not None else ""))
     shape, stride = t.shape, t.stride()
     if shape[0] != rows or shape[2] != dim or (heads is not None and shape[1] != heads) or (stride[2] != 1 and dim > 1):
         raise ValueError(f"{name}: expected [{rows}, {heads if heads is not None else 'heads'}, {dim}] with the elements of a head side by side, "
@@ -71,7 +71,7 @@ def _rows(t, dtype, rows, heads, dim, name):
     return t.data_ptr(), stride[0], stride[1]
 
 
-def _batch(cache, block_table, kv_len, max_kv_len, row_start, max_rows, rows, q_heads, dtype):
+def _batch(cache, block_table, kv_len, max_kv_len, row_start, max_rows, rows, q_heads, dtype, here=None):
     k, v, k_scale, v_scale = cache
     shape, stride = k.shape, k.stride()
     if k.dtype != _E4M3 or v.dtype != _E4M3 or not k.is_cuda or not v.is_cuda or len(shape) != 4 or shape != v.shape:
@@ -81,6 +81,8 @@ def _batch(cache, block_table, kv_len, max_kv_len, row_start, max_rows, rows, q_
         raise ValueError("cache: keys and values need the same strides, the elements of a token side by side")
     if dtype not in _DTYPE:
         raise ValueError(f"activations are float32, float16 or bfloat16, not {dtype}")
+    if here is not None and (k.get_device() != here or v.get_device() != here or block_table.get_device() != here):
+        raise ValueError(f"cache and block_table: expected on device {here}")
     table_shape, table_strides = block_table.shape, block_table.stride()
     if block_table.dtype != _I32 or not block_table.is_cuda or len(table_shape) != 2 or table_strides[1] != 1 and table_shape[1] > 1:
         raise ValueError("block_table: expected an int32 CUDA tensor [sequences, blocks]")
@@ -92,9 +94,9 @@ def _batch(cache, block_table, kv_len, max_kv_len, row_start, max_rows, rows, q_
         raise ValueError(f"{rows} rows for {seqs} sequences need row_start")
     return _PAGED_BATCH(seqs, rows, 1 if row_start is None else max_rows, max_kv_len, q_heads, kv_heads, dim, page_tokens, pages,
                         table_stride, _DTYPE[dtype], 0, stride[0], stride[1], stride[2],
-                        _vector(row_start, _I32, seqs + 1, "row_start"), _vector(kv_len, _I32, seqs, "kv_len"), block_table.data_ptr(),
-                        k.data_ptr(), v.data_ptr(), _vector(k_scale, _F32, pages * kv_heads, "k_scale"),
-                        _vector(v_scale, _F32, pages * kv_heads, "v_scale"))
+                        _vector(row_start, _I32, seqs + 1, "row_start", here), _vector(kv_len, _I32, seqs, "kv_len", here), block_table.data_ptr(),
+                        k.data_ptr(), v.data_ptr(), _vector(k_scale, _F32, pages * kv_heads, "k_scale", here),
+                        _vector(v_scale, _F32, pages * kv_heads, "v_scale", here))
 
 
 def append(k, v, cache, block_table, kv_len, max_kv_len, row_start=None, max_rows=1, q=None, rotary=None, interleaved=False, out=None):
@@ -195,9 +197,16 @@ def adjust_logits(logits, tokens=None, token_start=None, prompt_len=None, repeti
     return out
 
 
-def _here(t):
-    """The current stream, which is the one of t's device: a call does not go to another."""
-    device = t.get_device()
+def _device(t, name):
+    """Number of the device that a call's first tensor lies on: the others have to, too."""
+    here = t.get_device()
+    if here < 0:
+        raise ValueError(f"{name}: expected a CUDA tensor")
+    return here
+
+
+def _here(device):
+    """The current stream, which is one of the call's device: a call does not go to another."""
     if device != torch.cuda.current_device():
         raise ValueError(f"tensors of device {device}, but the current one is {torch.cuda.current_device()}")
     return torch._C._cuda_getCurrentRawStream(device)
@@ -218,11 +227,11 @@ def _results(like, ints, workspace):
     return out, out.data_ptr(), held.data_ptr(), held
 
 
-def _table(t, name):
+def _table(t, name, here):
     """(sequences, blocks, row stride) of a block table."""
     shape, stride = t.shape, t.stride()
-    if t.dtype != _I32 or not t.is_cuda or len(shape) != 2 or stride[1] != 1 and shape[1] > 1:
-        raise ValueError(f"{name}: expected an int32 CUDA tensor [sequences, blocks]")
+    if t.dtype != _I32 or t.get_device() != here or len(shape) != 2 or stride[1] != 1 and shape[1] > 1:
+        raise ValueError(f"{name}: expected an int32 CUDA tensor [sequences, blocks] on device {here}")
     return shape[0], shape[1], stride[0] if shape[0] > 1 else shape[1]
 
 
@@ -235,6 +244,7 @@ def beam_step(logits, scores, beams, count, ends=None):
     if logits.dim() != 2 or not logits.is_cuda or logits.dtype not in _DTYPE or logits.stride(1) != 1 and logits.shape[1] > 1:
         raise ValueError("logits: expected a CUDA tensor [rows, vocab] in float32, float16 or bfloat16, a row's elements side by side")
     rows, vocab = logits.shape
+    here = _device(logits, "logits")
     if beams < 1 or rows % beams != 0:
         raise ValueError(f"{rows} rows are no whole groups of {beams} beams")
     groups = rows // beams
@@ -242,11 +252,11 @@ def beam_step(logits, scores, beams, count, ends=None):
     n = groups * count
     lib = _lib.cuda_lib()
     given = (groups, beams, vocab, count, _DTYPE[logits.dtype], ends.numel() if ends is not None else 0, logits.stride(0) if rows > 1 else vocab,
-             logits.data_ptr(), _vector(scores, _F32, rows, "scores"), _vector(ends, _I32, None, "ends"))
+             logits.data_ptr(), _vector(scores, _F32, rows, "scores", here), _vector(ends, _I32, None, "ends", here))
     size = lib.ogle_cuda_beam_step_workspace_bytes(_BEAM(*given, 0, 0, 0, 0, 0, 0))
     out, at, workspace, held = _results(logits, 3 * (n + max(rows, 1)), size)
     p = _BEAM(*given, at, at + 4 * n, at + 8 * n, at + 12 * n, at + 12 * n + 4 * rows, at + 12 * n + 8 * rows)
-    check(lib.ogle_cuda_beam_step(p, workspace, size, _here(logits)), "beam_step")
+    check(lib.ogle_cuda_beam_step(p, workspace, size, _here(here)), "beam_step")
     shape, stride, out32 = (groups, count), (count, 1), out.view(_F32)
     return (out32.as_strided(shape, stride), out.as_strided(shape, stride, n), out.as_strided(shape, stride, 2 * n),
             out.as_strided((rows,), (1,), 3 * n), out.as_strided((rows,), (1,), 3 * n + rows), out32.as_strided((rows,), (1,), 3 * n + 2 * rows))
@@ -259,17 +269,19 @@ def advance_pages(block_table, kv_len, parent, new, refs, page_tokens, blocks=No
     are gone. Nothing is changed in place. Returns (table [texts, blocks], kv_len with the new tokens, refs, copies int32 [texts, 3] for
     copy_pages, state): state[0] pages are free for the next call, state[1] requests found none (an entry of -1: take the old table
     again, with fewer texts). blocks: columns of the new table, as the old one where None."""
-    seqs, old_blocks, stride = _table(block_table, "block_table")
+    here = _device(refs, "refs")
+    seqs, old_blocks, stride = _table(block_table, "block_table", here)
     n, pages = parent.numel(), refs.numel()
     blocks = old_blocks if blocks is None else blocks
     tokens = new if isinstance(new, torch.Tensor) else None
     lib = _lib.cuda_lib()
     given = (seqs, n, old_blocks, blocks, page_tokens, pages, 0 if tokens is not None else new, 0, stride, blocks, block_table.data_ptr(),
-             _vector(kv_len, _I32, seqs, "kv_len"), _vector(parent, _I32, n, "parent"), _vector(tokens, _I32, n, "new"), _vector(refs, _I32, pages, "refs"))
+             _vector(kv_len, _I32, seqs, "kv_len", here), _vector(parent, _I32, n, "parent", here), _vector(tokens, _I32, n, "new", here),
+             _vector(refs, _I32, pages, "refs", here))
     size = lib.ogle_cuda_advance_pages_workspace_bytes(_ADVANCE(*given, 0, 0, 0, 0, 0))
     out, at, workspace, held = _results(refs, n * (blocks + 4) + pages + 2, size)      # one allocation for all five
     p = _ADVANCE(*given, at, at + 4 * n * blocks, at + 4 * n * (blocks + 4), at + 4 * n * (blocks + 1), at + 4 * (n * (blocks + 4) + pages))
-    check(lib.ogle_cuda_advance_pages(p, workspace, size, _here(refs)), "advance_pages")
+    check(lib.ogle_cuda_advance_pages(p, workspace, size, _here(here)), "advance_pages")
     at = n * blocks
     return (out.as_strided((n, blocks), (blocks, 1)), out.as_strided((n,), (1,), at), out.as_strided((pages,), (1,), at + 4 * n),
             out.as_strided((n, 3), (3, 1), at + n), out.as_strided((2,), (1,), at + 4 * n + pages))
@@ -278,14 +290,15 @@ def advance_pages(block_table, kv_len, parent, new, refs, page_tokens, blocks=No
 def compact_pages(block_table, refs, most, page_tokens):
     """Moves used pages to the front of the pool (ogle_cuda_compact_pages), `most` of them at most. Nothing is changed in place. Returns
     (table, refs, copies int32 [most, 3] for copy_pages, state): state[0] pages are in use, state[1] moves are left for another call."""
-    seqs, blocks, stride = _table(block_table, "block_table")
+    here = _device(refs, "refs")
+    seqs, blocks, stride = _table(block_table, "block_table", here)
     pages = refs.numel()
     lib = _lib.cuda_lib()
-    given = (seqs, blocks, page_tokens, pages, most, 0, stride, blocks, block_table.data_ptr(), _vector(refs, _I32, pages, "refs"))
+    given = (seqs, blocks, page_tokens, pages, most, 0, stride, blocks, block_table.data_ptr(), _vector(refs, _I32, pages, "refs", here))
     size = lib.ogle_cuda_compact_pages_workspace_bytes(_COMPACT(*given, 0, 0, 0, 0))
     out, at, workspace, held = _results(refs, seqs * blocks + pages + 3 * max(most, 0) + 2, size)
     p = _COMPACT(*given, at, at + 4 * seqs * blocks, at + 4 * (seqs * blocks + pages), at + 4 * (seqs * blocks + pages + 3 * most))
-    check(lib.ogle_cuda_compact_pages(p, workspace, size, _here(refs)), "compact_pages")
+    check(lib.ogle_cuda_compact_pages(p, workspace, size, _here(here)), "compact_pages")
     at = seqs * blocks
     return (out.as_strided((seqs, blocks), (blocks, 1)), out.as_strided((pages,), (1,), at), out.as_strided((most, 3), (3, 1), at + pages),
             out.as_strided((2,), (1,), at + pages + 3 * most))
@@ -301,25 +314,26 @@ def copy_pages(caches, copies, bounds=None):
     if len(shape) != 4 or stride[3] != 1:
         raise ValueError("caches: expected keys and values [pages, kv heads, page tokens, head dim], the elements of a token side by side")
     pages, heads, page_tokens, dim = shape
+    here = _device(k0, "caches")
     layers = []
     for i, (k, v, k_scale, v_scale) in enumerate(caches):
-        if k.dtype != _E4M3 or v.dtype != _E4M3 or not k.is_cuda or not v.is_cuda or k.shape != shape or v.shape != shape or k.stride() != stride or v.stride() != stride:
-            raise ValueError("caches: expected float8_e4m3fn CUDA tensors of the same shape and strides for all keys and values")
-        b = (0, 0) if bounds is None else _bounds(bounds[i], pages, heads, dim)
-        layers.append(_PAGE_TENSORS(k.data_ptr(), v.data_ptr(), _vector(k_scale, _F32, pages * heads, "k_scale"),
-                                    _vector(v_scale, _F32, pages * heads, "v_scale"), *b))
+        if k.dtype != _E4M3 or v.dtype != _E4M3 or k.get_device() != here or v.get_device() != here or k.shape != shape or v.shape != shape or k.stride() != stride or v.stride() != stride:
+            raise ValueError(f"caches: expected float8_e4m3fn CUDA tensors of the same shape and strides for all keys and values, on device {here}")
+        b = (0, 0) if bounds is None else _bounds(bounds[i], pages, heads, dim, here)
+        layers.append(_PAGE_TENSORS(k.data_ptr(), v.data_ptr(), _vector(k_scale, _F32, pages * heads, "k_scale", here),
+                                    _vector(v_scale, _F32, pages * heads, "v_scale", here), *b))
     if copies.dim() != 2 or copies.shape[1] != 3:
         raise ValueError("copies: expected [n, 3]")
-    p = _COPY_PAGES(copies.shape[0], len(layers), heads, dim, page_tokens, pages, stride[0], stride[1], stride[2], _vector(copies, _I32, None, "copies"))
-    check(_lib.cuda_lib().ogle_cuda_copy_pages(p, b"".join(layers), _here(k0)), "copy_pages")
+    p = _COPY_PAGES(copies.shape[0], len(layers), heads, dim, page_tokens, pages, stride[0], stride[1], stride[2], _vector(copies, _I32, None, "copies", here))
+    check(_lib.cuda_lib().ogle_cuda_copy_pages(p, b"".join(layers), _here(here)), "copy_pages")
 
 
-def _bounds(bounds, pages, heads, dim):
+def _bounds(bounds, pages, heads, dim, here):
     """Addresses of a cache's bounds."""
     lo_hi, scale = bounds
     if lo_hi.shape != (pages, heads, 2, dim):
         raise ValueError(f"bounds: expected int8 [{pages}, {heads}, 2, {dim}]")
-    return _vector(lo_hi, torch.int8, None, "bounds"), _vector(scale, _F32, pages * heads, "the bounds' scale")
+    return _vector(lo_hi, torch.int8, None, "bounds", here), _vector(scale, _F32, pages * heads, "the bounds' scale", here)
 
 
 def new_bounds(cache):
@@ -334,8 +348,9 @@ def page_bounds(cache, bounds, block_table, kv_len, max_kv_len, row_start=None, 
     pages, heads, _, dim = cache[0].shape
     # rows are not looked at, but row_start is cut to their number: any that a batch could have, and any type
     rows = block_table.shape[0] if row_start is None else (1 << 30) // heads
-    b = _batch(cache, block_table, kv_len, max_kv_len, row_start, max_rows, rows, heads, torch.bfloat16)
-    check(_lib.cuda_lib().ogle_cuda_page_bounds(b, *_bounds(bounds, pages, heads, dim), _here(cache[0])), "page_bounds")
+    here = _device(cache[0], "cache")
+    b = _batch(cache, block_table, kv_len, max_kv_len, row_start, max_rows, rows, heads, torch.bfloat16, here)
+    check(_lib.cuda_lib().ogle_cuda_page_bounds(b, *_bounds(bounds, pages, heads, dim, here), _here(here)), "page_bounds")
 
 
 def choose_pages(q, cache, bounds, block_table, kv_len, max_kv_len, row_start=None, max_rows=1, count=16, first=1, last=1):
@@ -346,14 +361,15 @@ def choose_pages(q, cache, bounds, block_table, kv_len, max_kv_len, row_start=No
         raise ValueError("q: expected [rows, heads, head dim]")
     pages, kv_heads, _, dim = cache[0].shape
     rows, heads, _ = q.shape
-    b = _batch(cache, block_table, kv_len, max_kv_len, row_start, max_rows, rows, heads, q.dtype)
+    here = _device(q, "q")
+    b = _batch(cache, block_table, kv_len, max_kv_len, row_start, max_rows, rows, heads, q.dtype, here)
     chosen = q.new_empty(rows, kv_heads, max(count, 0), dtype=_I32)
-    p = _CHOOSE(*_rows(q, q.dtype, rows, heads, dim, "q"), *_bounds(bounds, pages, kv_heads, dim), chosen.data_ptr(), kv_heads * count, count,
+    p = _CHOOSE(*_rows(q, q.dtype, rows, heads, dim, "q", here), *_bounds(bounds, pages, kv_heads, dim, here), chosen.data_ptr(), kv_heads * count, count,
                 count, first, last, 0)
     lib = _lib.cuda_lib()
     n = lib.ogle_cuda_choose_pages_workspace_bytes(b, p)
     workspace = q.new_empty(n, dtype=torch.uint8) if n else None
-    check(lib.ogle_cuda_choose_pages(b, p, workspace.data_ptr() if n else 0, n, _here(q)), "choose_pages")
+    check(lib.ogle_cuda_choose_pages(b, p, workspace.data_ptr() if n else 0, n, _here(here)), "choose_pages")
     return chosen
 
 
@@ -366,15 +382,16 @@ def sparse_attention(q, cache, chosen, block_table, kv_len, max_kv_len, row_star
         raise ValueError("q: expected [rows, heads, head dim]")
     rows, heads, dim = q.shape
     kv_heads = cache[0].shape[1]
-    b = _batch(cache, block_table, kv_len, max_kv_len, row_start, max_rows, rows, heads, dtype)
-    pq = _rows(q, dtype, rows, heads, cache[0].shape[3], "q")
-    if chosen.dim() != 3 or chosen.dtype != _I32 or not chosen.is_cuda or chosen.shape[0] != rows or chosen.shape[1] != kv_heads or chosen.stride(2) != 1 and chosen.shape[2] > 1:
+    here = _device(q, "q")
+    b = _batch(cache, block_table, kv_len, max_kv_len, row_start, max_rows, rows, heads, dtype, here)
+    pq = _rows(q, dtype, rows, heads, cache[0].shape[3], "q", here)
+    if chosen.dim() != 3 or chosen.dtype != _I32 or chosen.get_device() != here or chosen.shape[0] != rows or chosen.shape[1] != kv_heads or chosen.stride(2) != 1 and chosen.shape[2] > 1:
         raise ValueError(f"chosen: expected an int32 CUDA tensor [{rows}, {kv_heads}, count], a choice's entries side by side")
     if out is None:
         out = q.new_empty(rows, heads, dim)
         po = out.data_ptr(), heads * dim, dim
     else:
-        po = _rows(out, dtype, rows, heads, dim, "out")
+        po = _rows(out, dtype, rows, heads, dim, "out", here)
     lse = q.new_empty(rows, heads, dtype=_F32)
     p = _ATTENTION(pq[0], po[0], lse.data_ptr(), pq[1], pq[2], po[1], po[2], dim ** -0.5 if scale is None else scale, 1, 0, 0)
     count = chosen.shape[2]
@@ -382,5 +399,5 @@ def sparse_attention(q, cache, chosen, block_table, kv_len, max_kv_len, row_star
     lib = _lib.cuda_lib()
     n = lib.ogle_cuda_sparse_attention_workspace_bytes(b, p, c) if row_start is not None and max_rows > 1 else 0       # of single rows none
     workspace = q.new_empty(n, dtype=torch.uint8) if n else None
-    check(lib.ogle_cuda_sparse_attention(b, p, c, workspace.data_ptr() if n else 0, n, _here(q)), "sparse_attention")
+    check(lib.ogle_cuda_sparse_attention(b, p, c, workspace.data_ptr() if n else 0, n, _here(here)), "sparse_attention")
     return out, lse

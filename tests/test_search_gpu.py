@@ -959,3 +959,40 @@ def test_choices_of_two_threads_with_queries_of_different_sizes():
     for t in threads:
         t.join()
     assert not failed, failed
+
+
+class OfAnotherDevice(torch.Tensor):
+    """Says that it lies on device 1; its memory is the current one's."""
+    def get_device(self):
+        return 1
+
+
+def elsewhere(t):
+    return t.as_subclass(OfAnotherDevice)
+
+
+def test_every_tensor_of_another_device_is_refused():
+    batch, total = lm_checks.make_batch([1, 1], [50, 20], 16, 2, 64)
+    cache, bounds = batch["cache"], with_bounds(batch, total)
+    q, one = torch.randn(2, 4, 64).cuda(), ints([1, 1])
+    chosen, copies = ints([[[0, -1]] * 2] * 2), ints([[-1, -1, 0]])
+    named = dict(block_table=batch["block_table"], kv_len=batch["kv_len"], row_start=batch["row_start"])
+    most = dict(max_kv_len=batch["max_kv_len"], max_rows=1)
+    calls = [
+        (lambda logits, scores, ends: lm.beam_step(logits, scores, 2, 4, ends=ends), dict(logits=torch.zeros(2, 9, device="cuda"), scores=torch.zeros(2, device="cuda"), ends=one)),
+        (lambda **t: lm.advance_pages(page_tokens=16, **t), dict(block_table=batch["block_table"], kv_len=one, parent=one, new=one, refs=ints([1] * 8))),
+        (lambda **t: lm.compact_pages(most=1, page_tokens=16, **t), dict(block_table=batch["block_table"], refs=ints([1] * 8))),
+        (lambda copies, k, v, ks, vs, lo_hi, unit: lm.copy_pages([cache, (k, v, ks, vs)], copies, bounds=[bounds, (lo_hi, unit)]),
+         dict(copies=copies, k=cache[0], v=cache[1], ks=cache[2], vs=cache[3], lo_hi=bounds[0], unit=bounds[1])),
+        (lambda k, v, ks, vs, lo_hi, unit, **t: lm.page_bounds((k, v, ks, vs), (lo_hi, unit), **t, **most),
+         dict(k=cache[0], v=cache[1], ks=cache[2], vs=cache[3], lo_hi=bounds[0], unit=bounds[1], **named)),
+        (lambda q, k, v, ks, vs, lo_hi, unit, **t: lm.choose_pages(q, (k, v, ks, vs), (lo_hi, unit), count=2, **t, **most),
+         dict(q=q, k=cache[0], v=cache[1], ks=cache[2], vs=cache[3], lo_hi=bounds[0], unit=bounds[1], **named)),
+        (lambda q, k, v, ks, vs, chosen, out, **t: lm.sparse_attention(q, (k, v, ks, vs), chosen, out=out, **t, **most),
+         dict(q=q, k=cache[0], v=cache[1], ks=cache[2], vs=cache[3], chosen=chosen, out=torch.zeros_like(q), **named))]
+    for call, tensors in calls:
+        call(**tensors)
+        for name in tensors:
+            with pytest.raises(ValueError):
+                call(**{**tensors, name: elsewhere(tensors[name])})
+                pytest.fail(f"{name} of {call}")
