@@ -120,6 +120,8 @@ class Search:
     """Beam search over the answers to prompts: `beams` texts of each, whose pages, scores and parents stay on the device."""
 
     def __init__(self, model, prompts, beams, page_tokens=16, pages=512, ends=(), steps=100):
+        if not all(len(p) for p in prompts):
+            raise ValueError("a prompt without a token has no next one")
         self.model, self.beams, self.page_tokens, self.prompts, self.steps = model, beams, page_tokens, [list(p) for p in prompts], steps
         self.caches = model.new_caches(pages, page_tokens)
         self.bounds = model.new_bounds(self.caches)

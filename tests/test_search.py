@@ -174,3 +174,9 @@ def test_structures_lie_as_the_header_says(tmp_path):
     include = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
     done = subprocess.run([compiler, "-std=c++17", "-fsyntax-only", "-I", include, str(source)], capture_output=True, text=True)
     assert done.returncode == 0, done.stderr
+
+
+def test_a_search_refuses_empty_prompts():
+    from ogle_b200 import lm_example
+    with pytest.raises(ValueError):
+        lm_example.Search(None, [[3, 4], []], 2)
