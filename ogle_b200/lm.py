@@ -356,7 +356,7 @@ def page_bounds(cache, bounds, block_table, kv_len, max_kv_len, row_start=None, 
 def choose_pages(q, cache, bounds, block_table, kv_len, max_kv_len, row_start=None, max_rows=1, count=16, first=1, last=1):
     """The `count` pages that each row of q [rows, heads, head dim] attends (ogle_cuda_choose_pages), for each kv head as blocks of the row's
     sequence: the `first` ones, the row's own with the last - 1 before it, and of the others those whose keys, going by their bounds, can have
-    the largest product with one of the head's queries. Returns int32 [rows, kv heads, count], rising, filled up with -1."""
+    the largest product with one of the head's queries, in 8 bits. Returns int32 [rows, kv heads, count], rising, filled up with -1."""
     if q.dim() != 3:
         raise ValueError("q: expected [rows, heads, head dim]")
     pages, kv_heads, _, dim = cache[0].shape
