@@ -528,10 +528,11 @@ int ogle_cuda_adjust_logits(const OgleLogitsParams* p, ogle_stream_t stream);
  *   scores[row] + x_t - log sum_u exp(x_u),    x = logits[row]
  * in 64 bits, where a NaN logit counts as minus infinity and plus infinity as the largest number of the logits' type. A logit of minus
  * infinity is no continuation; a beam whose score is not finite has none. scores NULL: 0 for all.
- * Of each group the `count` largest totals, in falling order, equal ones by beam, then by logit (where 64 bits have lost the difference) and token,
- * go to out_score (rounded to fp32), out_beam and out_token [n_groups][count]; behind the last there are minus infinity, -1, -1. Of these the first `beams` whose token is
- * none of ends[0 .. n_ends) go on: next_row (the parent's row, g * beams + out_beam), next_token and next_score [n_groups][beams], filled
- * up with -1, -1, minus infinity. (A count of beams * (1 + n_ends), of different end tokens, is enough for all to go on.)
+ * Of each group the `count` largest totals, in falling order, equal ones by beam, then by logit (where 64 bits have lost the difference) and
+ * token, go to out_score (rounded to fp32), out_beam and out_token [n_groups][count]; behind the last there are minus infinity, -1, -1. Of
+ * these the first `beams` whose token is none of ends[0 .. n_ends) go on: next_row (the parent's row, g * beams + out_beam), next_token and
+ * next_score [n_groups][beams], filled up with -1, -1, minus infinity. (A count of beams * (1 + n_ends), of different end tokens, is enough
+ * for all to go on.)
  * Exponentials are of fp32, but those of most rows' largest logits, and sums of 64 bits: the logarithm of a row's sum is within 2^-19 of
  * its value - that far off where thousands of equal logits far below the largest make up most of it -, most often within 2^-23. Beams of the
  * same largest logit whose logarithms are within 2^-18 of each other count as having the same sum.

@@ -133,7 +133,7 @@ __device__ __forceinline__ void range_of(const BeamArgs& a, const T* row, int r,
 // exp(x - m) as the sums have it: 2^(x log2(e) - c) in one rounding of the exponent, which is small where the weight is large. c is an fp32
 // number, m what it stands for; log2(e) in fp32 makes a weight wrong by 2^-26 of its distance from m. What a sum is off by is at most
 // 2^-19 of it: 2^-20 ln 2 where nearly all of it comes of alike logits 11 to 22 below m, all rounded alike, 2^-26 of that distance, 2^-22
-// for the exponentials and six roundings of 2^-24 in fp32. The roundings of logits that differ do so too, and cancel.
+// for the exponentials and six roundings of 2^-24 in fp32. Those of logits that differ are not alike, and cancel.
 constexpr float kLog2e = 1.442695022f;
 __device__ __forceinline__ float weight(float x, float c) { return exp2_fast(fmaf(x, kLog2e, -c)); }
 
